@@ -15,19 +15,12 @@
 #include <unordered_map>
 #include <vector>
 
+#include "bindings.h"
 #include "launchers.h"
 
 namespace {
 
 using at::Tensor;
-
-#define CHECK_CUDA(x) TORCH_CHECK((x).is_cuda(), #x " must be a CUDA tensor")
-#define CHECK_BF16(x) TORCH_CHECK((x).scalar_type() == at::kBFloat16, #x " must be bfloat16")
-// every tensor a kernel dereferences must live on the launching tensor's CUDA device (a host pointer faults)
-#define CHECK_ON(x, ref)                                                                                         \
-  TORCH_CHECK((x).is_cuda() && (x).get_device() == (ref).get_device(), #x " must be on the device of " #ref)
-#define CHECK_I32(x) TORCH_CHECK((x).scalar_type() == at::kInt, #x " must be int32")
-#define CHECK_I64(x) TORCH_CHECK((x).scalar_type() == at::kLong, #x " must be int64")
 
 int num_sms(int device) {
   static std::vector<int> cache(64, 0);
@@ -1529,6 +1522,14 @@ int64_t gemm_cluster_splits(int64_t M, int64_t N, int64_t K, int64_t sms) {
 // Raises a formatted error: a host-only check that exceptions thrown in this library reach Python.
 void raise_formatted(int64_t n) { TORCH_CHECK(n < 0, "formatted error ", n, " from economize_b200._C"); }
 
+namespace ecz {
+
+int device_sms(int device) { return num_sms(device); }
+
+unsigned* device_status(const at::Device& device) { return status_word(device); }
+
+}  // namespace ecz
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "economize_b200 sm_100a kernels (tcgen05 / TMA)";
   m.def("rmsnorm", &rmsnorm, "fused residual add + RMSNorm");
@@ -1609,6 +1610,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sp_linear_ag", &sp_linear_ag, "all-gather -> GEMM (the GEMM waits for every rank's rows)");
   m.def("sp_linear_rs", &sp_linear_rs, "GEMM -> reduce-scatter (rows stored into their owner's partial slot)");
   m.def("reduce_rmsnorm", &reduce_rmsnorm, "wait for every rank's partial, sum, add residual, RMSNorm");
+  ecz::bind_training(m);
   m.def("status", &status, "read and clear the device status word of bounded waits");
   m.def("attention_plan", &attention_plan, "(m_tiles, splits, chunks_per_split) of an attention launch",
         py::arg("B"), py::arg("T"), py::arg("H"), py::arg("Hkv"), py::arg("S"), py::arg("sms"), py::arg("window") = 0);

@@ -1,0 +1,194 @@
+// PyTorch bindings of the training operators (readout.cu, packed_attention.cu): argument checks, workspaces from
+// PyTorch's caching allocator, tensor maps, and the launches on the current stream.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <algorithm>
+#include <cstring>
+#include <tuple>
+
+#include "bindings.h"
+#include "launchers.h"
+
+namespace {
+
+using at::Tensor;
+
+// bf16 [rows, cols] (row stride in elements), 128-byte swizzle, box {64, box_rows}.
+CUtensorMap map_2d(const void* base, int64_t rows, int64_t cols, int64_t stride, int box_rows) {
+  CUtensorMap map;
+  std::memset(&map, 0, sizeof(map));
+  const int rc = ecz::make_tmap_2d(&map, 2, base, rows, cols, stride * 2, 64, box_rows, 128);
+  TORCH_CHECK(rc == 0, "cuTensorMapEncodeTiled failed (code ", rc, ") for rows=", rows, " cols=", cols);
+  return map;
+}
+
+// Elements from one row to the next (a single row's stride says nothing).
+int64_t row_stride(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
+
+// A row-major operand the kernels read in 16-byte groups: rows may be further apart than they are long.
+Tensor rows_of(const Tensor& x) {
+  const bool ok = x.stride(1) == 1 && row_stride(x) >= x.size(1) && row_stride(x) % 8 == 0 &&
+                  reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  if (ok) return x;
+  Tensor y = x.contiguous();
+  return reinterpret_cast<uintptr_t>(y.data_ptr()) % 16 == 0 ? y : y.clone();
+}
+
+// What a chunk of rows may hold of unnormalised probabilities (2 bytes each).
+constexpr int64_t kChunkBytes = int64_t{1} << 30;
+
+// Losses and, where asked for, gradients of the readout (see ops.linear_cross_entropy). reduction 0: per-row losses
+// [T]; 1 / 2: their mean / sum as a scalar. grad_rows: the per-row upstream gradient of reduction 0 (then no loss is
+// returned); reductions 1 and 2 compute the gradients of the scalar itself.
+std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> readout(
+    Tensor hidden, Tensor weight, Tensor targets, int64_t ignore_index, double logit_scale, int64_t reduction,
+    bool need_dx, bool need_dw, c10::optional<Tensor> grad_rows, int64_t chunk_rows) {
+  CHECK_CUDA(hidden);
+  CHECK_BF16(hidden);
+  CHECK_BF16(weight);
+  CHECK_I64(targets);
+  CHECK_ON(weight, hidden);
+  CHECK_ON(targets, hidden);
+  TORCH_CHECK(hidden.dim() == 2 && weight.dim() == 2 && targets.dim() == 1,
+              "readout expects hidden [T, H], weight [V, H] and targets [T]");
+  const int64_t T = hidden.size(0), H = hidden.size(1), V = weight.size(0);
+  TORCH_CHECK(weight.size(1) == H, "hidden has ", H, " columns, weight ", weight.size(1));
+  TORCH_CHECK(targets.size(0) == T, "hidden has ", T, " rows, targets ", targets.size(0));
+  TORCH_CHECK(H >= 8 && H % 8 == 0, "readout: the hidden size must be a multiple of 8 (got ", H, ")");
+  TORCH_CHECK(V >= 1 && V <= (int64_t{1} << 22), "readout: 1 to 4194304 vocabulary rows (got ", V, ")");
+  TORCH_CHECK(H <= (int64_t{1} << 17) && T <= (int64_t{1} << 30), "readout: hidden size or row count too large");
+  TORCH_CHECK(reduction >= 0 && reduction <= 2, "unknown reduction ", reduction);
+  c10::cuda::CUDAGuard guard(hidden.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const int sms = ecz::device_sms(hidden.get_device());
+  unsigned* status = ecz::device_status(hidden.device());
+  Tensor x = T > 0 ? rows_of(hidden) : hidden, w = rows_of(weight);
+  targets = targets.contiguous();
+  const auto f32 = hidden.options().dtype(at::kFloat), i32 = hidden.options().dtype(at::kInt);
+  const bool per_row = reduction == ecz::kReduceNone;
+  const bool want_loss = !grad_rows.has_value();
+  Tensor loss = want_loss ? (per_row ? at::empty({T}, f32) : at::empty({}, f32)) : Tensor();
+  c10::optional<Tensor> dx, dw;
+  if (need_dx) dx = at::empty({T, H}, hidden.options());
+  if (need_dw) dw = at::empty({V, H}, weight.options());
+  if (grad_rows.has_value()) {
+    TORCH_CHECK(per_row && grad_rows->scalar_type() == at::kFloat && grad_rows->dim() == 1 && grad_rows->size(0) == T,
+                "grad_rows must be fp32 [T] of a per-row loss");
+    CHECK_ON(*grad_rows, hidden);
+    grad_rows = grad_rows->contiguous();
+  }
+  if (T == 0) {
+    if (want_loss && !per_row) loss.zero_();
+    if (dw) dw->zero_();
+    return {loss, dx, dw};
+  }
+  const bool grads = need_dx || need_dw;
+  const int64_t ld = (V + 7) / 8 * 8;
+  // Rows of a chunk: 1 GiB of e; with dW as much as the fp32 sum of several chunks would take (4 V H bytes).
+  int64_t chunk = T;
+  if (chunk_rows > 0) {
+    chunk = chunk_rows;
+  } else if (grads) {
+    const int64_t budget = std::max(kChunkBytes, need_dw ? 4 * V * H : int64_t{0});
+    chunk = std::max<int64_t>(256, budget / (2 * ld) / 256 * 256);
+  } else {
+    chunk = std::max<int64_t>(256, kChunkBytes / (8 * ecz::readout_pieces(V)) / 256 * 256);
+  }
+  chunk = std::min((T + 63) / 64 * 64, (chunk + 63) / 64 * 64);
+  const int64_t chunks = (T + chunk - 1) / chunk;
+
+  Tensor index = at::empty({3 * T + 1}, i32);  // rows, positions, targets, count
+  int* rows = index.data_ptr<int>();
+  int *pos = rows + T, *target_of = rows + 2 * T, *count = rows + 3 * T;
+  Tensor xs = at::empty({T + 64, H}, hidden.options());
+  Tensor stats = at::empty({chunk, ecz::readout_pieces(static_cast<int>(V)), 2}, f32);
+  Tensor nll = at::empty({T + chunk}, f32);  // losses of the packed rows, then a chunk's picked logits
+  Tensor e = grads ? at::empty({chunk, ld}, hidden.options()) : Tensor();
+  Tensor sum = need_dw && chunks > 1 ? at::empty({V, H}, f32) : Tensor();
+
+  auto check = [](int rc, const char* what) { TORCH_CHECK(rc == 0, "readout: ", what, " launch failed"); };
+  check(ecz::launch_readout_plan(targets.data_ptr<int64_t>(), static_cast<int>(T), static_cast<int>(V), ignore_index,
+                                 rows, pos, target_of, count, status, stream),
+        "plan");
+  check(ecz::launch_readout_gather(x.data_ptr(), row_stride(x), static_cast<int>(T), static_cast<int>(H), pos, count,
+                                   xs.data_ptr(), need_dx ? dx->data_ptr() : nullptr,
+                                   want_loss && per_row ? loss.data_ptr<float>() : nullptr, stream),
+        "gather");
+  const CUtensorMap w_rows = map_2d(w.data_ptr(), V, H, row_stride(w), 128);
+  const CUtensorMap w_cols = map_2d(w.data_ptr(), V, H, row_stride(w), 64);
+  for (int64_t i = 0; i < chunks; ++i) {
+    ecz::ReadoutChunk c;
+    c.row0 = static_cast<int>(i * chunk);
+    c.chunk = static_cast<int>(std::min(chunk, T - i * chunk));
+    c.H = static_cast<int>(H);
+    c.V = static_cast<int>(V);
+    c.rows = rows;
+    c.target = target_of;
+    c.count = count;
+    c.stats = stats.data_ptr();
+    c.picked = nll.data_ptr<float>() + T;
+    c.e = grads ? e.data_ptr() : nullptr;
+    c.ld = ld;
+    c.logit_scale = static_cast<float>(logit_scale);
+    const int64_t padded = (c.chunk + 63) / 64 * 64;  // rows of xs and e that the maps may read
+    uint8_t* xs0 = static_cast<uint8_t*>(xs.data_ptr()) + static_cast<int64_t>(c.row0) * H * 2;
+    const CUtensorMap x_rows = map_2d(xs0, padded, H, H, 128);
+    check(ecz::launch_readout_logits(&x_rows, &w_rows, c, sms, status, stream), "logits");
+    check(ecz::launch_readout_finish(c, static_cast<int>(reduction),
+                                     grad_rows.has_value() ? grad_rows->data_ptr<float>() : nullptr,
+                                     want_loss && !per_row ? nll.data_ptr<float>() : nullptr,
+                                     want_loss && per_row ? loss.data_ptr<float>() : nullptr, stream),
+          "finish");
+    if (need_dx) {
+      const CUtensorMap dz = map_2d(e.data_ptr(), padded, V, ld, 128);
+      const long tiles = ((c.chunk + 255) / 256) * ((H + 255) / 256);
+      const int splits = ecz::readout_splits(tiles, (V + 63) / 64, sms);
+      Tensor part = splits > 1 ? at::empty({splits, c.chunk, H}, f32) : Tensor();
+      check(ecz::launch_readout_dx(&dz, &w_cols, c, splits, splits > 1 ? part.data_ptr<float>() : nullptr,
+                                   dx->data_ptr(), sms, status, stream),
+            "dx");
+    }
+    if (need_dw) {
+      const CUtensorMap dz = map_2d(e.data_ptr(), padded, V, ld, 64);
+      const CUtensorMap x_cols = map_2d(xs0, padded, H, H, 64);
+      check(ecz::launch_readout_dw(&dz, &x_cols, c, chunks > 1 ? sum.data_ptr<float>() : nullptr, i == 0,
+                                   i == chunks - 1, dw->data_ptr(), sms, status, stream),
+            "dw");
+    }
+  }
+  if (want_loss && !per_row)
+    check(ecz::launch_readout_loss(nll.data_ptr<float>(), count, static_cast<int>(reduction), loss.data_ptr<float>(),
+                                   stream),
+          "loss");
+  return {loss, dx, dw};
+}
+
+// x *= g (a scalar on the device) in place.
+void scale_by(Tensor x, Tensor g) {
+  CHECK_CUDA(x);
+  CHECK_BF16(x);
+  CHECK_ON(g, x);
+  TORCH_CHECK(x.is_contiguous() && x.numel() % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0,
+              "scale_by takes a contiguous tensor of 8 n values");
+  TORCH_CHECK(g.scalar_type() == at::kFloat && g.numel() == 1, "scale_by takes an fp32 scalar");
+  c10::cuda::CUDAGuard guard(x.device());
+  TORCH_CHECK(ecz::launch_scale_by(x.data_ptr(), x.numel(), g.data_ptr<float>(), ecz::device_sms(x.get_device()),
+                                   at::cuda::getCurrentCUDAStream()) == 0,
+              "scale_by: launch failed");
+}
+
+}  // namespace
+
+namespace ecz {
+
+void bind_training(pybind11::module_& m) {
+  namespace py = pybind11;
+  m.def("readout", &readout, "softmax cross-entropy of hidden @ weight.T without keeping the logits, with gradients",
+        py::arg("hidden"), py::arg("weight"), py::arg("targets"), py::arg("ignore_index"), py::arg("logit_scale"),
+        py::arg("reduction"), py::arg("need_dx"), py::arg("need_dw"), py::arg("grad_rows") = py::none(),
+        py::arg("chunk_rows") = 0);
+  m.def("scale_by", &scale_by, "x *= g in place for a device scalar g (no memory pass when g is 1)");
+}
+
+}  // namespace ecz

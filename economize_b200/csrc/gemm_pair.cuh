@@ -1,0 +1,290 @@
+// Large-tile GEMM core of the training operators: D[M, N] = A . B^T with either operand K-major ([M, K] / [N, K]
+// rows) or MN-major ([K, M] / [K, N] rows), bf16 in, fp32 accumulation, for products with thousands of rows (the
+// decode GEMMs of gemm_tc.cu swap the operands instead, for a few dozen rows).
+//
+// A cluster of two CTAs computes one 256 x 256 tile with cta_group::2 MMAs (M = 256, N = 256): each CTA holds its
+// own 128 rows of A and half of the columns of B in shared memory (32 KB per 64-element K step) and 128 x 256 fp32
+// accumulators in TMEM, so per 128 x 256 outputs a CTA reads 32 KB from L2 where a one-CTA tile of the same shape
+// reads 48 KB. The accumulators are double-buffered (2 x 256 TMEM columns): the epilogue of a tile runs under the
+// next tile's MMAs.
+//
+//   warp 0      TMA producer (both CTAs; completion counted on the even CTA's barrier)
+//   warp 1      MMA issuer (even CTA only)
+//   warps 2-9   epilogue: warp w reads TMEM lanes 32 (w % 4) .. + 31 and 128 of the 256 columns
+//
+// The grid is persistent over (tile, split) units; every wait is bounded (common.cuh).
+#pragma once
+
+#include "common.cuh"
+
+namespace ecz {
+namespace pair {
+
+constexpr int kTile = 256;    // output tile (both dimensions) of a CTA pair
+constexpr int kHalf = 128;    // A rows and B rows (columns of the output) a CTA loads
+constexpr int kBK = 64;       // K elements per stage
+constexpr int kOperandBytes = kHalf * kBK * 2;
+constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kStages = 5;
+constexpr int kThreads = 320;
+constexpr int kEpiWarps = 8;
+constexpr int kPatchStride = 144;                 // bytes per row of an epilogue warp's [32 rows, 64 bf16] patch
+constexpr int kPatchBytes = 32 * kPatchStride;
+constexpr int kSmem = kStages * kStageBytes + kEpiWarps * kPatchBytes + 1024 + 256;
+static_assert(kSmem <= 232448, "227 KB of shared memory");
+
+// What a launch computes. Counts on the device (rows_dev) clip M (clip_m) or K (clip_k) of a chunk of rows that
+// starts at row0: limit = clamp(*rows_dev - row0, 0, M or K).
+struct Shape {
+  int M, N, K;
+  const int* rows_dev;
+  int row0;
+  bool clip_m, clip_k;
+  int splits;      // K is divided over this many units per tile
+  bool n_fastest;  // order of the tiles: N varies fastest (else M)
+};
+
+__device__ __forceinline__ uint32_t mapa_u32(uint32_t addr, uint32_t rank) {
+  uint32_t out;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
+  return out;
+}
+
+// TMA load into this CTA's shared memory whose bytes are counted on barrier `bar` (a shared::cluster address, of the
+// pair's even CTA).
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, "
+      "%4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+
+__device__ __forceinline__ void umma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Arrive on barrier `bar` (same offset) of both CTAs once every MMA issued so far by this thread has completed.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  const uint16_t mask = 3;
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(mask)
+      : "memory");
+}
+
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// An operand stage of 128 MN rows x 64 K: K-major, one {64 (K), 128} box; MN-major, two {64 (MN), 64 (K)} boxes.
+template <bool MN>
+__device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap* map, uint32_t bar, int mn, int k) {
+  if (MN) {
+    tma_load_pair(dst, map, bar, mn, k);
+    tma_load_pair(dst + kOperandBytes / 2, map, bar, mn + 64, k);
+  } else {
+    tma_load_pair(dst, map, bar, k, mn);
+  }
+}
+
+template <bool MN>
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, int kk) {
+  return MN ? desc_mnmajor_sw128(addr + kk * 16 * 128, kOperandBytes / 2) : desc_kmajor_sw128(addr + kk * 32);
+}
+
+// A unit of the persistent grid: tile (m0, n0) and the K blocks [kb0, kb0 + nkb) of its split.
+struct Unit {
+  int m0, n0, split, kb0, nkb;
+};
+
+struct Schedule {
+  int m_tiles, n_tiles, units, kblocks, per_split;
+  const Shape& s;
+  int M, K;
+  __device__ __forceinline__ explicit Schedule(const Shape& shape) : s(shape) {
+    int rows = 0;
+    if (s.rows_dev != nullptr) rows = max(0, *s.rows_dev - s.row0);
+    M = s.clip_m ? min(s.M, rows) : s.M;
+    K = s.clip_k ? min(s.K, rows) : s.K;
+    m_tiles = (M + kTile - 1) / kTile;
+    n_tiles = (s.N + kTile - 1) / kTile;
+    units = m_tiles * n_tiles * s.splits;
+    kblocks = (K + kBK - 1) / kBK;
+    per_split = (kblocks + s.splits - 1) / s.splits;
+  }
+  __device__ __forceinline__ Unit unit(int u) const {
+    Unit r;
+    r.split = u % s.splits;
+    const int t = u / s.splits;
+    const int mt = s.n_fastest ? t / n_tiles : t % m_tiles;
+    const int nt = s.n_fastest ? t % n_tiles : t / m_tiles;
+    r.m0 = mt * kTile;
+    r.n0 = nt * kTile;
+    r.kb0 = min(kblocks, r.split * per_split);
+    r.nkb = min(per_split, kblocks - r.kb0);
+    return r;
+  }
+};
+
+// Epi: a functor `void operator()(const Unit&, int M, int row0, int col0, uint32_t taddr, bool zero, uint8_t* patch,
+// int lane)` of one warp: rows row0 + lane (of the whole output), columns [col0, col0 + 128), accumulators at TMEM
+// address taddr (this warp's lanes), or zeros where the unit has no K block.
+template <bool A_MN, bool B_MN, class Epi>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                     const __grid_constant__ Shape shape, const __grid_constant__ Epi epi, unsigned* status) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* patches = smem + kStages * kStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(patches + kEpiWarps * kPatchBytes);
+  uint64_t* empty = full + kStages;
+  uint64_t* acc_full = empty + kStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 2 * kEpiWarps);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_a);
+    tma_prefetch_desc(&tm_b);
+  }
+  __syncwarp();
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // the peer's barriers are initialised before anything is counted on them
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_trigger();
+  pdl_wait();
+
+  const Schedule sched(shape);
+  const int pairs = gridDim.x >> 1, pair_id = blockIdx.x >> 1;
+  if (warp == 0 && lane == 0) {
+    // ---- producer ----
+    const uint32_t base = smem_u32(smem);
+    uint32_t it = 0;
+    bool ok = true;
+    for (int u = pair_id; ok && u < sched.units; u += pairs) {
+      const Unit t = sched.unit(u);
+      for (int kb = 0; kb < t.nkb; ++kb, ++it) {
+        const int s = it % kStages;
+        if (!mbar_wait(&empty[s], ((it / kStages) & 1u) ^ 1u, status, kStatusWaitEmpty, abort_flag)) {
+          ok = false;
+          break;
+        }
+        const uint32_t bar = mapa_u32(smem_u32(&full[s]), 0);
+        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kStageBytes);
+        const uint32_t dst = base + s * kStageBytes;
+        const int k = (t.kb0 + kb) * kBK;
+        load_operand<A_MN>(dst, &tm_a, bar, t.m0 + static_cast<int>(rank) * kHalf, k);
+        load_operand<B_MN>(dst + kOperandBytes, &tm_b, bar, t.n0 + static_cast<int>(rank) * kHalf, k);
+      }
+    }
+    // every copy in flight has landed before the pair leaves (its barriers' phases have been consumed, or a wait gave
+    // up): the last stages' loads were waited for by the MMA issuer; after an abort, give them time
+    if (!ok) {
+      const unsigned long long t0 = global_timer_ns();
+      while (global_timer_ns() - t0 < 1000000ull) {
+      }
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    // ---- MMA issuer ----
+    constexpr uint32_t idesc = idesc_bf16_f32(256, 256, B_MN) | ((A_MN ? 1u : 0u) << 15);
+    const uint32_t base = smem_u32(smem);
+    uint32_t it = 0, tile = 0;
+    bool ok = true;
+    for (int u = pair_id; ok && u < sched.units; u += pairs) {
+      const Unit t = sched.unit(u);
+      if (t.nkb <= 0) continue;
+      const uint32_t buf = tile & 1u;
+      if (!mbar_wait(&acc_empty[buf], ((tile >> 1) & 1u) ^ 1u, status, kStatusWaitAccum, abort_flag)) break;
+      tc_fence_after();
+      const uint32_t d = tmem + buf * 256u;
+      for (int kb = 0; kb < t.nkb; ++kb, ++it) {
+        const int s = it % kStages;
+        if (!mbar_wait(&full[s], (it / kStages) & 1u, status, kStatusWaitFull, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t a = base + s * kStageBytes, b = a + kOperandBytes;
+#pragma unroll
+        for (int kk = 0; kk < kBK / 16; ++kk)
+          umma_pair(d, operand_desc<A_MN>(a, kk), operand_desc<B_MN>(b, kk), idesc, (kb | kk) != 0 ? 1u : 0u);
+        commit_pair(&empty[s]);
+      }
+      commit_pair(&acc_full[buf]);
+      ++tile;
+    }
+  } else if (warp >= 2) {
+    // ---- epilogue ----
+    const int ew = warp - 2;
+    const int quad = warp & 3, half = ew >> 2;
+    uint8_t* patch = patches + ew * kPatchBytes;
+    uint32_t tile = 0;
+    for (int u = pair_id; u < sched.units; u += pairs) {
+      const Unit t = sched.unit(u);
+      const int row0 = t.m0 + static_cast<int>(rank) * kHalf + quad * 32, col0 = t.n0 + half * 128;
+      if (t.nkb <= 0) {
+        epi(t, sched.M, row0, col0, 0u, true, patch, lane);
+        continue;
+      }
+      const uint32_t buf = tile & 1u;
+      const bool ok = mbar_wait(&acc_full[buf], (tile >> 1) & 1u, status, kStatusWaitAccum, abort_flag);
+      if (__any_sync(0xffffffffu, !ok)) break;
+      tc_fence_after();
+      epi(t, sched.M, row0, col0, tmem + (static_cast<uint32_t>(quad * 32) << 16) + buf * 256u + half * 128u, false,
+          patch, lane);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(mapa_u32(smem_u32(&acc_empty[buf]), 0));
+      ++tile;
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs are done with each other's barriers and with the accumulators
+  tc_fence_after();
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+template <bool A_MN, bool B_MN, class Epi>
+inline int launch_pair(const CUtensorMap& a, const CUtensorMap& b, const Shape& shape, const Epi& epi, int num_sms,
+                       unsigned* status, cudaStream_t stream) {
+  const long tiles = static_cast<long>((shape.M + kTile - 1) / kTile) * ((shape.N + kTile - 1) / kTile) * shape.splits;
+  if (tiles <= 0) return 0;
+  const int pairs = static_cast<int>(tiles < num_sms / 2 ? tiles : num_sms / 2);
+  auto kernel = gemm_pair_kernel<A_MN, B_MN, Epi>;
+  if (set_max_smem(kernel, kSmem) != cudaSuccess) return -1;
+  return launch_pdl(kernel, dim3(2 * pairs), dim3(kThreads), kSmem, stream, a, b, shape, epi, status) == cudaSuccess ? 0
+                                                                                                                    : -1;
+}
+
+}  // namespace pair
+}  // namespace ecz

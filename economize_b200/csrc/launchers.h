@@ -273,6 +273,38 @@ int launch_ep_combine(const void* y, const int* seg_start, const int* seg_end, c
 int launch_ep_finish(const PeerPtrs& peers, const EpLayout& L, int rank, const int* pos, const float* w, void* out,
                      int tokens, int k, unsigned* status, cudaStream_t stream);
 
+// readout.cu: softmax cross-entropy of a vocabulary readout without keeping the logits (see the file comment). A chunk
+// is the packed rows [row0, row0 + chunk) of those with a target; row0 is a multiple of 64 (the K block of dz^T . X).
+enum ReadoutReduction : int { kReduceNone = 0, kReduceMean = 1, kReduceSum = 2 };
+struct ReadoutChunk {
+  int row0 = 0, chunk = 0, H = 0, V = 0;
+  const int* rows = nullptr;    // [T] packed row -> row
+  const int* target = nullptr;  // [T] target of a packed row
+  const int* count = nullptr;   // packed rows (device)
+  void* stats = nullptr;        // float2 [chunk, readout_pieces(V)]
+  float* picked = nullptr;      // [chunk]
+  void* e = nullptr;            // fp16 e, then bf16 dz [chunk up to a multiple of 64, ld], or null (losses only)
+  long ld = 0;                  // a multiple of 8
+  float logit_scale = 1.f;
+};
+int readout_pieces(int V);
+int readout_splits(long tiles, long kblocks, int num_sms);
+int launch_readout_plan(const int64_t* targets, int T, int V, int64_t ignore, int* rows, int* pos, int* target_of,
+                        int* count, unsigned* status, cudaStream_t stream);
+int launch_readout_gather(const void* x, long x_stride, int T, int H, const int* pos, const int* count, void* xs,
+                          void* dx, float* losses, cudaStream_t stream);
+int launch_readout_logits(const CUtensorMap* xs, const CUtensorMap* w, const ReadoutChunk& c, int num_sms,
+                          unsigned* status, cudaStream_t stream);
+int launch_readout_finish(const ReadoutChunk& c, int reduction, const float* grad_rows, float* nll, float* losses,
+                          cudaStream_t stream);
+int launch_readout_loss(const float* nll, const int* count, int reduction, float* loss, cudaStream_t stream);
+int launch_readout_dx(const CUtensorMap* dz, const CUtensorMap* w, const ReadoutChunk& c, int splits, float* part,
+                      void* dx, int num_sms, unsigned* status, cudaStream_t stream);
+int launch_readout_dw(const CUtensorMap* dz, const CUtensorMap* xs, const ReadoutChunk& c, float* sum, bool first,
+                      bool last, void* dw, int num_sms, unsigned* status, cudaStream_t stream);
+// x *= *g in place (bf16, n a multiple of 8).
+int launch_scale_by(void* x, long n, const float* g, int num_sms, cudaStream_t stream);
+
 // tmap.cpp: a 2-D tensor map over a row-major [rows, cols] matrix of 1- or 2-byte elements (elem_bytes), with a
 // {box_cols, box_rows} box and the given swizzle (0, 32, 64 or 128 bytes). Returns 0 on success.
 int make_tmap_2d(CUtensorMap* map, int elem_bytes, const void* base, uint64_t rows, uint64_t cols,

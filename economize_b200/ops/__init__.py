@@ -14,6 +14,7 @@ from ._ext import available, load_error, require
 from .fp8 import FP8BlockWeight
 from .quant import QWeight
 from .sparse import Sparse24Weight
+from .training import linear_cross_entropy
 
 __all__ = [
     "argmax",
@@ -25,6 +26,7 @@ __all__ = [
     "kivi_quantize",
     "kv_compact",
     "linear",
+    "linear_cross_entropy",
     "linear_parts",
     "Partials",
     "load_error",

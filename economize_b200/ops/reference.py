@@ -19,6 +19,7 @@ __all__ = [
     "greedy_accept",
     "kv_compact",
     "linear",
+    "linear_cross_entropy",
     "rmsnorm",
     "rope_store",
     "silu_mul",
@@ -446,3 +447,16 @@ def kivi_quantize(cache: torch.Tensor, kivi: torch.Tensor, kv_len: torch.Tensor,
             v = cache[:, 1, b, :, c * 128:(c + 1) * 128]
             kivi[:, b, :, c] = pack_chunks(k, v, bits)
         chunks[b] = max(start, stop)
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100,
+                         reduction: str = "mean", logit_scale: float = 1.0) -> torch.Tensor:
+    """Cross-entropy of ``logit_scale * hidden [T, H] @ weight.T`` over the rows whose target is not
+    ``ignore_index`` (the other rows never enter a product); fp32 at least. ``"mean"`` of no row is 0."""
+    rows = (targets != ignore_index).nonzero()[:, 0]
+    wide = torch.promote_types(hidden.dtype, torch.float32)
+    logits = F.linear(hidden[rows].to(wide), weight.to(wide)) * logit_scale
+    nll = F.cross_entropy(logits, targets[rows], reduction="none")
+    if reduction == "none":
+        return torch.zeros(targets.shape, dtype=wide, device=hidden.device).index_copy(0, rows, nll)
+    return nll.sum() if reduction == "sum" else nll.sum() / max(1, rows.numel())

@@ -1,0 +1,99 @@
+"""Operators of training steps, with autograd: the readout cross-entropy and causal attention over packed documents.
+
+On CUDA both directions are the hand-written kernels of ``csrc/readout.cu`` and ``csrc/packed_attention.cu``; CPU
+tensors take the formulas of :mod:`.reference` (autograd differentiates them). There is no third path.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import reference
+from ._ext import require
+
+__all__ = ["linear_cross_entropy"]
+
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _autocast(*tensors: torch.Tensor) -> tuple[torch.Tensor, ...]:
+    """Under CUDA autocast to bfloat16, the operands in bfloat16 (their gradients return in their own type)."""
+    if tensors[0].is_cuda and torch.is_autocast_enabled("cuda") and \
+            torch.get_autocast_dtype("cuda") == torch.bfloat16:
+        return tuple(t.to(torch.bfloat16) for t in tensors)
+    return tensors
+
+
+class _Readout(torch.autograd.Function):
+    """Losses of the readout. A scalar loss computes its gradients in the forward pass, where the unnormalised
+    probabilities are at hand, and the backward pass scales them by the upstream gradient; per-row losses, whose
+    upstream gradients are not known by then, run the products again in the backward pass."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, ignore_index, logit_scale, reduction, chunk_rows):
+        ctx.need = ctx.needs_input_grad[:2]
+        ctx.args = (ignore_index, logit_scale)
+        ctx.reduction, ctx.chunk_rows = reduction, chunk_rows
+        ctx.save_for_backward(hidden, weight, targets)
+        now = reduction != 0
+        loss, dx, dw = require().readout(hidden, weight, targets, ignore_index, logit_scale, reduction,
+                                         now and ctx.need[0], now and ctx.need[1], None, chunk_rows)
+        ctx.grads = (dx, dw) if now else None
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        need_dx, need_dw = ctx.need
+        grads, ctx.grads = ctx.grads, None
+        hidden, weight, targets = ctx.saved_tensors
+        if grads is None and ctx.reduction == 0:
+            _, dx, dw = require().readout(hidden, weight, targets, *ctx.args, 0, need_dx, need_dw, grad.float(),
+                                          ctx.chunk_rows)
+        else:
+            if grads is None:  # a second pass over a retained graph: the first one gave the buffers away
+                grads = require().readout(hidden, weight, targets, *ctx.args, ctx.reduction, need_dx, need_dw, None,
+                                          ctx.chunk_rows)[1:]
+            dx, dw = grads
+            scale = grad.float()
+            for t in (dx, dw):
+                if t is not None:
+                    require().scale_by(t, scale)
+        return dx, dw, None, None, None, None, None
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *,
+                         ignore_index: int = -100, reduction: str = "mean", logit_scale: float = 1.0,
+                         chunk_rows: int = 0) -> torch.Tensor:
+    """Softmax cross-entropy of ``logit_scale * hidden @ weight.T`` against ``targets`` without keeping the logits,
+    differentiable in ``hidden`` and ``weight``.
+
+    Args:
+        hidden: States ``[..., H]`` (bf16 on CUDA, ``H`` a multiple of 8; cast under bf16 autocast).
+        weight: The vocabulary rows ``[V, H]``.
+        targets: Target ids ``[...]`` (int64). Rows whose target is ``ignore_index`` cost nothing, add nothing to the
+            loss and get zero gradients, whatever their states hold (NaN included). A target outside ``[0, V)`` is
+            ignored on CUDA and reported in the device status word.
+        reduction: ``"mean"`` over the rows with a target (0 when there is none), ``"sum"``, or ``"none"``:
+            per-row losses ``[...]`` (0 for ignored rows), whose backward pass computes the logits again.
+        chunk_rows: Rows processed at a time (0: as many as 1 GiB of 16-bit probabilities hold, more where a trained
+            ``weight`` needs as much for the sum over several chunks).
+    """
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {tuple(_REDUCTIONS)}, got {reduction!r}")
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} do not match")
+    if targets.shape != hidden.shape[:-1]:
+        raise ValueError(f"targets {tuple(targets.shape)} do not match hidden {tuple(hidden.shape)}")
+    hidden, weight = _autocast(hidden, weight)
+    flat = hidden.reshape(-1, hidden.shape[-1])
+    if hidden.is_cuda:
+        args = (flat, weight, targets.reshape(-1), int(ignore_index), float(logit_scale), _REDUCTIONS[reduction])
+        if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+            loss = _Readout.apply(*args, int(chunk_rows))
+        else:
+            loss = require().readout(*args, False, False, None, int(chunk_rows))[0]
+    else:
+        loss = reference.linear_cross_entropy(flat, weight, targets.reshape(-1), ignore_index, reduction, logit_scale)
+    return loss.reshape(targets.shape) if reduction == "none" else loss

@@ -1,0 +1,283 @@
+"""The readout cross-entropy against the same formula in 64 bits, element by element.
+
+Tolerances (bf16 inputs are exact in 64 bits, so only the kernels round):
+
+* a logit is an fp32 accumulation of H products: at most ``H 2^-23`` of the sum of their magnitudes;
+* ``dz`` is rounded to bf16 once (8 significant bits: ``2^-8`` relative) from an fp16 probability (``2^-11`` relative, ``2^-25`` of its
+  piece's largest absolute) and a log-sum-exp off by a logit's error;
+* ``dx`` and ``dW`` sum ``dz`` times exact factors in fp32 and are rounded to bf16 once more.
+"""
+
+import pytest
+import torch
+
+from economize_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def _inputs(dev, rows, hidden, vocab, masked=0.0, seed=0, lean=8.0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    w = (torch.randn(vocab, hidden, device=dev, generator=g) * 0.05).bfloat16()
+    y = torch.randint(0, vocab, (rows,), device=dev, generator=g)
+    x = torch.randn(rows, hidden, device=dev, generator=g)
+    near = w[y].float()
+    x = x + lean * torch.rand(rows, 1, device=dev, generator=g) * near / near.norm(dim=-1, keepdim=True)
+    y[torch.rand(rows, device=dev, generator=g) < masked] = -100
+    return x.bfloat16(), w, y
+
+
+def _oracle(x, w, y, scale, g_rows):
+    """64-bit losses and gradients, and the bounds of each output's error."""
+    keep = y != -100
+    h = x.shape[1]
+    xd, wd = torch.where(keep[:, None], x, 0).double(), w.double()
+    z = scale * xd @ wd.t()
+    eps = abs(scale) * (xd.abs() @ wd.t().abs()).amax(-1) * h * 2.0 ** -23 + z.abs().amax(-1) * 2.0 ** -22
+    logp = torch.log_softmax(z, -1)
+    at = torch.where(keep, y, 0)
+    nll = torch.where(keep, -logp.gather(1, at[:, None])[:, 0], 0.0)
+    p = logp.exp()
+    dz = p.clone()
+    dz[torch.arange(len(y)), at] -= 1
+    g = torch.where(keep, g_rows.double(), 0.0)[:, None] * scale
+    dz, p = dz * g, p * g.abs()
+    rel = 2.0 ** -8 + 2.0 ** -11 + 2.0 ** -16  # dz, e, the exponentials and factors
+    dz_err = dz.abs() * rel + p * (2.5 * eps[:, None]) + g.abs() * 2.0 ** -25
+    dx, dw = dz @ wd, dz.t() @ xd
+    dx_err = dz_err @ wd.abs() + dx.abs() * 2.0 ** -8 + dz.abs() @ wd.abs() * 2.0 ** -14
+    dw_err = dz_err.t() @ xd.abs() + dw.abs() * 2.0 ** -8 + dz.abs().t() @ xd.abs() * 2.0 ** -14
+    return dict(nll=nll, dx=dx, dw=dw, nll_err=2.5 * eps + nll.abs() * 2.0 ** -20 + 2.0 ** -21, dx_err=dx_err,
+                dw_err=dw_err, keep=keep)
+
+
+def _within(got, want, err, what):
+    off = (got.double() - want).abs()
+    assert (off <= err + 1e-30).all(), f"{what}: {(off / (err + 1e-30)).max().item():.2f} times the bound"
+
+
+SIZES = [(1, 8, 1), (1, 64, 7), (3, 72, 129), (16, 256, 1000), (65, 136, 255), (128, 64, 256), (129, 512, 4099),
+         (300, 1000, 50257), (513, 256, 2048)]
+
+
+@pytest.mark.parametrize("rows,hidden,vocab", SIZES)
+@pytest.mark.parametrize("masked", [0.0, 0.4])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_losses_and_gradients(cuda, rows, hidden, vocab, masked, reduction):
+    x, w, y = _inputs(cuda, rows, hidden, vocab, masked)
+    x.requires_grad_()
+    w.requires_grad_()
+    scale = 0.75 if masked else 1.0
+    loss = ops.linear_cross_entropy(x, w, y, reduction=reduction, logit_scale=scale)
+    count = max(1, int((y != -100).sum()))
+    if reduction == "none":
+        up = torch.linspace(-1.0, 2.0, rows, device=cuda)
+        g_rows = up
+    else:
+        up = torch.tensor(1.0, device=cuda)
+        g_rows = torch.full((rows,), 1.0 / count if reduction == "mean" else 1.0, device=cuda)
+    dx, dw = torch.autograd.grad(loss, (x, w), up)
+    o = _oracle(x.detach(), w.detach(), y, scale, g_rows)
+    if reduction == "none":
+        _within(loss, o["nll"], o["nll_err"], "losses")
+    else:
+        div = count if reduction == "mean" else 1
+        total, err = o["nll"].sum() / div, o["nll_err"][o["keep"]].sum() / div
+        _within(loss, total, err + total.abs() * 2.0 ** -20, "loss")
+    _within(dx, o["dx"], o["dx_err"], "dx")
+    _within(dw, o["dw"], o["dw_err"], "dw")
+    assert ops.require().status(0) == 0
+
+
+@pytest.mark.parametrize("chunk", [64, 128, 320])
+def test_chunks_of_rows(cuda, chunk):
+    """Several chunks: every output as from one, weight gradients summed in fp32 in between."""
+    x, w, y = _inputs(cuda, 333, 200, 1500, 0.2, seed=3)
+    x.requires_grad_()
+    w.requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, y, chunk_rows=chunk)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    count = int((y != -100).sum())
+    o = _oracle(x.detach(), w.detach(), y, 1.0, torch.full((333,), 1.0 / count, device=cuda))
+    _within(loss, o["nll"].sum() / count, o["nll_err"].sum() / count + 1e-6, "loss")
+    _within(dx, o["dx"], o["dx_err"], "dx")
+    _within(dw, o["dw"], o["dw_err"], "dw")
+
+
+@pytest.mark.parametrize("rows", [1, 70, 300])
+def test_no_row_has_a_target(cuda, rows):
+    x, w, y = _inputs(cuda, rows, 64, 500)
+    y.fill_(-100)
+    x.fill_(float("nan"))
+    x.requires_grad_()
+    w.requires_grad_()
+    for reduction in ("mean", "sum", "none"):
+        loss = ops.linear_cross_entropy(x, w, y, reduction=reduction)
+        dx, dw = torch.autograd.grad(loss.sum(), (x, w))
+        assert (loss == 0).all() and (dx == 0).all() and (dw == 0).all()
+
+
+def test_no_rows_at_all(cuda):
+    w = torch.randn(40, 64, device=cuda).bfloat16().requires_grad_()
+    x = torch.empty(0, 64, device=cuda, dtype=torch.bfloat16, requires_grad=True)
+    y = torch.empty(0, dtype=torch.long, device=cuda)
+    dx, dw = torch.autograd.grad(ops.linear_cross_entropy(x, w, y), (x, w))
+    assert dx.shape == x.shape and (dw == 0).all()
+    assert ops.linear_cross_entropy(x, w, y, reduction="none").shape == (0,)
+
+
+def test_masked_rows_hold_anything(cuda):
+    """NaN and infinities in ignored rows reach neither the loss nor a gradient."""
+    x, w, y = _inputs(cuda, 200, 128, 700, 0.3, seed=5)
+    clean = torch.where((y == -100)[:, None], torch.zeros_like(x), x)
+    dirty = x.clone()
+    dirty[y == -100] = float("nan")
+    dirty[(y == -100).nonzero()[::2, 0]] = float("inf")
+    out = []
+    for states in (clean, dirty):
+        s, v = states.clone().requires_grad_(), w.clone().requires_grad_()
+        loss = ops.linear_cross_entropy(s, v, y)
+        out.append((loss.detach(), *torch.autograd.grad(loss, (s, v))))
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+    assert torch.isfinite(out[1][0])
+
+
+def test_a_row_with_nan_states(cuda):
+    """Its loss is NaN, as the formula's is, and only its own row of dx."""
+    x, w, y = _inputs(cuda, 40, 64, 300, seed=6)
+    x[7, 3] = float("nan")
+    x.requires_grad_()
+    losses = ops.linear_cross_entropy(x, w, y, reduction="none")
+    (dx,) = torch.autograd.grad(losses, (x,), torch.ones_like(losses))
+    bad = torch.arange(40, device=cuda) == 7
+    assert torch.equal(torch.isnan(losses), bad)
+    assert torch.equal(torch.isnan(dx).any(-1), bad)
+
+
+def test_infinite_logits(cuda):
+    """Vocabulary rows whose logit is minus infinity have probability zero (their gradient is that of zero weight)."""
+    x, w, y = _inputs(cuda, 33, 64, 400, seed=7)
+    x = x.abs()
+    w[5:300] = float("-inf")
+    y = torch.where((y >= 5) & (y < 300), 0, y)
+    losses = ops.linear_cross_entropy(x, w, y, reduction="none")
+    keep = torch.cat([torch.arange(5), torch.arange(300, 400)]).to(cuda)
+    z = x.double() @ w[keep].double().t()
+    at = torch.where(y < 5, y, y - 295)
+    want = torch.logsumexp(z, -1) - z.gather(1, at[:, None])[:, 0]
+    assert ((losses.double() - want).abs() <= 64 * 2.0 ** -22 * z.abs().amax(-1) + 1e-6).all()
+
+
+def test_large_logits_do_not_overflow(cuda):
+    x, w, y = _inputs(cuda, 60, 256, 900, seed=8)
+    x, w = x * 40, w * 40
+    x.requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, y)
+    (dx,) = torch.autograd.grad(loss, (x,))
+    o = _oracle(x.detach(), w, y, 1.0, torch.full((60,), 1 / 60, device=cuda))
+    _within(loss, o["nll"].mean(), o["nll_err"].mean() + o["nll"].mean() * 2.0 ** -20, "loss")
+    assert torch.isfinite(dx).all()
+
+
+def test_strided_operands_and_leading_dimensions(cuda):
+    x, w, y = _inputs(cuda, 96, 128, 640, 0.1, seed=9)
+    wide_x = torch.full((96, 256), float("nan"), device=cuda, dtype=torch.bfloat16)
+    wide_w = torch.full((640, 136), float("nan"), device=cuda, dtype=torch.bfloat16)
+    wide_x[:, 64:192] = x
+    wide_w[:, 8:] = w
+    odd_x = torch.empty(96 * 129, device=cuda, dtype=torch.bfloat16)[: 96 * 129].view(96, 129)
+    odd_x[:, 1:] = x
+    want = ops.linear_cross_entropy(x, w, y)
+    assert torch.equal(want, ops.linear_cross_entropy(wide_x[:, 64:192], wide_w[:, 8:], y))
+    assert torch.equal(want, ops.linear_cross_entropy(odd_x[:, 1:], w.t().contiguous().t(), y))
+    both = ops.linear_cross_entropy(x.view(4, 24, 128), w, y.view(4, 24), reduction="none")
+    assert both.shape == (4, 24)
+    assert torch.equal(both.flatten(), ops.linear_cross_entropy(x, w, y, reduction="none"))
+
+
+def test_same_bits_every_time_and_twice_through_one_graph(cuda):
+    x, w, y = _inputs(cuda, 257, 264, 3001, 0.2, seed=10)
+    x.requires_grad_()
+    w.requires_grad_()
+    runs = []
+    for _ in range(3):
+        loss = ops.linear_cross_entropy(x, w, y)
+        runs.append((loss, *torch.autograd.grad(loss, (x, w))))
+    for a in runs[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(a, runs[0]))
+    loss = ops.linear_cross_entropy(x, w, y)
+    first = [t.clone() for t in torch.autograd.grad(loss * 2, (x, w), retain_graph=True)]
+    second = torch.autograd.grad(loss * 2, (x, w))
+    assert all(torch.equal(p, q) for p, q in zip(first, second))
+    assert torch.equal(first[0], runs[0][1] * 2) and torch.equal(first[1], runs[0][2] * 2)
+
+
+def test_only_what_is_asked_for(cuda):
+    """A frozen weight or frozen states get no gradient; without any the losses are the same."""
+    x, w, y = _inputs(cuda, 100, 128, 1000, 0.1, seed=11)
+    base = ops.linear_cross_entropy(x, w, y)
+    a = x.clone().requires_grad_()
+    la = ops.linear_cross_entropy(a, w, y)
+    la.backward()
+    b = w.clone().requires_grad_()
+    lb = ops.linear_cross_entropy(x, b, y)
+    lb.backward()
+    assert torch.equal(base, la.detach()) and torch.equal(base, lb.detach())
+    with torch.no_grad():
+        assert not ops.linear_cross_entropy(a, b, y).requires_grad
+
+
+def test_autocast_takes_fp32_masters(cuda):
+    x, w, y = _inputs(cuda, 50, 64, 300, seed=12)
+    xf, wf = x.float().requires_grad_(), w.float().requires_grad_()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        loss = ops.linear_cross_entropy(xf, wf, y)
+    loss.backward()
+    xb, wb = x.clone().requires_grad_(), w.clone().requires_grad_()
+    ops.linear_cross_entropy(xb, wb, y).backward()
+    assert xf.grad.dtype == torch.float32
+    assert torch.equal(xf.grad, xb.grad.float()) and torch.equal(wf.grad, wb.grad.float())
+
+
+def test_on_another_stream(cuda):
+    x, w, y = _inputs(cuda, 120, 128, 2000, seed=13)
+    want = ops.linear_cross_entropy(x, w, y)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.linear_cross_entropy(x, w, y)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(want, got)
+
+
+def test_target_out_of_range_is_ignored_and_reported(cuda):
+    x, w, y = _inputs(cuda, 30, 64, 200, seed=14)
+    y[4], y[9] = 200, -3
+    masked = y.clone()
+    masked[4] = masked[9] = -100
+    ops.require().status(0)
+    got = ops.linear_cross_entropy(x, w, y)
+    assert ops.require().status(0) & 32
+    assert torch.equal(got, ops.linear_cross_entropy(x, w, masked))
+    assert ops.require().status(0) == 0
+
+
+def test_refusals(cuda):
+    x, w, y = _inputs(cuda, 10, 64, 50, seed=15)
+    with pytest.raises(ValueError, match="reduction"):
+        ops.linear_cross_entropy(x, w, y, reduction="max")
+    with pytest.raises(ValueError, match="do not match"):
+        ops.linear_cross_entropy(x[:, :32], w, y)
+    with pytest.raises(ValueError, match="do not match"):
+        ops.linear_cross_entropy(x, w, y[:5])
+    with pytest.raises(RuntimeError, match="bfloat16"):
+        ops.linear_cross_entropy(x.float(), w, y)
+    with pytest.raises(RuntimeError, match="bfloat16"):
+        ops.linear_cross_entropy(x, w.half(), y)
+    with pytest.raises(RuntimeError, match="int64"):
+        ops.linear_cross_entropy(x, w, y.int())
+    with pytest.raises(RuntimeError, match="device"):
+        ops.linear_cross_entropy(x, w.cpu(), y)
+    with pytest.raises(RuntimeError, match="multiple of 8"):
+        ops.linear_cross_entropy(x[:, :60].contiguous(), w[:, :60].contiguous(), y)
