@@ -4,6 +4,7 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <tuple>
 
@@ -164,6 +165,143 @@ std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> readout(
   return {loss, dx, dw};
 }
 
+// A [T, heads, D] operand as TMA reads it: unit stride along D, 16-byte strides and base.
+Tensor heads_of(const Tensor& x) {
+  const auto step = [&](int d) { return x.size(d) > 1 ? x.stride(d) : int64_t{8}; };
+  const bool ok = x.stride(2) == 1 && step(0) > 0 && step(1) > 0 && step(0) % 8 == 0 && step(1) % 8 == 0 &&
+                  reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  if (ok) return x;
+  Tensor y = x.contiguous();
+  return reinterpret_cast<uintptr_t>(y.data_ptr()) % 16 == 0 ? y : y.clone();
+}
+
+CUtensorMap map_heads(const Tensor& x, int box_tokens) {
+  CUtensorMap map;
+  std::memset(&map, 0, sizeof(map));
+  const auto step = [&](int d, int64_t one) { return x.size(d) > 1 ? x.stride(d) : one; };
+  const int rc = ecz::make_tmap_heads(&map, x.data_ptr(), x.size(0), x.size(1), x.size(2),
+                                      step(0, x.size(1) * x.size(2)), step(1, x.size(2)), box_tokens);
+  TORCH_CHECK(rc == 0, "cuTensorMapEncodeTiled failed (code ", rc, ") for a [", x.size(0), ", ", x.size(1), ", ",
+              x.size(2), "] operand");
+  return map;
+}
+
+void check_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, double scale) {
+  CHECK_CUDA(q);
+  CHECK_BF16(q);
+  CHECK_BF16(k);
+  CHECK_BF16(v);
+  CHECK_I32(cu);
+  CHECK_ON(k, q);
+  CHECK_ON(v, q);
+  CHECK_ON(cu, q);
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, "packed_attention expects q [T, H, D], k / v [T, Hkv, D]");
+  TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(2) == q.size(2),
+              "packed_attention: q ", q.sizes(), ", k ", k.sizes(), " and v ", v.sizes(), " do not match");
+  const int64_t T = q.size(0), H = q.size(1), Hkv = k.size(1), D = q.size(2);
+  TORCH_CHECK(Hkv >= 1 && H >= 1 && H % Hkv == 0, "packed_attention: ", H, " query heads over ", Hkv, " K/V heads");
+  TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "packed_attention: head dimensions 8 to 128 in steps of 8 (got ", D,
+              ")");
+  TORCH_CHECK(cu.dim() == 1 && cu.size(0) >= 1, "packed_attention: cu_seqlens must be [B + 1]");
+  TORCH_CHECK(T <= (int64_t{1} << 30) && cu.size(0) <= (int64_t{1} << 24), "packed_attention: too many tokens");
+  TORCH_CHECK(scale > 0 && std::isfinite(scale), "packed_attention: the scale must be positive (got ", scale, ")");
+}
+
+// Tile table of packed sequences (rows 128 or 256) in `buf`; fills args.
+Tensor packed_plan(const Tensor& q, const Tensor& k, const Tensor& cu, int rows, double scale, ecz::PackedArgs& a,
+                   cudaStream_t stream) {
+  const int T = static_cast<int>(q.size(0)), B = static_cast<int>(cu.size(0)) - 1;
+  a.T = T;
+  a.H = static_cast<int>(q.size(1));
+  a.Hkv = static_cast<int>(k.size(1));
+  a.D = static_cast<int>(q.size(2));
+  a.scale = static_cast<float>(scale);
+  a.max_tiles = std::max(1, ecz::packed_max_tiles(T, B, rows));
+  Tensor buf = at::empty({int64_t{4} * a.max_tiles + 4 + 2 * (int64_t{B} + 1)}, cu.options());
+  int* base = buf.data_ptr<int>();
+  a.table = base;
+  a.head = base + int64_t{4} * a.max_tiles;
+  TORCH_CHECK(ecz::launch_packed_plan(cu.data_ptr<int>(), B, T, rows, a.max_tiles, base, base + int64_t{4} * a.max_tiles,
+                                      base + int64_t{4} * a.max_tiles + 4, ecz::device_status(q.device()), stream) == 0,
+              "packed_attention: plan launch failed");
+  return buf;
+}
+
+// Output [T, H, D] and, for a backward pass, the log2-domain log-sum-exp of every row [H, T].
+std::tuple<Tensor, c10::optional<Tensor>> packed_forward(Tensor q, Tensor k, Tensor v, Tensor cu, double scale,
+                                                         bool need_lse) {
+  check_packed(q, k, v, cu, scale);
+  c10::cuda::CUDAGuard guard(q.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  Tensor out = at::empty(q.sizes(), q.options());
+  c10::optional<Tensor> lse;
+  if (need_lse) lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+  if (q.size(0) == 0) return {out, lse};
+  q = heads_of(q);
+  k = heads_of(k);
+  v = heads_of(v);
+  cu = cu.contiguous();
+  const bool row_pairs = (q.size(1) / k.size(1)) % 2 != 0;
+  ecz::PackedArgs a;
+  Tensor plan = packed_plan(q, k, cu, row_pairs ? 256 : 128, scale, a, stream);
+  ecz::PackedMaps maps;
+  maps.q = map_heads(q, 128);
+  maps.k = map_heads(k, 128);
+  maps.v = map_heads(v, 128);
+  const int rc = ecz::launch_packed_forward(maps, a, out.data_ptr(), need_lse ? lse->data_ptr<float>() : nullptr,
+                                            row_pairs, ecz::device_status(q.device()), stream);
+  TORCH_CHECK(rc == 0, "packed_attention: forward launch failed (", rc, ")");
+  return {out, lse};
+}
+
+// Gradients of q, k and v (those asked for) given the output's.
+std::tuple<c10::optional<Tensor>, c10::optional<Tensor>, c10::optional<Tensor>> packed_backward(
+    Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor cu, double scale, bool need_dq,
+    bool need_dkv) {
+  check_packed(q, k, v, cu, scale);
+  CHECK_BF16(dout);
+  CHECK_ON(dout, q);
+  CHECK_ON(out, q);
+  CHECK_ON(lse, q);
+  TORCH_CHECK(dout.sizes() == q.sizes() && out.sizes() == q.sizes() && out.is_contiguous() &&
+                  out.scalar_type() == at::kBFloat16,
+              "packed_attention: the output and its gradient have the queries' shape");
+  TORCH_CHECK(lse.is_contiguous() && lse.scalar_type() == at::kFloat && lse.numel() == q.size(0) * q.size(1),
+              "packed_attention: lse must be fp32 [H, T]");
+  c10::cuda::CUDAGuard guard(q.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  c10::optional<Tensor> dq, dk, dv;
+  if (need_dq) dq = at::empty(q.sizes(), q.options());
+  if (need_dkv) {
+    dk = at::empty(k.sizes(), k.options());
+    dv = at::empty(v.sizes(), v.options());
+  }
+  if (q.size(0) == 0 || (!need_dq && !need_dkv)) return {dq, dk, dv};
+  q = heads_of(q);
+  k = heads_of(k);
+  v = heads_of(v);
+  dout = heads_of(dout);
+  cu = cu.contiguous();
+  const int T = static_cast<int>(q.size(0)), H = static_cast<int>(q.size(1)), D = static_cast<int>(q.size(2));
+  ecz::PackedArgs a;
+  Tensor plan = packed_plan(q, k, cu, 128, scale, a, stream);
+  Tensor delta = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+  TORCH_CHECK(ecz::launch_packed_delta(out.data_ptr(), dout.data_ptr(), dout.stride(0), dout.stride(1), T, H, D,
+                                       delta.data_ptr<float>(), stream) == 0,
+              "packed_attention: delta launch failed");
+  ecz::PackedMaps maps;
+  maps.q = map_heads(q, 128);
+  maps.k = map_heads(k, 128);
+  maps.v = map_heads(v, 128);
+  maps.dout = map_heads(dout, 128);
+  const int rc = ecz::launch_packed_backward(maps, a, lse.data_ptr<float>(), delta.data_ptr<float>(),
+                                             need_dq ? dq->data_ptr() : nullptr, need_dkv ? dk->data_ptr() : nullptr,
+                                             need_dkv ? dv->data_ptr() : nullptr, ecz::device_status(q.device()),
+                                             stream);
+  TORCH_CHECK(rc == 0, "packed_attention: backward launch failed (", rc, ")");
+  return {dq, dk, dv};
+}
+
 // x *= g (a scalar on the device) in place.
 void scale_by(Tensor x, Tensor g) {
   CHECK_CUDA(x);
@@ -188,6 +326,11 @@ void bind_training(pybind11::module_& m) {
         py::arg("hidden"), py::arg("weight"), py::arg("targets"), py::arg("ignore_index"), py::arg("logit_scale"),
         py::arg("reduction"), py::arg("need_dx"), py::arg("need_dw"), py::arg("grad_rows") = py::none(),
         py::arg("chunk_rows") = 0);
+  m.def("packed_forward", &packed_forward, "causal attention over packed sequences (tcgen05)", py::arg("q"),
+        py::arg("k"), py::arg("v"), py::arg("cu_seqlens"), py::arg("scale"), py::arg("need_lse"));
+  m.def("packed_backward", &packed_backward, "gradients of packed_forward", py::arg("dout"), py::arg("q"),
+        py::arg("k"), py::arg("v"), py::arg("out"), py::arg("lse"), py::arg("cu_seqlens"), py::arg("scale"),
+        py::arg("need_dq"), py::arg("need_dkv"));
   m.def("scale_by", &scale_by, "x *= g in place for a device scalar g (no memory pass when g is 1)");
 }
 

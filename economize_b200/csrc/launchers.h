@@ -305,6 +305,37 @@ int launch_readout_dw(const CUtensorMap* dz, const CUtensorMap* xs, const Readou
 // x *= *g in place (bf16, n a multiple of 8).
 int launch_scale_by(void* x, long n, const float* g, int num_sms, cudaStream_t stream);
 
+// packed_attention.cu: causal attention over packed sequences (see the file comment). Maps: 3-D {D, heads, T}, box
+// {64, 1, 128}, 128-byte swizzle.
+struct PackedMaps {
+  CUtensorMap q, k, v, dout;
+};
+struct PackedArgs {
+  const void* table = nullptr;  // int4 [max_tiles] of launch_packed_plan
+  const int* head = nullptr;    // int [4]
+  int max_tiles = 0, T = 0, H = 0, Hkv = 0, D = 0;
+  float scale = 1.f;
+};
+// Most tiles of `rows` rows that B sequences of T tokens in all can have.
+int packed_max_tiles(int T, int B, int rows);
+// scratch: 2 (B + 1) ints.
+int launch_packed_plan(const int* cu, int B, int T, int rows, int max_tiles, void* table, int* head, int* scratch,
+                       unsigned* status, cudaStream_t stream);
+// The table's tiles are 256 rows with row_pairs, else 128 (then H / Hkv is even).
+int launch_packed_forward(const PackedMaps& maps, const PackedArgs& a, void* out, float* lse, bool row_pairs,
+                          unsigned* status, cudaStream_t stream);
+
+// packed_attention_bwd.cu: delta [H, T] = rows of dout . out (out contiguous [T, H, D]), then the gradients (dq null:
+// not computed; dk and dv null: not computed). The table's tiles are 128 rows.
+int launch_packed_delta(const void* out, const void* dout, long stride_t, long stride_h, int T, int H, int D,
+                        float* delta, cudaStream_t stream);
+int launch_packed_backward(const PackedMaps& maps, const PackedArgs& a, const float* lse, const float* delta, void* dq,
+                           void* dk, void* dv, unsigned* status, cudaStream_t stream);
+
+// tmap.cpp: 3-D bf16 tensor map {d, heads, tokens} with strides in elements, box {64, 1, box_tokens}, 128-byte swizzle.
+int make_tmap_heads(CUtensorMap* map, const void* base, uint64_t tokens, uint64_t heads, uint64_t d,
+                    uint64_t token_stride, uint64_t head_stride, uint32_t box_tokens);
+
 // tmap.cpp: a 2-D tensor map over a row-major [rows, cols] matrix of 1- or 2-byte elements (elem_bytes), with a
 // {box_cols, box_rows} box and the given swizzle (0, 32, 64 or 128 bytes). Returns 0 on success.
 int make_tmap_2d(CUtensorMap* map, int elem_bytes, const void* base, uint64_t rows, uint64_t cols,

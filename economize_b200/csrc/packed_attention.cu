@@ -1,0 +1,440 @@
+// Causal attention over packed sequences with grouped heads: the forward pass (training and scoring prompts).
+//
+//   s_ij = scale q_i . k_j (a <= j <= i < b for the sequence [a, b) of token i)     L_i = log sum_j exp s_ij
+//   o_i = sum_j exp(s_ij - L_i) v_j
+//
+// Tokens of all sequences lie one after another, q [T, H, D], k / v [T, Hkv, D]; sequence n holds the tokens
+// [cu[n], cu[n + 1]). The plan kernel cuts every sequence into tiles of 128 (or 256) rows that start at the
+// sequence's first token, so a tile never mixes sequences, and lists them heaviest first (a causal row tile's work is
+// its distance from the start): the grid's last CTAs are the short ones.
+//
+// Forward CTA: two query tiles of 128 rows that share the K / V chunks: the same rows of two heads of a group (an even
+// number of heads per K/V head), else 256 rows of one head. One warp loads (TMA, a ring of 128-key K and V chunks), one
+// issues the MMAs, and two warpgroups run the softmax of a tile each, one thread per row, so the tensor cores work on
+// one tile while the other's exponentials run. S and P share TMEM columns (P overwrites S as bf16 and is the A operand
+// of P . V), O accumulates in TMEM. A row's reference maximum moves only when a chunk raises it by more than 2^8
+// (lazy rescaling), so O is rarely read back before the end.
+//
+// A chunk that reaches past its sequence's end holds other rows (the next sequence's, or unwritten padding): their
+// scores are replaced, not multiplied, and the at most 15 V rows that P . V reads in its last K step beyond the end
+// are zeroed in shared memory, so NaN or infinities there reach nothing.
+#include <algorithm>
+
+#include "launchers.h"
+#include "packed_common.cuh"
+
+namespace ecz {
+
+using namespace packed;
+
+namespace {
+
+constexpr float kLazy = 8.f;  // log2 units
+
+// ---- plan ----------------------------------------------------------------------------------------------------------
+// Tile list of `rows`-row tiles, heaviest first: table[i] = (first token, end, tile, tiles of its sequence). head =
+// (tiles, first token of the first sequence, end of the last, 0). Offsets outside [0, T] or falling are clamped (a
+// sequence starts where the one before it ended at the earliest) and reported. lo / base: [B + 1] scratch.
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanBins = 4096;
+
+__device__ __forceinline__ int scan_add(int v, int* warp_sums, int& total) {  // exclusive, over the block
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    if (w < warp) before += warp_sums[w];
+    total += warp_sums[w];
+  }
+  __syncthreads();
+  return before + x - v;
+}
+
+__device__ __forceinline__ int scan_max(int v, int* warp_max) {  // inclusive
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v = max(v, y);
+  }
+  if (lane == 31) warp_max[warp] = v;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) v = max(v, warp_max[w]);
+  __syncthreads();
+  return v;
+}
+
+__global__ void __launch_bounds__(kPlanThreads)
+    packed_plan_kernel(const int* __restrict__ cu, int B, int T, int rows, int max_tiles, int4* __restrict__ table,
+                       int* __restrict__ head, int* __restrict__ lo, int* __restrict__ base, unsigned* status) {
+  __shared__ int sums[32];
+  __shared__ int hist[kPlanBins];  // tiles of weight bin w, then the place of the next one
+  __shared__ int carry_max, carry_tiles;
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x;
+  // weight of tile i: i + 1 chunks; bins of `per` weights each
+  const int per = (max_tiles + kPlanBins - 2) / (kPlanBins - 1);
+  for (int i = tid; i < kPlanBins; i += kPlanThreads) hist[i] = 0;
+  if (tid == 0) {
+    carry_max = 0;
+    carry_tiles = 0;
+  }
+  __syncthreads();
+  for (int s0 = 0; s0 <= B; s0 += kPlanThreads) {
+    const int s = s0 + tid;
+    const int raw = s <= B ? cu[s] : 0;
+    int edge = max(0, min(T, raw));
+    const int before = carry_max;
+    edge = max(before, scan_max(edge, sums));
+    if (s <= B) {
+      if (edge != raw) atomicOr(status, kStatusBadIndex);
+      lo[s] = edge;
+    }
+    __syncthreads();
+    if (tid == kPlanThreads - 1) carry_max = edge;
+    __syncthreads();
+  }
+  for (int s0 = 0; s0 < B; s0 += kPlanThreads) {
+    const int s = s0 + tid;
+    const int n = s < B ? (lo[s + 1] - lo[s] + rows - 1) / rows : 0;
+    int total;
+    const int at = carry_tiles + scan_add(n, sums, total);
+    if (s < B) base[s] = at;
+    // one tile of every weight 1 .. n: in bins 0 .. (n - 1) / per
+    for (int b = 0; b * per < n; ++b) atomicAdd(&hist[b], min(per, n - b * per));
+    __syncthreads();
+    if (tid == 0) carry_tiles += total;
+    __syncthreads();
+  }
+  const int tiles = min(carry_tiles, max_tiles);
+  if (tid == 0) {
+    base[B] = carry_tiles;
+    head[0] = tiles;
+    head[1] = lo[0];
+    head[2] = lo[B];
+  }
+  __syncthreads();
+  // places: heaviest bin first
+  {
+    int v[kPlanBins / kPlanThreads];
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < kPlanBins / kPlanThreads; ++j) {
+      v[j] = hist[kPlanBins - 1 - (tid * (kPlanBins / kPlanThreads) + j)];
+      mine += v[j];
+    }
+    int total;
+    int at = scan_add(mine, sums, total);
+#pragma unroll
+    for (int j = 0; j < kPlanBins / kPlanThreads; ++j) {
+      hist[kPlanBins - 1 - (tid * (kPlanBins / kPlanThreads) + j)] = at;
+      at += v[j];
+    }
+  }
+  __syncthreads();
+  for (int t = tid; t < tiles; t += kPlanThreads) {
+    int a = 0, b = B - 1;  // the last sequence whose first tile is t or earlier
+    while (a < b) {
+      const int m = (a + b + 1) >> 1;
+      if (base[m] <= t) a = m; else b = m - 1;
+    }
+    const int i = t - base[a];
+    const int at = atomicAdd(&hist[i / per], 1);
+    if (at < max_tiles) table[at] = make_int4(lo[a], lo[a + 1], i, (lo[a + 1] - lo[a] + rows - 1) / rows);
+  }
+}
+
+// ---- forward -------------------------------------------------------------------------------------------------------
+constexpr int kFwdThreads = 384;
+
+template <int DP>
+struct FwdCfg {
+  static constexpr int kTileBytes = kRowsT * DP * 2;
+  static constexpr int kRing = DP == 64 ? 10 : 5;  // K and V chunks in turn
+  static constexpr int kSmem = (2 + kRing) * kTileBytes + 1024 + 256;
+  static_assert(kSmem <= 232448, "227 KB of shared memory");
+};
+
+struct FwdArgs {
+  bf16* out;   // [T, H, D]
+  float* lse;  // [H, T] log2-domain log-sum-exp, or null
+  const int4* table;
+  const int* head;
+  int T, H, Hkv, D;
+  float scale2;    // scale times log2(e)
+  bool row_pairs;  // tiles of 256 rows of one head (else 128 rows of two heads of a group)
+};
+
+template <int DP>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+    packed_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FwdArgs p, unsigned* status) {
+  using Cfg = FwdCfg<DP>;
+  constexpr int kRing = Cfg::kRing, kTileBytes = Cfg::kTileBytes;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_tiles = smem;
+  uint8_t* ring = smem + 2 * kTileBytes;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + kRing * kTileBytes);
+  uint64_t* kv_full = q_full + 1;
+  uint64_t* kv_empty = kv_full + kRing;
+  uint64_t* s_full = kv_empty + kRing;   // [2] scores of a tile's chunk are in TMEM
+  uint64_t* p_ready = s_full + 2;        // [2] its probabilities are
+  uint64_t* o_done = p_ready + 2;        // [2] P . V of the chunk is complete
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_ready[i], 4);
+      mbar_init(&o_done[i], 1);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  __syncwarp();
+  if (warp == 0) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_trigger();
+  pdl_wait();
+
+  const int per = p.row_pairs ? p.H : p.H / 2;
+  const int entry = blockIdx.x / per, sub = blockIdx.x % per;
+  zero_padding(p.out, p.T, static_cast<long>(p.H) * p.D, p.head);
+  if (entry < p.head[0]) {
+    const int4 tile = p.table[entry];
+    const int lo = tile.x, hi = tile.y;
+    const int group = p.H / p.Hkv;
+    int head[2], row0[2], chunks[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      head[i] = p.row_pairs ? sub : 2 * sub + i;
+      row0[i] = p.row_pairs ? lo + tile.z * 256 + i * 128 : lo + tile.z * 128;
+      chunks[i] = row0[i] < hi ? (row0[i] - lo) / kRowsT + 1 : 0;  // the last one holds the diagonal
+    }
+    const int kvh = head[0] / group;
+    const int n_chunks = max(chunks[0], chunks[1]);
+    const int ksteps = (p.D + 15) / 16;
+
+    if (warp == 0) {
+      if (lane == 0) {
+        // ---- loads: Q, then K and V chunks in turn ----
+        const uint32_t qa = smem_u32(q_tiles), ra = smem_u32(ring);
+        mbar_arrive_expect_tx(q_full, (chunks[1] > 0 ? 2 : 1) * kTileBytes);
+        load_tile<DP>(qa, &tm_q, q_full, head[0], row0[0]);
+        if (chunks[1] > 0) load_tile<DP>(qa + kTileBytes, &tm_q, q_full, head[1], row0[1]);
+        for (int it = 0; it < 2 * n_chunks; ++it) {
+          const int s = it % kRing;
+          if (!mbar_wait(&kv_empty[s], ((it / kRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag)) break;
+          mbar_arrive_expect_tx(&kv_full[s], kTileBytes);
+          load_tile<DP>(ra + s * kTileBytes, (it & 1) ? &tm_v : &tm_k, &kv_full[s], kvh, lo + (it >> 1) * kRowsT);
+        }
+      }
+    } else if (warp == 1) {
+      // ---- MMAs ----
+      const uint32_t qa = smem_u32(q_tiles), ra = smem_u32(ring);
+      auto wait_ring = [&](int it) {
+        return warp_wait(&kv_full[it % kRing], (it / kRing) & 1, status, kStatusWaitFull,
+                                                 abort_flag);
+      };
+      auto keys_of = [&](int c) { return min(kRowsT, hi - (lo + c * kRowsT)); };
+      bool ok = warp_wait(q_full, 0, status, kStatusWaitFull, abort_flag) && wait_ring(0);
+      tc_fence_after();
+      if (ok && lane == 0) {
+        const int n = (keys_of(0) + 15) & ~15;
+        for (int i = 0; i < 2; ++i) {
+          if (chunks[i] == 0) continue;
+          mma_dims(tmem + i * 128, qa + i * kTileBytes, ra, n, ksteps);
+          umma_commit(&s_full[i]);
+        }
+        umma_commit(&kv_empty[0]);
+      }
+      for (int c = 0; ok && c < n_chunks; ++c) {
+        const int v_it = 2 * c + 1, k_it = 2 * c + 2;
+        const bool more = c + 1 < n_chunks;
+        ok = wait_ring(v_it) && (!more || wait_ring(k_it));
+        if (!ok) break;
+        const int n = keys_of(c), n16 = (n + 15) & ~15;
+        uint8_t* v_tile = ring + (v_it % kRing) * kTileBytes;
+        if (n16 != n) zero_rows<DP>(v_tile, n, n16, lane);
+        for (int i = 0; ok && i < 2; ++i) {
+          if (c >= chunks[i]) continue;
+          ok = warp_wait(&p_ready[i], c & 1, status, kStatusWaitAccum, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            mma_rows(tmem + 256 + i * DP, tmem + i * 128, 32, smem_u32(v_tile), ksteps * 16, n16 / 16, c > 0);
+            umma_commit(&o_done[i]);
+            if (c + 1 < chunks[i]) {
+              mma_dims(tmem + i * 128, qa + i * kTileBytes, ra + (k_it % kRing) * kTileBytes,
+                       (keys_of(c + 1) + 15) & ~15, ksteps);
+              umma_commit(&s_full[i]);
+            }
+          }
+          __syncwarp();
+        }
+        if (lane == 0) {
+          umma_commit(&kv_empty[v_it % kRing]);
+          if (more) umma_commit(&kv_empty[k_it % kRing]);
+        }
+      }
+    } else if (warp >= 4) {
+      // ---- softmax: one thread per row ----
+      const int i = (warp - 4) >> 2, quad = warp & 3;
+      const int n_mine = i == 0 ? chunks[0] : chunks[1];
+      const int first_row = i == 0 ? row0[0] : row0[1], my_head = i == 0 ? head[0] : head[1];
+      const int row = first_row + quad * 32 + lane;
+      const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+      const uint32_t s_addr = lane_base + i * 128, o_addr = lane_base + 256 + i * DP;
+      float ref = -INFINITY, sum = 0.f;
+      bool ok = true;
+      for (int c = 0; c < n_mine; ++c) {
+        ok = warp_wait(&s_full[i], c & 1, status, kStatusWaitAccum, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        float v[128];
+        tmem_load128(s_addr, v);
+        if (c == n_mine - 1) {  // the diagonal and the sequence's end
+          const int limit = min(hi, row + 1) - (lo + c * kRowsT);
+#pragma unroll
+          for (int j = 0; j < 128; ++j) v[j] = j < limit ? v[j] : -INFINITY;
+        }
+        float m0 = v[0], m1 = v[1], m2 = v[2], m3 = v[3];
+#pragma unroll
+        for (int j = 4; j < 128; j += 4) {
+          m0 = fmaxf(m0, v[j]);
+          m1 = fmaxf(m1, v[j + 1]);
+          m2 = fmaxf(m2, v[j + 2]);
+          m3 = fmaxf(m3, v[j + 3]);
+        }
+        const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * p.scale2;
+        const bool raise = top > ref + kLazy;  // also the first finite maximum (ref = -inf)
+        const float new_ref = raise ? top : ref;
+        if (c > 0 && __any_sync(0xffffffffu, raise && sum != 0.f)) {
+          const float f = raise ? ex2(ref - new_ref) : 1.f;
+          ok = warp_wait(&o_done[i], (c - 1) & 1, status, kStatusWaitAccum, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          sum *= f;
+#pragma unroll 1
+          for (int d = 0; d < DP; d += 16) {
+            float o[16];
+            tmem_ld16(o_addr + d, o);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j] *= f;
+            tmem_st16(o_addr + d, o);
+          }
+        }
+        ref = new_ref;
+        const float shift = ref == -INFINITY ? 0.f : ref;
+        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+        uint32_t w[32];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float a = ex2(fmaf(v[h * 64 + 2 * j], p.scale2, -shift));
+            const float b = ex2(fmaf(v[h * 64 + 2 * j + 1], p.scale2, -shift));
+            const float x = ex2(fmaf(v[h * 64 + 2 * j + 2], p.scale2, -shift));
+            const float y = ex2(fmaf(v[h * 64 + 2 * j + 3], p.scale2, -shift));
+            s0 += a;
+            s1 += b;
+            s2 += x;
+            s3 += y;
+            w[j] = pack_bf16(a, b);
+            w[j + 1] = pack_bf16(x, y);
+          }
+          tmem_store32(s_addr + h * 32, w);
+        }
+        sum += (s0 + s1) + (s2 + s3);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[i]);
+      }
+      if (n_mine > 0 && ok) {
+        ok = warp_wait(&o_done[i], (n_mine - 1) & 1, status, kStatusWaitAccum, abort_flag);
+        if (ok) {
+          tc_fence_after();
+          const float inv = 1.f / sum;
+          const bool real = row < hi;
+          bf16* dst = p.out + (static_cast<long>(row) * p.H + my_head) * p.D;
+#pragma unroll 1
+          for (int d = 0; d < DP; d += 32) {
+            float o[32];
+            tmem_load32(o_addr + d, o);
+            if (real) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 8)
+                if (d + j < p.D)
+                  *reinterpret_cast<uint4*>(dst + d + j) =
+                      make_uint4(pack_bf16(o[j] * inv, o[j + 1] * inv), pack_bf16(o[j + 2] * inv, o[j + 3] * inv),
+                                 pack_bf16(o[j + 4] * inv, o[j + 5] * inv), pack_bf16(o[j + 6] * inv, o[j + 7] * inv));
+            }
+          }
+          if (real && p.lse != nullptr) p.lse[static_cast<long>(my_head) * p.T + row] = ref + log2f(sum);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  settle(*abort_flag != 0);
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+template <int DP>
+int run_fwd(const PackedMaps& maps, const PackedArgs& a, void* out, float* lse, bool row_pairs, unsigned* status,
+            cudaStream_t stream) {
+  auto kernel = packed_fwd_kernel<DP>;
+  if (set_max_smem(kernel, FwdCfg<DP>::kSmem) != cudaSuccess) return -1;
+  const FwdArgs args{static_cast<bf16*>(out), lse, static_cast<const int4*>(a.table), a.head, a.T, a.H, a.Hkv, a.D,
+                     a.scale * kLog2e, row_pairs};
+  const long grid = static_cast<long>(a.max_tiles) * (row_pairs ? a.H : a.H / 2);
+  if (grid > 0x7fffffffl) return -2;
+  return launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(kFwdThreads), FwdCfg<DP>::kSmem, stream, maps.q,
+                    maps.k, maps.v, args, status) == cudaSuccess ? 0 : -1;
+}
+
+}  // namespace
+
+int packed_max_tiles(int T, int B, int rows) {
+  return static_cast<int>(std::min<long>(T, static_cast<long>(T) / rows + B));
+}
+
+int launch_packed_plan(const int* cu, int B, int T, int rows, int max_tiles, void* table, int* head, int* scratch,
+                       unsigned* status, cudaStream_t stream) {
+  return launch_pdl(packed_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, cu, B, T, rows, max_tiles,
+                    static_cast<int4*>(table), head, scratch, scratch + B + 1, status) == cudaSuccess ? 0 : -1;
+}
+
+int launch_packed_forward(const PackedMaps& maps, const PackedArgs& a, void* out, float* lse, bool row_pairs,
+                          unsigned* status, cudaStream_t stream) {
+  return a.D <= 64 ? run_fwd<64>(maps, a, out, lse, row_pairs, status, stream)
+                   : run_fwd<128>(maps, a, out, lse, row_pairs, status, stream);
+}
+
+}  // namespace ecz

@@ -1,0 +1,546 @@
+// Gradients of the packed causal attention (packed_attention.cu).
+//
+//   d_i = do_i . o_i      p_ij = exp(s_ij - L_i)      ds_ij = p_ij (do_i . v_j - d_i)
+//   dv_j = sum_i p_ij do_i      dk_j = scale sum_i ds_ij q_i      dq_i = scale sum_j ds_ij k_j
+//
+// Two kernels, one per reduction axis, so every sum has one owner and a fixed order: no atomics, the same bits every
+// time, and the shared heads of a group add up inside a CTA. The price is that s and do . v are computed twice (seven
+// tile products instead of five).
+//
+// dkv  CTA: 128 keys of one K/V head; walks the query tiles from the diagonal to the sequence's end for every query
+//      head of the group. S^T = K Q^T and dP^T = V dO^T put keys on the TMEM lanes, so P^T and dS^T are the A operands
+//      of dV += P^T dO and dK += dS^T Q where they lie (bf16 over the fp32 scores they came from): nothing of a
+//      128 x 128 tile passes through shared memory. TMEM: S, dP, dV, dK of 128 columns each, all 512. The tensor cores
+//      run dV and the next S while the threads turn dP into dS, and dK and the next dP while they turn S into P.
+// dq   CTA: 128 queries of one head; walks the key chunks up to the diagonal. S (two buffers), dP, dQ in TMEM.
+#include <algorithm>
+
+#include "launchers.h"
+#include "packed_common.cuh"
+
+namespace ecz {
+
+using namespace packed;
+
+namespace {
+
+constexpr int kBwdThreads = 384;
+
+struct BwdArgs {
+  bf16 *dq, *dk, *dv;
+  const float *lse, *delta;  // [H, T]
+  const int4* table;
+  const int* head;
+  int T, H, Hkv, D;
+  float scale, scale2;
+};
+
+// delta[h, t] = dout[t, h] . out[t, h]; 16 lanes per row.
+__global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restrict__ out, const bf16* __restrict__ dout,
+                                                           long stride_t, long stride_h, int T, int H, int D,
+                                                           float* __restrict__ delta) {
+  pdl_trigger();
+  pdl_wait();
+  const long row = (static_cast<long>(blockIdx.x) * 256 + threadIdx.x) >> 4;
+  const int c = (threadIdx.x & 15) * 8;
+  const bool real = row < static_cast<long>(T) * H;
+  const long t = real ? row / H : 0;
+  const int h = real ? static_cast<int>(row % H) : 0;
+  float acc = 0.f;
+  if (real && c < D) {
+    const uint4 a = *reinterpret_cast<const uint4*>(out + row * D + c);
+    const uint4 b = *reinterpret_cast<const uint4*>(dout + t * stride_t + h * stride_h + c);
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 u = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x[k]));
+      const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&y[k]));
+      acc = fmaf(u.x, v.x, acc);
+      acc = fmaf(u.y, v.y, acc);
+    }
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+  if (real && c == 0) delta[static_cast<long>(h) * T + t] = acc;
+}
+
+// A thread's TMEM row of `cols` fp32 values, times f, as bf16 at dst (D values).
+template <int DP>
+__device__ __forceinline__ void store_row(uint32_t taddr, float f, bf16* dst, int D, bool real) {
+#pragma unroll 1
+  for (int d = 0; d < DP; d += 32) {
+    float o[32];
+    tmem_load32(taddr + d, o);
+    if (real) {
+#pragma unroll
+      for (int j = 0; j < 32; j += 8)
+        if (d + j < D)
+          *reinterpret_cast<uint4*>(dst + d + j) =
+              make_uint4(pack_bf16(o[j] * f, o[j + 1] * f), pack_bf16(o[j + 2] * f, o[j + 3] * f),
+                         pack_bf16(o[j + 4] * f, o[j + 5] * f), pack_bf16(o[j + 6] * f, o[j + 7] * f));
+    }
+  }
+}
+
+template <int DP>
+struct BwdCfg {
+  static constexpr int kTileBytes = kRowsT * DP * 2;
+  static constexpr int kRing = DP == 64 ? 4 : 2;  // stages of two tiles
+  static constexpr int kStats = 2 * 128 * 4;      // lse and delta of a query tile
+  static constexpr int kSmem = (2 + 2 * kRing) * kTileBytes + kRing * kStats + 1024 + 256;
+  static_assert(kSmem <= 232448, "227 KB of shared memory");
+};
+
+// ---- dK and dV -----------------------------------------------------------------------------------------------------
+template <int DP>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    packed_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
+                      const __grid_constant__ BwdArgs p, unsigned* status) {
+  using Cfg = BwdCfg<DP>;
+  constexpr int kRing = Cfg::kRing, kTileBytes = Cfg::kTileBytes;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *k_tile = smem, *v_tile = smem + kTileBytes;
+  uint8_t* ring = smem + 2 * kTileBytes;  // stage s: Q at 2 s, dO at 2 s + 1
+  float* stats = reinterpret_cast<float*>(ring + 2 * kRing * kTileBytes);  // stage s: lse [128], delta [128]
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(stats) + kRing * Cfg::kStats);
+  uint64_t* q_full = kv_full + 1;
+  uint64_t* do_full = q_full + kRing;
+  uint64_t* st_full = do_full + kRing;
+  uint64_t* empty = st_full + kRing;
+  uint64_t* s_full = empty + kRing;
+  uint64_t* p_ready = s_full + 1;
+  uint64_t* dp_full = p_ready + 1;
+  uint64_t* ds_ready = dp_full + 1;
+  uint64_t* done = ds_ready + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&do_full[i], 1);
+      mbar_init(&st_full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(p_ready, 8);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_ready, 8);
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncwarp();
+  if (warp == 0) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
+  pdl_trigger();
+  pdl_wait();
+
+  zero_padding(p.dk, p.T, static_cast<long>(p.Hkv) * p.D, p.head);
+  zero_padding(p.dv, p.T, static_cast<long>(p.Hkv) * p.D, p.head);
+  const int entry = blockIdx.x / p.Hkv, kvh = blockIdx.x % p.Hkv;
+  if (entry < p.head[0]) {
+    const int4 tile = p.table[entry];
+    const int lo = tile.x, hi = tile.y;
+    const int first = tile.w - 1 - tile.z;  // the tile of keys: as many query tiles follow as the entry weighs
+    const int n_q = tile.z + 1;
+    const int group = p.H / p.Hkv;
+    const int total = group * n_q;
+    const int key0 = lo + first * kRowsT;
+    const int ksteps = (p.D + 15) / 16;
+    auto head_of = [&](int it) { return kvh * group + it / n_q; };
+    auto row_of = [&](int it) { return key0 + (it % n_q) * kRowsT; };
+
+    if (warp == 0) {
+      if (lane == 0) {
+        const uint32_t ra = smem_u32(ring);
+        mbar_arrive_expect_tx(kv_full, 2 * kTileBytes);
+        load_tile<DP>(smem_u32(k_tile), &tm_k, kv_full, kvh, key0);
+        load_tile<DP>(smem_u32(v_tile), &tm_v, kv_full, kvh, key0);
+        for (int it = 0; it < total; ++it) {
+          const int s = it % kRing;
+          if (!mbar_wait(&empty[s], ((it / kRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag)) break;
+          mbar_arrive_expect_tx(&q_full[s], kTileBytes);
+          load_tile<DP>(ra + 2 * s * kTileBytes, &tm_q, &q_full[s], head_of(it), row_of(it));
+          mbar_arrive_expect_tx(&do_full[s], kTileBytes);
+          load_tile<DP>(ra + (2 * s + 1) * kTileBytes, &tm_do, &do_full[s], head_of(it), row_of(it));
+        }
+      }
+    } else if (warp == 1) {
+      const uint32_t ka = smem_u32(k_tile), va = smem_u32(v_tile), ra = smem_u32(ring);
+      auto rows16 = [&](int it) { return (min(kRowsT, hi - row_of(it)) + 15) & ~15; };
+      // the tile of iteration it (Q: which 0, dO: which 1), rows past the sequence's end zeroed
+      auto ready = [&](int it, int which) {
+        const int s = it % kRing;
+        if (!warp_wait(which ? &do_full[s] : &q_full[s], (it / kRing) & 1, status, kStatusWaitFull, abort_flag))
+          return false;
+        const int n = min(kRowsT, hi - row_of(it)), n16 = (n + 15) & ~15;
+        if (n != n16) zero_rows<DP>(ring + (2 * s + which) * kTileBytes, n, n16, lane);
+        tc_fence_after();
+        return true;
+      };
+      bool ok = warp_wait(kv_full, 0, status, kStatusWaitFull, abort_flag) && ready(0, 0);
+      if (ok && lane == 0) {
+        mma_dims(t_s, ka, ra, rows16(0), ksteps);
+        umma_commit(s_full);
+      }
+      ok = ok && ready(0, 1);
+      if (ok && lane == 0) {
+        mma_dims(t_dp, va, ra + kTileBytes, rows16(0), ksteps);
+        umma_commit(dp_full);
+      }
+      __syncwarp();
+      for (int it = 0; ok && it < total; ++it) {
+        const int s = it % kRing, s1 = (it + 1) % kRing;
+        const bool more = it + 1 < total;
+        const uint32_t qa = ra + 2 * s * kTileBytes, da = qa + kTileBytes;
+        ok = warp_wait(p_ready, it & 1, status, kStatusWaitAccum, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) mma_rows(t_dv, t_s, 64, da, ksteps * 16, rows16(it) / 16, it > 0);
+        if (more) {
+          ok = ready(it + 1, 0);
+          if (!ok) break;
+          if (lane == 0) {
+            mma_dims(t_s, ka, ra + 2 * s1 * kTileBytes, rows16(it + 1), ksteps);
+            umma_commit(s_full);
+          }
+        }
+        __syncwarp();
+        ok = warp_wait(ds_ready, it & 1, status, kStatusWaitAccum, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          mma_rows(t_dk, t_dp, 64, qa, ksteps * 16, rows16(it) / 16, it > 0);
+          umma_commit(&empty[s]);
+        }
+        if (more) {
+          ok = ready(it + 1, 1);
+          if (!ok) break;
+          if (lane == 0) {
+            mma_dims(t_dp, va, ra + (2 * s1 + 1) * kTileBytes, rows16(it + 1), ksteps);
+            umma_commit(dp_full);
+          }
+        }
+        __syncwarp();
+      }
+      if (ok && lane == 0) umma_commit(done);
+    } else if (warp == 2) {
+      // ---- lse and delta of the query tiles ----
+      for (int it = 0; it < total; ++it) {
+        const int s = it % kRing;
+        if (!warp_wait(&empty[s], ((it / kRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag)) break;
+        const long base = static_cast<long>(head_of(it)) * p.T;
+        float* dst = stats + s * 256;
+#pragma unroll
+        for (int j = lane; j < kRowsT; j += 32) {
+          const int row = row_of(it) + j;
+          dst[j] = row < hi ? p.lse[base + row] : 0.f;
+          dst[128 + j] = row < hi ? p.delta[base + row] : 0.f;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&st_full[s]);
+      }
+    } else if (warp >= 4) {
+      // ---- P^T and dS^T: one thread per key and half of the queries ----
+      const int half = (warp - 4) >> 2, quad = warp & 3;
+      const int key = quad * 32 + lane;  // relative to key0
+      const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+      const uint32_t s_addr = t_s + lane_base + half * 64, dp_addr = t_dp + lane_base + half * 64;
+      bool ok = true;
+      for (int it = 0; it < total; ++it) {
+        const int s = it % kRing;
+        const float* lse = stats + s * 256 + half * 64;
+        const float* delta = lse + 128;
+        ok = warp_wait(&st_full[s], (it / kRing) & 1, status, kStatusWaitFull, abort_flag) &&
+             warp_wait(s_full, it & 1, status, kStatusWaitAccum, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        float v[64];
+        tmem_load64(s_addr, v);
+        // queries [from, to) of this half see the key
+        const int q0 = row_of(it) - key0;
+        const int from = q0 == 0 ? key - half * 64 : 0, to = hi - row_of(it) - half * 64;
+        const bool masked = q0 == 0 || to < 64;
+#pragma unroll
+        for (int j = 0; j < 64; j += 4) {
+          const float4 l = *reinterpret_cast<const float4*>(lse + j);
+          v[j] = ex2(fmaf(v[j], p.scale2, -l.x));
+          v[j + 1] = ex2(fmaf(v[j + 1], p.scale2, -l.y));
+          v[j + 2] = ex2(fmaf(v[j + 2], p.scale2, -l.z));
+          v[j + 3] = ex2(fmaf(v[j + 3], p.scale2, -l.w));
+        }
+        if (masked) {
+#pragma unroll
+          for (int j = 0; j < 64; ++j) v[j] = (j >= from && j < to) ? v[j] : 0.f;
+        }
+        uint32_t w[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+        tmem_store32(s_addr, w);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready);
+        ok = warp_wait(dp_full, it & 1, status, kStatusWaitAccum, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        float g[64];
+        tmem_load64(dp_addr, g);
+#pragma unroll
+        for (int j = 0; j < 64; j += 4) {
+          const float4 d = *reinterpret_cast<const float4*>(delta + j);
+          g[j] = v[j] * (g[j] - d.x);
+          g[j + 1] = v[j + 1] * (g[j + 1] - d.y);
+          g[j + 2] = v[j + 2] * (g[j + 2] - d.z);
+          g[j + 3] = v[j + 3] * (g[j + 3] - d.w);
+        }
+        if (masked) {
+#pragma unroll
+          for (int j = 0; j < 64; ++j) g[j] = (j >= from && j < to) ? g[j] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) w[j] = pack_bf16(g[2 * j], g[2 * j + 1]);
+        tmem_store32(dp_addr, w);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_ready);
+      }
+      if (ok && warp_wait(done, 0, status, kStatusWaitAccum, abort_flag)) {
+        tc_fence_after();
+        const int row = key0 + key;
+        const bool real = row < hi;
+        const long at = (static_cast<long>(row) * p.Hkv + kvh) * p.D;
+        if (half == 0) store_row<DP>(t_dv + lane_base, 1.f, p.dv + at, p.D, real);
+        else store_row<DP>(t_dk + lane_base, p.scale, p.dk + at, p.D, real);
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  settle(*abort_flag != 0);
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+// ---- dQ --------------------------------------------------------------------------------------------------------------
+template <int DP>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
+                     const __grid_constant__ BwdArgs p, unsigned* status) {
+  using Cfg = BwdCfg<DP>;
+  constexpr int kRing = Cfg::kRing, kTileBytes = Cfg::kTileBytes;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *q_tile = smem, *do_tile = smem + kTileBytes;
+  uint8_t* ring = smem + 2 * kTileBytes;  // stage s: K at 2 s, V at 2 s + 1
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + 2 * kRing * kTileBytes);
+  uint64_t* k_full = q_full + 1;
+  uint64_t* v_full = k_full + kRing;
+  uint64_t* empty = v_full + kRing;
+  uint64_t* s_full = empty + kRing;  // one per S buffer: S of chunk c + 1 may complete before c's is looked at
+  uint64_t* dp_full = s_full + 2;
+  uint64_t* ds_ready = dp_full + 1;
+  uint64_t* done = ds_ready + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_ready, 8);
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncwarp();
+  if (warp == 0) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t t_s = tmem, t_dp = tmem + 256, t_dq = tmem + 384;  // S: two buffers of 128 columns
+  pdl_trigger();
+  pdl_wait();
+
+  zero_padding(p.dq, p.T, static_cast<long>(p.H) * p.D, p.head);
+  const int entry = blockIdx.x / p.H, head = blockIdx.x % p.H;
+  if (entry < p.head[0]) {
+    const int4 tile = p.table[entry];
+    const int lo = tile.x, hi = tile.y;
+    const int row0 = lo + tile.z * kRowsT;
+    const int n = tile.z + 1;  // key chunks, the last one on the diagonal
+    const int kvh = head / (p.H / p.Hkv);
+    const int ksteps = (p.D + 15) / 16;
+
+    if (warp == 0) {
+      if (lane == 0) {
+        const uint32_t ra = smem_u32(ring);
+        mbar_arrive_expect_tx(q_full, 2 * kTileBytes);
+        load_tile<DP>(smem_u32(q_tile), &tm_q, q_full, head, row0);
+        load_tile<DP>(smem_u32(do_tile), &tm_do, q_full, head, row0);
+        for (int c = 0; c < n; ++c) {
+          const int s = c % kRing;
+          if (!mbar_wait(&empty[s], ((c / kRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag)) break;
+          mbar_arrive_expect_tx(&k_full[s], kTileBytes);
+          load_tile<DP>(ra + 2 * s * kTileBytes, &tm_k, &k_full[s], kvh, lo + c * kRowsT);
+          mbar_arrive_expect_tx(&v_full[s], kTileBytes);
+          load_tile<DP>(ra + (2 * s + 1) * kTileBytes, &tm_v, &v_full[s], kvh, lo + c * kRowsT);
+        }
+      }
+    } else if (warp == 1) {
+      const uint32_t qa = smem_u32(q_tile), da = smem_u32(do_tile), ra = smem_u32(ring);
+      auto keys16 = [&](int c) { return (min(kRowsT, hi - (lo + c * kRowsT)) + 15) & ~15; };
+      auto scores = [&](int c) {  // S of chunk c into its buffer; K rows past the end zeroed
+        const int s = c % kRing;
+        if (!warp_wait(&k_full[s], (c / kRing) & 1, status, kStatusWaitFull, abort_flag)) return false;
+        const int keys = min(kRowsT, hi - (lo + c * kRowsT));
+        if (keys != keys16(c)) zero_rows<DP>(ring + 2 * s * kTileBytes, keys, keys16(c), lane);
+        tc_fence_after();
+        if (lane == 0) {
+          mma_dims(t_s + (c & 1) * 128, qa, ra + 2 * s * kTileBytes, keys16(c), ksteps);
+          umma_commit(&s_full[c & 1]);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto products = [&](int c) {  // dP of chunk c
+        const int s = c % kRing;
+        if (!warp_wait(&v_full[s], (c / kRing) & 1, status, kStatusWaitFull, abort_flag)) return false;
+        tc_fence_after();
+        if (lane == 0) {
+          mma_dims(t_dp, da, ra + (2 * s + 1) * kTileBytes, keys16(c), ksteps);
+          umma_commit(dp_full);
+        }
+        __syncwarp();
+        return true;
+      };
+      bool ok = warp_wait(q_full, 0, status, kStatusWaitFull, abort_flag) && scores(0) && products(0);
+      for (int c = 0; ok && c < n; ++c) {
+        const bool more = c + 1 < n;
+        if (more) ok = scores(c + 1);
+        ok = ok && warp_wait(ds_ready, c & 1, status, kStatusWaitAccum, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        if (more) ok = products(c + 1);
+        if (!ok) break;
+        if (lane == 0) {
+          mma_rows(t_dq, t_s + (c & 1) * 128, 64, ra + 2 * (c % kRing) * kTileBytes, ksteps * 16, keys16(c) / 16,
+                   c > 0);
+          umma_commit(&empty[c % kRing]);
+        }
+        __syncwarp();
+      }
+      if (ok && lane == 0) umma_commit(done);
+    } else if (warp >= 4) {
+      // ---- dS: one thread per query and half of the keys ----
+      const int half = (warp - 4) >> 2, quad = warp & 3;
+      const int row = row0 + quad * 32 + lane;
+      const bool real = row < hi;
+      const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+      const float lse = real ? p.lse[static_cast<long>(head) * p.T + row] : 0.f;
+      const float delta = real ? p.delta[static_cast<long>(head) * p.T + row] : 0.f;
+      bool ok = true;
+      for (int c = 0; c < n; ++c) {
+        const uint32_t s_addr = t_s + (c & 1) * 128 + lane_base + half * 64;
+        ok = warp_wait(&s_full[c & 1], (c >> 1) & 1, status, kStatusWaitAccum, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        float v[64], g[64];
+        tmem_load64(s_addr, v);
+#pragma unroll
+        for (int j = 0; j < 64; ++j) v[j] = ex2(fmaf(v[j], p.scale2, -lse));
+        ok = warp_wait(dp_full, c & 1, status, kStatusWaitAccum, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        tmem_load64(t_dp + lane_base + half * 64, g);
+#pragma unroll
+        for (int j = 0; j < 64; ++j) g[j] = v[j] * (g[j] - delta);
+        if (c == n - 1) {
+          const int limit = min(hi, row + 1) - (lo + c * kRowsT) - half * 64;
+#pragma unroll
+          for (int j = 0; j < 64; ++j) g[j] = j < limit ? g[j] : 0.f;
+        }
+        uint32_t w[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) w[j] = pack_bf16(g[2 * j], g[2 * j + 1]);
+        tmem_store32(s_addr, w);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_ready);
+      }
+      if (ok && warp_wait(done, 0, status, kStatusWaitAccum, abort_flag)) {
+        tc_fence_after();
+        if (half == 0)  // half of the columns each would save little: one store per row
+          store_row<DP>(t_dq + lane_base, p.scale, p.dq + (static_cast<long>(row) * p.H + head) * p.D, p.D, real);
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  settle(*abort_flag != 0);
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+template <int DP>
+int run_bwd(const PackedMaps& m, const PackedArgs& a, const BwdArgs& args, bool want_dq, bool want_dkv,
+            unsigned* status, cudaStream_t stream) {
+  const long grid_kv = static_cast<long>(a.max_tiles) * a.Hkv, grid_q = static_cast<long>(a.max_tiles) * a.H;
+  if (grid_q > 0x7fffffffl) return -2;
+  if (want_dkv) {
+    auto kernel = packed_dkv_kernel<DP>;
+    if (set_max_smem(kernel, BwdCfg<DP>::kSmem) != cudaSuccess) return -1;
+    if (launch_pdl(kernel, dim3(static_cast<unsigned>(grid_kv)), dim3(kBwdThreads), BwdCfg<DP>::kSmem, stream, m.q,
+                   m.k, m.v, m.dout, args, status) != cudaSuccess)
+      return -1;
+  }
+  if (want_dq) {
+    auto kernel = packed_dq_kernel<DP>;
+    if (set_max_smem(kernel, BwdCfg<DP>::kSmem) != cudaSuccess) return -1;
+    if (launch_pdl(kernel, dim3(static_cast<unsigned>(grid_q)), dim3(kBwdThreads), BwdCfg<DP>::kSmem, stream, m.q, m.k,
+                   m.v, m.dout, args, status) != cudaSuccess)
+      return -1;
+  }
+  return 0;
+}
+
+}  // namespace
+
+int launch_packed_delta(const void* out, const void* dout, long stride_t, long stride_h, int T, int H, int D,
+                        float* delta, cudaStream_t stream) {
+  const long rows = static_cast<long>(T) * H;
+  return launch_pdl(packed_delta_kernel, dim3(static_cast<unsigned>((rows + 15) / 16)), dim3(256), 0, stream,
+                    static_cast<const bf16*>(out), static_cast<const bf16*>(dout), stride_t, stride_h, T, H, D,
+                    delta) == cudaSuccess ? 0 : -1;
+}
+
+int launch_packed_backward(const PackedMaps& maps, const PackedArgs& a, const float* lse, const float* delta, void* dq,
+                           void* dk, void* dv, unsigned* status, cudaStream_t stream) {
+  const BwdArgs args{static_cast<bf16*>(dq), static_cast<bf16*>(dk), static_cast<bf16*>(dv), lse, delta,
+                     static_cast<const int4*>(a.table), a.head, a.T, a.H, a.Hkv, a.D, a.scale, a.scale * kLog2e};
+  const bool want_dkv = dk != nullptr;
+  return a.D <= 64 ? run_bwd<64>(maps, a, args, dq != nullptr, want_dkv, status, stream)
+                   : run_bwd<128>(maps, a, args, dq != nullptr, want_dkv, status, stream);
+}
+
+}  // namespace ecz

@@ -14,7 +14,7 @@ from ._ext import available, load_error, require
 from .fp8 import FP8BlockWeight
 from .quant import QWeight
 from .sparse import Sparse24Weight
-from .training import linear_cross_entropy
+from .training import linear_cross_entropy, packed_attention
 
 __all__ = [
     "argmax",
@@ -30,6 +30,7 @@ __all__ = [
     "linear_parts",
     "Partials",
     "load_error",
+    "packed_attention",
     "require",
     "rmsnorm",
     "ngram",

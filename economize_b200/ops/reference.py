@@ -20,6 +20,7 @@ __all__ = [
     "kv_compact",
     "linear",
     "linear_cross_entropy",
+    "packed_attention",
     "rmsnorm",
     "rope_store",
     "silu_mul",
@@ -460,3 +461,31 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     if reduction == "none":
         return torch.zeros(targets.shape, dtype=wide, device=hidden.device).index_copy(0, rows, nll)
     return nll.sum() if reduction == "sum" else nll.sum() / max(1, rows.numel())
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                     scale: float) -> torch.Tensor:
+    """Causal attention of the packed sequences ``cu_seqlens [B + 1]`` of ``q [T, H, D]`` over ``k, v [T, H_kv, D]``,
+    sequence by sequence; rows outside every sequence are zero."""
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] \
+            or q.shape[1] % k.shape[1]:
+        raise ValueError(f"packed_attention expects q [T, H, D] and k, v [T, H_kv, D], got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)} and {tuple(v.shape)}")
+    if cu_seqlens.dim() != 1 or cu_seqlens.dtype != torch.int32:
+        raise ValueError("packed_attention: cu_seqlens must be int32 [B + 1]")
+    group = q.shape[1] // k.shape[1]
+    wide = torch.promote_types(q.dtype, torch.float32)
+    out = torch.zeros_like(q)
+    edges = cu_seqlens.tolist()
+    if edges and (edges[0] < 0 or edges[-1] > q.shape[0] or any(a > b for a, b in zip(edges, edges[1:]))):
+        raise ValueError(f"packed_attention: offsets {edges} do not rise from 0 to {q.shape[0]} at most")
+    for a, b in zip(edges, edges[1:]):
+        if a == b:
+            continue
+        qs, ks, vs = (x[a:b].to(wide).transpose(0, 1) for x in (q, k, v))
+        ks, vs = ks.repeat_interleave(group, 0), vs.repeat_interleave(group, 0)
+        s = torch.matmul(qs, ks.transpose(1, 2)) * scale
+        s = s.masked_fill(torch.ones(b - a, b - a, dtype=torch.bool, device=q.device).triu(1), float("-inf"))
+        o = torch.matmul(torch.softmax(s, -1), vs).transpose(0, 1).to(q.dtype)
+        out = torch.cat([out[:a], o, out[b:]])
+    return out

@@ -12,7 +12,7 @@ from torch.autograd.function import once_differentiable
 from . import reference
 from ._ext import require
 
-__all__ = ["linear_cross_entropy"]
+__all__ = ["linear_cross_entropy", "packed_attention"]
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
@@ -97,3 +97,46 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     else:
         loss = reference.linear_cross_entropy(flat, weight, targets.reshape(-1), ignore_index, reduction, logit_scale)
     return loss.reshape(targets.shape) if reduction == "none" else loss
+
+
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_seqlens, scale):
+        out, lse = require().packed_forward(q, k, v, cu_seqlens, scale, True)
+        ctx.scale = scale
+        ctx.save_for_backward(q, k, v, out, lse, cu_seqlens)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        q, k, v, out, lse, cu_seqlens = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dq, dk, dv = require().packed_backward(grad, q, k, v, out, lse, cu_seqlens, ctx.scale, need[0],
+                                               need[1] or need[2])
+        return dq, dk, dv, None, None
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                     scale: float | None = None) -> torch.Tensor:
+    """Causal attention of packed sequences with grouped heads, differentiable in ``q``, ``k`` and ``v``.
+
+    Args:
+        q: Queries ``[T, H, D]`` of all sequences one after another (bf16 on CUDA; cast under bf16 autocast). Views
+            with 16-byte strides (parts of a fused projection) are read in place.
+        k, v: Keys and values ``[T, H_kv, D]``; query head ``h`` reads head ``h // (H / H_kv)``.
+        cu_seqlens: int32 ``[B + 1]``: sequence ``i`` holds tokens ``cu_seqlens[i]`` to ``cu_seqlens[i + 1]``. A token
+            attends itself and those before it in its sequence; empty sequences are allowed. Tokens outside every
+            sequence (a row's padding) may hold anything: their outputs and gradients are zero.
+        scale: Of the scores (``D ** -0.5``); positive.
+
+    Head dimensions 8 to 128 in steps of 8 on CUDA. Offsets that fall or lie outside ``[0, T]`` are clamped on CUDA and
+    reported in the device status word.
+    """
+    scale = float(scale if scale is not None else q.shape[-1] ** -0.5)
+    q, k, v = _autocast(q, k, v)
+    if not q.is_cuda:
+        return reference.packed_attention(q, k, v, cu_seqlens, scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _PackedAttention.apply(q, k, v, cu_seqlens, scale)
+    return require().packed_forward(q, k, v, cu_seqlens, scale, False)[0]
