@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     for (int i = 0; i < kRing; ++i) {
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   pdl_trigger();
   pdl_wait();
 
@@ -225,13 +225,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   zero_padding(p.out, p.T, static_cast<long>(p.H) * p.D, p.head);
   if (entry < p.head[0]) {
     const int4 tile = p.table[entry];
-    const int lo = tile.x, hi = tile.y;
+    const int lo = uniform(tile.x), hi = uniform(tile.y), at = uniform(tile.z);
     const int group = p.H / p.Hkv;
     int head[2], row0[2], chunks[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       head[i] = p.row_pairs ? sub : 2 * sub + i;
-      row0[i] = p.row_pairs ? lo + tile.z * 256 + i * 128 : lo + tile.z * 128;
+      row0[i] = p.row_pairs ? lo + at * 256 + i * 128 : lo + at * 128;
       chunks[i] = row0[i] < hi ? (row0[i] - lo) / kRowsT + 1 : 0;  // the last one holds the diagonal
     }
     const int kvh = head[0] / group;
@@ -254,6 +254,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       }
     } else if (warp == 1) {
       // ---- MMAs ----
+      const bool leader = elect_one();
       const uint32_t qa = smem_u32(q_tiles), ra = smem_u32(ring);
       auto wait_ring = [&](int it) {
         return warp_wait(&kv_full[it % kRing], (it / kRing) & 1, status, kStatusWaitFull,
@@ -262,11 +263,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       auto keys_of = [&](int c) { return min(kRowsT, hi - (lo + c * kRowsT)); };
       bool ok = warp_wait(q_full, 0, status, kStatusWaitFull, abort_flag) && wait_ring(0);
       tc_fence_after();
-      if (ok && lane == 0) {
+      if (ok && leader) {
         const int n = (keys_of(0) + 15) & ~15;
         for (int i = 0; i < 2; ++i) {
           if (chunks[i] == 0) continue;
-          mma_dims(tmem + i * 128, qa + i * kTileBytes, ra, n, ksteps);
+          mma_dims<DP>(tmem + i * 128, qa + i * kTileBytes, ra, n, ksteps);
           umma_commit(&s_full[i]);
         }
         umma_commit(&kv_empty[0]);
@@ -284,18 +285,18 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           ok = warp_wait(&p_ready[i], c & 1, status, kStatusWaitAccum, abort_flag);
           if (!ok) break;
           tc_fence_after();
-          if (lane == 0) {
-            mma_rows(tmem + 256 + i * DP, tmem + i * 128, 32, smem_u32(v_tile), ksteps * 16, n16 / 16, c > 0);
+          if (leader) {
+            mma_rows<32>(tmem + 256 + i * DP, tmem + i * 128, smem_u32(v_tile), ksteps * 16, n16 / 16, c > 0);
             umma_commit(&o_done[i]);
             if (c + 1 < chunks[i]) {
-              mma_dims(tmem + i * 128, qa + i * kTileBytes, ra + (k_it % kRing) * kTileBytes,
+              mma_dims<DP>(tmem + i * 128, qa + i * kTileBytes, ra + (k_it % kRing) * kTileBytes,
                        (keys_of(c + 1) + 15) & ~15, ksteps);
               umma_commit(&s_full[i]);
             }
           }
           __syncwarp();
         }
-        if (lane == 0) {
+        if (leader) {
           umma_commit(&kv_empty[v_it % kRing]);
           if (more) umma_commit(&kv_empty[k_it % kRing]);
         }

@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
     for (int i = 0; i < kRing; ++i) {
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   const uint32_t t_s = tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
   pdl_trigger();
   pdl_wait();
@@ -149,9 +149,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int entry = blockIdx.x / p.Hkv, kvh = blockIdx.x % p.Hkv;
   if (entry < p.head[0]) {
     const int4 tile = p.table[entry];
-    const int lo = tile.x, hi = tile.y;
-    const int first = tile.w - 1 - tile.z;  // the tile of keys: as many query tiles follow as the entry weighs
-    const int n_q = tile.z + 1;
+    const int lo = uniform(tile.x), hi = uniform(tile.y);
+    const int n_q = uniform(tile.z) + 1;
+    const int first = uniform(tile.w) - n_q;  // the tile of keys: as many query tiles follow as the entry weighs
     const int group = p.H / p.Hkv;
     const int total = group * n_q;
     const int key0 = lo + first * kRowsT;
@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
       }
     } else if (warp == 1) {
+      const bool leader = elect_one();
       const uint32_t ka = smem_u32(k_tile), va = smem_u32(v_tile), ra = smem_u32(ring);
       auto rows16 = [&](int it) { return (min(kRowsT, hi - row_of(it)) + 15) & ~15; };
       // the tile of iteration it (Q: which 0, dO: which 1), rows past the sequence's end zeroed
@@ -188,13 +189,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         return true;
       };
       bool ok = warp_wait(kv_full, 0, status, kStatusWaitFull, abort_flag) && ready(0, 0);
-      if (ok && lane == 0) {
-        mma_dims(t_s, ka, ra, rows16(0), ksteps);
+      if (ok && leader) {
+        mma_dims<DP>(t_s, ka, ra, rows16(0), ksteps);
         umma_commit(s_full);
       }
       ok = ok && ready(0, 1);
-      if (ok && lane == 0) {
-        mma_dims(t_dp, va, ra + kTileBytes, rows16(0), ksteps);
+      if (ok && leader) {
+        mma_dims<DP>(t_dp, va, ra + kTileBytes, rows16(0), ksteps);
         umma_commit(dp_full);
       }
       __syncwarp();
@@ -205,12 +206,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         ok = warp_wait(p_ready, it & 1, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        if (lane == 0) mma_rows(t_dv, t_s, 64, da, ksteps * 16, rows16(it) / 16, it > 0);
+        if (leader) mma_rows<64>(t_dv, t_s, da, ksteps * 16, rows16(it) / 16, it > 0);
         if (more) {
           ok = ready(it + 1, 0);
           if (!ok) break;
-          if (lane == 0) {
-            mma_dims(t_s, ka, ra + 2 * s1 * kTileBytes, rows16(it + 1), ksteps);
+          if (leader) {
+            mma_dims<DP>(t_s, ka, ra + 2 * s1 * kTileBytes, rows16(it + 1), ksteps);
             umma_commit(s_full);
           }
         }
@@ -218,21 +219,21 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         ok = warp_wait(ds_ready, it & 1, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        if (lane == 0) {
-          mma_rows(t_dk, t_dp, 64, qa, ksteps * 16, rows16(it) / 16, it > 0);
+        if (leader) {
+          mma_rows<64>(t_dk, t_dp, qa, ksteps * 16, rows16(it) / 16, it > 0);
           umma_commit(&empty[s]);
         }
         if (more) {
           ok = ready(it + 1, 1);
           if (!ok) break;
-          if (lane == 0) {
-            mma_dims(t_dp, va, ra + (2 * s1 + 1) * kTileBytes, rows16(it + 1), ksteps);
+          if (leader) {
+            mma_dims<DP>(t_dp, va, ra + (2 * s1 + 1) * kTileBytes, rows16(it + 1), ksteps);
             umma_commit(dp_full);
           }
         }
         __syncwarp();
       }
-      if (ok && lane == 0) umma_commit(done);
+      if (ok && leader) umma_commit(done);
     } else if (warp == 2) {
       // ---- lse and delta of the query tiles ----
       for (int it = 0; it < total; ++it) {
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     for (int i = 0; i < kRing; ++i) {
@@ -376,7 +377,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   const uint32_t t_s = tmem, t_dp = tmem + 256, t_dq = tmem + 384;  // S: two buffers of 128 columns
   pdl_trigger();
   pdl_wait();
@@ -385,9 +386,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int entry = blockIdx.x / p.H, head = blockIdx.x % p.H;
   if (entry < p.head[0]) {
     const int4 tile = p.table[entry];
-    const int lo = tile.x, hi = tile.y;
-    const int row0 = lo + tile.z * kRowsT;
-    const int n = tile.z + 1;  // key chunks, the last one on the diagonal
+    const int lo = uniform(tile.x), hi = uniform(tile.y);
+    const int n = uniform(tile.z) + 1;  // key chunks, the last one on the diagonal
+    const int row0 = lo + (n - 1) * kRowsT;
     const int kvh = head / (p.H / p.Hkv);
     const int ksteps = (p.D + 15) / 16;
 
@@ -407,6 +408,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
       }
     } else if (warp == 1) {
+      const bool leader = elect_one();
       const uint32_t qa = smem_u32(q_tile), da = smem_u32(do_tile), ra = smem_u32(ring);
       auto keys16 = [&](int c) { return (min(kRowsT, hi - (lo + c * kRowsT)) + 15) & ~15; };
       auto scores = [&](int c) {  // S of chunk c into its buffer; K rows past the end zeroed
@@ -415,8 +417,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const int keys = min(kRowsT, hi - (lo + c * kRowsT));
         if (keys != keys16(c)) zero_rows<DP>(ring + 2 * s * kTileBytes, keys, keys16(c), lane);
         tc_fence_after();
-        if (lane == 0) {
-          mma_dims(t_s + (c & 1) * 128, qa, ra + 2 * s * kTileBytes, keys16(c), ksteps);
+        if (leader) {
+          mma_dims<DP>(t_s + (c & 1) * 128, qa, ra + 2 * s * kTileBytes, keys16(c), ksteps);
           umma_commit(&s_full[c & 1]);
         }
         __syncwarp();
@@ -426,8 +428,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const int s = c % kRing;
         if (!warp_wait(&v_full[s], (c / kRing) & 1, status, kStatusWaitFull, abort_flag)) return false;
         tc_fence_after();
-        if (lane == 0) {
-          mma_dims(t_dp, da, ra + (2 * s + 1) * kTileBytes, keys16(c), ksteps);
+        if (leader) {
+          mma_dims<DP>(t_dp, da, ra + (2 * s + 1) * kTileBytes, keys16(c), ksteps);
           umma_commit(dp_full);
         }
         __syncwarp();
@@ -442,14 +444,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_fence_after();
         if (more) ok = products(c + 1);
         if (!ok) break;
-        if (lane == 0) {
-          mma_rows(t_dq, t_s + (c & 1) * 128, 64, ra + 2 * (c % kRing) * kTileBytes, ksteps * 16, keys16(c) / 16,
+        if (leader) {
+          mma_rows<64>(t_dq, t_s + (c & 1) * 128, ra + 2 * (c % kRing) * kTileBytes, ksteps * 16, keys16(c) / 16,
                    c > 0);
           umma_commit(&empty[c % kRing]);
         }
         __syncwarp();
       }
-      if (ok && lane == 0) umma_commit(done);
+      if (ok && leader) umma_commit(done);
     } else if (warp >= 4) {
       // ---- dS: one thread per query and half of the keys ----
       const int half = (warp - 4) >> 2, quad = warp & 3;

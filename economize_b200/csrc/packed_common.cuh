@@ -51,23 +51,46 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int from, int to, int l
   __syncwarp();
 }
 
-// D[128, n] (+)= A[128, :k] . B[n, :k]^T, both K-major tiles of [128, DP] (k the head dimension, in steps of 16).
+// The MMA loops below are unrolled around one descriptor per operand and constant steps, added to its low word (the
+// address field, which does not overflow); the issuing warp's tile fields are broadcast from lane 0 (uniform()) so that
+// descriptors live in uniform registers. With descriptors built in a run-time loop a 128 x 128 x 16 MMA took 115 cycles
+// to issue (64 to execute).
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+__device__ __forceinline__ uint64_t desc_step(uint64_t desc, uint32_t bytes) {
+  const uint32_t lo = static_cast<uint32_t>(desc) + (bytes >> 4), hi = static_cast<uint32_t>(desc >> 32);
+  return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+
+// D[128, n] = A[128, :16 ksteps] . B[n, :16 ksteps]^T, both K-major tiles of [128, DP] (K the head dimension).
+template <int DP>
 __device__ __forceinline__ void mma_dims(uint32_t d, uint32_t a, uint32_t b, int n, int ksteps) {
   const uint32_t idesc = idesc_bf16_f32(128, n);
-  for (int kk = 0; kk < ksteps; ++kk) {
+  const uint64_t da = desc_kmajor_sw128(a), db = desc_kmajor_sw128(b);
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk) {
     const uint32_t off = (kk >> 2) * kRowsT * 128 + (kk & 3) * 32;
-    umma_bf16(d, desc_kmajor_sw128(a + off), desc_kmajor_sw128(b + off), idesc, kk != 0 ? 1u : 0u);
+    if (kk < ksteps) umma_bf16(d, desc_step(da, off), desc_step(db, off), idesc, kk != 0 ? 1u : 0u);
   }
 }
 
-// D[128, n] (+)= P[128, :16 ksteps] . B[:16 ksteps, n], P packed bf16 in TMEM (k step kk at column pcol(kk)), B's rows
-// along K (MN-major).
-__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t p, int half_cols, uint32_t b, int n, int ksteps,
-                                         bool accumulate) {
+// D[128, n] (+)= P[128, :16 ksteps] . B[:16 ksteps, n], P packed bf16 in TMEM (64 of its columns every kHalf 32-bit
+// columns), B's rows along K (MN-major).
+template <int kHalf>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t p, uint32_t b, int n, int ksteps, bool accumulate) {
   const uint32_t idesc = idesc_bf16_f32(128, n, true);
-  for (int kk = 0; kk < ksteps; ++kk) {
-    const uint32_t pc = p + (kk >> 2) * half_cols + (kk & 3) * 8;
-    umma_bf16_ta(d, pc, desc_mnmajor_sw128(b + kk * 16 * 128, kRowsT * 128), idesc, (accumulate || kk != 0) ? 1u : 0u);
+  const uint64_t db = desc_mnmajor_sw128(b, kRowsT * 128);
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) {
+    const uint32_t pc = p + (kk >> 2) * kHalf + (kk & 3) * 8;
+    if (kk < ksteps) umma_bf16_ta(d, pc, desc_step(db, kk * 16 * 128), idesc, kk != 0 ? 1u : (accumulate ? 1u : 0u));
   }
 }
 
