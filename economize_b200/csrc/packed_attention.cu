@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           if (!ok) break;
           tc_fence_after();
           if (leader) {
-            mma_rows<32>(tmem + 256 + i * DP, tmem + i * 128, smem_u32(v_tile), ksteps * 16, n16 / 16, c > 0);
+            mma_rows<8, 64>(tmem + 256 + i * DP, tmem + i * 128, smem_u32(v_tile), ksteps * 16, n16 / 16, c > 0);
             umma_commit(&o_done[i]);
             if (c + 1 < chunks[i]) {
               mma_dims<DP>(tmem + i * 128, qa + i * kTileBytes, ra + (k_it % kRing) * kTileBytes,

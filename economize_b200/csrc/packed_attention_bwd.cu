@@ -24,7 +24,10 @@ using namespace packed;
 
 namespace {
 
-constexpr int kBwdThreads = 384;
+// Warps 0-2 load, issue and fetch row statistics; sixteen compute warps, so that four per scheduler hide the latencies
+// of the tile's short phases (eight with twice the columns each spent 3000 of 4700 cycles per tile in them).
+constexpr int kComputeWarps = 16;
+constexpr int kBwdThreads = 128 + 32 * kComputeWarps;
 
 struct BwdArgs {
   bf16 *dq, *dk, *dv;
@@ -64,17 +67,17 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restric
   if (real && c == 0) delta[static_cast<long>(h) * T + t] = acc;
 }
 
-// A thread's TMEM row of `cols` fp32 values, times f, as bf16 at dst (D values).
-template <int DP>
-__device__ __forceinline__ void store_row(uint32_t taddr, float f, bf16* dst, int D, bool real) {
+// `kCols` fp32 columns of a thread's TMEM row, times f, as bf16 at dst (those of the `left` that are).
+template <int kCols>
+__device__ __forceinline__ void store_row(uint32_t taddr, float f, bf16* dst, int left, bool real) {
 #pragma unroll 1
-  for (int d = 0; d < DP; d += 32) {
-    float o[32];
-    tmem_load32(taddr + d, o);
+  for (int d = 0; d < kCols; d += 16) {
+    float o[16];
+    tmem_ld16(taddr + d, o);
     if (real) {
 #pragma unroll
-      for (int j = 0; j < 32; j += 8)
-        if (d + j < D)
+      for (int j = 0; j < 16; j += 8)
+        if (d + j < left)
           *reinterpret_cast<uint4*>(dst + d + j) =
               make_uint4(pack_bf16(o[j] * f, o[j + 1] * f), pack_bf16(o[j + 2] * f, o[j + 3] * f),
                          pack_bf16(o[j + 4] * f, o[j + 5] * f), pack_bf16(o[j + 6] * f, o[j + 7] * f));
@@ -85,10 +88,25 @@ __device__ __forceinline__ void store_row(uint32_t taddr, float f, bf16* dst, in
 template <int DP>
 struct BwdCfg {
   static constexpr int kTileBytes = kRowsT * DP * 2;
-  static constexpr int kRing = DP == 64 ? 4 : 2;  // stages of two tiles
-  static constexpr int kStats = 2 * 128 * 4;      // lse and delta of a query tile
-  static constexpr int kSmem = (2 + 2 * kRing) * kTileBytes + kRing * kStats + 1024 + 256;
+  static constexpr int kRing = DP == 64 ? 10 : 5;  // streamed tiles
+  static constexpr int kStatRing = 3;
+  static constexpr int kStats = 2 * 128 * 4;  // lse and delta of a query tile
+  // no slack for alignment: dynamic shared memory starts on a 1024-byte boundary where nothing static precedes it (the
+  // kernels check)
+  static constexpr int kSmem = (2 + kRing) * kTileBytes + (DP == 64 ? kStatRing : 2) * kStats + 512;
   static_assert(kSmem <= 232448, "227 KB of shared memory");
+};
+
+// The stream of tiles of a backward kernel: item 2 i + which, ring slot item % kRing.
+template <int DP>
+struct Stream {
+  static constexpr int kRing = BwdCfg<DP>::kRing;
+  uint8_t* tiles;
+  uint64_t *full, *empty;
+  __device__ __forceinline__ uint8_t* tile(int item) const { return tiles + (item % kRing) * BwdCfg<DP>::kTileBytes; }
+  __device__ __forceinline__ uint64_t* full_of(int item) const { return &full[item % kRing]; }
+  __device__ __forceinline__ uint64_t* empty_of(int item) const { return &empty[item % kRing]; }
+  __device__ __forceinline__ uint32_t use(int item) const { return (item / kRing) & 1; }
 };
 
 // ---- dK and dV -----------------------------------------------------------------------------------------------------
@@ -98,18 +116,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
                       const __grid_constant__ BwdArgs p, unsigned* status) {
   using Cfg = BwdCfg<DP>;
-  constexpr int kRing = Cfg::kRing, kTileBytes = Cfg::kTileBytes;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr int kRing = Cfg::kRing, kTileBytes = Cfg::kTileBytes, kStatRing = DP == 64 ? Cfg::kStatRing : 2;
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t *k_tile = smem, *v_tile = smem + kTileBytes;
-  uint8_t* ring = smem + 2 * kTileBytes;  // stage s: Q at 2 s, dO at 2 s + 1
-  float* stats = reinterpret_cast<float*>(ring + 2 * kRing * kTileBytes);  // stage s: lse [128], delta [128]
-  uint64_t* kv_full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(stats) + kRing * Cfg::kStats);
-  uint64_t* q_full = kv_full + 1;
-  uint64_t* do_full = q_full + kRing;
-  uint64_t* st_full = do_full + kRing;
-  uint64_t* empty = st_full + kRing;
-  uint64_t* s_full = empty + kRing;
+  float* stats = reinterpret_cast<float*>(smem + (2 + kRing) * kTileBytes);  // stage s: lse [128], delta [128]
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(stats) + kStatRing * Cfg::kStats);
+  Stream<DP> ring{smem + 2 * kTileBytes, kv_full + 1, kv_full + 1 + kRing};
+  uint64_t* st_full = kv_full + 1 + 2 * kRing;
+  uint64_t* st_empty = st_full + kStatRing;
+  uint64_t* s_full = st_empty + kStatRing;
   uint64_t* p_ready = s_full + 1;
   uint64_t* dp_full = p_ready + 1;
   uint64_t* ds_ready = dp_full + 1;
@@ -118,18 +133,24 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (threadIdx.x == 0) atomicOr(status, kStatusBadShape);
+    return;
+  }
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
     for (int i = 0; i < kRing; ++i) {
-      mbar_init(&q_full[i], 1);
-      mbar_init(&do_full[i], 1);
+      mbar_init(&ring.full[i], 1);
+      mbar_init(&ring.empty[i], 1);
+    }
+    for (int i = 0; i < kStatRing; ++i) {
       mbar_init(&st_full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&st_empty[i], kComputeWarps);
     }
     mbar_init(s_full, 1);
-    mbar_init(p_ready, 8);
+    mbar_init(p_ready, kComputeWarps);
     mbar_init(dp_full, 1);
-    mbar_init(ds_ready, 8);
+    mbar_init(ds_ready, kComputeWarps);
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -161,57 +182,54 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
     if (warp == 0) {
       if (lane == 0) {
-        const uint32_t ra = smem_u32(ring);
         mbar_arrive_expect_tx(kv_full, 2 * kTileBytes);
         load_tile<DP>(smem_u32(k_tile), &tm_k, kv_full, kvh, key0);
         load_tile<DP>(smem_u32(v_tile), &tm_v, kv_full, kvh, key0);
-        for (int it = 0; it < total; ++it) {
-          const int s = it % kRing;
-          if (!mbar_wait(&empty[s], ((it / kRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag)) break;
-          mbar_arrive_expect_tx(&q_full[s], kTileBytes);
-          load_tile<DP>(ra + 2 * s * kTileBytes, &tm_q, &q_full[s], head_of(it), row_of(it));
-          mbar_arrive_expect_tx(&do_full[s], kTileBytes);
-          load_tile<DP>(ra + (2 * s + 1) * kTileBytes, &tm_do, &do_full[s], head_of(it), row_of(it));
+        for (int x = 0; x < 2 * total; ++x) {  // Q, dO of every iteration in turn
+          if (!mbar_wait(ring.empty_of(x), ring.use(x) ^ 1, status, kStatusWaitEmpty, abort_flag)) break;
+          mbar_arrive_expect_tx(ring.full_of(x), kTileBytes);
+          load_tile<DP>(smem_u32(ring.tile(x)), (x & 1) ? &tm_do : &tm_q, ring.full_of(x), head_of(x >> 1),
+                        row_of(x >> 1));
         }
       }
     } else if (warp == 1) {
       const bool leader = elect_one();
-      const uint32_t ka = smem_u32(k_tile), va = smem_u32(v_tile), ra = smem_u32(ring);
+      const uint32_t ka = smem_u32(k_tile), va = smem_u32(v_tile);
       auto rows16 = [&](int it) { return (min(kRowsT, hi - row_of(it)) + 15) & ~15; };
-      // the tile of iteration it (Q: which 0, dO: which 1), rows past the sequence's end zeroed
-      auto ready = [&](int it, int which) {
-        const int s = it % kRing;
-        if (!warp_wait(which ? &do_full[s] : &q_full[s], (it / kRing) & 1, status, kStatusWaitFull, abort_flag))
-          return false;
-        const int n = min(kRowsT, hi - row_of(it)), n16 = (n + 15) & ~15;
-        if (n != n16) zero_rows<DP>(ring + (2 * s + which) * kTileBytes, n, n16, lane);
+      // item x is in shared memory, its rows past the sequence's end zeroed
+      auto ready = [&](int x) {
+        if (!warp_wait(ring.full_of(x), ring.use(x), status, kStatusWaitFull, abort_flag)) return false;
+        const int n = min(kRowsT, hi - row_of(x >> 1)), n16 = (n + 15) & ~15;
+        if (n != n16) zero_rows<DP>(ring.tile(x), n, n16, lane);
         tc_fence_after();
         return true;
       };
-      bool ok = warp_wait(kv_full, 0, status, kStatusWaitFull, abort_flag) && ready(0, 0);
+      bool ok = warp_wait(kv_full, 0, status, kStatusWaitFull, abort_flag) && ready(0);
       if (ok && leader) {
-        mma_dims<DP>(t_s, ka, ra, rows16(0), ksteps);
+        mma_dims<DP>(t_s, ka, smem_u32(ring.tile(0)), rows16(0), ksteps);
         umma_commit(s_full);
       }
-      ok = ok && ready(0, 1);
+      ok = ok && ready(1);
       if (ok && leader) {
-        mma_dims<DP>(t_dp, va, ra + kTileBytes, rows16(0), ksteps);
+        mma_dims<DP>(t_dp, va, smem_u32(ring.tile(1)), rows16(0), ksteps);
         umma_commit(dp_full);
       }
       __syncwarp();
       for (int it = 0; ok && it < total; ++it) {
-        const int s = it % kRing, s1 = (it + 1) % kRing;
         const bool more = it + 1 < total;
-        const uint32_t qa = ra + 2 * s * kTileBytes, da = qa + kTileBytes;
+        const int xq = 2 * it, xd = xq + 1;
         ok = warp_wait(p_ready, it & 1, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        if (leader) mma_rows<64>(t_dv, t_s, da, ksteps * 16, rows16(it) / 16, it > 0);
+        if (leader) {
+          mma_rows<2, 32>(t_dv, t_s, smem_u32(ring.tile(xd)), ksteps * 16, rows16(it) / 16, it > 0);
+          umma_commit(ring.empty_of(xd));
+        }
         if (more) {
-          ok = ready(it + 1, 0);
+          ok = ready(xq + 2);
           if (!ok) break;
           if (leader) {
-            mma_dims<DP>(t_s, ka, ra + 2 * s1 * kTileBytes, rows16(it + 1), ksteps);
+            mma_dims<DP>(t_s, ka, smem_u32(ring.tile(xq + 2)), rows16(it + 1), ksteps);
             umma_commit(s_full);
           }
         }
@@ -220,14 +238,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!ok) break;
         tc_fence_after();
         if (leader) {
-          mma_rows<64>(t_dk, t_dp, qa, ksteps * 16, rows16(it) / 16, it > 0);
-          umma_commit(&empty[s]);
+          mma_rows<2, 32>(t_dk, t_dp, smem_u32(ring.tile(xq)), ksteps * 16, rows16(it) / 16, it > 0);
+          umma_commit(ring.empty_of(xq));
         }
         if (more) {
-          ok = ready(it + 1, 1);
+          ok = ready(xd + 2);
           if (!ok) break;
           if (leader) {
-            mma_dims<DP>(t_dp, va, ra + (2 * s1 + 1) * kTileBytes, rows16(it + 1), ksteps);
+            mma_dims<DP>(t_dp, va, smem_u32(ring.tile(xd + 2)), rows16(it + 1), ksteps);
             umma_commit(dp_full);
           }
         }
@@ -237,8 +255,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     } else if (warp == 2) {
       // ---- lse and delta of the query tiles ----
       for (int it = 0; it < total; ++it) {
-        const int s = it % kRing;
-        if (!warp_wait(&empty[s], ((it / kRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag)) break;
+        const int s = it % kStatRing;
+        if (!warp_wait(&st_empty[s], ((it / kStatRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag)) break;
         const long base = static_cast<long>(head_of(it)) * p.T;
         float* dst = stats + s * 256;
 #pragma unroll
@@ -251,28 +269,28 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (lane == 0) mbar_arrive(&st_full[s]);
       }
     } else if (warp >= 4) {
-      // ---- P^T and dS^T: one thread per key and half of the queries ----
-      const int half = (warp - 4) >> 2, quad = warp & 3;
+      // ---- P^T and dS^T: one thread per key and quarter of the queries ----
+      const int part = (warp - 4) >> 2, quad = warp & 3;
       const int key = quad * 32 + lane;  // relative to key0
       const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
-      const uint32_t s_addr = t_s + lane_base + half * 64, dp_addr = t_dp + lane_base + half * 64;
+      const uint32_t s_addr = t_s + lane_base + part * 32, dp_addr = t_dp + lane_base + part * 32;
       bool ok = true;
       for (int it = 0; it < total; ++it) {
-        const int s = it % kRing;
-        const float* lse = stats + s * 256 + half * 64;
+        const int s = it % kStatRing;
+        const float* lse = stats + s * 256 + part * 32;
         const float* delta = lse + 128;
-        ok = warp_wait(&st_full[s], (it / kRing) & 1, status, kStatusWaitFull, abort_flag) &&
+        ok = warp_wait(&st_full[s], (it / kStatRing) & 1, status, kStatusWaitFull, abort_flag) &&
              warp_wait(s_full, it & 1, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        float v[64];
-        tmem_load64(s_addr, v);
-        // queries [from, to) of this half see the key
+        float v[32];
+        tmem_load32(s_addr, v);
+        // queries [from, to) of this part see the key
         const int q0 = row_of(it) - key0;
-        const int from = q0 == 0 ? key - half * 64 : 0, to = hi - row_of(it) - half * 64;
-        const bool masked = q0 == 0 || to < 64;
+        const int from = q0 == 0 ? key - part * 32 : 0, to = hi - row_of(it) - part * 32;
+        const bool masked = q0 == 0 || to < 32;
 #pragma unroll
-        for (int j = 0; j < 64; j += 4) {
+        for (int j = 0; j < 32; j += 4) {
           const float4 l = *reinterpret_cast<const float4*>(lse + j);
           v[j] = ex2(fmaf(v[j], p.scale2, -l.x));
           v[j + 1] = ex2(fmaf(v[j + 1], p.scale2, -l.y));
@@ -281,12 +299,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         if (masked) {
 #pragma unroll
-          for (int j = 0; j < 64; ++j) v[j] = (j >= from && j < to) ? v[j] : 0.f;
+          for (int j = 0; j < 32; ++j) v[j] = (j >= from && j < to) ? v[j] : 0.f;
         }
-        uint32_t w[32];
+        uint32_t w[16];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
-        tmem_store32(s_addr, w);
+        for (int j = 0; j < 16; ++j) w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+        tmem_st_u32x16(s_addr, w);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -294,10 +312,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         ok = warp_wait(dp_full, it & 1, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        float g[64];
-        tmem_load64(dp_addr, g);
+        float g[32];
+        tmem_load32(dp_addr, g);
 #pragma unroll
-        for (int j = 0; j < 64; j += 4) {
+        for (int j = 0; j < 32; j += 4) {
           const float4 d = *reinterpret_cast<const float4*>(delta + j);
           g[j] = v[j] * (g[j] - d.x);
           g[j + 1] = v[j + 1] * (g[j + 1] - d.y);
@@ -306,23 +324,26 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         if (masked) {
 #pragma unroll
-          for (int j = 0; j < 64; ++j) g[j] = (j >= from && j < to) ? g[j] : 0.f;
+          for (int j = 0; j < 32; ++j) g[j] = (j >= from && j < to) ? g[j] : 0.f;
         }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) w[j] = pack_bf16(g[2 * j], g[2 * j + 1]);
-        tmem_store32(dp_addr, w);
+        for (int j = 0; j < 16; ++j) w[j] = pack_bf16(g[2 * j], g[2 * j + 1]);
+        tmem_st_u32x16(dp_addr, w);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(ds_ready);
+        if (lane == 0) {
+          mbar_arrive(ds_ready);
+          mbar_arrive(&st_empty[s]);
+        }
       }
       if (ok && warp_wait(done, 0, status, kStatusWaitAccum, abort_flag)) {
         tc_fence_after();
-        const int row = key0 + key;
+        const int row = key0 + key, col = (part & 1) * (DP / 2);
         const bool real = row < hi;
-        const long at = (static_cast<long>(row) * p.Hkv + kvh) * p.D;
-        if (half == 0) store_row<DP>(t_dv + lane_base, 1.f, p.dv + at, p.D, real);
-        else store_row<DP>(t_dk + lane_base, p.scale, p.dk + at, p.D, real);
+        const long at = (static_cast<long>(row) * p.Hkv + kvh) * p.D + col;
+        if (part < 2) store_row<DP / 2>(t_dv + lane_base + col, 1.f, p.dv + at, p.D - col, real);
+        else store_row<DP / 2>(t_dk + lane_base + col, p.scale, p.dk + at, p.D - col, real);
       }
     }
   }
@@ -341,15 +362,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                      const __grid_constant__ BwdArgs p, unsigned* status) {
   using Cfg = BwdCfg<DP>;
   constexpr int kRing = Cfg::kRing, kTileBytes = Cfg::kTileBytes;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t *q_tile = smem, *do_tile = smem + kTileBytes;
-  uint8_t* ring = smem + 2 * kTileBytes;  // stage s: K at 2 s, V at 2 s + 1
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + 2 * kRing * kTileBytes);
-  uint64_t* k_full = q_full + 1;
-  uint64_t* v_full = k_full + kRing;
-  uint64_t* empty = v_full + kRing;
-  uint64_t* s_full = empty + kRing;  // one per S buffer: S of chunk c + 1 may complete before c's is looked at
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + (2 + kRing) * kTileBytes);
+  Stream<DP> ring{smem + 2 * kTileBytes, q_full + 1, q_full + 1 + kRing};
+  uint64_t* s_full = q_full + 1 + 2 * kRing;  // one per S buffer: S of chunk c + 1 may complete before c's is looked at
   uint64_t* dp_full = s_full + 2;
   uint64_t* ds_ready = dp_full + 1;
   uint64_t* done = ds_ready + 1;
@@ -357,17 +374,20 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (threadIdx.x == 0) atomicOr(status, kStatusBadShape);
+    return;
+  }
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     for (int i = 0; i < kRing; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&v_full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&ring.full[i], 1);
+      mbar_init(&ring.empty[i], 1);
     }
     mbar_init(&s_full[0], 1);
     mbar_init(&s_full[1], 1);
     mbar_init(dp_full, 1);
-    mbar_init(ds_ready, 8);
+    mbar_init(ds_ready, kComputeWarps);
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -394,43 +414,39 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
     if (warp == 0) {
       if (lane == 0) {
-        const uint32_t ra = smem_u32(ring);
         mbar_arrive_expect_tx(q_full, 2 * kTileBytes);
         load_tile<DP>(smem_u32(q_tile), &tm_q, q_full, head, row0);
         load_tile<DP>(smem_u32(do_tile), &tm_do, q_full, head, row0);
-        for (int c = 0; c < n; ++c) {
-          const int s = c % kRing;
-          if (!mbar_wait(&empty[s], ((c / kRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag)) break;
-          mbar_arrive_expect_tx(&k_full[s], kTileBytes);
-          load_tile<DP>(ra + 2 * s * kTileBytes, &tm_k, &k_full[s], kvh, lo + c * kRowsT);
-          mbar_arrive_expect_tx(&v_full[s], kTileBytes);
-          load_tile<DP>(ra + (2 * s + 1) * kTileBytes, &tm_v, &v_full[s], kvh, lo + c * kRowsT);
+        for (int x = 0; x < 2 * n; ++x) {  // K, V of every chunk in turn
+          if (!mbar_wait(ring.empty_of(x), ring.use(x) ^ 1, status, kStatusWaitEmpty, abort_flag)) break;
+          mbar_arrive_expect_tx(ring.full_of(x), kTileBytes);
+          load_tile<DP>(smem_u32(ring.tile(x)), (x & 1) ? &tm_v : &tm_k, ring.full_of(x), kvh,
+                        lo + (x >> 1) * kRowsT);
         }
       }
     } else if (warp == 1) {
       const bool leader = elect_one();
-      const uint32_t qa = smem_u32(q_tile), da = smem_u32(do_tile), ra = smem_u32(ring);
+      const uint32_t qa = smem_u32(q_tile), da = smem_u32(do_tile);
       auto keys16 = [&](int c) { return (min(kRowsT, hi - (lo + c * kRowsT)) + 15) & ~15; };
       auto scores = [&](int c) {  // S of chunk c into its buffer; K rows past the end zeroed
-        const int s = c % kRing;
-        if (!warp_wait(&k_full[s], (c / kRing) & 1, status, kStatusWaitFull, abort_flag)) return false;
+        if (!warp_wait(ring.full_of(2 * c), ring.use(2 * c), status, kStatusWaitFull, abort_flag)) return false;
         const int keys = min(kRowsT, hi - (lo + c * kRowsT));
-        if (keys != keys16(c)) zero_rows<DP>(ring + 2 * s * kTileBytes, keys, keys16(c), lane);
+        if (keys != keys16(c)) zero_rows<DP>(ring.tile(2 * c), keys, keys16(c), lane);
         tc_fence_after();
         if (leader) {
-          mma_dims<DP>(t_s + (c & 1) * 128, qa, ra + 2 * s * kTileBytes, keys16(c), ksteps);
+          mma_dims<DP>(t_s + (c & 1) * 128, qa, smem_u32(ring.tile(2 * c)), keys16(c), ksteps);
           umma_commit(&s_full[c & 1]);
         }
         __syncwarp();
         return true;
       };
-      auto products = [&](int c) {  // dP of chunk c
-        const int s = c % kRing;
-        if (!warp_wait(&v_full[s], (c / kRing) & 1, status, kStatusWaitFull, abort_flag)) return false;
+      auto products = [&](int c) {  // dP of chunk c, the only use of its V
+        if (!warp_wait(ring.full_of(2 * c + 1), ring.use(2 * c + 1), status, kStatusWaitFull, abort_flag)) return false;
         tc_fence_after();
         if (leader) {
-          mma_dims<DP>(t_dp, da, ra + (2 * s + 1) * kTileBytes, keys16(c), ksteps);
+          mma_dims<DP>(t_dp, da, smem_u32(ring.tile(2 * c + 1)), keys16(c), ksteps);
           umma_commit(dp_full);
+          umma_commit(ring.empty_of(2 * c + 1));
         }
         __syncwarp();
         return true;
@@ -445,16 +461,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (more) ok = products(c + 1);
         if (!ok) break;
         if (leader) {
-          mma_rows<64>(t_dq, t_s + (c & 1) * 128, ra + 2 * (c % kRing) * kTileBytes, ksteps * 16, keys16(c) / 16,
-                   c > 0);
-          umma_commit(&empty[c % kRing]);
+          mma_rows<2, 32>(t_dq, t_s + (c & 1) * 128, smem_u32(ring.tile(2 * c)), ksteps * 16, keys16(c) / 16, c > 0);
+          umma_commit(ring.empty_of(2 * c));
         }
         __syncwarp();
       }
       if (ok && leader) umma_commit(done);
     } else if (warp >= 4) {
-      // ---- dS: one thread per query and half of the keys ----
-      const int half = (warp - 4) >> 2, quad = warp & 3;
+      // ---- dS: one thread per query and quarter of the keys ----
+      const int part = (warp - 4) >> 2, quad = warp & 3;
       const int row = row0 + quad * 32 + lane;
       const bool real = row < hi;
       const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
@@ -462,29 +477,29 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const float delta = real ? p.delta[static_cast<long>(head) * p.T + row] : 0.f;
       bool ok = true;
       for (int c = 0; c < n; ++c) {
-        const uint32_t s_addr = t_s + (c & 1) * 128 + lane_base + half * 64;
+        const uint32_t s_addr = t_s + (c & 1) * 128 + lane_base + part * 32;
         ok = warp_wait(&s_full[c & 1], (c >> 1) & 1, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        float v[64], g[64];
-        tmem_load64(s_addr, v);
+        float v[32], g[32];
+        tmem_load32(s_addr, v);
 #pragma unroll
-        for (int j = 0; j < 64; ++j) v[j] = ex2(fmaf(v[j], p.scale2, -lse));
+        for (int j = 0; j < 32; ++j) v[j] = ex2(fmaf(v[j], p.scale2, -lse));
         ok = warp_wait(dp_full, c & 1, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        tmem_load64(t_dp + lane_base + half * 64, g);
+        tmem_load32(t_dp + lane_base + part * 32, g);
 #pragma unroll
-        for (int j = 0; j < 64; ++j) g[j] = v[j] * (g[j] - delta);
+        for (int j = 0; j < 32; ++j) g[j] = v[j] * (g[j] - delta);
         if (c == n - 1) {
-          const int limit = min(hi, row + 1) - (lo + c * kRowsT) - half * 64;
+          const int limit = min(hi, row + 1) - (lo + c * kRowsT) - part * 32;
 #pragma unroll
-          for (int j = 0; j < 64; ++j) g[j] = j < limit ? g[j] : 0.f;
+          for (int j = 0; j < 32; ++j) g[j] = j < limit ? g[j] : 0.f;
         }
-        uint32_t w[32];
+        uint32_t w[16];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) w[j] = pack_bf16(g[2 * j], g[2 * j + 1]);
-        tmem_store32(s_addr, w);
+        for (int j = 0; j < 16; ++j) w[j] = pack_bf16(g[2 * j], g[2 * j + 1]);
+        tmem_st_u32x16(s_addr, w);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -492,8 +507,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       if (ok && warp_wait(done, 0, status, kStatusWaitAccum, abort_flag)) {
         tc_fence_after();
-        if (half == 0)  // half of the columns each would save little: one store per row
-          store_row<DP>(t_dq + lane_base, p.scale, p.dq + (static_cast<long>(row) * p.H + head) * p.D, p.D, real);
+        const int col = part * (DP / 4);
+        store_row<DP / 4>(t_dq + lane_base + col, p.scale, p.dq + (static_cast<long>(row) * p.H + head) * p.D + col,
+                          p.D - col, real);
       }
     }
   }

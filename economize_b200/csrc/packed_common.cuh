@@ -81,15 +81,15 @@ __device__ __forceinline__ void mma_dims(uint32_t d, uint32_t a, uint32_t b, int
   }
 }
 
-// D[128, n] (+)= P[128, :16 ksteps] . B[:16 ksteps, n], P packed bf16 in TMEM (64 of its columns every kHalf 32-bit
-// columns), B's rows along K (MN-major).
-template <int kHalf>
+// D[128, n] (+)= P[128, :16 ksteps] . B[:16 ksteps, n], P packed bf16 in TMEM (kPer K steps of 8 columns side by side in
+// every group of kStride columns), B's rows along K (MN-major).
+template <int kPer, int kStride>
 __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t p, uint32_t b, int n, int ksteps, bool accumulate) {
   const uint32_t idesc = idesc_bf16_f32(128, n, true);
   const uint64_t db = desc_mnmajor_sw128(b, kRowsT * 128);
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk) {
-    const uint32_t pc = p + (kk >> 2) * kHalf + (kk & 3) * 8;
+    const uint32_t pc = p + (kk / kPer) * kStride + (kk % kPer) * 8;
     if (kk < ksteps) umma_bf16_ta(d, pc, desc_step(db, kk * 16 * 128), idesc, kk != 0 ? 1u : (accumulate ? 1u : 0u));
   }
 }
