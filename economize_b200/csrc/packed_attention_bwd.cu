@@ -379,10 +379,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   uint8_t *q_tile = smem, *do_tile = smem + kTileBytes;
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + (2 + kRing) * kTileBytes);
   Stream<DP> ring{smem + 2 * kTileBytes, q_full + 1, q_full + 1 + kRing};
-  uint64_t* s_full = q_full + 1 + 2 * kRing;  // one per S buffer: S of chunk c + 1 may complete before c's is looked at
-  uint64_t* dp_full = s_full + 2;
-  uint64_t* ds_ready = dp_full + 1;
-  uint64_t* done = ds_ready + 1;
+  uint64_t* s_full = q_full + 1 + 2 * kRing;  // [2], of the S buffer of even and odd chunks
+  uint64_t* dp_full = s_full + 2;             // [2], by chunk parity: each is waited for by one group
+  uint64_t* dp_free = dp_full + 2;
+  uint64_t* ds_ready = dp_free + 2;
+  uint64_t* done = ds_ready + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -397,10 +398,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&ring.full[i], 1);
       mbar_init(&ring.empty[i], 1);
     }
-    mbar_init(&s_full[0], 1);
-    mbar_init(&s_full[1], 1);
-    mbar_init(dp_full, 1);
-    mbar_init(ds_ready, kComputeWarps);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&dp_full[i], 1);
+      mbar_init(&dp_free[i], kComputeWarps / 2);
+      mbar_init(&ds_ready[i], kComputeWarps / 2);
+    }
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -458,64 +461,89 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       };
       auto products = [&](int c) {  // dP of chunk c, the only use of its V (leader only)
         mma_dims<DP>(t_dp, da, smem_u32(ring.tile(2 * c + 1)), keys16(c), ksteps);
-        umma_commit(dp_full);
+        umma_commit(&dp_full[c & 1]);
         umma_commit(ring.empty_of(2 * c + 1));
       };
       bool ok = warp_wait(q_full, 0, status, kStatusWaitFull, abort_flag) && scores(0) && values(0);
       tc_fence_after();
       if (ok && leader) products(0);
       __syncwarp();
+      if (ok && n > 1) ok = scores(1);
       for (int c = 0; ok && c < n; ++c) {
-        const bool more = c + 1 < n;
-        if (more) ok = scores(c + 1) && values(c + 1);
-        ok = ok && warp_wait(ds_ready, c & 1, status, kStatusWaitAccum, abort_flag);
+        const uint32_t use = (c >> 1) & 1;
+        if (c + 1 < n) {  // dP of the next chunk as soon as this one's is in registers
+          ok = values(c + 1) && warp_wait(&dp_free[c & 1], use, status, kStatusWaitAccum, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) products(c + 1);
+          __syncwarp();
+        }
+        ok = warp_wait(&ds_ready[c & 1], use, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
         if (leader) {
-          if (more) products(c + 1);
-          mma_rows<2, 32>(t_dq, t_s + (c & 1) * 128, smem_u32(ring.tile(2 * c)), ksteps * 16, keys16(c) / 16, c > 0);
+          mma_rows<4, 64>(t_dq, t_s + (c & 1) * 128, smem_u32(ring.tile(2 * c)), ksteps * 16, keys16(c) / 16, c > 0);
           umma_commit(ring.empty_of(2 * c));
         }
         __syncwarp();
+        if (c + 2 < n) ok = scores(c + 2);
       }
       if (ok && leader) umma_commit(done);
     } else if (warp >= 4) {
-      // ---- dS: one thread per query and quarter of the keys ----
+      // ---- dS: two groups of eight warps take the even and the odd chunks, so that the exponentials of one chunk run
+      // beside the products of the other; one thread per query and half of the chunk's keys ----
       const int part = (warp - 4) >> 2, quad = warp & 3;
+      const int mine = part >> 1, half = part & 1;
       const int row = row0 + quad * 32 + lane;
       const bool real = row < hi;
       const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
       const float lse = real ? p.lse[static_cast<long>(head) * p.T + row] : 0.f;
       const float delta = real ? p.delta[static_cast<long>(head) * p.T + row] : 0.f;
+      const uint32_t s_addr = t_s + mine * 128 + lane_base + half * 64, dp_addr = t_dp + lane_base + half * 64;
       bool ok = true;
-      for (int c = 0; c < n; ++c) {
-        const uint32_t s_addr = t_s + (c & 1) * 128 + lane_base + part * 32;
-        ok = warp_wait(&s_full[c & 1], (c >> 1) & 1, status, kStatusWaitAccum, abort_flag);
+      for (int c = mine; c < n; c += 2) {
+        const uint32_t use = (c >> 1) & 1;
+        ok = warp_wait(&s_full[mine], use, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        float v[32], g[32];
-        tmem_load32(s_addr, v);
+        const bool last = c == n - 1;
+        const int limit = min(hi, row + 1) - (lo + c * kRowsT) - half * 64;  // visible keys, of the last chunk
+        // P waits for dP in the columns S came from: 64 more registers would spill
+        float v[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = ex2(fmaf(v[j], p.scale2, -lse));
-        ok = warp_wait(dp_full, c & 1, status, kStatusWaitAccum, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        tmem_load32(t_dp + lane_base + part * 32, g);
+        for (int h = 0; h < 64; h += 32) {
+          tmem_load32(s_addr + h, v);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) g[j] = v[j] * (g[j] - delta);
-        if (c == n - 1) {
-          const int limit = min(hi, row + 1) - (lo + c * kRowsT) - part * 32;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) g[j] = j < limit ? g[j] : 0.f;
+          for (int j = 0; j < 32; ++j) v[j] = ex2(fmaf(v[j], p.scale2, -lse));
+          tmem_store32(s_addr + h, reinterpret_cast<const uint32_t*>(v));
         }
-        uint32_t w[16];
+        tmem_wait_st();
+        ok = warp_wait(&dp_full[mine], use, status, kStatusWaitAccum, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        float g[32];
+        uint32_t w[32];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = pack_bf16(g[2 * j], g[2 * j + 1]);
-        tmem_st_u32x16(s_addr, w);
+        for (int h = 0; h < 64; h += 32) {
+          tmem_load32(s_addr + h, v);
+          tmem_load32(dp_addr + h, g);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) g[j] = v[j] * (g[j] - delta);
+          if (last) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) g[j] = h + j < limit ? g[j] : 0.f;
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) w[h / 2 + j] = pack_bf16(g[2 * j], g[2 * j + 1]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&dp_free[mine]);
+        tmem_store32(s_addr, w);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(ds_ready);
+        if (lane == 0) mbar_arrive(&ds_ready[mine]);
       }
       if (ok && warp_wait(done, 0, status, kStatusWaitAccum, abort_flag)) {
         tc_fence_after();
