@@ -302,18 +302,111 @@ std::tuple<c10::optional<Tensor>, c10::optional<Tensor>, c10::optional<Tensor>> 
   return {dq, dk, dv};
 }
 
-// x *= g (a scalar on the device) in place.
-void scale_by(Tensor x, Tensor g) {
-  CHECK_CUDA(x);
-  CHECK_BF16(x);
-  CHECK_ON(g, x);
-  TORCH_CHECK(x.is_contiguous() && x.numel() % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0,
-              "scale_by takes a contiguous tensor of 8 n values");
-  TORCH_CHECK(g.scalar_type() == at::kFloat && g.numel() == 1, "scale_by takes an fp32 scalar");
-  c10::cuda::CUDAGuard guard(x.device());
-  TORCH_CHECK(ecz::launch_scale_by(x.data_ptr(), x.numel(), g.data_ptr<float>(), ecz::device_sms(x.get_device()),
+// The gradients times a scalar on the device, in place (one launch; undefined ones are skipped).
+void scale_both(const Tensor& dx, const Tensor& dw, const Tensor& g) {
+  const Tensor& any = dx.defined() ? dx : dw;
+  if (!any.defined()) return;
+  c10::cuda::CUDAGuard guard(any.device());
+  TORCH_CHECK(ecz::launch_scale_by(dx.defined() ? dx.data_ptr() : nullptr, dx.defined() ? dx.numel() : 0,
+                                   dw.defined() ? dw.data_ptr() : nullptr, dw.defined() ? dw.numel() : 0,
+                                   g.data_ptr<float>(), ecz::device_sms(any.get_device()),
                                    at::cuda::getCurrentCUDAStream()) == 0,
-              "scale_by: launch failed");
+              "linear_cross_entropy: scaling launch failed");
+}
+
+// ---- autograd ------------------------------------------------------------------------------------------------------
+// In C++: a training step's small calls would otherwise spend more time in Python's autograd hooks than on the GPU
+// (a forward and backward pair of either operator took 100 to 120 us on the host as Python functions).
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void once(const char* name) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), name, " cannot be differentiated twice");
+}
+
+// Losses of the readout. A scalar loss computes its gradients in the forward pass, where the unnormalised probabilities
+// are at hand, and the backward pass scales them by the upstream gradient; per-row losses, whose upstream gradients are
+// not known by then, run the products again in the backward pass.
+struct ReadoutFunction : torch::autograd::Function<ReadoutFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& targets,
+                        int64_t ignore_index, double logit_scale, int64_t reduction, int64_t chunk_rows) {
+    const bool now = reduction != ecz::kReduceNone;
+    auto r = readout(hidden, weight, targets, ignore_index, logit_scale, reduction, now && hidden.requires_grad(),
+                     now && weight.requires_grad(), c10::nullopt, chunk_rows);
+    ctx->save_for_backward({hidden, weight, targets});
+    ctx->saved_data["ignore"] = ignore_index;
+    ctx->saved_data["scale"] = logit_scale;
+    ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["chunk"] = chunk_rows;
+    if (std::get<1>(r)) ctx->saved_data["dx"] = *std::get<1>(r);
+    if (std::get<2>(r)) ctx->saved_data["dw"] = *std::get<2>(r);
+    ctx->saved_data["held"] = now;
+    return std::get<0>(r);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("linear_cross_entropy");
+    auto& data = ctx->saved_data;
+    const bool need_dx = ctx->needs_input_grad(0), need_dw = ctx->needs_input_grad(1);
+    const int64_t reduction = data["reduction"].toInt();
+    variable_list out(7);
+    Tensor g = grads[0].to(at::kFloat).contiguous();
+    const bool per_row = reduction == ecz::kReduceNone;
+    if (!per_row && data["held"].toBool()) {
+      // the buffers are given away: a second pass over a retained graph computes them again
+      if (need_dx) out[0] = data["dx"].toTensor();
+      if (need_dw) out[1] = data["dw"].toTensor();
+      data.erase("dx");
+      data.erase("dw");
+      data["held"] = false;
+    } else {
+      const auto saved = ctx->get_saved_variables();
+      auto r = readout(saved[0], saved[1], saved[2], data["ignore"].toInt(), data["scale"].toDouble(), reduction,
+                       need_dx, need_dw, per_row ? c10::optional<Tensor>(g) : c10::nullopt, data["chunk"].toInt());
+      if (need_dx) out[0] = *std::get<1>(r);
+      if (need_dw) out[1] = *std::get<2>(r);
+    }
+    if (!per_row) scale_both(out[0], out[1], g);
+    return out;
+  }
+};
+
+Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t ignore_index,
+                            double logit_scale, int64_t reduction, int64_t chunk_rows) {
+  if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad()))
+    return ReadoutFunction::apply(hidden, weight, targets, ignore_index, logit_scale, reduction, chunk_rows);
+  return std::get<0>(
+      readout(hidden, weight, targets, ignore_index, logit_scale, reduction, false, false, c10::nullopt, chunk_rows));
+}
+
+struct PackedFunction : torch::autograd::Function<PackedFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu,
+                        double scale) {
+    auto r = packed_forward(q, k, v, cu, scale, true);
+    ctx->save_for_backward({q, k, v, std::get<0>(r), *std::get<1>(r), cu});
+    ctx->saved_data["scale"] = scale;
+    return std::get<0>(r);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("packed_attention");
+    const auto s = ctx->get_saved_variables();
+    const bool need_dq = ctx->needs_input_grad(0);
+    const bool need_dk = ctx->needs_input_grad(1), need_dv = ctx->needs_input_grad(2);
+    auto r = packed_backward(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble(),
+                             need_dq, need_dk || need_dv);
+    variable_list out(5);
+    if (need_dq) out[0] = *std::get<0>(r);
+    if (need_dk) out[1] = *std::get<1>(r);
+    if (need_dv) out[2] = *std::get<2>(r);
+    return out;
+  }
+};
+
+Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, double scale) {
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    return PackedFunction::apply(q, k, v, cu, scale);
+  return std::get<0>(packed_forward(q, k, v, cu, scale, false));
 }
 
 }  // namespace
@@ -322,16 +415,12 @@ namespace ecz {
 
 void bind_training(pybind11::module_& m) {
   namespace py = pybind11;
-  m.def("readout", &readout, "softmax cross-entropy of hidden @ weight.T without keeping the logits, with gradients",
-        py::arg("hidden"), py::arg("weight"), py::arg("targets"), py::arg("ignore_index"), py::arg("logit_scale"),
-        py::arg("reduction"), py::arg("need_dx"), py::arg("need_dw"), py::arg("grad_rows") = py::none(),
+  m.def("linear_cross_entropy", &linear_cross_entropy,
+        "softmax cross-entropy of hidden @ weight.T without keeping the logits (autograd)", py::arg("hidden"),
+        py::arg("weight"), py::arg("targets"), py::arg("ignore_index"), py::arg("logit_scale"), py::arg("reduction"),
         py::arg("chunk_rows") = 0);
-  m.def("packed_forward", &packed_forward, "causal attention over packed sequences (tcgen05)", py::arg("q"),
-        py::arg("k"), py::arg("v"), py::arg("cu_seqlens"), py::arg("scale"), py::arg("need_lse"));
-  m.def("packed_backward", &packed_backward, "gradients of packed_forward", py::arg("dout"), py::arg("q"),
-        py::arg("k"), py::arg("v"), py::arg("out"), py::arg("lse"), py::arg("cu_seqlens"), py::arg("scale"),
-        py::arg("need_dq"), py::arg("need_dkv"));
-  m.def("scale_by", &scale_by, "x *= g in place for a device scalar g (no memory pass when g is 1)");
+  m.def("packed_attention", &packed_attention, "causal attention over packed sequences (tcgen05, autograd)",
+        py::arg("q"), py::arg("k"), py::arg("v"), py::arg("cu_seqlens"), py::arg("scale"));
 }
 
 }  // namespace ecz

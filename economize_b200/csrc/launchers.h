@@ -302,8 +302,8 @@ int launch_readout_dx(const CUtensorMap* dz, const CUtensorMap* w, const Readout
                       void* dx, int num_sms, unsigned* status, cudaStream_t stream);
 int launch_readout_dw(const CUtensorMap* dz, const CUtensorMap* xs, const ReadoutChunk& c, float* sum, bool first,
                       bool last, void* dw, int num_sms, unsigned* status, cudaStream_t stream);
-// x *= *g in place (bf16, n a multiple of 8).
-int launch_scale_by(void* x, long n, const float* g, int num_sms, cudaStream_t stream);
+// x and y (bf16, sizes multiples of 8) times *g in place.
+int launch_scale_by(void* x, long nx, void* y, long ny, const float* g, int num_sms, cudaStream_t stream);
 
 // packed_attention.cu: causal attention over packed sequences (see the file comment). Maps: 3-D {D, heads, T}, box
 // {64, 1, 128}, 128-byte swizzle.

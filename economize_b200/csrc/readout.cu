@@ -391,14 +391,18 @@ __global__ void __launch_bounds__(256) readout_join_kernel(const float* __restri
   *reinterpret_cast<uint2*>(out + static_cast<long>(rows[m]) * N + c) = w;
 }
 
-// x *= *g in place (bf16, n a multiple of 8); reads nothing more when *g is 1, what a loss's own backward passes.
-__global__ void __launch_bounds__(256) scale_by_kernel(bf16* __restrict__ x, long n8, const float* __restrict__ g) {
+// x and y times *g in place (bf16, sizes in groups of 8); reads nothing more when *g is 1, what a loss's own backward
+// passes.
+__global__ void __launch_bounds__(256) scale_by_kernel(uint4* __restrict__ x, long nx, uint4* __restrict__ y, long ny,
+                                                       const float* __restrict__ g) {
   pdl_trigger();
   pdl_wait();
   const float s = *g;
   if (s == 1.f) return;
-  for (long i = static_cast<long>(blockIdx.x) * 256 + threadIdx.x; i < n8; i += static_cast<long>(gridDim.x) * 256) {
-    uint4 v = reinterpret_cast<uint4*>(x)[i];
+  for (long i = static_cast<long>(blockIdx.x) * 256 + threadIdx.x; i < nx + ny;
+       i += static_cast<long>(gridDim.x) * 256) {
+    uint4* at = i < nx ? x + i : y + (i - nx);
+    uint4 v = *at;
     uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -406,7 +410,7 @@ __global__ void __launch_bounds__(256) scale_by_kernel(bf16* __restrict__ x, lon
       __nv_bfloat162 o = __floats2bfloat162_rn(f.x * s, f.y * s);
       w[k] = *reinterpret_cast<uint32_t*>(&o);
     }
-    reinterpret_cast<uint4*>(x)[i] = v;
+    *at = v;
   }
 }
 
@@ -478,12 +482,11 @@ int launch_readout_dw(const CUtensorMap* dz, const CUtensorMap* xs, const Readou
   return pair::launch_pair<true, true>(*dz, *xs, shape, epi, num_sms, status, stream);
 }
 
-int launch_scale_by(void* x, long n, const float* g, int num_sms, cudaStream_t stream) {
-  const long n8 = n / 8;
-  const long blocks = std::min((n8 + 255) / 256, static_cast<long>(num_sms) * 8);
+int launch_scale_by(void* x, long nx, void* y, long ny, const float* g, int num_sms, cudaStream_t stream) {
+  const long blocks = std::min(((nx + ny) / 8 + 255) / 256, static_cast<long>(num_sms) * 8);
   if (blocks <= 0) return 0;
-  return launch_pdl(scale_by_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, static_cast<bf16*>(x),
-                    n8, g) == cudaSuccess ? 0 : -1;
+  return launch_pdl(scale_by_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, static_cast<uint4*>(x),
+                    nx / 8, static_cast<uint4*>(y), ny / 8, g) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace ecz

@@ -1,13 +1,12 @@
 """Operators of training steps, with autograd: the readout cross-entropy and causal attention over packed documents.
 
-On CUDA both directions are the hand-written kernels of ``csrc/readout.cu`` and ``csrc/packed_attention.cu``; CPU
-tensors take the formulas of :mod:`.reference` (autograd differentiates them). There is no third path.
+On CUDA both directions are the hand-written kernels of ``csrc/readout.cu``, ``csrc/packed_attention.cu`` and
+``csrc/packed_attention_bwd.cu`` (autograd functions in ``csrc/bindings_train.cpp``); CPU tensors take the formulas of :mod:`.reference` (autograd differentiates them). There is no third path.
 """
 
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import reference
 from ._ext import require
@@ -23,44 +22,6 @@ def _autocast(*tensors: torch.Tensor) -> tuple[torch.Tensor, ...]:
             torch.get_autocast_dtype("cuda") == torch.bfloat16:
         return tuple(t.to(torch.bfloat16) for t in tensors)
     return tensors
-
-
-class _Readout(torch.autograd.Function):
-    """Losses of the readout. A scalar loss computes its gradients in the forward pass, where the unnormalised
-    probabilities are at hand, and the backward pass scales them by the upstream gradient; per-row losses, whose
-    upstream gradients are not known by then, run the products again in the backward pass."""
-
-    @staticmethod
-    def forward(ctx, hidden, weight, targets, ignore_index, logit_scale, reduction, chunk_rows):
-        ctx.need = ctx.needs_input_grad[:2]
-        ctx.args = (ignore_index, logit_scale)
-        ctx.reduction, ctx.chunk_rows = reduction, chunk_rows
-        ctx.save_for_backward(hidden, weight, targets)
-        now = reduction != 0
-        loss, dx, dw = require().readout(hidden, weight, targets, ignore_index, logit_scale, reduction,
-                                         now and ctx.need[0], now and ctx.need[1], None, chunk_rows)
-        ctx.grads = (dx, dw) if now else None
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        need_dx, need_dw = ctx.need
-        grads, ctx.grads = ctx.grads, None
-        hidden, weight, targets = ctx.saved_tensors
-        if grads is None and ctx.reduction == 0:
-            _, dx, dw = require().readout(hidden, weight, targets, *ctx.args, 0, need_dx, need_dw, grad.float(),
-                                          ctx.chunk_rows)
-        else:
-            if grads is None:  # a second pass over a retained graph: the first one gave the buffers away
-                grads = require().readout(hidden, weight, targets, *ctx.args, ctx.reduction, need_dx, need_dw, None,
-                                          ctx.chunk_rows)[1:]
-            dx, dw = grads
-            scale = grad.float()
-            for t in (dx, dw):
-                if t is not None:
-                    require().scale_by(t, scale)
-        return dx, dw, None, None, None, None, None
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *,
@@ -87,34 +48,15 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     if targets.shape != hidden.shape[:-1]:
         raise ValueError(f"targets {tuple(targets.shape)} do not match hidden {tuple(hidden.shape)}")
     hidden, weight = _autocast(hidden, weight)
-    flat = hidden.reshape(-1, hidden.shape[-1])
+    shape = targets.shape
+    if hidden.dim() != 2:
+        hidden, targets = hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1)
     if hidden.is_cuda:
-        args = (flat, weight, targets.reshape(-1), int(ignore_index), float(logit_scale), _REDUCTIONS[reduction])
-        if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-            loss = _Readout.apply(*args, int(chunk_rows))
-        else:
-            loss = require().readout(*args, False, False, None, int(chunk_rows))[0]
+        loss = require().linear_cross_entropy(hidden, weight, targets, ignore_index, logit_scale,
+                                              _REDUCTIONS[reduction], chunk_rows)
     else:
-        loss = reference.linear_cross_entropy(flat, weight, targets.reshape(-1), ignore_index, reduction, logit_scale)
-    return loss.reshape(targets.shape) if reduction == "none" else loss
-
-
-class _PackedAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, cu_seqlens, scale):
-        out, lse = require().packed_forward(q, k, v, cu_seqlens, scale, True)
-        ctx.scale = scale
-        ctx.save_for_backward(q, k, v, out, lse, cu_seqlens)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        q, k, v, out, lse, cu_seqlens = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dq, dk, dv = require().packed_backward(grad, q, k, v, out, lse, cu_seqlens, ctx.scale, need[0],
-                                               need[1] or need[2])
-        return dq, dk, dv, None, None
+        loss = reference.linear_cross_entropy(hidden, weight, targets, ignore_index, reduction, logit_scale)
+    return loss.reshape(shape) if reduction == "none" and len(shape) != 1 else loss
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -137,6 +79,4 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     q, k, v = _autocast(q, k, v)
     if not q.is_cuda:
         return reference.packed_attention(q, k, v, cu_seqlens, scale)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _PackedAttention.apply(q, k, v, cu_seqlens, scale)
-    return require().packed_forward(q, k, v, cu_seqlens, scale, False)[0]
+    return require().packed_attention(q, k, v, cu_seqlens, scale)
