@@ -216,6 +216,7 @@ Tensor packed_plan(const Tensor& q, const Tensor& k, const Tensor& cu, int rows,
   a.Hkv = static_cast<int>(k.size(1));
   a.D = static_cast<int>(q.size(2));
   a.scale = static_cast<float>(scale);
+  a.num_sms = ecz::device_sms(q.get_device());
   a.max_tiles = std::max(1, ecz::packed_max_tiles(T, B, rows));
   Tensor buf = at::empty({int64_t{4} * a.max_tiles + 4 + 2 * (int64_t{B} + 1)}, cu.options());
   int* base = buf.data_ptr<int>();

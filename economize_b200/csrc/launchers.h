@@ -313,7 +313,7 @@ struct PackedMaps {
 struct PackedArgs {
   const void* table = nullptr;  // int4 [max_tiles] of launch_packed_plan
   const int* head = nullptr;    // int [4]
-  int max_tiles = 0, T = 0, H = 0, Hkv = 0, D = 0;
+  int max_tiles = 0, T = 0, H = 0, Hkv = 0, D = 0, num_sms = 0;
   float scale = 1.f;
 };
 // Most tiles of `rows` rows that B sequences of T tokens in all can have.

@@ -11,7 +11,7 @@
 // Forward CTA: two query tiles of 128 rows that share the K / V chunks: the same rows of two heads of a group (an even
 // number of heads per K/V head), else 256 rows of one head. One warp loads (TMA, a ring of 128-key K and V chunks), one
 // issues the MMAs, and two warpgroups run the softmax of a tile each, one thread per row, so the tensor cores work on
-// one tile while the other's exponentials run. S and P share TMEM columns (P overwrites S as bf16 and is the A operand
+// one tile while the other's exponentials run. CTAs are persistent (see Items). S and P share TMEM columns (P overwrites S as bf16 and is the A operand
 // of P . V), O accumulates in TMEM. A row's reference maximum moves only when a chunk raises it by more than 2^8
 // (lazy rescaling), so O is rarely read back before the end.
 //
@@ -30,6 +30,7 @@ using namespace packed;
 namespace {
 
 constexpr float kLazy = 8.f;  // log2 units
+constexpr float kFar = 60.f;
 
 // ---- plan ----------------------------------------------------------------------------------------------------------
 // Tile list of `rows`-row tiles, heaviest first: table[i] = (first token, end, tile, tiles of its sequence). head =
@@ -154,13 +155,17 @@ __global__ void __launch_bounds__(kPlanThreads)
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------
-constexpr int kFwdThreads = 384;
+// Eight softmax warps, one thread per row. Two threads per row (sixteen warps that exchange their maxima) were slower:
+// 973 against 885 us for a document of 16384 tokens, 16 heads over 4.
+constexpr int kSoftmaxWarps = 8;
+constexpr int kFwdThreads = 128 + 32 * kSoftmaxWarps;
 
 template <int DP>
 struct FwdCfg {
   static constexpr int kTileBytes = kRowsT * DP * 2;
-  static constexpr int kRing = DP == 64 ? 10 : 5;  // K and V chunks in turn
-  static constexpr int kSmem = (2 + kRing) * kTileBytes + 1024 + 256;
+  static constexpr int kRing = DP == 64 ? 8 : 4;  // K and V chunks in turn
+  static constexpr int kStage = kSoftmaxWarps * 4096;  // 4 KB for each softmax warp's output rows
+  static constexpr int kSmem = (2 + kRing) * kTileBytes + kStage + 1024 + 512;
   static_assert(kSmem <= 232448, "227 KB of shared memory");
 };
 
@@ -184,25 +189,29 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_tiles = smem;
   uint8_t* ring = smem + 2 * kTileBytes;
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(ring + kRing * kTileBytes);
-  uint64_t* kv_full = q_full + 1;
+  uint8_t* stages = ring + kRing * kTileBytes;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(stages + Cfg::kStage);
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* kv_full = q_empty + 1;
   uint64_t* kv_empty = kv_full + kRing;
   uint64_t* s_full = kv_empty + kRing;   // [2] scores of a tile's chunk are in TMEM
-  uint64_t* p_ready = s_full + 2;        // [2] its probabilities are
-  uint64_t* o_done = p_ready + 2;        // [2] P . V of the chunk is complete
+  uint64_t* p_ready = s_full + 2;        // [2][2] its probabilities are, by halves of the chunk's keys
+  uint64_t* o_done = p_ready + 4;        // [2] P . V of the chunk is complete
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_ready[i], 4);
+      mbar_init(&p_ready[2 * i], 4);
+      mbar_init(&p_ready[2 * i + 1], 4);
       mbar_init(&o_done[i], 1);
     }
     *abort_flag = 0;
@@ -220,60 +229,83 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   pdl_trigger();
   pdl_wait();
 
-  const int per = p.row_pairs ? p.H : p.H / 2;
-  const int entry = blockIdx.x / per, sub = blockIdx.x % per;
   zero_padding(p.out, p.T, static_cast<long>(p.H) * p.D, p.head);
-  if (entry < p.head[0]) {
-    const int4 tile = p.table[entry];
-    const int lo = uniform(tile.x), hi = uniform(tile.y), at = uniform(tile.z);
-    const int group = p.H / p.Hkv;
-    int head[2], row0[2], chunks[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      head[i] = p.row_pairs ? sub : 2 * sub + i;
-      row0[i] = p.row_pairs ? lo + at * 256 + i * 128 : lo + at * 128;
-      chunks[i] = row0[i] < hi ? (row0[i] - lo) / kRowsT + 1 : 0;  // the last one holds the diagonal
-    }
-    const int kvh = head[0] / group;
-    const int n_chunks = max(chunks[0], chunks[1]);
-    const int ksteps = (p.D + 15) / 16;
+  const int group = p.H / p.Hkv;
+  const int ksteps = (p.D + 15) / 16;
+  const int per = p.row_pairs ? p.H : p.H / 2;
+  // an item's query tile i: its head, first row and number of key chunks (the last one holds the diagonal)
+  auto head_of = [&](const auto& items, int i) { return p.row_pairs ? items.sub : 2 * items.sub + i; };
+  auto row_of = [&](const auto& items, int i) {
+    return items.tile.x + (p.row_pairs ? items.tile.z * 256 + i * kRowsT : items.tile.z * kRowsT);
+  };
+  auto chunks_of = [&](const auto& items, int i) {
+    const int row = row_of(items, i);
+    return row < items.tile.y ? (row - items.tile.x) / kRowsT + 1 : 0;
+  };
 
-    if (warp == 0) {
+  if (warp == 0) {
+    // ---- loads: an item's Q, then its K and V chunks in turn ----
+    Items<> items(p.table, p.head, per);
+    const uint32_t qa = smem_u32(q_tiles), ra = smem_u32(ring);
+    int it = 0;
+    bool ok = true;
+    for (int n_items = 0; ok && items.next(); ++n_items) {
+      const int lo = items.tile.x, c1 = chunks_of(items, 1), n = max(chunks_of(items, 0), c1), kvh = head_of(items, 0) / group;
+      const int head0 = head_of(items, 0), head1 = head_of(items, 1), row0 = row_of(items, 0), row1 = row_of(items, 1);
+      items.look();
       if (lane == 0) {
-        // ---- loads: Q, then K and V chunks in turn ----
-        const uint32_t qa = smem_u32(q_tiles), ra = smem_u32(ring);
-        mbar_arrive_expect_tx(q_full, (chunks[1] > 0 ? 2 : 1) * kTileBytes);
-        load_tile<DP>(qa, &tm_q, q_full, head[0], row0[0]);
-        if (chunks[1] > 0) load_tile<DP>(qa + kTileBytes, &tm_q, q_full, head[1], row0[1]);
-        for (int it = 0; it < 2 * n_chunks; ++it) {
-          const int s = it % kRing;
-          if (!mbar_wait(&kv_empty[s], ((it / kRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag)) break;
+        auto chunk = [&](int x) {  // K (even) or V (odd) of a chunk
+          const int s = (it + x) % kRing;
+          if (!mbar_wait(&kv_empty[s], (((it + x) / kRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag)) return false;
           mbar_arrive_expect_tx(&kv_full[s], kTileBytes);
-          load_tile<DP>(ra + s * kTileBytes, (it & 1) ? &tm_v : &tm_k, &kv_full[s], kvh, lo + (it >> 1) * kRowsT);
+          load_tile<DP>(ra + s * kTileBytes, (x & 1) ? &tm_v : &tm_k, &kv_full[s], kvh, lo + (x >> 1) * kRowsT);
+          return true;
+        };
+        // the first chunk does not wait for the previous item's queries to be read
+        ok = chunk(0) && chunk(1) && mbar_wait(q_empty, (n_items & 1) ^ 1, status, kStatusWaitEmpty, abort_flag);
+        if (ok) {
+          mbar_arrive_expect_tx(q_full, (c1 > 0 ? 2 : 1) * kTileBytes);
+          load_tile<DP>(qa, &tm_q, q_full, head0, row0);
+          if (c1 > 0) load_tile<DP>(qa + kTileBytes, &tm_q, q_full, head1, row1);
         }
+        for (int x = 2; ok && x < 2 * n; ++x) ok = chunk(x);
       }
-    } else if (warp == 1) {
-      // ---- MMAs ----
-      const bool leader = elect_one();
-      const uint32_t qa = smem_u32(q_tiles), ra = smem_u32(ring);
-      auto wait_ring = [&](int it) {
-        return warp_wait(&kv_full[it % kRing], (it / kRing) & 1, status, kStatusWaitFull,
-                                                 abort_flag);
-      };
+      it += 2 * n;
+      ok = uniform(ok);
+    }
+  } else if (warp == 1) {
+    // ---- MMAs ----
+    Items<> items(p.table, p.head, per);
+    const bool leader = elect_one();
+    const uint32_t qa = smem_u32(q_tiles), ra = smem_u32(ring);
+    int base = 0;            // ring position of the item's first chunk
+    uint32_t used[2] = {0, 0};  // chunks of tile i so far, over all items
+    bool ok = true;
+    auto wait_ring = [&](int it) {
+      return warp_wait(&kv_full[it % kRing], (it / kRing) & 1, status, kStatusWaitFull, abort_flag);
+    };
+    for (int n_items = 0; ok && items.next(); ++n_items) {
+      const int lo = items.tile.x, hi = items.tile.y;
+      const int chunks[2] = {chunks_of(items, 0), chunks_of(items, 1)};
+      const int n_chunks = max(chunks[0], chunks[1]);
       auto keys_of = [&](int c) { return min(kRowsT, hi - (lo + c * kRowsT)); };
-      bool ok = warp_wait(q_full, 0, status, kStatusWaitFull, abort_flag) && wait_ring(0);
+      ok = warp_wait(q_full, n_items & 1, status, kStatusWaitFull, abort_flag) && wait_ring(base);
+      if (!ok) break;
       tc_fence_after();
-      if (ok && leader) {
+      if (leader) {
         const int n = (keys_of(0) + 15) & ~15;
         for (int i = 0; i < 2; ++i) {
           if (chunks[i] == 0) continue;
-          mma_dims<DP>(tmem + i * 128, qa + i * kTileBytes, ra, n, ksteps);
+          mma_dims<DP>(tmem + i * 128, qa + i * kTileBytes, ra + (base % kRing) * kTileBytes, n, ksteps);
           umma_commit(&s_full[i]);
         }
-        umma_commit(&kv_empty[0]);
+        umma_commit(&kv_empty[base % kRing]);
+        if (n_chunks == 1) umma_commit(q_empty);
       }
+      __syncwarp();
+      items.look();
       for (int c = 0; ok && c < n_chunks; ++c) {
-        const int v_it = 2 * c + 1, k_it = 2 * c + 2;
+        const int v_it = base + 2 * c + 1, k_it = v_it + 1;
         const bool more = c + 1 < n_chunks;
         ok = wait_ring(v_it) && (!more || wait_ring(k_it));
         if (!ok) break;
@@ -282,15 +314,22 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         if (n16 != n) zero_rows<DP>(v_tile, n, n16, lane);
         for (int i = 0; ok && i < 2; ++i) {
           if (c >= chunks[i]) continue;
-          ok = warp_wait(&p_ready[i], c & 1, status, kStatusWaitAccum, abort_flag);
+          // the first half of P . V runs under the exponentials of the second
+          ok = warp_wait(&p_ready[2 * i], (used[i] + c) & 1, status, kStatusWaitAccum, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          if (leader)
+            mma_rows<8, 64, 0, 4>(tmem + 256 + i * DP, tmem + i * 128, smem_u32(v_tile), ksteps * 16, n16 / 16, c > 0);
+          __syncwarp();
+          ok = warp_wait(&p_ready[2 * i + 1], (used[i] + c) & 1, status, kStatusWaitAccum, abort_flag);
           if (!ok) break;
           tc_fence_after();
           if (leader) {
-            mma_rows<8, 64>(tmem + 256 + i * DP, tmem + i * 128, smem_u32(v_tile), ksteps * 16, n16 / 16, c > 0);
+            mma_rows<8, 64, 4, 8>(tmem + 256 + i * DP, tmem + i * 128, smem_u32(v_tile), ksteps * 16, n16 / 16, true);
             umma_commit(&o_done[i]);
             if (c + 1 < chunks[i]) {
               mma_dims<DP>(tmem + i * 128, qa + i * kTileBytes, ra + (k_it % kRing) * kTileBytes,
-                       (keys_of(c + 1) + 15) & ~15, ksteps);
+                           (keys_of(c + 1) + 15) & ~15, ksteps);
               umma_commit(&s_full[i]);
             }
           }
@@ -299,20 +338,32 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         if (leader) {
           umma_commit(&kv_empty[v_it % kRing]);
           if (more) umma_commit(&kv_empty[k_it % kRing]);
+          if (c + 2 == n_chunks) umma_commit(q_empty);  // the last scores are under way
         }
+        __syncwarp();
       }
-    } else if (warp >= 4) {
-      // ---- softmax: one thread per row ----
-      const int i = (warp - 4) >> 2, quad = warp & 3;
-      const int n_mine = i == 0 ? chunks[0] : chunks[1];
-      const int first_row = i == 0 ? row0[0] : row0[1], my_head = i == 0 ? head[0] : head[1];
-      const int row = first_row + quad * 32 + lane;
-      const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-      const uint32_t s_addr = lane_base + i * 128, o_addr = lane_base + 256 + i * DP;
-      float ref = -INFINITY, sum = 0.f;
-      bool ok = true;
+      base += 2 * n_chunks;
+      used[0] += chunks[0];
+      used[1] += chunks[1];
+    }
+  } else if (warp >= 4) {
+    // ---- softmax: one thread per row ----
+    const int i = (warp - 4) >> 2, quad = warp & 3;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t s_addr = lane_base + i * 128, o_addr = lane_base + 256 + i * DP;
+    Items<false> items(p.table, p.head, per);
+    uint32_t used = 0;  // chunks of this tile so far, over all items
+    bool ok = true;
+    while (ok && items.next()) {
+      const int lo = items.tile.x, hi = items.tile.y;
+      const int n_mine = chunks_of(items, i), my_head = head_of(items, i);
+      const int row0 = row_of(items, i) + quad * 32, row = row0 + lane;
+      // Exponentials are taken against a reference that is settled beforehand (0 for a row's first chunk): the chunk's
+      // maximum is reduced beside them, and only where it lies more than kLazy above (or far below, in the first chunk,
+      // where small sums would underflow) does the row take it as its reference and repeat.
+      float ref = 0.f, sum = 0.f;
       for (int c = 0; c < n_mine; ++c) {
-        ok = warp_wait(&s_full[i], c & 1, status, kStatusWaitAccum, abort_flag);
+        ok = warp_wait(&s_full[i], (used + c) & 1, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
         float v[128];
@@ -320,83 +371,95 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         if (c == n_mine - 1) {  // the diagonal and the sequence's end
           const int limit = min(hi, row + 1) - (lo + c * kRowsT);
 #pragma unroll
-          for (int j = 0; j < 128; ++j) v[j] = j < limit ? v[j] : -INFINITY;
-        }
-        float m0 = v[0], m1 = v[1], m2 = v[2], m3 = v[3];
+          for (int h = 0; h < 4; ++h) {
+            const uint32_t bits = low_bits(limit - h * 32);
 #pragma unroll
-        for (int j = 4; j < 128; j += 4) {
-          m0 = fmaxf(m0, v[j]);
-          m1 = fmaxf(m1, v[j + 1]);
-          m2 = fmaxf(m2, v[j + 2]);
-          m3 = fmaxf(m3, v[j + 3]);
-        }
-        const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * p.scale2;
-        const bool raise = top > ref + kLazy;  // also the first finite maximum (ref = -inf)
-        const float new_ref = raise ? top : ref;
-        if (c > 0 && __any_sync(0xffffffffu, raise && sum != 0.f)) {
-          const float f = raise ? ex2(ref - new_ref) : 1.f;
-          ok = warp_wait(&o_done[i], (c - 1) & 1, status, kStatusWaitAccum, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          sum *= f;
-#pragma unroll 1
-          for (int d = 0; d < DP; d += 16) {
-            float o[16];
-            tmem_ld16(o_addr + d, o);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] *= f;
-            tmem_st16(o_addr + d, o);
+            for (int j = 0; j < 32; ++j) v[h * 32 + j] = (bits >> j) & 1u ? v[h * 32 + j] : -INFINITY;
           }
         }
-        ref = new_ref;
-        const float shift = ref == -INFINITY ? 0.f : ref;
-        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-        uint32_t w[32];
+        uint64_t part[2];  // sums of exponentials, by halves
+        // 64 probabilities to TMEM, their sum to part[h]
+        auto exponentials = [&](int h) {
+          const float shift = ref == -INFINITY ? 0.f : ref;
+          const uint64_t scale2 = pair_of(p.scale2, p.scale2), minus = pair_of(-shift, -shift);
+          uint64_t a = 0, b = 0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+          for (int q = 0; q < 2; ++q) {
+            uint32_t w[16];
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float a = ex2(fmaf(v[h * 64 + 2 * j], p.scale2, -shift));
-            const float b = ex2(fmaf(v[h * 64 + 2 * j + 1], p.scale2, -shift));
-            const float x = ex2(fmaf(v[h * 64 + 2 * j + 2], p.scale2, -shift));
-            const float y = ex2(fmaf(v[h * 64 + 2 * j + 3], p.scale2, -shift));
-            s0 += a;
-            s1 += b;
-            s2 += x;
-            s3 += y;
-            w[j] = pack_bf16(a, b);
-            w[j + 1] = pack_bf16(x, y);
+            for (int j = 0; j < 16; j += 2) {
+              const float* x = v + h * 64 + q * 32 + 2 * j;
+              float x0, x1, y0, y1;
+              unpair(fma2(pair_of(x[0], x[1]), scale2, minus), x0, x1);
+              unpair(fma2(pair_of(x[2], x[3]), scale2, minus), y0, y1);
+              x0 = ex2(x0);
+              x1 = ex2(x1);
+              y0 = ex2(y0);
+              y1 = ex2(y1);
+              a = add2(a, pair_of(x0, x1));
+              b = add2(b, pair_of(y0, y1));
+              w[j] = pack_bf16(x0, x1);
+              w[j + 1] = pack_bf16(y0, y1);
+            }
+            tmem_st_u32x16(s_addr + h * 32 + q * 16, w);
           }
-          tmem_store32(s_addr + h * 32, w);
-        }
-        sum += (s0 + s1) + (s2 + s3);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[i]);
-      }
-      if (n_mine > 0 && ok) {
-        ok = warp_wait(&o_done[i], (n_mine - 1) & 1, status, kStatusWaitAccum, abort_flag);
-        if (ok) {
-          tc_fence_after();
-          const float inv = 1.f / sum;
-          const bool real = row < hi;
-          bf16* dst = p.out + (static_cast<long>(row) * p.H + my_head) * p.D;
-#pragma unroll 1
-          for (int d = 0; d < DP; d += 32) {
-            float o[32];
-            tmem_load32(o_addr + d, o);
-            if (real) {
+          part[h] = add2(a, b);
+        };
+        auto publish = [&](int h) {
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_ready[2 * i + h]);
+        };
+        float m0 = max3(v[0], v[1], v[2]), m1 = max3(v[3], v[4], v[5]);
 #pragma unroll
-              for (int j = 0; j < 32; j += 8)
-                if (d + j < p.D)
-                  *reinterpret_cast<uint4*>(dst + d + j) =
-                      make_uint4(pack_bf16(o[j] * inv, o[j + 1] * inv), pack_bf16(o[j + 2] * inv, o[j + 3] * inv),
-                                 pack_bf16(o[j + 4] * inv, o[j + 5] * inv), pack_bf16(o[j + 6] * inv, o[j + 7] * inv));
+        for (int j = 6; j < 126; j += 4) {
+          m0 = max3(m0, v[j], v[j + 1]);
+          m1 = max3(m1, v[j + 2], v[j + 3]);
+        }
+        const float top = max3(fmaxf(m0, m1), v[126], v[127]) * p.scale2;
+        exponentials(0);
+        const bool move = top > ref + kLazy || (c == 0 && top < -kFar);
+        if (__any_sync(0xffffffffu, move)) {
+          const float f = move ? ex2(ref - top) : 1.f;
+          if (move) ref = top;
+          if (c > 0) {
+            ok = warp_wait(&o_done[i], (used + c - 1) & 1, status, kStatusWaitAccum, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            sum *= f;
+#pragma unroll 1
+            for (int d = 0; d < DP; d += 16) {
+              float o[16];
+              tmem_ld16(o_addr + d, o);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] *= f;
+              tmem_st16(o_addr + d, o);
             }
           }
-          if (real && p.lse != nullptr) p.lse[static_cast<long>(my_head) * p.T + row] = ref + log2f(sum);
+          exponentials(0);
         }
+        publish(0);
+        exponentials(1);
+        publish(1);
+        float a, b;
+        unpair(add2(part[0], part[1]), a, b);
+        sum += a + b;
+      }
+      if (!ok) break;
+      if (n_mine > 0) {
+        used += n_mine;
+        ok = warp_wait(&o_done[i], (used - 1) & 1, status, kStatusWaitAccum, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const float inv = 1.f / sum;
+        if (row < hi && p.lse != nullptr) p.lse[static_cast<long>(my_head) * p.T + row] = ref + log2f(sum);
+        const long stride = static_cast<long>(p.H) * p.D;
+        bf16* dst = p.out + row0 * stride + static_cast<long>(my_head) * p.D;
+#pragma unroll 1
+        for (int d = 0; d < p.D; d += 64)
+          stage_tmem64(o_addr + d, inv, stages + (warp - 4) * 4096, dst + d, stride, hi - row0, p.D - d, lane);
+        tc_fence_before();  // the next item's first P . V overwrites O after this warp's next p_ready
       }
     }
   }
@@ -414,8 +477,9 @@ int run_fwd(const PackedMaps& maps, const PackedArgs& a, void* out, float* lse, 
   if (set_max_smem(kernel, FwdCfg<DP>::kSmem) != cudaSuccess) return -1;
   const FwdArgs args{static_cast<bf16*>(out), lse, static_cast<const int4*>(a.table), a.head, a.T, a.H, a.Hkv, a.D,
                      a.scale * kLog2e, row_pairs};
-  const long grid = static_cast<long>(a.max_tiles) * (row_pairs ? a.H : a.H / 2);
-  if (grid > 0x7fffffffl) return -2;
+  const long most = static_cast<long>(a.max_tiles) * (row_pairs ? a.H : a.H / 2);
+  if (most > 0x7fff0000l) return -2;
+  const long grid = std::min(most, static_cast<long>(a.num_sms));
   return launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(kFwdThreads), FwdCfg<DP>::kSmem, stream, maps.q,
                     maps.k, maps.v, args, status) == cudaSuccess ? 0 : -1;
 }

@@ -22,6 +22,41 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
+// Two fp32 values in a 64-bit register and the operations on both at once, and the maximum of three.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// The low n bits (0 <= n <= 32 after clamping).
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+}
+
 // 3-D tiled load: box {64 (d), 1 (head), 128 (tokens)} at (d, head, token). d is a multiple of 64.
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int d, int head,
                                             int token) {
@@ -82,13 +117,13 @@ __device__ __forceinline__ void mma_dims(uint32_t d, uint32_t a, uint32_t b, int
 }
 
 // D[128, n] (+)= P[128, :16 ksteps] . B[:16 ksteps, n], P packed bf16 in TMEM (kPer K steps of 8 columns side by side in
-// every group of kStride columns), B's rows along K (MN-major).
-template <int kPer, int kStride>
+// every group of kStride columns), B's rows along K (MN-major); K steps [kFrom, kTo) of them.
+template <int kPer, int kStride, int kFrom = 0, int kTo = 8>
 __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t p, uint32_t b, int n, int ksteps, bool accumulate) {
   const uint32_t idesc = idesc_bf16_f32(128, n, true);
   const uint64_t db = desc_mnmajor_sw128(b, kRowsT * 128);
 #pragma unroll
-  for (int kk = 0; kk < 8; ++kk) {
+  for (int kk = kFrom; kk < kTo; ++kk) {
     const uint32_t pc = p + (kk / kPer) * kStride + (kk % kPer) * 8;
     if (kk < ksteps) umma_bf16_ta(d, pc, desc_step(db, kk * 16 * 128), idesc, kk != 0 ? 1u : (accumulate ? 1u : 0u));
   }
@@ -104,6 +139,127 @@ __device__ __forceinline__ void zero_padding(bf16* x, int T, long width, const i
     if (row >= first) row += last - first;
     *reinterpret_cast<uint4*>(x + row * width + (i % (width / 8)) * 8) = make_uint4(0, 0, 0, 0);
   }
+}
+
+// The work of a persistent CTA: items (table entry, sub) with sub < per varying fastest, heaviest first, dealt to the
+// grid in alternating direction so that no CTA always gets a round's heaviest. Persistent because an item of a short
+// sequence is one or two tiles: with a CTA for each, set-up, first loads and last stores took two thirds of the time.
+// A role calls next() to take an item and look() while it would wait anyway: look() finds the following item and starts
+// the load of its table entry (a division and an L2 access, off the path between two items).
+// kAhead false: next() does both (for roles short of registers, whose wait for the item's first scores covers it).
+template <bool kAhead = true>
+struct Items {
+  const int4* table;
+  const int* head;  // (entries, ...)
+  int per, round;
+  int4 ahead;
+  int ahead_sub;
+  bool more;  // there is a following item
+  int4 tile;  // of the item taken: (first token, end, tile, tiles of its sequence)
+  int sub;
+
+  __device__ __forceinline__ Items(const int4* t, const int* h, int per_entry)
+      : table(t), head(h), per(per_entry), round(0) {
+    if (kAhead) look();
+  }
+  __device__ __forceinline__ void look() {
+    const int g = gridDim.x, c = blockIdx.x;
+    const int index = round * g + ((round & 1) ? g - 1 - c : c);
+    ++round;
+    more = index < head[0] * per;
+    if (!more) return;
+    const int entry = index / per;
+    ahead = table[entry];
+    ahead_sub = index - entry * per;
+  }
+  __device__ __forceinline__ bool next() {
+    if (!kAhead) look();
+    if (!more) return false;
+    tile = make_int4(uniform(ahead.x), uniform(ahead.y), uniform(ahead.z), uniform(ahead.w));
+    sub = ahead_sub;
+    return true;
+  }
+};
+
+// Stores 64 columns of a warp's 32 rows: lane r holds row r's as eight 16-byte groups c[0..7]. An 8 x 8 transpose over
+// groups of eight lanes (three exchanges) first, so that eight lanes write a row's 128 bytes at once: rows written by
+// their own lanes touch 32 lines per store and took 3900 cycles for a 128 x 128 tile. Row r goes to dst + r stride for
+// r < rows, columns below `cols`.
+__device__ __forceinline__ void store_rows64(uint4 (&c)[8], bf16* dst, long stride, int rows, int cols, int lane) {
+#pragma unroll
+  for (int m = 4; m > 0; m >>= 1) {
+    const bool up = (lane & m) != 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i & m) continue;
+      uint4 out = up ? c[i] : c[i | m];
+      out.x = __shfl_xor_sync(0xffffffffu, out.x, m);
+      out.y = __shfl_xor_sync(0xffffffffu, out.y, m);
+      out.z = __shfl_xor_sync(0xffffffffu, out.z, m);
+      out.w = __shfl_xor_sync(0xffffffffu, out.w, m);
+      if (up) c[i] = out;
+      else c[i | m] = out;
+    }
+  }
+  const int col = (lane & 7) * 8;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int row = (lane & 24) + j;
+    if (row < rows && col < cols) *reinterpret_cast<uint4*>(dst + row * stride + col) = c[j];
+  }
+}
+
+// 64 fp32 columns of the warp's TMEM lanes, times each lane's f, as bf16 rows through 4 KB of shared memory of the warp
+// (16-byte groups swizzled by the row, so that neither side conflicts); arguments as store_rows64.
+__device__ __forceinline__ void stage_tmem64(uint32_t taddr, float f, uint8_t* stage, bf16* dst, long stride, int rows,
+                                             int cols, int lane) {
+  const uint64_t ff = pair_of(f, f);
+  uint8_t* mine = stage + lane * 128;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float o[32];
+    tmem_load32(taddr + h * 32, o);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float a, b;
+        unpair(mul2(pair_of(o[8 * j + 2 * k], o[8 * j + 2 * k + 1]), ff), a, b);
+        w[k] = pack_bf16(a, b);
+      }
+      *reinterpret_cast<uint4*>(mine + (((h * 4 + j) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  __syncwarp();
+  const int g = lane & 7;
+  if (g * 8 < cols) {
+    bf16* at = dst + (lane >> 3) * stride + g * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i, at += 4 * stride) {
+      const int row = i * 4 + (lane >> 3);
+      if (row < rows)
+        *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(stage + row * 128 + ((g ^ (row & 7)) << 4));
+    }
+  }
+  __syncwarp();
+}
+
+// 64 columns of the warp's TMEM lanes, times each lane's f, as bf16 rows through registers (store_rows64).
+__device__ __forceinline__ void store_tmem64(uint32_t taddr, float f, bf16* dst, long stride, int rows, int cols,
+                                             int lane) {
+  uint4 c[8];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float o[32];
+    tmem_load32(taddr + h * 32, o);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      c[h * 4 + j] = make_uint4(pack_bf16(o[8 * j] * f, o[8 * j + 1] * f), pack_bf16(o[8 * j + 2] * f, o[8 * j + 3] * f),
+                                pack_bf16(o[8 * j + 4] * f, o[8 * j + 5] * f),
+                                pack_bf16(o[8 * j + 6] * f, o[8 * j + 7] * f));
+  }
+  store_rows64(c, dst, stride, rows, cols, lane);
 }
 
 // The end of a CTA whose waits may have given up: copies in flight land before the shared memory goes.
