@@ -67,24 +67,6 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restric
   if (real && c == 0) delta[static_cast<long>(h) * T + t] = acc;
 }
 
-// `kCols` fp32 columns of a thread's TMEM row, times f, as bf16 at dst (those of the `left` that are).
-template <int kCols>
-__device__ __forceinline__ void store_row(uint32_t taddr, float f, bf16* dst, int left, bool real) {
-#pragma unroll 1
-  for (int d = 0; d < kCols; d += 16) {
-    float o[16];
-    tmem_ld16(taddr + d, o);
-    if (real) {
-#pragma unroll
-      for (int j = 0; j < 16; j += 8)
-        if (d + j < left)
-          *reinterpret_cast<uint4*>(dst + d + j) =
-              make_uint4(pack_bf16(o[j] * f, o[j + 1] * f), pack_bf16(o[j + 2] * f, o[j + 3] * f),
-                         pack_bf16(o[j + 4] * f, o[j + 5] * f), pack_bf16(o[j + 6] * f, o[j + 7] * f));
-    }
-  }
-}
-
 template <int DP>
 struct BwdCfg {
   static constexpr int kTileBytes = kRowsT * DP * 2;
@@ -146,7 +128,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   uint64_t* dp_full = p_ready + 1;
   uint64_t* ds_ready = dp_full + 1;
   uint64_t* done = ds_ready + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* kv_empty = done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -156,6 +139,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   }
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
+    mbar_init(kv_empty, 1);
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&ring.full[i], 1);
       mbar_init(&ring.empty[i], 1);
@@ -184,34 +168,48 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
   zero_padding(p.dk, p.T, static_cast<long>(p.Hkv) * p.D, p.head);
   zero_padding(p.dv, p.T, static_cast<long>(p.Hkv) * p.D, p.head);
-  const int entry = blockIdx.x / p.Hkv, kvh = blockIdx.x % p.Hkv;
-  if (entry < p.head[0]) {
-    const int4 tile = p.table[entry];
-    const int lo = uniform(tile.x), hi = uniform(tile.y);
-    const int n_q = uniform(tile.z) + 1;
-    const int first = uniform(tile.w) - n_q;  // the tile of keys: as many query tiles follow as the entry weighs
-    const int group = p.H / p.Hkv;
-    const int total = group * n_q;
-    const int key0 = lo + first * kRowsT;
-    const int ksteps = (p.D + 15) / 16;
+  Items<> items(p.table, p.head, p.Hkv);  // sub: the K/V head
+  const int group = p.H / p.Hkv;
+  const int ksteps = (p.D + 15) / 16;
+  // an item's query tiles (as many as the entry weighs, from the tile of keys on) and its first token
+  auto tiles_of = [&]() { return items.tile.z + 1; };
+  auto key0_of = [&]() { return items.tile.x + (items.tile.w - items.tile.z - 1) * kRowsT; };
 
-    if (warp == 0) {
+  if (warp == 0) {
+    int x = 0;  // ring item
+    bool ok = true;
+    for (int n_items = 0; ok && items.next(); ++n_items) {
+      const int n_q = tiles_of(), key0 = key0_of(), kvh = items.sub, total = group * n_q;
+      items.look();
       if (lane == 0) {
-        mbar_arrive_expect_tx(kv_full, 2 * kTileBytes);
-        load_tile<DP>(smem_u32(k_tile), &tm_k, kv_full, kvh, key0);
-        load_tile<DP>(smem_u32(v_tile), &tm_v, kv_full, kvh, key0);
         Walk at(kvh * group, key0, n_q);
-        for (int x = 0; x < 2 * total; ++x) {  // Q, dO of every iteration in turn
-          if (!mbar_wait(ring.empty_of(x), ring.use(x) ^ 1, status, kStatusWaitEmpty, abort_flag)) break;
-          mbar_arrive_expect_tx(ring.full_of(x), kTileBytes);
-          load_tile<DP>(smem_u32(ring.tile(x)), (x & 1) ? &tm_do : &tm_q, ring.full_of(x), at.head, at.row);
-          if (x & 1) at.next();
+        auto load = [&](int i) {  // Q (even) or dO (odd) of an iteration
+          if (!mbar_wait(ring.empty_of(x + i), ring.use(x + i) ^ 1, status, kStatusWaitEmpty, abort_flag)) return false;
+          mbar_arrive_expect_tx(ring.full_of(x + i), kTileBytes);
+          load_tile<DP>(smem_u32(ring.tile(x + i)), (i & 1) ? &tm_do : &tm_q, ring.full_of(x + i), at.head, at.row);
+          if (i & 1) at.next();
+          return true;
+        };
+        // the first query tile does not wait for the previous item's keys to be read
+        ok = load(0) && load(1) && mbar_wait(kv_empty, (n_items & 1) ^ 1, status, kStatusWaitEmpty, abort_flag);
+        if (ok) {
+          mbar_arrive_expect_tx(kv_full, 2 * kTileBytes);
+          load_tile<DP>(smem_u32(k_tile), &tm_k, kv_full, kvh, key0);
+          load_tile<DP>(smem_u32(v_tile), &tm_v, kv_full, kvh, key0);
         }
+        for (int i = 2; ok && i < 2 * total; ++i) ok = load(i);
       }
-    } else if (warp == 1) {
-      const bool leader = elect_one();
-      const uint32_t ka = smem_u32(k_tile), va = smem_u32(v_tile);
-      // item x, of the query tile at `row`, is in shared memory and its rows past the sequence's end are zeroed
+      x += 2 * total;
+      ok = uniform(ok);
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    const uint32_t ka = smem_u32(k_tile), va = smem_u32(v_tile);
+    int base = 0;  // iterations before the item
+    bool ok = true;
+    for (int n_items = 0; ok && items.next(); ++n_items) {
+      const int hi = items.tile.y, n_q = tiles_of(), key0 = key0_of(), kvh = items.sub, total = group * n_q;
+      // ring item x, of the query tile at `row`, is in shared memory and its rows past the sequence's end are zeroed
       auto ready = [&](int x, int row) {
         if (!warp_wait(ring.full_of(x), ring.use(x), status, kStatusWaitFull, abort_flag)) return false;
         const int n = min(kRowsT, hi - row), n16 = (n + 15) & ~15;
@@ -220,17 +218,20 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       };
       Walk at(kvh * group, key0, n_q);
       int rows16 = (min(kRowsT, hi - at.row) + 15) & ~15;  // of the current iteration's query tile
-      bool ok = warp_wait(kv_full, 0, status, kStatusWaitFull, abort_flag) && ready(0, at.row) && ready(1, at.row);
+      ok = ready(2 * base, at.row) && ready(2 * base + 1, at.row) &&
+           warp_wait(kv_full, n_items & 1, status, kStatusWaitFull, abort_flag);
       tc_fence_after();
       if (ok && leader) {
-        mma_dims<DP>(t_s, ka, smem_u32(ring.tile(0)), rows16, ksteps);
+        mma_dims<DP>(t_s, ka, smem_u32(ring.tile(2 * base)), rows16, ksteps);
         umma_commit(s_full);
-        mma_dims<DP>(t_dp, va, smem_u32(ring.tile(1)), rows16, ksteps);
+        mma_dims<DP>(t_dp, va, smem_u32(ring.tile(2 * base + 1)), rows16, ksteps);
         umma_commit(dp_full);
+        if (total == 1) umma_commit(kv_empty);
       }
       __syncwarp();
-      for (int it = 0; ok && it < total; ++it) {
-        const bool more = it + 1 < total;
+      items.look();
+      for (int it = base; ok && it < base + total; ++it) {
+        const bool more = it + 1 < base + total;
         const int xq = 2 * it, xd = xq + 1;
         at.next();
         const int next16 = (min(kRowsT, hi - at.row) + 15) & ~15;
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!ok) break;
         tc_fence_after();
         if (leader) {
-          mma_rows<2, 32>(t_dv, t_s, smem_u32(ring.tile(xd)), ksteps * 16, rows16 / 16, it > 0);
+          mma_rows<2, 32>(t_dv, t_s, smem_u32(ring.tile(xd)), ksteps * 16, rows16 / 16, it > base);
           umma_commit(ring.empty_of(xd));
           if (more) {
             mma_dims<DP>(t_s, ka, smem_u32(ring.tile(xq + 2)), next16, ksteps);
@@ -252,43 +253,59 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!ok) break;
         tc_fence_after();
         if (leader) {
-          mma_rows<2, 32>(t_dk, t_dp, smem_u32(ring.tile(xq)), ksteps * 16, rows16 / 16, it > 0);
+          mma_rows<2, 32>(t_dk, t_dp, smem_u32(ring.tile(xq)), ksteps * 16, rows16 / 16, it > base);
           umma_commit(ring.empty_of(xq));
           if (more) {
             mma_dims<DP>(t_dp, va, smem_u32(ring.tile(xd + 2)), next16, ksteps);
             umma_commit(dp_full);
+            if (it + 2 == base + total) umma_commit(kv_empty);  // the last use of K and V is under way
+          } else {
+            umma_commit(done);
           }
         }
         __syncwarp();
         rows16 = next16;
       }
-      if (ok && leader) umma_commit(done);
-    } else if (warp == 2) {
-      // ---- lse and delta of the query tiles ----
-      Walk at(kvh * group, key0, n_q);
-      for (int it = 0; it < total; ++it, at.next()) {
+      base += total;
+    }
+  } else if (warp == 2) {
+    // ---- lse and delta of the query tiles ----
+    int base = 0;
+    bool ok = true;
+    while (ok && items.next()) {
+      const int hi = items.tile.y, n_q = tiles_of(), total = group * n_q;
+      Walk at(items.sub * group, key0_of(), n_q);
+      items.look();
+      for (int it = base; it < base + total; ++it, at.next()) {
         const int s = it % kStatRing;
-        if (!warp_wait(&st_empty[s], ((it / kStatRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag)) break;
-        const long base = static_cast<long>(at.head) * p.T;
+        ok = warp_wait(&st_empty[s], ((it / kStatRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag);
+        if (!ok) break;
+        const long first = static_cast<long>(at.head) * p.T;
         float* dst = stats + s * 256;
 #pragma unroll
         for (int j = lane; j < kRowsT; j += 32) {
           const int row = at.row + j;
-          dst[j] = row < hi ? p.lse[base + row] : 0.f;
-          dst[128 + j] = row < hi ? p.delta[base + row] : 0.f;
+          dst[j] = row < hi ? p.lse[first + row] : 0.f;
+          dst[128 + j] = row < hi ? p.delta[first + row] : 0.f;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&st_full[s]);
       }
-    } else if (warp >= 4) {
-      // ---- P^T and dS^T: one thread per key and quarter of the queries ----
-      const int part = (warp - 4) >> 2, quad = warp & 3;
-      const int key = quad * 32 + lane;  // relative to key0
-      const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
-      const uint32_t s_addr = t_s + lane_base + part * 32, dp_addr = t_dp + lane_base + part * 32;
-      bool ok = true;
+      base += total;
+    }
+  } else if (warp >= 4) {
+    // ---- P^T and dS^T: one thread per key and quarter of the queries ----
+    const int part = (warp - 4) >> 2, quad = warp & 3;
+    const int key = quad * 32 + lane;  // relative to key0
+    const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t s_addr = t_s + lane_base + part * 32, dp_addr = t_dp + lane_base + part * 32;
+    int base = 0;
+    bool ok = true;
+    for (int n_items = 0; ok && items.next(); ++n_items) {
+      const int hi = items.tile.y, n_q = tiles_of(), key0 = key0_of(), kvh = items.sub, total = group * n_q;
+      items.look();
       Walk at(kvh * group, key0, n_q);
-      for (int it = 0; it < total; ++it, at.next()) {
+      for (int it = base; it < base + total; ++it, at.next()) {
         const int s = it % kStatRing;
         const float* lse = stats + s * 256 + part * 32;
         const float* delta = lse + 128;
@@ -302,6 +319,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const bool diagonal = at.row == key0;
         const int from = diagonal ? key - part * 32 : 0, to = hi - at.row - part * 32;
         const bool masked = diagonal || to < 32;
+        const uint32_t seen = low_bits(to) & ~low_bits(from);
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
           const float4 l = *reinterpret_cast<const float4*>(lse + j);
@@ -312,7 +330,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         if (masked) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = (j >= from && j < to) ? v[j] : 0.f;
+          for (int j = 0; j < 32; ++j) v[j] = (seen >> j) & 1u ? v[j] : 0.f;
         }
         uint32_t w[16];
 #pragma unroll
@@ -337,7 +355,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         if (masked) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) g[j] = (j >= from && j < to) ? g[j] : 0.f;
+          for (int j = 0; j < 32; ++j) g[j] = (seen >> j) & 1u ? g[j] : 0.f;
         }
 #pragma unroll
         for (int j = 0; j < 16; ++j) w[j] = pack_bf16(g[2 * j], g[2 * j + 1]);
@@ -350,14 +368,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           mbar_arrive(&st_empty[s]);
         }
       }
-      if (ok && warp_wait(done, 0, status, kStatusWaitAccum, abort_flag)) {
-        tc_fence_after();
-        const int row = key0 + key, col = (part & 1) * (DP / 2);
-        const bool real = row < hi;
-        const long at = (static_cast<long>(row) * p.Hkv + kvh) * p.D + col;
-        if (part < 2) store_row<DP / 2>(t_dv + lane_base + col, 1.f, p.dv + at, p.D - col, real);
-        else store_row<DP / 2>(t_dk + lane_base + col, p.scale, p.dk + at, p.D - col, real);
+      base += total;
+      ok = ok && warp_wait(done, n_items & 1, status, kStatusWaitAccum, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      const int col = (part & 1) * 64, row0 = key0 + quad * 32;
+      if (col < p.D) {
+        const long stride = static_cast<long>(p.Hkv) * p.D, at0 = row0 * stride + static_cast<long>(kvh) * p.D + col;
+        const bool values = part < 2;
+        store_tmem64((values ? t_dv : t_dk) + lane_base + col, values ? 1.f : p.scale, (values ? p.dv : p.dk) + at0,
+                     stride, hi - row0, p.D - col, lane);
       }
+      tc_fence_before();  // the next item's first dV overwrites this one's after this warp's next p_ready
     }
   }
   __syncwarp();
@@ -368,6 +390,38 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 }
 
 // ---- dQ --------------------------------------------------------------------------------------------------------------
+// The chunks of a persistent CTA's items in one sequence: `chunk` of the item's `n`, counted over all items by `k`. The
+// issuing warp runs three of them (scores, dP and dQ are issued two, one and no chunks ahead, across items), a compute
+// group steps by two.
+struct ChunkWalk {
+  Items<> items;
+  int chunk, n, k, item;
+  bool valid;
+  __device__ __forceinline__ ChunkWalk(const int4* table, const int* head, int per) : items(table, head, per), k(0), item(-1) {
+    take();
+  }
+  __device__ __forceinline__ void take() {
+    valid = items.next();
+    chunk = 0;
+    ++item;
+    if (!valid) return;
+    n = items.tile.z + 1;  // key chunks, the last one on the diagonal
+    items.look();
+  }
+  __device__ __forceinline__ void step() {
+    ++k;
+    if (++chunk == n) take();
+  }
+  __device__ __forceinline__ bool first() const { return chunk == 0; }
+  __device__ __forceinline__ bool last() const { return chunk + 1 == n; }
+  __device__ __forceinline__ int lo() const { return items.tile.x; }
+  __device__ __forceinline__ int hi() const { return items.tile.y; }
+  __device__ __forceinline__ int row0() const { return items.tile.x + (n - 1) * kRowsT; }
+  __device__ __forceinline__ int head() const { return items.sub; }
+  __device__ __forceinline__ int keys() const { return min(kRowsT, hi() - (lo() + chunk * kRowsT)); }
+  __device__ __forceinline__ int keys16() const { return (keys() + 15) & ~15; }
+};
+
 template <int DP>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -383,8 +437,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   uint64_t* dp_full = s_full + 2;             // [2], by chunk parity: each is waited for by one group
   uint64_t* dp_free = dp_full + 2;
   uint64_t* ds_ready = dp_free + 2;
-  uint64_t* done = ds_ready + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  // [2], by item parity: an item's dQ is complete. One barrier would not do: a group that is through with the next item's
+  // only chunk before this item's last dQ would take the phase before this one for its own.
+  uint64_t* dq_full = ds_ready + 2;
+  uint64_t* dq_free = dq_full + 2;   // dQ is in registers
+  uint64_t* q_empty = dq_free + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_empty + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -404,7 +462,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&dp_free[i], kComputeWarps / 2);
       mbar_init(&ds_ready[i], kComputeWarps / 2);
     }
-    mbar_init(done, 1);
+    mbar_init(&dq_full[0], 1);
+    mbar_init(&dq_full[1], 1);
+    mbar_init(dq_free, kComputeWarps / 2);
+    mbar_init(q_empty, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -419,137 +480,166 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   pdl_wait();
 
   zero_padding(p.dq, p.T, static_cast<long>(p.H) * p.D, p.head);
-  const int entry = blockIdx.x / p.H, head = blockIdx.x % p.H;
-  if (entry < p.head[0]) {
-    const int4 tile = p.table[entry];
-    const int lo = uniform(tile.x), hi = uniform(tile.y);
-    const int n = uniform(tile.z) + 1;  // key chunks, the last one on the diagonal
-    const int row0 = lo + (n - 1) * kRowsT;
-    const int kvh = head / (p.H / p.Hkv);
-    const int ksteps = (p.D + 15) / 16;
+  const int group = p.H / p.Hkv;
+  const int ksteps = (p.D + 15) / 16;
 
-    if (warp == 0) {
+  if (warp == 0) {
+    Items<> items(p.table, p.head, p.H);
+    int x = 0;  // ring item
+    bool ok = true;
+    for (int n_items = 0; ok && items.next(); ++n_items) {
+      const int lo = items.tile.x, n = items.tile.z + 1, head = items.sub, kvh = head / group;
+      items.look();
       if (lane == 0) {
-        mbar_arrive_expect_tx(q_full, 2 * kTileBytes);
-        load_tile<DP>(smem_u32(q_tile), &tm_q, q_full, head, row0);
-        load_tile<DP>(smem_u32(do_tile), &tm_do, q_full, head, row0);
-        for (int x = 0; x < 2 * n; ++x) {  // K, V of every chunk in turn
-          if (!mbar_wait(ring.empty_of(x), ring.use(x) ^ 1, status, kStatusWaitEmpty, abort_flag)) break;
-          mbar_arrive_expect_tx(ring.full_of(x), kTileBytes);
-          load_tile<DP>(smem_u32(ring.tile(x)), (x & 1) ? &tm_v : &tm_k, ring.full_of(x), kvh,
-                        lo + (x >> 1) * kRowsT);
+        auto load = [&](int i) {  // K (even) or V (odd) of a chunk
+          if (!mbar_wait(ring.empty_of(x + i), ring.use(x + i) ^ 1, status, kStatusWaitEmpty, abort_flag)) return false;
+          mbar_arrive_expect_tx(ring.full_of(x + i), kTileBytes);
+          load_tile<DP>(smem_u32(ring.tile(x + i)), (i & 1) ? &tm_v : &tm_k, ring.full_of(x + i), kvh,
+                        lo + (i >> 1) * kRowsT);
+          return true;
+        };
+        // the first chunk does not wait for the previous item's queries to be read
+        ok = load(0) && load(1) && mbar_wait(q_empty, (n_items & 1) ^ 1, status, kStatusWaitEmpty, abort_flag);
+        if (ok) {
+          mbar_arrive_expect_tx(q_full, 2 * kTileBytes);
+          load_tile<DP>(smem_u32(q_tile), &tm_q, q_full, head, lo + (n - 1) * kRowsT);
+          load_tile<DP>(smem_u32(do_tile), &tm_do, q_full, head, lo + (n - 1) * kRowsT);
         }
+        for (int i = 2; ok && i < 2 * n; ++i) ok = load(i);
       }
-    } else if (warp == 1) {
-      const bool leader = elect_one();
-      const uint32_t qa = smem_u32(q_tile), da = smem_u32(do_tile);
-      auto keys16 = [&](int c) { return (min(kRowsT, hi - (lo + c * kRowsT)) + 15) & ~15; };
-      auto scores = [&](int c) {  // S of chunk c into its buffer; K rows past the end zeroed
-        if (!warp_wait(ring.full_of(2 * c), ring.use(2 * c), status, kStatusWaitFull, abort_flag)) return false;
-        const int keys = min(kRowsT, hi - (lo + c * kRowsT));
-        if (keys != keys16(c)) zero_rows<DP>(ring.tile(2 * c), keys, keys16(c), lane);
-        tc_fence_after();
-        if (leader) {
-          mma_dims<DP>(t_s + (c & 1) * 128, qa, smem_u32(ring.tile(2 * c)), keys16(c), ksteps);
-          umma_commit(&s_full[c & 1]);
-        }
-        __syncwarp();
-        return true;
-      };
-      auto values = [&](int c) {
-        return warp_wait(ring.full_of(2 * c + 1), ring.use(2 * c + 1), status, kStatusWaitFull, abort_flag);
-      };
-      auto products = [&](int c) {  // dP of chunk c, the only use of its V (leader only)
-        mma_dims<DP>(t_dp, da, smem_u32(ring.tile(2 * c + 1)), keys16(c), ksteps);
-        umma_commit(&dp_full[c & 1]);
-        umma_commit(ring.empty_of(2 * c + 1));
-      };
-      bool ok = warp_wait(q_full, 0, status, kStatusWaitFull, abort_flag) && scores(0) && values(0);
+      x += 2 * n;
+      ok = uniform(ok);
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    const uint32_t qa = smem_u32(q_tile), da = smem_u32(do_tile);
+    auto scores = [&](ChunkWalk& a) {  // S of a chunk into its buffer; K rows past the end zeroed
+      if (!a.valid) return true;
+      if (a.first() && !warp_wait(q_full, a.item & 1, status, kStatusWaitFull, abort_flag)) return false;
+      const int x = 2 * a.k;
+      if (!warp_wait(ring.full_of(x), ring.use(x), status, kStatusWaitFull, abort_flag)) return false;
+      if (a.keys() != a.keys16()) zero_rows<DP>(ring.tile(x), a.keys(), a.keys16(), lane);
       tc_fence_after();
-      if (ok && leader) products(0);
+      if (leader) {
+        mma_dims<DP>(t_s + (a.k & 1) * 128, qa, smem_u32(ring.tile(x)), a.keys16(), ksteps);
+        umma_commit(&s_full[a.k & 1]);
+      }
       __syncwarp();
-      if (ok && n > 1) ok = scores(1);
-      for (int c = 0; ok && c < n; ++c) {
-        const uint32_t use = (c >> 1) & 1;
-        if (c + 1 < n) {  // dP of the next chunk as soon as this one's is in registers
-          ok = values(c + 1) && warp_wait(&dp_free[c & 1], use, status, kStatusWaitAccum, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          if (leader) products(c + 1);
-          __syncwarp();
-        }
-        ok = warp_wait(&ds_ready[c & 1], use, status, kStatusWaitAccum, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        if (leader) {
-          mma_rows<4, 64>(t_dq, t_s + (c & 1) * 128, smem_u32(ring.tile(2 * c)), ksteps * 16, keys16(c) / 16, c > 0);
-          umma_commit(ring.empty_of(2 * c));
-        }
-        __syncwarp();
-        if (c + 2 < n) ok = scores(c + 2);
+      a.step();
+      return true;
+    };
+    auto products = [&](ChunkWalk& b) {  // dP of a chunk once the one before is in registers; the only use of its V
+      if (!b.valid) return true;
+      const int x = 2 * b.k + 1, before = b.k - 1;
+      if (!warp_wait(ring.full_of(x), ring.use(x), status, kStatusWaitFull, abort_flag)) return false;
+      if (b.k > 0 && !warp_wait(&dp_free[before & 1], (before >> 1) & 1, status, kStatusWaitAccum, abort_flag))
+        return false;
+      tc_fence_after();
+      if (leader) {
+        mma_dims<DP>(t_dp, da, smem_u32(ring.tile(x)), b.keys16(), ksteps);
+        umma_commit(&dp_full[b.k & 1]);
+        umma_commit(ring.empty_of(x));
+        if (b.last()) umma_commit(q_empty);  // Q and dO of the item have been used
       }
-      if (ok && leader) umma_commit(done);
-    } else if (warp >= 4) {
-      // ---- dS: two groups of eight warps take the even and the odd chunks, so that the exponentials of one chunk run
-      // beside the products of the other; one thread per query and half of the chunk's keys ----
-      const int part = (warp - 4) >> 2, quad = warp & 3;
-      const int mine = part >> 1, half = part & 1;
-      const int row = row0 + quad * 32 + lane;
-      const bool real = row < hi;
-      const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
-      const float lse = real ? p.lse[static_cast<long>(head) * p.T + row] : 0.f;
-      const float delta = real ? p.delta[static_cast<long>(head) * p.T + row] : 0.f;
-      const uint32_t s_addr = t_s + mine * 128 + lane_base + half * 64, dp_addr = t_dp + lane_base + half * 64;
-      bool ok = true;
-      for (int c = mine; c < n; c += 2) {
-        const uint32_t use = (c >> 1) & 1;
-        ok = warp_wait(&s_full[mine], use, status, kStatusWaitAccum, abort_flag);
+      __syncwarp();
+      b.step();
+      return true;
+    };
+    ChunkWalk a(p.table, p.head, p.H), b = a, c = a;
+    bool ok = scores(a) && products(b) && scores(a);
+    while (ok && c.valid) {
+      ok = products(b) && warp_wait(&ds_ready[c.k & 1], (c.k >> 1) & 1, status, kStatusWaitAccum, abort_flag);
+      if (ok && c.first() && c.item > 0)
+        ok = warp_wait(dq_free, (c.item - 1) & 1, status, kStatusWaitAccum, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      if (leader) {
+        const int x = 2 * c.k;
+        mma_rows<4, 64>(t_dq, t_s + (c.k & 1) * 128, smem_u32(ring.tile(x)), ksteps * 16, c.keys16() / 16, !c.first());
+        umma_commit(ring.empty_of(x));
+        if (c.last()) umma_commit(&dq_full[c.item & 1]);
+      }
+      __syncwarp();
+      c.step();
+      ok = scores(a);
+    }
+  } else if (warp >= 4) {
+    // ---- dS: two groups of eight warps take the even and the odd chunks, so that the exponentials of one chunk run
+    // beside the products of the other; one thread per query and half of the chunk's keys. The group that had an item's
+    // last chunk stores its dQ. ----
+    const int part = (warp - 4) >> 2, quad = warp & 3;
+    const int mine = part >> 1, half = part & 1;
+    const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t s_addr = t_s + mine * 128 + lane_base + half * 64, dp_addr = t_dp + lane_base + half * 64;
+    ChunkWalk at(p.table, p.head, p.H);
+    if (mine == 1 && at.valid) at.step();
+    bool ok = true;
+    while (ok && at.valid) {
+      const uint32_t use = (at.k >> 1) & 1;
+      const int row0 = at.row0() + quad * 32, row = row0 + lane, hi = at.hi();
+      const bool last = at.last();
+      const int limit = min(hi, row + 1) - (at.lo() + at.chunk * kRowsT) - half * 64;  // visible keys, of the last chunk
+      float lse = 0.f, delta = 0.f;
+      if (row < hi) {
+        lse = p.lse[static_cast<long>(at.head()) * p.T + row];
+        delta = p.delta[static_cast<long>(at.head()) * p.T + row];
+      }
+      ok = warp_wait(&s_full[mine], use, status, kStatusWaitAccum, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      // P waits for dP in the columns S came from: 64 more registers would spill
+      float v[32];
+#pragma unroll
+      for (int h = 0; h < 64; h += 32) {
+        tmem_load32(s_addr + h, v);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = ex2(fmaf(v[j], p.scale2, -lse));
+        tmem_store32(s_addr + h, reinterpret_cast<const uint32_t*>(v));
+      }
+      tmem_wait_st();
+      ok = warp_wait(&dp_full[mine], use, status, kStatusWaitAccum, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      float g[32];
+      uint32_t w[32];
+#pragma unroll
+      for (int h = 0; h < 64; h += 32) {
+        tmem_load32(s_addr + h, v);
+        tmem_load32(dp_addr + h, g);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) g[j] = v[j] * (g[j] - delta);
+        if (last) {
+          const uint32_t seen = low_bits(limit - h);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) g[j] = (seen >> j) & 1u ? g[j] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[h / 2 + j] = pack_bf16(g[2 * j], g[2 * j + 1]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&dp_free[mine]);
+      tmem_store32(s_addr, w);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ds_ready[mine]);
+      const int head = at.head(), item = at.item;
+      at.step();
+      if (at.valid) at.step();
+      if (last) {
+        ok = warp_wait(&dq_full[item & 1], (item >> 1) & 1, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const bool last = c == n - 1;
-        const int limit = min(hi, row + 1) - (lo + c * kRowsT) - half * 64;  // visible keys, of the last chunk
-        // P waits for dP in the columns S came from: 64 more registers would spill
-        float v[32];
-#pragma unroll
-        for (int h = 0; h < 64; h += 32) {
-          tmem_load32(s_addr + h, v);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = ex2(fmaf(v[j], p.scale2, -lse));
-          tmem_store32(s_addr + h, reinterpret_cast<const uint32_t*>(v));
-        }
-        tmem_wait_st();
-        ok = warp_wait(&dp_full[mine], use, status, kStatusWaitAccum, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        float g[32];
-        uint32_t w[32];
-#pragma unroll
-        for (int h = 0; h < 64; h += 32) {
-          tmem_load32(s_addr + h, v);
-          tmem_load32(dp_addr + h, g);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) g[j] = v[j] * (g[j] - delta);
-          if (last) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) g[j] = h + j < limit ? g[j] : 0.f;
-          }
-#pragma unroll
-          for (int j = 0; j < 16; ++j) w[h / 2 + j] = pack_bf16(g[2 * j], g[2 * j + 1]);
-        }
+        const int col = half * 64;
+        uint4 c[8];
+        if (col < p.D) load_packed64(t_dq + lane_base + col, p.scale, c);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&dp_free[mine]);
-        tmem_store32(s_addr, w);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ds_ready[mine]);
-      }
-      if (ok && warp_wait(done, 0, status, kStatusWaitAccum, abort_flag)) {
-        tc_fence_after();
-        const int col = part * (DP / 4);
-        store_row<DP / 4>(t_dq + lane_base + col, p.scale, p.dq + (static_cast<long>(row) * p.H + head) * p.D + col,
-                          p.D - col, real);
+        if (lane == 0) mbar_arrive(dq_free);
+        if (col < p.D)
+          store_rows64(c, p.dq + (static_cast<long>(row0) * p.H + head) * p.D + col, static_cast<long>(p.H) * p.D,
+                       hi - row0, p.D - col, lane);
       }
     }
   }
@@ -563,8 +653,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 template <int DP>
 int run_bwd(const PackedMaps& m, const PackedArgs& a, const BwdArgs& args, bool want_dq, bool want_dkv,
             unsigned* status, cudaStream_t stream) {
-  const long grid_kv = static_cast<long>(a.max_tiles) * a.Hkv, grid_q = static_cast<long>(a.max_tiles) * a.H;
-  if (grid_q > 0x7fffffffl) return -2;
+  const long items = static_cast<long>(a.max_tiles) * a.H;
+  if (items > 0x7fff0000l) return -2;
+  const long grid_kv = std::min(static_cast<long>(a.max_tiles) * a.Hkv, static_cast<long>(a.num_sms));
+  const long grid_q = std::min(items, static_cast<long>(a.num_sms));
   if (want_dkv) {
     auto kernel = packed_dkv_kernel<DP>;
     if (set_max_smem(kernel, BwdCfg<DP>::kSmem) != cudaSuccess) return -1;

@@ -245,20 +245,32 @@ __device__ __forceinline__ void stage_tmem64(uint32_t taddr, float f, uint8_t* s
   __syncwarp();
 }
 
-// 64 columns of the warp's TMEM lanes, times each lane's f, as bf16 rows through registers (store_rows64).
-__device__ __forceinline__ void store_tmem64(uint32_t taddr, float f, bf16* dst, long stride, int rows, int cols,
-                                             int lane) {
-  uint4 c[8];
+// 64 fp32 columns of a lane's TMEM row, times f, as eight groups of eight bf16.
+__device__ __forceinline__ void load_packed64(uint32_t taddr, float f, uint4 (&c)[8]) {
+  const uint64_t ff = pair_of(f, f);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float o[32];
     tmem_load32(taddr + h * 32, o);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      c[h * 4 + j] = make_uint4(pack_bf16(o[8 * j] * f, o[8 * j + 1] * f), pack_bf16(o[8 * j + 2] * f, o[8 * j + 3] * f),
-                                pack_bf16(o[8 * j + 4] * f, o[8 * j + 5] * f),
-                                pack_bf16(o[8 * j + 6] * f, o[8 * j + 7] * f));
+    for (int j = 0; j < 4; ++j) {
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float a, b;
+        unpair(mul2(pair_of(o[8 * j + 2 * k], o[8 * j + 2 * k + 1]), ff), a, b);
+        w[k] = pack_bf16(a, b);
+      }
+      c[h * 4 + j] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
+}
+
+// 64 columns of the warp's TMEM lanes, times each lane's f, as bf16 rows through registers (store_rows64).
+__device__ __forceinline__ void store_tmem64(uint32_t taddr, float f, bf16* dst, long stride, int rows, int cols,
+                                             int lane) {
+  uint4 c[8];
+  load_packed64(taddr, f, c);
   store_rows64(c, dst, stride, rows, cols, lane);
 }
 
