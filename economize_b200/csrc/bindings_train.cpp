@@ -229,8 +229,9 @@ Tensor packed_plan(const Tensor& q, const Tensor& k, const Tensor& cu, int rows,
 }
 
 // Output [T, H, D] and, for a backward pass, the log2-domain log-sum-exp of every row [H, T].
+// tiles: query tiles a CTA works on (0: by the mean length).
 std::tuple<Tensor, c10::optional<Tensor>> packed_forward(Tensor q, Tensor k, Tensor v, Tensor cu, double scale,
-                                                         bool need_lse) {
+                                                         bool need_lse, int64_t tiles) {
   check_packed(q, k, v, cu, scale);
   c10::cuda::CUDAGuard guard(q.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
@@ -242,15 +243,19 @@ std::tuple<Tensor, c10::optional<Tensor>> packed_forward(Tensor q, Tensor k, Ten
   k = heads_of(k);
   v = heads_of(v);
   cu = cu.contiguous();
-  const bool row_pairs = (q.size(1) / k.size(1)) % 2 != 0;
+  TORCH_CHECK(tiles >= 0 && tiles <= 2, "packed_attention: tiles must be 0, 1 or 2");
+  if (tiles == 0)
+    tiles = ecz::packed_single_tiles(static_cast<int>(q.size(0)), static_cast<int>(cu.size(0)) - 1) ? 1 : 2;
+  const int rows = ecz::packed_tile_rows(static_cast<int>(q.size(1)), static_cast<int>(k.size(1)),
+                                         static_cast<int>(tiles));
   ecz::PackedArgs a;
-  Tensor plan = packed_plan(q, k, cu, row_pairs ? 256 : 128, scale, a, stream);
+  Tensor plan = packed_plan(q, k, cu, rows, scale, a, stream);
   ecz::PackedMaps maps;
   maps.q = map_heads(q, 128);
   maps.k = map_heads(k, 128);
   maps.v = map_heads(v, 128);
   const int rc = ecz::launch_packed_forward(maps, a, out.data_ptr(), need_lse ? lse->data_ptr<float>() : nullptr,
-                                            row_pairs, ecz::device_status(q.device()), stream);
+                                            static_cast<int>(tiles), ecz::device_status(q.device()), stream);
   TORCH_CHECK(rc == 0, "packed_attention: forward launch failed (", rc, ")");
   return {out, lse};
 }
@@ -382,8 +387,8 @@ Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Te
 
 struct PackedFunction : torch::autograd::Function<PackedFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu,
-                        double scale) {
-    auto r = packed_forward(q, k, v, cu, scale, true);
+                        double scale, int64_t tiles) {
+    auto r = packed_forward(q, k, v, cu, scale, true, tiles);
     ctx->save_for_backward({q, k, v, std::get<0>(r), *std::get<1>(r), cu});
     ctx->saved_data["scale"] = scale;
     return std::get<0>(r);
@@ -396,7 +401,7 @@ struct PackedFunction : torch::autograd::Function<PackedFunction> {
     const bool need_dk = ctx->needs_input_grad(1), need_dv = ctx->needs_input_grad(2);
     auto r = packed_backward(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble(),
                              need_dq, need_dk || need_dv);
-    variable_list out(5);
+    variable_list out(6);
     if (need_dq) out[0] = *std::get<0>(r);
     if (need_dk) out[1] = *std::get<1>(r);
     if (need_dv) out[2] = *std::get<2>(r);
@@ -404,10 +409,11 @@ struct PackedFunction : torch::autograd::Function<PackedFunction> {
   }
 };
 
-Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, double scale) {
+Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, double scale,
+                        int64_t tiles) {
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
-    return PackedFunction::apply(q, k, v, cu, scale);
-  return std::get<0>(packed_forward(q, k, v, cu, scale, false));
+    return PackedFunction::apply(q, k, v, cu, scale, tiles);
+  return std::get<0>(packed_forward(q, k, v, cu, scale, false, tiles));
 }
 
 }  // namespace
@@ -421,7 +427,8 @@ void bind_training(pybind11::module_& m) {
         py::arg("weight"), py::arg("targets"), py::arg("ignore_index"), py::arg("logit_scale"), py::arg("reduction"),
         py::arg("chunk_rows") = 0);
   m.def("packed_attention", &packed_attention, "causal attention over packed sequences (tcgen05, autograd)",
-        py::arg("q"), py::arg("k"), py::arg("v"), py::arg("cu_seqlens"), py::arg("scale"));
+        py::arg("q"), py::arg("k"), py::arg("v"), py::arg("cu_seqlens"), py::arg("scale"),
+        py::arg("tiles") = 0);
 }
 
 }  // namespace ecz

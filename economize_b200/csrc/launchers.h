@@ -321,8 +321,11 @@ int packed_max_tiles(int T, int B, int rows);
 // scratch: 2 (B + 1) ints.
 int launch_packed_plan(const int* cu, int B, int T, int rows, int max_tiles, void* table, int* head, int* scratch,
                        unsigned* status, cudaStream_t stream);
-// The table's tiles are 256 rows with row_pairs, else 128 (then H / Hkv is even).
-int launch_packed_forward(const PackedMaps& maps, const PackedArgs& a, void* out, float* lse, bool row_pairs,
+// tiles: query tiles a CTA works on, 1 or 2 (packed_single_tiles: whether 1 is the better for T tokens in B sequences);
+// the table's tiles have packed_tile_rows rows.
+int packed_tile_rows(int H, int Hkv, int tiles);
+bool packed_single_tiles(int T, int B);
+int launch_packed_forward(const PackedMaps& maps, const PackedArgs& a, void* out, float* lse, int tiles,
                           unsigned* status, cudaStream_t stream);
 
 // packed_attention_bwd.cu: delta [H, T] = rows of dout . out (out contiguous [T, H, D]), then the gradients (dq null:

@@ -155,18 +155,21 @@ __global__ void __launch_bounds__(kPlanThreads)
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------
-// Eight softmax warps, one thread per row. Two threads per row (sixteen warps that exchange their maxima) were slower:
-// 973 against 885 us for a document of 16384 tokens, 16 heads over 4.
-constexpr int kSoftmaxWarps = 8;
-constexpr int kFwdThreads = 128 + 32 * kSoftmaxWarps;
-
-template <int DP>
+// kTiles 2: a CTA per SM works on two tiles that share the K / V chunks. kTiles 1: two CTAs per SM work on a tile each, with
+// half the shared memory and TMEM: they load K and V twice, but are not tied to one another's phases, which is what
+// counts where an item is a chunk or two (see packed_single_tiles).
+// One thread per row: with two (sixteen softmax warps that exchange their maxima) a document of 16384 tokens, 16 heads
+// over 4, took 973 us instead of 885.
+template <int DP, int kTiles>
 struct FwdCfg {
   static constexpr int kTileBytes = kRowsT * DP * 2;
-  static constexpr int kRing = DP == 64 ? 8 : 4;  // K and V chunks in turn
-  static constexpr int kStage = kSoftmaxWarps * 4096;  // 4 KB for each softmax warp's output rows
-  static constexpr int kSmem = (2 + kRing) * kTileBytes + kStage + 1024 + 512;
-  static_assert(kSmem <= 232448, "227 KB of shared memory");
+  static constexpr int kRing = (DP == 64 ? 4 : 2) * kTiles;  // K and V chunks in turn
+  static constexpr int kStage = kTiles * 4 * 4096;           // 4 KB for each softmax warp's output rows
+  static constexpr int kSmem = (kTiles + kRing) * kTileBytes + kStage + 512;
+  static constexpr int kSoftmaxWarps = 4 * kTiles;
+  static constexpr int kThreads = 32 * (kSoftmaxWarps + 2);  // and a warp each for loads and MMAs
+  static constexpr int kTmem = 256 * kTiles;                 // S of every tile, then O of every tile
+  static_assert(kSmem + 1024 <= 233472 / (3 - kTiles), "the CTAs of an SM fit its 228 KB, 1 KB each reserved");
 };
 
 struct FwdArgs {
@@ -176,19 +179,19 @@ struct FwdArgs {
   const int* head;
   int T, H, Hkv, D;
   float scale2;    // scale times log2(e)
-  bool row_pairs;  // tiles of 256 rows of one head (else 128 rows of two heads of a group)
+  bool row_pairs;  // two tiles are 256 rows of one head (else 128 rows of two heads of a group)
 };
 
-template <int DP>
-__global__ void __launch_bounds__(kFwdThreads, 1)
+template <int DP, int kTiles>
+__global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
     packed_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FwdArgs p, unsigned* status) {
-  using Cfg = FwdCfg<DP>;
+  using Cfg = FwdCfg<DP, kTiles>;
   constexpr int kRing = Cfg::kRing, kTileBytes = Cfg::kTileBytes;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr int kLoadWarp = Cfg::kSoftmaxWarps, kMmaWarp = kLoadWarp + 1;
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* q_tiles = smem;
-  uint8_t* ring = smem + 2 * kTileBytes;
+  uint8_t* ring = smem + kTiles * kTileBytes;
   uint8_t* stages = ring + kRing * kTileBytes;
   uint64_t* q_full = reinterpret_cast<uint64_t*>(stages + Cfg::kStage);
   uint64_t* q_empty = q_full + 1;
@@ -201,6 +204,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (misplaced(smem, status)) return;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
@@ -221,7 +225,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     tma_prefetch_desc(&tm_v);
   }
   __syncwarp();
-  if (warp == 0) tmem_alloc(tmem_slot, 512);
+  if (warp == 0) tmem_alloc(tmem_slot, Cfg::kTmem);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -232,18 +236,20 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   zero_padding(p.out, p.T, static_cast<long>(p.H) * p.D, p.head);
   const int group = p.H / p.Hkv;
   const int ksteps = (p.D + 15) / 16;
-  const int per = p.row_pairs ? p.H : p.H / 2;
+  const bool row_pairs = kTiles == 1 || p.row_pairs;
+  const int per = row_pairs ? p.H : p.H / 2;
   // an item's query tile i: its head, first row and number of key chunks (the last one holds the diagonal)
-  auto head_of = [&](const auto& items, int i) { return p.row_pairs ? items.sub : 2 * items.sub + i; };
+  auto head_of = [&](const auto& items, int i) { return row_pairs ? items.sub : 2 * items.sub + i; };
   auto row_of = [&](const auto& items, int i) {
-    return items.tile.x + (p.row_pairs ? items.tile.z * 256 + i * kRowsT : items.tile.z * kRowsT);
+    return items.tile.x + (row_pairs ? (items.tile.z * kTiles + i) * kRowsT : items.tile.z * kRowsT);
   };
   auto chunks_of = [&](const auto& items, int i) {
     const int row = row_of(items, i);
+    if (i >= kTiles) return 0;
     return row < items.tile.y ? (row - items.tile.x) / kRowsT + 1 : 0;
   };
 
-  if (warp == 0) {
+  if (warp == kLoadWarp) {
     // ---- loads: an item's Q, then its K and V chunks in turn ----
     Items<> items(p.table, p.head, per);
     const uint32_t qa = smem_u32(q_tiles), ra = smem_u32(ring);
@@ -261,19 +267,19 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           load_tile<DP>(ra + s * kTileBytes, (x & 1) ? &tm_v : &tm_k, &kv_full[s], kvh, lo + (x >> 1) * kRowsT);
           return true;
         };
-        // the first chunk does not wait for the previous item's queries to be read
-        ok = chunk(0) && chunk(1) && mbar_wait(q_empty, (n_items & 1) ^ 1, status, kStatusWaitEmpty, abort_flag);
+        // the first K does not wait for the previous item's queries to be read, nor the queries for its last V
+        ok = chunk(0) && mbar_wait(q_empty, (n_items & 1) ^ 1, status, kStatusWaitEmpty, abort_flag);
         if (ok) {
           mbar_arrive_expect_tx(q_full, (c1 > 0 ? 2 : 1) * kTileBytes);
           load_tile<DP>(qa, &tm_q, q_full, head0, row0);
           if (c1 > 0) load_tile<DP>(qa + kTileBytes, &tm_q, q_full, head1, row1);
         }
-        for (int x = 2; ok && x < 2 * n; ++x) ok = chunk(x);
+        for (int x = 1; ok && x < 2 * n; ++x) ok = chunk(x);
       }
       it += 2 * n;
       ok = uniform(ok);
     }
-  } else if (warp == 1) {
+  } else if (warp == kMmaWarp) {
     // ---- MMAs ----
     Items<> items(p.table, p.head, per);
     const bool leader = elect_one();
@@ -294,7 +300,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       tc_fence_after();
       if (leader) {
         const int n = (keys_of(0) + 15) & ~15;
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kTiles; ++i) {
           if (chunks[i] == 0) continue;
           mma_dims<DP>(tmem + i * 128, qa + i * kTileBytes, ra + (base % kRing) * kTileBytes, n, ksteps);
           umma_commit(&s_full[i]);
@@ -312,20 +318,20 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         const int n = keys_of(c), n16 = (n + 15) & ~15;
         uint8_t* v_tile = ring + (v_it % kRing) * kTileBytes;
         if (n16 != n) zero_rows<DP>(v_tile, n, n16, lane);
-        for (int i = 0; ok && i < 2; ++i) {
+        for (int i = 0; ok && i < kTiles; ++i) {
           if (c >= chunks[i]) continue;
           // the first half of P . V runs under the exponentials of the second
           ok = warp_wait(&p_ready[2 * i], (used[i] + c) & 1, status, kStatusWaitAccum, abort_flag);
           if (!ok) break;
           tc_fence_after();
           if (leader)
-            mma_rows<8, 64, 0, 4>(tmem + 256 + i * DP, tmem + i * 128, smem_u32(v_tile), ksteps * 16, n16 / 16, c > 0);
+            mma_rows<8, 64, 0, 4>(tmem + kTiles * 128 + i * DP, tmem + i * 128, smem_u32(v_tile), ksteps * 16, n16 / 16, c > 0);
           __syncwarp();
           ok = warp_wait(&p_ready[2 * i + 1], (used[i] + c) & 1, status, kStatusWaitAccum, abort_flag);
           if (!ok) break;
           tc_fence_after();
           if (leader) {
-            mma_rows<8, 64, 4, 8>(tmem + 256 + i * DP, tmem + i * 128, smem_u32(v_tile), ksteps * 16, n16 / 16, true);
+            mma_rows<8, 64, 4, 8>(tmem + kTiles * 128 + i * DP, tmem + i * 128, smem_u32(v_tile), ksteps * 16, n16 / 16, true);
             umma_commit(&o_done[i]);
             if (c + 1 < chunks[i]) {
               mma_dims<DP>(tmem + i * 128, qa + i * kTileBytes, ra + (k_it % kRing) * kTileBytes,
@@ -346,11 +352,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       used[0] += chunks[0];
       used[1] += chunks[1];
     }
-  } else if (warp >= 4) {
+  } else {
     // ---- softmax: one thread per row ----
-    const int i = (warp - 4) >> 2, quad = warp & 3;
+    const int i = warp >> 2, quad = warp & 3;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t s_addr = lane_base + i * 128, o_addr = lane_base + 256 + i * DP;
+    const uint32_t s_addr = lane_base + i * 128, o_addr = lane_base + kTiles * 128 + i * DP;
     Items<false> items(p.table, p.head, per);
     uint32_t used = 0;  // chunks of this tile so far, over all items
     bool ok = true;
@@ -458,7 +464,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         bf16* dst = p.out + row0 * stride + static_cast<long>(my_head) * p.D;
 #pragma unroll 1
         for (int d = 0; d < p.D; d += 64)
-          stage_tmem64(o_addr + d, inv, stages + (warp - 4) * 4096, dst + d, stride, hi - row0, p.D - d, lane);
+          stage_tmem64(o_addr + d, inv, stages + warp * 4096, dst + d, stride, hi - row0, p.D - d, lane);
         tc_fence_before();  // the next item's first P . V overwrites O after this warp's next p_ready
       }
     }
@@ -467,21 +473,23 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   tc_fence_before();
   __syncthreads();
   settle(*abort_flag != 0);
-  if (warp == 0) tmem_dealloc(tmem, 512);
+  if (warp == 0) tmem_dealloc(tmem, Cfg::kTmem);
 }
 
-template <int DP>
-int run_fwd(const PackedMaps& maps, const PackedArgs& a, void* out, float* lse, bool row_pairs, unsigned* status,
+template <int DP, int kTiles>
+int run_fwd(const PackedMaps& maps, const PackedArgs& a, void* out, float* lse, unsigned* status,
             cudaStream_t stream) {
-  auto kernel = packed_fwd_kernel<DP>;
-  if (set_max_smem(kernel, FwdCfg<DP>::kSmem) != cudaSuccess) return -1;
+  using Cfg = FwdCfg<DP, kTiles>;
+  auto kernel = packed_fwd_kernel<DP, kTiles>;
+  if (set_max_smem(kernel, Cfg::kSmem) != cudaSuccess) return -1;
+  const bool row_pairs = kTiles == 1 || packed_tile_rows(a.H, a.Hkv, kTiles) == 256;
   const FwdArgs args{static_cast<bf16*>(out), lse, static_cast<const int4*>(a.table), a.head, a.T, a.H, a.Hkv, a.D,
                      a.scale * kLog2e, row_pairs};
   const long most = static_cast<long>(a.max_tiles) * (row_pairs ? a.H : a.H / 2);
   if (most > 0x7fff0000l) return -2;
-  const long grid = std::min(most, static_cast<long>(a.num_sms));
-  return launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(kFwdThreads), FwdCfg<DP>::kSmem, stream, maps.q,
-                    maps.k, maps.v, args, status) == cudaSuccess ? 0 : -1;
+  const long grid = std::min(most, static_cast<long>(a.num_sms) * (3 - kTiles));
+  return launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(Cfg::kThreads), Cfg::kSmem, stream, maps.q, maps.k,
+                    maps.v, args, status) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace
@@ -496,10 +504,17 @@ int launch_packed_plan(const int* cu, int B, int T, int rows, int max_tiles, voi
                     static_cast<int4*>(table), head, scratch, scratch + B + 1, status) == cudaSuccess ? 0 : -1;
 }
 
-int launch_packed_forward(const PackedMaps& maps, const PackedArgs& a, void* out, float* lse, bool row_pairs,
+int packed_tile_rows(int H, int Hkv, int tiles) { return tiles == 2 && (H / Hkv) % 2 != 0 ? 256 : 128; }
+
+bool packed_single_tiles(int T, int B) { return static_cast<long>(T) < 512l * B; }
+
+int launch_packed_forward(const PackedMaps& maps, const PackedArgs& a, void* out, float* lse, int tiles,
                           unsigned* status, cudaStream_t stream) {
-  return a.D <= 64 ? run_fwd<64>(maps, a, out, lse, row_pairs, status, stream)
-                   : run_fwd<128>(maps, a, out, lse, row_pairs, status, stream);
+  if (tiles == 1)
+    return a.D <= 64 ? run_fwd<64, 1>(maps, a, out, lse, status, stream)
+                     : run_fwd<128, 1>(maps, a, out, lse, status, stream);
+  return a.D <= 64 ? run_fwd<64, 2>(maps, a, out, lse, status, stream)
+                   : run_fwd<128, 2>(maps, a, out, lse, status, stream);
 }
 
 }  // namespace ecz

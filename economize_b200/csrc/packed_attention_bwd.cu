@@ -73,8 +73,6 @@ struct BwdCfg {
   static constexpr int kRing = DP == 64 ? 10 : 5;  // streamed tiles
   static constexpr int kStatRing = 3;
   static constexpr int kStats = 2 * 128 * 4;  // lse and delta of a query tile
-  // no slack for alignment: dynamic shared memory starts on a 1024-byte boundary where nothing static precedes it (the
-  // kernels check)
   static constexpr int kSmem = (2 + kRing) * kTileBytes + (DP == 64 ? kStatRing : 2) * kStats + 512;
   static_assert(kSmem <= 232448, "227 KB of shared memory");
 };
@@ -133,10 +131,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if ((smem_u32(smem) & 1023u) != 0) {
-    if (threadIdx.x == 0) atomicOr(status, kStatusBadShape);
-    return;
-  }
+  if (misplaced(smem, status)) return;
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
     mbar_init(kv_empty, 1);
@@ -393,8 +388,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 // The chunks of a persistent CTA's items in one sequence: `chunk` of the item's `n`, counted over all items by `k`. The
 // issuing warp runs three of them (scores, dP and dQ are issued two, one and no chunks ahead, across items), a compute
 // group steps by two.
+template <bool kAhead>
 struct ChunkWalk {
-  Items<> items;
+  Items<kAhead> items;
   int chunk, n, k, item;
   bool valid;
   __device__ __forceinline__ ChunkWalk(const int4* table, const int* head, int per) : items(table, head, per), k(0), item(-1) {
@@ -406,7 +402,7 @@ struct ChunkWalk {
     ++item;
     if (!valid) return;
     n = items.tile.z + 1;  // key chunks, the last one on the diagonal
-    items.look();
+    if (kAhead) items.look();
   }
   __device__ __forceinline__ void step() {
     ++k;
@@ -441,15 +437,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   // only chunk before this item's last dQ would take the phase before this one for its own.
   uint64_t* dq_full = ds_ready + 2;
   uint64_t* dq_free = dq_full + 2;   // dQ is in registers
-  uint64_t* q_empty = dq_free + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_empty + 1);
+  uint64_t* q_empty = dq_free + 1;   // an item's last scores are computed: Q may be overwritten, some time before dO
+  uint64_t* do_full = q_empty + 1;
+  uint64_t* do_empty = do_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(do_empty + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if ((smem_u32(smem) & 1023u) != 0) {
-    if (threadIdx.x == 0) atomicOr(status, kStatusBadShape);
-    return;
-  }
+  if (misplaced(smem, status)) return;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     for (int i = 0; i < kRing; ++i) {
@@ -466,6 +461,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     mbar_init(&dq_full[1], 1);
     mbar_init(dq_free, kComputeWarps / 2);
     mbar_init(q_empty, 1);
+    mbar_init(do_full, 1);
+    mbar_init(do_empty, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -498,12 +495,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                         lo + (i >> 1) * kRowsT);
           return true;
         };
-        // the first chunk does not wait for the previous item's queries to be read
-        ok = load(0) && load(1) && mbar_wait(q_empty, (n_items & 1) ^ 1, status, kStatusWaitEmpty, abort_flag);
+        const uint32_t turn = (n_items & 1) ^ 1;
+        ok = load(0) && mbar_wait(q_empty, turn, status, kStatusWaitEmpty, abort_flag);
         if (ok) {
-          mbar_arrive_expect_tx(q_full, 2 * kTileBytes);
+          mbar_arrive_expect_tx(q_full, kTileBytes);
           load_tile<DP>(smem_u32(q_tile), &tm_q, q_full, head, lo + (n - 1) * kRowsT);
-          load_tile<DP>(smem_u32(do_tile), &tm_do, q_full, head, lo + (n - 1) * kRowsT);
+        }
+        ok = ok && load(1) && mbar_wait(do_empty, turn, status, kStatusWaitEmpty, abort_flag);
+        if (ok) {
+          mbar_arrive_expect_tx(do_full, kTileBytes);
+          load_tile<DP>(smem_u32(do_tile), &tm_do, do_full, head, lo + (n - 1) * kRowsT);
         }
         for (int i = 2; ok && i < 2 * n; ++i) ok = load(i);
       }
@@ -513,7 +514,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   } else if (warp == 1) {
     const bool leader = elect_one();
     const uint32_t qa = smem_u32(q_tile), da = smem_u32(do_tile);
-    auto scores = [&](ChunkWalk& a) {  // S of a chunk into its buffer; K rows past the end zeroed
+    auto scores = [&](ChunkWalk<true>& a) {  // S of a chunk into its buffer; K rows past the end zeroed
       if (!a.valid) return true;
       if (a.first() && !warp_wait(q_full, a.item & 1, status, kStatusWaitFull, abort_flag)) return false;
       const int x = 2 * a.k;
@@ -523,14 +524,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (leader) {
         mma_dims<DP>(t_s + (a.k & 1) * 128, qa, smem_u32(ring.tile(x)), a.keys16(), ksteps);
         umma_commit(&s_full[a.k & 1]);
+        if (a.last()) umma_commit(q_empty);
       }
       __syncwarp();
       a.step();
       return true;
     };
-    auto products = [&](ChunkWalk& b) {  // dP of a chunk once the one before is in registers; the only use of its V
+    auto products = [&](ChunkWalk<true>& b) {  // dP of a chunk once the one before is in registers; the only use of its V
       if (!b.valid) return true;
       const int x = 2 * b.k + 1, before = b.k - 1;
+      if (b.first() && !warp_wait(do_full, b.item & 1, status, kStatusWaitFull, abort_flag)) return false;
       if (!warp_wait(ring.full_of(x), ring.use(x), status, kStatusWaitFull, abort_flag)) return false;
       if (b.k > 0 && !warp_wait(&dp_free[before & 1], (before >> 1) & 1, status, kStatusWaitAccum, abort_flag))
         return false;
@@ -539,13 +542,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         mma_dims<DP>(t_dp, da, smem_u32(ring.tile(x)), b.keys16(), ksteps);
         umma_commit(&dp_full[b.k & 1]);
         umma_commit(ring.empty_of(x));
-        if (b.last()) umma_commit(q_empty);  // Q and dO of the item have been used
+        if (b.last()) umma_commit(do_empty);
       }
       __syncwarp();
       b.step();
       return true;
     };
-    ChunkWalk a(p.table, p.head, p.H), b = a, c = a;
+    ChunkWalk<true> a(p.table, p.head, p.H), b = a, c = a;
     bool ok = scores(a) && products(b) && scores(a);
     while (ok && c.valid) {
       ok = products(b) && warp_wait(&ds_ready[c.k & 1], (c.k >> 1) & 1, status, kStatusWaitAccum, abort_flag);
@@ -571,7 +574,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int mine = part >> 1, half = part & 1;
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t s_addr = t_s + mine * 128 + lane_base + half * 64, dp_addr = t_dp + lane_base + half * 64;
-    ChunkWalk at(p.table, p.head, p.H);
+    ChunkWalk<false> at(p.table, p.head, p.H);
     if (mine == 1 && at.valid) at.step();
     bool ok = true;
     while (ok && at.valid) {

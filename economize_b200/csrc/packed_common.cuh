@@ -274,6 +274,14 @@ __device__ __forceinline__ void store_tmem64(uint32_t taddr, float f, bf16* dst,
   store_rows64(c, dst, stride, rows, cols, lane);
 }
 
+// Tiles need 1024-byte boundaries, and there is no room to align them: dynamic shared memory starts on such a boundary
+// where nothing static precedes it. Should it not, every thread leaves and the status says so.
+__device__ __forceinline__ bool misplaced(const uint8_t* smem, unsigned* status) {
+  if ((smem_u32(smem) & 1023u) == 0) return false;
+  if (threadIdx.x == 0) atomicOr(status, kStatusBadShape);
+  return true;
+}
+
 // The end of a CTA whose waits may have given up: copies in flight land before the shared memory goes.
 __device__ __forceinline__ void settle(bool aborted) {
   if (!aborted) return;

@@ -76,9 +76,10 @@ def _within(got, z, name):
     assert (off <= err).all(), f"{name}: {(off / err).max().item():.2f} times the bound"
 
 
-def _run(q, k, v, cu, dout, scale=None):
+def _run(q, k, v, cu, dout, scale=None, tiles=0):
     q, k, v = (x.detach().requires_grad_() for x in (q, k, v))
-    out = ops.packed_attention(q, k, v, cu, scale)
+    out = ops.packed_attention(q, k, v, cu, scale) if tiles == 0 else \
+        ops.require().packed_attention(q, k, v, cu, scale or q.shape[-1] ** -0.5, tiles)
     return (out.detach(), *torch.autograd.grad(out, (q, k, v), dout))
 
 
@@ -94,6 +95,18 @@ def test_outputs_and_gradients(cuda, lens, heads, kv_heads, dim):
     for name, x in zip(("out", "dq", "dk", "dv"), got):
         _within(x, z, name)
     assert torch.equal(ops.packed_attention(q, k, v, cu), got[0])  # without gradients
+    assert ops.require().status(0) == 0
+
+
+@pytest.mark.parametrize("tiles", [1, 2])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 128), (3, 3, 64), (6, 2, 96)])
+def test_both_forms_of_the_forward_pass(cuda, tiles, heads, kv_heads, dim):
+    """A CTA works on one query tile or on two, chosen by the mean length; every shape goes through either."""
+    for lens, pad in (([700], 0), ([5, 300, 129, 0, 64, 1], 20), ([256] * 3, 0), ([1] * 200, 3)):
+        q, k, v, cu, dout = _inputs(cuda, lens, heads, kv_heads, dim, pad=pad, seed=20)
+        z = _oracle(q, k, v, lens, dout, dim ** -0.5)
+        for name, got in zip(("out", "dq", "dk", "dv"), _run(q, k, v, cu, dout, tiles=tiles)):
+            _within(got, z, name)
     assert ops.require().status(0) == 0
 
 
