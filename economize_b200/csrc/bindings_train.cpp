@@ -175,12 +175,12 @@ Tensor heads_of(const Tensor& x) {
   return reinterpret_cast<uintptr_t>(y.data_ptr()) % 16 == 0 ? y : y.clone();
 }
 
-CUtensorMap map_heads(const Tensor& x, int box_tokens) {
+CUtensorMap map_heads(const Tensor& x, int box_heads, int box_tokens) {
   CUtensorMap map;
   std::memset(&map, 0, sizeof(map));
   const auto step = [&](int d, int64_t one) { return x.size(d) > 1 ? x.stride(d) : one; };
   const int rc = ecz::make_tmap_heads(&map, x.data_ptr(), x.size(0), x.size(1), x.size(2),
-                                      step(0, x.size(1) * x.size(2)), step(1, x.size(2)), box_tokens);
+                                      step(0, x.size(1) * x.size(2)), step(1, x.size(2)), box_heads, box_tokens);
   TORCH_CHECK(rc == 0, "cuTensorMapEncodeTiled failed (code ", rc, ") for a [", x.size(0), ", ", x.size(1), ", ",
               x.size(2), "] operand");
   return map;
@@ -203,80 +203,87 @@ void check_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
   TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "packed_attention: head dimensions 8 to 128 in steps of 8 (got ", D,
               ")");
   TORCH_CHECK(cu.dim() == 1 && cu.size(0) >= 1, "packed_attention: cu_seqlens must be [B + 1]");
-  TORCH_CHECK(T <= (int64_t{1} << 30) && cu.size(0) <= (int64_t{1} << 24), "packed_attention: too many tokens");
+  TORCH_CHECK(T <= (int64_t{1} << 26) && cu.size(0) <= (int64_t{1} << 24), "packed_attention: too many tokens");
   TORCH_CHECK(scale > 0 && std::isfinite(scale), "packed_attention: the scale must be positive (got ", scale, ")");
 }
 
-// Tile table of packed sequences (rows 128 or 256) in `buf`; fills args.
-Tensor packed_plan(const Tensor& q, const Tensor& k, const Tensor& cu, int rows, double scale, ecz::PackedArgs& a,
-                   cudaStream_t stream) {
-  const int T = static_cast<int>(q.size(0)), B = static_cast<int>(cu.size(0)) - 1;
-  a.T = T;
+// Shapes and the places of the tile tables of `count` kernels (1: the forward pass, 3: the gradients' too) in `buf`.
+ecz::PackedArgs packed_args(const Tensor& q, const Tensor& k, int64_t B, double scale, int tiles, int count,
+                            const Tensor& buf) {
+  ecz::PackedArgs a;
+  a.T = static_cast<int>(q.size(0));
   a.H = static_cast<int>(q.size(1));
   a.Hkv = static_cast<int>(k.size(1));
   a.D = static_cast<int>(q.size(2));
-  a.scale = static_cast<float>(scale);
+  a.lp = ecz::packed_heads_log2(a.H, a.Hkv);
   a.num_sms = ecz::device_sms(q.get_device());
-  a.max_tiles = std::max(1, ecz::packed_max_tiles(T, B, rows));
-  Tensor buf = at::empty({int64_t{4} * a.max_tiles + 4 + 2 * (int64_t{B} + 1)}, cu.options());
-  int* base = buf.data_ptr<int>();
-  a.table = base;
-  a.head = base + int64_t{4} * a.max_tiles;
-  TORCH_CHECK(ecz::launch_packed_plan(cu.data_ptr<int>(), B, T, rows, a.max_tiles, base, base + int64_t{4} * a.max_tiles,
-                                      base + int64_t{4} * a.max_tiles + 4, ecz::device_status(q.device()), stream) == 0,
-              "packed_attention: plan launch failed");
-  return buf;
+  a.scale = static_cast<float>(scale);
+  int* at = buf.defined() ? buf.data_ptr<int>() : nullptr;
+  ecz::PackedTable* tables[3] = {&a.fwd, &a.dq, &a.dkv};
+  const int rows[3] = {(128 >> a.lp) * tiles, 128 >> a.lp, 128};
+  for (int i = 0; i < count; ++i) {
+    tables[i]->rows = rows[i];
+    tables[i]->max_tiles = std::max(1, ecz::packed_max_tiles(a.T, static_cast<int>(B), rows[i]));
+    if (at == nullptr) continue;
+    tables[i]->entries = at;
+    tables[i]->head = at + int64_t{4} * tables[i]->max_tiles;
+    tables[i]->scratch = tables[i]->head + 4;
+    at = tables[i]->scratch + (2 * (B + 1) + 3) / 4 * 4;
+  }
+  return a;
 }
 
-// Output [T, H, D] and, for a backward pass, the log2-domain log-sum-exp of every row [H, T].
+// Output [T, H, D] and, for a backward pass, the log2-domain log-sum-exp of every row [H, T] and the tile tables.
 // tiles: query tiles a CTA works on (0: by the mean length).
-std::tuple<Tensor, c10::optional<Tensor>> packed_forward(Tensor q, Tensor k, Tensor v, Tensor cu, double scale,
-                                                         bool need_lse, int64_t tiles) {
+std::tuple<Tensor, Tensor, Tensor> packed_forward(Tensor q, Tensor k, Tensor v, Tensor cu, double scale, bool training,
+                                                  int64_t tiles) {
   check_packed(q, k, v, cu, scale);
+  TORCH_CHECK(tiles >= 0 && tiles <= 2, "packed_attention: tiles must be 0, 1 or 2");
   c10::cuda::CUDAGuard guard(q.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  Tensor out = at::empty(q.sizes(), q.options());
-  c10::optional<Tensor> lse;
-  if (need_lse) lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
-  if (q.size(0) == 0) return {out, lse};
+  Tensor out = at::empty(q.sizes(), q.options()), lse, plan;
+  if (training) lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+  if (q.size(0) == 0) return {out, lse, plan};
   q = heads_of(q);
   k = heads_of(k);
   v = heads_of(v);
   cu = cu.contiguous();
-  TORCH_CHECK(tiles >= 0 && tiles <= 2, "packed_attention: tiles must be 0, 1 or 2");
-  if (tiles == 0)
-    tiles = ecz::packed_single_tiles(static_cast<int>(q.size(0)), static_cast<int>(cu.size(0)) - 1) ? 1 : 2;
-  const int rows = ecz::packed_tile_rows(static_cast<int>(q.size(1)), static_cast<int>(k.size(1)),
-                                         static_cast<int>(tiles));
-  ecz::PackedArgs a;
-  Tensor plan = packed_plan(q, k, cu, rows, scale, a, stream);
+  const int T = static_cast<int>(q.size(0)), B = static_cast<int>(cu.size(0)) - 1;
+  if (tiles == 0) tiles = ecz::packed_single_tiles(T, B) ? 1 : 2;
+  const int count = training ? 3 : 1;
+  ecz::PackedArgs a = packed_args(q, k, B, scale, static_cast<int>(tiles), count, Tensor());
+  int64_t ints = 0;
+  for (const auto* t : {&a.fwd, &a.dq, &a.dkv})
+    ints += t->max_tiles > 0 ? int64_t{4} * t->max_tiles + 4 + (2 * (int64_t{B} + 1) + 3) / 4 * 4 : 0;
+  plan = at::empty({ints}, cu.options());
+  a = packed_args(q, k, B, scale, static_cast<int>(tiles), count, plan);
+  unsigned* status = ecz::device_status(q.device());
+  const ecz::PackedTable tables[3] = {a.fwd, a.dq, a.dkv};
+  TORCH_CHECK(ecz::launch_packed_plan(cu.data_ptr<int>(), B, T, tables, count, status, stream) == 0,
+              "packed_attention: plan launch failed");
   ecz::PackedMaps maps;
-  maps.q = map_heads(q, 128);
-  maps.k = map_heads(k, 128);
-  maps.v = map_heads(v, 128);
-  const int rc = ecz::launch_packed_forward(maps, a, out.data_ptr(), need_lse ? lse->data_ptr<float>() : nullptr,
-                                            static_cast<int>(tiles), ecz::device_status(q.device()), stream);
+  maps.q = map_heads(q, 1 << a.lp, 128 >> a.lp);
+  maps.k = map_heads(k, 1, 128);
+  maps.v = map_heads(v, 1, 128);
+  maps.k32 = map_heads(k, 1, 32);
+  maps.v32 = map_heads(v, 1, 32);
+  const int rc = ecz::launch_packed_forward(maps, a, out.data_ptr(), training ? lse.data_ptr<float>() : nullptr,
+                                            static_cast<int>(tiles), status, stream);
   TORCH_CHECK(rc == 0, "packed_attention: forward launch failed (", rc, ")");
-  return {out, lse};
+  return {out, lse, plan};
 }
 
-// Gradients of q, k and v (those asked for) given the output's.
-std::tuple<c10::optional<Tensor>, c10::optional<Tensor>, c10::optional<Tensor>> packed_backward(
-    Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, Tensor cu, double scale, bool need_dq,
-    bool need_dkv) {
-  check_packed(q, k, v, cu, scale);
+// Gradients of q, k and v (those asked for; undefined otherwise) given the output's. plan, tiles: of the forward pass
+// over B sequences.
+std::tuple<Tensor, Tensor, Tensor> packed_backward(Tensor dout, Tensor q, Tensor k, Tensor v, const Tensor& out,
+                                                   const Tensor& lse, const Tensor& plan, int64_t B, double scale,
+                                                   int64_t tiles, bool need_dq, bool need_dkv) {
   CHECK_BF16(dout);
   CHECK_ON(dout, q);
-  CHECK_ON(out, q);
-  CHECK_ON(lse, q);
-  TORCH_CHECK(dout.sizes() == q.sizes() && out.sizes() == q.sizes() && out.is_contiguous() &&
-                  out.scalar_type() == at::kBFloat16,
-              "packed_attention: the output and its gradient have the queries' shape");
-  TORCH_CHECK(lse.is_contiguous() && lse.scalar_type() == at::kFloat && lse.numel() == q.size(0) * q.size(1),
-              "packed_attention: lse must be fp32 [H, T]");
+  TORCH_CHECK(dout.sizes() == q.sizes(), "packed_attention: the output's gradient has the queries' shape");
   c10::cuda::CUDAGuard guard(q.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  c10::optional<Tensor> dq, dk, dv;
+  Tensor dq, dk, dv;
   if (need_dq) dq = at::empty(q.sizes(), q.options());
   if (need_dkv) {
     dk = at::empty(k.sizes(), k.options());
@@ -287,22 +294,21 @@ std::tuple<c10::optional<Tensor>, c10::optional<Tensor>, c10::optional<Tensor>> 
   k = heads_of(k);
   v = heads_of(v);
   dout = heads_of(dout);
-  cu = cu.contiguous();
-  const int T = static_cast<int>(q.size(0)), H = static_cast<int>(q.size(1)), D = static_cast<int>(q.size(2));
-  ecz::PackedArgs a;
-  Tensor plan = packed_plan(q, k, cu, 128, scale, a, stream);
+  const ecz::PackedArgs a = packed_args(q, k, B, scale, static_cast<int>(tiles), 3, plan);
   Tensor delta = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
-  TORCH_CHECK(ecz::launch_packed_delta(out.data_ptr(), dout.data_ptr(), dout.stride(0), dout.stride(1), T, H, D,
+  TORCH_CHECK(ecz::launch_packed_delta(out.data_ptr(), dout.data_ptr(), dout.stride(0), dout.stride(1), a.T, a.H, a.D,
                                        delta.data_ptr<float>(), stream) == 0,
               "packed_attention: delta launch failed");
   ecz::PackedMaps maps;
-  maps.q = map_heads(q, 128);
-  maps.k = map_heads(k, 128);
-  maps.v = map_heads(v, 128);
-  maps.dout = map_heads(dout, 128);
+  maps.q = map_heads(q, 1 << a.lp, 128 >> a.lp);
+  maps.dout = map_heads(dout, 1 << a.lp, 128 >> a.lp);
+  maps.k = map_heads(k, 1, 128);
+  maps.v = map_heads(v, 1, 128);
+  maps.k32 = map_heads(k, 1, 32);
+  maps.v32 = map_heads(v, 1, 32);
   const int rc = ecz::launch_packed_backward(maps, a, lse.data_ptr<float>(), delta.data_ptr<float>(),
-                                             need_dq ? dq->data_ptr() : nullptr, need_dkv ? dk->data_ptr() : nullptr,
-                                             need_dkv ? dv->data_ptr() : nullptr, ecz::device_status(q.device()),
+                                             need_dq ? dq.data_ptr() : nullptr, need_dkv ? dk.data_ptr() : nullptr,
+                                             need_dkv ? dv.data_ptr() : nullptr, ecz::device_status(q.device()),
                                              stream);
   TORCH_CHECK(rc == 0, "packed_attention: backward launch failed (", rc, ")");
   return {dq, dk, dv};
@@ -388,23 +394,30 @@ Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Te
 struct PackedFunction : torch::autograd::Function<PackedFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu,
                         double scale, int64_t tiles) {
+    const int64_t B = cu.dim() == 1 ? cu.size(0) - 1 : 0;
+    if (tiles == 0 && q.dim() == 3)
+      tiles = ecz::packed_single_tiles(static_cast<int>(q.size(0)), static_cast<int>(B)) ? 1 : 2;
     auto r = packed_forward(q, k, v, cu, scale, true, tiles);
-    ctx->save_for_backward({q, k, v, std::get<0>(r), *std::get<1>(r), cu});
+    ctx->save_for_backward({q, k, v, std::get<0>(r), std::get<1>(r)});
+    ctx->saved_data["plan"] = std::get<2>(r);
+    ctx->saved_data["B"] = B;
     ctx->saved_data["scale"] = scale;
+    ctx->saved_data["tiles"] = tiles;
     return std::get<0>(r);
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("packed_attention");
     const auto s = ctx->get_saved_variables();
+    auto& data = ctx->saved_data;
     const bool need_dq = ctx->needs_input_grad(0);
     const bool need_dk = ctx->needs_input_grad(1), need_dv = ctx->needs_input_grad(2);
-    auto r = packed_backward(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["scale"].toDouble(),
-                             need_dq, need_dk || need_dv);
+    auto r = packed_backward(grads[0], s[0], s[1], s[2], s[3], s[4], data["plan"].toTensor(), data["B"].toInt(),
+                             data["scale"].toDouble(), data["tiles"].toInt(), need_dq, need_dk || need_dv);
     variable_list out(6);
-    if (need_dq) out[0] = *std::get<0>(r);
-    if (need_dk) out[1] = *std::get<1>(r);
-    if (need_dv) out[2] = *std::get<2>(r);
+    if (need_dq) out[0] = std::get<0>(r);
+    if (need_dk) out[1] = std::get<1>(r);
+    if (need_dv) out[2] = std::get<2>(r);
     return out;
   }
 };

@@ -305,39 +305,45 @@ int launch_readout_dw(const CUtensorMap* dz, const CUtensorMap* xs, const Readou
 // x and y (bf16, sizes multiples of 8) times *g in place.
 int launch_scale_by(void* x, long nx, void* y, long ny, const float* g, int num_sms, cudaStream_t stream);
 
-// packed_attention.cu: causal attention over packed sequences (see the file comment). Maps: 3-D {D, heads, T}, box
-// {64, 1, 128}, 128-byte swizzle.
+// packed_attention.cu: causal attention over packed sequences (see the file comment). A tile of queries is 128 rows: 128 >>
+// lp tokens of 1 << lp heads of a group (packed_heads_log2). Maps, 3-D {D, heads, T} with the 128-byte swizzle: q and
+// dout with boxes {64, 1 << lp, 128 >> lp}; k and v {64, 1, 128}, k32 and v32 {64, 1, 32}.
 struct PackedMaps {
-  CUtensorMap q, k, v, dout;
+  CUtensorMap q, dout, k, v, k32, v32;
+};
+// A list of tiles of `rows` tokens, heaviest first, that packed_plan_kernel writes: int4 entries [max_tiles], head [4].
+struct PackedTable {
+  void* entries = nullptr;
+  int* head = nullptr;
+  int* scratch = nullptr;  // 2 (B + 1)
+  int rows = 0, max_tiles = 0;
 };
 struct PackedArgs {
-  const void* table = nullptr;  // int4 [max_tiles] of launch_packed_plan
-  const int* head = nullptr;    // int [4]
-  int max_tiles = 0, T = 0, H = 0, Hkv = 0, D = 0, num_sms = 0;
+  PackedTable fwd, dq, dkv;  // rows: (128 >> lp) times the tiles of a CTA; 128 >> lp; 128
+  int T = 0, H = 0, Hkv = 0, D = 0, lp = 0, num_sms = 0;
   float scale = 1.f;
 };
-// Most tiles of `rows` rows that B sequences of T tokens in all can have.
+int packed_heads_log2(int H, int Hkv);
+// Most tiles of `rows` tokens that B sequences of T tokens in all can have.
 int packed_max_tiles(int T, int B, int rows);
-// scratch: 2 (B + 1) ints.
-int launch_packed_plan(const int* cu, int B, int T, int rows, int max_tiles, void* table, int* head, int* scratch,
-                       unsigned* status, cudaStream_t stream);
-// tiles: query tiles a CTA works on, 1 or 2 (packed_single_tiles: whether 1 is the better for T tokens in B sequences);
-// the table's tiles have packed_tile_rows rows.
-int packed_tile_rows(int H, int Hkv, int tiles);
+int launch_packed_plan(const int* cu, int B, int T, const PackedTable* tables, int count, unsigned* status,
+                       cudaStream_t stream);
+// tiles: query tiles a CTA works on, 1 or 2 (packed_single_tiles: whether 1 is the better for T tokens in B sequences).
 bool packed_single_tiles(int T, int B);
 int launch_packed_forward(const PackedMaps& maps, const PackedArgs& a, void* out, float* lse, int tiles,
                           unsigned* status, cudaStream_t stream);
 
 // packed_attention_bwd.cu: delta [H, T] = rows of dout . out (out contiguous [T, H, D]), then the gradients (dq null:
-// not computed; dk and dv null: not computed). The table's tiles are 128 rows.
+// not computed; dk and dv null: not computed).
 int launch_packed_delta(const void* out, const void* dout, long stride_t, long stride_h, int T, int H, int D,
                         float* delta, cudaStream_t stream);
 int launch_packed_backward(const PackedMaps& maps, const PackedArgs& a, const float* lse, const float* delta, void* dq,
                            void* dk, void* dv, unsigned* status, cudaStream_t stream);
 
-// tmap.cpp: 3-D bf16 tensor map {d, heads, tokens} with strides in elements, box {64, 1, box_tokens}, 128-byte swizzle.
+// tmap.cpp: 3-D bf16 tensor map {d, heads, tokens} with strides in elements, box {64, box_heads, box_tokens}, 128-byte
+// swizzle.
 int make_tmap_heads(CUtensorMap* map, const void* base, uint64_t tokens, uint64_t heads, uint64_t d,
-                    uint64_t token_stride, uint64_t head_stride, uint32_t box_tokens);
+                    uint64_t token_stride, uint64_t head_stride, uint32_t box_heads, uint32_t box_tokens);
 
 // tmap.cpp: a 2-D tensor map over a row-major [rows, cols] matrix of 1- or 2-byte elements (elem_bytes), with a
 // {box_cols, box_rows} box and the given swizzle (0, 32, 64 or 128 bytes). Returns 0 on success.

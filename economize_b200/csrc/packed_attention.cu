@@ -4,16 +4,17 @@
 //   o_i = sum_j exp(s_ij - L_i) v_j
 //
 // Tokens of all sequences lie one after another, q [T, H, D], k / v [T, Hkv, D]; sequence n holds the tokens
-// [cu[n], cu[n + 1]). The plan kernel cuts every sequence into tiles of 128 (or 256) rows that start at the
-// sequence's first token, so a tile never mixes sequences, and lists them heaviest first (a causal row tile's work is
-// its distance from the start): the grid's last CTAs are the short ones.
+// [cu[n], cu[n + 1]). A tile of queries is 128 rows of one sequence: (token, head) pairs of 1, 2, 4 or 8 heads of a group
+// (the largest of these that divides it) and 128, 64, 32 or 16 tokens. All heads of a pack read the same K / V chunk, a
+// short sequence fills its tiles better (85 tokens of four heads are three tiles, not four), and less of the diagonal
+// chunk is computed in vain. The plan kernel cuts every sequence into tiles from its first token on, so a tile never
+// mixes sequences, and lists them heaviest first: the last ones dealt to the persistent CTAs (see Items) are short.
 //
-// Forward CTA: two query tiles of 128 rows that share the K / V chunks: the same rows of two heads of a group (an even
-// number of heads per K/V head), else 256 rows of one head. One warp loads (TMA, a ring of 128-key K and V chunks), one
-// issues the MMAs, and two warpgroups run the softmax of a tile each, one thread per row, so the tensor cores work on
-// one tile while the other's exponentials run. CTAs are persistent (see Items). S and P share TMEM columns (P overwrites S as bf16 and is the A operand
-// of P . V), O accumulates in TMEM. A row's reference maximum moves only when a chunk raises it by more than 2^8
-// (lazy rescaling), so O is rarely read back before the end.
+// A CTA works on one or two neighbouring query tiles over the same K / V chunks. One warp loads (TMA, a ring of 128-key
+// K and V chunks), one issues the MMAs, and a warpgroup per tile runs its softmax, one thread per row, so the tensor
+// cores work on one tile while the other's exponentials run. S and P share TMEM columns (P overwrites S as bf16 and is
+// the A operand of P . V), O accumulates in TMEM. A row's reference maximum moves only when a chunk raises it by more
+// than 2^8 (lazy rescaling), so O is rarely read back before the end.
 //
 // A chunk that reaches past its sequence's end holds other rows (the next sequence's, or unwritten padding): their
 // scores are replaced, not multiplied, and the at most 15 V rows that P . V reads in its last K step beyond the end
@@ -33,11 +34,15 @@ constexpr float kLazy = 8.f;  // log2 units
 constexpr float kFar = 60.f;
 
 // ---- plan ----------------------------------------------------------------------------------------------------------
-// Tile list of `rows`-row tiles, heaviest first: table[i] = (first token, end, tile, tiles of its sequence). head =
-// (tiles, first token of the first sequence, end of the last, 0). Offsets outside [0, T] or falling are clamped (a
-// sequence starts where the one before it ended at the earliest) and reported. lo / base: [B + 1] scratch.
+// One CTA per table: a list of tiles of `rows` tokens, heaviest first: entry = (first token, end, tile, tiles of its
+// sequence); head = (tiles, first token of the first sequence, end of the last). Offsets outside [0, T] or falling are
+// clamped (a sequence starts where the one before it ended at the earliest) and reported.
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanBins = 4096;
+constexpr int kPlanTables = 3;
+
+struct PlanArgs {
+  PackedTable tables[kPlanTables];
+};
 
 __device__ __forceinline__ int scan_add(int v, int* warp_sums, int& total) {  // exclusive, over the block
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -74,17 +79,23 @@ __device__ __forceinline__ int scan_max(int v, int* warp_max) {  // inclusive
 }
 
 __global__ void __launch_bounds__(kPlanThreads)
-    packed_plan_kernel(const int* __restrict__ cu, int B, int T, int rows, int max_tiles, int4* __restrict__ table,
-                       int* __restrict__ head, int* __restrict__ lo, int* __restrict__ base, unsigned* status) {
+    packed_plan_kernel(const int* __restrict__ cu, int B, int T, const __grid_constant__ PlanArgs args,
+                       unsigned* status) {
+  // Tiles are sorted by bins of their weight (tile i reads i + 1 times as many keys as tile 0), a thread per bin:
+  // `change` counts how many tiles a bin has more than the one before, `rest` those of sequences that end in it.
+  __shared__ int change[kPlanThreads], rest[kPlanThreads];
   __shared__ int sums[32];
-  __shared__ int hist[kPlanBins];  // tiles of weight bin w, then the place of the next one
   __shared__ int carry_max, carry_tiles;
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x;
-  // weight of tile i: i + 1 chunks; bins of `per` weights each
-  const int per = (max_tiles + kPlanBins - 2) / (kPlanBins - 1);
-  for (int i = tid; i < kPlanBins; i += kPlanThreads) hist[i] = 0;
+  const PackedTable& table = args.tables[blockIdx.x];
+  int4* entries = static_cast<int4*>(table.entries);
+  const int rows = table.rows, max_tiles = table.max_tiles;
+  int *lo = table.scratch, *base = lo + B + 1;
+  const int per = (max_tiles + kPlanThreads - 2) / (kPlanThreads - 1);  // weights of a bin
+  change[tid] = 0;
+  rest[tid] = 0;
   if (tid == 0) {
     carry_max = 0;
     carry_tiles = 0;
@@ -110,37 +121,27 @@ __global__ void __launch_bounds__(kPlanThreads)
     int total;
     const int at = carry_tiles + scan_add(n, sums, total);
     if (s < B) base[s] = at;
-    // one tile of every weight 1 .. n: in bins 0 .. (n - 1) / per
-    for (int b = 0; b * per < n; ++b) atomicAdd(&hist[b], min(per, n - b * per));
+    if (n > 0) {  // `per` tiles in each of the first n / per bins, the rest in the next
+      atomicAdd(&change[0], per);
+      atomicSub(&change[n / per], per);
+      atomicAdd(&rest[n / per], n % per);
+    }
     __syncthreads();
     if (tid == 0) carry_tiles += total;
     __syncthreads();
   }
   const int tiles = min(carry_tiles, max_tiles);
   if (tid == 0) {
-    base[B] = carry_tiles;
-    head[0] = tiles;
-    head[1] = lo[0];
-    head[2] = lo[B];
+    table.head[0] = tiles;
+    table.head[1] = lo[0];
+    table.head[2] = lo[B];
   }
+  int total;
+  const int mine = scan_add(change[tid], sums, total) + change[tid] + rest[tid];
+  change[kPlanThreads - 1 - tid] = mine;  // heaviest bin first
   __syncthreads();
-  // places: heaviest bin first
-  {
-    int v[kPlanBins / kPlanThreads];
-    int mine = 0;
-#pragma unroll
-    for (int j = 0; j < kPlanBins / kPlanThreads; ++j) {
-      v[j] = hist[kPlanBins - 1 - (tid * (kPlanBins / kPlanThreads) + j)];
-      mine += v[j];
-    }
-    int total;
-    int at = scan_add(mine, sums, total);
-#pragma unroll
-    for (int j = 0; j < kPlanBins / kPlanThreads; ++j) {
-      hist[kPlanBins - 1 - (tid * (kPlanBins / kPlanThreads) + j)] = at;
-      at += v[j];
-    }
-  }
+  const int place = scan_add(change[tid], sums, total);
+  rest[kPlanThreads - 1 - tid] = place;  // of the bin's next tile
   __syncthreads();
   for (int t = tid; t < tiles; t += kPlanThreads) {
     int a = 0, b = B - 1;  // the last sequence whose first tile is t or earlier
@@ -149,8 +150,8 @@ __global__ void __launch_bounds__(kPlanThreads)
       if (base[m] <= t) a = m; else b = m - 1;
     }
     const int i = t - base[a];
-    const int at = atomicAdd(&hist[i / per], 1);
-    if (at < max_tiles) table[at] = make_int4(lo[a], lo[a + 1], i, (lo[a + 1] - lo[a] + rows - 1) / rows);
+    const int at = atomicAdd(&rest[i / per], 1);
+    if (at < max_tiles) entries[at] = make_int4(lo[a], lo[a + 1], i, (lo[a + 1] - lo[a] + rows - 1) / rows);
   }
 }
 
@@ -175,17 +176,17 @@ struct FwdCfg {
 struct FwdArgs {
   bf16* out;   // [T, H, D]
   float* lse;  // [H, T] log2-domain log-sum-exp, or null
-  const int4* table;
+  const int4* table;  // entries of kTiles query tiles
   const int* head;
-  int T, H, Hkv, D;
-  float scale2;    // scale times log2(e)
-  bool row_pairs;  // two tiles are 256 rows of one head (else 128 rows of two heads of a group)
+  int T, H, Hkv, D, lp;
+  float scale2;  // scale times log2(e)
 };
 
 template <int DP, int kTiles>
 __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
     packed_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FwdArgs p, unsigned* status) {
+                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_k32,
+                      const __grid_constant__ CUtensorMap tm_v32, const __grid_constant__ FwdArgs p, unsigned* status) {
   using Cfg = FwdCfg<DP, kTiles>;
   constexpr int kRing = Cfg::kRing, kTileBytes = Cfg::kTileBytes;
   constexpr int kLoadWarp = Cfg::kSoftmaxWarps, kMmaWarp = kLoadWarp + 1;
@@ -236,17 +237,17 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
   zero_padding(p.out, p.T, static_cast<long>(p.H) * p.D, p.head);
   const int group = p.H / p.Hkv;
   const int ksteps = (p.D + 15) / 16;
-  const bool row_pairs = kTiles == 1 || p.row_pairs;
-  const int per = row_pairs ? p.H : p.H / 2;
-  // an item's query tile i: its head, first row and number of key chunks (the last one holds the diagonal)
-  auto head_of = [&](const auto& items, int i) { return row_pairs ? items.sub : 2 * items.sub + i; };
-  auto row_of = [&](const auto& items, int i) {
-    return items.tile.x + (row_pairs ? (items.tile.z * kTiles + i) * kRowsT : items.tile.z * kRowsT);
-  };
+  const int tokens = kRowsT >> p.lp;  // of a query tile
+  const int per = p.H >> p.lp;        // items of a table entry: one for every 1 << lp heads
+  // an item's query tile i: its first token, its number of key chunks (the last one holds the diagonal), and the keys it
+  // needs of chunk c
+  auto token_of = [&](const auto& items, int i) { return items.tile.x + (items.tile.z * kTiles + i) * tokens; };
   auto chunks_of = [&](const auto& items, int i) {
-    const int row = row_of(items, i);
-    if (i >= kTiles) return 0;
-    return row < items.tile.y ? (row - items.tile.x) / kRowsT + 1 : 0;
+    const int first = token_of(items, i);
+    return i < kTiles && first < items.tile.y ? (first - items.tile.x) / kRowsT + 1 : 0;
+  };
+  auto keys_of = [&](const auto& items, int i, int c) {
+    return min(kRowsT, min(items.tile.y, token_of(items, i) + tokens) - (items.tile.x + c * kRowsT));
   };
 
   if (warp == kLoadWarp) {
@@ -256,23 +257,24 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
     int it = 0;
     bool ok = true;
     for (int n_items = 0; ok && items.next(); ++n_items) {
-      const int lo = items.tile.x, c1 = chunks_of(items, 1), n = max(chunks_of(items, 0), c1), kvh = head_of(items, 0) / group;
-      const int head0 = head_of(items, 0), head1 = head_of(items, 1), row0 = row_of(items, 0), row1 = row_of(items, 1);
+      const int lo = items.tile.x, c1 = chunks_of(items, 1), n = max(chunks_of(items, 0), c1);
+      const int head = items.sub << p.lp, kvh = head / group;
+      const int first = token_of(items, 0), last_keys = keys_of(items, c1 > 0 ? 1 : 0, n - 1);
       items.look();
       if (lane == 0) {
         auto chunk = [&](int x) {  // K (even) or V (odd) of a chunk
-          const int s = (it + x) % kRing;
+          const int s = (it + x) % kRing, c = x >> 1;
           if (!mbar_wait(&kv_empty[s], (((it + x) / kRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag)) return false;
-          mbar_arrive_expect_tx(&kv_full[s], kTileBytes);
-          load_tile<DP>(ra + s * kTileBytes, (x & 1) ? &tm_v : &tm_k, &kv_full[s], kvh, lo + (x >> 1) * kRowsT);
+          load_chunk<DP>(ra + s * kTileBytes, (x & 1) ? &tm_v : &tm_k, (x & 1) ? &tm_v32 : &tm_k32, &kv_full[s], kvh,
+                         lo + c * kRowsT, c + 1 < n ? kRowsT : last_keys);
           return true;
         };
         // the first K does not wait for the previous item's queries to be read, nor the queries for its last V
         ok = chunk(0) && mbar_wait(q_empty, (n_items & 1) ^ 1, status, kStatusWaitEmpty, abort_flag);
         if (ok) {
           mbar_arrive_expect_tx(q_full, (c1 > 0 ? 2 : 1) * kTileBytes);
-          load_tile<DP>(qa, &tm_q, q_full, head0, row0);
-          if (c1 > 0) load_tile<DP>(qa + kTileBytes, &tm_q, q_full, head1, row1);
+          load_tile<DP>(qa, &tm_q, q_full, head, first);
+          if (c1 > 0) load_tile<DP>(qa + kTileBytes, &tm_q, q_full, head, first + tokens);
         }
         for (int x = 1; ok && x < 2 * n; ++x) ok = chunk(x);
       }
@@ -291,18 +293,21 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
       return warp_wait(&kv_full[it % kRing], (it / kRing) & 1, status, kStatusWaitFull, abort_flag);
     };
     for (int n_items = 0; ok && items.next(); ++n_items) {
-      const int lo = items.tile.x, hi = items.tile.y;
       const int chunks[2] = {chunks_of(items, 0), chunks_of(items, 1)};
       const int n_chunks = max(chunks[0], chunks[1]);
-      auto keys_of = [&](int c) { return min(kRowsT, hi - (lo + c * kRowsT)); };
+      const int left = items.tile.y - items.tile.x;  // keys of the sequence
+      const int first0 = token_of(items, 0) - items.tile.x;
+      // columns of S and rows of V that tile i takes of chunk c, in steps of 16
+      auto width = [&](int i, int c) {
+        return (min(kRowsT, min(left, first0 + (i + 1) * tokens) - c * kRowsT) + 15) & ~15;
+      };
       ok = warp_wait(q_full, n_items & 1, status, kStatusWaitFull, abort_flag) && wait_ring(base);
       if (!ok) break;
       tc_fence_after();
       if (leader) {
-        const int n = (keys_of(0) + 15) & ~15;
         for (int i = 0; i < kTiles; ++i) {
           if (chunks[i] == 0) continue;
-          mma_dims<DP>(tmem + i * 128, qa + i * kTileBytes, ra + (base % kRing) * kTileBytes, n, ksteps);
+          mma_dims<DP>(tmem + i * 128, qa + i * kTileBytes, ra + (base % kRing) * kTileBytes, width(i, 0), ksteps);
           umma_commit(&s_full[i]);
         }
         umma_commit(&kv_empty[base % kRing]);
@@ -315,27 +320,32 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
         const bool more = c + 1 < n_chunks;
         ok = wait_ring(v_it) && (!more || wait_ring(k_it));
         if (!ok) break;
-        const int n = keys_of(c), n16 = (n + 15) & ~15;
         uint8_t* v_tile = ring + (v_it % kRing) * kTileBytes;
-        if (n16 != n) zero_rows<DP>(v_tile, n, n16, lane);
+        if (!more) {  // rows past the sequence's end that a K step of P . V reads
+          const int keys = left - c * kRowsT, widest = width(chunks[1] > 0 ? 1 : 0, c);
+          if (keys < widest) zero_rows<DP>(v_tile, keys, widest, lane);
+        }
         for (int i = 0; ok && i < kTiles; ++i) {
           if (c >= chunks[i]) continue;
           // the first half of P . V runs under the exponentials of the second
           ok = warp_wait(&p_ready[2 * i], (used[i] + c) & 1, status, kStatusWaitAccum, abort_flag);
           if (!ok) break;
           tc_fence_after();
+          const int vsteps = width(i, c) / 16;
           if (leader)
-            mma_rows<8, 64, 0, 4>(tmem + kTiles * 128 + i * DP, tmem + i * 128, smem_u32(v_tile), ksteps * 16, n16 / 16, c > 0);
+            mma_rows<8, 64, 0, 4>(tmem + kTiles * 128 + i * DP, tmem + i * 128, smem_u32(v_tile), ksteps * 16, vsteps,
+                                  c > 0);
           __syncwarp();
           ok = warp_wait(&p_ready[2 * i + 1], (used[i] + c) & 1, status, kStatusWaitAccum, abort_flag);
           if (!ok) break;
           tc_fence_after();
           if (leader) {
-            mma_rows<8, 64, 4, 8>(tmem + kTiles * 128 + i * DP, tmem + i * 128, smem_u32(v_tile), ksteps * 16, n16 / 16, true);
+            mma_rows<8, 64, 4, 8>(tmem + kTiles * 128 + i * DP, tmem + i * 128, smem_u32(v_tile), ksteps * 16, vsteps,
+                                  true);
             umma_commit(&o_done[i]);
             if (c + 1 < chunks[i]) {
-              mma_dims<DP>(tmem + i * 128, qa + i * kTileBytes, ra + (k_it % kRing) * kTileBytes,
-                           (keys_of(c + 1) + 15) & ~15, ksteps);
+              mma_dims<DP>(tmem + i * 128, qa + i * kTileBytes, ra + (k_it % kRing) * kTileBytes, width(i, c + 1),
+                           ksteps);
               umma_commit(&s_full[i]);
             }
           }
@@ -361,9 +371,8 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
     uint32_t used = 0;  // chunks of this tile so far, over all items
     bool ok = true;
     while (ok && items.next()) {
-      const int lo = items.tile.x, hi = items.tile.y;
-      const int n_mine = chunks_of(items, i), my_head = head_of(items, i);
-      const int row0 = row_of(items, i) + quad * 32, row = row0 + lane;
+      const int n_mine = chunks_of(items, i);
+      const int first = token_of(items, i), token = first + ((quad * 32 + lane) >> p.lp);
       // Exponentials are taken against a reference that is settled beforehand (0 for a row's first chunk): the chunk's
       // maximum is reduced beside them, and only where it lies more than kLazy above (or far below, in the first chunk,
       // where small sums would underflow) does the row take it as its reference and repeat.
@@ -374,8 +383,10 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
         tc_fence_after();
         float v[128];
         tmem_load128(s_addr, v);
+        int blocks = 4;           // of 32 columns, that hold scores
         if (c == n_mine - 1) {  // the diagonal and the sequence's end
-          const int limit = min(hi, row + 1) - (lo + c * kRowsT);
+          const int limit = min(items.tile.y, token + 1) - (items.tile.x + c * kRowsT);
+          blocks = (keys_of(items, i, c) + 31) >> 5;
 #pragma unroll
           for (int h = 0; h < 4; ++h) {
             const uint32_t bits = low_bits(limit - h * 32);
@@ -391,6 +402,7 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
           uint64_t a = 0, b = 0;
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
+            if (h * 2 + q >= blocks) break;
             uint32_t w[16];
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
@@ -459,12 +471,14 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
         if (!ok) break;
         tc_fence_after();
         const float inv = 1.f / sum;
-        if (row < hi && p.lse != nullptr) p.lse[static_cast<long>(my_head) * p.T + row] = ref + log2f(sum);
-        const long stride = static_cast<long>(p.H) * p.D;
-        bf16* dst = p.out + row0 * stride + static_cast<long>(my_head) * p.D;
+        const int head = items.sub << p.lp;
+        if (token < items.tile.y && p.lse != nullptr)
+          p.lse[static_cast<long>(head + (lane & ((1 << p.lp) - 1))) * p.T + token] = ref + log2f(sum);
+        TileOut to{p.out + (static_cast<long>(first) * p.H + head) * p.D, static_cast<long>(p.H) * p.D, p.D, p.lp,
+                   (items.tile.y - first) << p.lp, p.D};
 #pragma unroll 1
-        for (int d = 0; d < p.D; d += 64)
-          stage_tmem64(o_addr + d, inv, stages + warp * 4096, dst + d, stride, hi - row0, p.D - d, lane);
+        for (int d = 0; d < p.D; d += 64, to.dst += 64, to.cols -= 64)
+          stage_tmem64(o_addr + d, inv, stages + warp * 4096, to, quad * 32, lane);
         tc_fence_before();  // the next item's first P . V overwrites O after this warp's next p_ready
       }
     }
@@ -482,14 +496,13 @@ int run_fwd(const PackedMaps& maps, const PackedArgs& a, void* out, float* lse, 
   using Cfg = FwdCfg<DP, kTiles>;
   auto kernel = packed_fwd_kernel<DP, kTiles>;
   if (set_max_smem(kernel, Cfg::kSmem) != cudaSuccess) return -1;
-  const bool row_pairs = kTiles == 1 || packed_tile_rows(a.H, a.Hkv, kTiles) == 256;
-  const FwdArgs args{static_cast<bf16*>(out), lse, static_cast<const int4*>(a.table), a.head, a.T, a.H, a.Hkv, a.D,
-                     a.scale * kLog2e, row_pairs};
-  const long most = static_cast<long>(a.max_tiles) * (row_pairs ? a.H : a.H / 2);
+  const FwdArgs args{static_cast<bf16*>(out), lse, static_cast<const int4*>(a.fwd.entries), a.fwd.head, a.T, a.H,
+                     a.Hkv, a.D, a.lp, a.scale * kLog2e};
+  const long most = static_cast<long>(a.fwd.max_tiles) * (a.H >> a.lp);
   if (most > 0x7fff0000l) return -2;
   const long grid = std::min(most, static_cast<long>(a.num_sms) * (3 - kTiles));
   return launch_pdl(kernel, dim3(static_cast<unsigned>(grid)), dim3(Cfg::kThreads), Cfg::kSmem, stream, maps.q, maps.k,
-                    maps.v, args, status) == cudaSuccess ? 0 : -1;
+                    maps.v, maps.k32, maps.v32, args, status) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace
@@ -498,13 +511,20 @@ int packed_max_tiles(int T, int B, int rows) {
   return static_cast<int>(std::min<long>(T, static_cast<long>(T) / rows + B));
 }
 
-int launch_packed_plan(const int* cu, int B, int T, int rows, int max_tiles, void* table, int* head, int* scratch,
-                       unsigned* status, cudaStream_t stream) {
-  return launch_pdl(packed_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, cu, B, T, rows, max_tiles,
-                    static_cast<int4*>(table), head, scratch, scratch + B + 1, status) == cudaSuccess ? 0 : -1;
+int packed_heads_log2(int H, int Hkv) {
+  int lp = 0;
+  while (lp < 3 && (H / Hkv) % (2 << lp) == 0) ++lp;
+  return lp;
 }
 
-int packed_tile_rows(int H, int Hkv, int tiles) { return tiles == 2 && (H / Hkv) % 2 != 0 ? 256 : 128; }
+int launch_packed_plan(const int* cu, int B, int T, const PackedTable* tables, int count, unsigned* status,
+                       cudaStream_t stream) {
+  if (count < 1 || count > kPlanTables) return -2;
+  PlanArgs args;
+  for (int i = 0; i < count; ++i) args.tables[i] = tables[i];
+  return launch_pdl(packed_plan_kernel, dim3(count), dim3(kPlanThreads), 0, stream, cu, B, T, args, status) ==
+                 cudaSuccess ? 0 : -1;
+}
 
 bool packed_single_tiles(int T, int B) { return static_cast<long>(T) < 512l * B; }
 

@@ -32,9 +32,9 @@ constexpr int kBwdThreads = 128 + 32 * kComputeWarps;
 struct BwdArgs {
   bf16 *dq, *dk, *dv;
   const float *lse, *delta;  // [H, T]
-  const int4* table;
-  const int* head;
-  int T, H, Hkv, D;
+  const int4 *dq_table, *dkv_table;  // tiles of queries, tiles of 128 keys
+  const int *dq_head, *dkv_head;
+  int T, H, Hkv, D, lp;
   float scale, scale2;
 };
 
@@ -89,19 +89,20 @@ struct Stream {
   __device__ __forceinline__ uint32_t use(int item) const { return (item / kRing) & 1; }
 };
 
-// The query tiles of a key tile in order: `tiles` of one head, then the next head's. Counters instead of a division of
-// the iteration: that took the issuing warp a tenth of a tile's time.
+// The query tiles that see a key tile, in order: `tiles` of one pack of heads, then the next pack's. Counters instead of
+// a division of the iteration: that took the issuing warp a tenth of a tile's time.
 struct Walk {
-  int head, row;  // query head, first token of the tile
-  int left, tiles, row0;
-  __device__ __forceinline__ Walk(int first_head, int first_row, int n)
-      : head(first_head), row(first_row), left(n), tiles(n), row0(first_row) {}
+  int head, token;  // first head of the pack, first token of the tile
+  int left, tiles, token0, tokens, heads;
+  __device__ __forceinline__ Walk(int first_head, int first_token, int n, int lp)
+      : head(first_head), token(first_token), left(n), tiles(n), token0(first_token), tokens(kRowsT >> lp),
+        heads(1 << lp) {}
   __device__ __forceinline__ void next() {
-    row += kRowsT;
+    token += tokens;
     if (--left == 0) {
       left = tiles;
-      row = row0;
-      ++head;
+      token = token0;
+      head += heads;
     }
   }
 };
@@ -161,27 +162,28 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   pdl_trigger();
   pdl_wait();
 
-  zero_padding(p.dk, p.T, static_cast<long>(p.Hkv) * p.D, p.head);
-  zero_padding(p.dv, p.T, static_cast<long>(p.Hkv) * p.D, p.head);
-  Items<> items(p.table, p.head, p.Hkv);  // sub: the K/V head
+  zero_padding(p.dk, p.T, static_cast<long>(p.Hkv) * p.D, p.dkv_head);
+  zero_padding(p.dv, p.T, static_cast<long>(p.Hkv) * p.D, p.dkv_head);
+  Items<> items(p.dkv_table, p.dkv_head, p.Hkv);  // sub: the K/V head
   const int group = p.H / p.Hkv;
   const int ksteps = (p.D + 15) / 16;
-  // an item's query tiles (as many as the entry weighs, from the tile of keys on) and its first token
-  auto tiles_of = [&]() { return items.tile.z + 1; };
+  const int tokens = kRowsT >> p.lp, packs = group >> p.lp;
+  // an item's first key (the entry's weight counts from the sequence's end) and the query tiles that see it
   auto key0_of = [&]() { return items.tile.x + (items.tile.w - items.tile.z - 1) * kRowsT; };
+  auto tiles_of = [&]() { return (items.tile.y - key0_of() + tokens - 1) / tokens; };
 
   if (warp == 0) {
     int x = 0;  // ring item
     bool ok = true;
     for (int n_items = 0; ok && items.next(); ++n_items) {
-      const int n_q = tiles_of(), key0 = key0_of(), kvh = items.sub, total = group * n_q;
+      const int n_q = tiles_of(), key0 = key0_of(), kvh = items.sub, total = packs * n_q;
       items.look();
       if (lane == 0) {
-        Walk at(kvh * group, key0, n_q);
+        Walk at(kvh * group, key0, n_q, p.lp);
         auto load = [&](int i) {  // Q (even) or dO (odd) of an iteration
           if (!mbar_wait(ring.empty_of(x + i), ring.use(x + i) ^ 1, status, kStatusWaitEmpty, abort_flag)) return false;
           mbar_arrive_expect_tx(ring.full_of(x + i), kTileBytes);
-          load_tile<DP>(smem_u32(ring.tile(x + i)), (i & 1) ? &tm_do : &tm_q, ring.full_of(x + i), at.head, at.row);
+          load_tile<DP>(smem_u32(ring.tile(x + i)), (i & 1) ? &tm_do : &tm_q, ring.full_of(x + i), at.head, at.token);
           if (i & 1) at.next();
           return true;
         };
@@ -203,17 +205,19 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     int base = 0;  // iterations before the item
     bool ok = true;
     for (int n_items = 0; ok && items.next(); ++n_items) {
-      const int hi = items.tile.y, n_q = tiles_of(), key0 = key0_of(), kvh = items.sub, total = group * n_q;
-      // ring item x, of the query tile at `row`, is in shared memory and its rows past the sequence's end are zeroed
-      auto ready = [&](int x, int row) {
+      const int hi = items.tile.y, n_q = tiles_of(), key0 = key0_of(), kvh = items.sub, total = packs * n_q;
+      // rows of the query tile at `token`, all 128 or up to the sequence's end
+      auto rows_of = [&](int token) { return min(kRowsT, (hi - token) << p.lp); };
+      // ring item x, of the query tile at `token`, is in shared memory and its rows past the sequence's end are zeroed
+      auto ready = [&](int x, int token) {
         if (!warp_wait(ring.full_of(x), ring.use(x), status, kStatusWaitFull, abort_flag)) return false;
-        const int n = min(kRowsT, hi - row), n16 = (n + 15) & ~15;
+        const int n = rows_of(token), n16 = (n + 15) & ~15;
         if (n != n16) zero_rows<DP>(ring.tile(x), n, n16, lane);
         return true;
       };
-      Walk at(kvh * group, key0, n_q);
-      int rows16 = (min(kRowsT, hi - at.row) + 15) & ~15;  // of the current iteration's query tile
-      ok = ready(2 * base, at.row) && ready(2 * base + 1, at.row) &&
+      Walk at(kvh * group, key0, n_q, p.lp);
+      int rows16 = (rows_of(at.token) + 15) & ~15;  // of the current iteration's query tile
+      ok = ready(2 * base, at.token) && ready(2 * base + 1, at.token) &&
            warp_wait(kv_full, n_items & 1, status, kStatusWaitFull, abort_flag);
       tc_fence_after();
       if (ok && leader) {
@@ -229,8 +233,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const bool more = it + 1 < base + total;
         const int xq = 2 * it, xd = xq + 1;
         at.next();
-        const int next16 = (min(kRowsT, hi - at.row) + 15) & ~15;
-        if (more) ok = ready(xq + 2, at.row);
+        const int next16 = (rows_of(at.token) + 15) & ~15;
+        if (more) ok = ready(xq + 2, at.token);
         ok = ok && warp_wait(p_ready, it & 1, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
@@ -243,7 +247,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           }
         }
         __syncwarp();
-        if (more) ok = ready(xd + 2, at.row);
+        if (more) ok = ready(xd + 2, at.token);
         ok = ok && warp_wait(ds_ready, it & 1, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
@@ -268,20 +272,20 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     int base = 0;
     bool ok = true;
     while (ok && items.next()) {
-      const int hi = items.tile.y, n_q = tiles_of(), total = group * n_q;
-      Walk at(items.sub * group, key0_of(), n_q);
+      const int hi = items.tile.y, n_q = tiles_of(), total = packs * n_q;
+      Walk at(items.sub * group, key0_of(), n_q, p.lp);
       items.look();
       for (int it = base; it < base + total; ++it, at.next()) {
         const int s = it % kStatRing;
         ok = warp_wait(&st_empty[s], ((it / kStatRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag);
         if (!ok) break;
-        const long first = static_cast<long>(at.head) * p.T;
         float* dst = stats + s * 256;
 #pragma unroll
         for (int j = lane; j < kRowsT; j += 32) {
-          const int row = at.row + j;
-          dst[j] = row < hi ? p.lse[first + row] : 0.f;
-          dst[128 + j] = row < hi ? p.delta[first + row] : 0.f;
+          const int token = at.token + (j >> p.lp);
+          const long from = static_cast<long>(at.head + (j & ((1 << p.lp) - 1))) * p.T + token;
+          dst[j] = token < hi ? p.lse[from] : 0.f;
+          dst[128 + j] = token < hi ? p.delta[from] : 0.f;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&st_full[s]);
@@ -297,9 +301,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     int base = 0;
     bool ok = true;
     for (int n_items = 0; ok && items.next(); ++n_items) {
-      const int hi = items.tile.y, n_q = tiles_of(), key0 = key0_of(), kvh = items.sub, total = group * n_q;
+      const int hi = items.tile.y, n_q = tiles_of(), key0 = key0_of(), kvh = items.sub, total = packs * n_q;
       items.look();
-      Walk at(kvh * group, key0, n_q);
+      Walk at(kvh * group, key0, n_q, p.lp);
       for (int it = base; it < base + total; ++it, at.next()) {
         const int s = it % kStatRing;
         const float* lse = stats + s * 256 + part * 32;
@@ -310,10 +314,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_fence_after();
         float v[32];
         tmem_load32(s_addr, v);
-        // queries [from, to) of this part see the key
-        const bool diagonal = at.row == key0;
-        const int from = diagonal ? key - part * 32 : 0, to = hi - at.row - part * 32;
-        const bool masked = diagonal || to < 32;
+        // rows [from, to) of this part see the key: from its own token on, up to the sequence's end
+        const int from = ((key0 + key - at.token) << p.lp) - part * 32, to = ((hi - at.token) << p.lp) - part * 32;
+        const bool masked = at.token < key0 + kRowsT || to < 32;
         const uint32_t seen = low_bits(to) & ~low_bits(from);
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
@@ -367,12 +370,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       ok = ok && warp_wait(done, n_items & 1, status, kStatusWaitAccum, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      const int col = (part & 1) * 64, row0 = key0 + quad * 32;
+      const int col = (part & 1) * 64;
       if (col < p.D) {
-        const long stride = static_cast<long>(p.Hkv) * p.D, at0 = row0 * stride + static_cast<long>(kvh) * p.D + col;
         const bool values = part < 2;
-        store_tmem64((values ? t_dv : t_dk) + lane_base + col, values ? 1.f : p.scale, (values ? p.dv : p.dk) + at0,
-                     stride, hi - row0, p.D - col, lane);
+        const long stride = static_cast<long>(p.Hkv) * p.D;
+        const TileOut to{(values ? p.dv : p.dk) + key0 * stride + static_cast<long>(kvh) * p.D + col, stride, 0, 0,
+                         hi - key0, p.D - col};
+        store_tmem64((values ? t_dv : t_dk) + lane_base + col, values ? 1.f : p.scale, to, quad * 32, lane);
       }
       tc_fence_before();  // the next item's first dV overwrites this one's after this warp's next p_ready
     }
@@ -391,9 +395,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 template <bool kAhead>
 struct ChunkWalk {
   Items<kAhead> items;
-  int chunk, n, k, item;
+  int chunk, n, k, item, lp;
   bool valid;
-  __device__ __forceinline__ ChunkWalk(const int4* table, const int* head, int per) : items(table, head, per), k(0), item(-1) {
+  __device__ __forceinline__ ChunkWalk(const BwdArgs& p)
+      : items(p.dq_table, p.dq_head, p.H >> p.lp), k(0), item(-1), lp(p.lp) {
     take();
   }
   __device__ __forceinline__ void take() {
@@ -401,7 +406,7 @@ struct ChunkWalk {
     chunk = 0;
     ++item;
     if (!valid) return;
-    n = items.tile.z + 1;  // key chunks, the last one on the diagonal
+    n = items.tile.z * (kRowsT >> lp) / kRowsT + 1;  // key chunks, the last one on the diagonal
     if (kAhead) items.look();
   }
   __device__ __forceinline__ void step() {
@@ -412,16 +417,20 @@ struct ChunkWalk {
   __device__ __forceinline__ bool last() const { return chunk + 1 == n; }
   __device__ __forceinline__ int lo() const { return items.tile.x; }
   __device__ __forceinline__ int hi() const { return items.tile.y; }
-  __device__ __forceinline__ int row0() const { return items.tile.x + (n - 1) * kRowsT; }
-  __device__ __forceinline__ int head() const { return items.sub; }
-  __device__ __forceinline__ int keys() const { return min(kRowsT, hi() - (lo() + chunk * kRowsT)); }
-  __device__ __forceinline__ int keys16() const { return (keys() + 15) & ~15; }
+  __device__ __forceinline__ int token() const { return items.tile.x + items.tile.z * (kRowsT >> lp); }
+  __device__ __forceinline__ int head() const { return items.sub << lp; }
+  // keys of the sequence from the chunk on, and those the tile needs of it, in steps of 16
+  __device__ __forceinline__ int keys() const { return hi() - (lo() + chunk * kRowsT); }
+  __device__ __forceinline__ int width() const {
+    return (min(kRowsT, min(hi(), token() + (kRowsT >> lp)) - (lo() + chunk * kRowsT)) + 15) & ~15;
+  }
 };
 
 template <int DP>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     packed_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
+                     const __grid_constant__ CUtensorMap tm_k32, const __grid_constant__ CUtensorMap tm_v32,
                      const __grid_constant__ BwdArgs p, unsigned* status) {
   using Cfg = BwdCfg<DP>;
   constexpr int kRing = Cfg::kRing, kTileBytes = Cfg::kTileBytes;
@@ -476,35 +485,35 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   pdl_trigger();
   pdl_wait();
 
-  zero_padding(p.dq, p.T, static_cast<long>(p.H) * p.D, p.head);
+  zero_padding(p.dq, p.T, static_cast<long>(p.H) * p.D, p.dq_head);
   const int group = p.H / p.Hkv;
   const int ksteps = (p.D + 15) / 16;
 
   if (warp == 0) {
-    Items<> items(p.table, p.head, p.H);
+    ChunkWalk<true> at(p);
     int x = 0;  // ring item
     bool ok = true;
-    for (int n_items = 0; ok && items.next(); ++n_items) {
-      const int lo = items.tile.x, n = items.tile.z + 1, head = items.sub, kvh = head / group;
-      items.look();
+    for (int n_items = 0; ok && at.valid; ++n_items) {
+      const int lo = at.lo(), n = at.n, head = at.head(), kvh = head / group, token = at.token();
+      const int last = min(at.hi(), token + (kRowsT >> p.lp)) - (lo + (n - 1) * kRowsT);  // keys of the last chunk
+      at.take();
       if (lane == 0) {
         auto load = [&](int i) {  // K (even) or V (odd) of a chunk
           if (!mbar_wait(ring.empty_of(x + i), ring.use(x + i) ^ 1, status, kStatusWaitEmpty, abort_flag)) return false;
-          mbar_arrive_expect_tx(ring.full_of(x + i), kTileBytes);
-          load_tile<DP>(smem_u32(ring.tile(x + i)), (i & 1) ? &tm_v : &tm_k, ring.full_of(x + i), kvh,
-                        lo + (i >> 1) * kRowsT);
+          load_chunk<DP>(smem_u32(ring.tile(x + i)), (i & 1) ? &tm_v : &tm_k, (i & 1) ? &tm_v32 : &tm_k32,
+                         ring.full_of(x + i), kvh, lo + (i >> 1) * kRowsT, (i >> 1) + 1 < n ? kRowsT : last);
           return true;
         };
         const uint32_t turn = (n_items & 1) ^ 1;
         ok = load(0) && mbar_wait(q_empty, turn, status, kStatusWaitEmpty, abort_flag);
         if (ok) {
           mbar_arrive_expect_tx(q_full, kTileBytes);
-          load_tile<DP>(smem_u32(q_tile), &tm_q, q_full, head, lo + (n - 1) * kRowsT);
+          load_tile<DP>(smem_u32(q_tile), &tm_q, q_full, head, token);
         }
         ok = ok && load(1) && mbar_wait(do_empty, turn, status, kStatusWaitEmpty, abort_flag);
         if (ok) {
           mbar_arrive_expect_tx(do_full, kTileBytes);
-          load_tile<DP>(smem_u32(do_tile), &tm_do, do_full, head, lo + (n - 1) * kRowsT);
+          load_tile<DP>(smem_u32(do_tile), &tm_do, do_full, head, token);
         }
         for (int i = 2; ok && i < 2 * n; ++i) ok = load(i);
       }
@@ -519,10 +528,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (a.first() && !warp_wait(q_full, a.item & 1, status, kStatusWaitFull, abort_flag)) return false;
       const int x = 2 * a.k;
       if (!warp_wait(ring.full_of(x), ring.use(x), status, kStatusWaitFull, abort_flag)) return false;
-      if (a.keys() != a.keys16()) zero_rows<DP>(ring.tile(x), a.keys(), a.keys16(), lane);
+      if (a.keys() < a.width()) zero_rows<DP>(ring.tile(x), a.keys(), a.width(), lane);
       tc_fence_after();
       if (leader) {
-        mma_dims<DP>(t_s + (a.k & 1) * 128, qa, smem_u32(ring.tile(x)), a.keys16(), ksteps);
+        mma_dims<DP>(t_s + (a.k & 1) * 128, qa, smem_u32(ring.tile(x)), a.width(), ksteps);
         umma_commit(&s_full[a.k & 1]);
         if (a.last()) umma_commit(q_empty);
       }
@@ -530,7 +539,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       a.step();
       return true;
     };
-    auto products = [&](ChunkWalk<true>& b) {  // dP of a chunk once the one before is in registers; the only use of its V
+    auto products = [&](ChunkWalk<false>& b) {  // dP of a chunk once the one before is in registers; the only use of its V
       if (!b.valid) return true;
       const int x = 2 * b.k + 1, before = b.k - 1;
       if (b.first() && !warp_wait(do_full, b.item & 1, status, kStatusWaitFull, abort_flag)) return false;
@@ -539,7 +548,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         return false;
       tc_fence_after();
       if (leader) {
-        mma_dims<DP>(t_dp, da, smem_u32(ring.tile(x)), b.keys16(), ksteps);
+        mma_dims<DP>(t_dp, da, smem_u32(ring.tile(x)), b.width(), ksteps);
         umma_commit(&dp_full[b.k & 1]);
         umma_commit(ring.empty_of(x));
         if (b.last()) umma_commit(do_empty);
@@ -548,7 +557,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       b.step();
       return true;
     };
-    ChunkWalk<true> a(p.table, p.head, p.H), b = a, c = a;
+    ChunkWalk<true> a(p);
+    ChunkWalk<false> b(p), c(p);  // their table entries are in the cache by then
     bool ok = scores(a) && products(b) && scores(a);
     while (ok && c.valid) {
       ok = products(b) && warp_wait(&ds_ready[c.k & 1], (c.k >> 1) & 1, status, kStatusWaitAccum, abort_flag);
@@ -558,7 +568,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       tc_fence_after();
       if (leader) {
         const int x = 2 * c.k;
-        mma_rows<4, 64>(t_dq, t_s + (c.k & 1) * 128, smem_u32(ring.tile(x)), ksteps * 16, c.keys16() / 16, !c.first());
+        mma_rows<4, 64>(t_dq, t_s + (c.k & 1) * 128, smem_u32(ring.tile(x)), ksteps * 16, c.width() / 16, !c.first());
         umma_commit(ring.empty_of(x));
         if (c.last()) umma_commit(&dq_full[c.item & 1]);
       }
@@ -574,18 +584,19 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int mine = part >> 1, half = part & 1;
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t s_addr = t_s + mine * 128 + lane_base + half * 64, dp_addr = t_dp + lane_base + half * 64;
-    ChunkWalk<false> at(p.table, p.head, p.H);
+    ChunkWalk<false> at(p);
     if (mine == 1 && at.valid) at.step();
     bool ok = true;
     while (ok && at.valid) {
       const uint32_t use = (at.k >> 1) & 1;
-      const int row0 = at.row0() + quad * 32, row = row0 + lane, hi = at.hi();
+      const int first = at.token(), token = first + ((quad * 32 + lane) >> p.lp), hi = at.hi();
       const bool last = at.last();
-      const int limit = min(hi, row + 1) - (at.lo() + at.chunk * kRowsT) - half * 64;  // visible keys, of the last chunk
+      const int limit = min(hi, token + 1) - (at.lo() + at.chunk * kRowsT) - half * 64;  // visible keys, last chunk
       float lse = 0.f, delta = 0.f;
-      if (row < hi) {
-        lse = p.lse[static_cast<long>(at.head()) * p.T + row];
-        delta = p.delta[static_cast<long>(at.head()) * p.T + row];
+      if (token < hi) {
+        const long from = static_cast<long>(at.head() + (lane & ((1 << p.lp) - 1))) * p.T + token;
+        lse = p.lse[from];
+        delta = p.delta[from];
       }
       ok = warp_wait(&s_full[mine], use, status, kStatusWaitAccum, abort_flag);
       if (!ok) break;
@@ -603,10 +614,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       ok = warp_wait(&dp_full[mine], use, status, kStatusWaitAccum, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      float g[32];
-      uint32_t w[32];
 #pragma unroll
-      for (int h = 0; h < 64; h += 32) {
+      for (int h = 0; h < 64; h += 32) {  // dS of a half lies where its P has been read
+        float g[32];
+        uint32_t w[16];
         tmem_load32(s_addr + h, v);
         tmem_load32(dp_addr + h, g);
 #pragma unroll
@@ -617,12 +628,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           for (int j = 0; j < 32; ++j) g[j] = (seen >> j) & 1u ? g[j] : 0.f;
         }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) w[h / 2 + j] = pack_bf16(g[2 * j], g[2 * j + 1]);
+        for (int j = 0; j < 16; ++j) w[j] = pack_bf16(g[2 * j], g[2 * j + 1]);
+        if (h == 32) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&dp_free[mine]);
+        }
+        tmem_st_u32x16(s_addr + h / 2, w);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&dp_free[mine]);
-      tmem_store32(s_addr, w);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -640,9 +653,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(dq_free);
-        if (col < p.D)
-          store_rows64(c, p.dq + (static_cast<long>(row0) * p.H + head) * p.D + col, static_cast<long>(p.H) * p.D,
-                       hi - row0, p.D - col, lane);
+        if (col < p.D) {
+          const TileOut to{p.dq + (static_cast<long>(first) * p.H + head) * p.D + col, static_cast<long>(p.H) * p.D, p.D,
+                           p.lp, (hi - first) << p.lp, p.D - col};
+          store_rows64(c, to, quad * 32, lane);
+        }
       }
     }
   }
@@ -656,10 +671,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 template <int DP>
 int run_bwd(const PackedMaps& m, const PackedArgs& a, const BwdArgs& args, bool want_dq, bool want_dkv,
             unsigned* status, cudaStream_t stream) {
-  const long items = static_cast<long>(a.max_tiles) * a.H;
-  if (items > 0x7fff0000l) return -2;
-  const long grid_kv = std::min(static_cast<long>(a.max_tiles) * a.Hkv, static_cast<long>(a.num_sms));
-  const long grid_q = std::min(items, static_cast<long>(a.num_sms));
+  const long items_kv = static_cast<long>(a.dkv.max_tiles) * a.Hkv;
+  const long items_q = static_cast<long>(a.dq.max_tiles) * (a.H >> a.lp);
+  if (items_q > 0x7fff0000l || items_kv > 0x7fff0000l) return -2;
+  const long grid_kv = std::min(items_kv, static_cast<long>(a.num_sms));
+  const long grid_q = std::min(items_q, static_cast<long>(a.num_sms));
   if (want_dkv) {
     auto kernel = packed_dkv_kernel<DP>;
     if (set_max_smem(kernel, BwdCfg<DP>::kSmem) != cudaSuccess) return -1;
@@ -671,7 +687,7 @@ int run_bwd(const PackedMaps& m, const PackedArgs& a, const BwdArgs& args, bool 
     auto kernel = packed_dq_kernel<DP>;
     if (set_max_smem(kernel, BwdCfg<DP>::kSmem) != cudaSuccess) return -1;
     if (launch_pdl(kernel, dim3(static_cast<unsigned>(grid_q)), dim3(kBwdThreads), BwdCfg<DP>::kSmem, stream, m.q, m.k,
-                   m.v, m.dout, args, status) != cudaSuccess)
+                   m.v, m.dout, m.k32, m.v32, args, status) != cudaSuccess)
       return -1;
   }
   return 0;
@@ -690,7 +706,8 @@ int launch_packed_delta(const void* out, const void* dout, long stride_t, long s
 int launch_packed_backward(const PackedMaps& maps, const PackedArgs& a, const float* lse, const float* delta, void* dq,
                            void* dk, void* dv, unsigned* status, cudaStream_t stream) {
   const BwdArgs args{static_cast<bf16*>(dq), static_cast<bf16*>(dk), static_cast<bf16*>(dv), lse, delta,
-                     static_cast<const int4*>(a.table), a.head, a.T, a.H, a.Hkv, a.D, a.scale, a.scale * kLog2e};
+                     static_cast<const int4*>(a.dq.entries), static_cast<const int4*>(a.dkv.entries), a.dq.head, a.dkv.head,
+                     a.T, a.H, a.Hkv, a.D, a.lp, a.scale, a.scale * kLog2e};
   const bool want_dkv = dk != nullptr;
   return a.D <= 64 ? run_bwd<64>(maps, a, args, dq != nullptr, want_dkv, status, stream)
                    : run_bwd<128>(maps, a, args, dq != nullptr, want_dkv, status, stream);

@@ -57,7 +57,7 @@ __device__ __forceinline__ uint32_t low_bits(int n) {
   return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
 }
 
-// 3-D tiled load: box {64 (d), 1 (head), 128 (tokens)} at (d, head, token). d is a multiple of 64.
+// 3-D tiled load of the map's box at (d, head, token). d is a multiple of 64.
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int d, int head,
                                             int token) {
   asm volatile(
@@ -67,19 +67,38 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// [128 rows, DP] as DP / 64 atoms of 128 rows x 128 bytes.
+// A tile of 128 rows, [128, DP] as DP / 64 atoms of 128 rows x 128 bytes, with one box per atom. Rows are tokens of one
+// head, or (token, head) with the heads varying fastest: `1 << lp` heads of 128 >> lp tokens.
 template <int DP>
 __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int head, int token) {
 #pragma unroll
   for (int a = 0; a < DP / 64; ++a) tma_load_3d(dst + a * kRowsT * 128, map, bar, a * 64, head, token);
 }
 
+// A chunk of keys or values of which `rows` are needed: whole, or by boxes of 32 rows (map32), so that a short
+// sequence does not fetch a hundred rows of its successors. Counts the bytes on `bar` first.
+template <int DP>
+__device__ __forceinline__ void load_chunk(uint32_t dst, const CUtensorMap* map, const CUtensorMap* map32, uint64_t* bar,
+                                           int head, int token, int rows) {
+  if (rows > 96) {
+    mbar_arrive_expect_tx(bar, kRowsT * DP * 2);
+    load_tile<DP>(dst, map, bar, head, token);
+    return;
+  }
+  const int boxes = (rows + 31) >> 5;
+  mbar_arrive_expect_tx(bar, boxes * 32 * DP * 2);
+  for (int b = 0; b < boxes; ++b)
+#pragma unroll
+    for (int a = 0; a < DP / 64; ++a)
+      tma_load_3d(dst + a * kRowsT * 128 + b * 32 * 128, map32, bar, a * 64, head, token + b * 32);
+}
+
 // Zero rows [from, to) of a [128, DP] tile (the swizzle permutes 16-byte groups inside a row only); one warp.
 template <int DP>
 __device__ __forceinline__ void zero_rows(uint8_t* tile, int from, int to, int lane) {
-  const int per_row = DP / 8;
-  for (int i = lane; i < (to - from) * per_row; i += 32) {
-    const int row = from + i / per_row, c = i % per_row;
+  constexpr int kPerRow = DP / 8;
+  for (int i = lane; i < (to - from) * kPerRow; i += 32) {
+    const int row = from + i / kPerRow, c = i % kPerRow;
     *reinterpret_cast<uint4*>(tile + (c >> 3) * kRowsT * 128 + row * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
   }
   fence_async_smem();
@@ -181,11 +200,21 @@ struct Items {
   }
 };
 
-// Stores 64 columns of a warp's 32 rows: lane r holds row r's as eight 16-byte groups c[0..7]. An 8 x 8 transpose over
-// groups of eight lanes (three exchanges) first, so that eight lanes write a row's 128 bytes at once: rows written by
-// their own lanes touch 32 lines per store and took 3900 cycles for a 128 x 128 tile. Row r goes to dst + r stride for
-// r < rows, columns below `cols`.
-__device__ __forceinline__ void store_rows64(uint4 (&c)[8], bf16* dst, long stride, int rows, int cols, int lane) {
+// Where the rows of a tile go: row r (< rows) to dst + (r >> lp) token + (r & ((1 << lp) - 1)) head, its columns below
+// `cols`.
+struct TileOut {
+  bf16* dst;
+  long token, head;  // strides in elements
+  int lp, rows, cols;
+  __device__ __forceinline__ bf16* row(int r) const {
+    return dst + (r >> lp) * token + (r & ((1 << lp) - 1)) * head;
+  }
+};
+
+// Stores 64 columns of a warp's 32 rows, from `row0` of the tile on: lane r holds row r's as eight 16-byte groups
+// c[0..7]. An 8 x 8 transpose over groups of eight lanes (three exchanges) first, so that eight lanes write a row's 128
+// bytes at once: rows written by their own lanes touch 32 lines per store and took 3900 cycles for a 128 x 128 tile.
+__device__ __forceinline__ void store_rows64(uint4 (&c)[8], const TileOut& to, int row0, int lane) {
 #pragma unroll
   for (int m = 4; m > 0; m >>= 1) {
     const bool up = (lane & m) != 0;
@@ -204,45 +233,9 @@ __device__ __forceinline__ void store_rows64(uint4 (&c)[8], bf16* dst, long stri
   const int col = (lane & 7) * 8;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int row = (lane & 24) + j;
-    if (row < rows && col < cols) *reinterpret_cast<uint4*>(dst + row * stride + col) = c[j];
+    const int row = row0 + (lane & 24) + j;
+    if (row < to.rows && col < to.cols) *reinterpret_cast<uint4*>(to.row(row) + col) = c[j];
   }
-}
-
-// 64 fp32 columns of the warp's TMEM lanes, times each lane's f, as bf16 rows through 4 KB of shared memory of the warp
-// (16-byte groups swizzled by the row, so that neither side conflicts); arguments as store_rows64.
-__device__ __forceinline__ void stage_tmem64(uint32_t taddr, float f, uint8_t* stage, bf16* dst, long stride, int rows,
-                                             int cols, int lane) {
-  const uint64_t ff = pair_of(f, f);
-  uint8_t* mine = stage + lane * 128;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float o[32];
-    tmem_load32(taddr + h * 32, o);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t w[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float a, b;
-        unpair(mul2(pair_of(o[8 * j + 2 * k], o[8 * j + 2 * k + 1]), ff), a, b);
-        w[k] = pack_bf16(a, b);
-      }
-      *reinterpret_cast<uint4*>(mine + (((h * 4 + j) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
-  __syncwarp();
-  const int g = lane & 7;
-  if (g * 8 < cols) {
-    bf16* at = dst + (lane >> 3) * stride + g * 8;
-#pragma unroll
-    for (int i = 0; i < 8; ++i, at += 4 * stride) {
-      const int row = i * 4 + (lane >> 3);
-      if (row < rows)
-        *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(stage + row * 128 + ((g ^ (row & 7)) << 4));
-    }
-  }
-  __syncwarp();
 }
 
 // 64 fp32 columns of a lane's TMEM row, times f, as eight groups of eight bf16.
@@ -267,11 +260,46 @@ __device__ __forceinline__ void load_packed64(uint32_t taddr, float f, uint4 (&c
 }
 
 // 64 columns of the warp's TMEM lanes, times each lane's f, as bf16 rows through registers (store_rows64).
-__device__ __forceinline__ void store_tmem64(uint32_t taddr, float f, bf16* dst, long stride, int rows, int cols,
-                                             int lane) {
+__device__ __forceinline__ void store_tmem64(uint32_t taddr, float f, const TileOut& to, int row0, int lane) {
   uint4 c[8];
   load_packed64(taddr, f, c);
-  store_rows64(c, dst, stride, rows, cols, lane);
+  store_rows64(c, to, row0, lane);
+}
+
+// The same through 4 KB of shared memory of the warp (16-byte groups swizzled by the row, so that neither side
+// conflicts), with fewer instructions.
+__device__ __forceinline__ void stage_tmem64(uint32_t taddr, float f, uint8_t* stage, const TileOut& to, int row0,
+                                             int lane) {
+  const uint64_t ff = pair_of(f, f);
+  uint8_t* mine = stage + lane * 128;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float o[32];
+    tmem_load32(taddr + h * 32, o);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float a, b;
+        unpair(mul2(pair_of(o[8 * j + 2 * k], o[8 * j + 2 * k + 1]), ff), a, b);
+        w[k] = pack_bf16(a, b);
+      }
+      *reinterpret_cast<uint4*>(mine + (((h * 4 + j) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  __syncwarp();
+  const int g = lane & 7;
+  if (g * 8 < to.cols) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + (lane >> 3);
+      if (row0 + r < to.rows)
+        *reinterpret_cast<uint4*>(to.row(row0 + r) + g * 8) =
+            *reinterpret_cast<const uint4*>(stage + r * 128 + ((g ^ (r & 7)) << 4));
+    }
+  }
+  __syncwarp();
 }
 
 // Tiles need 1024-byte boundaries, and there is no room to align them: dynamic shared memory starts on such a boundary

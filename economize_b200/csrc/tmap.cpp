@@ -85,13 +85,13 @@ int make_tmap_2d(CUtensorMap* map, int elem_bytes, const void* base, uint64_t ro
 }
 
 int make_tmap_heads(CUtensorMap* map, const void* base, uint64_t tokens, uint64_t heads, uint64_t d,
-                    uint64_t token_stride, uint64_t head_stride, uint32_t box_tokens) {
+                    uint64_t token_stride, uint64_t head_stride, uint32_t box_heads, uint32_t box_tokens) {
   EncodeFn fn = encode_fn();
   if (fn == nullptr) return -2;
   if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || token_stride % 8 != 0 || head_stride % 8 != 0) return -3;
   cuuint64_t dims[3] = {d, heads, tokens};
   cuuint64_t strides[2] = {head_stride * 2, token_stride * 2};
-  cuuint32_t box[3] = {64, 1, box_tokens};
+  cuuint32_t box[3] = {64, box_heads, box_tokens};
   cuuint32_t elem[3] = {1, 1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, elem,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
