@@ -439,13 +439,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + (2 + kRing) * kTileBytes);
   Stream<DP> ring{smem + 2 * kTileBytes, q_full + 1, q_full + 1 + kRing};
   uint64_t* s_full = q_full + 1 + 2 * kRing;  // [2], of the S buffer of even and odd chunks
-  uint64_t* dp_full = s_full + 2;             // [2], by chunk parity: each is waited for by one group
-  uint64_t* dp_free = dp_full + 2;
-  uint64_t* ds_ready = dp_free + 2;
-  // [2], by item parity: an item's dQ is complete. One barrier would not do: a group that is through with the next item's
-  // only chunk before this item's last dQ would take the phase before this one for its own.
-  uint64_t* dq_full = ds_ready + 2;
-  uint64_t* dq_free = dq_full + 2;   // dQ is in registers
+  uint64_t* dp_full = s_full + 2;
+  uint64_t* ds_ready = dp_full + 1;
+  uint64_t* dq_full = ds_ready + 1;  // an item's dQ is complete
+  uint64_t* dq_free = dq_full + 1;   // and in registers
   uint64_t* q_empty = dq_free + 1;   // an item's last scores are computed: Q may be overwritten, some time before dO
   uint64_t* do_full = q_empty + 1;
   uint64_t* do_empty = do_full + 1;
@@ -460,14 +457,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&ring.full[i], 1);
       mbar_init(&ring.empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&dp_full[i], 1);
-      mbar_init(&dp_free[i], kComputeWarps / 2);
-      mbar_init(&ds_ready[i], kComputeWarps / 2);
-    }
-    mbar_init(&dq_full[0], 1);
-    mbar_init(&dq_full[1], 1);
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_ready, kComputeWarps);
+    mbar_init(dq_full, 1);
     mbar_init(dq_free, kComputeWarps / 2);
     mbar_init(q_empty, 1);
     mbar_init(do_full, 1);
@@ -539,115 +533,109 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       a.step();
       return true;
     };
-    auto products = [&](ChunkWalk<false>& b) {  // dP of a chunk once the one before is in registers; the only use of its V
-      if (!b.valid) return true;
-      const int x = 2 * b.k + 1, before = b.k - 1;
-      if (b.first() && !warp_wait(do_full, b.item & 1, status, kStatusWaitFull, abort_flag)) return false;
-      if (!warp_wait(ring.full_of(x), ring.use(x), status, kStatusWaitFull, abort_flag)) return false;
-      if (b.k > 0 && !warp_wait(&dp_free[before & 1], (before >> 1) & 1, status, kStatusWaitAccum, abort_flag))
-        return false;
+    ChunkWalk<true> a(p);
+    ChunkWalk<false> c(p);  // its table entries are in the cache by then
+    bool ok = scores(a);
+    if (ok && c.valid) {
+      ok = warp_wait(do_full, 0, status, kStatusWaitFull, abort_flag) &&
+           warp_wait(ring.full_of(1), 0, status, kStatusWaitFull, abort_flag);
       tc_fence_after();
-      if (leader) {
-        mma_dims<DP>(t_dp, da, smem_u32(ring.tile(x)), b.width(), ksteps);
-        umma_commit(&dp_full[b.k & 1]);
-        umma_commit(ring.empty_of(x));
-        if (b.last()) umma_commit(do_empty);
+      if (ok && leader) {
+        mma_dims<DP>(t_dp, da, smem_u32(ring.tile(1)), c.width(), ksteps);
+        umma_commit(dp_full);
+        umma_commit(ring.empty_of(1));
+        if (c.last()) umma_commit(do_empty);
       }
       __syncwarp();
-      b.step();
-      return true;
-    };
-    ChunkWalk<true> a(p);
-    ChunkWalk<false> b(p), c(p);  // their table entries are in the cache by then
-    bool ok = scores(a) && products(b) && scores(a);
+    }
     while (ok && c.valid) {
-      ok = products(b) && warp_wait(&ds_ready[c.k & 1], (c.k >> 1) & 1, status, kStatusWaitAccum, abort_flag);
-      if (ok && c.first() && c.item > 0)
-        ok = warp_wait(dq_free, (c.item - 1) & 1, status, kStatusWaitAccum, abort_flag);
+      const int k = c.k, width = c.width();
+      const bool first = c.first(), last = c.last();
+      const int item = c.item;
+      c.step();
+      // while the threads work on chunk k: S of the next, and its V is waited for
+      if (c.valid) {
+        ok = scores(a) && warp_wait(ring.full_of(2 * k + 3), ring.use(2 * k + 3), status, kStatusWaitFull, abort_flag);
+        if (ok && c.first()) ok = warp_wait(do_full, c.item & 1, status, kStatusWaitFull, abort_flag);
+      }
+      if (ok && first && item > 0) ok = warp_wait(dq_free, (item - 1) & 1, status, kStatusWaitAccum, abort_flag);
+      ok = ok && warp_wait(ds_ready, k & 1, status, kStatusWaitAccum, abort_flag);
       if (!ok) break;
       tc_fence_after();
       if (leader) {
-        const int x = 2 * c.k;
-        mma_rows<4, 64>(t_dq, t_s + (c.k & 1) * 128, smem_u32(ring.tile(x)), ksteps * 16, c.width() / 16, !c.first());
-        umma_commit(ring.empty_of(x));
-        if (c.last()) umma_commit(&dq_full[c.item & 1]);
+        if (c.valid) {
+          mma_dims<DP>(t_dp, da, smem_u32(ring.tile(2 * k + 3)), c.width(), ksteps);
+          umma_commit(dp_full);
+          umma_commit(ring.empty_of(2 * k + 3));
+          if (c.last()) umma_commit(do_empty);
+        }
+        mma_rows<2, 32>(t_dq, t_s + (k & 1) * 128, smem_u32(ring.tile(2 * k)), ksteps * 16, width / 16, !first);
+        umma_commit(ring.empty_of(2 * k));
+        if (last) umma_commit(dq_full);
       }
       __syncwarp();
-      c.step();
-      ok = scores(a);
     }
   } else if (warp >= 4) {
-    // ---- dS: two groups of eight warps take the even and the odd chunks, so that the exponentials of one chunk run
-    // beside the products of the other; one thread per query and half of the chunk's keys. The group that had an item's
-    // last chunk stores its dQ. ----
+    // ---- dS: one thread per query and quarter of the chunk's keys ----
     const int part = (warp - 4) >> 2, quad = warp & 3;
-    const int mine = part >> 1, half = part & 1;
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
-    const uint32_t s_addr = t_s + mine * 128 + lane_base + half * 64, dp_addr = t_dp + lane_base + half * 64;
-    ChunkWalk<false> at(p);
-    if (mine == 1 && at.valid) at.step();
+    const uint32_t dp_addr = t_dp + lane_base + part * 32;
+    ChunkWalk<true> at(p);
     bool ok = true;
+    float lse = 0.f, delta = 0.f;
     while (ok && at.valid) {
-      const uint32_t use = (at.k >> 1) & 1;
+      const uint32_t s_addr = t_s + (at.k & 1) * 128 + lane_base + part * 32;
       const int first = at.token(), token = first + ((quad * 32 + lane) >> p.lp), hi = at.hi();
       const bool last = at.last();
-      const int limit = min(hi, token + 1) - (at.lo() + at.chunk * kRowsT) - half * 64;  // visible keys, last chunk
-      float lse = 0.f, delta = 0.f;
-      if (token < hi) {
-        const long from = static_cast<long>(at.head() + (lane & ((1 << p.lp) - 1))) * p.T + token;
-        lse = p.lse[from];
-        delta = p.delta[from];
+      const int limit = min(hi, token + 1) - (at.lo() + at.chunk * kRowsT) - part * 32;  // visible keys, last chunk
+      if (at.first()) {
+        lse = delta = 0.f;
+        if (token < hi) {
+          const long from = static_cast<long>(at.head() + (lane & ((1 << p.lp) - 1))) * p.T + token;
+          lse = p.lse[from];
+          delta = p.delta[from];
+        }
       }
-      ok = warp_wait(&s_full[mine], use, status, kStatusWaitAccum, abort_flag);
+      ok = warp_wait(&s_full[at.k & 1], (at.k >> 1) & 1, status, kStatusWaitAccum, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      // P waits for dP in the columns S came from: 64 more registers would spill
-      float v[32];
+      float v[32], g[32];
+      tmem_load32(s_addr, v);
+      const uint64_t scale2 = pair_of(p.scale2, p.scale2), minus_lse = pair_of(-lse, -lse);
 #pragma unroll
-      for (int h = 0; h < 64; h += 32) {
-        tmem_load32(s_addr + h, v);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = ex2(fmaf(v[j], p.scale2, -lse));
-        tmem_store32(s_addr + h, reinterpret_cast<const uint32_t*>(v));
+      for (int j = 0; j < 32; j += 2) {
+        unpair(fma2(pair_of(v[j], v[j + 1]), scale2, minus_lse), v[j], v[j + 1]);
+        v[j] = ex2(v[j]);
+        v[j + 1] = ex2(v[j + 1]);
       }
-      tmem_wait_st();
-      ok = warp_wait(&dp_full[mine], use, status, kStatusWaitAccum, abort_flag);
+      ok = warp_wait(dp_full, at.k & 1, status, kStatusWaitAccum, abort_flag);
       if (!ok) break;
       tc_fence_after();
+      tmem_load32(dp_addr, g);
+      const uint64_t minus_delta = pair_of(-delta, -delta);
 #pragma unroll
-      for (int h = 0; h < 64; h += 32) {  // dS of a half lies where its P has been read
-        float g[32];
-        uint32_t w[16];
-        tmem_load32(s_addr + h, v);
-        tmem_load32(dp_addr + h, g);
+      for (int j = 0; j < 32; j += 2)
+        unpair(mul2(pair_of(v[j], v[j + 1]), add2(pair_of(g[j], g[j + 1]), minus_delta)), g[j], g[j + 1]);
+      if (last) {
+        const uint32_t seen = low_bits(limit);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) g[j] = v[j] * (g[j] - delta);
-        if (last) {
-          const uint32_t seen = low_bits(limit - h);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) g[j] = (seen >> j) & 1u ? g[j] : 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = pack_bf16(g[2 * j], g[2 * j + 1]);
-        if (h == 32) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&dp_free[mine]);
-        }
-        tmem_st_u32x16(s_addr + h / 2, w);
+        for (int j = 0; j < 32; ++j) g[j] = (seen >> j) & 1u ? g[j] : 0.f;
       }
+      uint32_t w[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) w[j] = pack_bf16(g[2 * j], g[2 * j + 1]);
+      tmem_st_u32x16(s_addr, w);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ds_ready[mine]);
+      if (lane == 0) mbar_arrive(ds_ready);
       const int head = at.head(), item = at.item;
       at.step();
-      if (at.valid) at.step();
-      if (last) {
-        ok = warp_wait(&dq_full[item & 1], (item >> 1) & 1, status, kStatusWaitAccum, abort_flag);
+      if (last && part < 2) {  // half of the warps store the item's dQ
+        ok = warp_wait(dq_full, item & 1, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const int col = half * 64;
+        const int col = part * 64;
         uint4 c[8];
         if (col < p.D) load_packed64(t_dq + lane_base + col, p.scale, c);
         tc_fence_before();
