@@ -72,7 +72,7 @@ struct BwdCfg {
   static constexpr int kTileBytes = kRowsT * DP * 2;
   static constexpr int kRing = DP == 64 ? 10 : 5;  // streamed tiles
   static constexpr int kStatRing = 3;
-  static constexpr int kStats = 2 * 128 * 4;  // lse and delta of a query tile
+  static constexpr int kStats = 2 * 128 * 4;  // -lse and -delta of a query tile
   static constexpr int kSmem = (2 + kRing) * kTileBytes + (DP == 64 ? kStatRing : 2) * kStats + 512;
   static_assert(kSmem <= 232448, "227 KB of shared memory");
 };
@@ -117,14 +117,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   constexpr int kRing = Cfg::kRing, kTileBytes = Cfg::kTileBytes, kStatRing = DP == 64 ? Cfg::kStatRing : 2;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t *k_tile = smem, *v_tile = smem + kTileBytes;
-  float* stats = reinterpret_cast<float*>(smem + (2 + kRing) * kTileBytes);  // stage s: lse [128], delta [128]
+  float* stats = reinterpret_cast<float*>(smem + (2 + kRing) * kTileBytes);  // stage s: -lse [128], -delta [128]
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(stats) + kStatRing * Cfg::kStats);
   Stream<DP> ring{smem + 2 * kTileBytes, kv_full + 1, kv_full + 1 + kRing};
   uint64_t* st_full = kv_full + 1 + 2 * kRing;
   uint64_t* st_empty = st_full + kStatRing;
   uint64_t* s_full = st_empty + kStatRing;
-  uint64_t* p_ready = s_full + 1;
-  uint64_t* dp_full = p_ready + 1;
+  uint64_t* p_ready = s_full + 1;  // [2], by halves of every warp's queries
+  uint64_t* dp_full = p_ready + 2;
   uint64_t* ds_ready = dp_full + 1;
   uint64_t* done = ds_ready + 1;
   uint64_t* kv_empty = done + 1;
@@ -145,7 +145,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&st_empty[i], kComputeWarps);
     }
     mbar_init(s_full, 1);
-    mbar_init(p_ready, kComputeWarps);
+    mbar_init(&p_ready[0], kComputeWarps);
+    mbar_init(&p_ready[1], kComputeWarps);
     mbar_init(dp_full, 1);
     mbar_init(ds_ready, kComputeWarps);
     mbar_init(done, 1);
@@ -235,11 +236,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         at.next();
         const int next16 = (rows_of(at.token) + 15) & ~15;
         if (more) ok = ready(xq + 2, at.token);
-        ok = ok && warp_wait(p_ready, it & 1, status, kStatusWaitAccum, abort_flag);
+        // the first half of dV runs under the exponentials of the second
+        ok = ok && warp_wait(&p_ready[0], it & 1, status, kStatusWaitAccum, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader)
+          mma_rows<2, 32, 0, 8, 2>(t_dv, t_s, smem_u32(ring.tile(xd)), ksteps * 16, rows16 / 16, it > base);
+        __syncwarp();
+        ok = warp_wait(&p_ready[1], it & 1, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
         if (leader) {
-          mma_rows<2, 32>(t_dv, t_s, smem_u32(ring.tile(xd)), ksteps * 16, rows16 / 16, it > base);
+          mma_rows<2, 32, 1, 8, 2>(t_dv, t_s, smem_u32(ring.tile(xd)), ksteps * 16, rows16 / 16, true);
           umma_commit(ring.empty_of(xd));
           if (more) {
             mma_dims<DP>(t_s, ka, smem_u32(ring.tile(xq + 2)), next16, ksteps);
@@ -268,7 +276,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       base += total;
     }
   } else if (warp == 2) {
-    // ---- lse and delta of the query tiles ----
+    // ---- -lse and -delta of the query tiles ----
     int base = 0;
     bool ok = true;
     while (ok && items.next()) {
@@ -284,8 +292,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         for (int j = lane; j < kRowsT; j += 32) {
           const int token = at.token + (j >> p.lp);
           const long from = static_cast<long>(at.head + (j & ((1 << p.lp) - 1))) * p.T + token;
-          dst[j] = token < hi ? p.lse[from] : 0.f;
-          dst[128 + j] = token < hi ? p.delta[from] : 0.f;
+          dst[j] = token < hi ? -p.lse[from] : 0.f;
+          dst[128 + j] = token < hi ? -p.delta[from] : 0.f;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&st_full[s]);
@@ -318,26 +326,30 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const int from = ((key0 + key - at.token) << p.lp) - part * 32, to = ((hi - at.token) << p.lp) - part * 32;
         const bool masked = at.token < key0 + kRowsT || to < 32;
         const uint32_t seen = low_bits(to) & ~low_bits(from);
+        const uint64_t scale2 = pair_of(p.scale2, p.scale2);
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 l = *reinterpret_cast<const float4*>(lse + j);
-          v[j] = ex2(fmaf(v[j], p.scale2, -l.x));
-          v[j + 1] = ex2(fmaf(v[j + 1], p.scale2, -l.y));
-          v[j + 2] = ex2(fmaf(v[j + 2], p.scale2, -l.z));
-          v[j + 3] = ex2(fmaf(v[j + 3], p.scale2, -l.w));
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[8];
+#pragma unroll
+          for (int j = h * 16; j < h * 16 + 16; j += 4) {
+            const float4 l = *reinterpret_cast<const float4*>(lse + j);
+            unpair(fma2(pair_of(v[j], v[j + 1]), scale2, pair_of(l.x, l.y)), v[j], v[j + 1]);
+            unpair(fma2(pair_of(v[j + 2], v[j + 3]), scale2, pair_of(l.z, l.w)), v[j + 2], v[j + 3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[j + e] = ex2(v[j + e]);
+          }
+          if (masked) {
+#pragma unroll
+            for (int j = h * 16; j < h * 16 + 16; ++j) v[j] = (seen >> j) & 1u ? v[j] : 0.f;
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = pack_bf16(v[h * 16 + 2 * j], v[h * 16 + 2 * j + 1]);
+          tmem_st_u32x8(s_addr + h * 8, w);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_ready[h]);
         }
-        if (masked) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = (seen >> j) & 1u ? v[j] : 0.f;
-        }
-        uint32_t w[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
-        tmem_st_u32x16(s_addr, w);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_ready);
         ok = warp_wait(dp_full, it & 1, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
@@ -346,11 +358,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
           const float4 d = *reinterpret_cast<const float4*>(delta + j);
-          g[j] = v[j] * (g[j] - d.x);
-          g[j + 1] = v[j + 1] * (g[j + 1] - d.y);
-          g[j + 2] = v[j + 2] * (g[j + 2] - d.z);
-          g[j + 3] = v[j + 3] * (g[j + 3] - d.w);
+          unpair(mul2(pair_of(v[j], v[j + 1]), add2(pair_of(g[j], g[j + 1]), pair_of(d.x, d.y))), g[j], g[j + 1]);
+          unpair(mul2(pair_of(v[j + 2], v[j + 3]), add2(pair_of(g[j + 2], g[j + 3]), pair_of(d.z, d.w))), g[j + 2],
+                 g[j + 3]);
         }
+        uint32_t w[16];
         if (masked) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) g[j] = (seen >> j) & 1u ? g[j] : 0.f;

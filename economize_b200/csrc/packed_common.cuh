@@ -136,13 +136,13 @@ __device__ __forceinline__ void mma_dims(uint32_t d, uint32_t a, uint32_t b, int
 }
 
 // D[128, n] (+)= P[128, :16 ksteps] . B[:16 ksteps, n], P packed bf16 in TMEM (kPer K steps of 8 columns side by side in
-// every group of kStride columns), B's rows along K (MN-major); K steps [kFrom, kTo) of them.
-template <int kPer, int kStride, int kFrom = 0, int kTo = 8>
+// every group of kStride columns), B's rows along K (MN-major); K steps kFrom, kFrom + kStep, ... < kTo of them.
+template <int kPer, int kStride, int kFrom = 0, int kTo = 8, int kStep = 1>
 __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t p, uint32_t b, int n, int ksteps, bool accumulate) {
   const uint32_t idesc = idesc_bf16_f32(128, n, true);
   const uint64_t db = desc_mnmajor_sw128(b, kRowsT * 128);
 #pragma unroll
-  for (int kk = kFrom; kk < kTo; ++kk) {
+  for (int kk = kFrom; kk < kTo; kk += kStep) {
     const uint32_t pc = p + (kk / kPer) * kStride + (kk % kPer) * 8;
     if (kk < ksteps) umma_bf16_ta(d, pc, desc_step(db, kk * 16 * 128), idesc, kk != 0 ? 1u : (accumulate ? 1u : 0u));
   }
