@@ -66,7 +66,7 @@ std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> readout(
   unsigned* status = ecz::device_status(hidden.device());
   Tensor x = T > 0 ? rows_of(hidden) : hidden, w = rows_of(weight);
   targets = targets.contiguous();
-  const auto f32 = hidden.options().dtype(at::kFloat), i32 = hidden.options().dtype(at::kInt);
+  const auto f32 = hidden.options().dtype(at::kFloat);
   const bool per_row = reduction == ecz::kReduceNone;
   const bool want_loss = !grad_rows.has_value();
   Tensor loss = want_loss ? (per_row ? at::empty({T}, f32) : at::empty({}, f32)) : Tensor();
@@ -99,69 +99,88 @@ std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> readout(
   chunk = std::min((T + 63) / 64 * 64, (chunk + 63) / 64 * 64);
   const int64_t chunks = (T + chunk - 1) / chunk;
 
-  Tensor index = at::empty({3 * T + 1}, i32);  // rows, positions, targets, count
-  int* rows = index.data_ptr<int>();
-  int *pos = rows + T, *target_of = rows + 2 * T, *count = rows + 3 * T;
-  Tensor xs = at::empty({T + 64, H}, hidden.options());
-  Tensor stats = at::empty({chunk, ecz::readout_pieces(static_cast<int>(V)), 2}, f32);
-  Tensor nll = at::empty({T + chunk}, f32);  // losses of the packed rows, then a chunk's picked logits
-  Tensor e = grads ? at::empty({chunk, ld}, hidden.options()) : Tensor();
-  Tensor sum = need_dw && chunks > 1 ? at::empty({V, H}, f32) : Tensor();
+  // One workspace: row lists, losses, target logits, statistics, packed states, e, partial products.
+  const int64_t pieces = ecz::readout_pieces(static_cast<int>(V));
+  const long tiles = ((chunk + 255) / 256) * ((H + 255) / 256);
+  const int splits = need_dx ? ecz::readout_splits(tiles, (V + 63) / 64, sms) : 1;
+  int64_t bytes = 0;
+  auto place = [&](int64_t n) {
+    const int64_t at = bytes;
+    bytes += (n + 255) / 256 * 256;
+    return at;
+  };
+  const bool planned = ecz::readout_needs_plan(static_cast<int>(T));
+  const int64_t o_rows = place(4 * T), o_target = place(4 * T), o_pos = place(planned ? 4 * T : 0), o_count = place(8);
+  const int64_t o_picked = place(4 * T), o_nll = place(4 * T), o_stats = place(8 * chunk * pieces);
+  const int64_t o_xs = place(2 * (T + 64) * H), o_e = place(grads ? 2 * chunk * ld : 0);
+  const int64_t o_part = place(splits > 1 ? 4 * splits * chunk * H : 0);
+  const int64_t o_sum = place(need_dw && chunks > 1 ? 4 * V * H : 0);
+  Tensor workspace = at::empty({bytes}, hidden.options().dtype(at::kByte));
+  uint8_t* ws = workspace.data_ptr<uint8_t>();
+  int *rows = reinterpret_cast<int*>(ws + o_rows), *target_of = reinterpret_cast<int*>(ws + o_target);
+  int *pos = planned ? reinterpret_cast<int*>(ws + o_pos) : nullptr, *count = reinterpret_cast<int*>(ws + o_count);
+  float *picked = reinterpret_cast<float*>(ws + o_picked), *nll = reinterpret_cast<float*>(ws + o_nll);
+  uint8_t* xs = ws + o_xs;
+  void* e = grads ? ws + o_e : nullptr;
 
   auto check = [](int rc, const char* what) { TORCH_CHECK(rc == 0, "readout: ", what, " launch failed"); };
-  check(ecz::launch_readout_plan(targets.data_ptr<int64_t>(), static_cast<int>(T), static_cast<int>(V), ignore_index,
-                                 rows, pos, target_of, count, status, stream),
-        "plan");
-  check(ecz::launch_readout_gather(x.data_ptr(), row_stride(x), static_cast<int>(T), static_cast<int>(H), pos, count,
-                                   xs.data_ptr(), need_dx ? dx->data_ptr() : nullptr,
-                                   want_loss && per_row ? loss.data_ptr<float>() : nullptr, stream),
+  ecz::ReadoutRows r;
+  r.x = x.data_ptr();
+  r.w = w.data_ptr();
+  r.x_stride = row_stride(x);
+  r.w_stride = row_stride(w);
+  r.targets = targets.data_ptr<int64_t>();
+  r.T = static_cast<int>(T);
+  r.H = static_cast<int>(H);
+  r.V = static_cast<int>(V);
+  r.ignore = ignore_index;
+  r.logit_scale = static_cast<float>(logit_scale);
+  if (planned)
+    check(ecz::launch_readout_plan(r.targets, r.T, r.V, ignore_index, pos, count, status, stream), "plan");
+  check(ecz::launch_readout_gather(r, pos, rows, target_of, count, picked, xs, need_dx ? dx->data_ptr() : nullptr,
+                                   want_loss && per_row ? loss.data_ptr<float>() : nullptr, status, stream),
         "gather");
   const CUtensorMap w_rows = map_2d(w.data_ptr(), V, H, row_stride(w), 128);
-  const CUtensorMap w_cols = map_2d(w.data_ptr(), V, H, row_stride(w), 64);
+  CUtensorMap w_cols;
+  if (need_dx) w_cols = map_2d(w.data_ptr(), V, H, row_stride(w), 64);
   for (int64_t i = 0; i < chunks; ++i) {
     ecz::ReadoutChunk c;
     c.row0 = static_cast<int>(i * chunk);
     c.chunk = static_cast<int>(std::min(chunk, T - i * chunk));
-    c.H = static_cast<int>(H);
-    c.V = static_cast<int>(V);
+    c.H = r.H;
+    c.V = r.V;
     c.rows = rows;
     c.target = target_of;
     c.count = count;
-    c.stats = stats.data_ptr();
-    c.picked = nll.data_ptr<float>() + T;
-    c.e = grads ? e.data_ptr() : nullptr;
+    c.stats = ws + o_stats;
+    c.picked = picked;
+    c.e = e;
     c.ld = ld;
-    c.logit_scale = static_cast<float>(logit_scale);
+    c.logit_scale = r.logit_scale;
     const int64_t padded = (c.chunk + 63) / 64 * 64;  // rows of xs and e that the maps may read
-    uint8_t* xs0 = static_cast<uint8_t*>(xs.data_ptr()) + static_cast<int64_t>(c.row0) * H * 2;
+    uint8_t* xs0 = xs + static_cast<int64_t>(c.row0) * H * 2;
     const CUtensorMap x_rows = map_2d(xs0, padded, H, H, 128);
     check(ecz::launch_readout_logits(&x_rows, &w_rows, c, sms, status, stream), "logits");
+    const bool sums = want_loss && !per_row;
     check(ecz::launch_readout_finish(c, static_cast<int>(reduction),
                                      grad_rows.has_value() ? grad_rows->data_ptr<float>() : nullptr,
-                                     want_loss && !per_row ? nll.data_ptr<float>() : nullptr,
-                                     want_loss && per_row ? loss.data_ptr<float>() : nullptr, stream),
+                                     sums ? nll : nullptr, want_loss && per_row ? loss.data_ptr<float>() : nullptr,
+                                     sums && i == chunks - 1 ? loss.data_ptr<float>() : nullptr, count + 1, sms, stream),
           "finish");
     if (need_dx) {
-      const CUtensorMap dz = map_2d(e.data_ptr(), padded, V, ld, 128);
-      const long tiles = ((c.chunk + 255) / 256) * ((H + 255) / 256);
-      const int splits = ecz::readout_splits(tiles, (V + 63) / 64, sms);
-      Tensor part = splits > 1 ? at::empty({splits, c.chunk, H}, f32) : Tensor();
-      check(ecz::launch_readout_dx(&dz, &w_cols, c, splits, splits > 1 ? part.data_ptr<float>() : nullptr,
-                                   dx->data_ptr(), sms, status, stream),
+      const CUtensorMap dz = map_2d(e, padded, V, ld, 128);
+      check(ecz::launch_readout_dx(&dz, &w_cols, c, splits, reinterpret_cast<float*>(ws + o_part), dx->data_ptr(), sms,
+                                   status, stream),
             "dx");
     }
     if (need_dw) {
-      const CUtensorMap dz = map_2d(e.data_ptr(), padded, V, ld, 64);
+      const CUtensorMap dz = map_2d(e, padded, V, ld, 64);
       const CUtensorMap x_cols = map_2d(xs0, padded, H, H, 64);
-      check(ecz::launch_readout_dw(&dz, &x_cols, c, chunks > 1 ? sum.data_ptr<float>() : nullptr, i == 0,
+      check(ecz::launch_readout_dw(&dz, &x_cols, c, chunks > 1 ? reinterpret_cast<float*>(ws + o_sum) : nullptr, i == 0,
                                    i == chunks - 1, dw->data_ptr(), sms, status, stream),
             "dw");
     }
   }
-  if (want_loss && !per_row)
-    check(ecz::launch_readout_loss(nll.data_ptr<float>(), count, static_cast<int>(reduction), loss.data_ptr<float>(),
-                                   stream),
-          "loss");
   return {loss, dx, dw};
 }
 

@@ -282,22 +282,33 @@ struct ReadoutChunk {
   const int* target = nullptr;  // [T] target of a packed row
   const int* count = nullptr;   // packed rows (device)
   void* stats = nullptr;        // float2 [chunk, readout_pieces(V)]
-  float* picked = nullptr;      // [chunk]
+  const float* picked = nullptr;  // [T] target's logit of a packed row, log2 units
   void* e = nullptr;            // fp16 e, then bf16 dz [chunk up to a multiple of 64, ld], or null (losses only)
   long ld = 0;                  // a multiple of 8
   float logit_scale = 1.f;
 };
 int readout_pieces(int V);
 int readout_splits(long tiles, long kblocks, int num_sms);
-int launch_readout_plan(const int64_t* targets, int T, int V, int64_t ignore, int* rows, int* pos, int* target_of,
-                        int* count, unsigned* status, cudaStream_t stream);
-int launch_readout_gather(const void* x, long x_stride, int T, int H, const int* pos, const int* count, void* xs,
-                          void* dx, float* losses, cudaStream_t stream);
+// The states and head as given.
+struct ReadoutRows {
+  const void *x = nullptr, *w = nullptr;
+  long x_stride = 0, w_stride = 0;
+  const int64_t* targets = nullptr;
+  int T = 0, H = 0, V = 0;
+  int64_t ignore = 0;
+  float logit_scale = 1.f;
+};
+// Whether T rows are planned by a kernel of their own (else the gather kernel gets pos = null).
+bool readout_needs_plan(int T);
+int launch_readout_plan(const int64_t* targets, int T, int V, int64_t ignore, int* pos, int* count, unsigned* status,
+                        cudaStream_t stream);
+int launch_readout_gather(const ReadoutRows& r, const int* pos, int* rows, int* target_of, int* count, float* picked,
+                          void* xs, void* dx, float* losses, unsigned* status, cudaStream_t stream);
 int launch_readout_logits(const CUtensorMap* xs, const CUtensorMap* w, const ReadoutChunk& c, int num_sms,
                           unsigned* status, cudaStream_t stream);
+// loss, done (a zeroed counter): of the last chunk of a scalar loss, else null.
 int launch_readout_finish(const ReadoutChunk& c, int reduction, const float* grad_rows, float* nll, float* losses,
-                          cudaStream_t stream);
-int launch_readout_loss(const float* nll, const int* count, int reduction, float* loss, cudaStream_t stream);
+                          float* loss, int* done, int num_sms, cudaStream_t stream);
 int launch_readout_dx(const CUtensorMap* dz, const CUtensorMap* w, const ReadoutChunk& c, int splits, float* part,
                       void* dx, int num_sms, unsigned* status, cudaStream_t stream);
 int launch_readout_dw(const CUtensorMap* dz, const CUtensorMap* xs, const ReadoutChunk& c, float* sum, bool first,

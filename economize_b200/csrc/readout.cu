@@ -3,18 +3,20 @@
 //   z_tv = s x_t . w_v     L_t = log sum_v exp z_tv     nll_t = L_t - z_{t, y_t}
 //   dz_tv = g_t (exp(z_tv - L_t) - [v = y_t])     dx_t = s sum_v dz_tv w_v     dW_v = s sum_t dz_tv x_t
 //
-// Rows whose target is the ignored index are left out before the first product: the plan kernel lists the other rows
-// in order and the gather kernel packs their states, so a prompt mask saves its share of all three products and
-// nothing that stands in a masked row (not even NaN) reaches a result. Packed rows are processed in chunks:
+// Rows whose target is the ignored index are left out before the first product: the gather kernel packs the other rows'
+// states in order, so a prompt mask saves its share of all three products and nothing that stands in a masked row (not
+// even NaN) reaches a result. It also computes each row's target logit on the CUDA cores, in fp32 with rounding: the
+// tensor cores' accumulation of 4096 products is off by up to 1e-5 of a logit of 10, and the target's is the large one.
+// Packed rows are processed in chunks:
 //
-//   logits    256 x 256 tiles of X . W^T (gemm_pair.cuh); the epilogue reduces each row's 128-column piece to its
-//             maximum m and sum of exp(z - m), picks the target's logit and, when gradients follow, stores
-//             e = exp(z - m) in fp16. e lies in (0, 1] with its piece's largest at 1, so fp16 keeps 11 bits of
-//             everything that counts (bf16 would add a second 8-bit rounding to the gradients); the logits
-//             themselves are never stored.
-//   finish    joins a row's pieces to L_t and nll_t and rewrites e in place as dz = g s (e exp(m - L)) in bf16, the
-//             one rounding of the gradient's left factor. The target's entry is g s expm1(-nll), which keeps its
-//             digits where the probability is near one.
+//   logits    256 x 256 tiles of X . W^T (gemm_pair.cuh); the epilogue reduces each row's 128-column piece, without the
+//             target's column, to its maximum m and sum of exp(z - m) and, when gradients follow, stores e = exp(z - m)
+//             in fp16. e lies in (0, 1] with its piece's largest at 1, so fp16 keeps 11 bits of everything that counts
+//             (bf16 would add a second 8-bit rounding to the gradients); the logits themselves are never stored.
+//   finish    joins a row's pieces to S, the sum over the other tokens. nll = log(1 + S exp(-z_y)) and the target's
+//             gradient -S / (S + exp(z_y)) keep their digits where the target's probability is near one. Rewrites e in
+//             place as dz = g s (e exp(m - L)) in bf16, the one rounding of the gradient's left factor. The last CTA of
+//             the last chunk adds the losses up in row order.
 //   products  dX = dz . W (K = V, W read MN-major) and dW = dz^T . X (K = rows, both operands MN-major), no
 //             transposes. Over several chunks dW is summed in an fp32 buffer in chunk order.
 //
@@ -38,12 +40,17 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// ---- plan ------------------------------------------------------------------------------------------------------
-// One CTA: rows[i] = the i-th row with a target, pos[t] = its place or -1, target_of[i] = its target, *count = how
-// many. A target outside [0, V) that is not the ignored index counts as ignored and sets kStatusBadIndex.
+// ---- plan and gather -------------------------------------------------------------------------------------------
+__device__ __forceinline__ bool has_target(int64_t y, int V, int64_t ignore, unsigned* status) {
+  if (y == ignore) return false;
+  if (y >= 0 && y < V) return true;
+  atomicOr(status, kStatusBadIndex);  // counts as ignored
+  return false;
+}
+
+// One CTA, for many rows: pos[t] = the place of row t among those with a target, or -1; *count = how many.
 __global__ void __launch_bounds__(1024) readout_plan_kernel(const int64_t* __restrict__ targets, int T, int V,
-                                                            int64_t ignore, int* __restrict__ rows,
-                                                            int* __restrict__ pos, int* __restrict__ target_of,
+                                                            int64_t ignore, int* __restrict__ pos,
                                                             int* __restrict__ count, unsigned* status) {
   __shared__ int warp_count[32];
   __shared__ int base;
@@ -54,12 +61,7 @@ __global__ void __launch_bounds__(1024) readout_plan_kernel(const int64_t* __res
   __syncthreads();
   for (int t0 = 0; t0 < T; t0 += 1024) {
     const int t = t0 + threadIdx.x;
-    int64_t y = t < T ? targets[t] : ignore;
-    bool keep = t < T && y != ignore;
-    if (keep && (y < 0 || y >= V)) {
-      atomicOr(status, kStatusBadIndex);
-      keep = false;
-    }
+    const bool keep = t < T && has_target(targets[t], V, ignore, status);
     const unsigned ballot = __ballot_sync(0xffffffffu, keep);
     if (lane == 0) warp_count[warp] = __popc(ballot);
     __syncthreads();
@@ -71,12 +73,7 @@ __global__ void __launch_bounds__(1024) readout_plan_kernel(const int64_t* __res
       if (w < warp) before += c;
       total += c;
     }
-    const int at = before + __popc(ballot & ((1u << lane) - 1u));
-    if (keep) {
-      rows[at] = t;
-      target_of[at] = static_cast<int>(y);
-    }
-    if (t < T) pos[t] = keep ? at : -1;
+    if (t < T) pos[t] = keep ? before + __popc(ballot & ((1u << lane) - 1u)) : -1;
     __syncthreads();
     if (threadIdx.x == 0) base += total;
     __syncthreads();
@@ -84,41 +81,102 @@ __global__ void __launch_bounds__(1024) readout_plan_kernel(const int64_t* __res
   if (threadIdx.x == 0) *count = base;
 }
 
-// ---- gather ----------------------------------------------------------------------------------------------------
-// Warp per row t: its state to xs[pos[t]], or zeros to dx[t] (and losses[t]) where it is ignored. The rows behind
-// the last packed one are zeroed up to the K block that reads them.
-__global__ void __launch_bounds__(256) readout_gather_kernel(const bf16* __restrict__ x, long x_stride, int T, int H,
-                                                             const int* __restrict__ pos,
-                                                             const int* __restrict__ count, bf16* __restrict__ xs,
-                                                             bf16* __restrict__ dx, float* __restrict__ losses) {
+// Warp per row t, eight to a CTA: its state to xs, its target's logit to picked, or zeros to dx (and losses[t]) where it
+// is ignored. The rows behind the last packed one are zeroed up to the K block that reads them. Without a plan (pos
+// null, few rows) every CTA counts the rows before its own itself, which saves a launch.
+constexpr int kPlanRows = 2048;  // rows up to which counting costs less than a plan
+
+struct GatherArgs {
+  const bf16 *x, *w;
+  long x_stride, w_stride;
+  const int64_t* targets;
+  int T, H, V;
+  int64_t ignore;
+  float scale2;      // logit scale times log2(e)
+  const int* pos;
+  int *rows, *target_of, *count;  // packed row -> row, target; how many, and the finish kernel's counter
+  float* picked;
+  bf16 *xs, *dx;
+  float* losses;
+};
+
+__global__ void __launch_bounds__(256) readout_gather_kernel(const __grid_constant__ GatherArgs a, unsigned* status) {
+  __shared__ int before, total;
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int t = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int t0 = blockIdx.x * 8, t = t0 + warp;
+  int p = -1, n = 0;
+  if (a.pos == nullptr) {
+    if (threadIdx.x == 0) before = total = 0;
+    __syncthreads();
+    int mine = 0, all = 0;
+    for (int i = threadIdx.x; i < a.T; i += 256) {
+      const int64_t y = a.targets[i];
+      const bool keep = y != a.ignore && y >= 0 && y < a.V;
+      all += keep;
+      mine += keep && i < t0;
+    }
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    all = __reduce_add_sync(0xffffffffu, all);
+    if (lane == 0) {
+      atomicAdd(&before, mine);
+      atomicAdd(&total, all);
+    }
+    __syncthreads();
+    n = total;
+    if (t < a.T && has_target(a.targets[t], a.V, a.ignore, status)) {
+      p = before;
+      for (int i = t0; i < t; ++i) {
+        const int64_t y = a.targets[i];
+        p += y != a.ignore && y >= 0 && y < a.V;
+      }
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.count = n;
+  } else {
+    n = *a.count;
+    if (t < a.T) p = a.pos[t];
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.count[1] = 0;
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  if (t >= T) {
-    const int n = *count;
-    const int r = n + (t - T);
-    if (t - T < pair::kBK && r < (n + pair::kBK - 1) / pair::kBK * pair::kBK)
-      for (int c = lane * 8; c < H; c += 256) *reinterpret_cast<uint4*>(xs + static_cast<size_t>(r) * H + c) = zero;
+  if (t >= a.T) {
+    const int r = n + (t - a.T);
+    if (t - a.T < pair::kBK && r < (n + pair::kBK - 1) / pair::kBK * pair::kBK)
+      for (int c = lane * 8; c < a.H; c += 256) *reinterpret_cast<uint4*>(a.xs + static_cast<size_t>(r) * a.H + c) = zero;
     return;
   }
-  const int p = pos[t];
-  if (p >= 0) {
-    for (int c = lane * 8; c < H; c += 256)
-      *reinterpret_cast<uint4*>(xs + static_cast<size_t>(p) * H + c) =
-          *reinterpret_cast<const uint4*>(x + static_cast<size_t>(t) * x_stride + c);
-  } else {
-    if (dx != nullptr)
-      for (int c = lane * 8; c < H; c += 256) *reinterpret_cast<uint4*>(dx + static_cast<size_t>(t) * H + c) = zero;
-    if (losses != nullptr && lane == 0) losses[t] = 0.f;
+  if (p < 0) {
+    if (a.dx != nullptr)
+      for (int c = lane * 8; c < a.H; c += 256) *reinterpret_cast<uint4*>(a.dx + static_cast<size_t>(t) * a.H + c) = zero;
+    if (a.losses != nullptr && lane == 0) a.losses[t] = 0.f;
+    return;
+  }
+  const int y = static_cast<int>(a.targets[t]);
+  const bf16 *x = a.x + static_cast<size_t>(t) * a.x_stride, *w = a.w + static_cast<size_t>(y) * a.w_stride;
+  float acc[2] = {0.f, 0.f};
+  for (int c = lane * 8; c < a.H; c += 256) {
+    const uint4 u = *reinterpret_cast<const uint4*>(x + c), v = *reinterpret_cast<const uint4*>(w + c);
+    *reinterpret_cast<uint4*>(a.xs + static_cast<size_t>(p) * a.H + c) = u;
+    const uint32_t l[4] = {u.x, u.y, u.z, u.w}, r[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&l[k]));
+      const float2 g = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r[k]));
+      acc[0] = fmaf(f.x, g.x, acc[0]);
+      acc[1] = fmaf(f.y, g.y, acc[1]);
+    }
+  }
+  const float z = warp_sum(acc[0] + acc[1]);
+  if (lane == 0) {
+    a.rows[p] = t;
+    a.target_of[p] = y;
+    a.picked[p] = z * a.scale2;
   }
 }
 
 // ---- logits: statistics (and e) of a tile's rows -----------------------------------------------------------------
 struct LogitsEpi {
-  float2* stats;      // [rows of the chunk, pieces]: (max, sum of exp2(z - max)), log2 units
-  float* picked;      // [rows]: the target's logit, log2 units
+  float2* stats;      // [rows of the chunk, pieces]: (max, sum of exp2(z - max)) without the target, log2 units
   const int* target;  // [rows] of the chunk
   __half* e;          // [rows, ld] or null
   long ld;
@@ -136,13 +194,14 @@ struct LogitsEpi {
     for (int c = 0; c < kPiece; c += 32) {
       float v[32];
       tmem_ld32(taddr + c, v);
-      if (c + 32 <= cols) {
+      const int skip = mine - c;
+      if (c + 32 <= cols && !__any_sync(0xffffffffu, skip >= 0 && skip < 32)) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) top = fmaxf(top, v[j] * scale2);
       } else {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          if (c + j < cols) top = fmaxf(top, v[j] * scale2);
+          if (c + j < cols && j != skip) top = fmaxf(top, v[j] * scale2);
       }
     }
     const float ref = top == -INFINITY ? 0.f : top;
@@ -151,15 +210,19 @@ struct LogitsEpi {
     for (int c = 0; c < kPiece; c += 32) {
       float v[32];
       tmem_ld32(taddr + c, v);
-      if (mine >= c && mine < c + 32) {
+      const int skip = mine - c;
+      if (c + 32 <= cols && !__any_sync(0xffffffffu, skip >= 0 && skip < 32)) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (c + j == mine) picked[row] = v[j] * scale2;
-      }
+        for (int j = 0; j < 32; ++j) {
+          v[j] = ex2(fmaf(v[j], scale2, -ref));
+          sum += v[j];
+        }
+      } else {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        v[j] = c + j < cols ? ex2(fmaf(v[j], scale2, -ref)) : 0.f;
-        sum += v[j];
+        for (int j = 0; j < 32; ++j) {
+          v[j] = c + j < cols && j != skip ? ex2(fmaf(v[j], scale2, -ref)) : 0.f;
+          sum += v[j];
+        }
       }
       if (e != nullptr) {
 #pragma unroll
@@ -203,92 +266,112 @@ __device__ __forceinline__ float block_reduce(float v, float* red, bool want_max
   return r;
 }
 
-// One CTA per packed row of the chunk: joins its pieces, writes nll, and (with e) turns e into dz in place. NaN
-// statistics give NaN, as the plain formula does.
+// CTAs (row, part) of the packed rows of a chunk: every part joins the row's pieces and turns its columns of e into dz
+// in place; part 0 writes nll. NaN statistics give NaN, as the plain formula does. Counts itself on *done where a loss
+// is wanted of the last chunk: the last CTA adds up.
 constexpr int kFinishThreads = 256;
 
-__global__ void __launch_bounds__(kFinishThreads)
-    readout_finish_kernel(const float2* __restrict__ stats, const float* __restrict__ picked,
-                          const int* __restrict__ target, const int* __restrict__ rows,
-                          const int* __restrict__ count, int row0, int chunk, int V, int pieces, void* e_dz, long ld,
-                          float logit_scale, int reduction, const float* __restrict__ grad_rows,
-                          float* __restrict__ nll, float* __restrict__ losses) {
-  extern __shared__ float factor[];  // [pieces]: exp2(m - L) g s
-  __shared__ float red[kFinishThreads / 32];
-  pdl_trigger();
-  pdl_wait();
-  const int total = *count;
-  const int n = min(chunk, total - row0);
-  const int r = blockIdx.x;
-  if (n <= 0) return;
-  if (r >= n) {  // zero rows up to the K block of dz^T . X that reads them
-    if (e_dz != nullptr && r < (n + pair::kBK - 1) / pair::kBK * pair::kBK) {
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(e_dz) + static_cast<size_t>(r) * ld);
-      for (int c = threadIdx.x; c < ld / 8; c += kFinishThreads) dst[c] = make_uint4(0, 0, 0, 0);
-    }
-    return;
-  }
-  const float2* st = stats + static_cast<size_t>(r) * pieces;
-  float top = -INFINITY;
+struct FinishArgs {
+  const float2* stats;
+  const float* picked;  // of the chunk's rows
+  const int *target, *rows, *count;
+  int row0, chunk, V, pieces;
+  void* e_dz;
+  long ld;
+  float logit_scale;
+  int reduction;
+  const float* grad_rows;
+  float *nll, *losses;
+  float* loss;  // null but for the last chunk of a scalar loss
+  int* done;
+};
+
+// loss = the sum of nll in a fixed order (thread t sums rows t, t + 256, ..., then a tree), / count, 0 without rows.
+__device__ __forceinline__ void add_up(const FinishArgs& a, float* red) {
+  __shared__ bool last;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(a.done, 1) == static_cast<int>(gridDim.x * gridDim.y) - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  const int n = *a.count;
+  float v = 0.f;
+  for (int i = threadIdx.x; i < n; i += kFinishThreads) v += __ldcg(a.nll + i);
+  v = block_reduce(v, red, false);
+  if (threadIdx.x == 0) *a.loss = a.reduction == kReduceMean ? (n > 0 ? v / static_cast<float>(n) : 0.f) : v;
+}
+
+__device__ __forceinline__ void finish_row(const FinishArgs& a, int r, int total, float* factor, float* red) {
+  const float2* st = a.stats + static_cast<size_t>(r) * a.pieces;
+  const float z = a.picked[r];
+  float top = z;
   bool nan = false;
-  for (int j = threadIdx.x; j < pieces; j += kFinishThreads) {
+  for (int j = threadIdx.x; j < a.pieces; j += kFinishThreads) {
     top = fmaxf(top, st[j].x);
     nan |= st[j].y != st[j].y;
   }
   top = block_reduce(top, red, true);
   const float ref = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
-  for (int j = threadIdx.x; j < pieces; j += kFinishThreads) {
+  for (int j = threadIdx.x; j < a.pieces; j += kFinishThreads) {
     const float2 v = st[j];
     sum += v.y * exp2f(v.x - ref);
   }
-  sum = block_reduce(sum, red, false);
   if (nan) sum = NAN;
-  const float lse2 = ref + log2f(sum);
-  const float loss = (lse2 - picked[r]) * kLn2;
-  const int orig = rows[row0 + r];
-  if (threadIdx.x == 0) {
-    if (nll != nullptr) nll[row0 + r] = loss;
-    if (losses != nullptr) losses[orig] = loss;
+  sum = block_reduce(sum, red, false);
+  const float own = exp2f(z - ref);
+  const float lse2 = ref + log2f(sum + own);
+  const float loss = z >= ref ? log1pf(sum) : (lse2 - z) * kLn2;
+  const int orig = a.rows[a.row0 + r];
+  if (threadIdx.x == 0 && blockIdx.y == 0) {
+    if (a.nll != nullptr) a.nll[a.row0 + r] = loss;
+    if (a.losses != nullptr) a.losses[orig] = loss;
   }
-  if (e_dz == nullptr) return;
-  float g = logit_scale;
-  if (grad_rows != nullptr) g *= grad_rows[orig];
-  else if (reduction == kReduceMean) g /= static_cast<float>(total);
-  for (int j = threadIdx.x; j < pieces; j += kFinishThreads) factor[j] = exp2f(st[j].x - lse2) * g;
+  if (a.e_dz == nullptr) return;
+  float g = a.logit_scale;
+  if (a.grad_rows != nullptr) g *= a.grad_rows[orig];
+  else if (a.reduction == kReduceMean) g /= static_cast<float>(total);
+  for (int j = threadIdx.x; j < a.pieces; j += kFinishThreads) factor[j] = exp2f(st[j].x - lse2) * g;
   __syncthreads();
-  const int tgt = target[r];
-  const float at_target = g * expm1f(-loss);
-  uint16_t* row = static_cast<uint16_t*>(e_dz) + static_cast<size_t>(r) * ld;
-  for (int c = threadIdx.x * 8; c < V; c += kFinishThreads * 8) {
+  const int tgt = a.target[r];
+  const float at_target = -g * (sum / (sum + own));
+  uint16_t* row = static_cast<uint16_t*>(a.e_dz) + static_cast<size_t>(r) * a.ld;
+  const int step = kFinishThreads * 8, begin = blockIdx.y * step;
+  for (int c = begin + threadIdx.x * 8; c < a.V; c += step * gridDim.y) {
     uint4 v = *reinterpret_cast<const uint4*>(row + c);
     const float f = factor[c / kPiece];
     uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const float2 ev = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-      float a = ev.x * f, b = ev.y * f;
-      if (c + 2 * k == tgt) a = at_target;
-      if (c + 2 * k + 1 == tgt) b = at_target;
-      __nv_bfloat162 o = __floats2bfloat162_rn(a, b);
+      float p = ev.x * f, q = ev.y * f;
+      if (c + 2 * k == tgt) p = at_target;
+      if (c + 2 * k + 1 == tgt) q = at_target;
+      __nv_bfloat162 o = __floats2bfloat162_rn(p, q);
       w[k] = *reinterpret_cast<uint32_t*>(&o);
     }
     *reinterpret_cast<uint4*>(row + c) = v;
   }
 }
 
-// loss = sum of nll (in a fixed order: thread t sums rows t, t + 1024, ..., then a tree) / count, 0 without rows.
-__global__ void __launch_bounds__(1024) readout_loss_kernel(const float* __restrict__ nll,
-                                                            const int* __restrict__ count, int reduction,
-                                                            float* __restrict__ loss) {
-  __shared__ float red[32];
+__global__ void __launch_bounds__(kFinishThreads) readout_finish_kernel(const __grid_constant__ FinishArgs a) {
+  extern __shared__ float factor[];  // [pieces]: exp2(m - L) g s
+  __shared__ float red[kFinishThreads / 32];
   pdl_trigger();
   pdl_wait();
-  const int n = *count;
-  float v = 0.f;
-  for (int i = threadIdx.x; i < n; i += 1024) v += nll[i];
-  v = block_reduce(v, red, false);
-  if (threadIdx.x == 0) *loss = reduction == kReduceMean ? (n > 0 ? v / static_cast<float>(n) : 0.f) : v;
+  const int total = *a.count;
+  const int n = min(a.chunk, total - a.row0);
+  const int r = blockIdx.x;
+  if (r < n) {
+    finish_row(a, r, total, factor, red);
+  } else if (n > 0 && a.e_dz != nullptr && r < (n + pair::kBK - 1) / pair::kBK * pair::kBK) {
+    // zero rows up to the K block of dz^T . X that reads them
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.e_dz) + static_cast<size_t>(r) * a.ld);
+    for (int c = blockIdx.y * kFinishThreads + threadIdx.x; c < a.ld / 8; c += kFinishThreads * gridDim.y)
+      dst[c] = make_uint4(0, 0, 0, 0);
+  }
+  if (a.loss != nullptr) add_up(a, red);
 }
 
 // ---- product epilogues ---------------------------------------------------------------------------------------------
@@ -365,18 +448,21 @@ struct StoreEpi {
   }
 };
 
+constexpr int kJoinThreads = 128;
+
 // out[rows[m]] = bf16(sum over splits, in order, of part[s, m]).
-__global__ void __launch_bounds__(256) readout_join_kernel(const float* __restrict__ part, int splits, long part_rows,
+__global__ void __launch_bounds__(kJoinThreads) readout_join_kernel(const float* __restrict__ part, int splits, long part_rows,
                                                            int N, const int* __restrict__ rows,
                                                            const int* __restrict__ count, int row0, int chunk,
                                                            bf16* __restrict__ out) {
   pdl_trigger();
   pdl_wait();
   const int n = min(chunk, *count - row0);
-  const long i = (static_cast<long>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  const long i = (static_cast<long>(blockIdx.x) * kJoinThreads + threadIdx.x) * 4;
   const long m = i / N, c = i % N;
   if (m >= n) return;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
   for (int s = 0; s < splits; ++s) {
     const float4 v = *reinterpret_cast<const float4*>(part + (s * part_rows + m) * N + c);
     acc.x += v.x;
@@ -426,41 +512,44 @@ int readout_splits(long tiles, long kblocks, int num_sms) {
   return static_cast<int>(std::max(1l, std::min(pairs / std::max(1l, tiles), kblocks / 8)));
 }
 
-int launch_readout_plan(const int64_t* targets, int T, int V, int64_t ignore, int* rows, int* pos, int* target_of,
-                        int* count, unsigned* status, cudaStream_t stream) {
-  return launch_pdl(readout_plan_kernel, dim3(1), dim3(1024), 0, stream, targets, T, V, ignore, rows, pos, target_of,
-                    count, status) == cudaSuccess ? 0 : -1;
+bool readout_needs_plan(int T) { return T > kPlanRows; }
+
+int launch_readout_plan(const int64_t* targets, int T, int V, int64_t ignore, int* pos, int* count, unsigned* status,
+                        cudaStream_t stream) {
+  return launch_pdl(readout_plan_kernel, dim3(1), dim3(1024), 0, stream, targets, T, V, ignore, pos, count, status) ==
+                 cudaSuccess ? 0 : -1;
 }
 
-int launch_readout_gather(const void* x, long x_stride, int T, int H, const int* pos, const int* count, void* xs,
-                          void* dx, float* losses, cudaStream_t stream) {
-  return launch_pdl(readout_gather_kernel, dim3((T + pair::kBK + 7) / 8), dim3(256), 0, stream,
-                    static_cast<const bf16*>(x), x_stride, T, H, pos, count, static_cast<bf16*>(xs),
-                    static_cast<bf16*>(dx), losses) == cudaSuccess ? 0 : -1;
+int launch_readout_gather(const ReadoutRows& r, const int* pos, int* rows, int* target_of, int* count, float* picked,
+                          void* xs, void* dx, float* losses, unsigned* status, cudaStream_t stream) {
+  const GatherArgs a{static_cast<const bf16*>(r.x), static_cast<const bf16*>(r.w), r.x_stride, r.w_stride, r.targets, r.T,
+                     r.H, r.V, r.ignore, r.logit_scale * kLog2e, pos, rows, target_of, count, picked,
+                     static_cast<bf16*>(xs), static_cast<bf16*>(dx), losses};
+  return launch_pdl(readout_gather_kernel, dim3((r.T + pair::kBK + 7) / 8), dim3(256), 0, stream, a, status) ==
+                 cudaSuccess ? 0 : -1;
 }
 
 int launch_readout_logits(const CUtensorMap* xs, const CUtensorMap* w, const ReadoutChunk& c, int num_sms,
                           unsigned* status, cudaStream_t stream) {
-  LogitsEpi epi{static_cast<float2*>(c.stats), c.picked, c.target + c.row0, static_cast<__half*>(c.e), c.ld, c.V,
+  LogitsEpi epi{static_cast<float2*>(c.stats), c.target + c.row0, static_cast<__half*>(c.e), c.ld, c.V,
                 readout_pieces(c.V), c.logit_scale * kLog2e};
   const pair::Shape shape{c.chunk, c.V, c.H, c.count, c.row0, true, false, 1, false};
   return pair::launch_pair<false, false>(*xs, *w, shape, epi, num_sms, status, stream);
 }
 
 int launch_readout_finish(const ReadoutChunk& c, int reduction, const float* grad_rows, float* nll, float* losses,
-                          cudaStream_t stream) {
+                          float* loss, int* done, int num_sms, cudaStream_t stream) {
   const int pieces = readout_pieces(c.V);
   const int smem = c.e != nullptr ? pieces * 4 : 0;
-  if (smem > 48 * 1024 && set_max_smem(readout_finish_kernel, smem) != cudaSuccess) return -1;
-  return launch_pdl(readout_finish_kernel, dim3((c.chunk + pair::kBK - 1) / pair::kBK * pair::kBK),
-                    dim3(kFinishThreads), smem, stream, static_cast<const float2*>(c.stats), c.picked,
-                    c.target + c.row0, c.rows, c.count, c.row0, c.chunk, c.V, pieces, c.e, c.ld, c.logit_scale,
-                    reduction, grad_rows, nll, losses) == cudaSuccess ? 0 : -1;
-}
-
-int launch_readout_loss(const float* nll, const int* count, int reduction, float* loss, cudaStream_t stream) {
-  return launch_pdl(readout_loss_kernel, dim3(1), dim3(1024), 0, stream, nll, count, reduction, loss) == cudaSuccess
-             ? 0 : -1;
+  if (smem > 40 * 1024 && set_max_smem(readout_finish_kernel, smem) != cudaSuccess) return -1;
+  const FinishArgs a{static_cast<const float2*>(c.stats), c.picked + c.row0, c.target + c.row0, c.rows, c.count, c.row0,
+                     c.chunk, c.V, pieces, c.e, c.ld, c.logit_scale, reduction, grad_rows, nll, losses, loss, done};
+  const int rows = (c.chunk + pair::kBK - 1) / pair::kBK * pair::kBK;
+  // few rows: several CTAs to a row, so that eight on every SM share the columns
+  const int most = c.e == nullptr ? 1 : (c.V + kFinishThreads * 8 - 1) / (kFinishThreads * 8);
+  const int parts = std::max(1, std::min(most, num_sms * 8 / rows));
+  return launch_pdl(readout_finish_kernel, dim3(rows, parts), dim3(kFinishThreads), smem, stream, a) == cudaSuccess ? 0
+                                                                                                                   : -1;
 }
 
 int launch_readout_dx(const CUtensorMap* dz, const CUtensorMap* w, const ReadoutChunk& c, int splits, float* part,
@@ -470,7 +559,7 @@ int launch_readout_dx(const CUtensorMap* dz, const CUtensorMap* w, const Readout
   int rc = pair::launch_pair<false, true>(*dz, *w, shape, epi, num_sms, status, stream);
   if (rc != 0 || splits == 1) return rc;
   const long groups = static_cast<long>(c.chunk) * c.H / 4;
-  return launch_pdl(readout_join_kernel, dim3(static_cast<unsigned>((groups + 255) / 256)), dim3(256), 0, stream, part,
+  return launch_pdl(readout_join_kernel, dim3(static_cast<unsigned>((groups + kJoinThreads - 1) / kJoinThreads)), dim3(kJoinThreads), 0, stream, part,
                     splits, static_cast<long>(c.chunk), c.H, c.rows + c.row0, c.count, c.row0, c.chunk,
                     static_cast<bf16*>(dx)) == cudaSuccess ? 0 : -1;
 }
