@@ -252,17 +252,21 @@ ecz::PackedArgs packed_args(const Tensor& q, const Tensor& k, int64_t B, double 
   return a;
 }
 
-// Output [T, H, D] and, for a backward pass, the log2-domain log-sum-exp of every row [H, T] and the tile tables.
+// Output [T, H, D] and, for a backward pass, what its rounding left, the log2-domain log-sum-exp of every row [H, T] and
+// the tile tables.
 // tiles: query tiles a CTA works on (0: by the mean length).
-std::tuple<Tensor, Tensor, Tensor> packed_forward(Tensor q, Tensor k, Tensor v, Tensor cu, double scale, bool training,
+std::tuple<Tensor, Tensor, Tensor, Tensor> packed_forward(Tensor q, Tensor k, Tensor v, Tensor cu, double scale, bool training,
                                                   int64_t tiles) {
   check_packed(q, k, v, cu, scale);
   TORCH_CHECK(tiles >= 0 && tiles <= 2, "packed_attention: tiles must be 0, 1 or 2");
   c10::cuda::CUDAGuard guard(q.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  Tensor out = at::empty(q.sizes(), q.options()), lse, plan;
-  if (training) lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
-  if (q.size(0) == 0) return {out, lse, plan};
+  Tensor out = at::empty(q.sizes(), q.options()), rest, lse, plan;
+  if (training) {
+    rest = at::empty(q.sizes(), q.options());
+    lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+  }
+  if (q.size(0) == 0) return {out, rest, lse, plan};
   q = heads_of(q);
   k = heads_of(k);
   v = heads_of(v);
@@ -286,16 +290,17 @@ std::tuple<Tensor, Tensor, Tensor> packed_forward(Tensor q, Tensor k, Tensor v, 
   maps.v = map_heads(v, 1, 128);
   maps.k32 = map_heads(k, 1, 32);
   maps.v32 = map_heads(v, 1, 32);
-  const int rc = ecz::launch_packed_forward(maps, a, out.data_ptr(), training ? lse.data_ptr<float>() : nullptr,
+  const int rc = ecz::launch_packed_forward(maps, a, out.data_ptr(), training ? rest.data_ptr() : nullptr,
+                                            training ? lse.data_ptr<float>() : nullptr,
                                             static_cast<int>(tiles), status, stream);
   TORCH_CHECK(rc == 0, "packed_attention: forward launch failed (", rc, ")");
-  return {out, lse, plan};
+  return {out, rest, lse, plan};
 }
 
 // Gradients of q, k and v (those asked for; undefined otherwise) given the output's. plan, tiles: of the forward pass
 // over B sequences.
 std::tuple<Tensor, Tensor, Tensor> packed_backward(Tensor dout, Tensor q, Tensor k, Tensor v, const Tensor& out,
-                                                   const Tensor& lse, const Tensor& plan, int64_t B, double scale,
+                                                   const Tensor& rest, const Tensor& lse, const Tensor& plan, int64_t B, double scale,
                                                    int64_t tiles, bool need_dq, bool need_dkv) {
   CHECK_BF16(dout);
   CHECK_ON(dout, q);
@@ -315,7 +320,7 @@ std::tuple<Tensor, Tensor, Tensor> packed_backward(Tensor dout, Tensor q, Tensor
   dout = heads_of(dout);
   const ecz::PackedArgs a = packed_args(q, k, B, scale, static_cast<int>(tiles), 3, plan);
   Tensor delta = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
-  TORCH_CHECK(ecz::launch_packed_delta(out.data_ptr(), dout.data_ptr(), dout.stride(0), dout.stride(1), a.T, a.H, a.D,
+  TORCH_CHECK(ecz::launch_packed_delta(out.data_ptr(), rest.data_ptr(), dout.data_ptr(), dout.stride(0), dout.stride(1), a.T, a.H, a.D,
                                        delta.data_ptr<float>(), stream) == 0,
               "packed_attention: delta launch failed");
   ecz::PackedMaps maps;
@@ -417,8 +422,10 @@ struct PackedFunction : torch::autograd::Function<PackedFunction> {
     if (tiles == 0 && q.dim() == 3)
       tiles = ecz::packed_single_tiles(static_cast<int>(q.size(0)), static_cast<int>(B)) ? 1 : 2;
     auto r = packed_forward(q, k, v, cu, scale, true, tiles);
-    ctx->save_for_backward({q, k, v, std::get<0>(r), std::get<1>(r)});
-    ctx->saved_data["plan"] = std::get<2>(r);
+    ctx->save_for_backward({q, k, v, std::get<0>(r)});
+    ctx->saved_data["rest"] = std::get<1>(r);
+    ctx->saved_data["lse"] = std::get<2>(r);
+    ctx->saved_data["plan"] = std::get<3>(r);
     ctx->saved_data["B"] = B;
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["tiles"] = tiles;
@@ -431,7 +438,8 @@ struct PackedFunction : torch::autograd::Function<PackedFunction> {
     auto& data = ctx->saved_data;
     const bool need_dq = ctx->needs_input_grad(0);
     const bool need_dk = ctx->needs_input_grad(1), need_dv = ctx->needs_input_grad(2);
-    auto r = packed_backward(grads[0], s[0], s[1], s[2], s[3], s[4], data["plan"].toTensor(), data["B"].toInt(),
+    auto r = packed_backward(grads[0], s[0], s[1], s[2], s[3], data["rest"].toTensor(), data["lse"].toTensor(),
+                             data["plan"].toTensor(), data["B"].toInt(),
                              data["scale"].toDouble(), data["tiles"].toInt(), need_dq, need_dk || need_dv);
     variable_list out(6);
     if (need_dq) out[0] = std::get<0>(r);

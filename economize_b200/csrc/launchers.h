@@ -341,12 +341,13 @@ int launch_packed_plan(const int* cu, int B, int T, const PackedTable* tables, i
                        cudaStream_t stream);
 // tiles: query tiles a CTA works on, 1 or 2 (packed_single_tiles: whether 1 is the better for T tokens in B sequences).
 bool packed_single_tiles(int T, int B);
-int launch_packed_forward(const PackedMaps& maps, const PackedArgs& a, void* out, float* lse, int tiles,
+// rest: what out's rounding to bf16 left of the output (for the backward pass), or null.
+int launch_packed_forward(const PackedMaps& maps, const PackedArgs& a, void* out, void* rest, float* lse, int tiles,
                           unsigned* status, cudaStream_t stream);
 
-// packed_attention_bwd.cu: delta [H, T] = rows of dout . out (out contiguous [T, H, D]), then the gradients (dq null:
+// packed_attention_bwd.cu: delta [H, T] = rows of dout . (out + rest) (both contiguous [T, H, D]), then the gradients (dq null:
 // not computed; dk and dv null: not computed).
-int launch_packed_delta(const void* out, const void* dout, long stride_t, long stride_h, int T, int H, int D,
+int launch_packed_delta(const void* out, const void* rest, const void* dout, long stride_t, long stride_h, int T, int H, int D,
                         float* delta, cudaStream_t stream);
 int launch_packed_backward(const PackedMaps& maps, const PackedArgs& a, const float* lse, const float* delta, void* dq,
                            void* dk, void* dv, unsigned* status, cudaStream_t stream);

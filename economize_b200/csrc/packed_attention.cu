@@ -16,6 +16,10 @@
 // the A operand of P . V), O accumulates in TMEM. A row's reference maximum moves only when a chunk raises it by more
 // than 2^8 (lazy rescaling), so O is rarely read back before the end.
 //
+// P is rounded to bf16 for P . V: one rounding of the output's left factor, as its result's is of the whole. Over many
+// keys these errors average out; a tile of one chunk multiplies what the rounding leaves of P as well (eight MMAs more),
+// so that the output's rows of few keys, and the backward pass's delta, where dp - delta cancels, do not carry it.
+//
 // A chunk that reaches past its sequence's end holds other rows (the next sequence's, or unwritten padding): their
 // scores are replaced, not multiplied, and the at most 15 V rows that P . V reads in its last K step beyond the end
 // are zeroed in shared memory, so NaN or infinities there reach nothing.
@@ -175,6 +179,7 @@ struct FwdCfg {
 
 struct FwdArgs {
   bf16* out;   // [T, H, D]
+  bf16* rest;  // [T, H, D] what out's rounding left of the output, for the backward pass, or null
   float* lse;  // [H, T] log2-domain log-sum-exp, or null
   const int4* table;  // entries of kTiles query tiles
   const int* head;
@@ -332,16 +337,27 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
           if (!ok) break;
           tc_fence_after();
           const int vsteps = width(i, c) / 16;
-          if (leader)
-            mma_rows<8, 64, 0, 4>(tmem + kTiles * 128 + i * DP, tmem + i * 128, smem_u32(v_tile), ksteps * 16, vsteps,
-                                  c > 0);
+          const uint32_t t_o = tmem + kTiles * 128 + i * DP, t_p = tmem + i * 128;
+          const bool single = chunks[i] == 1;  // P and its rest, 16 columns each in turn
+          if (leader) {
+            if (single) {
+              mma_rows<2, 32, 0, 4>(t_o, t_p, smem_u32(v_tile), ksteps * 16, vsteps, false);
+              mma_rows<2, 32, 0, 4>(t_o, t_p + 16, smem_u32(v_tile), ksteps * 16, vsteps, true);
+            } else {
+              mma_rows<8, 64, 0, 4>(t_o, t_p, smem_u32(v_tile), ksteps * 16, vsteps, c > 0);
+            }
+          }
           __syncwarp();
           ok = warp_wait(&p_ready[2 * i + 1], (used[i] + c) & 1, status, kStatusWaitAccum, abort_flag);
           if (!ok) break;
           tc_fence_after();
           if (leader) {
-            mma_rows<8, 64, 4, 8>(tmem + kTiles * 128 + i * DP, tmem + i * 128, smem_u32(v_tile), ksteps * 16, vsteps,
-                                  true);
+            if (single) {
+              mma_rows<2, 32, 4, 8>(t_o, t_p, smem_u32(v_tile), ksteps * 16, vsteps, true);
+              mma_rows<2, 32, 4, 8>(t_o, t_p + 16, smem_u32(v_tile), ksteps * 16, vsteps, true);
+            } else {
+              mma_rows<8, 64, 4, 8>(t_o, t_p, smem_u32(v_tile), ksteps * 16, vsteps, true);
+            }
             umma_commit(&o_done[i]);
             if (c + 1 < chunks[i]) {
               mma_dims<DP>(tmem + i * 128, qa + i * kTileBytes, ra + (k_it % kRing) * kTileBytes, width(i, c + 1),
@@ -377,66 +393,107 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
       // maximum is reduced beside them, and only where it lies more than kLazy above (or far below, in the first chunk,
       // where small sums would underflow) does the row take it as its reference and repeat.
       float ref = 0.f, sum = 0.f;
-      for (int c = 0; c < n_mine; ++c) {
+      auto publish = [&](int h) {
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[2 * i + h]);
+      };
+      if (n_mine == 1) {
+        // The only chunk: its maximum first, and what P's rounding leaves beside P. 32 columns at a time, read twice.
+        ok = warp_wait(&s_full[i], used & 1, status, kStatusWaitAccum, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const int limit = min(items.tile.y, token + 1) - items.tile.x, blocks = (keys_of(items, i, 0) + 31) >> 5;
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int b = 0; b < blocks; ++b) {
+          float v[32];
+          tmem_load32(s_addr + b * 32, v);
+          const uint32_t bits = low_bits(limit - b * 32);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) top = (bits >> j) & 1u ? fmaxf(top, v[j]) : top;
+        }
+        ref = top * p.scale2;
+        const float shift = ref == -INFINITY ? 0.f : ref;
+#pragma unroll 1
+        for (int b = 0; b < blocks; ++b) {
+          float v[32];
+          uint32_t w[16], rest[16];
+          tmem_load32(s_addr + b * 32, v);
+          const uint32_t bits = low_bits(limit - b * 32);
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float x = (bits >> j) & 1u ? ex2(fmaf(v[j], p.scale2, -shift)) : 0.f;
+            const float y = (bits >> (j + 1)) & 1u ? ex2(fmaf(v[j + 1], p.scale2, -shift)) : 0.f;
+            sum += x + y;
+            w[j / 2] = pack_bf16(x, y);
+            rest[j / 2] = rest_of(w[j / 2], x, y);
+          }
+          tmem_st_u32x16(s_addr + b * 32, w);
+          tmem_st_u32x16(s_addr + b * 32 + 16, rest);
+          if (b == 1) publish(0);
+        }
+        if (blocks < 2) publish(0);
+        publish(1);
+      }
+      for (int c = n_mine == 1 ? 1 : 0; c < n_mine; ++c) {
         ok = warp_wait(&s_full[i], (used + c) & 1, status, kStatusWaitAccum, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        float v[128];
-        tmem_load128(s_addr, v);
-        int blocks = 4;           // of 32 columns, that hold scores
-        if (c == n_mine - 1) {  // the diagonal and the sequence's end
-          const int limit = min(items.tile.y, token + 1) - (items.tile.x + c * kRowsT);
-          blocks = (keys_of(items, i, c) + 31) >> 5;
+        const bool masked = c == n_mine - 1;  // the diagonal and the sequence's end
+        const int limit = min(items.tile.y, token + 1) - (items.tile.x + c * kRowsT);
+        const bool both = !masked || keys_of(items, i, c) > 64;  // the second half of the columns holds scores
+        float v[64];
+        float high;
+        auto scores = [&](int h) {  // 64 columns, those of hidden keys replaced, to v; their maximum to high
+          tmem_load64(s_addr + h * 64, v);
+          if (masked) {
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            const uint32_t bits = low_bits(limit - h * 32);
+            for (int g = 0; g < 2; ++g) {
+              const uint32_t bits = low_bits(limit - h * 64 - g * 32);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[h * 32 + j] = (bits >> j) & 1u ? v[h * 32 + j] : -INFINITY;
+              for (int j = 0; j < 32; ++j) v[g * 32 + j] = (bits >> j) & 1u ? v[g * 32 + j] : -INFINITY;
+            }
           }
-        }
-        uint64_t part[2];  // sums of exponentials, by halves
-        // 64 probabilities to TMEM, their sum to part[h]
-        auto exponentials = [&](int h) {
+          float m0 = max3(v[0], v[1], v[2]), m1 = max3(v[3], v[4], v[5]);
+#pragma unroll
+          for (int j = 6; j < 62; j += 4) {
+            m0 = max3(m0, v[j], v[j + 1]);
+            m1 = max3(m1, v[j + 2], v[j + 3]);
+          }
+          high = max3(fmaxf(m0, m1), v[62], v[63]);
+        };
+        uint32_t w[32];
+        auto exponentials = [&]() {  // of v, packed to w; their sum
           const float shift = ref == -INFINITY ? 0.f : ref;
           const uint64_t scale2 = pair_of(p.scale2, p.scale2), minus = pair_of(-shift, -shift);
           uint64_t a = 0, b = 0;
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            if (h * 2 + q >= blocks) break;
-            uint32_t w[16];
-#pragma unroll
-            for (int j = 0; j < 16; j += 2) {
-              const float* x = v + h * 64 + q * 32 + 2 * j;
-              float x0, x1, y0, y1;
-              unpair(fma2(pair_of(x[0], x[1]), scale2, minus), x0, x1);
-              unpair(fma2(pair_of(x[2], x[3]), scale2, minus), y0, y1);
-              x0 = ex2(x0);
-              x1 = ex2(x1);
-              y0 = ex2(y0);
-              y1 = ex2(y1);
-              a = add2(a, pair_of(x0, x1));
-              b = add2(b, pair_of(y0, y1));
-              w[j] = pack_bf16(x0, x1);
-              w[j + 1] = pack_bf16(y0, y1);
-            }
-            tmem_st_u32x16(s_addr + h * 32 + q * 16, w);
+          for (int j = 0; j < 32; j += 2) {
+            float x0, x1, y0, y1;
+            unpair(fma2(pair_of(v[2 * j], v[2 * j + 1]), scale2, minus), x0, x1);
+            unpair(fma2(pair_of(v[2 * j + 2], v[2 * j + 3]), scale2, minus), y0, y1);
+            x0 = ex2(x0);
+            x1 = ex2(x1);
+            y0 = ex2(y0);
+            y1 = ex2(y1);
+            a = add2(a, pair_of(x0, x1));
+            b = add2(b, pair_of(y0, y1));
+            w[j] = pack_bf16(x0, x1);
+            w[j + 1] = pack_bf16(y0, y1);
           }
-          part[h] = add2(a, b);
+          float x, y;
+          unpair(add2(a, b), x, y);
+          return x + y;
         };
-        auto publish = [&](int h) {
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_ready[2 * i + h]);
-        };
-        float m0 = max3(v[0], v[1], v[2]), m1 = max3(v[3], v[4], v[5]);
-#pragma unroll
-        for (int j = 6; j < 126; j += 4) {
-          m0 = max3(m0, v[j], v[j + 1]);
-          m1 = max3(m1, v[j + 2], v[j + 3]);
+        scores(0);
+        float top = high, part = exponentials();
+        if (both) {
+          scores(1);
+          top = fmaxf(top, high);
         }
-        const float top = max3(fmaxf(m0, m1), v[126], v[127]) * p.scale2;
-        exponentials(0);
+        top *= p.scale2;
         const bool move = top > ref + kLazy || (c == 0 && top < -kFar);
         if (__any_sync(0xffffffffu, move)) {
           const float f = move ? ex2(ref - top) : 1.f;
@@ -455,14 +512,18 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
               tmem_st16(o_addr + d, o);
             }
           }
-          exponentials(0);
+          scores(0);  // P has not overwritten them yet
+          part = exponentials();
+          if (both) scores(1);
         }
+        tmem_store32(s_addr, w);
         publish(0);
-        exponentials(1);
+        if (both) {
+          part += exponentials();
+          tmem_store32(s_addr + 32, w);
+        }
         publish(1);
-        float a, b;
-        unpair(add2(part[0], part[1]), a, b);
-        sum += a + b;
+        sum += part;
       }
       if (!ok) break;
       if (n_mine > 0) {
@@ -478,7 +539,14 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
                    (items.tile.y - first) << p.lp, p.D};
 #pragma unroll 1
         for (int d = 0; d < p.D; d += 64, to.dst += 64, to.cols -= 64)
-          stage_tmem64(o_addr + d, inv, stages + warp * 4096, to, quad * 32, lane);
+          stage_tmem64<false>(o_addr + d, inv, stages + warp * 4096, to, quad * 32, lane);
+        if (p.rest != nullptr) {
+          to.dst += p.rest - p.out - (p.D + 63) / 64 * 64;
+          to.cols = p.D;
+#pragma unroll 1
+          for (int d = 0; d < p.D; d += 64, to.dst += 64, to.cols -= 64)
+            stage_tmem64<true>(o_addr + d, inv, stages + warp * 4096, to, quad * 32, lane);
+        }
         tc_fence_before();  // the next item's first P . V overwrites O after this warp's next p_ready
       }
     }
@@ -491,12 +559,12 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
 }
 
 template <int DP, int kTiles>
-int run_fwd(const PackedMaps& maps, const PackedArgs& a, void* out, float* lse, unsigned* status,
+int run_fwd(const PackedMaps& maps, const PackedArgs& a, void* out, void* rest, float* lse, unsigned* status,
             cudaStream_t stream) {
   using Cfg = FwdCfg<DP, kTiles>;
   auto kernel = packed_fwd_kernel<DP, kTiles>;
   if (set_max_smem(kernel, Cfg::kSmem) != cudaSuccess) return -1;
-  const FwdArgs args{static_cast<bf16*>(out), lse, static_cast<const int4*>(a.fwd.entries), a.fwd.head, a.T, a.H,
+  const FwdArgs args{static_cast<bf16*>(out), static_cast<bf16*>(rest), lse, static_cast<const int4*>(a.fwd.entries), a.fwd.head, a.T, a.H,
                      a.Hkv, a.D, a.lp, a.scale * kLog2e};
   const long most = static_cast<long>(a.fwd.max_tiles) * (a.H >> a.lp);
   if (most > 0x7fff0000l) return -2;
@@ -528,13 +596,13 @@ int launch_packed_plan(const int* cu, int B, int T, const PackedTable* tables, i
 
 bool packed_single_tiles(int T, int B) { return static_cast<long>(T) < 512l * B; }
 
-int launch_packed_forward(const PackedMaps& maps, const PackedArgs& a, void* out, float* lse, int tiles,
+int launch_packed_forward(const PackedMaps& maps, const PackedArgs& a, void* out, void* rest, float* lse, int tiles,
                           unsigned* status, cudaStream_t stream) {
   if (tiles == 1)
-    return a.D <= 64 ? run_fwd<64, 1>(maps, a, out, lse, status, stream)
-                     : run_fwd<128, 1>(maps, a, out, lse, status, stream);
-  return a.D <= 64 ? run_fwd<64, 2>(maps, a, out, lse, status, stream)
-                   : run_fwd<128, 2>(maps, a, out, lse, status, stream);
+    return a.D <= 64 ? run_fwd<64, 1>(maps, a, out, rest, lse, status, stream)
+                     : run_fwd<128, 1>(maps, a, out, rest, lse, status, stream);
+  return a.D <= 64 ? run_fwd<64, 2>(maps, a, out, rest, lse, status, stream)
+                   : run_fwd<128, 2>(maps, a, out, rest, lse, status, stream);
 }
 
 }  // namespace ecz

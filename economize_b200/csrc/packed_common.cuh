@@ -22,6 +22,12 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
+// What packing a and b into `packed` rounded away, packed the same way.
+__device__ __forceinline__ uint32_t rest_of(uint32_t packed, float a, float b) {
+  const float2 kept = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&packed));
+  return pack_bf16(a - kept.x, b - kept.y);
+}
+
 // Two fp32 values in a 64-bit register and the operations on both at once, and the maximum of three.
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
   uint64_t r;
@@ -267,7 +273,8 @@ __device__ __forceinline__ void store_tmem64(uint32_t taddr, float f, const Tile
 }
 
 // The same through 4 KB of shared memory of the warp (16-byte groups swizzled by the row, so that neither side
-// conflicts), with fewer instructions.
+// conflicts), with fewer instructions. kRest: what bf16 rounds away of the values instead (itself rounded to bf16).
+template <bool kRest>
 __device__ __forceinline__ void stage_tmem64(uint32_t taddr, float f, uint8_t* stage, const TileOut& to, int row0,
                                              int lane) {
   const uint64_t ff = pair_of(f, f);
@@ -284,6 +291,7 @@ __device__ __forceinline__ void stage_tmem64(uint32_t taddr, float f, uint8_t* s
         float a, b;
         unpair(mul2(pair_of(o[8 * j + 2 * k], o[8 * j + 2 * k + 1]), ff), a, b);
         w[k] = pack_bf16(a, b);
+        if (kRest) w[k] = rest_of(w[k], a, b);
       }
       *reinterpret_cast<uint4*>(mine + (((h * 4 + j) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
     }

@@ -238,6 +238,16 @@ def test_same_bits_every_time(cuda):
         assert all(torch.equal(a, b) for a, b in zip(first, _run(q, k, v, cu, dout)))
 
 
+@pytest.mark.parametrize("lens", [[2] * 40, [1, 2, 3, 4] * 10, [1] * 30 + [2], [3] * 50], ids=lambda x: f"{len(x)} of {x[0]}-{x[-1]}")
+def test_gradients_of_sequences_of_a_few_tokens(cuda, lens):
+    """dp - delta cancels there: delta needs more of the output than its bf16 rounding keeps. The whole gradient is as
+    near its 64-bit value as two roundings to bf16 leave it (u / sqrt(3) each, operand and result, a fifth added)."""
+    q, k, v, cu, dout = _inputs(cuda, lens, 8, 2, 64, seed=21)
+    z = _oracle(q, k, v, lens, dout, 0.125)
+    for name, got in zip(("dq", "dk", "dv"), _run(q, k, v, cu, dout)[1:]):
+        assert (got.double() - z[name]).norm() <= 1.2 * U * math.sqrt(2 / 3) * z[name].norm(), name
+
+
 def test_gradients_by_differences(cuda):
     """The slope of the 64-bit formula along random directions, against the kernels' gradients."""
     lens, dim, h = [70, 131], 64, 1e-4
