@@ -85,7 +85,8 @@ std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> readout(
     return {loss, dx, dw};
   }
   const bool grads = need_dx || need_dw;
-  const int64_t ld = (V + 7) / 8 * 8;
+  // rows of e and of the packed states start on 128-byte lines, or every row of a TMA box would touch two
+  const int64_t ld = (V + 63) / 64 * 64, xld = (H + 63) / 64 * 64;
   // Rows of a chunk: 1 GiB of e; with dW as much as the fp32 sum of several chunks would take (4 V H bytes).
   int64_t chunk = T;
   if (chunk_rows > 0) {
@@ -112,7 +113,7 @@ std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> readout(
   const bool planned = ecz::readout_needs_plan(static_cast<int>(T));
   const int64_t o_rows = place(4 * T), o_target = place(4 * T), o_pos = place(planned ? 4 * T : 0), o_count = place(8);
   const int64_t o_picked = place(4 * T), o_nll = place(4 * T), o_stats = place(8 * chunk * pieces);
-  const int64_t o_xs = place(2 * (T + 64) * H), o_e = place(grads ? 2 * chunk * ld : 0);
+  const int64_t o_xs = place(2 * (T + 64) * xld), o_e = place(grads ? 2 * chunk * ld : 0);
   const int64_t o_part = place(splits > 1 ? 4 * splits * chunk * H : 0);
   const int64_t o_sum = place(need_dw && chunks > 1 ? 4 * V * H : 0);
   Tensor workspace = at::empty({bytes}, hidden.options().dtype(at::kByte));
@@ -129,6 +130,7 @@ std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> readout(
   r.w = w.data_ptr();
   r.x_stride = row_stride(x);
   r.w_stride = row_stride(w);
+  r.xs_stride = xld;
   r.targets = targets.data_ptr<int64_t>();
   r.T = static_cast<int>(T);
   r.H = static_cast<int>(H);
@@ -158,8 +160,8 @@ std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> readout(
     c.ld = ld;
     c.logit_scale = r.logit_scale;
     const int64_t padded = (c.chunk + 63) / 64 * 64;  // rows of xs and e that the maps may read
-    uint8_t* xs0 = xs + static_cast<int64_t>(c.row0) * H * 2;
-    const CUtensorMap x_rows = map_2d(xs0, padded, H, H, 128);
+    uint8_t* xs0 = xs + static_cast<int64_t>(c.row0) * xld * 2;
+    const CUtensorMap x_rows = map_2d(xs0, padded, H, xld, 128);
     check(ecz::launch_readout_logits(&x_rows, &w_rows, c, sms, status, stream), "logits");
     const bool sums = want_loss && !per_row;
     check(ecz::launch_readout_finish(c, static_cast<int>(reduction),
@@ -175,7 +177,7 @@ std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> readout(
     }
     if (need_dw) {
       const CUtensorMap dz = map_2d(e, padded, V, ld, 64);
-      const CUtensorMap x_cols = map_2d(xs0, padded, H, H, 64);
+      const CUtensorMap x_cols = map_2d(xs0, padded, H, xld, 64);
       check(ecz::launch_readout_dw(&dz, &x_cols, c, chunks > 1 ? reinterpret_cast<float*>(ws + o_sum) : nullptr, i == 0,
                                    i == chunks - 1, dw->data_ptr(), sms, status, stream),
             "dw");

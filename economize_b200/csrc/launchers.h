@@ -284,7 +284,7 @@ struct ReadoutChunk {
   void* stats = nullptr;        // float2 [chunk, readout_pieces(V)]
   const float* picked = nullptr;  // [T] target's logit of a packed row, log2 units
   void* e = nullptr;            // fp16 e, then bf16 dz [chunk up to a multiple of 64, ld], or null (losses only)
-  long ld = 0;                  // a multiple of 8
+  long ld = 0;                  // a multiple of 64
   float logit_scale = 1.f;
 };
 int readout_pieces(int V);
@@ -292,7 +292,7 @@ int readout_splits(long tiles, long kblocks, int num_sms);
 // The states and head as given.
 struct ReadoutRows {
   const void *x = nullptr, *w = nullptr;
-  long x_stride = 0, w_stride = 0;
+  long x_stride = 0, w_stride = 0, xs_stride = 0;
   const int64_t* targets = nullptr;
   int T = 0, H = 0, V = 0;
   int64_t ignore = 0;

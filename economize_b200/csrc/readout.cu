@@ -88,7 +88,7 @@ constexpr int kPlanRows = 2048;  // rows up to which counting costs less than a 
 
 struct GatherArgs {
   const bf16 *x, *w;
-  long x_stride, w_stride;
+  long x_stride, w_stride, xs_stride;
   const int64_t* targets;
   int T, H, V;
   int64_t ignore;
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(256) readout_gather_kernel(const __grid_consta
   if (t >= a.T) {
     const int r = n + (t - a.T);
     if (t - a.T < pair::kBK && r < (n + pair::kBK - 1) / pair::kBK * pair::kBK)
-      for (int c = lane * 8; c < a.H; c += 256) *reinterpret_cast<uint4*>(a.xs + static_cast<size_t>(r) * a.H + c) = zero;
+      for (int c = lane * 8; c < a.H; c += 256) *reinterpret_cast<uint4*>(a.xs + static_cast<size_t>(r) * a.xs_stride + c) = zero;
     return;
   }
   if (p < 0) {
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(256) readout_gather_kernel(const __grid_consta
   float acc[2] = {0.f, 0.f};
   for (int c = lane * 8; c < a.H; c += 256) {
     const uint4 u = *reinterpret_cast<const uint4*>(x + c), v = *reinterpret_cast<const uint4*>(w + c);
-    *reinterpret_cast<uint4*>(a.xs + static_cast<size_t>(p) * a.H + c) = u;
+    *reinterpret_cast<uint4*>(a.xs + static_cast<size_t>(p) * a.xs_stride + c) = u;
     const uint32_t l[4] = {u.x, u.y, u.z, u.w}, r[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -522,7 +522,7 @@ int launch_readout_plan(const int64_t* targets, int T, int V, int64_t ignore, in
 
 int launch_readout_gather(const ReadoutRows& r, const int* pos, int* rows, int* target_of, int* count, float* picked,
                           void* xs, void* dx, float* losses, unsigned* status, cudaStream_t stream) {
-  const GatherArgs a{static_cast<const bf16*>(r.x), static_cast<const bf16*>(r.w), r.x_stride, r.w_stride, r.targets, r.T,
+  const GatherArgs a{static_cast<const bf16*>(r.x), static_cast<const bf16*>(r.w), r.x_stride, r.w_stride, r.xs_stride, r.targets, r.T,
                      r.H, r.V, r.ignore, r.logit_scale * kLog2e, pos, rows, target_of, count, picked,
                      static_cast<bf16*>(xs), static_cast<bf16*>(dx), losses};
   return launch_pdl(readout_gather_kernel, dim3((r.T + pair::kBK + 7) / 8), dim3(256), 0, stream, a, status) ==
