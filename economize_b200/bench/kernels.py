@@ -21,6 +21,11 @@ peaks. Ops:
 * ``glu``        CATS's gated rows (``glu_rows``: up rows of the channels with ``|silu(gate)| > t``, ``--n`` = FFN
   width, ``--k`` = hidden) at ``--sparsity``, vs the dense up projection GEMM
 
+* ``packed_attention`` forward and backward of causal attention over ``--batch`` packed documents of ``--ctx`` tokens
+  (32 heads over 8, head dimension 128), vs the library's attention document by document after repeating K and V
+* ``readout``    cross-entropy of ``--m`` rows over a vocabulary of ``--n`` (hidden ``--k``) with both gradients, vs fp32
+  logits through the library's product and loss
+
 ``--once`` runs a single call without timing (the case a profiler captures).
 """
 
@@ -338,10 +343,64 @@ def bench_hadamard(a) -> None:
             a.m * F_ * (block.bit_length() - 1), plain)
 
 
+def bench_packed_attention(a) -> None:
+    from .. import ops
+
+    dev = torch.device("cuda")
+    heads, kv_heads, dim, total = 32, 8, 128, a.batch * a.ctx
+    q, k, v = (torch.randn(total, h, dim, device=dev).bfloat16().requires_grad_() for h in (heads, kv_heads, kv_heads))
+    dout = torch.randn(total, heads, dim, device=dev).bfloat16()
+    cu = torch.arange(a.batch + 1, device=dev, dtype=torch.int32) * a.ctx
+
+    def ours():
+        return torch.autograd.grad(ops.packed_attention(q, k, v, cu), (q, k, v), dout)
+
+    def library():
+        def rows(x, n):
+            x = x.view(a.batch, a.ctx, n, dim).transpose(1, 2)
+            return x.repeat_interleave(heads // n, 1)
+
+        o = torch.nn.functional.scaled_dot_product_attention(rows(q, heads), rows(k, kv_heads), rows(v, kv_heads),
+                                                             is_causal=True)
+        return torch.autograd.grad(o.transpose(1, 2).reshape(total, heads, dim), (q, k, v), dout)
+
+    if a.once:
+        ours()
+        torch.cuda.synchronize()
+        return
+    pairs = heads * a.batch * a.ctx * (a.ctx + 1) // 2
+    _report("packed_attention", {"documents": a.batch, "tokens": a.ctx, "heads": heads, "kv_heads": kv_heads},
+            time_call(ours, a.iters, a.warmup).median_ms, 8 * total * dim * (heads + kv_heads), 14 * dim * pairs,
+            time_call(library, a.iters, a.warmup).median_ms)
+
+
+def bench_readout(a) -> None:
+    from .. import ops
+
+    dev = torch.device("cuda")
+    x = torch.randn(a.m, a.k, device=dev).bfloat16().requires_grad_()
+    w = (torch.randn(a.n, a.k, device=dev) * 0.02).bfloat16().requires_grad_()
+    y = torch.randint(0, a.n, (a.m,), device=dev)
+
+    def ours():
+        return torch.autograd.grad(ops.linear_cross_entropy(x, w, y), (x, w))
+
+    def library():
+        logits = torch.nn.functional.linear(x, w).float()
+        return torch.autograd.grad(torch.nn.functional.cross_entropy(logits, y), (x, w))
+
+    if a.once:
+        ours()
+        torch.cuda.synchronize()
+        return
+    _report("readout", {"rows": a.m, "vocab": a.n, "hidden": a.k}, time_call(ours, a.iters, a.warmup).median_ms,
+            4 * (a.m + a.n) * a.k, 6 * a.m * a.n * a.k, time_call(library, a.iters, a.warmup).median_ms)
+
+
 def main(argv: list[str] | None = None) -> None:
     p = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     p.add_argument("op", choices=["gemm", "gemm_sweep", "gemm_wq", "attention", "layer", "teal", "glu", "topk",
-                                  "hadamard"])
+                                  "hadamard", "packed_attention", "readout"])
     p.add_argument("--ms", type=int, nargs="+", default=[1, 8, 61, 488], help="gemm_sweep: token counts")
     p.add_argument("--topk", type=int, default=10)
     p.add_argument("--m", type=int, default=61)
@@ -362,7 +421,8 @@ def main(argv: list[str] | None = None) -> None:
     p.add_argument("--trace", action="store_true", help="attention: per-CTA phase timeline from the kernel's stamps")
     a = p.parse_args(argv)
     {"gemm": bench_gemm, "gemm_sweep": bench_gemm_sweep, "gemm_wq": bench_gemm_wq, "attention": bench_attention, "layer": bench_layer,
-     "teal": bench_teal, "glu": bench_glu, "topk": bench_topk, "hadamard": bench_hadamard}[a.op](a)
+     "teal": bench_teal, "glu": bench_glu, "topk": bench_topk, "hadamard": bench_hadamard,
+     "packed_attention": bench_packed_attention, "readout": bench_readout}[a.op](a)
 
 
 if __name__ == "__main__":

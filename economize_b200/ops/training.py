@@ -1,7 +1,8 @@
 """Operators of training steps, with autograd: the readout cross-entropy and causal attention over packed documents.
 
 On CUDA both directions are the hand-written kernels of ``csrc/readout.cu``, ``csrc/packed_attention.cu`` and
-``csrc/packed_attention_bwd.cu`` (autograd functions in ``csrc/bindings_train.cpp``); CPU tensors take the formulas of :mod:`.reference` (autograd differentiates them). There is no third path.
+``csrc/packed_attention_bwd.cu`` (autograd functions in ``csrc/bindings_train.cpp``); CPU tensors take the formulas of
+:mod:`.reference` (autograd differentiates them). There is no third path.
 """
 
 from __future__ import annotations

@@ -11,7 +11,8 @@ channels are dropped without it. Refuses tensor-parallel models, like the refere
 ``recovery_rank > 0`` adds LLM-Pruner's recovery stage (economize ``width_prune/recovery.py:25``): a LoRA update
 (rank ``recovery_rank``, ``alpha = recovery_alpha``) of every pruned layer's projections that is always applied (the
 pruned model is the base, there is no exact path to protect); ``train.fit(model, tokens)`` trains it with the
-``recovery_ce`` objective (next-token cross-entropy of the pruned model), and the adapters are listed by
+``recovery_ce`` objective (next-token cross-entropy of the pruned model), or over packed documents with
+``objective="packed_recovery_ce"`` (:mod:`economize_b200.train.packed`), and the adapters are listed by
 :meth:`WidthPruneTechnique.lora_targets` for PEFT export.
 """
 

@@ -9,11 +9,12 @@ from .config import TrainConfig
 from .data import TensorSource, greedy_continuations
 from .loop import TrainResult, fit
 from .objective import OBJECTIVES, Eagle3TTT, Objective, OptimDefaults, default_objective, teacher_pass
+from .packed import PackedBatch, PackedSource, pack
 from .teacher import larger_teacher
 
-__all__ = ["larger_teacher", "OBJECTIVES", "Eagle3TTT", "Objective", "OptimDefaults", "RunCheckpointer", "TensorSource",
-           "TrainConfig", "TrainResult", "default_objective", "fit", "fit_eagle3_on_greedy", "greedy_continuations",
-           "teacher_pass"]
+__all__ = ["larger_teacher", "OBJECTIVES", "Eagle3TTT", "Objective", "OptimDefaults", "PackedBatch", "PackedSource",
+           "RunCheckpointer", "TensorSource", "TrainConfig", "TrainResult", "default_objective", "fit",
+           "fit_eagle3_on_greedy", "greedy_continuations", "pack", "teacher_pass"]
 
 
 def fit_eagle3_on_greedy(model, steps: int = 200, n_rows: int = 64, prompt_len: int = 256, new_tokens: int = 128,

@@ -207,9 +207,12 @@ def _check_plain_block(config) -> None:
                           f"{', '.join(found)}")
 
 
-def torch_block(layer, h: torch.Tensor, config, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+def torch_block(layer, h: torch.Tensor, config, cos: torch.Tensor, sin: torch.Tensor,
+                cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
     """A pre-norm decoder block in plain PyTorch (autograd, causal attention over the whole row): the residual
-    stream ``h [B, S, H]`` in, the block's output stream out. Used to train technique-owned blocks and adapters."""
+    stream ``h [B, S, H]`` in, the block's output stream out. Used to train technique-owned blocks and adapters.
+    With ``cu_seqlens`` the one row ``h [1, T, H]`` is packed sequences, each attended by itself
+    (:func:`~economize_b200.ops.packed_attention`), and ``cos`` / ``sin [T, D / 2]`` are those of its positions."""
     import torch.nn.functional as F
 
     from ..ops.reference import rmsnorm
@@ -231,12 +234,15 @@ def torch_block(layer, h: torch.Tensor, config, cos: torch.Tensor, sin: torch.Te
         a, b = t[..., : hd // 2], t[..., hd // 2:]
         return torch.cat([a * c - b * s, b * c + a * s], -1)
 
-    q, k = rot(q).transpose(1, 2), rot(k).transpose(1, 2)
-    v = v.reshape(batch, length, kv_heads, hd).transpose(1, 2)
-    group = heads // kv_heads
-    o = F.scaled_dot_product_attention(q, k.repeat_interleave(group, 1), v.repeat_interleave(group, 1),
-                                       is_causal=True)
-    h = h + lin(o.transpose(1, 2).reshape(batch, length, heads * hd), layer.wo)
+    if cu_seqlens is None:
+        q, k = rot(q).transpose(1, 2), rot(k).transpose(1, 2)
+        v = v.reshape(batch, length, kv_heads, hd).transpose(1, 2)
+        group = heads // kv_heads
+        o = F.scaled_dot_product_attention(q, k.repeat_interleave(group, 1), v.repeat_interleave(group, 1),
+                                           is_causal=True).transpose(1, 2)
+    else:
+        o = ops.packed_attention(rot(q)[0], rot(k)[0], v.reshape(length, kv_heads, hd), cu_seqlens)
+    h = h + lin(o.reshape(batch, length, heads * hd), layer.wo)
     x = rmsnorm(h, layer.mlp_norm, eps)[0]
     g, u = lin(x, layer.w_gate_up).chunk(2, -1)
     a = F.silu(g) * u
