@@ -274,7 +274,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> packed_forward(Tensor q, Tensor k, Te
   v = heads_of(v);
   cu = cu.contiguous();
   const int T = static_cast<int>(q.size(0)), B = static_cast<int>(cu.size(0)) - 1;
-  if (tiles == 0) tiles = ecz::packed_single_tiles(T, B) ? 1 : 2;
+  if (tiles == 0) tiles = ecz::packed_single_tiles(T, B, static_cast<int>(q.size(2))) ? 1 : 2;
   const int count = training ? 3 : 1;
   ecz::PackedArgs a = packed_args(q, k, B, scale, static_cast<int>(tiles), count, Tensor());
   int64_t ints = 0;
@@ -321,9 +321,15 @@ std::tuple<Tensor, Tensor, Tensor> packed_backward(Tensor dout, Tensor q, Tensor
   v = heads_of(v);
   dout = heads_of(dout);
   const ecz::PackedArgs a = packed_args(q, k, B, scale, static_cast<int>(tiles), 3, plan);
-  Tensor delta = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
-  TORCH_CHECK(ecz::launch_packed_delta(out.data_ptr(), rest.data_ptr(), dout.data_ptr(), dout.stride(0), dout.stride(1), a.T, a.H, a.D,
-                                       delta.data_ptr<float>(), stream) == 0,
+  // delta [H, T] and the two kernels' item counters
+  const int64_t rows = q.size(1) * q.size(0);
+  Tensor delta = at::empty({rows + 2}, q.options().dtype(at::kFloat));
+  int* taken = reinterpret_cast<int*>(delta.data_ptr<float>() + rows);
+  const int splits = need_dkv ? ecz::packed_dkv_splits(a, static_cast<int>(B)) : 1;
+  Tensor part;
+  if (splits > 1) part = at::empty({splits, 2, k.size(0), k.size(1), k.size(2)}, delta.options());
+  TORCH_CHECK(ecz::launch_packed_delta(a, out.data_ptr(), rest.data_ptr(), dout.data_ptr(), dout.stride(0),
+                                       dout.stride(1), delta.data_ptr<float>(), taken, stream) == 0,
               "packed_attention: delta launch failed");
   ecz::PackedMaps maps;
   maps.q = map_heads(q, 1 << a.lp, 128 >> a.lp);
@@ -334,8 +340,9 @@ std::tuple<Tensor, Tensor, Tensor> packed_backward(Tensor dout, Tensor q, Tensor
   maps.v32 = map_heads(v, 1, 32);
   const int rc = ecz::launch_packed_backward(maps, a, lse.data_ptr<float>(), delta.data_ptr<float>(),
                                              need_dq ? dq.data_ptr() : nullptr, need_dkv ? dk.data_ptr() : nullptr,
-                                             need_dkv ? dv.data_ptr() : nullptr, ecz::device_status(q.device()),
-                                             stream);
+                                             need_dkv ? dv.data_ptr() : nullptr, splits,
+                                             splits > 1 ? part.data_ptr<float>() : nullptr, taken,
+                                             ecz::device_status(q.device()), stream);
   TORCH_CHECK(rc == 0, "packed_attention: backward launch failed (", rc, ")");
   return {dq, dk, dv};
 }
@@ -422,7 +429,8 @@ struct PackedFunction : torch::autograd::Function<PackedFunction> {
                         double scale, int64_t tiles) {
     const int64_t B = cu.dim() == 1 ? cu.size(0) - 1 : 0;
     if (tiles == 0 && q.dim() == 3)
-      tiles = ecz::packed_single_tiles(static_cast<int>(q.size(0)), static_cast<int>(B)) ? 1 : 2;
+      tiles = ecz::packed_single_tiles(static_cast<int>(q.size(0)), static_cast<int>(B), static_cast<int>(q.size(2)))
+                  ? 1 : 2;
     auto r = packed_forward(q, k, v, cu, scale, true, tiles);
     ctx->save_for_backward({q, k, v, std::get<0>(r)});
     ctx->saved_data["rest"] = std::get<1>(r);

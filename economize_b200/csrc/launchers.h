@@ -340,17 +340,21 @@ int packed_max_tiles(int T, int B, int rows);
 int launch_packed_plan(const int* cu, int B, int T, const PackedTable* tables, int count, unsigned* status,
                        cudaStream_t stream);
 // tiles: query tiles a CTA works on, 1 or 2 (packed_single_tiles: whether 1 is the better for T tokens in B sequences).
-bool packed_single_tiles(int T, int B);
+bool packed_single_tiles(int T, int B, int D);
 // rest: what out's rounding to bf16 left of the output (for the backward pass), or null.
 int launch_packed_forward(const PackedMaps& maps, const PackedArgs& a, void* out, void* rest, float* lse, int tiles,
                           unsigned* status, cudaStream_t stream);
 
 // packed_attention_bwd.cu: delta [H, T] = rows of dout . (out + rest) (both contiguous [T, H, D]), then the gradients (dq null:
 // not computed; dk and dv null: not computed).
-int launch_packed_delta(const void* out, const void* rest, const void* dout, long stride_t, long stride_h, int T, int H, int D,
-                        float* delta, cudaStream_t stream);
+// taken: two counters, set to zero by the first for the second. part: fp32 [splits, 2, T, Hkv, D], for
+// splits > 1 (packed_dkv_splits: how many CTAs share a key tile's queries).
+int packed_dkv_splits(const PackedArgs& a, int B);
+int launch_packed_delta(const PackedArgs& a, const void* out, const void* rest, const void* dout, long stride_t,
+                        long stride_h, float* delta, int* taken, cudaStream_t stream);
 int launch_packed_backward(const PackedMaps& maps, const PackedArgs& a, const float* lse, const float* delta, void* dq,
-                           void* dk, void* dv, unsigned* status, cudaStream_t stream);
+                           void* dk, void* dv, int splits, float* part, int* taken, unsigned* status,
+                           cudaStream_t stream);
 
 // tmap.cpp: 3-D bf16 tensor map {d, heads, tokens} with strides in elements, box {64, box_heads, box_tokens}, 128-byte
 // swizzle.

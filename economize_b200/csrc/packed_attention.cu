@@ -8,7 +8,7 @@
 // (the largest of these that divides it) and 128, 64, 32 or 16 tokens. All heads of a pack read the same K / V chunk, a
 // short sequence fills its tiles better (85 tokens of four heads are three tiles, not four), and less of the diagonal
 // chunk is computed in vain. The plan kernel cuts every sequence into tiles from its first token on, so a tile never
-// mixes sequences, and lists them heaviest first: the last ones dealt to the persistent CTAs (see Items) are short.
+// mixes sequences, and lists them heaviest first: the last ones dealt to the persistent CTAs (see Feed) are short.
 //
 // A CTA works on one or two neighbouring query tiles over the same K / V chunks. One warp loads (TMA, a ring of 128-key
 // K and V chunks), one issues the MMAs, and a warpgroup per tile runs its softmax, one thread per row, so the tensor
@@ -39,7 +39,7 @@ constexpr float kFar = 60.f;
 
 // ---- plan ----------------------------------------------------------------------------------------------------------
 // One CTA per table: a list of tiles of `rows` tokens, heaviest first: entry = (first token, end, tile, tiles of its
-// sequence); head = (tiles, first token of the first sequence, end of the last). Offsets outside [0, T] or falling are
+// sequence); head = (tiles, first token of the first sequence, end of the last, items taken). Offsets outside [0, T] or falling are
 // clamped (a sequence starts where the one before it ended at the earliest) and reported.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanTables = 3;
@@ -139,6 +139,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     table.head[0] = tiles;
     table.head[1] = lo[0];
     table.head[2] = lo[B];
+    table.head[3] = 0;
   }
   int total;
   const int mine = scan_add(change[tid], sums, total) + change[tid] + rest[tid];
@@ -170,7 +171,7 @@ struct FwdCfg {
   static constexpr int kTileBytes = kRowsT * DP * 2;
   static constexpr int kRing = (DP == 64 ? 4 : 2) * kTiles;  // K and V chunks in turn
   static constexpr int kStage = kTiles * 4 * 4096;           // 4 KB for each softmax warp's output rows
-  static constexpr int kSmem = (kTiles + kRing) * kTileBytes + kStage + 512;
+  static constexpr int kSmem = (kTiles + kRing) * kTileBytes + kStage + 512;  // and barriers, WorkRing
   static constexpr int kSoftmaxWarps = 4 * kTiles;
   static constexpr int kThreads = 32 * (kSoftmaxWarps + 2);  // and a warp each for loads and MMAs
   static constexpr int kTmem = 256 * kTiles;                 // S of every tile, then O of every tile
@@ -183,6 +184,7 @@ struct FwdArgs {
   float* lse;  // [H, T] log2-domain log-sum-exp, or null
   const int4* table;  // entries of kTiles query tiles
   const int* head;
+  int* taken;  // items given out
   int T, H, Hkv, D, lp;
   float scale2;  // scale times log2(e)
 };
@@ -206,7 +208,8 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
   uint64_t* s_full = kv_empty + kRing;   // [2] scores of a tile's chunk are in TMEM
   uint64_t* p_ready = s_full + 2;        // [2][2] its probabilities are, by halves of the chunk's keys
   uint64_t* o_done = p_ready + 4;        // [2] P . V of the chunk is complete
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+  const WorkRing work(o_done + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(work.empty + kWorkRing);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -224,6 +227,7 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
       mbar_init(&p_ready[2 * i + 1], 4);
       mbar_init(&o_done[i], 1);
     }
+    work.init(Cfg::kSoftmaxWarps + 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tm_q);
@@ -257,18 +261,18 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
 
   if (warp == kLoadWarp) {
     // ---- loads: an item's Q, then its K and V chunks in turn ----
-    Items<> items(p.table, p.head, per);
+    Feed items(work, p.table, p.head, p.taken, per);
     const uint32_t qa = smem_u32(q_tiles), ra = smem_u32(ring);
     int it = 0;
     bool ok = true;
-    for (int n_items = 0; ok && items.next(); ++n_items) {
+    for (int n_items = 0; ok && items.next(lane, status, abort_flag); ++n_items) {
       const int lo = items.tile.x, c1 = chunks_of(items, 1), n = max(chunks_of(items, 0), c1);
       const int head = items.sub << p.lp, kvh = head / group;
       const int first = token_of(items, 0), last_keys = keys_of(items, c1 > 0 ? 1 : 0, n - 1);
-      items.look();
       if (lane == 0) {
         auto chunk = [&](int x) {  // K (even) or V (odd) of a chunk
           const int s = (it + x) % kRing, c = x >> 1;
+          if (x == 2 * n - 2) items.reserve();
           if (!mbar_wait(&kv_empty[s], (((it + x) / kRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag)) return false;
           load_chunk<DP>(ra + s * kTileBytes, (x & 1) ? &tm_v : &tm_k, (x & 1) ? &tm_v32 : &tm_k32, &kv_full[s], kvh,
                          lo + c * kRowsT, c + 1 < n ? kRowsT : last_keys);
@@ -288,7 +292,7 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
     }
   } else if (warp == kMmaWarp) {
     // ---- MMAs ----
-    Items<> items(p.table, p.head, per);
+    Items items(work);
     const bool leader = elect_one();
     const uint32_t qa = smem_u32(q_tiles), ra = smem_u32(ring);
     int base = 0;            // ring position of the item's first chunk
@@ -297,7 +301,7 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
     auto wait_ring = [&](int it) {
       return warp_wait(&kv_full[it % kRing], (it / kRing) & 1, status, kStatusWaitFull, abort_flag);
     };
-    for (int n_items = 0; ok && items.next(); ++n_items) {
+    for (int n_items = 0; ok && items.next(status, abort_flag); ++n_items) {
       const int chunks[2] = {chunks_of(items, 0), chunks_of(items, 1)};
       const int n_chunks = max(chunks[0], chunks[1]);
       const int left = items.tile.y - items.tile.x;  // keys of the sequence
@@ -319,7 +323,6 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
         if (n_chunks == 1) umma_commit(q_empty);
       }
       __syncwarp();
-      items.look();
       for (int c = 0; ok && c < n_chunks; ++c) {
         const int v_it = base + 2 * c + 1, k_it = v_it + 1;
         const bool more = c + 1 < n_chunks;
@@ -383,10 +386,10 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
     const int i = warp >> 2, quad = warp & 3;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t s_addr = lane_base + i * 128, o_addr = lane_base + kTiles * 128 + i * DP;
-    Items<false> items(p.table, p.head, per);
+    Items items(work);
     uint32_t used = 0;  // chunks of this tile so far, over all items
     bool ok = true;
-    while (ok && items.next()) {
+    while (ok && items.next(status, abort_flag)) {
       const int n_mine = chunks_of(items, i);
       const int first = token_of(items, i), token = first + ((quad * 32 + lane) >> p.lp);
       // Exponentials are taken against a reference that is settled beforehand (0 for a row's first chunk): the chunk's
@@ -564,8 +567,8 @@ int run_fwd(const PackedMaps& maps, const PackedArgs& a, void* out, void* rest, 
   using Cfg = FwdCfg<DP, kTiles>;
   auto kernel = packed_fwd_kernel<DP, kTiles>;
   if (set_max_smem(kernel, Cfg::kSmem) != cudaSuccess) return -1;
-  const FwdArgs args{static_cast<bf16*>(out), static_cast<bf16*>(rest), lse, static_cast<const int4*>(a.fwd.entries), a.fwd.head, a.T, a.H,
-                     a.Hkv, a.D, a.lp, a.scale * kLog2e};
+  const FwdArgs args{static_cast<bf16*>(out), static_cast<bf16*>(rest), lse, static_cast<const int4*>(a.fwd.entries),
+                     a.fwd.head, a.fwd.head + 3, a.T, a.H, a.Hkv, a.D, a.lp, a.scale * kLog2e};
   const long most = static_cast<long>(a.fwd.max_tiles) * (a.H >> a.lp);
   if (most > 0x7fff0000l) return -2;
   const long grid = std::min(most, static_cast<long>(a.num_sms) * (3 - kTiles));
@@ -594,7 +597,11 @@ int launch_packed_plan(const int* cu, int B, int T, const PackedTable* tables, i
                  cudaSuccess ? 0 : -1;
 }
 
-bool packed_single_tiles(int T, int B) { return static_cast<long>(T) < 512l * B; }
+// Measured on one B200, us for one / two tiles: D = 64, 12 heads of their own, 8192 tokens in sequences of 16: 61 / 112, of
+// 128: 23.8 / 31.4, of 1024: 35.9 / 39.0, one of 8192: 152 / 164. D = 128, 32 heads over 8, of 16: 56 / 96, of 128:
+// 47.7 / 46.6, of 512: 69.8 / 63.3, of 1024: 96.5 / 87.0, of 8192: 496 / 447; 6490 tokens in 18 sequences 73.2 / 70.5;
+// 4096 tokens in 48: 32.6 / 35.4.
+bool packed_single_tiles(int T, int B, int D) { return D <= 64 || static_cast<long>(T) < 512l * B; }
 
 int launch_packed_forward(const PackedMaps& maps, const PackedArgs& a, void* out, void* rest, float* lse, int tiles,
                           unsigned* status, cudaStream_t stream) {

@@ -34,19 +34,23 @@ struct BwdArgs {
   const float *lse, *delta;  // [H, T]
   const int4 *dq_table, *dkv_table;  // tiles of queries, tiles of 128 keys
   const int *dq_head, *dkv_head;
+  int* taken;  // [2] items given out: key tiles, query tiles
   int T, H, Hkv, D, lp;
   float scale, scale2;
+  int splits;   // CTAs that share the query tiles of a key tile
+  float* part;  // [splits, 2 (dV, dK), T, Hkv, D] their sums where splits > 1
 };
 
 // delta[h, t] = dout[t, h] . (out[t, h] + rest[t, h]); 16 lanes per row. dp - delta cancels where a row attends few keys:
 // with the output rounded to bf16 alone, dQ and dK of sequences of a few tokens were off by 0.8% (5 times their own
 // rounding), so the forward pass keeps what its rounding leaves.
 __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restrict__ out, const bf16* __restrict__ rest,
-                                                           const bf16* __restrict__ dout,
+                                                           const bf16* __restrict__ dout, int* __restrict__ taken,
                                                            long stride_t, long stride_h, int T, int H, int D,
                                                            float* __restrict__ delta) {
   pdl_trigger();
   pdl_wait();
+  if (blockIdx.x == 0 && threadIdx.x < 2) taken[threadIdx.x] = 0;  // by the kernels that follow
   const long row = (static_cast<long>(blockIdx.x) * 256 + threadIdx.x) >> 4;
   const int c = (threadIdx.x & 15) * 8;
   const bool real = row < static_cast<long>(T) * H;
@@ -102,6 +106,11 @@ struct Walk {
   __device__ __forceinline__ Walk(int first_head, int first_token, int n, int lp)
       : head(first_head), token(first_token), left(n), tiles(n), token0(first_token), tokens(kRowsT >> lp),
         heads(1 << lp) {}
+  __device__ __forceinline__ void skip(int n) {
+    head += n / tiles * heads;
+    token += n % tiles * tokens;
+    left -= n % tiles;
+  }
   __device__ __forceinline__ void next() {
     token += tokens;
     if (--left == 0) {
@@ -113,7 +122,8 @@ struct Walk {
 };
 
 // ---- dK and dV -----------------------------------------------------------------------------------------------------
-template <int DP>
+// kSplit: p.splits CTAs share the query tiles of a key tile and leave their sums, in fp32, to packed_join_kernel.
+template <int DP, bool kSplit>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     packed_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
@@ -133,7 +143,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   uint64_t* ds_ready = dp_full + 1;
   uint64_t* done = ds_ready + 1;
   uint64_t* kv_empty = done + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + 1);
+  const WorkRing work(kv_empty + 1);  // an even number of barriers: on 16 bytes
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(work.empty + kWorkRing);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -155,6 +166,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     mbar_init(dp_full, 1);
     mbar_init(ds_ready, kComputeWarps);
     mbar_init(done, 1);
+    work.init(kComputeWarps + 2);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -168,25 +180,55 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   pdl_trigger();
   pdl_wait();
 
-  zero_padding(p.dk, p.T, static_cast<long>(p.Hkv) * p.D, p.dkv_head);
-  zero_padding(p.dv, p.T, static_cast<long>(p.Hkv) * p.D, p.dkv_head);
-  Items<> items(p.dkv_table, p.dkv_head, p.Hkv);  // sub: the K/V head
+  const int splits = kSplit ? p.splits : 1;
+  if (!kSplit) {
+    zero_padding(p.dk, p.T, static_cast<long>(p.Hkv) * p.D, p.dkv_head);
+    zero_padding(p.dv, p.T, static_cast<long>(p.Hkv) * p.D, p.dkv_head);
+  }
   const int group = p.H / p.Hkv;
   const int ksteps = (p.D + 15) / 16;
   const int tokens = kRowsT >> p.lp, packs = group >> p.lp;
-  // an item's first key (the entry's weight counts from the sequence's end) and the query tiles that see it
-  auto key0_of = [&]() { return items.tile.x + (items.tile.w - items.tile.z - 1) * kRowsT; };
-  auto tiles_of = [&]() { return (items.tile.y - key0_of() + tokens - 1) / tokens; };
+  // What an item stands for: its K/V head and split, first key (the entry's weight counts from the sequence's end), the
+  // query tiles that see it, and its iterations over them (of every pack of heads).
+  struct Keys {
+    int kvh, split, key0, end, tiles, first, total;
+    __device__ __forceinline__ Keys(const int4& tile, int sub, int splits, int tokens, int packs) {
+      kvh = sub / splits;
+      split = sub - kvh * splits;
+      end = tile.y;
+      key0 = tile.x + (tile.w - tile.z - 1) * kRowsT;
+      tiles = (end - key0 + tokens - 1) / tokens;
+      first = 0;
+      total = packs * tiles;
+      if (kSplit) {
+        const long all = total;
+        first = static_cast<int>(all * split / splits);
+        total = static_cast<int>(all * (split + 1) / splits) - first;
+      }
+    }
+    __device__ __forceinline__ Walk walk(int group, int lp) const {
+      Walk at(kvh * group, key0, tiles, lp);
+      if (kSplit) at.skip(first);
+      return at;
+    }
+  };
 
   if (warp == 0) {
     int x = 0;  // ring item
     bool ok = true;
-    for (int n_items = 0; ok && items.next(); ++n_items) {
-      const int n_q = tiles_of(), key0 = key0_of(), kvh = items.sub, total = packs * n_q;
-      items.look();
+    Feed items(work, p.dkv_table, p.dkv_head, p.taken, p.Hkv * splits);
+    int n_loaded = 0;  // items with anything to load
+    while (ok && items.next(lane, status, abort_flag)) {
+      const Keys keys(items.tile, items.sub, splits, tokens, packs);
+      const int total = keys.total;
+      if (kSplit && total == 0) {
+        if (lane == 0) items.reserve();
+        continue;
+      }
       if (lane == 0) {
-        Walk at(kvh * group, key0, n_q, p.lp);
+        Walk at = keys.walk(group, p.lp);
         auto load = [&](int i) {  // Q (even) or dO (odd) of an iteration
+          if (i == 2 * total - 2) items.reserve();
           if (!mbar_wait(ring.empty_of(x + i), ring.use(x + i) ^ 1, status, kStatusWaitEmpty, abort_flag)) return false;
           mbar_arrive_expect_tx(ring.full_of(x + i), kTileBytes);
           load_tile<DP>(smem_u32(ring.tile(x + i)), (i & 1) ? &tm_do : &tm_q, ring.full_of(x + i), at.head, at.token);
@@ -194,15 +236,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           return true;
         };
         // the first query tile does not wait for the previous item's keys to be read
-        ok = load(0) && load(1) && mbar_wait(kv_empty, (n_items & 1) ^ 1, status, kStatusWaitEmpty, abort_flag);
+        ok = load(0) && load(1) && mbar_wait(kv_empty, (n_loaded & 1) ^ 1, status, kStatusWaitEmpty, abort_flag);
         if (ok) {
           mbar_arrive_expect_tx(kv_full, 2 * kTileBytes);
-          load_tile<DP>(smem_u32(k_tile), &tm_k, kv_full, kvh, key0);
-          load_tile<DP>(smem_u32(v_tile), &tm_v, kv_full, kvh, key0);
+          load_tile<DP>(smem_u32(k_tile), &tm_k, kv_full, keys.kvh, keys.key0);
+          load_tile<DP>(smem_u32(v_tile), &tm_v, kv_full, keys.kvh, keys.key0);
         }
         for (int i = 2; ok && i < 2 * total; ++i) ok = load(i);
       }
       x += 2 * total;
+      ++n_loaded;
       ok = uniform(ok);
     }
   } else if (warp == 1) {
@@ -210,8 +253,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const uint32_t ka = smem_u32(k_tile), va = smem_u32(v_tile);
     int base = 0;  // iterations before the item
     bool ok = true;
-    for (int n_items = 0; ok && items.next(); ++n_items) {
-      const int hi = items.tile.y, n_q = tiles_of(), key0 = key0_of(), kvh = items.sub, total = packs * n_q;
+    Items items(work);
+    int n_items = 0;  // with anything to multiply
+    while (ok && items.next(status, abort_flag)) {
+      const Keys keys(items.tile, items.sub, splits, tokens, packs);
+      const int hi = keys.end, total = keys.total;
+      if (kSplit && total == 0) continue;
       // rows of the query tile at `token`, all 128 or up to the sequence's end
       auto rows_of = [&](int token) { return min(kRowsT, (hi - token) << p.lp); };
       // ring item x, of the query tile at `token`, is in shared memory and its rows past the sequence's end are zeroed
@@ -221,7 +268,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (n != n16) zero_rows<DP>(ring.tile(x), n, n16, lane);
         return true;
       };
-      Walk at(kvh * group, key0, n_q, p.lp);
+      Walk at = keys.walk(group, p.lp);
       int rows16 = (rows_of(at.token) + 15) & ~15;  // of the current iteration's query tile
       ok = ready(2 * base, at.token) && ready(2 * base + 1, at.token) &&
            warp_wait(kv_full, n_items & 1, status, kStatusWaitFull, abort_flag);
@@ -234,7 +281,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (total == 1) umma_commit(kv_empty);
       }
       __syncwarp();
-      items.look();
       for (int it = base; ok && it < base + total; ++it) {
         const bool more = it + 1 < base + total;
         const int xq = 2 * it, xd = xq + 1;
@@ -279,15 +325,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         rows16 = next16;
       }
       base += total;
+      ++n_items;
     }
   } else if (warp == 2) {
     // ---- -lse and -delta of the query tiles ----
     int base = 0;
     bool ok = true;
-    while (ok && items.next()) {
-      const int hi = items.tile.y, n_q = tiles_of(), total = packs * n_q;
-      Walk at(items.sub * group, key0_of(), n_q, p.lp);
-      items.look();
+    Items items(work);
+    while (ok && items.next(status, abort_flag)) {
+      const Keys keys(items.tile, items.sub, splits, tokens, packs);
+      const int hi = keys.end, total = keys.total;
+      Walk at = keys.walk(group, p.lp);
       for (int it = base; it < base + total; ++it, at.next()) {
         const int s = it % kStatRing;
         ok = warp_wait(&st_empty[s], ((it / kStatRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag);
@@ -313,10 +361,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const uint32_t s_addr = t_s + lane_base + part * 32, dp_addr = t_dp + lane_base + part * 32;
     int base = 0;
     bool ok = true;
-    for (int n_items = 0; ok && items.next(); ++n_items) {
-      const int hi = items.tile.y, n_q = tiles_of(), key0 = key0_of(), kvh = items.sub, total = packs * n_q;
-      items.look();
-      Walk at(kvh * group, key0, n_q, p.lp);
+    Items items(work);
+    int n_items = 0;  // with anything summed
+    while (ok && items.next(status, abort_flag)) {
+      const Keys keys(items.tile, items.sub, splits, tokens, packs);
+      const int hi = keys.end, key0 = keys.key0, kvh = keys.kvh, total = keys.total;
+      Walk at = keys.walk(group, p.lp);
       for (int it = base; it < base + total; ++it, at.next()) {
         const int s = it % kStatRing;
         const float* lse = stats + s * 256 + part * 32;
@@ -384,16 +434,34 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
       }
       base += total;
-      ok = ok && warp_wait(done, n_items & 1, status, kStatusWaitAccum, abort_flag);
+      if (!kSplit || total > 0) {
+        ok = ok && warp_wait(done, n_items & 1, status, kStatusWaitAccum, abort_flag);
+        ++n_items;
+      }
       if (!ok) break;
       tc_fence_after();
       const int col = (part & 1) * 64;
       if (col < p.D) {
         const bool values = part < 2;
+        const uint32_t t_sum = (values ? t_dv : t_dk) + lane_base + col;
         const long stride = static_cast<long>(p.Hkv) * p.D;
-        const TileOut to{(values ? p.dv : p.dk) + key0 * stride + static_cast<long>(kvh) * p.D + col, stride, 0, 0,
-                         hi - key0, p.D - col};
-        store_tmem64((values ? t_dv : t_dk) + lane_base + col, values ? 1.f : p.scale, to, quad * 32, lane);
+        const long at0 = key0 * stride + static_cast<long>(kvh) * p.D + col;
+        if (!kSplit) {
+          const TileOut to{(values ? p.dv : p.dk) + at0, stride, 0, 0, hi - key0, p.D - col};
+          store_tmem64(t_sum, values ? 1.f : p.scale, to, quad * 32, lane);
+        } else {  // this split's sum, fp32, or zeros of a split without query tiles
+          float* dst = p.part + (static_cast<long>(keys.split) * 2 + (values ? 0 : 1)) * p.T * stride + at0 + key * stride;
+#pragma unroll 1
+          for (int d = 0; d < 64; d += 16) {
+            float o[16];
+            if (total > 0) tmem_ld16(t_sum + d, o);
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+              if (key0 + key < hi && col + d + j < p.D)
+                *reinterpret_cast<float4*>(dst + d + j) =
+                    total > 0 ? make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+        }
       }
       tc_fence_before();  // the next item's first dV overwrites this one's after this warp's next p_ready
     }
@@ -405,26 +473,50 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
+// dV and dK from the splits' sums, in split order; rows outside the sequences are zero.
+__global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant__ BwdArgs p) {
+  pdl_trigger();
+  pdl_wait();
+  const long stride = static_cast<long>(p.Hkv) * p.D, size = p.T * stride;
+  const long i = (static_cast<long>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i >= size) return;
+  const int token = static_cast<int>(i / stride);
+  const bool inside = token >= p.dkv_head[1] && token < p.dkv_head[2];
+  const int which = blockIdx.y;  // 0: dV, 1: dK
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (inside) {
+    for (int s = 0; s < p.splits; ++s) {
+      const float4 v = *reinterpret_cast<const float4*>(p.part + (static_cast<long>(s) * 2 + which) * size + i);
+      acc.x += v.x;
+      acc.y += v.y;
+      acc.z += v.z;
+      acc.w += v.w;
+    }
+  }
+  const float f = which ? p.scale : 1.f;
+  *reinterpret_cast<uint2*>((which ? p.dk : p.dv) + i) =
+      make_uint2(pack_bf16(acc.x * f, acc.y * f), pack_bf16(acc.z * f, acc.w * f));
+}
+
 // ---- dQ --------------------------------------------------------------------------------------------------------------
 // The chunks of a persistent CTA's items in one sequence: `chunk` of the item's `n`, counted over all items by `k`. The
 // issuing warp runs three of them (scores, dP and dQ are issued two, one and no chunks ahead, across items), a compute
 // group steps by two.
-template <bool kAhead>
 struct ChunkWalk {
-  Items<kAhead> items;
+  Items items;
   int chunk, n, k, item, lp;
   bool valid;
-  __device__ __forceinline__ ChunkWalk(const BwdArgs& p)
-      : items(p.dq_table, p.dq_head, p.H >> p.lp), k(0), item(-1), lp(p.lp) {
+  unsigned* status;
+  volatile int* abort_flag;
+  __device__ __forceinline__ ChunkWalk(const WorkRing& work, int lp_, unsigned* st, volatile int* ab)
+      : items(work), k(0), item(-1), lp(lp_), status(st), abort_flag(ab) {
     take();
   }
   __device__ __forceinline__ void take() {
-    valid = items.next();
+    valid = items.next(status, abort_flag);
     chunk = 0;
     ++item;
-    if (!valid) return;
     n = items.tile.z * (kRowsT >> lp) / kRowsT + 1;  // key chunks, the last one on the diagonal
-    if (kAhead) items.look();
   }
   __device__ __forceinline__ void step() {
     ++k;
@@ -463,7 +555,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   uint64_t* q_empty = dq_free + 1;   // an item's last scores are computed: Q may be overwritten, some time before dO
   uint64_t* do_full = q_empty + 1;
   uint64_t* do_empty = do_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(do_empty + 1);
+  const WorkRing work(do_empty + 1);  // an even number of barriers: on 16 bytes
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(work.empty + kWorkRing);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -483,6 +576,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     mbar_init(q_empty, 1);
     mbar_init(do_full, 1);
     mbar_init(do_empty, 1);
+    work.init(kComputeWarps + 2);  // the issuing warp follows the items twice
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -501,15 +595,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int ksteps = (p.D + 15) / 16;
 
   if (warp == 0) {
-    ChunkWalk<true> at(p);
+    Feed items(work, p.dq_table, p.dq_head, p.taken + 1, p.H >> p.lp);
+    const int tokens = kRowsT >> p.lp;
     int x = 0;  // ring item
     bool ok = true;
-    for (int n_items = 0; ok && at.valid; ++n_items) {
-      const int lo = at.lo(), n = at.n, head = at.head(), kvh = head / group, token = at.token();
-      const int last = min(at.hi(), token + (kRowsT >> p.lp)) - (lo + (n - 1) * kRowsT);  // keys of the last chunk
-      at.take();
+    for (int n_items = 0; ok && items.next(lane, status, abort_flag); ++n_items) {
+      const int lo = items.tile.x, n = items.tile.z * tokens / kRowsT + 1, head = items.sub << p.lp, kvh = head / group;
+      const int token = lo + items.tile.z * tokens;
+      const int last = min(items.tile.y, token + tokens) - (lo + (n - 1) * kRowsT);  // keys of the last chunk
       if (lane == 0) {
         auto load = [&](int i) {  // K (even) or V (odd) of a chunk
+          if (i == 2 * n - 2) items.reserve();
           if (!mbar_wait(ring.empty_of(x + i), ring.use(x + i) ^ 1, status, kStatusWaitEmpty, abort_flag)) return false;
           load_chunk<DP>(smem_u32(ring.tile(x + i)), (i & 1) ? &tm_v : &tm_k, (i & 1) ? &tm_v32 : &tm_k32,
                          ring.full_of(x + i), kvh, lo + (i >> 1) * kRowsT, (i >> 1) + 1 < n ? kRowsT : last);
@@ -534,7 +630,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   } else if (warp == 1) {
     const bool leader = elect_one();
     const uint32_t qa = smem_u32(q_tile), da = smem_u32(do_tile);
-    auto scores = [&](ChunkWalk<true>& a) {  // S of a chunk into its buffer; K rows past the end zeroed
+    auto scores = [&](ChunkWalk& a) {  // S of a chunk into its buffer; K rows past the end zeroed
       if (!a.valid) return true;
       if (a.first() && !warp_wait(q_full, a.item & 1, status, kStatusWaitFull, abort_flag)) return false;
       const int x = 2 * a.k;
@@ -550,8 +646,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       a.step();
       return true;
     };
-    ChunkWalk<true> a(p);
-    ChunkWalk<false> c(p);  // its table entries are in the cache by then
+    ChunkWalk a(work, p.lp, status, abort_flag), c(work, p.lp, status, abort_flag);
     bool ok = scores(a);
     if (ok && c.valid) {
       ok = warp_wait(do_full, 0, status, kStatusWaitFull, abort_flag) &&
@@ -597,7 +692,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int part = (warp - 4) >> 2, quad = warp & 3;
     const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t dp_addr = t_dp + lane_base + part * 32;
-    ChunkWalk<true> at(p);
+    ChunkWalk at(work, p.lp, status, abort_flag);
     bool ok = true;
     float lse = 0.f, delta = 0.f;
     while (ok && at.valid) {
@@ -676,17 +771,24 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 template <int DP>
 int run_bwd(const PackedMaps& m, const PackedArgs& a, const BwdArgs& args, bool want_dq, bool want_dkv,
             unsigned* status, cudaStream_t stream) {
-  const long items_kv = static_cast<long>(a.dkv.max_tiles) * a.Hkv;
+  const long items_kv = static_cast<long>(a.dkv.max_tiles) * a.Hkv * args.splits;
   const long items_q = static_cast<long>(a.dq.max_tiles) * (a.H >> a.lp);
   if (items_q > 0x7fff0000l || items_kv > 0x7fff0000l) return -2;
   const long grid_kv = std::min(items_kv, static_cast<long>(a.num_sms));
   const long grid_q = std::min(items_q, static_cast<long>(a.num_sms));
   if (want_dkv) {
-    auto kernel = packed_dkv_kernel<DP>;
+    const bool split = args.splits > 1;
+    auto kernel = split ? packed_dkv_kernel<DP, true> : packed_dkv_kernel<DP, false>;
     if (set_max_smem(kernel, BwdCfg<DP>::kSmem) != cudaSuccess) return -1;
     if (launch_pdl(kernel, dim3(static_cast<unsigned>(grid_kv)), dim3(kBwdThreads), BwdCfg<DP>::kSmem, stream, m.q,
                    m.k, m.v, m.dout, args, status) != cudaSuccess)
       return -1;
+    if (args.splits > 1) {
+      const long groups = static_cast<long>(a.T) * a.Hkv * a.D / 4;
+      if (launch_pdl(packed_join_kernel, dim3(static_cast<unsigned>((groups + 255) / 256), 2), dim3(256), 0, stream,
+                     args) != cudaSuccess)
+        return -1;
+    }
   }
   if (want_dq) {
     auto kernel = packed_dq_kernel<DP>;
@@ -700,19 +802,31 @@ int run_bwd(const PackedMaps& m, const PackedArgs& a, const BwdArgs& args, bool 
 
 }  // namespace
 
-int launch_packed_delta(const void* out, const void* rest, const void* dout, long stride_t, long stride_h, int T, int H, int D,
-                        float* delta, cudaStream_t stream) {
-  const long rows = static_cast<long>(T) * H;
+// Splits of a key tile's query tiles, where the key tiles are too few for the SMs (a sequence's first tile has twice the
+// mean work, so two per SM are wanted), each of eight iterations of the mean tile at least. Measured with delta, us for
+// 1 / 2 / 4 / 8 splits, D = 128, by key tiles x iterations of the mean one: 16 x 64 194 / 129 / 75 / 53, 64 x 32
+// 110 / 85 / 69 / 93, 64 x 16 68 / 55 / 55 / 75, 128 x 128 427 / 277 / 280 / 349, 8 x 8 51 / 54 / 53 / 53,
+// 256 x 128 471 / 536 / 619 / 711.
+int packed_dkv_splits(const PackedArgs& a, int B) {
+  const long items = static_cast<long>(std::max(1, a.T / 128)) * a.Hkv;
+  const long mean = (static_cast<long>(a.T) / std::max(1, B)) * (a.H / a.Hkv) / 256;  // iterations of 128 rows
+  return static_cast<int>(std::max(1l, std::min({2l * a.num_sms / items, mean / 8, 8l})));
+}
+
+int launch_packed_delta(const PackedArgs& a, const void* out, const void* rest, const void* dout, long stride_t,
+                        long stride_h, float* delta, int* taken, cudaStream_t stream) {
+  const long rows = static_cast<long>(a.T) * a.H;
   return launch_pdl(packed_delta_kernel, dim3(static_cast<unsigned>((rows + 15) / 16)), dim3(256), 0, stream,
-                    static_cast<const bf16*>(out), static_cast<const bf16*>(rest), static_cast<const bf16*>(dout), stride_t, stride_h, T, H, D,
-                    delta) == cudaSuccess ? 0 : -1;
+                    static_cast<const bf16*>(out), static_cast<const bf16*>(rest), static_cast<const bf16*>(dout),
+                    taken, stride_t, stride_h, a.T, a.H, a.D, delta) == cudaSuccess ? 0 : -1;
 }
 
 int launch_packed_backward(const PackedMaps& maps, const PackedArgs& a, const float* lse, const float* delta, void* dq,
-                           void* dk, void* dv, unsigned* status, cudaStream_t stream) {
+                           void* dk, void* dv, int splits, float* part, int* taken, unsigned* status,
+                           cudaStream_t stream) {
   const BwdArgs args{static_cast<bf16*>(dq), static_cast<bf16*>(dk), static_cast<bf16*>(dv), lse, delta,
-                     static_cast<const int4*>(a.dq.entries), static_cast<const int4*>(a.dkv.entries), a.dq.head, a.dkv.head,
-                     a.T, a.H, a.Hkv, a.D, a.lp, a.scale, a.scale * kLog2e};
+                     static_cast<const int4*>(a.dq.entries), static_cast<const int4*>(a.dkv.entries), a.dq.head,
+                     a.dkv.head, taken, a.T, a.H, a.Hkv, a.D, a.lp, a.scale, a.scale * kLog2e, splits, part};
   const bool want_dkv = dk != nullptr;
   return a.D <= 64 ? run_bwd<64>(maps, a, args, dq != nullptr, want_dkv, status, stream)
                    : run_bwd<128>(maps, a, args, dq != nullptr, want_dkv, status, stream);

@@ -166,43 +166,96 @@ __device__ __forceinline__ void zero_padding(bf16* x, int T, long width, const i
   }
 }
 
-// The work of a persistent CTA: items (table entry, sub) with sub < per varying fastest, heaviest first, dealt to the
-// grid in alternating direction so that no CTA always gets a round's heaviest. Persistent because an item of a short
-// sequence is one or two tiles: with a CTA for each, set-up, first loads and last stores took two thirds of the time.
-// A role calls next() to take an item and look() while it would wait anyway: look() finds the following item and starts
-// the load of its table entry (a division and an L2 access, off the path between two items).
-// kAhead false: next() does both (for roles short of registers, whose wait for the item's first scores covers it).
-template <bool kAhead = true>
-struct Items {
-  const int4* table;
-  const int* head;  // (entries, ...)
-  int per, round;
-  int4 ahead;
-  int ahead_sub;
-  bool more;  // there is a following item
-  int4 tile;  // of the item taken: (first token, end, tile, tiles of its sequence)
-  int sub;
+// ---- the work of persistent CTAs --------------------------------------------------------------------------------
+// Items (table entry, sub) with sub < per varying fastest, heaviest first. A CTA's first item is its own index; the next
+// ones it takes from a counter when its loading warp comes to the last chunk of an item, so that no CTA is left with a
+// heavy item at the end (dealt out beforehand, the busiest CTA had 12 to 50% more than the mean). The loading warp
+// publishes an item in a ring in shared memory from which the other warps read it. CTAs are persistent because an item
+// of a short sequence is one or two tiles: with a CTA for each, set-up, first loads and last stores took two thirds of
+// the time.
+struct WorkItem {
+  int4 tile;  // (first token, end, tile, tiles of its sequence)
+  int sub, valid;
+  int pad[2];
+};
 
-  __device__ __forceinline__ Items(const int4* t, const int* h, int per_entry)
-      : table(t), head(h), per(per_entry), round(0) {
-    if (kAhead) look();
+constexpr int kWorkRing = 4;
+
+struct WorkRing {
+  WorkItem* slots;         // [kWorkRing]
+  uint64_t *full, *empty;  // [kWorkRing] each
+  static constexpr int kBytes = kWorkRing * (static_cast<int>(sizeof(WorkItem)) + 16);
+  __device__ __forceinline__ explicit WorkRing(void* base)
+      : slots(static_cast<WorkItem*>(base)), full(reinterpret_cast<uint64_t*>(slots + kWorkRing)),
+        empty(full + kWorkRing) {}
+  __device__ __forceinline__ void init(int readers) const {
+    for (int i = 0; i < kWorkRing; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], readers);
+    }
   }
-  __device__ __forceinline__ void look() {
-    const int g = gridDim.x, c = blockIdx.x;
-    const int index = round * g + ((round & 1) ? g - 1 - c : c);
-    ++round;
-    more = index < head[0] * per;
-    if (!more) return;
-    const int entry = index / per;
-    ahead = table[entry];
-    ahead_sub = index - entry * per;
+};
+
+// The loading warp's side.
+struct Feed {
+  WorkRing ring;
+  const int4* table;
+  const int* head;
+  int* taken;
+  int per, n, index;
+  int4 tile;
+  int sub;
+  __device__ __forceinline__ Feed(const WorkRing& r, const int4* t, const int* h, int* counter, int per_entry)
+      : ring(r), table(t), head(h), taken(counter), per(per_entry), n(0), index(blockIdx.x) {}
+  // One lane, once for every item: the next one is known to be wanted, and its index on its way.
+  __device__ __forceinline__ void reserve() { index = static_cast<int>(gridDim.x) + atomicAdd(taken, 1); }
+  // Publishes the next item; false when there is none (published too) or a wait gave up.
+  __device__ __forceinline__ bool next(int lane, unsigned* status, volatile int* abort_flag) {
+    int valid = 0;
+    const int slot = n % kWorkRing;
+    if (lane == 0 && mbar_wait(&ring.empty[slot], ((n / kWorkRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag)) {
+      valid = index < head[0] * per;
+      WorkItem item{};
+      if (valid) {
+        const int entry = index / per;
+        item.tile = table[entry];
+        item.sub = index - entry * per;
+      }
+      item.valid = valid;
+      ring.slots[slot] = item;
+      mbar_arrive(&ring.full[slot]);
+      tile = item.tile;
+      sub = item.sub;
+    }
+    ++n;
+    valid = uniform(valid);
+    tile = make_int4(uniform(tile.x), uniform(tile.y), uniform(tile.z), uniform(tile.w));
+    sub = uniform(sub);
+    return valid != 0;
   }
-  __device__ __forceinline__ bool next() {
-    if (!kAhead) look();
-    if (!more) return false;
-    tile = make_int4(uniform(ahead.x), uniform(ahead.y), uniform(ahead.z), uniform(ahead.w));
-    sub = ahead_sub;
-    return true;
+};
+
+// A reading warp's side; a warp that follows the items twice counts as two readers.
+struct Items {
+  WorkRing ring;
+  int n;
+  int4 tile;
+  int sub;
+  __device__ __forceinline__ explicit Items(const WorkRing& r) : ring(r), n(0) {}
+  // Moves to the next item; false when there is none or a wait gave up.
+  __device__ __forceinline__ bool next(unsigned* status, volatile int* abort_flag) {
+    const int slot = n % kWorkRing;
+    if (!__all_sync(0xffffffffu,
+                    mbar_wait(&ring.full[slot], (n / kWorkRing) & 1, status, kStatusWaitFull, abort_flag)))
+      return false;
+    const WorkItem& item = ring.slots[slot];
+    tile = make_int4(uniform(item.tile.x), uniform(item.tile.y), uniform(item.tile.z), uniform(item.tile.w));
+    sub = uniform(item.sub);
+    const int valid = uniform(item.valid);
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&ring.empty[slot]);
+    ++n;
+    return valid != 0;
   }
 };
 

@@ -6,7 +6,7 @@ Tolerances (bf16 inputs are exact in 64 bits, so only the kernels round; u = 2^-
   times the scale); a probability is off by 2 eps of itself (score and log-sum-exp) and the exponential's ``2^-20``;
 * P and dS are rounded to bf16 once as operands (u relative), products accumulate in fp32 (``2^-14`` of the sum of
   magnitudes covers thousands of terms), every output is rounded once more (u);
-* delta is taken from the rounded output: off by the output's error times the gradient's magnitude.
+* delta is allowed the rounded output's error times the gradient's magnitude.
 """
 
 import math
@@ -107,6 +107,42 @@ def test_both_forms_of_the_forward_pass(cuda, tiles, heads, kv_heads, dim):
         z = _oracle(q, k, v, lens, dout, dim ** -0.5)
         for name, got in zip(("out", "dq", "dk", "dv"), _run(q, k, v, cu, dout, tiles=tiles)):
             _within(got, z, name)
+    assert ops.require().status(0) == 0
+
+
+@pytest.mark.parametrize("lens,heads,kv_heads,dim", [
+    ([700], 8, 1, 128),               # two CTAs share a key tile's queries
+    ([2049], 8, 1, 64),               # eight
+    ([5, 1300, 1, 0, 1294], 16, 1, 64),  # four, of which some get none of a short sequence's
+    ([1000, 700], 12, 2, 96),         # two, six heads in packs of two
+    ([1600], 32, 4, 80),              # six
+])
+def test_gradients_of_few_key_tiles(cuda, lens, heads, kv_heads, dim):
+    """A key tile's queries are shared by several CTAs where there are few key tiles; their sums are joined in order."""
+    q, k, v, cu, dout = _inputs(cuda, lens, heads, kv_heads, dim, pad=9, seed=21)
+    z = _oracle(q, k, v, lens, dout, dim ** -0.5)
+    first = _run(q, k, v, cu, dout)
+    for name, got in zip(("out", "dq", "dk", "dv"), first):
+        _within(got, z, name)
+        assert got[-9:].count_nonzero() == 0
+    for _ in range(20):
+        for got, want in zip(_run(q, k, v, cu, dout), first):
+            assert torch.equal(got, want)
+    assert ops.require().status(0) == 0
+
+
+def test_more_tiles_than_ctas(cuda):
+    """CTAs take their tiles as they come free; which one takes a tile leaves the results alone."""
+    g = torch.Generator().manual_seed(3)
+    lens = torch.randint(0, 260, (150,), generator=g).tolist()
+    q, k, v, cu, dout = _inputs(cuda, lens, 6, 3, 64, pad=5, seed=22)
+    z = _oracle(q, k, v, lens, dout, 64 ** -0.5)
+    first = _run(q, k, v, cu, dout)
+    for name, got in zip(("out", "dq", "dk", "dv"), first):
+        _within(got, z, name)
+    for _ in range(20):
+        for got, want in zip(_run(q, k, v, cu, dout), first):
+            assert torch.equal(got, want)
     assert ops.require().status(0) == 0
 
 
