@@ -159,14 +159,14 @@ std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> readout(
     c.e = e;
     c.ld = ld;
     c.logit_scale = r.logit_scale;
+    c.reduction = static_cast<int>(reduction);
+    c.grad_rows = grad_rows.has_value() ? grad_rows->data_ptr<float>() : nullptr;
     const int64_t padded = (c.chunk + 63) / 64 * 64;  // rows of xs and e that the maps may read
     uint8_t* xs0 = xs + static_cast<int64_t>(c.row0) * xld * 2;
     const CUtensorMap x_rows = map_2d(xs0, padded, H, xld, 128);
     check(ecz::launch_readout_logits(&x_rows, &w_rows, c, sms, status, stream), "logits");
     const bool sums = want_loss && !per_row;
-    check(ecz::launch_readout_finish(c, static_cast<int>(reduction),
-                                     grad_rows.has_value() ? grad_rows->data_ptr<float>() : nullptr,
-                                     sums ? nll : nullptr, want_loss && per_row ? loss.data_ptr<float>() : nullptr,
+    check(ecz::launch_readout_finish(c, sums ? nll : nullptr, want_loss && per_row ? loss.data_ptr<float>() : nullptr,
                                      sums && i == chunks - 1 ? loss.data_ptr<float>() : nullptr, count + 1, sms, stream),
           "finish");
     if (need_dx) {

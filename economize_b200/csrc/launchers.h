@@ -286,6 +286,8 @@ struct ReadoutChunk {
   void* e = nullptr;            // fp16 e, then bf16 dz [chunk up to a multiple of 64, ld], or null (losses only)
   long ld = 0;                  // a multiple of 64
   float logit_scale = 1.f;
+  int reduction = kReduceNone;
+  const float* grad_rows = nullptr;  // [T] gradients of losses by row, or null
 };
 int readout_pieces(int V);
 int readout_splits(long tiles, long kblocks, int num_sms);
@@ -307,8 +309,8 @@ int launch_readout_gather(const ReadoutRows& r, const int* pos, int* rows, int* 
 int launch_readout_logits(const CUtensorMap* xs, const CUtensorMap* w, const ReadoutChunk& c, int num_sms,
                           unsigned* status, cudaStream_t stream);
 // loss, done (a zeroed counter): of the last chunk of a scalar loss, else null.
-int launch_readout_finish(const ReadoutChunk& c, int reduction, const float* grad_rows, float* nll, float* losses,
-                          float* loss, int* done, int num_sms, cudaStream_t stream);
+int launch_readout_finish(const ReadoutChunk& c, float* nll, float* losses, float* loss, int* done, int num_sms,
+                          cudaStream_t stream);
 int launch_readout_dx(const CUtensorMap* dz, const CUtensorMap* w, const ReadoutChunk& c, int splits, float* part,
                       void* dx, int num_sms, unsigned* status, cudaStream_t stream);
 int launch_readout_dw(const CUtensorMap* dz, const CUtensorMap* xs, const ReadoutChunk& c, float* sum, bool first,

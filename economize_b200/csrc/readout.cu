@@ -15,8 +15,10 @@
 //             (bf16 would add a second 8-bit rounding to the gradients); the logits themselves are never stored.
 //   finish    joins a row's pieces to S, the sum over the other tokens. nll = log(1 + S exp(-z_y)) and the target's
 //             gradient -S / (S + exp(z_y)) keep their digits where the target's probability is near one. Rewrites e in
-//             place as dz = g s (e exp(m - L)) in bf16, the one rounding of the gradient's left factor. The last CTA of
-//             the last chunk adds the losses up in row order.
+//             place as dz = g (e exp(m - L)) in bf16, the one rounding of the gradient's left factor. What all rows share
+//             (s, 1 / count of a mean, the first row's g of losses by row) stays out of dz and is multiplied in at the
+//             end, in fp32: near -1 / count, most targets' entries were rounded the same way, and the whole gradient was
+//             off by up to 0.4%. The last CTA of the last chunk adds the losses up in row order.
 //   products  dX = dz . W (K = V, W read MN-major) and dW = dz^T . X (K = rows, both operands MN-major), no
 //             transposes. Over several chunks dW is summed in an fp32 buffer in chunk order.
 //
@@ -266,6 +268,23 @@ __device__ __forceinline__ float block_reduce(float v, float* red, bool want_max
   return r;
 }
 
+// The factor that the gradients' products leave to their end.
+struct Shared {
+  float logit_scale;
+  bool mean;
+  const float* grad_rows;   // of losses by row, or null
+  const int *rows, *count;  // all packed rows
+  // the first row's gradient: rows of one gradient, as a mean of the losses gives them, have entries as a sum's
+  __device__ __forceinline__ float grad() const {
+    const float g = grad_rows != nullptr && *count > 0 ? fabsf(grad_rows[rows[0]]) : 1.f;
+    return g > 0x1p-60f && g < 0x1p60f ? g : 1.f;  // and no quotient of two gradients overflows for it
+  }
+  __device__ __forceinline__ float value() const {
+    const float f = logit_scale * grad();
+    return mean ? f / static_cast<float>(max(1, *count)) : f;
+  }
+};
+
 // CTAs (row, part) of the packed rows of a chunk: every part joins the row's pieces and turns its columns of e into dz
 // in place; part 0 writes nll. NaN statistics give NaN, as the plain formula does. Counts itself on *done where a loss
 // is wanted of the last chunk: the last CTA adds up.
@@ -278,9 +297,7 @@ struct FinishArgs {
   int row0, chunk, V, pieces;
   void* e_dz;
   long ld;
-  float logit_scale;
-  int reduction;
-  const float* grad_rows;
+  Shared shared;
   float *nll, *losses;
   float* loss;  // null but for the last chunk of a scalar loss
   int* done;
@@ -299,10 +316,10 @@ __device__ __forceinline__ void add_up(const FinishArgs& a, float* red) {
   float v = 0.f;
   for (int i = threadIdx.x; i < n; i += kFinishThreads) v += __ldcg(a.nll + i);
   v = block_reduce(v, red, false);
-  if (threadIdx.x == 0) *a.loss = a.reduction == kReduceMean ? (n > 0 ? v / static_cast<float>(n) : 0.f) : v;
+  if (threadIdx.x == 0) *a.loss = a.shared.mean ? (n > 0 ? v / static_cast<float>(n) : 0.f) : v;
 }
 
-__device__ __forceinline__ void finish_row(const FinishArgs& a, int r, int total, float* factor, float* red) {
+__device__ __forceinline__ void finish_row(const FinishArgs& a, int r, float* factor, float* red) {
   const float2* st = a.stats + static_cast<size_t>(r) * a.pieces;
   const float z = a.picked[r];
   float top = z;
@@ -329,9 +346,7 @@ __device__ __forceinline__ void finish_row(const FinishArgs& a, int r, int total
     if (a.losses != nullptr) a.losses[orig] = loss;
   }
   if (a.e_dz == nullptr) return;
-  float g = a.logit_scale;
-  if (a.grad_rows != nullptr) g *= a.grad_rows[orig];
-  else if (a.reduction == kReduceMean) g /= static_cast<float>(total);
+  const float g = a.shared.grad_rows != nullptr ? a.shared.grad_rows[orig] / a.shared.grad() : 1.f;
   for (int j = threadIdx.x; j < a.pieces; j += kFinishThreads) factor[j] = exp2f(st[j].x - lse2) * g;
   __syncthreads();
   const int tgt = a.target[r];
@@ -356,7 +371,7 @@ __device__ __forceinline__ void finish_row(const FinishArgs& a, int r, int total
 }
 
 __global__ void __launch_bounds__(kFinishThreads) readout_finish_kernel(const __grid_constant__ FinishArgs a) {
-  extern __shared__ float factor[];  // [pieces]: exp2(m - L) g s
+  extern __shared__ float factor[];  // [pieces]: exp2(m - L) g
   __shared__ float red[kFinishThreads / 32];
   pdl_trigger();
   pdl_wait();
@@ -364,7 +379,7 @@ __global__ void __launch_bounds__(kFinishThreads) readout_finish_kernel(const __
   const int n = min(a.chunk, total - a.row0);
   const int r = blockIdx.x;
   if (r < n) {
-    finish_row(a, r, total, factor, red);
+    finish_row(a, r, factor, red);
   } else if (n > 0 && a.e_dz != nullptr && r < (n + pair::kBK - 1) / pair::kBK * pair::kBK) {
     // zero rows up to the K block of dz^T . X that reads them
     uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.e_dz) + static_cast<size_t>(r) * a.ld);
@@ -384,6 +399,7 @@ struct StoreEpi {
   int N;
   long part_rows;   // rows of a split's partials
   bool add, last;   // running sum: add to what is there; store the sum as bf16
+  Shared shared;    // what bf16 results are multiplied by
 
   __device__ __forceinline__ void operator()(const pair::Unit& u, int M, int row0, int col0, uint32_t taddr, bool zero,
                                              uint8_t* patch, int lane) const {
@@ -393,6 +409,7 @@ struct StoreEpi {
                       ? nullptr
                       : part + (static_cast<size_t>(u.split) * part_rows + row0 + lane) * static_cast<size_t>(N) + col0;
     const bool row_ok = row0 + lane < M;
+    const float factor = last ? shared.value() : 1.f;
 #pragma unroll 1
     for (int c = 0; c < cols; c += 32) {
       float v[32];
@@ -418,6 +435,8 @@ struct StoreEpi {
         }
       }
       if (!last) continue;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] *= factor;
 #pragma unroll
       for (int j = 0; j < 32; j += 8) {
         uint4 w;
@@ -450,14 +469,13 @@ struct StoreEpi {
 
 constexpr int kJoinThreads = 128;
 
-// out[rows[m]] = bf16(sum over splits, in order, of part[s, m]).
-__global__ void __launch_bounds__(kJoinThreads) readout_join_kernel(const float* __restrict__ part, int splits, long part_rows,
-                                                           int N, const int* __restrict__ rows,
-                                                           const int* __restrict__ count, int row0, int chunk,
-                                                           bf16* __restrict__ out) {
+// out[rows[m]] = bf16(the shared factor times the sum over splits, in order, of part[s, m]).
+__global__ void __launch_bounds__(kJoinThreads)
+    readout_join_kernel(const float* __restrict__ part, int splits, long part_rows, int N, int row0, int chunk,
+                        Shared shared, bf16* __restrict__ out) {
   pdl_trigger();
   pdl_wait();
-  const int n = min(chunk, *count - row0);
+  const int n = min(chunk, *shared.count - row0);
   const long i = (static_cast<long>(blockIdx.x) * kJoinThreads + threadIdx.x) * 4;
   const long m = i / N, c = i % N;
   if (m >= n) return;
@@ -470,11 +488,12 @@ __global__ void __launch_bounds__(kJoinThreads) readout_join_kernel(const float*
     acc.z += v.z;
     acc.w += v.w;
   }
-  __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x, acc.y), hi = __floats2bfloat162_rn(acc.z, acc.w);
+  const float f = shared.value();
+  __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * f, acc.y * f), hi = __floats2bfloat162_rn(acc.z * f, acc.w * f);
   uint2 w;
   w.x = *reinterpret_cast<uint32_t*>(&lo);
   w.y = *reinterpret_cast<uint32_t*>(&hi);
-  *reinterpret_cast<uint2*>(out + static_cast<long>(rows[m]) * N + c) = w;
+  *reinterpret_cast<uint2*>(out + static_cast<long>(shared.rows[row0 + m]) * N + c) = w;
 }
 
 // x and y times *g in place (bf16, sizes in groups of 8); reads nothing more when *g is 1, what a loss's own backward
@@ -537,13 +556,16 @@ int launch_readout_logits(const CUtensorMap* xs, const CUtensorMap* w, const Rea
   return pair::launch_pair<false, false>(*xs, *w, shape, epi, num_sms, status, stream);
 }
 
-int launch_readout_finish(const ReadoutChunk& c, int reduction, const float* grad_rows, float* nll, float* losses,
-                          float* loss, int* done, int num_sms, cudaStream_t stream) {
+static Shared shared_of(const ReadoutChunk& c) {
+  return Shared{c.logit_scale, c.reduction == kReduceMean, c.grad_rows, c.rows, c.count};
+}
+
+int launch_readout_finish(const ReadoutChunk& c, float* nll, float* losses, float* loss, int* done, int num_sms, cudaStream_t stream) {
   const int pieces = readout_pieces(c.V);
   const int smem = c.e != nullptr ? pieces * 4 : 0;
   if (smem > 40 * 1024 && set_max_smem(readout_finish_kernel, smem) != cudaSuccess) return -1;
   const FinishArgs a{static_cast<const float2*>(c.stats), c.picked + c.row0, c.target + c.row0, c.rows, c.count, c.row0,
-                     c.chunk, c.V, pieces, c.e, c.ld, c.logit_scale, reduction, grad_rows, nll, losses, loss, done};
+                     c.chunk, c.V, pieces, c.e, c.ld, shared_of(c), nll, losses, loss, done};
   const int rows = (c.chunk + pair::kBK - 1) / pair::kBK * pair::kBK;
   // few rows: several CTAs to a row, so that eight on every SM share the columns
   const int most = c.e == nullptr ? 1 : (c.V + kFinishThreads * 8 - 1) / (kFinishThreads * 8);
@@ -554,19 +576,20 @@ int launch_readout_finish(const ReadoutChunk& c, int reduction, const float* gra
 
 int launch_readout_dx(const CUtensorMap* dz, const CUtensorMap* w, const ReadoutChunk& c, int splits, float* part,
                       void* dx, int num_sms, unsigned* status, cudaStream_t stream) {
-  StoreEpi epi{static_cast<bf16*>(dx), splits > 1 ? part : nullptr, c.rows + c.row0, c.H, c.chunk, false, splits == 1};
+  StoreEpi epi{static_cast<bf16*>(dx), splits > 1 ? part : nullptr, c.rows + c.row0, c.H, c.chunk, false, splits == 1,
+               shared_of(c)};
   const pair::Shape shape{c.chunk, c.H, c.V, c.count, c.row0, true, false, splits, false};
   int rc = pair::launch_pair<false, true>(*dz, *w, shape, epi, num_sms, status, stream);
   if (rc != 0 || splits == 1) return rc;
   const long groups = static_cast<long>(c.chunk) * c.H / 4;
-  return launch_pdl(readout_join_kernel, dim3(static_cast<unsigned>((groups + kJoinThreads - 1) / kJoinThreads)), dim3(kJoinThreads), 0, stream, part,
-                    splits, static_cast<long>(c.chunk), c.H, c.rows + c.row0, c.count, c.row0, c.chunk,
-                    static_cast<bf16*>(dx)) == cudaSuccess ? 0 : -1;
+  return launch_pdl(readout_join_kernel, dim3(static_cast<unsigned>((groups + kJoinThreads - 1) / kJoinThreads)),
+                    dim3(kJoinThreads), 0, stream, part, splits, static_cast<long>(c.chunk), c.H, c.row0, c.chunk,
+                    shared_of(c), static_cast<bf16*>(dx)) == cudaSuccess ? 0 : -1;
 }
 
 int launch_readout_dw(const CUtensorMap* dz, const CUtensorMap* xs, const ReadoutChunk& c, float* sum, bool first,
                       bool last, void* dw, int num_sms, unsigned* status, cudaStream_t stream) {
-  StoreEpi epi{static_cast<bf16*>(dw), first && last ? nullptr : sum, nullptr, c.H, 0, !first, last};
+  StoreEpi epi{static_cast<bf16*>(dw), first && last ? nullptr : sum, nullptr, c.H, 0, !first, last, shared_of(c)};
   const pair::Shape shape{c.V, c.H, c.chunk, c.count, c.row0, false, true, 1, true};
   return pair::launch_pair<true, true>(*dz, *xs, shape, epi, num_sms, status, stream);
 }

@@ -89,6 +89,25 @@ def test_losses_and_gradients(cuda, rows, hidden, vocab, masked, reduction):
     assert ops.require().status(0) == 0
 
 
+@pytest.mark.parametrize("rows", [37, 119])
+def test_what_all_rows_share_is_not_rounded(cuda, rows):
+    """The mean's 1 / rows is no part of the gradients' rounded factor. Rounding dz ~ -1 / rows to bf16 shifts a whole
+    gradient (1 / 37 and 1 / 119 by 2 parts in 1000); the independent roundings of E elements move the slope of
+    one gradient against another by about 2^-8 / sqrt(E) = 2e-5 for the E here: 2e-4 is ten times that."""
+    x, w, y = _inputs(cuda, rows, 1024, 600, seed=9)
+
+    def grads(reduction):
+        a, b = x.detach().requires_grad_(), w.detach().requires_grad_()
+        loss = ops.linear_cross_entropy(a, b, y, reduction="none" if reduction == "rows" else reduction)
+        return torch.autograd.grad(loss.mean() if reduction == "rows" else loss, (a, b))
+
+    want = [g.double() for g in grads("sum")]
+    for reduction in ("mean", "rows"):
+        for got, ref in zip(grads(reduction), want):
+            slope = (got.double() * rows * ref).sum() / ref.square().sum()
+            assert abs(slope.item() - 1) < 2e-4
+
+
 @pytest.mark.parametrize("chunk", [64, 128, 320])
 def test_chunks_of_rows(cuda, chunk):
     """Several chunks: every output as from one, weight gradients summed in fp32 in between."""
