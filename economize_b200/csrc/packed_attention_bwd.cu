@@ -695,6 +695,25 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     ChunkWalk at(work, p.lp, status, abort_flag);
     bool ok = true;
     float lse = 0.f, delta = 0.f;
+    // Half of the warps store an item's dQ, after the first chunk of the next: the product has ended by then, and the
+    // next one waits for these loads at most.
+    int done_item = -1, done_first = 0, done_hi = 0, done_head = 0;
+    auto store = [&]() {
+      if (!warp_wait(dq_full, done_item & 1, status, kStatusWaitAccum, abort_flag)) return false;
+      tc_fence_after();
+      const int col = part * 64;
+      uint4 c[8];
+      if (col < p.D) load_packed64(t_dq + lane_base + col, p.scale, c);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(dq_free);
+      if (col < p.D) {
+        const TileOut to{p.dq + (static_cast<long>(done_first) * p.H + done_head) * p.D + col,
+                         static_cast<long>(p.H) * p.D, p.D, p.lp, (done_hi - done_first) << p.lp, p.D - col};
+        store_rows64(c, to, quad * 32, lane);
+      }
+      return true;
+    };
     while (ok && at.valid) {
       const uint32_t s_addr = t_s + (at.k & 1) * 128 + lane_base + part * 32;
       const int first = at.token(), token = first + ((quad * 32 + lane) >> p.lp), hi = at.hi();
@@ -741,25 +760,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_ready);
-      const int head = at.head(), item = at.item;
-      at.step();
-      if (last && part < 2) {  // half of the warps store the item's dQ
-        ok = warp_wait(dq_full, item & 1, status, kStatusWaitAccum, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        const int col = part * 64;
-        uint4 c[8];
-        if (col < p.D) load_packed64(t_dq + lane_base + col, p.scale, c);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(dq_free);
-        if (col < p.D) {
-          const TileOut to{p.dq + (static_cast<long>(first) * p.H + head) * p.D + col, static_cast<long>(p.H) * p.D, p.D,
-                           p.lp, (hi - first) << p.lp, p.D - col};
-          store_rows64(c, to, quad * 32, lane);
+      if (part < 2) {
+        if (at.first() && at.item > 0) ok = store();
+        if (last) {
+          done_item = at.item;
+          done_first = first;
+          done_hi = hi;
+          done_head = at.head();
         }
       }
+      at.step();
     }
+    if (ok && part < 2 && done_item >= 0) ok = store();
   }
   __syncwarp();
   tc_fence_before();
