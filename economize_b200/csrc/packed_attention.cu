@@ -273,6 +273,7 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
         auto chunk = [&](int x) {  // K (even) or V (odd) of a chunk
           const int s = (it + x) % kRing, c = x >> 1;
           if (x == 2 * n - 2) items.reserve();
+          if (x == 2 * n - 1) items.fetch();
           if (!mbar_wait(&kv_empty[s], (((it + x) / kRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag)) return false;
           load_chunk<DP>(ra + s * kTileBytes, (x & 1) ? &tm_v : &tm_k, (x & 1) ? &tm_v32 : &tm_k32, &kv_full[s], kvh,
                          lo + c * kRowsT, c + 1 < n ? kRowsT : last_keys);

@@ -222,13 +222,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const Keys keys(items.tile, items.sub, splits, tokens, packs);
       const int total = keys.total;
       if (kSplit && total == 0) {
-        if (lane == 0) items.reserve();
+        if (lane == 0) {
+          items.reserve();
+          items.fetch();
+        }
         continue;
       }
       if (lane == 0) {
         Walk at = keys.walk(group, p.lp);
         auto load = [&](int i) {  // Q (even) or dO (odd) of an iteration
           if (i == 2 * total - 2) items.reserve();
+          if (i == 2 * total - 1) items.fetch();
           if (!mbar_wait(ring.empty_of(x + i), ring.use(x + i) ^ 1, status, kStatusWaitEmpty, abort_flag)) return false;
           mbar_arrive_expect_tx(ring.full_of(x + i), kTileBytes);
           load_tile<DP>(smem_u32(ring.tile(x + i)), (i & 1) ? &tm_do : &tm_q, ring.full_of(x + i), at.head, at.token);
@@ -440,7 +444,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       if (!ok) break;
       tc_fence_after();
-      const int col = (part & 1) * 64;
+      constexpr int kCols = DP / 2;  // of a warp
+      const int col = (part & 1) * kCols;
       if (col < p.D) {
         const bool values = part < 2;
         const uint32_t t_sum = (values ? t_dv : t_dk) + lane_base + col;
@@ -448,11 +453,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const long at0 = key0 * stride + static_cast<long>(kvh) * p.D + col;
         if (!kSplit) {
           const TileOut to{(values ? p.dv : p.dk) + at0, stride, 0, 0, hi - key0, p.D - col};
-          store_tmem64(t_sum, values ? 1.f : p.scale, to, quad * 32, lane);
+          uint4 c[kCols / 8];
+          load_packed(t_sum, values ? 1.f : p.scale, c);
+          store_rows(c, to, quad * 32, lane);
         } else {  // this split's sum, fp32, or zeros of a split without query tiles
           float* dst = p.part + (static_cast<long>(keys.split) * 2 + (values ? 0 : 1)) * p.T * stride + at0 + key * stride;
 #pragma unroll 1
-          for (int d = 0; d < 64; d += 16) {
+          for (int d = 0; d < kCols; d += 16) {
             float o[16];
             if (total > 0) tmem_ld16(t_sum + d, o);
 #pragma unroll
@@ -572,11 +579,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     mbar_init(dp_full, 1);
     mbar_init(ds_ready, kComputeWarps);
     mbar_init(dq_full, 1);
-    mbar_init(dq_free, kComputeWarps / 2);
+    mbar_init(dq_free, kComputeWarps);
     mbar_init(q_empty, 1);
     mbar_init(do_full, 1);
     mbar_init(do_empty, 1);
-    work.init(kComputeWarps + 2);  // the issuing warp follows the items twice
+    work.init(kComputeWarps + 3);  // the issuing warp follows the items twice
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -595,36 +602,48 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int ksteps = (p.D + 15) / 16;
 
   if (warp == 0) {
+    // ---- loads of K and V ----
     Feed items(work, p.dq_table, p.dq_head, p.taken + 1, p.H >> p.lp);
     const int tokens = kRowsT >> p.lp;
     int x = 0;  // ring item
     bool ok = true;
-    for (int n_items = 0; ok && items.next(lane, status, abort_flag); ++n_items) {
-      const int lo = items.tile.x, n = items.tile.z * tokens / kRowsT + 1, head = items.sub << p.lp, kvh = head / group;
+    while (ok && items.next(lane, status, abort_flag)) {
+      const int lo = items.tile.x, n = items.tile.z * tokens / kRowsT + 1, kvh = (items.sub << p.lp) / group;
       const int token = lo + items.tile.z * tokens;
       const int last = min(items.tile.y, token + tokens) - (lo + (n - 1) * kRowsT);  // keys of the last chunk
       if (lane == 0) {
-        auto load = [&](int i) {  // K (even) or V (odd) of a chunk
+        for (int i = 0; ok && i < 2 * n; ++i) {  // K (even) or V (odd) of a chunk
           if (i == 2 * n - 2) items.reserve();
-          if (!mbar_wait(ring.empty_of(x + i), ring.use(x + i) ^ 1, status, kStatusWaitEmpty, abort_flag)) return false;
-          load_chunk<DP>(smem_u32(ring.tile(x + i)), (i & 1) ? &tm_v : &tm_k, (i & 1) ? &tm_v32 : &tm_k32,
-                         ring.full_of(x + i), kvh, lo + (i >> 1) * kRowsT, (i >> 1) + 1 < n ? kRowsT : last);
-          return true;
-        };
+          if (i == 2 * n - 1) items.fetch();
+          ok = mbar_wait(ring.empty_of(x + i), ring.use(x + i) ^ 1, status, kStatusWaitEmpty, abort_flag);
+          if (ok)
+            load_chunk<DP>(smem_u32(ring.tile(x + i)), (i & 1) ? &tm_v : &tm_k, (i & 1) ? &tm_v32 : &tm_k32,
+                           ring.full_of(x + i), kvh, lo + (i >> 1) * kRowsT, (i >> 1) + 1 < n ? kRowsT : last);
+        }
+      }
+      x += 2 * n;
+      ok = uniform(ok);
+    }
+  } else if (warp == 2) {
+    // ---- loads of Q and dO: not behind a K or V that waits for its place ----
+    Items items(work);
+    const int tokens = kRowsT >> p.lp;
+    bool ok = true;
+    for (int n_items = 0; ok && items.next(status, abort_flag); ++n_items) {
+      const int head = items.sub << p.lp, token = items.tile.x + items.tile.z * tokens;
+      if (lane == 0) {
         const uint32_t turn = (n_items & 1) ^ 1;
-        ok = load(0) && mbar_wait(q_empty, turn, status, kStatusWaitEmpty, abort_flag);
+        ok = mbar_wait(q_empty, turn, status, kStatusWaitEmpty, abort_flag);
         if (ok) {
           mbar_arrive_expect_tx(q_full, kTileBytes);
           load_tile<DP>(smem_u32(q_tile), &tm_q, q_full, head, token);
         }
-        ok = ok && load(1) && mbar_wait(do_empty, turn, status, kStatusWaitEmpty, abort_flag);
+        ok = ok && mbar_wait(do_empty, turn, status, kStatusWaitEmpty, abort_flag);
         if (ok) {
           mbar_arrive_expect_tx(do_full, kTileBytes);
           load_tile<DP>(smem_u32(do_tile), &tm_do, do_full, head, token);
         }
-        for (int i = 2; ok && i < 2 * n; ++i) ok = load(i);
       }
-      x += 2 * n;
       ok = uniform(ok);
     }
   } else if (warp == 1) {
@@ -695,22 +714,23 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     ChunkWalk at(work, p.lp, status, abort_flag);
     bool ok = true;
     float lse = 0.f, delta = 0.f;
-    // Half of the warps store an item's dQ, after the first chunk of the next: the product has ended by then, and the
-    // next one waits for these loads at most.
+    // An item's dQ is stored after the first chunk of the next: the product has ended by then, and the next one waits
+    // for these loads at most. A quarter of the columns to a warp (by halves of the warps it took twice as long).
+    constexpr int kCols = DP / 4;
     int done_item = -1, done_first = 0, done_hi = 0, done_head = 0;
     auto store = [&]() {
       if (!warp_wait(dq_full, done_item & 1, status, kStatusWaitAccum, abort_flag)) return false;
       tc_fence_after();
-      const int col = part * 64;
-      uint4 c[8];
-      if (col < p.D) load_packed64(t_dq + lane_base + col, p.scale, c);
+      const int col = part * kCols;
+      uint4 c[kCols / 8];
+      if (col < p.D) load_packed(t_dq + lane_base + col, p.scale, c);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(dq_free);
       if (col < p.D) {
         const TileOut to{p.dq + (static_cast<long>(done_first) * p.H + done_head) * p.D + col,
                          static_cast<long>(p.H) * p.D, p.D, p.lp, (done_hi - done_first) << p.lp, p.D - col};
-        store_rows64(c, to, quad * 32, lane);
+        store_rows(c, to, quad * 32, lane);
       }
       return true;
     };
@@ -760,18 +780,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_ready);
-      if (part < 2) {
-        if (at.first() && at.item > 0) ok = store();
-        if (last) {
-          done_item = at.item;
-          done_first = first;
-          done_hi = hi;
-          done_head = at.head();
-        }
+      if (at.first() && at.item > 0) ok = store();
+      if (last) {
+        done_item = at.item;
+        done_first = first;
+        done_hi = hi;
+        done_head = at.head();
       }
       at.step();
     }
-    if (ok && part < 2 && done_item >= 0) ok = store();
+    if (ok && done_item >= 0) ok = store();
   }
   __syncwarp();
   tc_fence_before();

@@ -86,7 +86,7 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
 template <int DP>
 __device__ __forceinline__ void load_chunk(uint32_t dst, const CUtensorMap* map, const CUtensorMap* map32, uint64_t* bar,
                                            int head, int token, int rows) {
-  if (rows > 96) {
+  if (rows > 64) {
     mbar_arrive_expect_tx(bar, kRowsT * DP * 2);
     load_tile<DP>(dst, map, bar, head, token);
     return;
@@ -196,36 +196,36 @@ struct WorkRing {
   }
 };
 
-// The loading warp's side.
+// The loading warp's side; lane 0 holds the item to come.
 struct Feed {
   WorkRing ring;
   const int4* table;
-  const int* head;
   int* taken;
-  int per, n, index;
-  int4 tile;
+  int per, count, n, index;
+  int4 ahead, tile;
   int sub;
-  __device__ __forceinline__ Feed(const WorkRing& r, const int4* t, const int* h, int* counter, int per_entry)
-      : ring(r), table(t), head(h), taken(counter), per(per_entry), n(0), index(blockIdx.x) {}
-  // One lane, once for every item: the next one is known to be wanted, and its index on its way.
+  // The first tile is read along with the number of items: a CTA's first entry is inside the table.
+  __device__ __forceinline__ Feed(const WorkRing& r, const int4* t, const int* head, int* counter, int per_entry)
+      : ring(r), table(t), taken(counter), per(per_entry), count(head[0] * per_entry), n(0), index(blockIdx.x),
+        ahead(t[blockIdx.x / per_entry]) {}
+  // Lane 0, once for every item, at its last chunk: the next item's index is on its way ...
   __device__ __forceinline__ void reserve() { index = static_cast<int>(gridDim.x) + atomicAdd(taken, 1); }
+  // ... and a load later its entry.
+  __device__ __forceinline__ void fetch() {
+    if (index < count) ahead = table[index / per];
+  }
   // Publishes the next item; false when there is none (published too) or a wait gave up.
   __device__ __forceinline__ bool next(int lane, unsigned* status, volatile int* abort_flag) {
     int valid = 0;
     const int slot = n % kWorkRing;
     if (lane == 0 && mbar_wait(&ring.empty[slot], ((n / kWorkRing) & 1) ^ 1, status, kStatusWaitEmpty, abort_flag)) {
-      valid = index < head[0] * per;
-      WorkItem item{};
-      if (valid) {
-        const int entry = index / per;
-        item.tile = table[entry];
-        item.sub = index - entry * per;
-      }
+      valid = index < count;
+      WorkItem item;
+      item.tile = tile = ahead;
+      item.sub = sub = index % per;
       item.valid = valid;
       ring.slots[slot] = item;
       mbar_arrive(&ring.full[slot]);
-      tile = item.tile;
-      sub = item.sub;
     }
     ++n;
     valid = uniform(valid);
@@ -270,15 +270,16 @@ struct TileOut {
   }
 };
 
-// Stores 64 columns of a warp's 32 rows, from `row0` of the tile on: lane r holds row r's as eight 16-byte groups
-// c[0..7]. An 8 x 8 transpose over groups of eight lanes (three exchanges) first, so that eight lanes write a row's 128
-// bytes at once: rows written by their own lanes touch 32 lines per store and took 3900 cycles for a 128 x 128 tile.
-__device__ __forceinline__ void store_rows64(uint4 (&c)[8], const TileOut& to, int row0, int lane) {
+// Stores 8 kG columns of a warp's 32 rows, from `row0` of the tile on: lane r holds row r's as kG 16-byte groups. A kG x
+// kG transpose over groups of kG lanes (log2 kG exchanges) first, so that kG lanes write a row's segment at once: rows
+// written by their own lanes touch 32 lines per store and took 3900 cycles for a 128 x 128 tile.
+template <int kG>
+__device__ __forceinline__ void store_rows(uint4 (&c)[kG], const TileOut& to, int row0, int lane) {
 #pragma unroll
-  for (int m = 4; m > 0; m >>= 1) {
+  for (int m = kG / 2; m > 0; m >>= 1) {
     const bool up = (lane & m) != 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kG; ++i) {
       if (i & m) continue;
       uint4 out = up ? c[i] : c[i | m];
       out.x = __shfl_xor_sync(0xffffffffu, out.x, m);
@@ -289,23 +290,27 @@ __device__ __forceinline__ void store_rows64(uint4 (&c)[8], const TileOut& to, i
       else c[i | m] = out;
     }
   }
-  const int col = (lane & 7) * 8;
+  const int col = (lane & (kG - 1)) * 8;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int row = row0 + (lane & 24) + j;
+  for (int j = 0; j < kG; ++j) {
+    const int row = row0 + (lane & (32 - kG)) + j;
     if (row < to.rows && col < to.cols) *reinterpret_cast<uint4*>(to.row(row) + col) = c[j];
   }
 }
 
-// 64 fp32 columns of a lane's TMEM row, times f, as eight groups of eight bf16.
-__device__ __forceinline__ void load_packed64(uint32_t taddr, float f, uint4 (&c)[8]) {
+// 8 kG fp32 columns of a lane's TMEM row, times f, as kG groups of eight bf16.
+template <int kG>
+__device__ __forceinline__ void load_packed(uint32_t taddr, float f, uint4 (&c)[kG]) {
+  static_assert(kG == 2 || kG % 4 == 0, "TMEM is read by 16 or 32 columns");
+  constexpr int kCols = kG == 2 ? 16 : 32;
   const uint64_t ff = pair_of(f, f);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float o[32];
-    tmem_load32(taddr + h * 32, o);
+  for (int h = 0; h < 8 * kG / kCols; ++h) {
+    float o[kCols];
+    if constexpr (kG == 2) tmem_ld16(taddr, o);
+    else tmem_load32(taddr + h * 32, o);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kCols / 8; ++j) {
       uint32_t w[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -318,14 +323,7 @@ __device__ __forceinline__ void load_packed64(uint32_t taddr, float f, uint4 (&c
   }
 }
 
-// 64 columns of the warp's TMEM lanes, times each lane's f, as bf16 rows through registers (store_rows64).
-__device__ __forceinline__ void store_tmem64(uint32_t taddr, float f, const TileOut& to, int row0, int lane) {
-  uint4 c[8];
-  load_packed64(taddr, f, c);
-  store_rows64(c, to, row0, lane);
-}
-
-// The same through 4 KB of shared memory of the warp (16-byte groups swizzled by the row, so that neither side
+// 64 columns of the warp's TMEM lanes, times each lane's f, as bf16 rows through 4 KB of shared memory (16-byte groups swizzled by the row, so that neither side
 // conflicts), with fewer instructions. kRest: what bf16 rounds away of the values instead (itself rounded to bf16).
 template <bool kRest>
 __device__ __forceinline__ void stage_tmem64(uint32_t taddr, float f, uint8_t* stage, const TileOut& to, int row0,
