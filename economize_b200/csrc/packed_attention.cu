@@ -142,7 +142,8 @@ __global__ void __launch_bounds__(kPlanThreads)
     table.head[3] = 0;
   }
   int total;
-  const int mine = scan_add(change[tid], sums, total) + change[tid] + rest[tid];
+  const int own = change[tid], more = rest[tid];  // read before the scan's barriers: both arrays are overwritten after it
+  const int mine = scan_add(own, sums, total) + own + more;
   change[kPlanThreads - 1 - tid] = mine;  // heaviest bin first
   __syncthreads();
   const int place = scan_add(change[tid], sums, total);
