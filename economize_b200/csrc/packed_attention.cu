@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kPlanThreads)
                        unsigned* status) {
   // Tiles are sorted by bins of their weight (tile i reads i + 1 times as many keys as tile 0), a thread per bin:
   // `change` counts how many tiles a bin has more than the one before, `rest` those of sequences that end in it.
-  __shared__ int change[kPlanThreads], rest[kPlanThreads];
+  __shared__ int change[kPlanThreads], rest[kPlanThreads], near_lo[kPlanThreads + 1], near_base[kPlanThreads + 1];
   __shared__ int sums[32];
   __shared__ int carry_max, carry_tiles;
   pdl_trigger();
@@ -96,7 +96,9 @@ __global__ void __launch_bounds__(kPlanThreads)
   const PackedTable& table = args.tables[blockIdx.x];
   int4* entries = static_cast<int4*>(table.entries);
   const int rows = table.rows, max_tiles = table.max_tiles;
-  int *lo = table.scratch, *base = lo + B + 1;
+  // searched per tile, in shared memory where they fit
+  int* lo = B <= kPlanThreads ? near_lo : table.scratch;
+  int* base = B <= kPlanThreads ? near_base : table.scratch + B + 1;
   const int per = (max_tiles + kPlanThreads - 2) / (kPlanThreads - 1);  // weights of a bin
   change[tid] = 0;
   rest[tid] = 0;
@@ -244,7 +246,7 @@ __global__ void __launch_bounds__((FwdCfg<DP, kTiles>::kThreads), (3 - kTiles))
   pdl_trigger();
   pdl_wait();
 
-  zero_padding(p.out, p.T, static_cast<long>(p.H) * p.D, p.head);
+  zero_padding(p.out, p.T, static_cast<long>(p.H) * p.D, p.head, threadIdx.x, Cfg::kThreads);
   const int group = p.H / p.Hkv;
   const int ksteps = (p.D + 15) / 16;
   const int tokens = kRowsT >> p.lp;  // of a query tile

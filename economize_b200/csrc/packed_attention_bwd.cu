@@ -169,6 +169,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     work.init(kComputeWarps + 2);
     *abort_flag = 0;
     fence_mbar_init();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+    tma_prefetch_desc(&tm_do);
   }
   __syncwarp();
   if (warp == 0) tmem_alloc(tmem_slot, 512);
@@ -180,11 +184,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   pdl_trigger();
   pdl_wait();
 
-  const int splits = kSplit ? p.splits : 1;
-  if (!kSplit) {
-    zero_padding(p.dk, p.T, static_cast<long>(p.Hkv) * p.D, p.dkv_head);
-    zero_padding(p.dv, p.T, static_cast<long>(p.Hkv) * p.D, p.dkv_head);
+  if (!kSplit && warp >= 4) {
+    zero_padding(p.dk, p.T, static_cast<long>(p.Hkv) * p.D, p.dkv_head, threadIdx.x - 128, kComputeWarps * 32);
+    zero_padding(p.dv, p.T, static_cast<long>(p.Hkv) * p.D, p.dkv_head, threadIdx.x - 128, kComputeWarps * 32);
   }
+  const int splits = kSplit ? p.splits : 1;
   const int group = p.H / p.Hkv;
   const int ksteps = (p.D + 15) / 16;
   const int tokens = kRowsT >> p.lp, packs = group >> p.lp;
@@ -586,6 +590,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     work.init(kComputeWarps + 3);  // the issuing warp follows the items twice
     *abort_flag = 0;
     fence_mbar_init();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+    tma_prefetch_desc(&tm_do);
+    tma_prefetch_desc(&tm_k32);
+    tma_prefetch_desc(&tm_v32);
   }
   __syncwarp();
   if (warp == 0) tmem_alloc(tmem_slot, 512);
@@ -597,7 +607,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   pdl_trigger();
   pdl_wait();
 
-  zero_padding(p.dq, p.T, static_cast<long>(p.H) * p.D, p.dq_head);
+  if (warp >= 4)
+    zero_padding(p.dq, p.T, static_cast<long>(p.H) * p.D, p.dq_head, threadIdx.x - 128, kComputeWarps * 32);
   const int group = p.H / p.Hkv;
   const int ksteps = (p.D + 15) / 16;
 

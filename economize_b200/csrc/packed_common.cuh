@@ -154,12 +154,12 @@ __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t p, uint32_t b, int
   }
 }
 
-// Zero the rows of x [T, width] outside the sequences (16-byte groups), shared by the grid.
-__device__ __forceinline__ void zero_padding(bf16* x, int T, long width, const int* head) {
+// Zero the rows of x [T, width] outside the sequences (16-byte groups), shared by `threads` threads of every CTA, this
+// one the `tid`-th of them.
+__device__ __forceinline__ void zero_padding(bf16* x, int T, long width, const int* head, int tid, int threads) {
   const int first = head[1], last = head[2];
   const long groups = (static_cast<long>(first) + (T - last)) * (width / 8);
-  for (long i = static_cast<long>(blockIdx.x) * blockDim.x + threadIdx.x; i < groups;
-       i += static_cast<long>(gridDim.x) * blockDim.x) {
+  for (long i = static_cast<long>(blockIdx.x) * threads + tid; i < groups; i += static_cast<long>(gridDim.x) * threads) {
     long row = i / (width / 8);
     if (row >= first) row += last - first;
     *reinterpret_cast<uint4*>(x + row * width + (i % (width / 8)) * 8) = make_uint4(0, 0, 0, 0);
