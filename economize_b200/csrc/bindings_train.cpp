@@ -102,8 +102,6 @@ std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> readout(
 
   // One workspace: row lists, losses, target logits, statistics, packed states, e, partial products.
   const int64_t pieces = ecz::readout_pieces(static_cast<int>(V));
-  const long tiles = ((chunk + 255) / 256) * ((H + 255) / 256);
-  const int splits = need_dx ? ecz::readout_splits(tiles, (V + 63) / 64, sms) : 1;
   int64_t bytes = 0;
   auto place = [&](int64_t n) {
     const int64_t at = bytes;
@@ -114,7 +112,7 @@ std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> readout(
   const int64_t o_rows = place(4 * T), o_target = place(4 * T), o_pos = place(planned ? 4 * T : 0), o_count = place(8);
   const int64_t o_picked = place(4 * T), o_nll = place(4 * T), o_stats = place(8 * chunk * pieces);
   const int64_t o_xs = place(2 * (T + 64) * xld), o_e = place(grads ? 2 * chunk * ld : 0);
-  const int64_t o_part = place(splits > 1 ? 4 * splits * chunk * H : 0);
+  const int64_t o_part = place(grads ? ecz::readout_part_bytes(sms) : 0);
   const int64_t o_sum = place(need_dw && chunks > 1 ? 4 * V * H : 0);
   Tensor workspace = at::empty({bytes}, hidden.options().dtype(at::kByte));
   uint8_t* ws = workspace.data_ptr<uint8_t>();
@@ -171,14 +169,14 @@ std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> readout(
           "finish");
     if (need_dx) {
       const CUtensorMap dz = map_2d(e, padded, V, ld, 128);
-      check(ecz::launch_readout_dx(&dz, &w_cols, c, splits, reinterpret_cast<float*>(ws + o_part), dx->data_ptr(), sms,
+      check(ecz::launch_readout_dx(&dz, &w_cols, c, reinterpret_cast<float*>(ws + o_part), dx->data_ptr(), sms,
                                    status, stream),
             "dx");
     }
     if (need_dw) {
       const CUtensorMap dz = map_2d(e, padded, V, ld, 64);
       const CUtensorMap x_cols = map_2d(xs0, padded, H, xld, 64);
-      check(ecz::launch_readout_dw(&dz, &x_cols, c, chunks > 1 ? reinterpret_cast<float*>(ws + o_sum) : nullptr, i == 0,
+      check(ecz::launch_readout_dw(&dz, &x_cols, c, reinterpret_cast<float*>(ws + o_part), chunks > 1 ? reinterpret_cast<float*>(ws + o_sum) : nullptr, i == 0,
                                    i == chunks - 1, dw->data_ptr(), sms, status, stream),
             "dw");
     }

@@ -12,7 +12,13 @@
 //   warp 1      MMA issuer (even CTA only)
 //   warps 2-9   epilogue: warp w reads TMEM lanes 32 (w % 4) .. + 31 and 128 of the 256 columns
 //
-// The grid is persistent over (tile, split) units; every wait is bounded (common.cuh).
+// The grid is persistent over tiles. Tiles beyond whole rounds of all pairs are split along K where that fills the pairs
+// (Schedule): their units leave fp32 partial tiles that a joining kernel adds up in order. Every wait is bounded
+// (common.cuh).
+//
+// Measured on one B200, 4096 rows, K or N = 4096 and 32000 (burst): both operands K-major 1529 TFLOP/s, B MN-major 1415,
+// both MN-major 1567; the tensor pipes are busy 84 to 85% of the cycles, and at about 1.5 GHz the power limit of 1 kW is
+// what bounds it in a long step.
 #pragma once
 
 #include "common.cuh"
@@ -33,6 +39,8 @@ constexpr int kPatchBytes = 32 * kPatchStride;
 constexpr int kSmem = kStages * kStageBytes + kEpiWarps * kPatchBytes + 1024 + 256;
 static_assert(kSmem <= 232448, "227 KB of shared memory");
 
+constexpr int kSplitBlocks = 8, kTailBlocks = 64;  // see Schedule
+
 // What a launch computes. Counts on the device (rows_dev) clip M (clip_m) or K (clip_k) of a chunk of rows that
 // starts at row0: limit = clamp(*rows_dev - row0, 0, M or K).
 struct Shape {
@@ -40,7 +48,8 @@ struct Shape {
   const int* rows_dev;
   int row0;
   bool clip_m, clip_k;
-  int splits;      // K is divided over this many units per tile
+  int pairs;       // CTA pairs of the device
+  bool split;      // tiles beyond whole rounds may be split along K
   bool n_fastest;  // order of the tiles: N varies fastest (else M)
 };
 
@@ -100,13 +109,17 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, int kk) {
   return MN ? desc_mnmajor_sw128(addr + kk * 16 * 128, kOperandBytes / 2) : desc_kmajor_sw128(addr + kk * 32);
 }
 
-// A unit of the persistent grid: tile (m0, n0) and the K blocks [kb0, kb0 + nkb) of its split.
+// A unit of the persistent grid: tile (m0, n0) and the K blocks [kb0, kb0 + nkb) of its split; `tail`: the tile's place
+// among the split ones.
 struct Unit {
-  int m0, n0, split, kb0, nkb;
+  int m0, n0, split, splits, tail, kb0, nkb;
 };
 
+// Tiles in order of units, the first `whole` in one piece. The rest (fewer than the pairs) in as many as fill the pairs
+// once, each with eight K blocks at least (a shorter one is all prologue) and, behind whole rounds, of 64 K blocks or
+// more: a round of those takes 18 us, the joining kernel 5.
 struct Schedule {
-  int m_tiles, n_tiles, units, kblocks, per_split;
+  int m_tiles, n_tiles, whole, splits, units, kblocks;
   const Shape& s;
   int M, K;
   __device__ __forceinline__ explicit Schedule(const Shape& shape) : s(shape) {
@@ -116,23 +129,40 @@ struct Schedule {
     K = s.clip_k ? min(s.K, rows) : s.K;
     m_tiles = (M + kTile - 1) / kTile;
     n_tiles = (s.N + kTile - 1) / kTile;
-    units = m_tiles * n_tiles * s.splits;
     kblocks = (K + kBK - 1) / kBK;
-    per_split = (kblocks + s.splits - 1) / s.splits;
+    const int tiles = m_tiles * n_tiles, rest = tiles % s.pairs;
+    splits = s.split && rest > 0 && (rest == tiles || kblocks >= kTailBlocks)
+                 ? max(1, min(s.pairs / rest, kblocks / kSplitBlocks)) : 1;
+    whole = splits > 1 ? tiles - rest : tiles;
+    units = whole + (tiles - whole) * splits;
   }
   __device__ __forceinline__ Unit unit(int u) const {
     Unit r;
-    r.split = u % s.splits;
-    const int t = u / s.splits;
+    const bool part = u >= whole;
+    r.splits = part ? splits : 1;
+    r.tail = part ? (u - whole) / splits : 0;
+    r.split = part ? (u - whole) - r.tail * splits : 0;
+    const int t = part ? whole + r.tail : u;
     const int mt = s.n_fastest ? t / n_tiles : t % m_tiles;
     const int nt = s.n_fastest ? t % n_tiles : t / m_tiles;
     r.m0 = mt * kTile;
     r.n0 = nt * kTile;
-    r.kb0 = min(kblocks, r.split * per_split);
-    r.nkb = min(per_split, kblocks - r.kb0);
+    const int per = part ? (kblocks + splits - 1) / splits : kblocks;
+    r.kb0 = min(kblocks, r.split * per);
+    r.nkb = min(per, kblocks - r.kb0);
     return r;
   }
 };
+
+// Most split tiles of a launch, and whether it may have any.
+inline int most_tail(const Shape& s) {
+  const int tiles = ((s.M + kTile - 1) / kTile) * ((s.N + kTile - 1) / kTile);
+  const int kblocks = (s.K + kBK - 1) / kBK;
+  if (!s.split || kblocks < 2 * kSplitBlocks) return 0;
+  if (s.clip_m) return tiles < s.pairs / 2 ? tiles : s.pairs / 2;
+  const int rest = tiles % s.pairs;
+  return 2 * rest <= s.pairs && (rest == tiles || kblocks >= kTailBlocks) ? rest : 0;
+}
 
 // Epi: a functor `void operator()(const Unit&, int M, int row0, int col0, uint32_t taddr, bool zero, uint8_t* patch,
 // int lane)` of one warp: rows row0 + lane (of the whole output), columns [col0, col0 + 128), accumulators at TMEM
@@ -275,11 +305,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 template <bool A_MN, bool B_MN, class Epi>
-inline int launch_pair(const CUtensorMap& a, const CUtensorMap& b, const Shape& shape, const Epi& epi, int num_sms,
+inline int launch_pair(const CUtensorMap& a, const CUtensorMap& b, const Shape& shape, const Epi& epi,
                        unsigned* status, cudaStream_t stream) {
-  const long tiles = static_cast<long>((shape.M + kTile - 1) / kTile) * ((shape.N + kTile - 1) / kTile) * shape.splits;
+  const long tiles = static_cast<long>((shape.M + kTile - 1) / kTile) * ((shape.N + kTile - 1) / kTile);
   if (tiles <= 0) return 0;
-  const int pairs = static_cast<int>(tiles < num_sms / 2 ? tiles : num_sms / 2);
+  const int pairs = shape.split || tiles > shape.pairs ? shape.pairs : static_cast<int>(tiles);
   auto kernel = gemm_pair_kernel<A_MN, B_MN, Epi>;
   if (set_max_smem(kernel, kSmem) != cudaSuccess) return -1;
   return launch_pdl(kernel, dim3(2 * pairs), dim3(kThreads), kSmem, stream, a, b, shape, epi, status) == cudaSuccess ? 0

@@ -290,7 +290,8 @@ struct ReadoutChunk {
   const float* grad_rows = nullptr;  // [T] gradients of losses by row, or null
 };
 int readout_pieces(int V);
-int readout_splits(long tiles, long kblocks, int num_sms);
+// Workspace of the products' split tiles.
+long readout_part_bytes(int num_sms);
 // The states and head as given.
 struct ReadoutRows {
   const void *x = nullptr, *w = nullptr;
@@ -311,10 +312,11 @@ int launch_readout_logits(const CUtensorMap* xs, const CUtensorMap* w, const Rea
 // loss, done (a zeroed counter): of the last chunk of a scalar loss, else null.
 int launch_readout_finish(const ReadoutChunk& c, float* nll, float* losses, float* loss, int* done, int num_sms,
                           cudaStream_t stream);
-int launch_readout_dx(const CUtensorMap* dz, const CUtensorMap* w, const ReadoutChunk& c, int splits, float* part,
-                      void* dx, int num_sms, unsigned* status, cudaStream_t stream);
-int launch_readout_dw(const CUtensorMap* dz, const CUtensorMap* xs, const ReadoutChunk& c, float* sum, bool first,
-                      bool last, void* dw, int num_sms, unsigned* status, cudaStream_t stream);
+// part: readout_part_bytes. sum: dW's fp32 running sum [V, H] over several chunks.
+int launch_readout_dx(const CUtensorMap* dz, const CUtensorMap* w, const ReadoutChunk& c, float* part, void* dx,
+                      int num_sms, unsigned* status, cudaStream_t stream);
+int launch_readout_dw(const CUtensorMap* dz, const CUtensorMap* xs, const ReadoutChunk& c, float* part, float* sum,
+                      bool first, bool last, void* dw, int num_sms, unsigned* status, cudaStream_t stream);
 // x and y (bf16, sizes multiples of 8) times *g in place.
 int launch_scale_by(void* x, long nx, void* y, long ny, const float* g, int num_sms, cudaStream_t stream);
 

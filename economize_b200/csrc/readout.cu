@@ -390,14 +390,20 @@ __global__ void __launch_bounds__(kFinishThreads) readout_finish_kernel(const __
 }
 
 // ---- product epilogues ---------------------------------------------------------------------------------------------
-// Stores a warp's 32 x 128 accumulators: bf16 rows (through the patch, 128-byte row segments), fp32 partials of a K
-// split, or an fp32 running sum over the chunks whose last chunk stores bf16.
+// Where a split tile's partial keeps columns 32 cb + 4 q .. + 3 of row 32 rb + lane, in floats: a warp's lanes hold a row
+// each and write side by side.
+__device__ __forceinline__ int partial_at(int rb, int cb, int q, int lane) {
+  return (((rb * (pair::kTile / 32) + cb) * 8 + q) * 32 + lane) * 4;
+}
+
+// Stores a warp's 32 x 128 accumulators: bf16 rows (through the patch, 128-byte row segments), a split tile's fp32
+// partial, or an fp32 running sum over the chunks whose last chunk stores bf16.
 struct StoreEpi {
-  bf16* out;        // [.., N] or null
-  float* part;      // [splits, M, N] fp32 partials, or the running sum [M, N] (splits == 1), or null
+  bf16* out;        // [.., N]
+  float* part;      // partials of split tiles, [tile, split] and see partial_at
+  float* sum;       // running sum [M, N], or null
   const int* rows;  // destination row of row m (null: m)
   int N;
-  long part_rows;   // rows of a split's partials
   bool add, last;   // running sum: add to what is there; store the sum as bf16
   Shared shared;    // what bf16 results are multiplied by
 
@@ -405,9 +411,9 @@ struct StoreEpi {
                                              uint8_t* patch, int lane) const {
     if (row0 >= M || col0 >= N) return;
     const int cols = min(128, N - col0);
-    float* prow = part == nullptr
-                      ? nullptr
-                      : part + (static_cast<size_t>(u.split) * part_rows + row0 + lane) * static_cast<size_t>(N) + col0;
+    const bool split = u.splits > 1;
+    float* prow = sum == nullptr ? nullptr : sum + static_cast<size_t>(row0 + lane) * N + col0;
+    float* tile = part + (static_cast<size_t>(u.tail) * u.splits + u.split) * pair::kTile * pair::kTile;
     const bool row_ok = row0 + lane < M;
     const float factor = last ? shared.value() : 1.f;
 #pragma unroll 1
@@ -418,6 +424,13 @@ struct StoreEpi {
         for (int j = 0; j < 32; ++j) v[j] = 0.f;
       } else {
         tmem_ld32(taddr + c, v);
+      }
+      if (split) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+          *reinterpret_cast<float4*>(tile + partial_at((row0 - u.m0) / 32, (col0 - u.n0 + c) / 32, j / 4, lane)) =
+              make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        continue;
       }
       if (prow != nullptr && row_ok) {
 #pragma unroll
@@ -467,33 +480,49 @@ struct StoreEpi {
   }
 };
 
-constexpr int kJoinThreads = 128;
+constexpr int kJoinThreads = 256;
 
-// out[rows[m]] = bf16(the shared factor times the sum over splits, in order, of part[s, m]).
+// The split tiles of a product: out[rows[m]] = bf16(the shared factor times the sum of the partials, in order). A thread
+// adds up eight columns of a row; CTAs (32 rows, tile, place of the eight in every 32 columns).
 __global__ void __launch_bounds__(kJoinThreads)
-    readout_join_kernel(const float* __restrict__ part, int splits, long part_rows, int N, int row0, int chunk,
+    readout_join_kernel(const __grid_constant__ pair::Shape shape, const float* __restrict__ part, const int* rows,
                         Shared shared, bf16* __restrict__ out) {
   pdl_trigger();
   pdl_wait();
-  const int n = min(chunk, *shared.count - row0);
-  const long i = (static_cast<long>(blockIdx.x) * kJoinThreads + threadIdx.x) * 4;
-  const long m = i / N, c = i % N;
-  if (m >= n) return;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int s = 0; s < splits; ++s) {
-    const float4 v = *reinterpret_cast<const float4*>(part + (s * part_rows + m) * N + c);
-    acc.x += v.x;
-    acc.y += v.y;
-    acc.z += v.z;
-    acc.w += v.w;
-  }
+  const pair::Schedule sched(shape);
+  const int u = sched.whole + blockIdx.y * sched.splits;
+  if (sched.splits == 1 || u >= sched.units) return;
+  const pair::Unit t = sched.unit(u);
+  const int rb = blockIdx.x, cb = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int m = t.m0 + rb * 32 + lane;
+  if (m >= sched.M) return;
+  const float* tile = part + static_cast<size_t>(t.tail) * t.splits * pair::kTile * pair::kTile;
   const float f = shared.value();
-  __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * f, acc.y * f), hi = __floats2bfloat162_rn(acc.z * f, acc.w * f);
-  uint2 w;
-  w.x = *reinterpret_cast<uint32_t*>(&lo);
-  w.y = *reinterpret_cast<uint32_t*>(&hi);
-  *reinterpret_cast<uint2*>(out + static_cast<long>(shared.rows[row0 + m]) * N + c) = w;
+  bf16* row = out + static_cast<long>(rows != nullptr ? rows[m] : m) * shape.N;
+  const int q = blockIdx.z * 2, n = t.n0 + cb * 32 + q * 4;
+  if (n >= shape.N) return;
+  float acc[8] = {};
+#pragma unroll 4
+  for (int i = 0; i < t.splits; ++i) {
+    const float* from = tile + static_cast<size_t>(i) * pair::kTile * pair::kTile;
+    const float4 a = *reinterpret_cast<const float4*>(from + partial_at(rb, cb, q, lane));
+    const float4 b = *reinterpret_cast<const float4*>(from + partial_at(rb, cb, q + 1, lane));
+    acc[0] += a.x;
+    acc[1] += a.y;
+    acc[2] += a.z;
+    acc[3] += a.w;
+    acc[4] += b.x;
+    acc[5] += b.y;
+    acc[6] += b.z;
+    acc[7] += b.w;
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(acc[2 * k] * f, acc[2 * k + 1] * f);
+    w[k] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  *reinterpret_cast<uint4*>(row + n) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // x and y times *g in place (bf16, sizes in groups of 8); reads nothing more when *g is 1, what a loss's own backward
@@ -523,14 +552,6 @@ __global__ void __launch_bounds__(256) scale_by_kernel(uint4* __restrict__ x, lo
 
 int readout_pieces(int V) { return (V + kPiece - 1) / kPiece; }
 
-// Splits of K for a product of `tiles` 256 x 256 tiles and `kblocks` K blocks: as many as fill the pairs of SMs once,
-// each with eight K blocks at least (a shorter one is all prologue).
-int readout_splits(long tiles, long kblocks, int num_sms) {
-  const long pairs = num_sms / 2;
-  if (tiles >= pairs) return 1;
-  return static_cast<int>(std::max(1l, std::min(pairs / std::max(1l, tiles), kblocks / 8)));
-}
-
 bool readout_needs_plan(int T) { return T > kPlanRows; }
 
 int launch_readout_plan(const int64_t* targets, int T, int V, int64_t ignore, int* pos, int* count, unsigned* status,
@@ -552,8 +573,8 @@ int launch_readout_logits(const CUtensorMap* xs, const CUtensorMap* w, const Rea
                           unsigned* status, cudaStream_t stream) {
   LogitsEpi epi{static_cast<float2*>(c.stats), c.target + c.row0, static_cast<__half*>(c.e), c.ld, c.V,
                 readout_pieces(c.V), c.logit_scale * kLog2e};
-  const pair::Shape shape{c.chunk, c.V, c.H, c.count, c.row0, true, false, 1, false};
-  return pair::launch_pair<false, false>(*xs, *w, shape, epi, num_sms, status, stream);
+  const pair::Shape shape{c.chunk, c.V, c.H, c.count, c.row0, true, false, num_sms / 2, false, false};
+  return pair::launch_pair<false, false>(*xs, *w, shape, epi, status, stream);
 }
 
 static Shared shared_of(const ReadoutChunk& c) {
@@ -574,24 +595,32 @@ int launch_readout_finish(const ReadoutChunk& c, float* nll, float* losses, floa
                                                                                                                    : -1;
 }
 
-int launch_readout_dx(const CUtensorMap* dz, const CUtensorMap* w, const ReadoutChunk& c, int splits, float* part,
-                      void* dx, int num_sms, unsigned* status, cudaStream_t stream) {
-  StoreEpi epi{static_cast<bf16*>(dx), splits > 1 ? part : nullptr, c.rows + c.row0, c.H, c.chunk, false, splits == 1,
-               shared_of(c)};
-  const pair::Shape shape{c.chunk, c.H, c.V, c.count, c.row0, true, false, splits, false};
-  int rc = pair::launch_pair<false, true>(*dz, *w, shape, epi, num_sms, status, stream);
-  if (rc != 0 || splits == 1) return rc;
-  const long groups = static_cast<long>(c.chunk) * c.H / 4;
-  return launch_pdl(readout_join_kernel, dim3(static_cast<unsigned>((groups + kJoinThreads - 1) / kJoinThreads)),
-                    dim3(kJoinThreads), 0, stream, part, splits, static_cast<long>(c.chunk), c.H, c.row0, c.chunk,
-                    shared_of(c), static_cast<bf16*>(dx)) == cudaSuccess ? 0 : -1;
+static int launch_join(const pair::Shape& shape, const float* part, const int* rows, const ReadoutChunk& c, void* out,
+                       cudaStream_t stream) {
+  const int tail = pair::most_tail(shape);
+  if (tail == 0) return 0;
+  return launch_pdl(readout_join_kernel, dim3(pair::kTile / 32, tail, 4), dim3(kJoinThreads), 0,
+                    stream, shape, part, rows, shared_of(c), static_cast<bf16*>(out)) == cudaSuccess ? 0 : -1;
 }
 
-int launch_readout_dw(const CUtensorMap* dz, const CUtensorMap* xs, const ReadoutChunk& c, float* sum, bool first,
-                      bool last, void* dw, int num_sms, unsigned* status, cudaStream_t stream) {
-  StoreEpi epi{static_cast<bf16*>(dw), first && last ? nullptr : sum, nullptr, c.H, 0, !first, last, shared_of(c)};
-  const pair::Shape shape{c.V, c.H, c.chunk, c.count, c.row0, false, true, 1, true};
-  return pair::launch_pair<true, true>(*dz, *xs, shape, epi, num_sms, status, stream);
+long readout_part_bytes(int num_sms) { return static_cast<long>(num_sms / 2) * pair::kTile * pair::kTile * 4; }
+
+int launch_readout_dx(const CUtensorMap* dz, const CUtensorMap* w, const ReadoutChunk& c, float* part, void* dx,
+                      int num_sms, unsigned* status, cudaStream_t stream) {
+  const int* rows = c.rows + c.row0;
+  const StoreEpi epi{static_cast<bf16*>(dx), part, nullptr, rows, c.H, false, true, shared_of(c)};
+  const pair::Shape shape{c.chunk, c.H, c.V, c.count, c.row0, true, false, num_sms / 2, true, false};
+  const int rc = pair::launch_pair<false, true>(*dz, *w, shape, epi, status, stream);
+  return rc != 0 ? rc : launch_join(shape, part, rows, c, dx, stream);
+}
+
+int launch_readout_dw(const CUtensorMap* dz, const CUtensorMap* xs, const ReadoutChunk& c, float* part, float* sum,
+                      bool first, bool last, void* dw, int num_sms, unsigned* status, cudaStream_t stream) {
+  const bool once = first && last;
+  const StoreEpi epi{static_cast<bf16*>(dw), part, once ? nullptr : sum, nullptr, c.H, !first, last, shared_of(c)};
+  const pair::Shape shape{c.V, c.H, c.chunk, c.count, c.row0, false, true, num_sms / 2, once, true};
+  const int rc = pair::launch_pair<true, true>(*dz, *xs, shape, epi, status, stream);
+  return rc != 0 ? rc : launch_join(shape, part, nullptr, c, dw, stream);
 }
 
 int launch_scale_by(void* x, long nx, void* y, long ny, const float* g, int num_sms, cudaStream_t stream) {
