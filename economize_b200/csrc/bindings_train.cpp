@@ -176,7 +176,8 @@ std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>> readout(
     if (need_dw) {
       const CUtensorMap dz = map_2d(e, padded, V, ld, 64);
       const CUtensorMap x_cols = map_2d(xs0, padded, H, xld, 64);
-      check(ecz::launch_readout_dw(&dz, &x_cols, c, reinterpret_cast<float*>(ws + o_part), chunks > 1 ? reinterpret_cast<float*>(ws + o_sum) : nullptr, i == 0,
+      check(ecz::launch_readout_dw(&dz, &x_cols, c, reinterpret_cast<float*>(ws + o_part),
+                                   chunks > 1 ? reinterpret_cast<float*>(ws + o_sum) : nullptr, i == 0,
                                    i == chunks - 1, dw->data_ptr(), sms, status, stream),
             "dw");
     }
@@ -255,8 +256,8 @@ ecz::PackedArgs packed_args(const Tensor& q, const Tensor& k, int64_t B, double 
 // Output [T, H, D] and, for a backward pass, what its rounding left, the log2-domain log-sum-exp of every row [H, T] and
 // the tile tables.
 // tiles: query tiles a CTA works on (0: by the mean length).
-std::tuple<Tensor, Tensor, Tensor, Tensor> packed_forward(Tensor q, Tensor k, Tensor v, Tensor cu, double scale, bool training,
-                                                  int64_t tiles) {
+std::tuple<Tensor, Tensor, Tensor, Tensor> packed_forward(Tensor q, Tensor k, Tensor v, Tensor cu, double scale,
+                                                          bool training, int64_t tiles) {
   check_packed(q, k, v, cu, scale);
   TORCH_CHECK(tiles >= 0 && tiles <= 2, "packed_attention: tiles must be 0, 1 or 2");
   c10::cuda::CUDAGuard guard(q.device());
@@ -300,8 +301,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> packed_forward(Tensor q, Tensor k, Te
 // Gradients of q, k and v (those asked for; undefined otherwise) given the output's. plan, tiles: of the forward pass
 // over B sequences.
 std::tuple<Tensor, Tensor, Tensor> packed_backward(Tensor dout, Tensor q, Tensor k, Tensor v, const Tensor& out,
-                                                   const Tensor& rest, const Tensor& lse, const Tensor& plan, int64_t B, double scale,
-                                                   int64_t tiles, bool need_dq, bool need_dkv) {
+                                                   const Tensor& rest, const Tensor& lse, const Tensor& plan,
+                                                   int64_t B, double scale, int64_t tiles, bool need_dq, bool need_dkv) {
   CHECK_BF16(dout);
   CHECK_ON(dout, q);
   TORCH_CHECK(dout.sizes() == q.sizes(), "packed_attention: the output's gradient has the queries' shape");

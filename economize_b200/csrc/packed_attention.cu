@@ -39,8 +39,9 @@ constexpr float kFar = 60.f;
 
 // ---- plan ----------------------------------------------------------------------------------------------------------
 // One CTA per table: a list of tiles of `rows` tokens, heaviest first: entry = (first token, end, tile, tiles of its
-// sequence); head = (tiles, first token of the first sequence, end of the last, items taken). Offsets outside [0, T] or falling are
-// clamped (a sequence starts where the one before it ended at the earliest) and reported.
+// sequence); head = (tiles, first token of the first sequence, end of the last, items taken). Offsets outside [0, T] or
+// falling are clamped (a sequence starts where the one before it ended at the earliest) and reported. Latency bounds it:
+// scans and a search per tile, 10 us for the tables of all three kernels of 8192 tokens in 5 sequences, 32 heads over 8.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanTables = 3;
 
@@ -164,11 +165,17 @@ __global__ void __launch_bounds__(kPlanThreads)
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------
-// kTiles 2: a CTA per SM works on two tiles that share the K / V chunks. kTiles 1: two CTAs per SM work on a tile each, with
-// half the shared memory and TMEM: they load K and V twice, but are not tied to one another's phases, which is what
+// kTiles 2: a CTA per SM works on two tiles that share the K / V chunks. kTiles 1: two CTAs per SM work on a tile each,
+// with half the shared memory and TMEM: they load K and V twice, but are not tied to one another's phases, which is what
 // counts where an item is a chunk or two (see packed_single_tiles).
 // One thread per row: with two (sixteen softmax warps that exchange their maxima) a document of 16384 tokens, 16 heads
 // over 4, took 973 us instead of 885.
+//
+// Measured on one B200, D = 128: that document 830 us, 1320 TFLOP/s of its 4 D n (n + 1) / 2 useful operations, bound by
+// the tensor cores at the clock that 1 kW leaves them; 8 sequences of 1024, 32 heads over 8, 97 us, 830 TFLOP/s: the
+// diagonal chunks' hidden half and seven or eight items to a CTA cost the rest (49% of the tensor pipes' cycles at 1638
+// tokens in the mean); 4096 tokens in 48 sequences 33 us, 3.7 TB/s: an item is a chunk or two, and the latency of its
+// loads, softmax and store bounds it.
 template <int DP, int kTiles>
 struct FwdCfg {
   static constexpr int kTileBytes = kRowsT * DP * 2;
@@ -601,8 +608,8 @@ int launch_packed_plan(const int* cu, int B, int T, const PackedTable* tables, i
                  cudaSuccess ? 0 : -1;
 }
 
-// Measured on one B200, us for one / two tiles: D = 64, 12 heads of their own, 8192 tokens in sequences of 16: 61 / 112, of
-// 128: 23.8 / 31.4, of 1024: 35.9 / 39.0, one of 8192: 152 / 164. D = 128, 32 heads over 8, of 16: 56 / 96, of 128:
+// Measured on one B200, us for one / two tiles: D = 64, 12 heads of their own, 8192 tokens in sequences of 16: 61 / 112,
+// of 128: 23.8 / 31.4, of 1024: 35.9 / 39.0, one of 8192: 152 / 164. D = 128, 32 heads over 8, of 16: 56 / 96, of 128:
 // 47.7 / 46.6, of 512: 69.8 / 63.3, of 1024: 96.5 / 87.0, of 8192: 496 / 447; 6490 tokens in 18 sequences 73.2 / 70.5;
 // 4096 tokens in 48: 32.6 / 35.4.
 bool packed_single_tiles(int T, int B, int D) { return D <= 64 || static_cast<long>(T) < 512l * B; }

@@ -323,8 +323,9 @@ __device__ __forceinline__ void load_packed(uint32_t taddr, float f, uint4 (&c)[
   }
 }
 
-// 64 columns of the warp's TMEM lanes, times each lane's f, as bf16 rows through 4 KB of shared memory (16-byte groups swizzled by the row, so that neither side
-// conflicts), with fewer instructions. kRest: what bf16 rounds away of the values instead (itself rounded to bf16).
+// 64 columns of the warp's TMEM lanes, times each lane's f, as bf16 rows through 4 KB of shared memory (16-byte groups
+// swizzled by the row, so that neither side conflicts). kRest: what bf16 rounds away of the values instead (itself
+// rounded to bf16).
 template <bool kRest>
 __device__ __forceinline__ void stage_tmem64(uint32_t taddr, float f, uint8_t* stage, const TileOut& to, int row0,
                                              int lane) {
