@@ -287,7 +287,7 @@ struct Shared {
   // the first row's gradient: rows of one gradient, as a mean of the losses gives them, have entries as a sum's
   __device__ __forceinline__ float grad() const {
     const float g = grad_rows != nullptr && *count > 0 ? fabsf(grad_rows[rows[0]]) : 1.f;
-    return g > 0x1p-60f && g < 0x1p60f ? g : 1.f;  // and no quotient of two gradients overflows for it
+    return g > 0x1p-40f && g < 0x1p40f ? g : 1.f;  // a quotient of another row's, below 2^87, does not overflow
   }
   __device__ __forceinline__ float value() const {
     const float f = logit_scale * grad();

@@ -108,6 +108,19 @@ def test_what_all_rows_share_is_not_rounded(cuda, rows):
             assert abs(slope.item() - 1) < 2e-4
 
 
+@pytest.mark.parametrize("first", [0.0, 1e-30, 3e-9, -2e5, 1e30])
+def test_the_first_rows_gradient_is_any(cuda, first):
+    """Rows' gradients are kept relative to the first row's where that is neither zero nor extreme."""
+    x, w, y = _inputs(cuda, 40, 256, 700, seed=10)
+    g = torch.randn(40, device=cuda)
+    g[0] = first
+    a, b = x.detach().requires_grad_(), w.detach().requires_grad_()
+    dx, dw = torch.autograd.grad(ops.linear_cross_entropy(a, b, y, reduction="none"), (a, b), g)
+    o = _oracle(x, w, y, 1.0, g)
+    _within(dx, o["dx"], o["dx_err"], "dx")
+    _within(dw, o["dw"], o["dw_err"], "dw")
+
+
 @pytest.mark.parametrize("chunk", [64, 128, 320])
 def test_chunks_of_rows(cuda, chunk):
     """Several chunks: every output as from one, weight gradients summed in fp32 in between."""
