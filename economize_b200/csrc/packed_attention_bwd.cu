@@ -466,10 +466,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const long stride = static_cast<long>(p.Hkv) * p.D;
         const long at0 = key0 * stride + static_cast<long>(kvh) * p.D + col;
         if (!kSplit) {
-          const TileOut to{(values ? p.dv : p.dk) + at0, stride, 0, 0, hi - key0, p.D - col};
-          uint4 c[kCols / 8];
-          load_packed(t_sum, values ? 1.f : p.scale, c);
-          store_rows(c, to, quad * 32, lane);
+#pragma unroll
+          for (int d = 0; d < kCols; d += 32) {
+            const TileOut to{(values ? p.dv : p.dk) + at0 + d, stride, 0, 0, hi - key0, p.D - col - d};
+            uint4 c[4];
+            load_packed(t_sum + d, values ? 1.f : p.scale, c);
+            store_rows(c, to, quad * 32, lane);
+          }
         } else {  // this split's sum, fp32, or zeros of a split without query tiles
           const long sums = static_cast<long>(keys.split) * 2 + (values ? 0 : 1);
           float* dst = p.part + sums * p.T * stride + at0 + key * stride;
