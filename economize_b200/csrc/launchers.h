@@ -320,8 +320,8 @@ int launch_readout_dw(const CUtensorMap* dz, const CUtensorMap* xs, const Readou
 // x and y (bf16, sizes multiples of 8) times *g in place.
 int launch_scale_by(void* x, long nx, void* y, long ny, const float* g, int num_sms, cudaStream_t stream);
 
-// packed_attention.cu: causal attention over packed sequences (see the file comment). A tile of queries is 128 rows: 128 >>
-// lp tokens of 1 << lp heads of a group (packed_heads_log2). Maps, 3-D {D, heads, T} with the 128-byte swizzle: q and
+// packed_attention.cu: causal attention over packed sequences (see the file comment). A tile of queries is 128 rows:
+// 128 >> lp tokens of 1 << lp heads of a group (packed_heads_log2). Maps, 3-D {D, heads, T} with the 128-byte swizzle: q and
 // dout with boxes {64, 1 << lp, 128 >> lp}; k and v {64, 1, 128}, k32 and v32 {64, 1, 32}.
 struct PackedMaps {
   CUtensorMap q, dout, k, v, k32, v32;
@@ -349,10 +349,9 @@ bool packed_single_tiles(int T, int B, int D);
 int launch_packed_forward(const PackedMaps& maps, const PackedArgs& a, void* out, void* rest, float* lse, int tiles,
                           unsigned* status, cudaStream_t stream);
 
-// packed_attention_bwd.cu: delta [H, T] = rows of dout . (out + rest) (both contiguous [T, H, D]), then the gradients (dq null:
-// not computed; dk and dv null: not computed).
-// taken: two counters, set to zero by the first for the second. part: fp32 [splits, 2, T, Hkv, D], for
-// splits > 1 (packed_dkv_splits: how many CTAs share a key tile's queries).
+// packed_attention_bwd.cu: delta [H, T] = rows of dout . (out + rest) (both contiguous [T, H, D]), then the gradients
+// (dq null: not computed; dk and dv null: not computed). taken: two counters, set to zero by the first for the second.
+// part: fp32 [splits, 2, T, Hkv, D], for splits > 1 (packed_dkv_splits: how many CTAs share a key tile's queries).
 int packed_dkv_splits(const PackedArgs& a, int B);
 int launch_packed_delta(const PackedArgs& a, const void* out, const void* rest, const void* dout, long stride_t,
                         long stride_h, float* delta, int* taken, cudaStream_t stream);

@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     table.head[3] = 0;
   }
   int total;
-  const int own = change[tid], more = rest[tid];  // read before the scan's barriers: both arrays are overwritten after it
+  const int own = change[tid], more = rest[tid];  // read before the scan's barriers: both are overwritten after it
   const int mine = scan_add(own, sums, total) + own + more;
   change[kPlanThreads - 1 - tid] = mine;  // heaviest bin first
   __syncthreads();

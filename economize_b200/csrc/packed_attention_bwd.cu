@@ -34,8 +34,9 @@ using namespace packed;
 
 namespace {
 
-// Warps 0-2 load, issue and fetch row statistics; sixteen compute warps, so that four per scheduler hide the latencies
-// of the tile's short phases (eight with twice the columns each spent 3000 of 4700 cycles per tile in them).
+// Warp 0 loads, 1 issues, 2 fetches row statistics (dkv) or loads Q and dO (dq); sixteen compute warps, so that four per
+// scheduler hide the latencies of the tile's short phases (eight with twice the columns each spent 3000 of 4700 cycles
+// per tile in them).
 constexpr int kComputeWarps = 16;
 constexpr int kBwdThreads = 128 + 32 * kComputeWarps;
 
@@ -524,9 +525,8 @@ __global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant_
 }
 
 // ---- dQ --------------------------------------------------------------------------------------------------------------
-// The chunks of a persistent CTA's items in one sequence: `chunk` of the item's `n`, counted over all items by `k`. The
-// issuing warp runs three of them (scores, dP and dQ are issued two, one and no chunks ahead, across items), a compute
-// group steps by two.
+// The chunks of a persistent CTA's items in one row: `chunk` of the item's `n`, counted over all items by `k`. The
+// issuing warp follows them twice, scores one chunk ahead of dP and dQ, across items.
 struct ChunkWalk {
   Items items;
   int chunk, n, k, item, lp;

@@ -25,13 +25,13 @@
 // Without gradients only the statistics of the pieces are written (8 bytes per 128 logits).
 //
 // Measured on one B200, 4096 rows x 4096 x 32000: logits 715 us (1500 TFLOP/s), finish 101 us (e read and dz written
-// once, 5.2 TB/s), dX 715 us, dW 710 us (1510 each), launched one by one; 2.6 to 2.75 ms in a row, at the clock that the power
-// limit leaves. 1024 rows x 4096 x 128256, losses only: 755 us, 1425 TFLOP/s. 16 rows x 1024 x 32000 with both gradients:
-// 87 us, of which the two reads of W and the write of dW need 30: 25 each of the three products, whose tiles of 256 rows
-// stand almost empty, and the launches of a training step's call.
+// once, 5.2 TB/s), dX 715 us, dW 710 us (1510 each), one by one; 2.6 to 2.75 ms in a row, at the clock that the power
+// limit leaves. 1024 rows x 4096 x 128256, losses only: 755 us, 1425 TFLOP/s. 16 rows x 1024 x 32000 with both
+// gradients: 87 us, of which the two reads of W and the write of dW need 30: 25 for each of the three products, whose
+// tiles of 256 rows stand almost empty, and the launches of a training step's call.
 //
-// The tensor cores cut off, not round, what their fp32 sums cannot hold: over 4096 products a log-sum-exp is low by about
-// 4e-6, which is 1e-6 of a mean loss of 4. The target's logit does not share it (below).
+// The tensor cores cut off, not round, what their fp32 sums cannot hold: over 4096 products a log-sum-exp is low by
+// about 4e-6, which is 1e-6 of a mean loss of 4. The target's logit does not share it (see the gather kernel).
 #include <algorithm>
 
 #include "gemm_pair.cuh"
@@ -159,7 +159,8 @@ __global__ void __launch_bounds__(256) readout_gather_kernel(const __grid_consta
   }
   if (p < 0) {
     if (a.dx != nullptr)
-      for (int c = lane * 8; c < a.H; c += 256) *reinterpret_cast<uint4*>(a.dx + static_cast<size_t>(t) * a.H + c) = zero;
+      for (int c = lane * 8; c < a.H; c += 256)
+        *reinterpret_cast<uint4*>(a.dx + static_cast<size_t>(t) * a.H + c) = zero;
     if (a.losses != nullptr && lane == 0) a.losses[t] = 0.f;
     return;
   }
@@ -400,8 +401,8 @@ __global__ void __launch_bounds__(kFinishThreads) readout_finish_kernel(const __
 }
 
 // ---- product epilogues ---------------------------------------------------------------------------------------------
-// Where a split tile's partial keeps columns 32 cb + 4 q .. + 3 of row 32 rb + lane, in floats: a warp's lanes hold a row
-// each and write side by side.
+// Where a split tile's partial keeps columns 32 cb + 4 q .. + 3 of row 32 rb + lane, in floats: a warp's lanes hold a
+// row each and write side by side.
 __device__ __forceinline__ int partial_at(int rb, int cb, int q, int lane) {
   return (((rb * (pair::kTile / 32) + cb) * 8 + q) * 32 + lane) * 4;
 }
