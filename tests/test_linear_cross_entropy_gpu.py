@@ -245,6 +245,33 @@ def test_same_bits_every_time_and_twice_through_one_graph(cuda):
     assert torch.equal(first[0], runs[0][1] * 2) and torch.equal(first[1], runs[0][2] * 2)
 
 
+@pytest.mark.parametrize("rows", [40, 2500])
+def test_as_a_cuda_graph(cuda, rows):
+    x, w, y = _inputs(cuda, rows, 256, 1100, 0.3, seed=12)
+
+    def step():
+        a, b = x.detach().requires_grad_(), w.detach().requires_grad_()
+        loss = ops.linear_cross_entropy(a, b, y)
+        return (loss.detach(), *torch.autograd.grad(loss, (a, b)))
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        results = step()
+    for _ in range(3):
+        for t in results:
+            t.zero_()
+        graph.replay()
+        for got, ref in zip(results, want):
+            assert torch.equal(got, ref)
+    assert ops.require().status(0) == 0
+
+
 def test_only_what_is_asked_for(cuda):
     """A frozen weight or frozen states get no gradient; without any the losses are the same."""
     x, w, y = _inputs(cuda, 100, 128, 1000, 0.1, seed=11)

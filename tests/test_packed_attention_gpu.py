@@ -303,6 +303,35 @@ def test_gradients_by_differences(cuda):
         assert abs(got - slope) <= (z[name + "_err"] * step.abs()).sum() + 1e-5 * abs(slope)
 
 
+def test_twice_through_one_graph_and_as_a_cuda_graph(cuda):
+    """The counters from which CTAs take their tiles start anew with every pass and every replay."""
+    lens = [400, 3, 0, 129, 77] * 8
+    q, k, v, cu, dout = _inputs(cuda, lens, 8, 2, 64, pad=4, seed=30)
+    want = _run(q, k, v, cu, dout)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    out = ops.packed_attention(*leaves, cu)
+    for _ in range(2):
+        for got, ref in zip(torch.autograd.grad(out, leaves, dout, retain_graph=True), want[1:]):
+            assert torch.equal(got, ref)
+    for got, ref in zip(torch.autograd.grad(out, leaves[1:], dout), want[2:]):  # dQ not asked for
+        assert torch.equal(got, ref)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _run(q, k, v, cu, dout)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        results = _run(q, k, v, cu, dout)
+    for _ in range(3):
+        for x in results:
+            x.zero_()
+        graph.replay()
+        for got, ref in zip(results, want):
+            assert torch.equal(got, ref)
+    assert ops.require().status(0) == 0
+
+
 def test_another_stream(cuda):
     q, k, v, cu, dout = _inputs(cuda, [300, 77], 4, 2, 128, seed=11)
     want = _run(q, k, v, cu, dout)
