@@ -206,15 +206,13 @@ CUtensorMap map_heads(const Tensor& x, int box_heads, int box_tokens) {
   return map;
 }
 
-void check_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, double scale) {
+void check_operands(const Tensor& q, const Tensor& k, const Tensor& v) {
   CHECK_CUDA(q);
   CHECK_BF16(q);
   CHECK_BF16(k);
   CHECK_BF16(v);
-  CHECK_I32(cu);
   CHECK_ON(k, q);
   CHECK_ON(v, q);
-  CHECK_ON(cu, q);
   TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, "packed_attention expects q [T, H, D], k / v [T, Hkv, D]");
   TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(2) == q.size(2),
               "packed_attention: q ", q.sizes(), ", k ", k.sizes(), " and v ", v.sizes(), " do not match");
@@ -222,8 +220,15 @@ void check_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
   TORCH_CHECK(Hkv >= 1 && H >= 1 && H % Hkv == 0, "packed_attention: ", H, " query heads over ", Hkv, " K/V heads");
   TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "packed_attention: head dimensions 8 to 128 in steps of 8 (got ", D,
               ")");
+  TORCH_CHECK(T <= (int64_t{1} << 26), "packed_attention: too many tokens");
+}
+
+void check_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, double scale) {
+  check_operands(q, k, v);
+  CHECK_I32(cu);
+  CHECK_ON(cu, q);
   TORCH_CHECK(cu.dim() == 1 && cu.size(0) >= 1, "packed_attention: cu_seqlens must be [B + 1]");
-  TORCH_CHECK(T <= (int64_t{1} << 26) && cu.size(0) <= (int64_t{1} << 24), "packed_attention: too many tokens");
+  TORCH_CHECK(cu.size(0) <= (int64_t{1} << 24), "packed_attention: too many sequences");
   TORCH_CHECK(scale > 0 && std::isfinite(scale), "packed_attention: the scale must be positive (got ", scale, ")");
 }
 
@@ -253,6 +258,14 @@ ecz::PackedArgs packed_args(const Tensor& q, const Tensor& k, int64_t B, double 
   return a;
 }
 
+// Ints of the tile tables of PackedArgs, and of the forward pass's alone (count 1).
+int64_t plan_ints(const ecz::PackedArgs& a, int64_t B) {
+  int64_t ints = 0;
+  for (const auto* t : {&a.fwd, &a.dq, &a.dkv})
+    ints += t->max_tiles > 0 ? int64_t{4} * t->max_tiles + 4 + (2 * (B + 1) + 3) / 4 * 4 : 0;
+  return ints;
+}
+
 // Output [T, H, D] and, for a backward pass, what its rounding left, the log2-domain log-sum-exp of every row [H, T] and
 // the tile tables.
 // tiles: query tiles a CTA works on (0: by the mean length).
@@ -276,10 +289,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> packed_forward(Tensor q, Tensor k, Te
   if (tiles == 0) tiles = ecz::packed_single_tiles(T, B, static_cast<int>(q.size(2))) ? 1 : 2;
   const int count = training ? 3 : 1;
   ecz::PackedArgs a = packed_args(q, k, B, scale, static_cast<int>(tiles), count, Tensor());
-  int64_t ints = 0;
-  for (const auto* t : {&a.fwd, &a.dq, &a.dkv})
-    ints += t->max_tiles > 0 ? int64_t{4} * t->max_tiles + 4 + (2 * (int64_t{B} + 1) + 3) / 4 * 4 : 0;
-  plan = at::empty({ints}, cu.options());
+  plan = at::empty({plan_ints(a, B)}, cu.options());
   a = packed_args(q, k, B, scale, static_cast<int>(tiles), count, plan);
   unsigned* status = ecz::device_status(q.device());
   const ecz::PackedTable tables[3] = {a.fwd, a.dq, a.dkv};
@@ -298,6 +308,14 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> packed_forward(Tensor q, Tensor k, Te
   return {out, rest, lse, plan};
 }
 
+// A tensor that the forward pass saved is what it was: saved-tensor hooks may return anything, and kernels read it by its
+// pointer.
+void check_saved(const Tensor& x, const Tensor& like, at::ScalarType type, at::IntArrayRef sizes, const char* what) {
+  TORCH_CHECK(x.defined() && x.is_cuda() && x.get_device() == like.get_device() && x.scalar_type() == type &&
+                  x.sizes() == sizes && x.is_contiguous() && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0,
+              "the saved ", what, " did not come back as it was saved (device, type, sizes, contiguous)");
+}
+
 // Gradients of q, k and v (those asked for; undefined otherwise) given the output's. plan, tiles: of the forward pass
 // over B sequences.
 std::tuple<Tensor, Tensor, Tensor> packed_backward(Tensor dout, Tensor q, Tensor k, Tensor v, const Tensor& out,
@@ -306,6 +324,7 @@ std::tuple<Tensor, Tensor, Tensor> packed_backward(Tensor dout, Tensor q, Tensor
   CHECK_BF16(dout);
   CHECK_ON(dout, q);
   TORCH_CHECK(dout.sizes() == q.sizes(), "packed_attention: the output's gradient has the queries' shape");
+  check_operands(q, k, v);
   c10::cuda::CUDAGuard guard(q.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   Tensor dq, dk, dv;
@@ -315,6 +334,11 @@ std::tuple<Tensor, Tensor, Tensor> packed_backward(Tensor dout, Tensor q, Tensor
     dv = at::empty(v.sizes(), v.options());
   }
   if (q.size(0) == 0 || (!need_dq && !need_dkv)) return {dq, dk, dv};
+  check_saved(out, q, at::kBFloat16, q.sizes(), "output");
+  check_saved(rest, q, at::kBFloat16, q.sizes(), "rounding rest of the output");
+  check_saved(lse, q, at::kFloat, {q.size(1), q.size(0)}, "log-sum-exps");
+  check_saved(plan, q, at::kInt,
+              {plan_ints(packed_args(q, k, B, scale, static_cast<int>(tiles), 3, Tensor()), B)}, "plan");
   q = heads_of(q);
   k = heads_of(k);
   v = heads_of(v);
@@ -431,10 +455,9 @@ struct PackedFunction : torch::autograd::Function<PackedFunction> {
       tiles = ecz::packed_single_tiles(static_cast<int>(q.size(0)), static_cast<int>(B), static_cast<int>(q.size(2)))
                   ? 1 : 2;
     auto r = packed_forward(q, k, v, cu, scale, true, tiles);
-    ctx->save_for_backward({q, k, v, std::get<0>(r)});
-    ctx->saved_data["rest"] = std::get<1>(r);
-    ctx->saved_data["lse"] = std::get<2>(r);
-    ctx->saved_data["plan"] = std::get<3>(r);
+    // all of it as saved variables: saved_data would keep the output's rest until the graph itself goes, past the
+    // backward pass and unseen by saved-tensor hooks
+    ctx->save_for_backward({q, k, v, std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r)});
     ctx->saved_data["B"] = B;
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["tiles"] = tiles;
@@ -447,8 +470,7 @@ struct PackedFunction : torch::autograd::Function<PackedFunction> {
     auto& data = ctx->saved_data;
     const bool need_dq = ctx->needs_input_grad(0);
     const bool need_dk = ctx->needs_input_grad(1), need_dv = ctx->needs_input_grad(2);
-    auto r = packed_backward(grads[0], s[0], s[1], s[2], s[3], data["rest"].toTensor(), data["lse"].toTensor(),
-                             data["plan"].toTensor(), data["B"].toInt(),
+    auto r = packed_backward(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], data["B"].toInt(),
                              data["scale"].toDouble(), data["tiles"].toInt(), need_dq, need_dk || need_dv);
     variable_list out(6);
     if (need_dq) out[0] = std::get<0>(r);

@@ -390,3 +390,69 @@ def test_refusals(cuda):
         call(q, k, v, cu, -1.0)
     with pytest.raises(RuntimeError, match="expects"):
         call(q[None], k[None], v[None], cu)
+
+
+def _held(dev, make):
+    """What ``make`` returns and the bytes that stay allocated for it."""
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated(dev)
+    result = make()
+    return result, torch.cuda.memory_allocated(dev) - before
+
+
+def test_the_backward_pass_releases_what_the_forward_pass_kept(cuda):
+    """The output's rest and the log-sum-exps go with the graph's buffers, not with the output's last reference."""
+    q, k, v, cu, dout = _inputs(cuda, [512] * 8, 32, 4, 64, seed=40)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    size = q.numel() * 2
+
+    def step():
+        out = ops.packed_attention(*leaves, cu)
+        torch.autograd.grad(out, leaves, dout)
+        return out
+
+    step()
+    out, held = _held(cuda, step)
+    assert held < 1.25 * size and out.grad_fn is not None
+    with pytest.raises(RuntimeError, match="a second time"):
+        torch.autograd.grad(out, leaves, dout)
+
+
+def test_saved_tensor_hooks_and_checkpointing(cuda):
+    """Hooks see every large tensor that the backward pass reads; offloaded or recomputed, the gradients are the same."""
+    from torch.utils.checkpoint import checkpoint
+
+    q, k, v, cu, dout = _inputs(cuda, [512] * 8, 32, 4, 64, seed=41)
+    want = _run(q, k, v, cu, dout)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    size = q.numel() * 2
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: seen.append(x) or x, lambda x: x):
+        ops.packed_attention(*leaves, cu)
+    assert sum(x.shape == q.shape for x in seen) == 3  # queries, output, what its rounding left
+    assert sum(x.shape == (32, 4096) and x.dtype == torch.float32 for x in seen) == 1
+    seen.clear()
+    recomputed, held = _held(cuda, lambda: checkpoint(ops.packed_attention, *leaves, cu, use_reentrant=False))
+    assert held < 1.25 * size
+    with torch.autograd.graph.save_on_cpu():
+        offloaded, held = _held(cuda, lambda: ops.packed_attention(*leaves, cu))
+    assert held < 1.25 * size
+    for out in (recomputed, offloaded):
+        assert torch.equal(out.detach(), want[0])
+        for got, ref in zip(torch.autograd.grad(out, leaves, dout), want[1:]):
+            assert torch.equal(got, ref)
+    assert ops.require().status(0) == 0
+
+
+def test_a_hook_that_returns_something_else_is_refused(cuda):
+    """Saved tensors that come back on another device, of another type or size reach no kernel."""
+    q, k, v, cu, dout = _inputs(cuda, [40], 2, 1, 64, seed=42)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    for wrong in (lambda x: x.cpu(), lambda x: x.to(torch.float64), lambda x: x.flatten()[1:]):
+        for i in range(3, 7):  # output, rest, log-sum-exps, plan
+            count = iter(range(100))
+            with torch.autograd.graph.saved_tensors_hooks(lambda x: (next(count), x),
+                                                          lambda s: wrong(s[1]) if s[0] == i else s[1]):
+                out = ops.packed_attention(*leaves, cu)
+            with pytest.raises(RuntimeError, match="saved"):
+                torch.autograd.grad(out, leaves, dout)
