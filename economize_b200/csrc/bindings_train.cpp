@@ -2,6 +2,7 @@
 // PyTorch's caching allocator, tensor maps, and the launches on the current stream.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/graph_task.h>
 
 #include <algorithm>
 #include <cmath>
@@ -34,6 +35,14 @@ Tensor rows_of(const Tensor& x) {
   if (ok) return x;
   Tensor y = x.contiguous();
   return reinterpret_cast<uintptr_t>(y.data_ptr()) % 16 == 0 ? y : y.clone();
+}
+
+// A tensor that the forward pass saved is what it was: saved-tensor hooks may return anything, and kernels read it by its
+// pointer.
+void check_saved(const Tensor& x, const Tensor& like, at::ScalarType type, at::IntArrayRef sizes, const char* what) {
+  TORCH_CHECK(x.defined() && x.is_cuda() && x.get_device() == like.get_device() && x.scalar_type() == type &&
+                  x.sizes() == sizes && x.is_contiguous() && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0,
+              "the saved ", what, " did not come back as it was saved (device, type, sizes, contiguous)");
 }
 
 // What a chunk of rows may hold of unnormalised probabilities (2 bytes each).
@@ -308,14 +317,6 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> packed_forward(Tensor q, Tensor k, Te
   return {out, rest, lse, plan};
 }
 
-// A tensor that the forward pass saved is what it was: saved-tensor hooks may return anything, and kernels read it by its
-// pointer.
-void check_saved(const Tensor& x, const Tensor& like, at::ScalarType type, at::IntArrayRef sizes, const char* what) {
-  TORCH_CHECK(x.defined() && x.is_cuda() && x.get_device() == like.get_device() && x.scalar_type() == type &&
-                  x.sizes() == sizes && x.is_contiguous() && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0,
-              "the saved ", what, " did not come back as it was saved (device, type, sizes, contiguous)");
-}
-
 // Gradients of q, k and v (those asked for; undefined otherwise) given the output's. plan, tiles: of the forward pass
 // over B sequences.
 std::tuple<Tensor, Tensor, Tensor> packed_backward(Tensor dout, Tensor q, Tensor k, Tensor v, const Tensor& out,
@@ -393,22 +394,23 @@ void once(const char* name) {
 }
 
 // Losses of the readout. A scalar loss computes its gradients in the forward pass, where the unnormalised probabilities
-// are at hand, and the backward pass scales them by the upstream gradient; per-row losses, whose upstream gradients are
-// not known by then, run the products again in the backward pass.
+// are at hand, saves them (and nothing else), and its backward pass scales them by the upstream gradient; per-row losses,
+// whose upstream gradients are not known by then, save the operands and run the products in the backward pass.
 struct ReadoutFunction : torch::autograd::Function<ReadoutFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& targets,
                         int64_t ignore_index, double logit_scale, int64_t reduction, int64_t chunk_rows) {
-    const bool now = reduction != ecz::kReduceNone;
-    auto r = readout(hidden, weight, targets, ignore_index, logit_scale, reduction, now && hidden.requires_grad(),
-                     now && weight.requires_grad(), c10::nullopt, chunk_rows);
-    ctx->save_for_backward({hidden, weight, targets});
-    ctx->saved_data["ignore"] = ignore_index;
-    ctx->saved_data["scale"] = logit_scale;
+    const bool per_row = reduction == ecz::kReduceNone;
+    auto r = readout(hidden, weight, targets, ignore_index, logit_scale, reduction, !per_row && hidden.requires_grad(),
+                     !per_row && weight.requires_grad(), c10::nullopt, chunk_rows);
     ctx->saved_data["reduction"] = reduction;
-    ctx->saved_data["chunk"] = chunk_rows;
-    if (std::get<1>(r)) ctx->saved_data["dx"] = *std::get<1>(r);
-    if (std::get<2>(r)) ctx->saved_data["dw"] = *std::get<2>(r);
-    ctx->saved_data["held"] = now;
+    if (per_row) {
+      ctx->save_for_backward({hidden, weight, targets});
+      ctx->saved_data["ignore"] = ignore_index;
+      ctx->saved_data["scale"] = logit_scale;
+      ctx->saved_data["chunk"] = chunk_rows;
+    } else {
+      ctx->save_for_backward({std::get<1>(r).value_or(Tensor()), std::get<2>(r).value_or(Tensor())});
+    }
     return std::get<0>(r);
   }
 
@@ -417,24 +419,24 @@ struct ReadoutFunction : torch::autograd::Function<ReadoutFunction> {
     auto& data = ctx->saved_data;
     const bool need_dx = ctx->needs_input_grad(0), need_dw = ctx->needs_input_grad(1);
     const int64_t reduction = data["reduction"].toInt();
+    const auto saved = ctx->get_saved_variables();
     variable_list out(7);
     Tensor g = grads[0].to(at::kFloat).contiguous();
-    const bool per_row = reduction == ecz::kReduceNone;
-    if (!per_row && data["held"].toBool()) {
-      // the buffers are given away: a second pass over a retained graph computes them again
-      if (need_dx) out[0] = data["dx"].toTensor();
-      if (need_dw) out[1] = data["dw"].toTensor();
-      data.erase("dx");
-      data.erase("dw");
-      data["held"] = false;
-    } else {
-      const auto saved = ctx->get_saved_variables();
+    if (reduction == ecz::kReduceNone) {
       auto r = readout(saved[0], saved[1], saved[2], data["ignore"].toInt(), data["scale"].toDouble(), reduction,
-                       need_dx, need_dw, per_row ? c10::optional<Tensor>(g) : c10::nullopt, data["chunk"].toInt());
+                       need_dx, need_dw, c10::optional<Tensor>(g), data["chunk"].toInt());
       if (need_dx) out[0] = *std::get<1>(r);
       if (need_dw) out[1] = *std::get<2>(r);
+      return out;
     }
-    if (!per_row) scale_both(out[0], out[1], g);
+    // scaled in place and given away; a graph that is kept for another pass keeps its own
+    const bool keep = torch::autograd::get_current_graph_task_keep_graph();
+    for (int i = 0; i < 2; ++i) {
+      if (!(i == 0 ? need_dx : need_dw)) continue;
+      check_saved(saved[i], g, at::kBFloat16, saved[i].sizes(), "gradient");
+      out[i] = keep ? saved[i].clone() : saved[i];
+    }
+    scale_both(out[0], out[1], g);
     return out;
   }
 };

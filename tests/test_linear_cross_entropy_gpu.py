@@ -340,3 +340,54 @@ def test_refusals(cuda):
         ops.linear_cross_entropy(x, w.cpu(), y)
     with pytest.raises(RuntimeError, match="multiple of 8"):
         ops.linear_cross_entropy(x[:, :60].contiguous(), w[:, :60].contiguous(), y)
+
+
+def test_saved_tensor_hooks_and_checkpointing(cuda):
+    """The gradients that a mean or sum computes in its forward pass are saved as any other tensor: hooks see them, and
+    what is offloaded or recomputed gives the same."""
+    from torch.utils.checkpoint import checkpoint
+
+    x, w, y = _inputs(cuda, 256, 512, 40000, 0.2, seed=16)
+    x.requires_grad_()
+    w.requires_grad_()
+    want = torch.autograd.grad(ops.linear_cross_entropy(x, w, y), (x, w))
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t.shape) or t, lambda t: t):
+        ops.linear_cross_entropy(x, w, y)
+    assert sorted(seen) == sorted([x.shape, w.shape])
+
+    def held(make):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated(cuda)
+        loss = make()
+        return loss, torch.cuda.memory_allocated(cuda) - before
+
+    size = w.numel() * 2
+    recomputed, kept = held(lambda: checkpoint(ops.linear_cross_entropy, x, w, y, use_reentrant=False))
+    assert kept < size / 4
+    with torch.autograd.graph.save_on_cpu():
+        offloaded, kept = held(lambda: ops.linear_cross_entropy(x, w, y))
+    assert kept < size / 4
+    for loss in (recomputed, offloaded):
+        for got, ref in zip(torch.autograd.grad(loss, (x, w)), want):
+            assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_kept_graph_gives_the_same_again(cuda, reduction):
+    """What a pass over a kept graph returns is the caller's: writing to it leaves the next pass alone. After a pass that
+    does not keep it the graph is spent."""
+    x, w, y = _inputs(cuda, 70, 128, 900, 0.2, seed=17)
+    x.requires_grad_()
+    w.requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, y, reduction=reduction).sum()
+    want = [g.clone() for g in torch.autograd.grad(loss, (x, w), retain_graph=True)]
+    for _ in range(2):
+        got = torch.autograd.grad(loss, (x, w), retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        for g in got:
+            g.fill_(3.0)
+    (dx,) = torch.autograd.grad(loss, (x,))  # dW not asked for
+    assert torch.equal(dx, want[0])
+    with pytest.raises(RuntimeError, match="a second time"):
+        torch.autograd.grad(loss, (x, w))
