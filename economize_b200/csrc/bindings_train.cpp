@@ -1,6 +1,7 @@
 // PyTorch bindings of the training operators (readout.cu, packed_attention.cu): argument checks, workspaces from
 // PyTorch's caching allocator, tensor maps, and the launches on the current stream.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/graph_task.h>
 
@@ -393,6 +394,13 @@ void once(const char* name) {
   TORCH_CHECK(!at::GradMode::is_enabled(), name, " cannot be differentiated twice");
 }
 
+// The kernels carry no tangents: refused, or a dual number's would be dropped without a word.
+template <class... Operands>
+void no_tangent(const char* name, const Operands&... x) {
+  TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !(x._fw_grad(0).defined() || ...), name,
+              " has no forward-mode derivative on CUDA");
+}
+
 // Losses of the readout. A scalar loss computes its gradients in the forward pass, where the unnormalised probabilities
 // are at hand, saves them (and nothing else), and its backward pass scales them by the upstream gradient; per-row losses,
 // whose upstream gradients are not known by then, save the operands and run the products in the backward pass.
@@ -443,6 +451,7 @@ struct ReadoutFunction : torch::autograd::Function<ReadoutFunction> {
 
 Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t ignore_index,
                             double logit_scale, int64_t reduction, int64_t chunk_rows) {
+  no_tangent("linear_cross_entropy", hidden, weight);
   if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad()))
     return ReadoutFunction::apply(hidden, weight, targets, ignore_index, logit_scale, reduction, chunk_rows);
   return std::get<0>(
@@ -484,6 +493,7 @@ struct PackedFunction : torch::autograd::Function<PackedFunction> {
 
 Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, double scale,
                         int64_t tiles) {
+  no_tangent("packed_attention", q, k, v);
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
     return PackedFunction::apply(q, k, v, cu, scale, tiles);
   return std::get<0>(packed_forward(q, k, v, cu, scale, false, tiles));

@@ -2,7 +2,8 @@
 
 On CUDA both directions are the hand-written kernels of ``csrc/readout.cu``, ``csrc/packed_attention.cu`` and
 ``csrc/packed_attention_bwd.cu`` (autograd functions in ``csrc/bindings_train.cpp``); CPU tensors take the formulas of
-:mod:`.reference` (autograd differentiates them). There is no third path.
+:mod:`.reference`, which autograd differentiates in either mode and any number of times. The kernels have the first
+reverse-mode derivative: dual tensors and ``create_graph=True`` are refused on CUDA. There is no third path.
 """
 
 from __future__ import annotations

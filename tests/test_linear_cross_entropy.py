@@ -63,3 +63,12 @@ def test_leading_dimensions_and_refusals():
         ops.linear_cross_entropy(x, w[:, :3], y)
     with pytest.raises(ValueError, match="do not match"):
         ops.linear_cross_entropy(x, w, y[:3])
+
+
+def test_forward_mode_and_second_derivatives():
+    x, w, y = _inputs(rows=9, hidden=4, vocab=5, seed=4)
+    x.requires_grad_()
+    w.requires_grad_()
+    loss = lambda a, b: ops.linear_cross_entropy(a, b, y)  # noqa: E731
+    assert torch.autograd.gradcheck(loss, (x, w), check_forward_ad=True)
+    assert torch.autograd.gradgradcheck(loss, (x, w))

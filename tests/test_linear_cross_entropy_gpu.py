@@ -391,3 +391,21 @@ def test_a_kept_graph_gives_the_same_again(cuda, reduction):
     assert torch.equal(dx, want[0])
     with pytest.raises(RuntimeError, match="a second time"):
         torch.autograd.grad(loss, (x, w))
+
+
+def test_forward_mode_and_second_derivatives_are_refused(cuda):
+    """No tangent is dropped, no second derivative left out, without a word."""
+    import torch.autograd.forward_ad as fwd
+
+    x, w, y = _inputs(cuda, 10, 64, 50, seed=18)
+    with fwd.dual_level():
+        for i in range(2):
+            for requires_grad in (False, True):
+                args = [x.detach().clone().requires_grad_(requires_grad), w]
+                args[i] = fwd.make_dual(args[i], torch.ones_like(args[i]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    ops.linear_cross_entropy(*args, y)
+    assert torch.isfinite(ops.linear_cross_entropy(x, w, y))
+    x.requires_grad_()
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(ops.linear_cross_entropy(x, w, y), (x,), create_graph=True)

@@ -45,3 +45,10 @@ def test_refusals():
         ops.packed_attention(q, k, v, torch.tensor([0, 3, 2]).int())
     with pytest.raises(ValueError, match="offsets"):
         ops.packed_attention(q, k, v, torch.tensor([0, 9]).int())
+
+
+def test_forward_mode_and_second_derivatives():
+    q, k, v, cu = _inputs([3, 0, 2], heads=2, kv_heads=1, dim=3, pad=1)
+    args = [x.requires_grad_() for x in (q, k, v)]
+    assert torch.autograd.gradcheck(lambda *x: ops.packed_attention(*x, cu), args, check_forward_ad=True)
+    assert torch.autograd.gradgradcheck(lambda *x: ops.packed_attention(*x, cu), args)

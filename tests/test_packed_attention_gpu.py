@@ -456,3 +456,20 @@ def test_a_hook_that_returns_something_else_is_refused(cuda):
                 out = ops.packed_attention(*leaves, cu)
             with pytest.raises(RuntimeError, match="saved"):
                 torch.autograd.grad(out, leaves, dout)
+
+
+def test_forward_mode_and_second_derivatives_are_refused(cuda):
+    """No tangent is dropped, no second derivative left out, without a word."""
+    import torch.autograd.forward_ad as fwd
+
+    q, k, v, cu, dout = _inputs(cuda, [30], 4, 2, 64, seed=43)
+    with fwd.dual_level():
+        for i in range(3):
+            for requires_grad in (False, True):
+                args = [q.detach().clone().requires_grad_(requires_grad), k, v]
+                args[i] = fwd.make_dual(args[i], torch.ones_like(args[i]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    ops.packed_attention(*args, cu)
+    q.requires_grad_()
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(ops.packed_attention(q, k, v, cu), (q,), dout, create_graph=True)
