@@ -92,6 +92,8 @@ class CausalLM(nn.Module):
     #: class-level defaults, so views built without ``__init__`` (``techniques/_self_draft.py:layer_view``) have them
     placement = None
     _rope_local = None
+    #: tables that larger ones replaced: captured decode graphs read them by address for as long as they are replayed
+    _outgrown: tuple[tuple[torch.Tensor, torch.Tensor], ...] = ()
 
     def __init__(self, config: ModelConfig, dtype: torch.dtype = torch.bfloat16,
                  device: torch.device | str | None = None) -> None:
@@ -143,11 +145,12 @@ class CausalLM(nn.Module):
     def rope_tables(self, length: int | None = None, local: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
         """``cos, sin [P, D/2]`` fp32 for positions ``0..P-1`` (computed once per device, like HF: the angle is the
         fp32 product of the position and the inverse frequency). ``local``: the tables of the sliding-window layers
-        when their rotary parameters differ (Gemma-3)."""
+        when their rotary parameters differ (Gemma-3). Smaller tables that were handed out before stay allocated."""
         need = max(length or 0, self.config.max_position_embeddings)
         local = local and self.config.local_rope is not None
         cached = self._rope_local if local else self._rope
         if cached is None or cached[0].shape[0] < need or cached[0].device != self.device:
+            self._outgrow(cached)
             inv = rope_inv_freq(self.config, local=local).to(self.device)
             pos = torch.arange(need, device=self.device, dtype=torch.float32)
             angles = pos[:, None] * inv[None, :]
@@ -160,6 +163,11 @@ class CausalLM(nn.Module):
             else:
                 self._rope = cached
         return cached
+
+    def _outgrow(self, tables: tuple[torch.Tensor, torch.Tensor] | None) -> None:
+        """Keep ``tables``, which are about to be replaced (those of another device go: nothing replays there)."""
+        kept = (*self._outgrown, *(() if tables is None else (tables,)))
+        self._outgrown = tuple(t for t in kept if t[0].device == self.device)
 
     def _layer_rope(self, index: int, cos: torch.Tensor, sin: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """The rotary tables layer ``index`` uses: none (NoPE), the sliding layers' own, or the model's."""
@@ -216,6 +224,7 @@ class CausalLM(nn.Module):
         """cos = 1, sin = 0 tables of ``cos``'s shape: rotary embedding that leaves q and k unchanged (NoPE)."""
         cached = getattr(self, "_nope_tables", None)
         if cached is None or cached[0].shape != cos.shape or cached[0].device != cos.device:
+            self._outgrow(cached)
             cached = (torch.ones_like(cos), torch.zeros_like(cos))
             self._nope_tables = cached
         return cached

@@ -33,6 +33,8 @@ class DraftLayer(nn.Module):
         self.w_gate_up = nn.Parameter(torch.empty(2 * intermediate, hidden, **kw))
         self.w_down = nn.Parameter(torch.empty(hidden, intermediate, **kw))
         self._rope: tuple[torch.Tensor, torch.Tensor] | None = None
+        #: tables that larger ones replaced: captured decode graphs read them by address
+        self._outgrown: tuple[tuple[torch.Tensor, torch.Tensor], ...] = ()
         self._rope_config: ModelConfig | None = None
 
     def set_rope(self, config: ModelConfig) -> None:
@@ -41,10 +43,12 @@ class DraftLayer(nn.Module):
 
     def rope(self, length: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
         """``cos, sin`` tables with a row for every position below ``length`` (at least the configuration's
-        ``max_position_embeddings``)."""
+        ``max_position_embeddings``). Smaller tables that were handed out before stay allocated."""
         dev = self.wqkv.device
         need = max(length, self._rope_config.max_position_embeddings)
         if self._rope is None or self._rope[0].device != dev or self._rope[0].shape[0] < need:
+            kept = (*self._outgrown, *(() if self._rope is None else (self._rope,)))
+            self._outgrown = tuple(t for t in kept if t[0].device == dev)
             inv = rope_inv_freq(self._rope_config).to(dev)
             pos = torch.arange(need, device=dev, dtype=torch.float32)
             ang = pos[:, None] * inv[None]
