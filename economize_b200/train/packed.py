@@ -29,15 +29,18 @@ IGNORE = -100
 class PackedBatch:
     """Documents one after another: ``tokens [T]``; document ``i`` is tokens ``cu_seqlens[i]`` to ``cu_seqlens[i + 1]``
     (int32 ``[B + 1]``), what follows the last one is padding. ``positions [T]`` count within a document; ``targets
-    [T]`` are each position's next token in its document, ``-100`` at a document's last token and in the padding."""
+    [T]`` are each position's next token in its document, ``-100`` at a document's last token and in the padding.
+    ``longest``: the longest document's tokens (known on the host; None: read from ``positions``)."""
 
     tokens: torch.Tensor
     cu_seqlens: torch.Tensor
     positions: torch.Tensor
     targets: torch.Tensor
+    longest: int | None = None
 
     def to(self, device) -> PackedBatch:
-        return PackedBatch(*(t.to(device) for t in (self.tokens, self.cu_seqlens, self.positions, self.targets)))
+        return PackedBatch(*(t.to(device) for t in (self.tokens, self.cu_seqlens, self.positions, self.targets)),
+                           self.longest)
 
 
 def pack(documents: Sequence[torch.Tensor], length: int | None = None) -> PackedBatch:
@@ -54,7 +57,7 @@ def pack(documents: Sequence[torch.Tensor], length: int | None = None) -> Packed
     targets = torch.cat([tokens[1:], tokens[:1]])
     targets[(edges[1:] - 1)[torch.tensor(lens, dtype=torch.long) > 0].to(device)] = IGNORE
     targets[total:] = IGNORE
-    return PackedBatch(tokens, edges.to(torch.int32).to(device), positions.to(device), targets)
+    return PackedBatch(tokens, edges.to(torch.int32).to(device), positions.to(device), targets, max(lens, default=0))
 
 
 class PackedSource:
@@ -106,9 +109,11 @@ class PackedRecoveryCE(RecoveryCE):
         target = self.model.model
         c = target.config
         head = target.head_weight.detach()
+        # positions count within documents: a row of many does not need the tables of a sequence as long
+        longest = int(batch.positions.max()) + 1 if batch.longest is None else batch.longest
         batch = batch.to(head.device)
         dtype = head.dtype if head.is_cuda else torch.float32
-        cos, sin = target.rope_tables(batch.tokens.numel())
+        cos, sin = target.rope_tables(longest)
         cos, sin = cos[batch.positions], sin[batch.positions]
         h = target.embed_tokens(batch.tokens[None]).to(dtype)
         for layer in target.layers:

@@ -100,6 +100,22 @@ def test_fit_trains_the_adapters():
     assert float(after.detach()) < float(before.detach())
 
 
+def test_rows_longer_than_the_models_positions():
+    """The rotary tables cover the longest document, not the row: they are replaced only where a document needs it."""
+    em = _pruned(tiny_model(max_position_embeddings=128))
+    tables = em.model.rope_tables()
+    assert tables[0].shape[0] == 128
+    batch = pack(_documents([90, 1, 60, 5]), length=180)
+    obj = OBJECTIVES.get("packed_recovery_ce")(em)
+    loss, _ = obj.loss(batch)
+    assert em.model.rope_tables()[0] is tables[0]
+    assert batch.longest == 90 and batch.to("cpu").longest == 90 and pack([]).longest == 0
+    batch.longest = None
+    assert torch.equal(obj.loss(batch)[0], loss)
+    obj.loss(pack(_documents([130])))
+    assert em.model.rope_tables()[0].shape[0] == 130
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("head_dim,heads,kv_heads", [(128, 2, 1), (64, 6, 2)])
 def test_objective_on_the_kernels(cuda, head_dim, heads, kv_heads):
