@@ -84,14 +84,23 @@ def fit(model, data: Any, objective: Objective | str | None = None, config: Trai
     params = obj.parameters()
     if not params:
         raise ConfigError("the objective has no trainable parameters")
-    modules = {id(p): p for p in params}
     orig_dtype = params[0].dtype
     if dist_on:  # data parallelism: every rank starts from rank 0's parameters (as DDP does)
         with torch.no_grad():
             for p in params:
                 torch.distributed.broadcast(p.data, src=0)
-    for p in params:  # fp32 master weights while training
-        p.data = p.data.float()
+    try:
+        for p in params:  # fp32 master weights while training
+            p.data = p.data.float()
+        return _train(obj, source, cfg, ckpt, params)
+    finally:  # however training ends: decoders and graphs that were captured hold the storage the parameters had before
+        _restore_dtype(params, orig_dtype)
+        model.refresh()
+
+
+def _train(obj: Objective, source: Any, cfg: TrainConfig, ckpt: RunCheckpointer | None,
+           params: list[torch.nn.Parameter]) -> TrainResult:
+    """The steps of :func:`fit` over fp32 ``params``."""
     d = obj.defaults
     opt_cls = torch.optim.AdamW
     if cfg.offload_optimizer:
@@ -111,7 +120,6 @@ def fit(model, data: Any, objective: Objective | str | None = None, config: Trai
             if done is not None:
                 weights, state = RunCheckpointer.load(done)
                 _load(params, names, weights)
-                _restore_dtype(params, orig_dtype)
                 return TrainResult(steps=state["step"])
             resume_from = ckpt.latest()
         else:
@@ -138,7 +146,6 @@ def fit(model, data: Any, objective: Objective | str | None = None, config: Trai
                 loss, metrics = obj.loss(batch)
             if not torch.isfinite(loss):
                 if cfg.nonfinite == "raise":
-                    _restore_dtype(params, orig_dtype)
                     raise NonFiniteLossError(f"non-finite loss {float(loss)} at step {step}")
                 if cfg.nonfinite == "skip":
                     bad = True
@@ -174,9 +181,6 @@ def fit(model, data: Any, objective: Objective | str | None = None, config: Trai
         ckpt.save(result.steps, _state(params, names), opt, sched,
                   source.state() if hasattr(source, "state") else {}, final=True,
                   result={"step": result.steps, "final": result.final})
-    _restore_dtype(params, orig_dtype)
-    model.refresh()
-    del modules
     return result
 
 

@@ -208,3 +208,33 @@ def test_distill_from_a_larger_teacher():
     assert losses[-1] < losses[0]
     with pytest.raises(eco.ConfigError, match="smaller"):
         larger_teacher(big, vocab_size=4096)(tokens)
+
+
+@pytest.mark.parametrize("ends", ["a non-finite loss", "an interrupt", "a finished run"])
+def test_fit_drops_decoders_however_it_ends(ends, tmp_path):
+    """The parameters' storage has changed by then: captured decode graphs must not be replayed."""
+    from economize_b200.errors import NonFiniteLossError
+    from economize_b200.train.objective import OBJECTIVES
+
+    em = eco.apply(tiny_model().to(torch.bfloat16), MedusaConfig(num_heads=2))
+    data = torch.randint(0, 1024, (4, 16), generator=torch.Generator().manual_seed(0))
+    fit = eco.train.fit
+    obj = OBJECTIVES.get("medusa_ce")(em)
+    settings = dict(steps=2, batch_size=2, log_every=100, output_dir=tmp_path, resume=True)
+    if ends == "a finished run":
+        fit(em, data, obj, **settings)
+    em.decoder()
+    assert em._decoders
+    if ends == "a finished run":
+        assert fit(em, data, obj, **settings).history == []
+    else:
+        def loss(tokens):
+            if ends == "an interrupt":
+                raise KeyboardInterrupt
+            return torch.tensor(float("nan"), requires_grad=True), {}
+
+        obj.loss = loss
+        with pytest.raises(NonFiniteLossError if ends == "a non-finite loss" else KeyboardInterrupt):
+            fit(em, data, obj, **settings)
+    assert not em._decoders
+    assert all(p.dtype == torch.bfloat16 and p.grad is None for p in obj.parameters())
