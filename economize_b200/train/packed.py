@@ -62,33 +62,51 @@ def pack(documents: Sequence[torch.Tensor], length: int | None = None) -> Packed
 
 class PackedSource:
     """Packed rows of random documents, reproducible from ``seed`` and resumable. Documents are drawn until the row of
-    ``tokens_per_batch`` is full; the last one is cut to fit."""
+    ``tokens_per_batch`` is full; the last one is cut to fit. Every data-parallel rank draws rows of its own: ``rank`` is
+    the process's in the default group (0 without one); equal ranks draw equal rows, for a stream that is sharded
+    otherwise (:class:`~economize_b200.train.data.ShardedSource`)."""
 
-    def __init__(self, documents: Sequence[torch.Tensor], tokens_per_batch: int, seed: int = 0) -> None:
+    def __init__(self, documents: Sequence[torch.Tensor], tokens_per_batch: int, seed: int = 0,
+                 rank: int | None = None) -> None:
         self.documents = [d.reshape(-1) for d in documents if d.numel() > 0]
         if not self.documents:
             raise ConfigError("PackedSource needs at least one document that is not empty")
         if tokens_per_batch < 1:
             raise ConfigError(f"tokens_per_batch must be positive, got {tokens_per_batch}")
         self.tokens_per_batch = tokens_per_batch
-        self.gen = torch.Generator().manual_seed(seed)
+        if rank is None:
+            on = torch.distributed.is_available() and torch.distributed.is_initialized()
+            rank = torch.distributed.get_rank() if on else 0
+        self.rank = rank
+        self.seed = seed + 1000003 * rank  # as fit seeds the ranks' batches of a token tensor
+        self.gen = torch.Generator().manual_seed(self.seed)
         self.drawn = 0
 
-    def next(self) -> PackedBatch:
+    def _draw(self) -> list[torch.Tensor]:
         picked, left = [], self.tokens_per_batch
         while left > 0:
             doc = self.documents[int(torch.randint(0, len(self.documents), (1,), generator=self.gen))]
             picked.append(doc[:left])
             left -= picked[-1].numel()
         self.drawn += 1
-        return pack(picked)
+        return picked
+
+    def next(self) -> PackedBatch:
+        return pack(self._draw())
 
     def state(self) -> dict:
-        return {"drawn": self.drawn, "gen": self.gen.get_state()}
+        return {"drawn": self.drawn, "gen": self.gen.get_state(), "rank": self.rank}
 
     def restore(self, state: dict) -> None:
-        self.drawn = state["drawn"]
-        self.gen.set_state(state["gen"])
+        """Continue behind ``state``; a checkpoint holds one rank's, from which the others draw as many rows again."""
+        if state.get("rank", self.rank) == self.rank:
+            self.drawn = state["drawn"]
+            self.gen.set_state(state["gen"])
+            return
+        self.drawn = 0
+        self.gen.manual_seed(self.seed)
+        while self.drawn < state["drawn"]:
+            self._draw()
 
 
 @OBJECTIVES.register("packed_recovery_ce")

@@ -74,6 +74,56 @@ def test_source_fills_rows_and_resumes():
         PackedSource(_documents([3]), 0)
 
 
+def _rows_of_rank(rank, port, queue):
+    import datetime
+
+    torch.distributed.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{port}", rank=rank, world_size=2,
+                                         timeout=datetime.timedelta(seconds=60))
+    try:
+        src = PackedSource(_documents([5, 9, 30, 2]), 64, seed=1)
+        queue.put((rank, [src.next().tokens.tolist() for _ in range(3)]))
+        torch.distributed.barrier()
+    finally:
+        torch.distributed.destroy_process_group()
+
+
+@pytest.mark.slow
+def test_ranks_draw_rows_of_their_own():
+    import socket
+
+    import torch.multiprocessing as mp
+
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    queue = ctx.Queue()
+    procs = [ctx.Process(target=_rows_of_rank, args=(r, port, queue)) for r in range(2)]
+    for p in procs:
+        p.start()
+    rows = dict(queue.get(timeout=120) for _ in procs)
+    for p in procs:
+        p.join(60)
+    assert all(a != b for a, b in zip(rows[0], rows[1]))
+    alone = PackedSource(_documents([5, 9, 30, 2]), 64, seed=1)
+    assert [alone.next().tokens.tolist() for _ in range(3)] == rows[0]
+
+
+def test_ranks_resume_from_one_checkpoint():
+    """A run's checkpoint holds the position of one rank; another continues with the rows that it would have drawn."""
+    docs = _documents([5, 9, 30, 2])
+    a, b = (PackedSource(docs, 64, seed=1, rank=r) for r in (0, 1))
+    for _ in range(3):
+        a.next(), b.next()
+    state = a.state()
+    want = [s.next().tokens for s in (a, b)]
+    for rank in (0, 1):
+        src = PackedSource(docs, 64, seed=1, rank=rank)
+        src.next()
+        src.restore(state)
+        assert src.drawn == 3 and torch.equal(src.next().tokens, want[rank])
+
+
 def test_objective_is_the_mean_over_documents_by_themselves():
     em = _pruned()
     docs = _documents([17, 1, 30, 5])
