@@ -457,7 +457,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     rows = (targets != ignore_index).nonzero()[:, 0]
     wide = torch.promote_types(hidden.dtype, torch.float32)
     logits = F.linear(hidden[rows].to(wide), weight.to(wide)) * logit_scale
-    nll = F.cross_entropy(logits, targets[rows], reduction="none")
+    # no row is ignored any more: a target outside the vocabulary raises, whatever ignore_index is
+    nll = F.cross_entropy(logits, targets[rows], reduction="none", ignore_index=ignore_index)
     if reduction == "none":
         return torch.zeros(targets.shape, dtype=wide, device=hidden.device).index_copy(0, rows, nll)
     return nll.sum() if reduction == "sum" else nll.sum() / max(1, rows.numel())

@@ -36,8 +36,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
         hidden: States ``[..., H]`` (bf16 on CUDA, ``H`` a multiple of 8; cast under bf16 autocast).
         weight: The vocabulary rows ``[V, H]``.
         targets: Target ids ``[...]`` (int64). Rows whose target is ``ignore_index`` cost nothing, add nothing to the
-            loss and get zero gradients, whatever their states hold (NaN included). A target outside ``[0, V)`` is
-            ignored on CUDA and reported in the device status word.
+            loss and get zero gradients, whatever their states hold (NaN included). Any other target outside ``[0, V)``
+            is ignored on CUDA and reported in the device status word, and raises on the CPU.
         reduction: ``"mean"`` over the rows with a target (0 when there is none), ``"sum"``, or ``"none"``:
             per-row losses ``[...]`` (0 for ignored rows), whose backward pass computes the logits again.
         chunk_rows: Rows processed at a time (0: as many as 1 GiB of 16-bit probabilities hold, more where a trained

@@ -72,3 +72,19 @@ def test_forward_mode_and_second_derivatives():
     loss = lambda a, b: ops.linear_cross_entropy(a, b, y)  # noqa: E731
     assert torch.autograd.gradcheck(loss, (x, w), check_forward_ad=True)
     assert torch.autograd.gradgradcheck(loss, (x, w))
+
+
+@pytest.mark.parametrize("ignore", [-1, 3])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_only_ignore_index_is_ignored(ignore, reduction):
+    """Any index may be the ignored one; another target outside the vocabulary is an error, -100 included."""
+    x, w, y = _inputs(rows=12, seed=5)
+    y[2] = y[7] = ignore
+    got = ops.linear_cross_entropy(x, w, y, reduction=reduction, ignore_index=ignore)
+    want = F.cross_entropy(x @ w.t(), y, reduction=reduction, ignore_index=ignore)
+    torch.testing.assert_close(got, want, rtol=1e-12, atol=1e-12)
+    for target in (-100, 17):
+        bad = y.clone()
+        bad[4] = target
+        with pytest.raises(IndexError, match="out of bounds"):
+            ops.linear_cross_entropy(x, w, bad, reduction=reduction, ignore_index=ignore)
