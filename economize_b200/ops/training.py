@@ -49,6 +49,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
         raise ValueError(f"hidden {tuple(hidden.shape)} and weight {tuple(weight.shape)} do not match")
     if targets.shape != hidden.shape[:-1]:
         raise ValueError(f"targets {tuple(targets.shape)} do not match hidden {tuple(hidden.shape)}")
+    if chunk_rows < 0:
+        raise ValueError(f"chunk_rows must be 0 or more, got {chunk_rows}")
     hidden, weight = _autocast(hidden, weight)
     shape = targets.shape
     if hidden.dim() != 2:

@@ -88,3 +88,9 @@ def test_only_ignore_index_is_ignored(ignore, reduction):
         bad[4] = target
         with pytest.raises(IndexError, match="out of bounds"):
             ops.linear_cross_entropy(x, w, bad, reduction=reduction, ignore_index=ignore)
+
+
+def test_refuses_a_negative_chunk():
+    x, w, y = _inputs()
+    with pytest.raises(ValueError, match="chunk_rows"):
+        ops.linear_cross_entropy(x, w, y, chunk_rows=-64)
