@@ -474,6 +474,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
                          f"{tuple(k.shape)} and {tuple(v.shape)}")
     if cu_seqlens.dim() != 1 or cu_seqlens.dtype != torch.int32:
         raise ValueError("packed_attention: cu_seqlens must be int32 [B + 1]")
+    if not 0 < scale < float("inf"):
+        raise ValueError(f"packed_attention: the scale must be positive (got {scale})")
     group = q.shape[1] // k.shape[1]
     wide = torch.promote_types(q.dtype, torch.float32)
     out = torch.zeros_like(q)

@@ -52,3 +52,11 @@ def test_forward_mode_and_second_derivatives():
     args = [x.requires_grad_() for x in (q, k, v)]
     assert torch.autograd.gradcheck(lambda *x: ops.packed_attention(*x, cu), args, check_forward_ad=True)
     assert torch.autograd.gradgradcheck(lambda *x: ops.packed_attention(*x, cu), args)
+
+
+@pytest.mark.parametrize("scale", [0.0, -1.0, float("inf"), float("nan")])
+def test_refuses_a_scale_that_is_not_positive(scale):
+    """As the kernels do."""
+    q, k, v, cu = _inputs([4])
+    with pytest.raises(ValueError, match="scale"):
+        ops.packed_attention(q, k, v, cu, scale)
