@@ -409,3 +409,165 @@ def test_forward_mode_and_second_derivatives_are_refused(cuda):
     x.requires_grad_()
     with pytest.raises(RuntimeError, match="twice"):
         torch.autograd.grad(ops.linear_cross_entropy(x, w, y), (x,), create_graph=True)
+
+
+def _rowwise(x, w, y, scale, g_rows, rows=600):
+    """:func:`_oracle` over many rows, `rows` at a time."""
+    parts = [_oracle(x[i:i + rows], w, y[i:i + rows], scale, g_rows[i:i + rows]) for i in range(0, len(y), rows)]
+    o = {k: torch.cat([p[k] for p in parts]) for k in ("nll", "nll_err", "dx", "dx_err", "keep")}
+    o["dw"] = sum(p["dw"] for p in parts)
+    # the output is rounded once, not once for every part
+    o["dw_err"] = sum(p["dw_err"] - p["dw"].abs() * 2.0 ** -8 for p in parts) + o["dw"].abs() * 2.0 ** -8
+    return o
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_rows_planned_by_a_kernel_of_their_own(cuda, reduction):
+    """More rows than the gather kernel counts itself, and dW of few tiles, split along the rows."""
+    x, w, y = _inputs(cuda, 2500, 256, 1100, 0.3, seed=19)
+    x.requires_grad_()
+    w.requires_grad_()
+    count = int((y != -100).sum())
+    up = torch.linspace(-1.0, 2.0, 2500, device=cuda) if reduction == "none" else torch.tensor(1.0, device=cuda)
+    loss = ops.linear_cross_entropy(x, w, y, reduction=reduction)
+    dx, dw = torch.autograd.grad(loss, (x, w), up)
+    o = _oracle(x.detach(), w.detach(), y, 1.0, up if reduction == "none" else up.expand(2500) / count)
+    if reduction == "none":
+        _within(loss, o["nll"], o["nll_err"], "losses")
+    else:
+        total = o["nll"].sum() / count
+        _within(loss, total, o["nll_err"][o["keep"]].sum() / count + total * 2.0 ** -20, "loss")
+    _within(dx, o["dx"], o["dx_err"], "dx")
+    _within(dw, o["dw"], o["dw_err"], "dw")
+    assert ops.require().status(0) == 0
+
+
+def _whole_and_splits(m, n, k, pairs):
+    """Tiles of a product that are computed in one piece, and into how many the rest are split along K."""
+    tiles, blocks = -(-m // 256) * -(-n // 256), -(-k // 64)
+    rest = tiles % pairs
+    splits = max(1, min(pairs // rest, blocks // 8)) if rest and (rest == tiles or blocks >= 64) else 1
+    return (tiles - rest if splits > 1 else tiles), splits
+
+
+def test_split_tiles_behind_whole_rounds(cuda):
+    """Products of more tiles than CTA pairs whose last round is split along K: dX over the vocabulary, dW over the rows
+    that the device counts."""
+    rows, hidden, vocab = 5000, 1032, 5000
+    x, w, y = _inputs(cuda, rows, hidden, vocab, 0.1, seed=20)
+    count = int((y != -100).sum())
+    pairs = torch.cuda.get_device_properties(cuda).multi_processor_count // 2
+    if pairs == 74:
+        for m, n, k in ((count, hidden, vocab), (vocab, hidden, count)):
+            whole, splits = _whole_and_splits(m, n, k, pairs)
+            assert whole == pairs and splits > 1
+    x.requires_grad_()
+    w.requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, y)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    o = _rowwise(x.detach(), w.detach(), y, 1.0, torch.full((rows,), 1.0 / count, device=cuda), rows=1000)
+    total = o["nll"].sum() / count
+    _within(loss, total, o["nll_err"][o["keep"]].sum() / count + total * 2.0 ** -20, "loss")
+    _within(dx, o["dx"], o["dx_err"], "dx")
+    _within(dw, o["dw"], o["dw_err"], "dw")
+    assert ops.require().status(0) == 0
+
+
+@pytest.mark.parametrize("masked", [0.02, 0.2])
+def test_chunks_of_the_default_size(cuda, masked):
+    """More than 1 GiB of probabilities: 3840 rows to a chunk here, the second one with rows or left with none."""
+    rows, vocab = 4200, 131100
+    x, w, y = _inputs(cuda, rows, 72, vocab, masked, seed=21)
+    count = int((y != -100).sum())
+    assert (count > 3840) == (masked < 0.1)
+    x.requires_grad_()
+    w.requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, y, reduction="sum")
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    o = _rowwise(x.detach(), w.detach(), y, 1.0, torch.ones(rows, device=cuda))
+    total = o["nll"].sum()
+    _within(loss, total, o["nll_err"][o["keep"]].sum() + total * 2.0 ** -20, "loss")
+    _within(dx, o["dx"], o["dx_err"], "dx")
+    _within(dw, o["dw"], o["dw_err"], "dw")
+    assert ops.require().status(0) == 0
+
+
+def test_losses_in_chunks_of_the_default_size(cuda):
+    """Losses alone keep 8 bytes for 128 logits: more than 1 GiB of them."""
+    rows, vocab = 140000, 131100
+    x, w, y = _inputs(cuda, rows, 64, vocab, 0.02, seed=22)
+    losses = ops.linear_cross_entropy(x, w, y, reduction="none")
+    keep, wd = y != -100, w.double()
+    for i in range(0, rows, 2000):
+        s = slice(i, i + 2000)
+        xd, at = x[s].double(), torch.where(keep[s], y[s], 0)
+        z = xd @ wd.t()
+        want = torch.where(keep[s], torch.logsumexp(z, -1) - z.gather(1, at[:, None])[:, 0], 0.0)
+        # the sum of magnitudes of a logit's products by the norms of its factors
+        eps = xd.norm(dim=-1) * wd.norm(dim=-1).max() * 64 * 2.0 ** -23 + z.abs().amax(-1) * 2.0 ** -22
+        _within(losses[s], want, 2.5 * eps + want.abs() * 2.0 ** -20 + 2.0 ** -21, "losses")
+    assert ops.require().status(0) == 0
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_one_gradient_alone(cuda, reduction):
+    """The gradient of the states under a frozen head, and of a head under frozen states, as of both together."""
+    x, w, y = _inputs(cuda, 300, 136, 5000, 0.2, seed=23)
+    up = torch.linspace(-1.0, 2.0, 300, device=cuda) if reduction == "none" else torch.tensor(1.0, device=cuda)
+
+    def grads(*which):
+        args = [x.detach(), w.detach()]
+        for i in which:
+            args[i].requires_grad_()
+        loss = ops.linear_cross_entropy(*args, y, reduction=reduction)
+        return torch.autograd.grad(loss, [args[i] for i in which], up)
+
+    both = grads(0, 1)
+    count = int((y != -100).sum())
+    o = _oracle(x, w, y, 1.0, up if reduction == "none" else up.expand(300) / (count if reduction == "mean" else 1))
+    for i, name in enumerate(("dx", "dw")):
+        (alone,) = grads(i)
+        _within(alone, o[name], o[name + "_err"], name)
+        assert torch.equal(alone, both[i])
+
+
+def test_gradients_of_infinite_logits(cuda):
+    """Vocabulary rows of minus infinity have probability zero: their gradient is zero, the others' that of the rest of
+    the vocabulary. The states' gradient is NaN: the product multiplies the zeros with the infinite rows, as the plain
+    formula's does."""
+    x, w, y = _inputs(cuda, 33, 64, 400, seed=7)
+    x = x.abs()
+    y = torch.where((y >= 5) & (y < 300), 0, y)
+    keep = torch.cat([torch.arange(5), torch.arange(300, 400)]).to(cuda)
+    g = torch.linspace(-1.0, 2.0, 33, device=cuda)
+    o = _oracle(x, w[keep], torch.where(y < 5, y, y - 295), 1.0, g)
+    w[5:300] = float("-inf")
+    x.requires_grad_()
+    w.requires_grad_()
+    dx, dw = torch.autograd.grad(ops.linear_cross_entropy(x, w, y, reduction="none"), (x, w), g)
+    assert (dw[5:300] == 0).all() and torch.isnan(dx).all()
+    _within(dw[keep], o["dw"], o["dw_err"], "dw")
+
+
+def test_gradients_of_large_logits(cuda):
+    x, w, y = _inputs(cuda, 60, 256, 900, seed=8)
+    x, w = (x * 40).requires_grad_(), (w * 40).requires_grad_()
+    dx, dw = torch.autograd.grad(ops.linear_cross_entropy(x, w, y), (x, w))
+    o = _oracle(x.detach(), w.detach(), y, 1.0, torch.full((60,), 1 / 60, device=cuda))
+    _within(dx, o["dx"], o["dx_err"], "dx")
+    _within(dw, o["dw"], o["dw_err"], "dw")
+
+
+@pytest.mark.parametrize("upstream", [1 / 3, -0.7, 4.0])
+def test_upstream_gradients(cuda, upstream):
+    """The gradients of a mean are rounded before the upstream gradient is known: their product with it is rounded once
+    more (a power of two leaves them as they are)."""
+    x, w, y = _inputs(cuda, 90, 264, 1300, 0.2, seed=24)
+    x.requires_grad_()
+    w.requires_grad_()
+    dx, dw = torch.autograd.grad(ops.linear_cross_entropy(x, w, y) * upstream, (x, w))
+    count = int((y != -100).sum())
+    o = _oracle(x.detach(), w.detach(), y, 1.0, torch.full((90,), upstream / count, device=cuda))
+    again = 0.0 if upstream == 4.0 else 2.0 ** -8 * (1 + 2.0 ** -7)
+    _within(dx, o["dx"], o["dx_err"] + again * (o["dx"].abs() + o["dx_err"]), "dx")
+    _within(dw, o["dw"], o["dw_err"] + again * (o["dw"].abs() + o["dw_err"]), "dw")

@@ -473,3 +473,16 @@ def test_forward_mode_and_second_derivatives_are_refused(cuda):
     q.requires_grad_()
     with pytest.raises(RuntimeError, match="twice"):
         torch.autograd.grad(ops.packed_attention(q, k, v, cu), (q,), dout, create_graph=True)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (8, 1, 128), (3, 3, 80)])
+@pytest.mark.parametrize("first", [True, False])
+def test_one_long_sequence_beside_many_short_ones(cuda, heads, kv_heads, dim, first):
+    """The mean length, by which CTAs take one query tile or two and share key tiles or not, is that of neither."""
+    short = [1 + i % 5 for i in range(400)] + [0] * 30
+    lens = [2500, *short] if first else [*short[:200], 2500, *short[200:]]
+    q, k, v, cu, dout = _inputs(cuda, lens, heads, kv_heads, dim, pad=3, seed=44)
+    z = _oracle(q, k, v, lens, dout, dim ** -0.5)
+    for name, got in zip(("out", "dq", "dk", "dv"), _run(q, k, v, cu, dout)):
+        _within(got, z, name)
+    assert ops.require().status(0) == 0
