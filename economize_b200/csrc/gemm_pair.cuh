@@ -8,20 +8,27 @@
 // reads 48 KB. The accumulators are double-buffered (2 x 256 TMEM columns): the epilogue of a tile runs under the
 // next tile's MMAs.
 //
+// A product whose sums may not shrink takes them in parts of `part` K blocks, an accumulator buffer each, and its epilogue
+// adds the parts up in registers: the tensor cores cut off, towards zero, what an accumulator cannot hold, at every 16
+// products, so sums of 4096 came out 3.9e-6 of themselves too small. Parts of 1024 bring that to 1e-6, whatever K is.
+//
 //   warp 0      TMA producer (both CTAs; completion counted on the even CTA's barrier)
-//   warp 1      MMA issuer (even CTA only)
+//   warp 1      MMA issuer (even CTA only): the whole warp walks the K blocks, an elected lane issues from descriptors in
+//               uniform registers; issued by a branch of one lane, the MMAs came so slowly that every change of
+//               accumulators, a part's or a tile's, left the tensor pipes idle for 600 cycles
 //   warps 2-9   epilogue: warp w reads TMEM lanes 32 (w % 4) .. + 31 and 128 of the 256 columns
 //
 // The grid is persistent over tiles. Tiles beyond whole rounds of all pairs are split along K where that fills the pairs
 // (Schedule): their units leave fp32 partial tiles that a joining kernel adds up in order. Every wait is bounded
 // (common.cuh).
 //
-// Measured on one B200, 4096 rows, K or N = 4096 and 32000 (burst): both operands K-major 1529 TFLOP/s, B MN-major 1415,
-// both MN-major 1567; the tensor pipes are busy 84 to 85% of the cycles, and at about 1.5 GHz the power limit of 1 kW is
-// what bounds it in a long step.
+// Measured on one B200, 4096 x 4096 x 32000, single launches: both operands K-major with sums in one part 1600 to 1680
+// TFLOP/s, in parts of 1024 (logits) 1580 to 1670, the tensor pipes busy 98% of the cycles; in a long step the power limit
+// of 1 kW and the clock that it leaves are what bounds it.
 #pragma once
 
 #include "common.cuh"
+#include "packed_common.cuh"
 
 namespace ecz {
 namespace pair {
@@ -51,6 +58,7 @@ struct Shape {
   int pairs;       // CTA pairs of the device
   bool split;      // tiles beyond whole rounds may be split along K
   bool n_fastest;  // order of the tiles: N varies fastest (else M)
+  int part;        // K blocks of a part of a sum, for epilogues with kParts (no such product is split or clipped in K)
 };
 
 __device__ __forceinline__ uint32_t mapa_u32(uint32_t addr, uint32_t rank) {
@@ -166,7 +174,8 @@ inline int most_tail(const Shape& s) {
 
 // Epi: a functor `void operator()(const Unit&, int M, int row0, int col0, uint32_t taddr, bool zero, uint8_t* patch,
 // int lane)` of one warp: rows row0 + lane (of the whole output), columns [col0, col0 + 128), accumulators at TMEM
-// address taddr (this warp's lanes), or zeros where the unit has no K block.
+// address taddr (this warp's lanes), or zeros where the unit has no K block. With Epi::kParts the sums in registers, z[j]
+// of column col0 + j, in place of taddr and zero.
 template <bool A_MN, bool B_MN, class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
@@ -181,7 +190,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = packed::uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -208,7 +217,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   __syncthreads();
   cluster_sync();  // the peer's barriers are initialised before anything is counted on them
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = packed::uniform(*tmem_slot);
   pdl_trigger();
   pdl_wait();
 
@@ -242,34 +251,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       while (global_timer_ns() - t0 < 1000000ull) {
       }
     }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
-    // ---- MMA issuer ----
+  } else if (warp == 1 && rank == 0) {
+    // ---- MMA issuer: the whole warp walks, one lane issues, from descriptors in uniform registers ----
     constexpr uint32_t idesc = idesc_bf16_f32(256, 256, B_MN) | ((A_MN ? 1u : 0u) << 15);
     const uint32_t base = smem_u32(smem);
-    uint32_t it = 0, tile = 0;
+    const uint64_t a0 = operand_desc<A_MN>(base, 0), b0 = operand_desc<B_MN>(base + kOperandBytes, 0);
+    const bool leader = packed::elect_one();
+    uint32_t tile = 0, s = 0, turn = 0;  // stage, its phase
     bool ok = true;
     for (int u = pair_id; ok && u < sched.units; u += pairs) {
       const Unit t = sched.unit(u);
-      if (t.nkb <= 0) continue;
-      const uint32_t buf = tile & 1u;
-      if (!mbar_wait(&acc_empty[buf], ((tile >> 1) & 1u) ^ 1u, status, kStatusWaitAccum, abort_flag)) break;
-      tc_fence_after();
-      const uint32_t d = tmem + buf * 256u;
-      for (int kb = 0; kb < t.nkb; ++kb, ++it) {
-        const int s = it % kStages;
-        if (!mbar_wait(&full[s], (it / kStages) & 1u, status, kStatusWaitFull, abort_flag)) {
-          ok = false;
-          break;
-        }
+      const int part = Epi::kParts ? shape.part : t.nkb;
+      for (int kb0 = 0; ok && kb0 < t.nkb; kb0 += part) {
+        const uint32_t buf = tile & 1u;
+        ok = packed::warp_wait(&acc_empty[buf], ((tile >> 1) & 1u) ^ 1u, status, kStatusWaitAccum, abort_flag);
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t a = base + s * kStageBytes, b = a + kOperandBytes;
+        const uint32_t d = tmem + buf * 256u;
+        const int blocks = min(part, t.nkb - kb0);
+        for (int kb = 0; kb < blocks; ++kb) {
+          ok = packed::warp_wait(&full[s], turn, status, kStatusWaitFull, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
+            const uint64_t a = packed::desc_step(a0, s * kStageBytes), b = packed::desc_step(b0, s * kStageBytes);
 #pragma unroll
-        for (int kk = 0; kk < kBK / 16; ++kk)
-          umma_pair(d, operand_desc<A_MN>(a, kk), operand_desc<B_MN>(b, kk), idesc, (kb | kk) != 0 ? 1u : 0u);
-        commit_pair(&empty[s]);
+            for (int kk = 0; kk < kBK / 16; ++kk)
+              umma_pair(d, packed::desc_step(a, kk * (A_MN ? 16 * 128 : 32)),
+                        packed::desc_step(b, kk * (B_MN ? 16 * 128 : 32)), idesc, (kb | kk) != 0 ? 1u : 0u);
+            commit_pair(&empty[s]);
+          }
+          __syncwarp();
+          if (++s == kStages) {
+            s = 0;
+            turn ^= 1u;
+          }
+        }
+        if (leader) commit_pair(&acc_full[buf]);
+        __syncwarp();
+        ++tile;
       }
-      commit_pair(&acc_full[buf]);
-      ++tile;
     }
   } else if (warp >= 2) {
     // ---- epilogue ----
@@ -280,20 +301,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int u = pair_id; u < sched.units; u += pairs) {
       const Unit t = sched.unit(u);
       const int row0 = t.m0 + static_cast<int>(rank) * kHalf + quad * 32, col0 = t.n0 + half * 128;
-      if (t.nkb <= 0) {
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * 128u;
+      // waits for the accumulators that come next, hands them to `take`, and gives their buffer back
+      auto accumulators = [&](auto&& take) {
+        const uint32_t buf = tile & 1u;
+        const bool ok = mbar_wait(&acc_full[buf], (tile >> 1) & 1u, status, kStatusWaitAccum, abort_flag);
+        if (__any_sync(0xffffffffu, !ok)) return false;
+        tc_fence_after();
+        take(taddr + buf * 256u);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_cluster(mapa_u32(smem_u32(&acc_empty[buf]), 0));
+        ++tile;
+        return true;
+      };
+      if constexpr (Epi::kParts) {
+        float z[kHalf];  // the first part's sums, then the others' added
+        bool ok = accumulators([&](uint32_t at) {
+#pragma unroll
+          for (int c = 0; c < kHalf; c += 16) tmem_ld16(at + c, z + c);
+        });
+#pragma unroll 1
+        for (int kb = shape.part; ok && kb < t.nkb; kb += shape.part)
+          ok = accumulators([&](uint32_t at) {
+#pragma unroll
+            for (int c = 0; c < kHalf; c += 16) {
+              float v[16];
+              tmem_ld16(at + c, v);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) z[c + j] += v[j];
+            }
+          });
+        if (!ok) break;
+        epi(t, sched.M, row0, col0, z, patch, lane);
+      } else if (t.nkb <= 0) {
         epi(t, sched.M, row0, col0, 0u, true, patch, lane);
-        continue;
+      } else if (!accumulators([&](uint32_t at) { epi(t, sched.M, row0, col0, at, false, patch, lane); })) {
+        break;
       }
-      const uint32_t buf = tile & 1u;
-      const bool ok = mbar_wait(&acc_full[buf], (tile >> 1) & 1u, status, kStatusWaitAccum, abort_flag);
-      if (__any_sync(0xffffffffu, !ok)) break;
-      tc_fence_after();
-      epi(t, sched.M, row0, col0, tmem + (static_cast<uint32_t>(quad * 32) << 16) + buf * 256u + half * 128u, false,
-          patch, lane);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_cluster(mapa_u32(smem_u32(&acc_empty[buf]), 0));
-      ++tile;
     }
   }
   __syncwarp();

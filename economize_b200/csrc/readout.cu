@@ -30,8 +30,9 @@
 // gradients: 87 us, of which the two reads of W and the write of dW need 30: 25 for each of the three products, whose
 // tiles of 256 rows stand almost empty, and the launches of a training step's call.
 //
-// The tensor cores cut off, not round, what their fp32 sums cannot hold: over 4096 products a log-sum-exp is low by
-// about 4e-6, which is 1e-6 of a mean loss of 4. The target's logit does not share it (see the gather kernel).
+// The tensor cores cut off, not round, what their fp32 sums cannot hold, so the logits are summed in parts (LogitsEpi).
+// The target's logit does not share what is left of it (see the gather kernel). The gradients' products do: over K =
+// 128256 a sum is up to 1.2e-4 of itself too small by the same measure, a twentieth of the rounding to bf16 that follows.
 #include <algorithm>
 
 #include "gemm_pair.cuh"
@@ -188,7 +189,16 @@ __global__ void __launch_bounds__(256) readout_gather_kernel(const __grid_consta
 }
 
 // ---- logits: statistics (and e) of a tile's rows -----------------------------------------------------------------
+// kSums: of logits in registers, added up from parts of at most kPartBlocks K blocks (see gemm_pair.cuh), else read twice
+// from TMEM. One sum was 3.9e-6 of itself too small at H = 4096, and a mean loss of 4.2 by 1.1e-6 of itself; parts of
+// 1024 leave 1.0e-6 and 2.5e-7, of 512 half of that. What parts cost, us of the logits with e, one sum / 1024 / 512:
+// 4096 x 4096 x 32000 669 / 680 / 756, 2048 x 1088 x 50257 (losses) 141 / 152 / 179. Where H takes one part there is
+// nothing to add up, and the shorter form serves (16 x 1024 x 32000 with both gradients: 90, in registers 96).
+constexpr int kPartBlocks = 16;
+
+template <bool kSums>
 struct LogitsEpi {
+  static constexpr bool kParts = kSums;
   float2* stats;      // [rows of the chunk, pieces]: (max, sum of exp2(z - max)) without the target, log2 units
   const int* target;  // [rows] of the chunk
   __half* e;          // [rows, ld] or null
@@ -198,45 +208,59 @@ struct LogitsEpi {
 
   __device__ __forceinline__ void operator()(const pair::Unit&, int M, int row0, int col0, uint32_t taddr, bool,
                                              uint8_t* patch, int lane) const {
+    piece(M, row0, col0, patch, lane, [&](int c, float* v) {
+      tmem_ld32(taddr + c, v);
+      return v;
+    });
+  }
+
+  __device__ __forceinline__ void operator()(const pair::Unit&, int M, int row0, int col0, float (&z)[kPiece],
+                                             uint8_t* patch, int lane) const {
+    piece(M, row0, col0, patch, lane, [&](int c, float*) { return z + c; });
+  }
+
+  // `fetch`: the logits of 32 columns from c on, in the given place or one of their own, to be written over.
+  template <class Fetch>
+  __device__ __forceinline__ void piece(int M, int row0, int col0, uint8_t* patch, int lane, Fetch fetch) const {
+    constexpr int kUnroll = kSums ? kPiece / 32 : 1;
     if (row0 >= M || col0 >= V) return;  // uniform over the warp
     const int row = row0 + lane;
-    const int cols = min(kPiece, V - col0);
+    const int cols = V - col0;
     const int mine = row < M ? target[row] - col0 : -1;
+    // the columns of 32 from c on that count: inside the vocabulary and not the row's target
+    auto counted = [&](int c) {
+      const uint32_t inside = cols - c >= 32 ? ~0u : (1u << max(0, cols - c)) - 1u;
+      return (mine >> 5) == (c >> 5) ? inside & ~(1u << (mine & 31)) : inside;
+    };
     float top = -INFINITY;
-#pragma unroll 1
+#pragma unroll kUnroll
     for (int c = 0; c < kPiece; c += 32) {
-      float v[32];
-      tmem_ld32(taddr + c, v);
-      const int skip = mine - c;
-      if (c + 32 <= cols && !__any_sync(0xffffffffu, skip >= 0 && skip < 32)) {
+      float here[32];
+      float* v = fetch(c, here);
+      const uint32_t bits = counted(c);
+      if (__all_sync(0xffffffffu, bits == ~0u)) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) top = fmaxf(top, v[j] * scale2);
       } else {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (c + j < cols && j != skip) top = fmaxf(top, v[j] * scale2);
+        for (int j = 0; j < 32; ++j) top = (bits >> j) & 1u ? fmaxf(top, v[j] * scale2) : top;
       }
     }
     const float ref = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
-#pragma unroll 1
+#pragma unroll kUnroll
     for (int c = 0; c < kPiece; c += 32) {
-      float v[32];
-      tmem_ld32(taddr + c, v);
-      const int skip = mine - c;
-      if (c + 32 <= cols && !__any_sync(0xffffffffu, skip >= 0 && skip < 32)) {
+      float here[32];
+      float* v = fetch(c, here);
+      const uint32_t bits = counted(c);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          v[j] = ex2(fmaf(v[j], scale2, -ref));
-          sum += v[j];
-        }
-      } else {
+      for (int j = 0; j < 32; ++j) v[j] = ex2(fmaf(v[j], scale2, -ref));
+      if (!__all_sync(0xffffffffu, bits == ~0u)) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          v[j] = c + j < cols && j != skip ? ex2(fmaf(v[j], scale2, -ref)) : 0.f;
-          sum += v[j];
-        }
+        for (int j = 0; j < 32; ++j) v[j] = (bits >> j) & 1u ? v[j] : 0.f;
       }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) sum += v[j];
       if (e != nullptr) {
 #pragma unroll
         for (int j = 0; j < 32; j += 8) {
@@ -410,6 +434,7 @@ __device__ __forceinline__ int partial_at(int rb, int cb, int q, int lane) {
 // Stores a warp's 32 x 128 accumulators: bf16 rows (through the patch, 128-byte row segments), a split tile's fp32
 // partial, or an fp32 running sum over the chunks whose last chunk stores bf16.
 struct StoreEpi {
+  static constexpr bool kParts = false;
   bf16* out;        // [.., N]
   float* part;      // partials of split tiles, [tile, split] and see partial_at
   float* sum;       // running sum [M, N], or null
@@ -582,10 +607,16 @@ int launch_readout_gather(const ReadoutRows& r, const int* pos, int* rows, int* 
 
 int launch_readout_logits(const CUtensorMap* xs, const CUtensorMap* w, const ReadoutChunk& c, int num_sms,
                           unsigned* status, cudaStream_t stream) {
-  LogitsEpi epi{static_cast<float2*>(c.stats), c.target + c.row0, static_cast<__half*>(c.e), c.ld, c.V,
-                readout_pieces(c.V), c.logit_scale * kLog2e};
-  const pair::Shape shape{c.chunk, c.V, c.H, c.count, c.row0, true, false, num_sms / 2, false, false};
-  return pair::launch_pair<false, false>(*xs, *w, shape, epi, status, stream);
+  const int blocks = (c.H + pair::kBK - 1) / pair::kBK, parts = (blocks + kPartBlocks - 1) / kPartBlocks;
+  const pair::Shape shape{c.chunk, c.V, c.H, c.count, c.row0, true, false, num_sms / 2, false, false,
+                          (blocks + parts - 1) / parts};
+  auto launch = [&](auto epi) { return pair::launch_pair<false, false>(*xs, *w, shape, epi, status, stream); };
+  float2* stats = static_cast<float2*>(c.stats);
+  __half* e = static_cast<__half*>(c.e);
+  const int pieces = readout_pieces(c.V);
+  const float scale2 = c.logit_scale * kLog2e;
+  return parts > 1 ? launch(LogitsEpi<true>{stats, c.target + c.row0, e, c.ld, c.V, pieces, scale2})
+                   : launch(LogitsEpi<false>{stats, c.target + c.row0, e, c.ld, c.V, pieces, scale2});
 }
 
 static Shared shared_of(const ReadoutChunk& c) {
@@ -621,7 +652,7 @@ int launch_readout_dx(const CUtensorMap* dz, const CUtensorMap* w, const Readout
                       int num_sms, unsigned* status, cudaStream_t stream) {
   const int* rows = c.rows + c.row0;
   const StoreEpi epi{static_cast<bf16*>(dx), part, nullptr, rows, c.H, false, true, shared_of(c)};
-  const pair::Shape shape{c.chunk, c.H, c.V, c.count, c.row0, true, false, num_sms / 2, true, false};
+  const pair::Shape shape{c.chunk, c.H, c.V, c.count, c.row0, true, false, num_sms / 2, true, false, 0};
   const int rc = pair::launch_pair<false, true>(*dz, *w, shape, epi, status, stream);
   return rc != 0 ? rc : launch_join(shape, part, rows, c, dx, stream);
 }
@@ -630,7 +661,7 @@ int launch_readout_dw(const CUtensorMap* dz, const CUtensorMap* xs, const Readou
                       bool first, bool last, void* dw, int num_sms, unsigned* status, cudaStream_t stream) {
   const bool once = first && last;
   const StoreEpi epi{static_cast<bf16*>(dw), part, once ? nullptr : sum, nullptr, c.H, !first, last, shared_of(c)};
-  const pair::Shape shape{c.V, c.H, c.chunk, c.count, c.row0, false, true, num_sms / 2, once, true};
+  const pair::Shape shape{c.V, c.H, c.chunk, c.count, c.row0, false, true, num_sms / 2, once, true, 0};
   const int rc = pair::launch_pair<true, true>(*dz, *xs, shape, epi, status, stream);
   return rc != 0 ? rc : launch_join(shape, part, nullptr, c, dw, stream);
 }

@@ -571,3 +571,23 @@ def test_upstream_gradients(cuda, upstream):
     again = 0.0 if upstream == 4.0 else 2.0 ** -8 * (1 + 2.0 ** -7)
     _within(dx, o["dx"], o["dx_err"] + again * (o["dx"].abs() + o["dx_err"]), "dx")
     _within(dw, o["dw"], o["dw_err"] + again * (o["dw"].abs() + o["dw_err"]), "dw")
+
+
+@pytest.mark.parametrize("hidden", [512, 1000, 1032, 2560, 4096])
+def test_long_sums_do_not_shrink(cuda, hidden):
+    """The tensor cores cut off what an accumulator cannot hold, towards zero, at every 16 products: in one sum of 4096
+    the logits, and so every loss, came out 4 millionths too small. A sum of 1024 products is cut 64 times, by half of its
+    last place (2^-24 of itself) on average, while it grows to its full size: 64 2^-25 = 1.9e-6 of itself. Sums of sums
+    are rounded, which has no direction. Read from the losses of a vocabulary of two, of which one logit is zero:
+    nll = log(1 + exp z)."""
+    rows = 40000
+    g = torch.Generator(device=cuda).manual_seed(25)
+    w = torch.zeros(2, hidden, device=cuda)
+    w[1] = torch.randn(hidden, device=cuda, generator=g) * (1.28 / hidden ** 0.5)
+    w = w.bfloat16()
+    lean = (2 * torch.rand(rows, 1, device=cuda, generator=g) - 1) * 6.25
+    x = (torch.randn(rows, hidden, device=cuda, generator=g) + lean * w[1].float() / w[1].float().norm()).bfloat16()
+    z = x.double() @ w[1].double()
+    nll = ops.linear_cross_entropy(x, w, torch.zeros(rows, device=cuda, dtype=torch.long), reduction="none").double()
+    off = torch.log(torch.expm1(nll)) - z
+    assert abs((off * z).sum() / z.square().sum()) <= 64 * 2.0 ** -25
