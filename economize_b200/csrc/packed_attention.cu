@@ -16,6 +16,9 @@
 // the A operand of P . V), O accumulates in TMEM. A row's reference maximum moves only when a chunk raises it by more
 // than 2^8 (lazy rescaling), so O is rarely read back before the end.
 //
+// The running reference and sum are those of the online softmax (Milakov and Gimelshein, 2018), the recomputation of P
+// from the log-sum-exp in the backward pass is that of Dao et al. (2022).
+//
 // P is rounded to bf16 for P . V: one rounding of the output's left factor, as its result's is of the whole. Over many
 // keys these errors average out; a tile of one chunk multiplies what the rounding leaves of P as well (eight MMAs more),
 // so that the output's rows of few keys, and the backward pass's delta, where dp - delta cancels, do not carry it.
@@ -183,10 +186,10 @@ __global__ void __launch_bounds__(kPlanThreads)
 // over 4, took 973 us instead of 885.
 //
 // Measured on one B200, D = 128: that document 830 us, 1320 TFLOP/s of its 4 D n (n + 1) / 2 useful operations, bound by
-// the tensor cores at the clock that 1 kW leaves them; 8 sequences of 1024, 32 heads over 8, 97 us, 830 TFLOP/s: the
-// diagonal chunks' hidden half and seven or eight items to a CTA cost the rest (49% of the tensor pipes' cycles at 1638
-// tokens in the mean); 4096 tokens in 48 sequences 33 us, 3.7 TB/s: an item is a chunk or two, and the latency of its
-// loads, softmax and store bounds it.
+// the tensor cores at the clock that 1 kW leaves them; 8192 tokens in 8 sequences of 364 to 1587, 32 heads over 8, 97 us,
+// 830 TFLOP/s: the diagonal chunks' hidden half and seven or eight items to a CTA cost the rest (49% of the tensor pipes'
+// cycles at 1638 tokens in the mean); 4096 tokens in 48 sequences 33 us, 3.7 TB/s: an item is a chunk or two, and the
+// latency of its loads, softmax and store bounds it.
 template <int DP, int kTiles>
 struct FwdCfg {
   static constexpr int kTileBytes = kRowsT * DP * 2;
@@ -619,10 +622,12 @@ int launch_packed_plan(const int* cu, int B, int T, const PackedTable* tables, i
                  cudaSuccess ? 0 : -1;
 }
 
-// Measured on one B200, us for one / two tiles: D = 64, 12 heads of their own, 8192 tokens in sequences of 16: 61 / 112,
-// of 128: 23.8 / 31.4, of 1024: 35.9 / 39.0, one of 8192: 152 / 164. D = 128, 32 heads over 8, of 16: 56 / 96, of 128:
-// 47.7 / 46.6, of 512: 69.8 / 63.3, of 1024: 96.5 / 87.0, of 8192: 496 / 447; 6490 tokens in 18 sequences 73.2 / 70.5;
-// 4096 tokens in 48: 32.6 / 35.4.
+// Measured on one B200 with the plan, us for one / two tiles of 8192 tokens. D = 64, 12 heads of their own, in sequences
+// of 16: 60 / 113, of 128: 20.5 / 27.0, of 1024: 32.3 / 35.7, one of 8192: 148 / 161. D = 128, 32 heads over 8, of 16: 51 /
+// 95, of 64: 39.0 / 38.1, of 96: 41.7 / 44.3, of 128: 44.2 / 42.4, of 256: 49.2 / 45.0, of 384: 56.7 / 51.1, of 512: 65.3 /
+// 58.2, of 1024: 91.4 / 79.7, one of 8192: 500 / 450. At D = 128 they cross near 100 tokens; the rule keeps one tile up to
+// a mean of 511, at a cost of 4 to 11%. The mean says little of mixed lengths: one sequence of 8000 beside 24 of 8 counts
+// as short ones and takes 530 us where two tiles take 475; one of 4096 beside 256 of 16 is even (181 / 185).
 bool packed_single_tiles(int T, int B, int D) { return D <= 64 || static_cast<long>(T) < 512l * B; }
 
 int launch_packed_forward(const PackedMaps& maps, const PackedArgs& a, void* out, void* rest, float* lse, int tiles,

@@ -15,7 +15,11 @@
 // dq   CTA: a tile of queries, as in the forward pass; walks the key chunks up to the diagonal. S (two buffers), dP and
 //      dQ in TMEM; dS is dQ's A operand where S was.
 //
-// P^T and dS^T (dS) are rounded to bf16 once, as operands; the log-sum-exp, delta and all sums are fp32.
+// P^T and dS^T (dS) are rounded to bf16 once, as operands: the other factor of their products is bf16, and kind::f16 takes
+// both of one type. Those roundings are independent from entry to entry, so over a row's keys they add up to less than
+// the rounding of the bf16 result: gradients are 0.0024 of themselves from their 64-bit values where products of 32-bit
+// operands are 0.0017 from them. The rest of P that the forward pass multiplies for tiles of one chunk would cost a product
+// more here. The log-sum-exp, delta and all sums are fp32.
 //
 // Measured on one B200, D = 128. One sequence of 16384 tokens, 16 heads over 4: dkv 1600 us, 1370 TFLOP/s of its four
 // products' useful operations, dq 1340 us, 1230 of its three: the tensor cores at the clock that 1 kW leaves them (the
@@ -861,7 +865,9 @@ int run_bwd(const PackedMaps& m, const PackedArgs& a, const BwdArgs& args, bool 
 // mean work, so two per SM are wanted), each of eight iterations of the mean tile at least. Measured with delta, us
 // for 1 / 2 / 4 / 8 splits, D = 128, by key tiles x iterations of the mean one: 16 x 64 194 / 129 / 75 / 53, 64 x 32
 // 110 / 85 / 69 / 93, 64 x 16 68 / 55 / 55 / 75, 128 x 128 427 / 277 / 280 / 349, 8 x 8 51 / 54 / 53 / 53,
-// 256 x 128 471 / 536 / 619 / 711.
+// 256 x 128 471 / 536 / 619 / 711. Both numbers go by the mean length, which says little of mixed ones: a sequence of 2048
+// (8 heads over 2) beside 100 of 8 tokens gets no splits and takes 184 us with the forward pass, alone 123; one of 4096 (8
+// heads over 1) beside 200 of 4 tokens 523, alone 212.
 int packed_dkv_splits(const PackedArgs& a, int B) {
   const long items = static_cast<long>(std::max(1, a.T / 128)) * a.Hkv;
   const long mean = (static_cast<long>(a.T) / std::max(1, B)) * (a.H / a.Hkv) / 256;  // iterations of 128 rows

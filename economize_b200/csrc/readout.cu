@@ -24,11 +24,11 @@
 //
 // Without gradients only the statistics of the pieces are written (8 bytes per 128 logits).
 //
-// Measured on one B200, 4096 rows x 4096 x 32000: logits 715 us (1500 TFLOP/s), finish 101 us (e read and dz written
-// once, 5.2 TB/s), dX 715 us, dW 710 us (1510 each), one by one; 2.6 to 2.75 ms in a row, at the clock that the power
-// limit leaves. 1024 rows x 4096 x 128256, losses only: 755 us, 1425 TFLOP/s. 16 rows x 1024 x 32000 with both
-// gradients: 87 us, of which the two reads of W and the write of dW need 30: 25 for each of the three products, whose
-// tiles of 256 rows stand almost empty, and the launches of a training step's call.
+// Measured on one B200, 4096 rows x 4096 x 32000: logits 681 us (1580 TFLOP/s), finish 101 us (e read and dz written
+// once, 5.2 TB/s), dX 683 us, dW 687 us (1570 each), one by one; 2.55 to 2.65 ms in a row, at the clock that the power
+// limit leaves. 1024 rows x 4096 x 128256, losses only: 860 us in a row, 1250 TFLOP/s. 16 rows x 1024 x 32000 with both
+// gradients: 87 us, of which the two reads of W and the write of dW need 30: 17 to 25 for each of the three products,
+// whose tiles of 256 rows stand almost empty, and the launches of a training step's call.
 //
 // The tensor cores cut off, not round, what their fp32 sums cannot hold, so the logits are summed in parts (LogitsEpi).
 // The target's logit does not share what is left of it (see the gather kernel). The gradients' products do: over K =
@@ -96,7 +96,10 @@ __global__ void __launch_bounds__(1024) readout_plan_kernel(const int64_t* __res
 // Warp per row t, eight to a CTA: its state to xs, its target's logit to picked, or zeros to dx (and losses[t]) where it
 // is ignored. The rows behind the last packed one are zeroed up to the K block that reads them. Without a plan (pos
 // null, few rows) every CTA counts the rows before its own itself, which saves a launch.
-constexpr int kPlanRows = 2048;  // rows up to which counting costs less than a plan
+// Rows up to which every CTA counts. Losses of T rows x 256 x 1000 from a CUDA graph, us counted / planned: 1024 18.0 /
+// 18.7, 2048 21.3 / 23.7, 4096 30.6 / 32.7, 16384 95.8 / 98.1, 32768 206 / 182, 131072 1483 / 771 (every CTA reads all
+// targets: T^2 / 8 of them). Between 2048 and about 20000 the rule is 2 to 4 us on the safe side.
+constexpr int kPlanRows = 2048;
 
 struct GatherArgs {
   const bf16 *x, *w;
@@ -562,7 +565,9 @@ __global__ void __launch_bounds__(kJoinThreads)
 }
 
 // x and y times *g in place (bf16, sizes in groups of 8); reads nothing more when *g is 1, what a loss's own backward
-// passes.
+// passes. Unless *g is a power of two this is a second rounding to bf16 of the gradients of a mean or sum, which were
+// rounded before *g was known: as much again as the first at most. Keeping what the first rounding left would write
+// every gradient twice (65 MB more for 16 rows x 1024 x 32000: 10 of 90 us) for a case that is not the usual one.
 __global__ void __launch_bounds__(256) scale_by_kernel(uint4* __restrict__ x, long nx, uint4* __restrict__ y, long ny,
                                                        const float* __restrict__ g) {
   pdl_trigger();

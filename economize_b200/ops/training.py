@@ -42,6 +42,10 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
             per-row losses ``[...]`` (0 for ignored rows), whose backward pass computes the logits again.
         chunk_rows: Rows processed at a time (0: as many as 1 GiB of 16-bit probabilities hold, more where a trained
             ``weight`` needs as much for the sum over several chunks).
+
+    On CUDA a mean or sum computes the gradients of what requires them with the loss, three products instead of one: take
+    a loss that is not differentiated under ``torch.no_grad()``. They are rounded to bf16 there, and once more in the
+    backward pass where the upstream gradient is no power of two (a loss divided by three batches).
     """
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {tuple(_REDUCTIONS)}, got {reduction!r}")
