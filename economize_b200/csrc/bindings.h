@@ -22,4 +22,7 @@ unsigned* device_status(const at::Device& device);
 // bindings_train.cpp: the training operators.
 void bind_training(pybind11::module_& m);
 
+// bindings_block.cpp: 4-bit operands and products, norms around a block.
+void bind_block(pybind11::module_& m);
+
 }  // namespace ecz

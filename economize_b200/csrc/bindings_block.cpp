@@ -1,0 +1,457 @@
+// PyTorch bindings of the 4-bit operators (fp4.cu, gemm_fp4.cu) and of the norms around a block (block_norm.cu):
+// argument checks, workspaces from PyTorch's caching allocator, tensor maps, launches on the current stream.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <cmath>
+#include <cstring>
+#include <tuple>
+
+#include "bindings.h"
+#include "launchers.h"
+
+namespace {
+
+using at::Tensor;
+
+constexpr int64_t kMaxRows = int64_t{1} << 30;
+
+// Rows a kernel reads in place: unit stride along the row; others are copied.
+Tensor rows_of(const Tensor& x) {
+  const bool ok = (x.size(1) <= 1 || x.stride(1) == 1) && (x.size(0) <= 1 || x.stride(0) >= x.size(1));
+  return ok ? x : x.contiguous();
+}
+
+int64_t row_stride(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
+
+bool aligned(const Tensor& x) {
+  return !x.defined() || (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 &&
+                          (x.dim() < 2 || row_stride(x) * x.element_size() % 16 == 0));
+}
+
+// ---- 4-bit operands ------------------------------------------------------------------------------------------------
+struct Fp4Buffers {
+  Tensor codes, scales, row_scale;
+};
+
+void check_format(int64_t fmt) { TORCH_CHECK(fmt == 1 || fmt == 2, "unknown 4-bit format ", fmt); }
+
+Fp4Buffers fp4_buffers(const Tensor& like, int64_t rows, int64_t K, int64_t fmt) {
+  const auto bytes = like.options().dtype(at::kByte);
+  Fp4Buffers b;
+  b.codes = at::empty({rows, K / 2}, bytes);
+  b.scales = at::empty({(rows + 127) / 128, ecz::fp4_scale_tiles(static_cast<int>(fmt), static_cast<int>(K)), 512}, bytes);
+  b.row_scale = at::empty({fmt == 1 ? rows : 0}, like.options().dtype(at::kFloat));
+  return b;
+}
+
+void check_columns(int64_t K, const char* what) {
+  TORCH_CHECK(K >= 32 && K % 32 == 0 && K <= ecz::kFp4MaxK, what, ": columns must be a multiple of 32, up to ",
+              ecz::kFp4MaxK, " (got ", K, ")");
+}
+
+Fp4Buffers quantize(Tensor x, int64_t fmt, bool early) {
+  CHECK_CUDA(x);
+  CHECK_BF16(x);
+  check_format(fmt);
+  TORCH_CHECK(x.dim() == 2, "fp4_quantize expects x [M, K]");
+  const int64_t M = x.size(0), K = x.size(1);
+  check_columns(K, "fp4_quantize");
+  TORCH_CHECK(M <= kMaxRows, "fp4_quantize: too many rows");
+  c10::cuda::CUDAGuard guard(x.device());
+  Fp4Buffers b = fp4_buffers(x, M, K, fmt);
+  if (M == 0) return b;
+  x = rows_of(x);
+  if (!aligned(x)) x = x.clone(at::MemoryFormat::Contiguous);
+  const int rc = ecz::launch_fp4_quantize(x.data_ptr(), row_stride(x), static_cast<int>(fmt), b.codes.data_ptr(),
+                                          b.scales.data_ptr(), b.row_scale.data_ptr<float>(), static_cast<int>(M),
+                                          static_cast<int>(K), early, ecz::device_sms(x.get_device()),
+                                          at::cuda::getCurrentCUDAStream());
+  TORCH_CHECK(rc == 0, "fp4_quantize: launch failed");
+  return b;
+}
+
+std::tuple<Tensor, Tensor, Tensor> fp4_quantize(const Tensor& x, int64_t fmt) {
+  // the result may become a weight, which products fetch before the kernel in front of them ends: no early start
+  Fp4Buffers b = quantize(x, fmt, false);
+  return {b.codes, b.scales, b.row_scale};
+}
+
+// Codes, scales and row scales of one operand belong together.
+void check_operand(const Tensor& codes, const Tensor& scales, const Tensor& row_scale, int64_t fmt, const Tensor& ref,
+                   const char* what) {
+  check_format(fmt);
+  TORCH_CHECK(codes.is_cuda() && codes.get_device() == ref.get_device() && scales.is_cuda() &&
+                  scales.get_device() == ref.get_device(),
+              what, ": codes and scales must be on one CUDA device");
+  TORCH_CHECK(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte && codes.dim() == 2 &&
+                  codes.is_contiguous() && scales.is_contiguous(),
+              what, ": codes [rows, K / 2] and scales must be contiguous uint8");
+  check_columns(codes.size(1) * 2, what);
+  TORCH_CHECK(codes.size(0) <= kMaxRows, what, ": too many rows");
+  const int64_t tiles = ecz::fp4_scale_tiles(static_cast<int>(fmt), static_cast<int>(codes.size(1) * 2));
+  TORCH_CHECK(scales.dim() == 3 && scales.size(0) == (codes.size(0) + 127) / 128 && scales.size(1) == tiles &&
+                  scales.size(2) == 512,
+              what, ": scales must be [", (codes.size(0) + 127) / 128, ", ", tiles, ", 512], got ", scales.sizes());
+  if (fmt == 1) {
+    TORCH_CHECK(row_scale.is_cuda() && row_scale.get_device() == ref.get_device() &&
+                    row_scale.scalar_type() == at::kFloat && row_scale.dim() == 1 &&
+                    row_scale.size(0) == codes.size(0) && row_scale.is_contiguous(),
+                what, ": nvfp4 has an fp32 scale per row");
+  }
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0,
+              what, ": codes and scales must start on 16-byte boundaries");
+}
+
+Tensor fp4_dequantize(const Tensor& codes, const Tensor& scales, const Tensor& row_scale, int64_t fmt) {
+  CHECK_CUDA(codes);
+  check_operand(codes, scales, row_scale, fmt, codes, "fp4_dequantize");
+  c10::cuda::CUDAGuard guard(codes.device());
+  const int64_t M = codes.size(0), K = codes.size(1) * 2;
+  Tensor out = at::empty({M, K}, codes.options().dtype(at::kBFloat16));
+  if (M == 0) return out;
+  const int rc = ecz::launch_fp4_dequantize(codes.data_ptr(), scales.data_ptr(),
+                                            fmt == 1 ? row_scale.data_ptr<float>() : nullptr, static_cast<int>(fmt),
+                                            out.data_ptr(), static_cast<int>(M), static_cast<int>(K),
+                                            ecz::device_sms(codes.get_device()), at::cuda::getCurrentCUDAStream());
+  TORCH_CHECK(rc == 0, "fp4_dequantize: launch failed");
+  return out;
+}
+
+CUtensorMap codes_map(const Tensor& codes, int box_rows) {
+  CUtensorMap map;
+  std::memset(&map, 0, sizeof(map));
+  const int rc = ecz::make_tmap_2d(&map, 1, codes.data_ptr(), codes.size(0), codes.size(1), codes.size(1), 128, box_rows,
+                                   128);
+  TORCH_CHECK(rc == 0, "cuTensorMapEncodeTiled failed (code ", rc, ") for codes ", codes.sizes());
+  return map;
+}
+
+// Y [M, N] of two operands [M, K] and [N, K] of one format.
+Tensor fp4_matmul(const Tensor& x, const Tensor& xs, const Tensor& xr, const Tensor& w, const Tensor& ws, const Tensor& wr,
+                  int64_t fmt) {
+  CHECK_CUDA(x);
+  check_operand(x, xs, xr, fmt, x, "fp4_matmul: x");
+  check_operand(w, ws, wr, fmt, x, "fp4_matmul: w");
+  TORCH_CHECK(x.size(1) == w.size(1), "fp4_matmul: x has ", 2 * x.size(1), " columns, w ", 2 * w.size(1));
+  TORCH_CHECK(w.size(0) >= 1, "fp4_matmul: w has no rows");
+  c10::cuda::CUDAGuard guard(x.device());
+  const int64_t M = x.size(0), N = w.size(0), K = 2 * x.size(1);
+  Tensor y = at::empty({M, N}, x.options().dtype(at::kBFloat16));
+  if (M == 0) return y;
+  const CUtensorMap tw = codes_map(w, 128), tx = codes_map(x, ecz::fp4_block_rows(static_cast<int>(M)));
+  const int rc = ecz::launch_gemm_fp4(&tw, &tx, ws.data_ptr(), xs.data_ptr(), fmt == 1 ? wr.data_ptr<float>() : nullptr,
+                                      fmt == 1 ? xr.data_ptr<float>() : nullptr, static_cast<int>(fmt), y.data_ptr(),
+                                      static_cast<int>(M), static_cast<int>(N), static_cast<int>(K),
+                                      ecz::device_sms(x.get_device()), ecz::device_status(x.device()),
+                                      at::cuda::getCurrentCUDAStream());
+  TORCH_CHECK(rc == 0, "fp4_matmul: launch failed");
+  return y;
+}
+
+// bf16 activations [M, K] times a 4-bit weight [N, K]: quantised first, in a buffer of their own.
+Tensor linear_fp4(const Tensor& x, const Tensor& w, const Tensor& ws, const Tensor& wr, int64_t fmt) {
+  Fp4Buffers b = quantize(x, fmt, true);
+  return fp4_matmul(b.codes, b.scales, b.row_scale, w, ws, wr, fmt);
+}
+
+// ---- norms around a block ------------------------------------------------------------------------------------------
+ecz::NormType norm_type(const Tensor& x) {
+  switch (x.scalar_type()) {
+    case at::kBFloat16: return ecz::kNormBf16;
+    case at::kHalf: return ecz::kNormFp16;
+    case at::kFloat: return ecz::kNormFp32;
+    default: TORCH_CHECK(false, "block_norm takes bfloat16, float16 or float32, got ", x.scalar_type());
+  }
+}
+
+struct NormOperands {
+  Tensor x, residual, weight, post, gate;
+  int gate_mode = ecz::kGateNone;
+  bool vec = false;
+};
+
+// Checked operands, rows readable in place. Undefined: residual, post and gate that are not given.
+NormOperands norm_operands(const Tensor& x, const Tensor& residual, const Tensor& weight, const Tensor& post,
+                           const Tensor& gate, double scale, double eps) {
+  CHECK_CUDA(x);
+  norm_type(x);
+  TORCH_CHECK(x.dim() == 2, "block_norm expects x [T, H]");
+  const int64_t T = x.size(0), H = x.size(1);
+  TORCH_CHECK(H >= 1 && H <= ecz::kBlockNormMaxHidden, "block_norm: 1 to ", ecz::kBlockNormMaxHidden, " columns (got ", H,
+              ")");
+  TORCH_CHECK(T <= kMaxRows, "block_norm: too many rows");
+  TORCH_CHECK(std::isfinite(scale) && std::isfinite(eps) && eps >= 0, "block_norm: scale and eps must be finite, eps >= 0");
+  for (const Tensor* t : {&residual, &weight, &post, &gate}) {
+    if (!t->defined()) continue;
+    TORCH_CHECK(t->scalar_type() == x.scalar_type(), "block_norm: all operands have one type (", x.scalar_type(), " and ",
+                t->scalar_type(), ")");
+    TORCH_CHECK(t->is_cuda() && t->get_device() == x.get_device(), "block_norm: all operands must be on the device of x");
+  }
+  TORCH_CHECK(weight.defined() && weight.dim() == 1 && weight.size(0) == H, "block_norm: weight must be [", H, "]");
+  TORCH_CHECK(!post.defined() || (post.dim() == 1 && post.size(0) == H), "block_norm: post_weight must be [", H, "]");
+  TORCH_CHECK(!residual.defined() || residual.sizes() == x.sizes(), "block_norm: residual ", residual.sizes(),
+              " does not match x ", x.sizes());
+  NormOperands o;
+  o.x = rows_of(x);
+  o.weight = weight.contiguous();
+  if (residual.defined()) o.residual = rows_of(residual);
+  if (post.defined()) o.post = post.contiguous();
+  if (gate.defined()) {
+    TORCH_CHECK(gate.dim() == 2 && gate.size(0) == T && (gate.size(1) == 1 || gate.size(1) == H),
+                "block_norm: gate must be [", T, ", 1] or [", T, ", ", H, "], got ", gate.sizes());
+    o.gate_mode = gate.size(1) == 1 ? ecz::kGateToken : ecz::kGateFull;
+    o.gate = o.gate_mode == ecz::kGateFull ? rows_of(gate) : gate;
+  }
+  const bool full = o.gate_mode == ecz::kGateFull;
+  o.vec = H * x.element_size() % 16 == 0 && aligned(o.x) && aligned(o.weight) && aligned(o.residual) && aligned(o.post) &&
+          (!full || aligned(o.gate));
+  return o;
+}
+
+const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+ecz::BlockNormArgs norm_args(const NormOperands& o, double scale, double eps) {
+  ecz::BlockNormArgs a;
+  a.x = ptr(o.x);
+  a.residual = ptr(o.residual);
+  a.weight = ptr(o.weight);
+  a.post = ptr(o.post);
+  a.gate = ptr(o.gate);
+  a.x_stride = row_stride(o.x);
+  a.r_stride = o.residual.defined() ? row_stride(o.residual) : 0;
+  a.gate_stride = o.gate.defined() ? (o.gate.size(0) > 1 ? o.gate.stride(0) : 0) : 0;
+  a.gate_mode = o.gate_mode;
+  a.rows = static_cast<int>(o.x.size(0));
+  a.hidden = static_cast<int>(o.x.size(1));
+  a.scale = static_cast<float>(scale);
+  a.eps = static_cast<float>(eps);
+  return a;
+}
+
+struct NormResult {
+  Tensor normed, stream, inv_s, inv_x;
+};
+
+NormResult norm_forward(const Tensor& x, const Tensor& residual, const Tensor& weight, const Tensor& post,
+                        const Tensor& gate, double scale, double eps, bool training) {
+  const NormOperands o = norm_operands(x, residual, weight, post, gate, scale, eps);
+  c10::cuda::CUDAGuard guard(x.device());
+  const auto f32 = x.options().dtype(at::kFloat);
+  NormResult r;
+  r.normed = at::empty(x.sizes(), x.options());
+  r.stream = at::empty(x.sizes(), x.options());
+  if (training) {
+    r.inv_s = at::empty({x.size(0)}, f32);
+    r.inv_x = at::empty({post.defined() ? x.size(0) : 0}, f32);
+  }
+  if (x.size(0) == 0) return r;
+  ecz::BlockNormArgs a = norm_args(o, scale, eps);
+  a.normed = r.normed.data_ptr();
+  a.stream = r.stream.data_ptr();
+  if (training) {
+    a.inv_s = r.inv_s.data_ptr<float>();
+    if (post.defined()) a.inv_x = r.inv_x.data_ptr<float>();
+  }
+  TORCH_CHECK(ecz::launch_block_norm(a, norm_type(x), o.vec, 0, ecz::device_sms(x.get_device()),
+                                     at::cuda::getCurrentCUDAStream()) == 0,
+              "block_norm: launch failed");
+  return r;
+}
+
+Tensor value(const c10::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
+
+// Codes, scales and row scales of normed, and the stream.
+std::tuple<Tensor, Tensor, Tensor, Tensor> block_norm_fp4(const Tensor& x, const c10::optional<Tensor>& residual,
+                                                          const Tensor& weight, const c10::optional<Tensor>& post,
+                                                          const c10::optional<Tensor>& gate, double scale, double eps,
+                                                          int64_t fmt) {
+  check_format(fmt);
+  CHECK_CUDA(x);
+  CHECK_BF16(x);
+  NormOperands o = norm_operands(x, value(residual), weight, value(post), value(gate), scale, eps);
+  check_columns(x.size(1), "block_norm in 4 bits");
+  c10::cuda::CUDAGuard guard(x.device());
+  Fp4Buffers b = fp4_buffers(x, x.size(0), x.size(1), fmt);
+  Tensor stream = at::empty(x.sizes(), x.options());
+  if (x.size(0) == 0) return {b.codes, b.scales, b.row_scale, stream};
+  if (!o.vec) {  // rows that do not start on 16 bytes
+    for (Tensor* t : {&o.x, &o.residual, &o.weight, &o.post, &o.gate})
+      if (t->defined() && !(t == &o.gate && o.gate_mode == ecz::kGateToken) && !aligned(*t))
+        *t = t->clone(at::MemoryFormat::Contiguous);
+  }
+  ecz::BlockNormArgs a = norm_args(o, scale, eps);
+  a.stream = stream.data_ptr();
+  a.codes = b.codes.data_ptr<uint8_t>();
+  a.scales = b.scales.data_ptr<uint8_t>();
+  a.row_scale = b.row_scale.data_ptr<float>();
+  a.tiles = static_cast<int>(b.scales.size(1));
+  TORCH_CHECK(ecz::launch_block_norm(a, ecz::kNormBf16, true, static_cast<int>(fmt), ecz::device_sms(x.get_device()),
+                                     at::cuda::getCurrentCUDAStream()) == 0,
+              "block_norm: launch failed");
+  return {b.codes, b.scales, b.row_scale, stream};
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// A tensor that the forward pass saved is what it was: saved-tensor hooks may return anything, and kernels read it by its
+// pointer.
+void check_saved(const Tensor& x, const Tensor& like, at::ScalarType type, at::IntArrayRef sizes, const char* what) {
+  TORCH_CHECK(x.defined() && x.is_cuda() && x.get_device() == like.get_device() && x.scalar_type() == type &&
+                  x.sizes() == sizes && x.is_contiguous(),
+              "block_norm: the saved ", what, " did not come back as it was saved (device, type, sizes, contiguous)");
+}
+
+struct BlockNormFunction : torch::autograd::Function<BlockNormFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const c10::optional<Tensor>& residual_,
+                               const Tensor& weight, const c10::optional<Tensor>& post_,
+                               const c10::optional<Tensor>& gate_, double scale, double eps) {
+    const Tensor residual = value(residual_), post = value(post_), gate = value(gate_);
+    NormResult r = norm_forward(x, residual, weight, post, gate, scale, eps, true);
+    // without a norm behind the block and a gate the backward pass needs the stream alone: half of what x and the
+    // residual would be to read
+    const bool simple = !post.defined() && !gate.defined();
+    ctx->save_for_backward({simple ? Tensor() : x, simple ? Tensor() : residual, weight, post, gate,
+                            simple ? r.stream : Tensor(), r.inv_s, r.inv_x});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["residual"] = residual.defined();
+    ctx->set_materialize_grads(false);
+    return {r.normed, r.stream};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "block_norm cannot be differentiated twice");
+    const auto s = ctx->get_saved_variables();
+    const Tensor &weight = s[2], &post = s[3], &gate = s[4], &stream = s[5], &inv_s = s[6], &inv_x = s[7];
+    const double scale = ctx->saved_data["scale"].toDouble(), eps = ctx->saved_data["eps"].toDouble();
+    const bool simple = !post.defined() && !gate.defined();
+    size_t input = 0;  // tensors that were not given have no place among the inputs
+    auto needs = [&](bool given) { return given && ctx->needs_input_grad(input++); };
+    const bool need_x = needs(true), need_r = needs(ctx->saved_data["residual"].toBool()), need_w = needs(true);
+    const bool need_p = needs(post.defined()), need_g = needs(gate.defined());
+    variable_list out(7);
+    Tensor dn = grads[0], up = grads[1];
+    if (!dn.defined() && !up.defined()) return out;
+    const Tensor& like = dn.defined() ? dn : up;
+    const int64_t T = like.size(0), H = like.size(1);
+    if (simple) check_saved(stream, weight, weight.scalar_type(), {T, H}, "stream");
+    // the operands as in the forward pass (the stream in x's place where it alone was saved)
+    const NormOperands o = norm_operands(simple ? stream : s[0], simple ? Tensor() : s[1], weight, post, gate, scale, eps);
+    for (const Tensor* t : {&dn, &up})
+      TORCH_CHECK(!t->defined() || (t->is_cuda() && t->get_device() == o.x.get_device() &&
+                                    t->scalar_type() == o.x.scalar_type() && t->sizes() == o.x.sizes()),
+                  "block_norm: a gradient does not match its output");
+    check_saved(inv_s, o.x, at::kFloat, {T}, "norms");
+    check_saved(inv_x, o.x, at::kFloat, {post.defined() ? T : 0}, "norms of the block's output");
+    c10::cuda::CUDAGuard guard(o.x.device());
+    const auto opts = o.x.options();
+    const bool shared = simple && scale == 1.0;  // both gradients are the same values
+    Tensor dx, dr, dw, dp, dg;
+    if (need_x && !shared) dx = at::empty({T, H}, opts);
+    if (need_r || (need_x && shared)) dr = at::empty({T, H}, opts);
+    if (need_w) dw = at::empty({H}, opts);
+    if (need_p) dp = at::empty({H}, opts);
+    if (need_g) dg = at::empty(gate.sizes(), opts);
+    if (T == 0) {
+      if (need_w) dw.zero_();
+      if (need_p) dp.zero_();
+    } else {
+      if (dn.defined()) dn = rows_of(dn);
+      if (up.defined()) up = rows_of(up);
+      const bool vec = o.vec && aligned(dn) && aligned(up);
+      const ecz::NormType type = norm_type(o.x);
+      const int sms = ecz::device_sms(o.x.get_device());
+      ecz::BlockNormGrads a;
+      a.dnormed = ptr(dn);
+      a.dstream = ptr(up);
+      a.dn_stride = dn.defined() ? row_stride(dn) : 0;
+      a.ds_stride = up.defined() ? row_stride(up) : 0;
+      const ecz::BlockNormArgs f = norm_args(o, scale, eps);
+      a.x = f.x;
+      a.residual = f.residual;
+      a.stream = simple ? f.x : nullptr;
+      a.weight = f.weight;
+      a.post = f.post;
+      a.gate = f.gate;
+      a.x_stride = f.x_stride;
+      a.r_stride = f.r_stride;
+      a.gate_stride = f.gate_stride;
+      a.gate_mode = f.gate_mode;
+      a.inv_s = inv_s.data_ptr<float>();
+      a.inv_x = post.defined() ? inv_x.data_ptr<float>() : nullptr;
+      a.dx = const_cast<void*>(ptr(dx));
+      a.dresidual = const_cast<void*>(ptr(dr));
+      a.dgate = const_cast<void*>(ptr(dg));
+      a.dweight = const_cast<void*>(ptr(dw));
+      a.dpost = const_cast<void*>(ptr(dp));
+      a.rows = f.rows;
+      a.hidden = f.hidden;
+      a.scale = f.scale;
+      Tensor parts;
+      if (need_w || need_p) {
+        const int n = ecz::block_norm_parts(type, a.rows, a.hidden, vec, sms);
+        parts = at::empty({(need_w ? 1 : 0) + (need_p ? 1 : 0), n, H}, opts.dtype(at::kFloat));
+        float* p = parts.data_ptr<float>();
+        if (need_w) a.dw_part = p;
+        if (need_p) a.dpost_part = p + (need_w ? static_cast<int64_t>(n) * H : 0);
+      }
+      TORCH_CHECK(ecz::launch_block_norm_grads(a, type, vec, sms, at::cuda::getCurrentCUDAStream()) == 0,
+                  "block_norm: backward launch failed");
+    }
+    if (need_x) out[0] = shared ? dr : dx;
+    if (need_r) out[1] = dr;
+    if (need_w) out[2] = dw;
+    if (need_p) out[3] = dp;
+    if (need_g) out[4] = dg;
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor> block_norm(const Tensor& x, const c10::optional<Tensor>& residual, const Tensor& weight,
+                                      const c10::optional<Tensor>& post, const c10::optional<Tensor>& gate, double scale,
+                                      double eps) {
+  const Tensor r = value(residual), p = value(post), g = value(gate);
+  bool grad = false;
+  for (const Tensor* t : {&x, &r, &weight, &p, &g}) {
+    if (!t->defined()) continue;
+    grad |= t->requires_grad();
+    // the kernels carry no tangents: refused, or a dual number's would be dropped without a word
+    TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t->_fw_grad(0).defined(),
+                "block_norm has no forward-mode derivative on CUDA");
+  }
+  if (grad && at::GradMode::is_enabled()) {
+    auto given = [](const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; };
+    auto out = BlockNormFunction::apply(x, given(r), weight, given(p), given(g), scale, eps);
+    return {out[0], out[1]};
+  }
+  NormResult out = norm_forward(x, r, weight, p, g, scale, eps, false);
+  return {out.normed, out.stream};
+}
+
+}  // namespace
+
+namespace ecz {
+
+void bind_block(pybind11::module_& m) {
+  namespace py = pybind11;
+  m.def("fp4_quantize", &fp4_quantize, "bf16 rows as 4-bit codes with scales (fmt 1 nvfp4, 2 mxfp4)", py::arg("x"),
+        py::arg("fmt"));
+  m.def("fp4_dequantize", &fp4_dequantize, "the bf16 values of 4-bit codes", py::arg("codes"), py::arg("scales"),
+        py::arg("row_scale"), py::arg("fmt"));
+  m.def("fp4_matmul", &fp4_matmul, "product of two 4-bit operands (tcgen05 block-scaled MMA)", py::arg("x"),
+        py::arg("x_scales"), py::arg("x_row_scale"), py::arg("w"), py::arg("w_scales"), py::arg("w_row_scale"),
+        py::arg("fmt"));
+  m.def("linear_fp4", &linear_fp4, "bf16 activations quantised and multiplied with a 4-bit weight", py::arg("x"),
+        py::arg("w"), py::arg("w_scales"), py::arg("w_row_scale"), py::arg("fmt"));
+  m.def("block_norm", &block_norm, "norm after a block, gate, residual scale and sum, norm before the next (autograd)",
+        py::arg("x"), py::arg("residual"), py::arg("weight"), py::arg("post_weight"), py::arg("gate"), py::arg("scale"),
+        py::arg("eps"));
+  m.def("block_norm_fp4", &block_norm_fp4, "block_norm with its result in 4 bits", py::arg("x"), py::arg("residual"),
+        py::arg("weight"), py::arg("post_weight"), py::arg("gate"), py::arg("scale"), py::arg("eps"), py::arg("fmt"));
+}
+
+}  // namespace ecz

@@ -1,0 +1,338 @@
+// Products of 4-bit operands with block scales on tcgen05 (kind::mxf4nvf4 with e4m3 scales per 16 columns, kind::mxf4
+// with E8M0 scales per 32): Y[m, n] = rx[m] rw[n] sum_k (qx fx)[m, k] (qw fw)[n, k], fp32 sums, rounded to bf16 once.
+// The tensor cores multiply the scales in; rx and rw are the rows' powers of two of nvfp4. Layouts: fp4_common.cuh.
+//
+// gemm_fp4_kernel, for up to 128 rows of activations: weights are the MMA's 128 rows (A), activations its BN columns
+// (B), so a tile streams 128 rows of weights once. A K block is 256 columns (128 bytes of codes a row, one swizzle row).
+//
+//   warp 0      TMA: codes of the weights [128 x 128 B] and of the activations [BN x 128 B], both blocks' scales as bulk
+//               copies
+//   warp 1      copies a block's scales to tensor memory (tcgen05.cp, in one of kSlots places, reused once the MMAs that
+//               read it have completed) and issues its four MMAs of 64 columns
+//   warps 2-5   epilogue: TMEM lane = output feature
+//
+// Few tiles are split along K over the CTAs of a cluster; the partial sums are added up through distributed shared
+// memory in the order of the splits.
+#include <algorithm>
+
+#include "fp4_common.cuh"
+#include "launchers.h"
+
+namespace ecz {
+
+namespace {
+
+using namespace fp4;
+
+constexpr int kBM = 128;
+constexpr int kRowBytes = kBlockK / 2;  // a K block of codes
+constexpr int kABytes = kBM * kRowBytes;
+constexpr int kThreads = 192;
+constexpr int kSlots = 3;  // places for scales in tensor memory
+
+// Instruction descriptor of the block-scaled kinds: e2m1 operands, K-major, shape m x n, scales of type e4m3 (nvfp4) or
+// E8M0 (mxfp4); sf: which bytes of the 32-bit scale words the MMA's two scales per row are (kind::mxf4: 0 or 2).
+template <int FMT>
+__host__ __device__ constexpr uint32_t idesc_fp4(int m, int n, int sf = 0) {
+  return (static_cast<uint32_t>(sf) << 4)          // scale id of B
+         | (1u << 7) | (1u << 10)                  // A, B: e2m1
+         | (static_cast<uint32_t>(n >> 3) << 17)   // N >> 3
+         | ((FMT == kMx ? 1u : 0u) << 23)          // scale type
+         | (static_cast<uint32_t>(m >> 7) << 27)   // M >> 7
+         | (static_cast<uint32_t>(sf) << 29);      // scale id of A
+}
+
+template <int FMT>
+__device__ __forceinline__ void umma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         uint32_t accumulate) {
+  if constexpr (FMT == kNv) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  }
+}
+
+// 512 bytes of scales (32 rows of 16 bytes) to four TMEM columns, the same in all four groups of 32 lanes.
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// Descriptor of such a tile: no swizzle, 8-row groups of 16-byte rows 128 bytes apart.
+__device__ __forceinline__ uint64_t desc_scales(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128u >> 4) << 32) |
+         (static_cast<uint64_t>(1u) << 46);
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+__device__ __forceinline__ float ld_dsmem(uint32_t local_addr, uint32_t rank) {
+  uint32_t remote;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local_addr), "r"(rank));
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void wait_ns(unsigned long long ns) {
+  const unsigned long long start = global_timer_ns();
+  while (global_timer_ns() - start < ns) {
+  }
+}
+
+template <int FMT, int BN>
+struct Cfg {
+  static constexpr int kBBytes = BN * kRowBytes;
+  static constexpr int kScaleBytes = Format<FMT>::kBlockBytes;
+  static constexpr int kStageBytes = kABytes + kBBytes + 2 * kScaleBytes;
+  static constexpr int kOcc = BN <= 64 ? 2 : 1;
+  static constexpr int kStages = std::min(8, (kOcc == 2 ? 104 : 200) * 1024 / kStageBytes);
+  static constexpr int kSmem = kStages * kStageBytes + 1024 + 256;
+  static constexpr int kAccCols = BN < 32 ? 32 : BN;
+  static constexpr int kSlotCols = 2 * 4 * Format<FMT>::kTilesPerBlock;
+  static constexpr int kCols = kAccCols + kSlots * kSlotCols;
+  static constexpr int kTmemCols = kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+  static_assert(kStages >= kSlots, "a slot of scales is waited for by its stage's barrier");
+  static_assert(kStages * kStageBytes >= BN * kBM * 4, "the partial sums reuse the stages");
+};
+
+struct Fp4Args {
+  const uint8_t* w_scales;
+  const uint8_t* x_scales;
+  const float* w_row;  // nvfp4
+  const float* x_row;
+  bf16* y;
+  int M, N, kblocks, per_split;
+  unsigned* status;
+};
+
+template <int FMT, int BN>
+__global__ void __launch_bounds__(kThreads, Cfg<FMT, BN>::kOcc)
+    gemm_fp4_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                    const __grid_constant__ Fp4Args args) {
+  using C = Cfg<FMT, BN>;
+  constexpr int S = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* a_tiles = smem;
+  uint8_t* b_tiles = a_tiles + S * kABytes;
+  uint8_t* sa_tiles = b_tiles + S * C::kBBytes;
+  uint8_t* sb_tiles = sa_tiles + S * C::kScaleBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sb_tiles + S * C::kScaleBytes);
+  uint64_t* empty = full + S;
+  uint64_t* acc_full = empty + S;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n0 = blockIdx.x * kBM, m0 = blockIdx.y * BN, split = blockIdx.z, splits = gridDim.z;
+  const int kb0 = split * args.per_split;
+  const int nkb = max(0, min(args.per_split, args.kblocks - kb0));
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_w);
+    tma_prefetch_desc(&tm_x);
+  }
+  __syncwarp();
+  if (warp == 0) tmem_alloc(tmem_slot, C::kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0 && lane == 0) {
+    const size_t wide = static_cast<size_t>(args.kblocks) * C::kScaleBytes;  // scales of 128 rows
+    const uint8_t* ws = args.w_scales + (n0 / kBM) * wide;
+    const uint8_t* xs = args.x_scales + (m0 / 128) * wide;
+    auto weights = [&](int kb) {
+      const int s = kb % S, k = kb0 + kb;
+      mbar_arrive_expect_tx(&full[s], C::kStageBytes);
+      tma_load_2d(a_tiles + s * kABytes, &tm_w, &full[s], k * kRowBytes, n0);
+      bulk_load(sa_tiles + s * C::kScaleBytes, ws + static_cast<size_t>(k) * C::kScaleBytes, C::kScaleBytes, &full[s]);
+    };
+    auto activations = [&](int kb) {
+      const int s = kb % S, k = kb0 + kb;
+      tma_load_2d(b_tiles + s * C::kBBytes, &tm_x, &full[s], k * kRowBytes, m0);
+      bulk_load(sb_tiles + s * C::kScaleBytes, xs + static_cast<size_t>(k) * C::kScaleBytes, C::kScaleBytes, &full[s]);
+    };
+    // the weights do not come from the previous kernel: what fits is fetched before it ends
+    const int pre = min(nkb, S);
+    for (int kb = 0; kb < pre; ++kb) weights(kb);
+    pdl_wait();
+    for (int kb = 0; kb < pre; ++kb) activations(kb);
+    for (int kb = pre; kb < nkb; ++kb) {
+      const int s = kb % S;
+      if (!mbar_wait(&empty[s], ((kb / S) & 1u) ^ 1u, args.status, kStatusWaitEmpty, abort_flag)) break;
+      weights(kb);
+      activations(kb);
+    }
+  } else if (warp == 1 && lane == 0) {
+    for (int kb = 0; kb < nkb; ++kb) {
+      const int s = kb % S;
+      if (kb >= kSlots) {  // the MMAs that read this slot's last scales have completed
+        const int old = kb - kSlots;
+        if (!mbar_wait(&empty[old % S], (old / S) & 1u, args.status, kStatusWaitAccum, abort_flag)) break;
+      }
+      if (!mbar_wait(&full[s], (kb / S) & 1u, args.status, kStatusWaitFull, abort_flag)) break;
+      tc_fence_after();
+      const uint32_t sfa = tmem + C::kAccCols + (kb % kSlots) * C::kSlotCols;
+      const uint32_t sfb = sfa + 4 * Format<FMT>::kTilesPerBlock;
+      const uint32_t sa = smem_u32(sa_tiles + s * C::kScaleBytes), sb = smem_u32(sb_tiles + s * C::kScaleBytes);
+#pragma unroll
+      for (int t = 0; t < Format<FMT>::kTilesPerBlock; ++t) {
+        copy_scales(sfa + 4 * t, desc_scales(sa + t * kTileBytes));
+        copy_scales(sfb + 4 * t, desc_scales(sb + t * kTileBytes));
+      }
+      const uint32_t a = smem_u32(a_tiles + s * kABytes), b = smem_u32(b_tiles + s * C::kBBytes);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        const int t = FMT == kNv ? kk : kk / 2;
+        const uint32_t idesc = FMT == kNv ? idesc_fp4<FMT>(kBM, BN) : idesc_fp4<FMT>(kBM, BN, (kk & 1) * 2);
+        umma_fp4<FMT>(tmem, desc_kmajor_sw128(a + kk * 32), desc_kmajor_sw128(b + kk * 32), idesc, sfa + 4 * t,
+                      sfb + 4 * t, (kb | kk) != 0 ? 1u : 0u);
+      }
+      umma_commit(&empty[s]);
+    }
+    umma_commit(acc_full);
+  }
+  __syncwarp();
+  pdl_wait();
+  if (warp < 2 && *abort_flag) wait_ns(1000000);  // a wait gave up: copies in flight get time to land
+  bool ok = true;
+  const int quarter = warp & 3;
+  const int n = n0 + quarter * 32 + lane;
+  const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  if (warp >= 2) {
+    ok = mbar_wait(acc_full, 0, args.status, kStatusWaitAccum, abort_flag);
+    ok = __all_sync(0xffffffffu, ok) && !*abort_flag;
+    tc_fence_after();
+  }
+  const float rw = FMT == kNv && n < args.N ? args.w_row[n] : 1.f;
+  auto store = [&](int j, float v) {
+    const int m = m0 + j;
+    if (m < args.M && n < args.N) {
+      const float rx = FMT == kNv ? args.x_row[m] : 1.f;
+      args.y[static_cast<size_t>(m) * args.N + n] = __float2bfloat16(v * (rw * rx));
+    }
+  };
+  if (splits == 1) {
+    if (warp >= 2 && ok) {
+#pragma unroll
+      for (int c = 0; c < BN; c += 16) {
+        if (m0 + c < args.M) {
+          float v[16];
+          tmem_ld16(taddr + c, v);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) store(c + j, v[j]);
+        }
+      }
+    }
+  } else {
+    // this CTA's sums [BN][128] where its stages were (every copy has landed and was read), then a share of the columns
+    float* part = reinterpret_cast<float*>(smem);
+    if (warp >= 2) {
+#pragma unroll
+      for (int c = 0; c < BN; c += 16) {
+        if (m0 + c < args.M) {
+          float v[16];
+          if (ok && nkb > 0) tmem_ld16(taddr + c, v);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) part[(c + j) * kBM + quarter * 32 + lane] = ok && nkb > 0 ? v[j] : 0.f;
+        }
+      }
+    }
+    cluster_sync();
+    if (warp >= 2) {
+      const uint32_t at = smem_u32(part) + (quarter * 32 + lane) * 4;
+      for (int j = split; j < BN && m0 + j < args.M; j += splits) {
+        float sum = 0.f;
+        for (int r = 0; r < splits; ++r) sum += ld_dsmem(at + j * kBM * 4, r);
+        store(j, sum);
+      }
+    }
+    cluster_sync();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, C::kTmemCols);
+}
+
+template <int FMT, int BN>
+int run(const CUtensorMap& w, const CUtensorMap& x, Fp4Args args, int splits, cudaStream_t stream) {
+  using C = Cfg<FMT, BN>;
+  auto kernel = gemm_fp4_kernel<FMT, BN>;
+  if (set_max_smem(kernel, C::kSmem) != cudaSuccess) return -1;
+  args.per_split = (args.kblocks + splits - 1) / splits;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((args.N + kBM - 1) / kBM, (args.M + BN - 1) / BN, splits);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = splits;
+  cfg.attrs = attr;
+  cfg.numAttrs = splits > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, w, x, args) == cudaSuccess ? 0 : -1;
+}
+
+template <int FMT>
+int run_fmt(const CUtensorMap& w, const CUtensorMap& x, const Fp4Args& args, int bn, int splits, cudaStream_t stream) {
+  switch (bn) {
+    case 16: return run<FMT, 16>(w, x, args, splits, stream);
+    case 32: return run<FMT, 32>(w, x, args, splits, stream);
+    case 64: return run<FMT, 64>(w, x, args, splits, stream);
+    default: return run<FMT, 128>(w, x, args, splits, stream);
+  }
+}
+
+}  // namespace
+
+int fp4_block_rows(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128; }
+
+int launch_gemm_fp4(const CUtensorMap* w, const CUtensorMap* x, const void* w_scales, const void* x_scales,
+                    const float* w_row, const float* x_row, int fmt, void* y, int M, int N, int K, int sms,
+                    unsigned* status, cudaStream_t stream) {
+  if (M < 1 || N < 1 || K < 32 || K % 32 != 0 || K > kFp4MaxK) return -1;
+  Fp4Args args{};
+  args.w_scales = static_cast<const uint8_t*>(w_scales);
+  args.x_scales = static_cast<const uint8_t*>(x_scales);
+  args.w_row = w_row;
+  args.x_row = x_row;
+  args.y = static_cast<bf16*>(y);
+  args.M = M;
+  args.N = N;
+  args.kblocks = (K + kBlockK - 1) / kBlockK;
+  args.status = status;
+  const int bn = fp4_block_rows(M);
+  // splits by the weights' size alone, so that a row's sums do not depend on how many rows there are
+  const int tiles = (N + kBM - 1) / kBM;
+  int splits = 1;
+  while (splits < 8 && tiles * splits < sms && 2 * splits <= args.kblocks) splits *= 2;
+  return fmt == kNv ? run_fmt<kNv>(*w, *x, args, bn, splits, stream) : run_fmt<kMx>(*w, *x, args, bn, splits, stream);
+}
+
+}  // namespace ecz

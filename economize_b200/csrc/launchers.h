@@ -224,6 +224,74 @@ int grouped_block_n(int rows, int E);
 int launch_gemm_grouped(const CUtensorMap* tm_w, const CUtensorMap* tm_x, void* y, const int* offsets, int E,
                         int rows, int N, int K, unsigned* status, cudaStream_t stream);
 
+// fp4.cu: bf16 rows to 4-bit codes with scales per group and back (fmt 1 nvfp4, 2 mxfp4; layouts in fp4_common.cuh).
+// codes [rows, K / 2], scales [ceil(rows / 128), fp4_scale_tiles, 512], row_scale fp32 [rows] (nvfp4). early: the next
+// kernel may start before this one ends (it must then not read the result before its griddepcontrol.wait).
+constexpr int kFp4MaxK = 65536;
+int fp4_scale_tiles(int fmt, int K);
+int launch_fp4_quantize(const void* x, size_t x_stride, int fmt, void* codes, void* scales, float* row_scale, int rows,
+                        int K, bool early, int sms, cudaStream_t stream);
+int launch_fp4_dequantize(const void* codes, const void* scales, const float* row_scale, int fmt, void* out, int rows,
+                          int K, int sms, cudaStream_t stream);
+
+// gemm_fp4.cu: Y[M, N] = X . W^T of 4-bit operands. w / x: tensor maps over the codes as bytes ([N, K / 2] in boxes of
+// {128, 128}, [M, K / 2] in boxes of {128, fp4_block_rows(M)}, 128-byte swizzle).
+int fp4_block_rows(int M);
+int launch_gemm_fp4(const CUtensorMap* w, const CUtensorMap* x, const void* w_scales, const void* x_scales,
+                    const float* w_row, const float* x_row, int fmt, void* y, int M, int N, int K, int sms,
+                    unsigned* status, cudaStream_t stream);
+
+// block_norm.cu: norm after a block, gate, residual scale and sum, norm before the next block (see the file comment).
+// Strides in elements between rows; outputs are contiguous. vec: every operand allows 16-byte vectors.
+enum NormType { kNormBf16 = 0, kNormFp16 = 1, kNormFp32 = 2 };
+enum GateMode { kGateNone = 0, kGateToken = 1, kGateFull = 2 };
+constexpr int kBlockNormMaxHidden = 16384;
+struct BlockNormArgs {
+  const void* x = nullptr;
+  const void* residual = nullptr;  // or null
+  const void* weight = nullptr;
+  const void* post = nullptr;      // or null
+  const void* gate = nullptr;
+  int64_t x_stride = 0, r_stride = 0, gate_stride = 0;
+  int gate_mode = 0;
+  void* normed = nullptr;
+  void* stream = nullptr;
+  float* inv_s = nullptr;  // saved for the backward pass, or null
+  float* inv_x = nullptr;
+  uint8_t* codes = nullptr;  // normed in 4 bits
+  uint8_t* scales = nullptr;
+  float* row_scale = nullptr;
+  int tiles = 0;
+  int rows = 0, hidden = 0;
+  float scale = 1.f, eps = 0.f;
+};
+struct BlockNormGrads {
+  const void* dnormed = nullptr;  // or null: no gradient
+  const void* dstream = nullptr;  // or null
+  const void* x = nullptr;
+  const void* residual = nullptr;
+  const void* stream = nullptr;  // without post norm and gate: the rounded stream in place of x and residual
+  const void* weight = nullptr;
+  const void* post = nullptr;
+  const void* gate = nullptr;
+  const float* inv_s = nullptr;
+  const float* inv_x = nullptr;
+  int64_t dn_stride = 0, ds_stride = 0, x_stride = 0, r_stride = 0, gate_stride = 0;
+  int gate_mode = 0;
+  void* dx = nullptr;  // outputs, those that are not null
+  void* dresidual = nullptr;
+  void* dgate = nullptr;
+  void* dweight = nullptr;
+  void* dpost = nullptr;
+  float* dw_part = nullptr;  // fp32 [block_norm_parts, hidden]
+  float* dpost_part = nullptr;
+  int rows = 0, hidden = 0;
+  float scale = 1.f;
+};
+int launch_block_norm(const BlockNormArgs& args, NormType type, bool vec, int fmt, int sms, cudaStream_t stream);
+int block_norm_parts(NormType type, int rows, int hidden, bool vec, int sms);
+int launch_block_norm_grads(const BlockNormGrads& args, NormType type, bool vec, int sms, cudaStream_t stream);
+
 // gemm_fp8.cu: block-scaled fp8 GEMM (e4m3 weights [N, K] with fp32 scales [N / 128, K / 128]; activations
 // quantised per token and 128-wide K block by launch_act_quant_fp8 into codes [M, K] and scales [K / 128, >= M]).
 int fp8_block_n(int M);

@@ -11,10 +11,12 @@ import torch
 
 from . import reference
 from ._ext import available, load_error, require
+from .fp4 import FP4Tensor, FP4Weight
+from .fp4 import quantize as fp4_quantize
 from .fp8 import FP8BlockWeight
 from .quant import QWeight
 from .sparse import Sparse24Weight
-from .training import linear_cross_entropy, packed_attention
+from .training import block_norm, linear_cross_entropy, packed_attention
 
 __all__ = [
     "argmax",
@@ -22,6 +24,10 @@ __all__ = [
     "attention_scores",
     "attention_usage",
     "available",
+    "block_norm",
+    "FP4Tensor",
+    "FP4Weight",
+    "fp4_quantize",
     "greedy_accept",
     "kivi_quantize",
     "kv_compact",
@@ -270,8 +276,9 @@ def glu(gate_up: torch.Tensor | Partials, act: str = "silu", limit: float = 7.0,
 
 
 def linear(x: torch.Tensor, weight, bias: torch.Tensor | None = None) -> torch.Tensor:
-    """``x @ weight.T (+ bias)``; on CUDA the tcgen05/TMA GEMM of ``csrc/gemm_tc.cu``, or for a quantized
-    :class:`~economize_b200.ops.quant.QWeight` the weight-only GEMM of ``csrc/gemm_wq.cu``."""
+    """``x @ weight.T (+ bias)``; on CUDA the tcgen05/TMA GEMM of ``csrc/gemm_tc.cu``, for a quantized
+    :class:`~economize_b200.ops.quant.QWeight` the weight-only GEMM of ``csrc/gemm_wq.cu``, and for an
+    :class:`~economize_b200.ops.fp4.FP4Weight` the 4-bit GEMM of ``csrc/gemm_fp4.cu`` (``x`` bf16, or in 4 bits)."""
     if isinstance(weight, (QWeight, FP8BlockWeight, Sparse24Weight)) or hasattr(weight, "linear"):
         y = weight.linear(x)
         return y if bias is None else y + bias

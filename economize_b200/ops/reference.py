@@ -13,6 +13,7 @@ import torch.nn.functional as F
 
 __all__ = [
     "attention",
+    "block_norm",
     "ngram",
     "rejection",
     "sample",
@@ -35,6 +36,23 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float,
     h = summed.float()
     h = h * torch.rsqrt(h.pow(2).mean(-1, keepdim=True) + eps)
     return weight * h.to(x.dtype), summed
+
+
+def block_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, post: torch.Tensor | None,
+               gate: torch.Tensor | None, scale: float, eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(normed, stream)`` of :func:`economize_b200.ops.block_norm`, in fp32 (fp64 for fp64 operands) and rounded to
+    ``x.dtype`` at the end."""
+    def wide(t):
+        return t if t.dtype == torch.float64 else t.float()
+
+    branch = wide(x)
+    if post is not None:
+        branch = branch * torch.rsqrt(branch.pow(2).mean(-1, keepdim=True) + eps) * wide(post)
+    if gate is not None:
+        branch = branch * wide(gate)
+    stream = branch * scale if residual is None else wide(residual) + scale * branch
+    normed = stream * torch.rsqrt(stream.pow(2).mean(-1, keepdim=True) + eps) * wide(weight)
+    return normed.to(x.dtype), stream.to(x.dtype)
 
 
 def _rotate(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:

@@ -1,19 +1,26 @@
-"""Operators of training steps, with autograd: the readout cross-entropy and causal attention over packed documents.
+"""Operators of training steps, with autograd: the readout cross-entropy, causal attention over packed documents, and
+the norms around a block (which inference uses too).
 
-On CUDA both directions are the hand-written kernels of ``csrc/readout.cu``, ``csrc/packed_attention.cu`` and
-``csrc/packed_attention_bwd.cu`` (autograd functions in ``csrc/bindings_train.cpp``); CPU tensors take the formulas of
-:mod:`.reference`, which autograd differentiates in either mode and any number of times. The kernels have the first
-reverse-mode derivative: dual tensors and ``create_graph=True`` are refused on CUDA. There is no third path.
+On CUDA both directions are the hand-written kernels of ``csrc/readout.cu``, ``csrc/packed_attention.cu``,
+``csrc/packed_attention_bwd.cu`` and ``csrc/block_norm.cu`` (autograd functions in ``csrc/bindings_train.cpp`` and
+``csrc/bindings_block.cpp``); CPU tensors take the formulas of :mod:`.reference`, which autograd differentiates in either mode and any
+number of times. The kernels have the first reverse-mode derivative: dual tensors and ``create_graph=True`` are refused
+on CUDA. There is no third path.
 """
 
 from __future__ import annotations
 
+import math
+
 import torch
 
+from ..errors import ConfigError
 from . import reference
 from ._ext import require
+from .fp4 import FORMATS, FP4Tensor
+from .fp4 import quantize as fp4_quantize
 
-__all__ = ["linear_cross_entropy", "packed_attention"]
+__all__ = ["block_norm", "linear_cross_entropy", "packed_attention"]
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
@@ -88,3 +95,60 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     if not q.is_cuda:
         return reference.packed_attention(q, k, v, cu_seqlens, scale)
     return require().packed_attention(q, k, v, cu_seqlens, scale)
+
+
+def block_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, *,
+               post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None, scale: float = 1.0,
+               eps: float = 1e-6, quantize: str | None = None) -> tuple[torch.Tensor | FP4Tensor, torch.Tensor]:
+    """The norms on both sides of a block's end, its gate, residual scale and residual sum in one pass: ``(normed,
+    stream)`` with ``stream = residual + scale * gate * rms(x) * post_weight`` and ``normed = rms(stream) * weight``, where
+    ``rms(v) = v / sqrt(mean(v^2) + eps)`` over the last dimension. Differentiable in every tensor.
+
+    Args:
+        x: The block's output ``[..., H]`` (``H`` up to 16384; bf16, fp16 or fp32 on CUDA, rows may be strided).
+        residual: The stream that enters the block, like ``x``; ``None``: nothing is added.
+        weight: Of the norm before the next block, ``[H]``.
+        post_weight: Of the norm behind the block, ``[H]``; ``None``: no such norm.
+        gate: Per token ``[..., 1]`` or per element ``[..., H]``; ``None``: ungated.
+        scale: Factor of what joins the residual.
+        quantize: ``"nvfp4"`` or ``"mxfp4"``: ``normed`` comes in 4 bits, as an
+            :class:`~economize_b200.ops.fp4.FP4Tensor` of the bf16 result (bf16 on CUDA, ``H`` a multiple of 32; no
+            gradients).
+
+    All operands have one type (under bf16 autocast they are cast). Sums and what lies between are fp32; ``stream`` and
+    ``normed`` are rounded once each, so ``normed`` is the norm of the unrounded stream (unlike two calls of
+    :func:`~economize_b200.ops.rmsnorm`, which round in between as Hugging Face's modules do). Without ``post_weight`` and
+    ``gate`` the gradients are taken from the rounded stream, and with ``scale=1`` those of ``x`` and ``residual`` are one
+    tensor.
+    """
+    given = [t for t in (x, residual, weight, post_weight, gate) if t is not None]
+    given = _autocast(*given)
+    it = iter(given)
+    x, residual, weight, post_weight, gate = (None if t is None else next(it)
+                                              for t in (x, residual, weight, post_weight, gate))
+    if x.dim() < 1 or weight.dim() != 1 or x.shape[-1] != weight.shape[0]:
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
+    if post_weight is not None and post_weight.shape != weight.shape:
+        raise ValueError(f"post_weight {tuple(post_weight.shape)} and weight {tuple(weight.shape)} do not match")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
+    if gate is not None and gate.shape not in (x.shape, (*x.shape[:-1], 1)):
+        raise ValueError(f"gate {tuple(gate.shape)} must be {(*x.shape[:-1], 1)} or {tuple(x.shape)}")
+    if any(t.dtype != x.dtype or t.device != x.device for t in given):
+        raise ValueError("all operands must have one type and device, got "
+                         + ", ".join(f"{t.dtype} on {t.device}" for t in given))
+    if not x.is_floating_point() or not math.isfinite(scale) or not 0.0 <= eps < math.inf:
+        raise ValueError(f"block_norm takes floating point and a finite scale and eps >= 0, got {x.dtype}, {scale}, {eps}")
+    if quantize is not None and quantize not in FORMATS:
+        raise ConfigError(f"unknown 4-bit format {quantize!r} (one of {', '.join(FORMATS)})")
+    shape = x.shape
+    if x.is_cuda:
+        flat = [None if t is None else t if t.dim() == 2 else t.reshape(-1, t.shape[-1]) for t in (x, residual, gate)]
+        if quantize is not None:
+            *parts, stream = require().block_norm_fp4(flat[0], flat[1], weight, post_weight, flat[2], float(scale),
+                                                      float(eps), FORMATS[quantize])
+            return FP4Tensor(*parts, quantize, shape), stream.reshape(shape)
+        normed, stream = require().block_norm(flat[0], flat[1], weight, post_weight, flat[2], float(scale), float(eps))
+        return (normed, stream) if len(shape) == 2 else (normed.reshape(shape), stream.reshape(shape))
+    normed, stream = reference.block_norm(x, residual, weight, post_weight, gate, float(scale), float(eps))
+    return (normed, stream) if quantize is None else (fp4_quantize(normed, quantize), stream.detach())
