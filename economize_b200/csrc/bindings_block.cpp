@@ -97,8 +97,9 @@ void check_operand(const Tensor& codes, const Tensor& scales, const Tensor& row_
   if (fmt == 1) {
     TORCH_CHECK(row_scale.is_cuda() && row_scale.get_device() == ref.get_device() &&
                     row_scale.scalar_type() == at::kFloat && row_scale.dim() == 1 &&
-                    row_scale.size(0) == codes.size(0) && row_scale.is_contiguous(),
-                what, ": nvfp4 has an fp32 scale per row");
+                    row_scale.size(0) == codes.size(0) && row_scale.is_contiguous() &&
+                    reinterpret_cast<uintptr_t>(row_scale.data_ptr()) % 16 == 0,
+                what, ": nvfp4 has an fp32 scale per row, on a 16-byte boundary");
   }
   TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0 &&
                   reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0,
@@ -129,6 +130,15 @@ CUtensorMap codes_map(const Tensor& codes, int box_rows) {
   return map;
 }
 
+// Scales as rows of 128 bytes, one box the K block of 128 rows.
+CUtensorMap scales_map(const Tensor& scales, int64_t fmt) {
+  CUtensorMap map;
+  std::memset(&map, 0, sizeof(map));
+  const int rc = ecz::make_tmap_2d(&map, 1, scales.data_ptr(), scales.numel() / 128, 128, 128, 128, fmt == 1 ? 16 : 8, 0);
+  TORCH_CHECK(rc == 0, "cuTensorMapEncodeTiled failed (code ", rc, ") for scales ", scales.sizes());
+  return map;
+}
+
 // Y [M, N] of two operands [M, K] and [N, K] of one format.
 Tensor fp4_matmul(const Tensor& x, const Tensor& xs, const Tensor& xr, const Tensor& w, const Tensor& ws, const Tensor& wr,
                   int64_t fmt) {
@@ -141,12 +151,21 @@ Tensor fp4_matmul(const Tensor& x, const Tensor& xs, const Tensor& xr, const Ten
   const int64_t M = x.size(0), N = w.size(0), K = 2 * x.size(1);
   Tensor y = at::empty({M, N}, x.options().dtype(at::kBFloat16));
   if (M == 0) return y;
-  const CUtensorMap tw = codes_map(w, 128), tx = codes_map(x, ecz::fp4_block_rows(static_cast<int>(M)));
-  const int rc = ecz::launch_gemm_fp4(&tw, &tx, ws.data_ptr(), xs.data_ptr(), fmt == 1 ? wr.data_ptr<float>() : nullptr,
-                                      fmt == 1 ? xr.data_ptr<float>() : nullptr, static_cast<int>(fmt), y.data_ptr(),
-                                      static_cast<int>(M), static_cast<int>(N), static_cast<int>(K),
-                                      ecz::device_sms(x.get_device()), ecz::device_status(x.device()),
-                                      at::cuda::getCurrentCUDAStream());
+  const float* xr_ = fmt == 1 ? xr.data_ptr<float>() : nullptr;
+  const float* wr_ = fmt == 1 ? wr.data_ptr<float>() : nullptr;
+  const int sms = ecz::device_sms(x.get_device()), m = static_cast<int>(M), n = static_cast<int>(N), k = static_cast<int>(K);
+  unsigned* status = ecz::device_status(x.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  int rc;
+  if (M > 128) {
+    const CUtensorMap tx = codes_map(x, 128), tw = codes_map(w, 128), sx = scales_map(xs, fmt), sw = scales_map(ws, fmt);
+    rc = ecz::launch_gemm_fp4_pair(&tx, &tw, &sx, &sw, xr_, wr_, static_cast<int>(fmt), y.data_ptr(), m, n, k, sms, status,
+                                   stream);
+  } else {
+    const CUtensorMap tw = codes_map(w, 128), tx = codes_map(x, ecz::fp4_block_rows(m));
+    rc = ecz::launch_gemm_fp4(&tw, &tx, ws.data_ptr(), xs.data_ptr(), wr_, xr_, static_cast<int>(fmt), y.data_ptr(), m, n,
+                              k, sms, status, stream);
+  }
   TORCH_CHECK(rc == 0, "fp4_matmul: launch failed");
   return y;
 }

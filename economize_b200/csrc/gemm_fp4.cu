@@ -30,18 +30,6 @@ constexpr int kABytes = kBM * kRowBytes;
 constexpr int kThreads = 192;
 constexpr int kSlots = 3;  // places for scales in tensor memory
 
-// Instruction descriptor of the block-scaled kinds: e2m1 operands, K-major, shape m x n, scales of type e4m3 (nvfp4) or
-// E8M0 (mxfp4); sf: which bytes of the 32-bit scale words the MMA's two scales per row are (kind::mxf4: 0 or 2).
-template <int FMT>
-__host__ __device__ constexpr uint32_t idesc_fp4(int m, int n, int sf = 0) {
-  return (static_cast<uint32_t>(sf) << 4)          // scale id of B
-         | (1u << 7) | (1u << 10)                  // A, B: e2m1
-         | (static_cast<uint32_t>(n >> 3) << 17)   // N >> 3
-         | ((FMT == kMx ? 1u : 0u) << 23)          // scale type
-         | (static_cast<uint32_t>(m >> 7) << 27)   // M >> 7
-         | (static_cast<uint32_t>(sf) << 29);      // scale id of A
-}
-
 template <int FMT>
 __device__ __forceinline__ void umma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                          uint32_t accumulate) {
@@ -63,12 +51,6 @@ __device__ __forceinline__ void umma_fp4(uint32_t d, uint64_t a, uint64_t b, uin
 // 512 bytes of scales (32 rows of 16 bytes) to four TMEM columns, the same in all four groups of 32 lanes.
 __device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-
-// Descriptor of such a tile: no swizzle, 8-row groups of 16-byte rows 128 bytes apart.
-__device__ __forceinline__ uint64_t desc_scales(uint32_t addr) {
-  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128u >> 4) << 32) |
-         (static_cast<uint64_t>(1u) << 46);
 }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
