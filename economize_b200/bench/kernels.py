@@ -397,10 +397,82 @@ def bench_readout(a) -> None:
             4 * (a.m + a.n) * a.k, 6 * a.m * a.n * a.k, time_call(library, a.iters, a.warmup).median_ms)
 
 
+def bench_fp4(a) -> None:
+    """The W4A4 product with the quantisation of its activations, and without, against the library's bf16 product."""
+    from .. import ops
+    from ..ops.fp4 import FP4Weight
+
+    dev = torch.device("cuda")
+    n_copies = 1 if a.once else _copies(a.n * a.k // 2)
+    ws = [FP4Weight.from_weight((torch.randn(a.n, a.k, device=dev) * 0.02).bfloat16(), a.fmt) for _ in range(n_copies)]
+    x = torch.randn(a.m, a.k, device=dev).bfloat16()
+    q = ops.fp4_quantize(x, a.fmt)
+    if a.once:
+        ops.linear(x, ws[0])
+        torch.cuda.synchronize()
+        return
+    whole = time_graph([lambda w=w: ops.linear(x, w) for w in ws], a.iters, a.warmup)
+    product = time_graph([lambda w=w: ops.linear(q, w) for w in ws], a.iters, a.warmup)
+    dense = [w.dequantize() for w in ws[:2]]
+    library = time_graph([lambda w=w: torch.nn.functional.linear(x, w) for w in dense], a.iters, a.warmup)
+    nbytes = ws[0].nbytes() + 2 * a.m * (a.k + a.n)
+    for name, ms in (("fp4_linear", whole), ("fp4_product", product)):
+        _report(name, {"M": a.m, "N": a.n, "K": a.k, "fmt": a.fmt}, ms, nbytes, 2 * a.m * a.n * a.k, library)
+
+
+def bench_fp4_quantize(a) -> None:
+    from .. import ops
+
+    dev = torch.device("cuda")
+    xs = [torch.randn(a.m, a.k, device=dev).bfloat16() for _ in range(1 if a.once else _copies(2 * a.m * a.k))]
+    if a.once:
+        ops.fp4_quantize(xs[0], a.fmt).dequantize()
+        torch.cuda.synchronize()
+        return
+    qs = [ops.fp4_quantize(x, a.fmt) for x in xs]
+    stored = qs[0].nbytes()
+    ms = time_graph([lambda x=x: ops.fp4_quantize(x, a.fmt) for x in xs], a.iters, a.warmup)
+    _report("fp4_quantize", {"M": a.m, "K": a.k, "fmt": a.fmt}, ms, 2 * a.m * a.k + stored, a.m * a.k)
+    ms = time_graph([lambda q=q: q.dequantize() for q in qs], a.iters, a.warmup)
+    _report("fp4_dequantize", {"M": a.m, "K": a.k, "fmt": a.fmt}, ms, 2 * a.m * a.k + stored, a.m * a.k)
+
+
+def bench_block_norm(a) -> None:
+    """The norms around a block (``--post``: with the one behind it), forward, in 4 bits, and with all gradients."""
+    from .. import ops
+
+    dev = torch.device("cuda")
+    x, r = (torch.randn(a.m, a.k, device=dev).bfloat16().requires_grad_() for _ in range(2))
+    w, p = (torch.ones(a.k, device=dev).bfloat16().requires_grad_() for _ in range(2))
+    post = p if a.post else None
+    dn, ds = (torch.randn(a.m, a.k, device=dev).bfloat16() for _ in range(2))
+    leaves = [x, r, w] + ([p] if a.post else [])
+
+    def forward(**kw):
+        with torch.no_grad():
+            return ops.block_norm(x, r, w, post_weight=post, **kw)
+
+    def both():
+        return torch.autograd.grad(ops.block_norm(x, r, w, post_weight=post), leaves, (dn, ds))
+
+    if a.once:
+        forward()
+        both()
+        torch.cuda.synchronize()
+        return
+    size, shape = 2 * a.m * a.k, {"T": a.m, "H": a.k, "post": a.post}
+    _report("block_norm", shape, time_call(forward, a.iters, a.warmup).median_ms, 4 * size, a.m * a.k)
+    if a.k % 32 == 0:
+        ms = time_call(lambda: forward(quantize="nvfp4"), a.iters, a.warmup).median_ms
+        _report("block_norm_fp4", shape, ms, 3.28 * size, a.m * a.k)
+    _report("block_norm_grads", shape, time_call(both, a.iters, a.warmup).median_ms, (10 if a.post else 8) * size,
+            a.m * a.k)
+
+
 def main(argv: list[str] | None = None) -> None:
     p = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     p.add_argument("op", choices=["gemm", "gemm_sweep", "gemm_wq", "attention", "layer", "teal", "glu", "topk",
-                                  "hadamard", "packed_attention", "readout"])
+                                  "hadamard", "packed_attention", "readout", "fp4", "fp4_quantize", "block_norm"])
     p.add_argument("--ms", type=int, nargs="+", default=[1, 8, 61, 488], help="gemm_sweep: token counts")
     p.add_argument("--topk", type=int, default=10)
     p.add_argument("--m", type=int, default=61)
@@ -414,6 +486,7 @@ def main(argv: list[str] | None = None) -> None:
     p.add_argument("--ctx", type=int, default=768)
     p.add_argument("--tp", type=int, default=1)
     p.add_argument("--sparsity", type=float, default=0.5)
+    p.add_argument("--post", action="store_true", help="block_norm: with a norm behind the block")
     p.add_argument("--iters", type=int, default=20)
     p.add_argument("--warmup", type=int, default=3)
     p.add_argument("--once", action="store_true", help="one untimed call (for profiler captures)")
@@ -422,7 +495,8 @@ def main(argv: list[str] | None = None) -> None:
     a = p.parse_args(argv)
     {"gemm": bench_gemm, "gemm_sweep": bench_gemm_sweep, "gemm_wq": bench_gemm_wq, "attention": bench_attention, "layer": bench_layer,
      "teal": bench_teal, "glu": bench_glu, "topk": bench_topk, "hadamard": bench_hadamard,
-     "packed_attention": bench_packed_attention, "readout": bench_readout}[a.op](a)
+     "packed_attention": bench_packed_attention, "readout": bench_readout, "fp4": bench_fp4,
+     "fp4_quantize": bench_fp4_quantize, "block_norm": bench_block_norm}[a.op](a)
 
 
 if __name__ == "__main__":

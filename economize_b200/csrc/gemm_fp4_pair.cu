@@ -29,7 +29,7 @@ constexpr int kOperandBytes = kHalf * kBlockK / 2;
 constexpr int kThreads = 320;
 constexpr int kEpiWarps = 8;
 constexpr int kPatchStride = 144;  // bytes per row of an epilogue warp's [32 rows, 64 bf16] patch
-constexpr int kPatchBytes = 32 * kPatchStride;
+constexpr int kPatchBytes = 32 * kPatchStride + 512;
 constexpr int kSlots = 3;  // places for scales in tensor memory
 constexpr int kStrip = 8;
 
@@ -224,6 +224,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // ---- epilogue ----
     const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
     uint8_t* patch = patches + ew * kPatchBytes;
+    float* features = reinterpret_cast<float*>(patch + 32 * kPatchStride);  // row scales of this warp's 128 features
     const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * 128u;
     const bool wide = args.N % 8 == 0;  // 16-byte rows of y
     uint32_t tile = 0;
@@ -231,27 +232,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int m0, n0;
       tiles.at(t, m0, n0);
       const int row0 = m0 + static_cast<int>(rank) * kHalf + quad * 32, col0 = n0 + half * 128;
-      const float rx = FMT == kNv && row0 + lane < args.M ? args.x_row[row0 + lane] : 1.f;
+      float rx = 1.f;
+      if constexpr (FMT == kNv) {  // the rows' powers of two, at hand before the sums are
+        if (row0 + lane < args.M) rx = args.x_row[row0 + lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = col0 + i * 32 + lane;
+          features[i * 32 + lane] = n < args.N ? args.w_row[n] : 1.f;
+        }
+        __syncwarp();
+      }
       const bool ok = mbar_wait(acc_full, tile & 1u, args.status, kStatusWaitAccum, abort_flag);
       if (__any_sync(0xffffffffu, !ok)) break;
       tc_fence_after();
       uint32_t out[64];
 #pragma unroll
-      for (int c = 0; c < 128; c += 16) {
-        float v[16];
-        tmem_ld16(taddr + c, v);
+      for (int c = 0; c < 128; c += 32) {
+        float v[32];
+        tmem_ld32(taddr + c, v);
         if constexpr (FMT == kNv) {
 #pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            float4 w = make_float4(1.f, 1.f, 1.f, 1.f);
-            const int n = col0 + c + j;
-            if (n + 3 < args.N) {
-              w = *reinterpret_cast<const float4*>(args.w_row + n);
-            } else {
-              if (n < args.N) w.x = args.w_row[n];
-              if (n + 1 < args.N) w.y = args.w_row[n + 1];
-              if (n + 2 < args.N) w.z = args.w_row[n + 2];
-            }
+          for (int j = 0; j < 32; j += 4) {
+            const float4 w = *reinterpret_cast<const float4*>(features + c + j);
             v[j] *= rx * w.x;
             v[j + 1] *= rx * w.y;
             v[j + 2] *= rx * w.z;
@@ -259,7 +261,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) out[(c + j) / 2] = packed::pack_bf16(v[j], v[j + 1]);
+        for (int j = 0; j < 32; j += 2) out[(c + j) / 2] = packed::pack_bf16(v[j], v[j + 1]);
       }
       tc_fence_before();
       __syncwarp();
