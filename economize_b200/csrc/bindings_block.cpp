@@ -7,6 +7,7 @@
 #include <cmath>
 #include <cstring>
 #include <tuple>
+#include <vector>
 
 #include "bindings.h"
 #include "launchers.h"
@@ -25,155 +26,212 @@ Tensor rows_of(const Tensor& x) {
 
 int64_t row_stride(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
 
-bool aligned(const Tensor& x) {
-  return !x.defined() || (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 &&
-                          (x.dim() < 2 || row_stride(x) * x.element_size() % 16 == 0));
+// Whether every row starts on a boundary of `bytes`.
+bool aligned(const Tensor& x, int64_t bytes = 16) {
+  return !x.defined() || (reinterpret_cast<uintptr_t>(x.data_ptr()) % bytes == 0 &&
+                          (x.dim() < 2 || row_stride(x) * x.element_size() % bytes == 0));
+}
+
+// x, or a copy whose rows start on boundaries of 16 bytes (rows of whole 16-byte groups).
+Tensor on_boundary(const Tensor& x) { return aligned(x) ? x : x.clone(at::MemoryFormat::Contiguous); }
+
+// [..., C] as rows [R, C].
+Tensor as_rows(const Tensor& x) { return x.dim() == 2 ? x : x.reshape({-1, x.size(-1)}); }
+
+// The sizes of x with another last dimension.
+std::vector<int64_t> sizes_with(const Tensor& x, int64_t last) {
+  std::vector<int64_t> sizes = x.sizes().vec();
+  sizes.back() = last;
+  return sizes;
 }
 
 // ---- 4-bit operands ------------------------------------------------------------------------------------------------
-struct Fp4Buffers {
-  Tensor codes, scales, row_scale;
+// Where an operand's codes, scales and row scales lie.
+struct Fp4 {
+  uint8_t* codes = nullptr;
+  uint8_t* scales = nullptr;
+  float* row_scale = nullptr;
+  int64_t rows = 0, K = 0, tiles = 0;
+  int fmt = 0;
 };
 
-void check_format(int64_t fmt) { TORCH_CHECK(fmt == 1 || fmt == 2, "unknown 4-bit format ", fmt); }
+void check_format(int64_t fmt) { TORCH_CHECK_VALUE(fmt == 1 || fmt == 2, "unknown 4-bit format ", fmt); }
+
+void check_columns(int64_t K, const char* what) {
+  TORCH_CHECK_VALUE(K >= 32 && K % 32 == 0 && K <= ecz::kFp4MaxK, what, ": columns must be a multiple of 32, up to ",
+                    ecz::kFp4MaxK, " (got ", K, ")");
+}
+
+struct Fp4Buffers {
+  Tensor codes, scales, row_scale;
+  Fp4 at;
+};
 
 Fp4Buffers fp4_buffers(const Tensor& like, int64_t rows, int64_t K, int64_t fmt) {
   const auto bytes = like.options().dtype(at::kByte);
   Fp4Buffers b;
+  b.at.rows = rows;
+  b.at.K = K;
+  b.at.fmt = static_cast<int>(fmt);
+  b.at.tiles = ecz::fp4_scale_tiles(b.at.fmt, static_cast<int>(K));
   b.codes = at::empty({rows, K / 2}, bytes);
-  b.scales = at::empty({(rows + 127) / 128, ecz::fp4_scale_tiles(static_cast<int>(fmt), static_cast<int>(K)), 512}, bytes);
+  b.scales = at::empty({(rows + 127) / 128, b.at.tiles, 512}, bytes);
   b.row_scale = at::empty({fmt == 1 ? rows : 0}, like.options().dtype(at::kFloat));
+  b.at.codes = b.codes.data_ptr<uint8_t>();
+  b.at.scales = b.scales.data_ptr<uint8_t>();
+  b.at.row_scale = b.row_scale.data_ptr<float>();
   return b;
 }
 
-void check_columns(int64_t K, const char* what) {
-  TORCH_CHECK(K >= 32 && K % 32 == 0 && K <= ecz::kFp4MaxK, what, ": columns must be a multiple of 32, up to ",
-              ecz::kFp4MaxK, " (got ", K, ")");
+// x [M, K] into `to`. pad: scales of the rows up to a multiple of 128 become zeros; early: see launch_fp4_quantize.
+void quantize_into(Tensor x, const Fp4& to, bool pad, bool early) {
+  if (to.rows == 0) return;
+  x = rows_of(x);
+  if (!aligned(x, 32)) x = x.clone(at::MemoryFormat::Contiguous);
+  const int rc = ecz::launch_fp4_quantize(x.data_ptr(), row_stride(x), to.fmt, to.codes, to.scales, to.row_scale,
+                                          static_cast<int>(to.rows), static_cast<int>(to.K), pad, early,
+                                          ecz::device_sms(x.get_device()), at::cuda::getCurrentCUDAStream());
+  TORCH_CHECK(rc == 0, "fp4_quantize: launch failed");
 }
 
-Fp4Buffers quantize(Tensor x, int64_t fmt, bool early) {
+// Codes [M, K / 2], scales and row scales of x [..., K].
+std::tuple<Tensor, Tensor, Tensor> fp4_quantize(const Tensor& x, int64_t fmt) {
   CHECK_CUDA(x);
   CHECK_BF16(x);
   check_format(fmt);
-  TORCH_CHECK(x.dim() == 2, "fp4_quantize expects x [M, K]");
-  const int64_t M = x.size(0), K = x.size(1);
-  check_columns(K, "fp4_quantize");
-  TORCH_CHECK(M <= kMaxRows, "fp4_quantize: too many rows");
+  TORCH_CHECK_VALUE(x.dim() >= 1, "fp4_quantize expects x [..., K]");
+  check_columns(x.size(-1), "fp4_quantize");
   c10::cuda::CUDAGuard guard(x.device());
-  Fp4Buffers b = fp4_buffers(x, M, K, fmt);
-  if (M == 0) return b;
-  x = rows_of(x);
-  if (!aligned(x)) x = x.clone(at::MemoryFormat::Contiguous);
-  const int rc = ecz::launch_fp4_quantize(x.data_ptr(), row_stride(x), static_cast<int>(fmt), b.codes.data_ptr(),
-                                          b.scales.data_ptr(), b.row_scale.data_ptr<float>(), static_cast<int>(M),
-                                          static_cast<int>(K), early, ecz::device_sms(x.get_device()),
-                                          at::cuda::getCurrentCUDAStream());
-  TORCH_CHECK(rc == 0, "fp4_quantize: launch failed");
-  return b;
-}
-
-std::tuple<Tensor, Tensor, Tensor> fp4_quantize(const Tensor& x, int64_t fmt) {
+  const Tensor rows = as_rows(x);
+  TORCH_CHECK_VALUE(rows.size(0) <= kMaxRows, "fp4_quantize: too many rows");
+  Fp4Buffers b = fp4_buffers(x, rows.size(0), x.size(-1), fmt);
   // the result may become a weight, which products fetch before the kernel in front of them ends: no early start
-  Fp4Buffers b = quantize(x, fmt, false);
+  quantize_into(rows, b.at, true, false);
   return {b.codes, b.scales, b.row_scale};
 }
 
-// Codes, scales and row scales of one operand belong together.
-void check_operand(const Tensor& codes, const Tensor& scales, const Tensor& row_scale, int64_t fmt, const Tensor& ref,
-                   const char* what) {
+// Codes, scales and row scales of one operand belong together and lie on the device of ref.
+Fp4 check_operand(const Tensor& codes, const Tensor& scales, const Tensor& row_scale, int64_t fmt, const Tensor& ref,
+                  const char* what) {
   check_format(fmt);
   TORCH_CHECK(codes.is_cuda() && codes.get_device() == ref.get_device() && scales.is_cuda() &&
                   scales.get_device() == ref.get_device(),
-              what, ": codes and scales must be on one CUDA device");
+              what, ": codes and scales must be on the device of the call");
   TORCH_CHECK(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte && codes.dim() == 2 &&
                   codes.is_contiguous() && scales.is_contiguous(),
               what, ": codes [rows, K / 2] and scales must be contiguous uint8");
-  check_columns(codes.size(1) * 2, what);
-  TORCH_CHECK(codes.size(0) <= kMaxRows, what, ": too many rows");
-  const int64_t tiles = ecz::fp4_scale_tiles(static_cast<int>(fmt), static_cast<int>(codes.size(1) * 2));
-  TORCH_CHECK(scales.dim() == 3 && scales.size(0) == (codes.size(0) + 127) / 128 && scales.size(1) == tiles &&
+  Fp4 o;
+  o.fmt = static_cast<int>(fmt);
+  o.rows = codes.size(0);
+  o.K = codes.size(1) * 2;
+  check_columns(o.K, what);
+  TORCH_CHECK(o.rows <= kMaxRows, what, ": too many rows");
+  o.tiles = ecz::fp4_scale_tiles(o.fmt, static_cast<int>(o.K));
+  TORCH_CHECK(scales.dim() == 3 && scales.size(0) == (o.rows + 127) / 128 && scales.size(1) == o.tiles &&
                   scales.size(2) == 512,
-              what, ": scales must be [", (codes.size(0) + 127) / 128, ", ", tiles, ", 512], got ", scales.sizes());
+              what, ": scales must be [", (o.rows + 127) / 128, ", ", o.tiles, ", 512], got ", scales.sizes());
+  o.codes = codes.data_ptr<uint8_t>();
+  o.scales = scales.data_ptr<uint8_t>();
   if (fmt == 1) {
     TORCH_CHECK(row_scale.is_cuda() && row_scale.get_device() == ref.get_device() &&
-                    row_scale.scalar_type() == at::kFloat && row_scale.dim() == 1 &&
-                    row_scale.size(0) == codes.size(0) && row_scale.is_contiguous() &&
-                    reinterpret_cast<uintptr_t>(row_scale.data_ptr()) % 16 == 0,
-                what, ": nvfp4 has an fp32 scale per row, on a 16-byte boundary");
+                    row_scale.scalar_type() == at::kFloat && row_scale.dim() == 1 && row_scale.size(0) == o.rows &&
+                    row_scale.is_contiguous(),
+                what, ": nvfp4 has an fp32 scale per row");
+    o.row_scale = row_scale.data_ptr<float>();
   }
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0 &&
-                  reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0,
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(o.codes) % 16 == 0 && reinterpret_cast<uintptr_t>(o.scales) % 16 == 0,
               what, ": codes and scales must start on 16-byte boundaries");
+  return o;
 }
 
 Tensor fp4_dequantize(const Tensor& codes, const Tensor& scales, const Tensor& row_scale, int64_t fmt) {
   CHECK_CUDA(codes);
-  check_operand(codes, scales, row_scale, fmt, codes, "fp4_dequantize");
+  const Fp4 x = check_operand(codes, scales, row_scale, fmt, codes, "fp4_dequantize");
   c10::cuda::CUDAGuard guard(codes.device());
-  const int64_t M = codes.size(0), K = codes.size(1) * 2;
-  Tensor out = at::empty({M, K}, codes.options().dtype(at::kBFloat16));
-  if (M == 0) return out;
-  const int rc = ecz::launch_fp4_dequantize(codes.data_ptr(), scales.data_ptr(),
-                                            fmt == 1 ? row_scale.data_ptr<float>() : nullptr, static_cast<int>(fmt),
-                                            out.data_ptr(), static_cast<int>(M), static_cast<int>(K),
+  Tensor out = at::empty({x.rows, x.K}, codes.options().dtype(at::kBFloat16));
+  if (x.rows == 0) return out;
+  const int rc = ecz::launch_fp4_dequantize(x.codes, x.scales, x.row_scale, x.fmt, out.data_ptr(),
+                                            static_cast<int>(x.rows), static_cast<int>(x.K),
                                             ecz::device_sms(codes.get_device()), at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(rc == 0, "fp4_dequantize: launch failed");
   return out;
 }
 
-CUtensorMap codes_map(const Tensor& codes, int box_rows) {
+CUtensorMap codes_map(const Fp4& x, int box_rows) {
   CUtensorMap map;
   std::memset(&map, 0, sizeof(map));
-  const int rc = ecz::make_tmap_2d(&map, 1, codes.data_ptr(), codes.size(0), codes.size(1), codes.size(1), 128, box_rows,
-                                   128);
-  TORCH_CHECK(rc == 0, "cuTensorMapEncodeTiled failed (code ", rc, ") for codes ", codes.sizes());
+  const int rc = ecz::make_tmap_2d(&map, 1, x.codes, x.rows, x.K / 2, x.K / 2, 128, box_rows, 128);
+  TORCH_CHECK(rc == 0, "cuTensorMapEncodeTiled failed (code ", rc, ") for codes of ", x.rows, " x ", x.K);
   return map;
 }
 
 // Scales as rows of 128 bytes, one box the K block of 128 rows.
-CUtensorMap scales_map(const Tensor& scales, int64_t fmt) {
+CUtensorMap scales_map(const Fp4& x) {
   CUtensorMap map;
   std::memset(&map, 0, sizeof(map));
-  const int rc = ecz::make_tmap_2d(&map, 1, scales.data_ptr(), scales.numel() / 128, 128, 128, 128, fmt == 1 ? 16 : 8, 0);
-  TORCH_CHECK(rc == 0, "cuTensorMapEncodeTiled failed (code ", rc, ") for scales ", scales.sizes());
+  const int rc = ecz::make_tmap_2d(&map, 1, x.scales, (x.rows + 127) / 128 * x.tiles * 4, 128, 128, 128,
+                                   x.fmt == 1 ? 16 : 8, 0);
+  TORCH_CHECK(rc == 0, "cuTensorMapEncodeTiled failed (code ", rc, ") for scales of ", x.rows, " x ", x.K);
   return map;
 }
 
-// Y [M, N] of two operands [M, K] and [N, K] of one format.
-Tensor fp4_matmul(const Tensor& x, const Tensor& xs, const Tensor& xr, const Tensor& w, const Tensor& ws, const Tensor& wr,
-                  int64_t fmt) {
-  CHECK_CUDA(x);
-  check_operand(x, xs, xr, fmt, x, "fp4_matmul: x");
-  check_operand(w, ws, wr, fmt, x, "fp4_matmul: w");
-  TORCH_CHECK(x.size(1) == w.size(1), "fp4_matmul: x has ", 2 * x.size(1), " columns, w ", 2 * w.size(1));
-  TORCH_CHECK(w.size(0) >= 1, "fp4_matmul: w has no rows");
-  c10::cuda::CUDAGuard guard(x.device());
-  const int64_t M = x.size(0), N = w.size(0), K = 2 * x.size(1);
-  Tensor y = at::empty({M, N}, x.options().dtype(at::kBFloat16));
-  if (M == 0) return y;
-  const float* xr_ = fmt == 1 ? xr.data_ptr<float>() : nullptr;
-  const float* wr_ = fmt == 1 ? wr.data_ptr<float>() : nullptr;
-  const int sms = ecz::device_sms(x.get_device()), m = static_cast<int>(M), n = static_cast<int>(N), k = static_cast<int>(K);
-  unsigned* status = ecz::device_status(x.device());
+// y [M, N] of operands [M, K] and [N, K] of one format.
+void multiply(const Fp4& x, const Fp4& w, const Tensor& y, const at::Device& device) {
+  TORCH_CHECK_VALUE(x.K == w.K, "fp4 product: activations have ", x.K, " columns, the weight ", w.K);
+  TORCH_CHECK_VALUE(w.rows >= 1, "fp4 product: the weight has no rows");
+  if (x.rows == 0) return;
+  const int M = static_cast<int>(x.rows), N = static_cast<int>(w.rows), K = static_cast<int>(x.K);
+  const int sms = ecz::device_sms(device.index());
+  unsigned* status = ecz::device_status(device);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   int rc;
   if (M > 128) {
-    const CUtensorMap tx = codes_map(x, 128), tw = codes_map(w, 128), sx = scales_map(xs, fmt), sw = scales_map(ws, fmt);
-    rc = ecz::launch_gemm_fp4_pair(&tx, &tw, &sx, &sw, xr_, wr_, static_cast<int>(fmt), y.data_ptr(), m, n, k, sms, status,
+    const CUtensorMap tx = codes_map(x, 128), tw = codes_map(w, 128), sx = scales_map(x), sw = scales_map(w);
+    rc = ecz::launch_gemm_fp4_pair(&tx, &tw, &sx, &sw, x.row_scale, w.row_scale, x.fmt, y.data_ptr(), M, N, K, sms, status,
                                    stream);
   } else {
-    const CUtensorMap tw = codes_map(w, 128), tx = codes_map(x, ecz::fp4_block_rows(m));
-    rc = ecz::launch_gemm_fp4(&tw, &tx, ws.data_ptr(), xs.data_ptr(), wr_, xr_, static_cast<int>(fmt), y.data_ptr(), m, n,
-                              k, sms, status, stream);
+    const CUtensorMap tw = codes_map(w, 128), tx = codes_map(x, ecz::fp4_block_rows(M));
+    rc = ecz::launch_gemm_fp4(&tw, &tx, w.scales, x.scales, w.row_scale, x.row_scale, x.fmt, y.data_ptr(), M, N, K, sms,
+                              status, stream);
   }
-  TORCH_CHECK(rc == 0, "fp4_matmul: launch failed");
+  TORCH_CHECK(rc == 0, "fp4 product: launch failed");
+}
+
+Tensor fp4_matmul(const Tensor& x, const Tensor& xs, const Tensor& xr, const Tensor& w, const Tensor& ws, const Tensor& wr,
+                  int64_t fmt) {
+  CHECK_CUDA(x);
+  const Fp4 a = check_operand(x, xs, xr, fmt, x, "fp4_matmul: x"), b = check_operand(w, ws, wr, fmt, x, "fp4_matmul: w");
+  c10::cuda::CUDAGuard guard(x.device());
+  Tensor y = at::empty({a.rows, b.rows}, x.options().dtype(at::kBFloat16));
+  multiply(a, b, y, x.device());
   return y;
 }
 
-// bf16 activations [M, K] times a 4-bit weight [N, K]: quantised first, in a buffer of their own.
+// Activations [..., K] times a 4-bit weight [N, K]: quantised first, in a workspace. The result has x's type.
 Tensor linear_fp4(const Tensor& x, const Tensor& w, const Tensor& ws, const Tensor& wr, int64_t fmt) {
-  Fp4Buffers b = quantize(x, fmt, true);
-  return fp4_matmul(b.codes, b.scales, b.row_scale, w, ws, wr, fmt);
+  CHECK_CUDA(x);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.is_floating_point(), "linear_fp4 expects floating point x [..., K]");
+  const Fp4 b = check_operand(w, ws, wr, fmt, x, "linear_fp4: weight");
+  TORCH_CHECK_VALUE(x.size(-1) == b.K, "linear_fp4: x has ", x.size(-1), " columns, the weight ", b.K);
+  c10::cuda::CUDAGuard guard(x.device());
+  const bool cast = x.scalar_type() != at::kBFloat16;
+  const Tensor rows = as_rows(cast ? x.detach().to(at::kBFloat16) : x.detach());
+  Fp4 a;
+  a.fmt = static_cast<int>(fmt);
+  a.rows = rows.size(0);
+  a.K = b.K;
+  a.tiles = b.tiles;
+  TORCH_CHECK_VALUE(a.rows <= kMaxRows, "linear_fp4: too many rows");
+  // scales of the rows that complete a tile stay as they are: they reach only sums that nothing reads
+  const int64_t scale_bytes = (a.rows + 127) / 128 * a.tiles * 512, code_bytes = (a.rows * a.K / 2 + 255) / 256 * 256;
+  Tensor work = at::empty({scale_bytes + code_bytes + (fmt == 1 ? 4 * a.rows : 0)}, w.options());
+  a.scales = work.data_ptr<uint8_t>();
+  a.codes = a.scales + scale_bytes;
+  if (fmt == 1) a.row_scale = reinterpret_cast<float*>(a.codes + code_bytes);
+  Tensor y = at::empty(sizes_with(x, b.rows), rows.options());
+  quantize_into(rows, a, false, true);
+  multiply(a, b, y, x.device());
+  return cast ? y.to(x.scalar_type()) : y;
 }
 
 // ---- norms around a block ------------------------------------------------------------------------------------------
@@ -182,7 +240,7 @@ ecz::NormType norm_type(const Tensor& x) {
     case at::kBFloat16: return ecz::kNormBf16;
     case at::kHalf: return ecz::kNormFp16;
     case at::kFloat: return ecz::kNormFp32;
-    default: TORCH_CHECK(false, "block_norm takes bfloat16, float16 or float32, got ", x.scalar_type());
+    default: TORCH_CHECK_VALUE(false, "block_norm takes bfloat16, float16 or float32, got ", x.scalar_type());
   }
 }
 
@@ -195,38 +253,38 @@ struct NormOperands {
 // Checked operands, rows readable in place. Undefined: residual, post and gate that are not given.
 NormOperands norm_operands(const Tensor& x, const Tensor& residual, const Tensor& weight, const Tensor& post,
                            const Tensor& gate, double scale, double eps) {
-  CHECK_CUDA(x);
-  norm_type(x);
-  TORCH_CHECK(x.dim() == 2, "block_norm expects x [T, H]");
   const int64_t T = x.size(0), H = x.size(1);
-  TORCH_CHECK(H >= 1 && H <= ecz::kBlockNormMaxHidden, "block_norm: 1 to ", ecz::kBlockNormMaxHidden, " columns (got ", H,
-              ")");
-  TORCH_CHECK(T <= kMaxRows, "block_norm: too many rows");
-  TORCH_CHECK(std::isfinite(scale) && std::isfinite(eps) && eps >= 0, "block_norm: scale and eps must be finite, eps >= 0");
+  TORCH_CHECK_VALUE(H >= 1 && H <= ecz::kBlockNormMaxHidden, "block_norm: 1 to ", ecz::kBlockNormMaxHidden,
+                    " columns (got ", H, ")");
+  TORCH_CHECK_VALUE(T <= kMaxRows, "block_norm: too many rows");
+  TORCH_CHECK_VALUE(std::isfinite(scale) && std::isfinite(eps) && eps >= 0,
+                    "block_norm: scale and eps must be finite, eps >= 0");
   for (const Tensor* t : {&residual, &weight, &post, &gate}) {
     if (!t->defined()) continue;
-    TORCH_CHECK(t->scalar_type() == x.scalar_type(), "block_norm: all operands have one type (", x.scalar_type(), " and ",
-                t->scalar_type(), ")");
-    TORCH_CHECK(t->is_cuda() && t->get_device() == x.get_device(), "block_norm: all operands must be on the device of x");
+    TORCH_CHECK_VALUE(t->scalar_type() == x.scalar_type() && t->is_cuda() && t->get_device() == x.get_device(),
+                      "block_norm: all operands must have one type and device, got ", x.scalar_type(), " on ", x.device(),
+                      " and ", t->scalar_type(), " on ", t->device());
   }
-  TORCH_CHECK(weight.defined() && weight.dim() == 1 && weight.size(0) == H, "block_norm: weight must be [", H, "]");
-  TORCH_CHECK(!post.defined() || (post.dim() == 1 && post.size(0) == H), "block_norm: post_weight must be [", H, "]");
-  TORCH_CHECK(!residual.defined() || residual.sizes() == x.sizes(), "block_norm: residual ", residual.sizes(),
-              " does not match x ", x.sizes());
+  TORCH_CHECK_VALUE(weight.defined() && weight.dim() == 1 && weight.size(0) == H, "block_norm: weight must be [", H, "]");
+  TORCH_CHECK_VALUE(!post.defined() || (post.dim() == 1 && post.size(0) == H), "block_norm: post_weight must be [", H, "]");
+  TORCH_CHECK_VALUE(!residual.defined() || residual.sizes() == x.sizes(), "block_norm: the residual does not match x");
   NormOperands o;
   o.x = rows_of(x);
   o.weight = weight.contiguous();
   if (residual.defined()) o.residual = rows_of(residual);
   if (post.defined()) o.post = post.contiguous();
   if (gate.defined()) {
-    TORCH_CHECK(gate.dim() == 2 && gate.size(0) == T && (gate.size(1) == 1 || gate.size(1) == H),
-                "block_norm: gate must be [", T, ", 1] or [", T, ", ", H, "], got ", gate.sizes());
+    TORCH_CHECK_VALUE(gate.dim() == 2 && gate.size(0) == T && (gate.size(1) == 1 || gate.size(1) == H),
+                      "block_norm: the gate must have one value per token or per element");
     o.gate_mode = gate.size(1) == 1 ? ecz::kGateToken : ecz::kGateFull;
     o.gate = o.gate_mode == ecz::kGateFull ? rows_of(gate) : gate;
   }
-  const bool full = o.gate_mode == ecz::kGateFull;
-  o.vec = H * x.element_size() % 16 == 0 && aligned(o.x) && aligned(o.weight) && aligned(o.residual) && aligned(o.post) &&
-          (!full || aligned(o.gate));
+  // rows of whole 16-byte groups are read in such groups, from copies where they do not start on a boundary (a token's
+  // gate is read by itself): a row's sums then do not depend on where it lies
+  o.vec = H * x.element_size() % 16 == 0;
+  if (o.vec)
+    for (Tensor* t : {&o.x, &o.residual, &o.weight, &o.post, &o.gate})
+      if (!(t == &o.gate && o.gate_mode == ecz::kGateToken)) *t = on_boundary(*t);
   return o;
 }
 
@@ -256,8 +314,8 @@ struct NormResult {
 
 NormResult norm_forward(const Tensor& x, const Tensor& residual, const Tensor& weight, const Tensor& post,
                         const Tensor& gate, double scale, double eps, bool training) {
-  const NormOperands o = norm_operands(x, residual, weight, post, gate, scale, eps);
   c10::cuda::CUDAGuard guard(x.device());
+  const NormOperands o = norm_operands(x, residual, weight, post, gate, scale, eps);
   const auto f32 = x.options().dtype(at::kFloat);
   NormResult r;
   r.normed = at::empty(x.sizes(), x.options());
@@ -282,6 +340,29 @@ NormResult norm_forward(const Tensor& x, const Tensor& residual, const Tensor& w
 
 Tensor value(const c10::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 
+// The operands [..., H] of a call as rows.
+struct NormCall {
+  Tensor x, residual, post, gate;
+};
+
+NormCall norm_call(const Tensor& x, const c10::optional<Tensor>& residual, const c10::optional<Tensor>& post,
+                   const c10::optional<Tensor>& gate) {
+  CHECK_CUDA(x);
+  norm_type(x);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "block_norm expects x [..., H]");
+  NormCall c{x, value(residual), value(post), value(gate)};
+  TORCH_CHECK_VALUE(!c.residual.defined() || c.residual.sizes() == x.sizes(), "block_norm: residual ", c.residual.sizes(),
+                    " does not match x ", x.sizes());
+  TORCH_CHECK_VALUE(!c.gate.defined() || c.gate.sizes() == x.sizes() || c.gate.sizes() == at::IntArrayRef(sizes_with(x, 1)),
+                    "block_norm: gate ", c.gate.sizes(), " must be like x ", x.sizes(), " or have a last dimension of 1");
+  if (x.dim() != 2) {
+    c.x = as_rows(x);
+    if (c.residual.defined()) c.residual = as_rows(c.residual);
+    if (c.gate.defined()) c.gate = as_rows(c.gate);
+  }
+  return c;
+}
+
 // Codes, scales and row scales of normed, and the stream.
 std::tuple<Tensor, Tensor, Tensor, Tensor> block_norm_fp4(const Tensor& x, const c10::optional<Tensor>& residual,
                                                           const Tensor& weight, const c10::optional<Tensor>& post,
@@ -289,24 +370,20 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> block_norm_fp4(const Tensor& x, const
                                                           int64_t fmt) {
   check_format(fmt);
   CHECK_CUDA(x);
-  CHECK_BF16(x);
-  NormOperands o = norm_operands(x, value(residual), weight, value(post), value(gate), scale, eps);
-  check_columns(x.size(1), "block_norm in 4 bits");
+  TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16, "block_norm in 4 bits takes bfloat16, got ", x.scalar_type());
+  const NormCall c = norm_call(x, residual, post, gate);
+  check_columns(x.size(-1), "block_norm in 4 bits");
   c10::cuda::CUDAGuard guard(x.device());
-  Fp4Buffers b = fp4_buffers(x, x.size(0), x.size(1), fmt);
+  NormOperands o = norm_operands(c.x, c.residual, weight, c.post, c.gate, scale, eps);
+  Fp4Buffers b = fp4_buffers(x, c.x.size(0), c.x.size(1), fmt);
   Tensor stream = at::empty(x.sizes(), x.options());
-  if (x.size(0) == 0) return {b.codes, b.scales, b.row_scale, stream};
-  if (!o.vec) {  // rows that do not start on 16 bytes
-    for (Tensor* t : {&o.x, &o.residual, &o.weight, &o.post, &o.gate})
-      if (t->defined() && !(t == &o.gate && o.gate_mode == ecz::kGateToken) && !aligned(*t))
-        *t = t->clone(at::MemoryFormat::Contiguous);
-  }
+  if (c.x.size(0) == 0) return {b.codes, b.scales, b.row_scale, stream};
   ecz::BlockNormArgs a = norm_args(o, scale, eps);
   a.stream = stream.data_ptr();
-  a.codes = b.codes.data_ptr<uint8_t>();
-  a.scales = b.scales.data_ptr<uint8_t>();
-  a.row_scale = b.row_scale.data_ptr<float>();
-  a.tiles = static_cast<int>(b.scales.size(1));
+  a.codes = b.at.codes;
+  a.scales = b.at.scales;
+  a.row_scale = b.at.row_scale;
+  a.tiles = static_cast<int>(b.at.tiles);
   TORCH_CHECK(ecz::launch_block_norm(a, ecz::kNormBf16, true, static_cast<int>(fmt), ecz::device_sms(x.get_device()),
                                      at::cuda::getCurrentCUDAStream()) == 0,
               "block_norm: launch failed");
@@ -358,7 +435,9 @@ struct BlockNormFunction : torch::autograd::Function<BlockNormFunction> {
     const Tensor& like = dn.defined() ? dn : up;
     const int64_t T = like.size(0), H = like.size(1);
     if (simple) check_saved(stream, weight, weight.scalar_type(), {T, H}, "stream");
+    c10::cuda::CUDAGuard guard(weight.device());
     // the operands as in the forward pass (the stream in x's place where it alone was saved)
+    norm_type(weight);
     const NormOperands o = norm_operands(simple ? stream : s[0], simple ? Tensor() : s[1], weight, post, gate, scale, eps);
     for (const Tensor* t : {&dn, &up})
       TORCH_CHECK(!t->defined() || (t->is_cuda() && t->get_device() == o.x.get_device() &&
@@ -366,7 +445,6 @@ struct BlockNormFunction : torch::autograd::Function<BlockNormFunction> {
                   "block_norm: a gradient does not match its output");
     check_saved(inv_s, o.x, at::kFloat, {T}, "norms");
     check_saved(inv_x, o.x, at::kFloat, {post.defined() ? T : 0}, "norms of the block's output");
-    c10::cuda::CUDAGuard guard(o.x.device());
     const auto opts = o.x.options();
     const bool shared = simple && scale == 1.0;  // both gradients are the same values
     Tensor dx, dr, dw, dp, dg;
@@ -379,9 +457,8 @@ struct BlockNormFunction : torch::autograd::Function<BlockNormFunction> {
       if (need_w) dw.zero_();
       if (need_p) dp.zero_();
     } else {
-      if (dn.defined()) dn = rows_of(dn);
-      if (up.defined()) up = rows_of(up);
-      const bool vec = o.vec && aligned(dn) && aligned(up);
+      if (dn.defined()) dn = o.vec ? on_boundary(rows_of(dn)) : rows_of(dn);
+      if (up.defined()) up = o.vec ? on_boundary(rows_of(up)) : rows_of(up);
       const ecz::NormType type = norm_type(o.x);
       const int sms = ecz::device_sms(o.x.get_device());
       ecz::BlockNormGrads a;
@@ -412,13 +489,13 @@ struct BlockNormFunction : torch::autograd::Function<BlockNormFunction> {
       a.scale = f.scale;
       Tensor parts;
       if (need_w || need_p) {
-        const int n = ecz::block_norm_parts(type, a.rows, a.hidden, vec, sms);
+        const int n = ecz::block_norm_parts(type, a.rows, a.hidden, o.vec, sms);
         parts = at::empty({(need_w ? 1 : 0) + (need_p ? 1 : 0), n, H}, opts.dtype(at::kFloat));
         float* p = parts.data_ptr<float>();
         if (need_w) a.dw_part = p;
         if (need_p) a.dpost_part = p + (need_w ? static_cast<int64_t>(n) * H : 0);
       }
-      TORCH_CHECK(ecz::launch_block_norm_grads(a, type, vec, sms, at::cuda::getCurrentCUDAStream()) == 0,
+      TORCH_CHECK(ecz::launch_block_norm_grads(a, type, o.vec, sms, at::cuda::getCurrentCUDAStream()) == 0,
                   "block_norm: backward launch failed");
     }
     if (need_x) out[0] = shared ? dr : dx;
@@ -433,22 +510,28 @@ struct BlockNormFunction : torch::autograd::Function<BlockNormFunction> {
 std::tuple<Tensor, Tensor> block_norm(const Tensor& x, const c10::optional<Tensor>& residual, const Tensor& weight,
                                       const c10::optional<Tensor>& post, const c10::optional<Tensor>& gate, double scale,
                                       double eps) {
-  const Tensor r = value(residual), p = value(post), g = value(gate);
+  const NormCall c = norm_call(x, residual, post, gate);
   bool grad = false;
-  for (const Tensor* t : {&x, &r, &weight, &p, &g}) {
+  for (const Tensor* t : {&c.x, &c.residual, &weight, &c.post, &c.gate}) {
     if (!t->defined()) continue;
     grad |= t->requires_grad();
     // the kernels carry no tangents: refused, or a dual number's would be dropped without a word
     TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t->_fw_grad(0).defined(),
                 "block_norm has no forward-mode derivative on CUDA");
   }
+  Tensor normed, stream;
   if (grad && at::GradMode::is_enabled()) {
     auto given = [](const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; };
-    auto out = BlockNormFunction::apply(x, given(r), weight, given(p), given(g), scale, eps);
-    return {out[0], out[1]};
+    auto out = BlockNormFunction::apply(c.x, given(c.residual), weight, given(c.post), given(c.gate), scale, eps);
+    normed = out[0];
+    stream = out[1];
+  } else {
+    NormResult out = norm_forward(c.x, c.residual, weight, c.post, c.gate, scale, eps, false);
+    normed = out.normed;
+    stream = out.stream;
   }
-  NormResult out = norm_forward(x, r, weight, p, g, scale, eps, false);
-  return {out.normed, out.stream};
+  if (x.dim() != 2) return {normed.view(x.sizes()), stream.view(x.sizes())};
+  return {normed, stream};
 }
 
 }  // namespace

@@ -45,23 +45,97 @@ struct Cast<__half> {
   static __device__ __forceinline__ __half from(float v) { return __float2half(v); }
 };
 
-// VEC consecutive elements (VEC sizeof(T) = 16 bytes, aligned, or VEC = 1).
+// A lane's VEC consecutive elements, from element `at` of a row of `hidden` on: 32 bytes in two halves of 16, of which the
+// second may lie behind the row's end, or one element.
 template <typename T, int VEC>
 struct Pack {
-  T v[VEC];
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (VEC == 1) v[0] = *p;
-    else *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p);
-  }
-  __device__ __forceinline__ void store(T* p) const {
-    if constexpr (VEC == 1) *p = v[0];
-    else *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(v);
-  }
+  static constexpr int kPart = VEC == 1 ? 1 : VEC / 2;
+  static constexpr int kParts = VEC / kPart;
+  static constexpr int kWords = (VEC * static_cast<int>(sizeof(T)) + 3) / 4;
+  union {
+    T v[VEC];
+    uint32_t words[kWords];
+  };
+  __device__ __forceinline__ Pack() {}
   __device__ __forceinline__ float get(int i) const { return Cast<T>::to(v[i]); }
   __device__ __forceinline__ void set(int i, float f) { v[i] = Cast<T>::from(f); }
-  __device__ __forceinline__ void zero() {
+  // row[at ..], zeros where the row is null or has ended
+  __device__ __forceinline__ void fetch(const T* row, int at, int hidden) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = Cast<T>::from(0.f);
+    for (int i = 0; i < kWords; ++i) words[i] = 0;
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) {
+      if (row != nullptr && at + k * kPart < hidden) {
+        if constexpr (VEC == 1) v[0] = row[at];
+        else *reinterpret_cast<uint4*>(words + 4 * k) = *reinterpret_cast<const uint4*>(row + at + k * kPart);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* row, int at, int hidden) const {
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) {
+      if (at + k * kPart < hidden) {
+        if constexpr (VEC == 1) row[at] = v[0];
+        else *reinterpret_cast<uint4*>(row + at + k * kPart) = *reinterpret_cast<const uint4*>(words + 4 * k);
+      }
+    }
+  }
+};
+
+// Rows on their way: every thread copies the vectors that it will work on itself into shared memory (cp.async), DEPTH rows
+// ahead, so nothing is shared, no barrier is needed and no register is held. Operand k, vector i of a thread in slot s
+// lies in 16-byte planes of one entry per thread. DEPTH 0: operands are read when they are needed.
+template <typename T, int VEC, int NV, int OPS, int DEPTH>
+struct Rows {
+  using P = Pack<T, VEC>;
+  static constexpr bool kAhead = DEPTH > 0;
+  static_assert(!kAhead || VEC > 1, "single elements are not copied ahead");
+  static constexpr int kSlotPlanes = OPS * NV * P::kParts;
+  static constexpr int bytes(int threads) { return DEPTH * kSlotPlanes * threads * 16; }
+  uint32_t base;
+  int slot = 0;
+  const T* ptr[OPS];  // rows being worked on (DEPTH 0)
+  __device__ __forceinline__ Rows(void* smem) : base(smem_u32(smem) + threadIdx.x * 16) {}
+  __device__ __forceinline__ uint32_t plane(int s, int op, int i, int k) const {
+    return base + static_cast<uint32_t>((s * kSlotPlanes + (op * NV + i) * P::kParts + k) * blockDim.x * 16);
+  }
+  // start the copy of operand op's row (zeros for null) into slot s; first, step: this lane's vectors
+  __device__ __forceinline__ void start(int s, int op, const T* row, int first, int step, int hidden) {
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < P::kParts; ++k) {
+          const int at = (first + i * step) * VEC + k * P::kPart;
+          const uint32_t to = plane(s, op, i, k);
+          if (row != nullptr && at < hidden)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(row + at) : "memory");
+          else
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory");
+        }
+    } else {
+      ptr[op] = row;
+    }
+  }
+  __device__ __forceinline__ static void commit() {
+    if constexpr (kAhead) asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // the oldest slot's copies have landed
+  __device__ __forceinline__ static void wait() {
+    if constexpr (kAhead) asm volatile("cp.async.wait_group %0;" ::"n"(kAhead ? DEPTH - 1 : 0) : "memory");
+  }
+  __device__ __forceinline__ void get(P& out, int op, int i, int at, int hidden) const {
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int k = 0; k < P::kParts; ++k)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(out.words[4 * k]), "=r"(out.words[4 * k + 1]), "=r"(out.words[4 * k + 2]),
+                       "=r"(out.words[4 * k + 3])
+                     : "r"(plane(slot, op, i, k))
+                     : "memory");
+    } else {
+      out.fetch(ptr[op], at, hidden);
+    }
   }
 };
 
@@ -121,363 +195,423 @@ struct Team {
   }
 };
 
-// FMT 0: normed as T; else as 4-bit codes (VEC = 8 elements of bf16).
-template <typename T, int VEC, int NV, int FMT>
-__global__ void __launch_bounds__(1024) block_norm_kernel(const __grid_constant__ BlockNormArgs a, int warps) {
+// FMT 0: normed as T; else as 4-bit codes (bf16). POST: there may be a norm behind the block. Persistent over
+// rows: team t of all takes rows t, t + teams, ...
+template <typename T, int VEC, int NV, int FMT, bool POST, int THREADS, int BLOCKS, int DEPTH>
+__global__ void __launch_bounds__(THREADS, BLOCKS)
+    block_norm_kernel(const __grid_constant__ BlockNormArgs a, int warps) {
   __shared__ float2 scratch[2 * kMaxWarps];
+  extern __shared__ uint8_t ring[];
   pdl_trigger();
   Team team(warps, scratch);
+  Rows<T, VEC, NV, 2, DEPTH> rows(ring);
+  const int per_block = blockDim.x / (32 * warps);
+  const int teams = gridDim.x * per_block;
+  const bool post = POST && a.post != nullptr;
+  const int hidden = a.hidden;
+  const float mean = 1.f / static_cast<float>(hidden);
+  const int last = FMT == 0 ? a.rows : (a.rows + 127) / 128 * 128;
+  const T* xp = static_cast<const T*>(a.x);
+  const T* rp = static_cast<const T*>(a.residual);
+  const T* gp = static_cast<const T*>(a.gate);
+  auto start = [&](int slot, int row) {
+    const bool on = row < a.rows;
+    rows.start(slot, 0, on ? xp + row * a.x_stride : nullptr, team.first, team.step, hidden);
+    rows.start(slot, 1, on && rp != nullptr ? rp + row * a.r_stride : nullptr, team.first, team.step, hidden);
+    rows.commit();
+  };
   pdl_wait();
-  const int teams = blockDim.x / (32 * warps);
-  const T* weight = static_cast<const T*>(a.weight);
-  const T* post = static_cast<const T*>(a.post);
-  const int vecs = (a.hidden + VEC - 1) / VEC;
-  const float mean = 1.f / static_cast<float>(a.hidden);
-  const int row = blockIdx.x * teams + team.index;
-  if (FMT == 0 && row >= a.rows) return;
-  if (FMT != 0 && row >= (a.rows + 127) / 128 * 128) return;
-  const bool real = row < a.rows;
-  Pack<T, VEC> x[NV], r[NV];
-  float s[NV][VEC];
-  const T* xr = static_cast<const T*>(a.x) + row * a.x_stride;
-  const T* rr = static_cast<const T*>(a.residual) + row * a.r_stride;
+  int row = blockIdx.x * per_block + team.index;
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) start(d, row + d * teams);
+  Pack<T, VEC> w[NV], p[POST ? NV : 1];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int v = team.first + i * team.step;
-    x[i].zero();
-    r[i].zero();
-    if (real && v < vecs) {
-      x[i].load(xr + static_cast<size_t>(v) * VEC);
-      if (a.residual != nullptr) r[i].load(rr + static_cast<size_t>(v) * VEC);
-    }
+    const int at = (team.first + i * team.step) * VEC;
+    w[i].fetch(static_cast<const T*>(a.weight), at, hidden);
+    if constexpr (POST) p[i].fetch(static_cast<const T*>(a.post), at, hidden);
   }
-  float factor = a.scale;
-  if (a.gate_mode == kGateToken && real) factor *= Cast<T>::to(static_cast<const T*>(a.gate)[row * a.gate_stride]);
-  float ix = 1.f;
-  if (post != nullptr) {
+  for (; row < last; row += teams) {
+    const bool real = row < a.rows;
+    float factor = a.scale;
+    if (a.gate_mode == kGateToken && real) factor *= Cast<T>::to(gp[row * a.gate_stride]);
+    if constexpr (DEPTH == 0) start(0, row);
+    rows.wait();
+    float s[NV][VEC];
+    float ix = 1.f;
+    if (post) {
+      float q = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        Pack<T, VEC> x;
+        rows.get(x, 0, i, (team.first + i * team.step) * VEC, hidden);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          s[i][j] = x.get(j);
+          q = fmaf(s[i][j], s[i][j], q);
+        }
+      }
+      ix = rsqrtf(team.sum(q) * mean + a.eps);
+      if (a.inv_x != nullptr && team.first == 0 && real) a.inv_x[row] = ix;
+    }
     float q = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      const int at = (team.first + i * team.step) * VEC;
+      Pack<T, VEC> x, r, g;
+      if (!post) rows.get(x, 0, i, at, hidden);
+      rows.get(r, 1, i, at, hidden);
+      if (a.gate_mode == kGateFull) g.fetch(real ? gp + row * a.gate_stride : nullptr, at, hidden);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) q = fmaf(x[i].get(j), x[i].get(j), q);
-    ix = rsqrtf(team.sum(q) * mean + a.eps);
-    if (a.inv_x != nullptr && team.first == 0 && real) a.inv_x[row] = ix;
-  }
-  float q = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = team.first + i * team.step;
-    Pack<T, VEC> p, g;
-    if (post != nullptr && v < vecs) p.load(post + static_cast<size_t>(v) * VEC);
-    if (a.gate_mode == kGateFull && real && v < vecs)
-      g.load(static_cast<const T*>(a.gate) + row * a.gate_stride + static_cast<size_t>(v) * VEC);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      float b = x[i].get(j);
-      if (post != nullptr && v < vecs) b = b * ix * p.get(j);
-      if (a.gate_mode == kGateFull && real && v < vecs) b *= g.get(j);
-      s[i][j] = fmaf(factor, b, r[i].get(j));
-      q = fmaf(s[i][j], s[i][j], q);
-    }
-    if (real && v < vecs) {
-      Pack<T, VEC> out;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) out.set(j, s[i][j]);
-      out.store(static_cast<T*>(a.stream) + static_cast<size_t>(row) * a.hidden + static_cast<size_t>(v) * VEC);
-    }
-  }
-  const float is = rsqrtf(team.sum(q) * mean + a.eps);
-  if (a.inv_s != nullptr && team.first == 0 && real) a.inv_s[row] = is;
-  float top = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = team.first + i * team.step;
-    if (FMT != 0 || v < vecs) {
-      Pack<T, VEC> w, out;
-      w.zero();
-      if (v < vecs) w.load(weight + static_cast<size_t>(v) * VEC);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) out.set(j, real ? s[i][j] * is * w.get(j) : 0.f);
-      if constexpr (FMT == 0) {
-        out.store(static_cast<T*>(a.normed) + static_cast<size_t>(row) * a.hidden + static_cast<size_t>(v) * VEC);
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s[i][j] = out.get(j);  // what quantising the rounded result takes
-        bool bad;
-        if (FMT == fp4::kNv) top = fmaxf(top, fp4::finite_max8(s[i], bad));
+      for (int j = 0; j < VEC; ++j) {
+        float b = post ? s[i][j] * (ix * p[POST ? i : 0].get(j)) : x.get(j);
+        if (a.gate_mode == kGateFull) b *= g.get(j);
+        s[i][j] = fmaf(factor, b, r.get(j));
+        q = fmaf(s[i][j], s[i][j], q);
       }
     }
-  }
-  if constexpr (FMT != 0) {
-    float mul = 1.f;
-    if constexpr (FMT == fp4::kNv) {
-      const int e = fp4::row_exponent(team.max(top));
-      mul = fp4::pow2(-e);
-      if (real && team.first == 0) a.row_scale[row] = fp4::pow2(e);
+    if constexpr (DEPTH > 0) {  // this row's slot is read: the row DEPTH further
+      start(rows.slot, row + DEPTH * teams);
+      rows.slot = rows.slot + 1 == DEPTH ? 0 : rows.slot + 1;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int base = (team.warp + i * warps) * 32;
-      if (base >= a.tiles * fp4::Format<FMT>::kWordLanes) break;
-      fp4::store8<FMT>(s[i], mul, row, base + team.lane, real ? vecs : 0, a.tiles, a.codes, a.scales);
+      Pack<T, VEC> out;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) out.set(j, s[i][j]);
+      if (real)
+        out.store(static_cast<T*>(a.stream) + static_cast<size_t>(row) * hidden, (team.first + i * team.step) * VEC, hidden);
+    }
+    const float is = rsqrtf(team.sum(q) * mean + a.eps);
+    if (a.inv_s != nullptr && team.first == 0 && real) a.inv_s[row] = is;
+    Pack<T, VEC> out[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) out[i].set(j, real ? s[i][j] * is * w[i].get(j) : 0.f);
+      if (FMT == 0)
+        out[i].store(static_cast<T*>(a.normed) + static_cast<size_t>(row) * hidden, (team.first + i * team.step) * VEC,
+                     hidden);
+    }
+    if constexpr (FMT != 0) {
+      float mul = 1.f;
+      if constexpr (FMT == fp4::kNv) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) top = max(top, fp4::max_bits<8>(out[i].words));
+        if (top >= 0x7f80u) {
+          top = 0;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) top = max(top, fp4::finite_bits<8>(out[i].words));
+        }
+        const int e = fp4::row_exponent(team.max(fp4::bits_value(top)));
+        mul = fp4::pow2(-e);
+        if (real && team.first == 0) a.row_scale[row] = fp4::pow2(e);
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        fp4::store16<FMT>(out[i].words, mul, row, team.first + i * team.step, real ? hidden / 16 : 0, a.tiles, a.codes,
+                          a.scales);
     }
   }
 }
 
-// Persistent over rows: team t of all takes rows t, t + teams, ...; its sums for dweight and dpost go to row t of
-// a.dw_part / a.dpost_part (fp32 [teams, hidden]).
-template <typename T, int VEC, int NV, bool POST>
-__global__ void __launch_bounds__(NV * VEC > 16 ? 512 : 1024)
+// Persistent like the forward kernel. A team's sums for dweight and dpost go to its row of a.dw_part / a.dpost_part (fp32
+// [teams, hidden]). WHOLE: the stream is given in place of x and the residual.
+template <typename T, int VEC, int NV, bool POST, bool WHOLE, int THREADS, int BLOCKS, int DEPTH>
+__global__ void __launch_bounds__(THREADS, BLOCKS)
     block_norm_bwd_kernel(const __grid_constant__ BlockNormGrads a, int warps) {
   __shared__ float2 scratch[2 * kMaxWarps];
+  extern __shared__ uint8_t ring[];
   pdl_trigger();
   Team team(warps, scratch);
-  pdl_wait();
+  Rows<T, VEC, NV, WHOLE ? 3 : 4, DEPTH> rows(ring);
   const int per_block = blockDim.x / (32 * warps);
   const int teams = gridDim.x * per_block, self = blockIdx.x * per_block + team.index;
-  const int vecs = (a.hidden + VEC - 1) / VEC;
-  const float mean = 1.f / static_cast<float>(a.hidden);
-  const T* weight = static_cast<const T*>(a.weight);
-  const T* post = static_cast<const T*>(a.post);
-  float dw[NV][VEC], dp[NV][POST ? VEC : 1];
+  const bool post = POST && a.post != nullptr;
+  const int gate_mode = WHOLE ? kGateNone : a.gate_mode;
+  const int hidden = a.hidden;
+  const float mean = 1.f / static_cast<float>(hidden);
+  const T* np = static_cast<const T*>(a.dnormed);
+  const T* up = static_cast<const T*>(a.dstream);
+  const T* xp = static_cast<const T*>(a.x);
+  const T* rp = static_cast<const T*>(WHOLE ? a.stream : a.residual);
+  const T* gp = static_cast<const T*>(a.gate);
+  const int64_t r_stride = WHOLE ? hidden : a.r_stride;
+  auto start = [&](int slot, int row) {
+    const bool on = row < a.rows;
+    rows.start(slot, 0, on && np != nullptr ? np + row * a.dn_stride : nullptr, team.first, team.step, hidden);
+    rows.start(slot, 1, on && up != nullptr ? up + row * a.ds_stride : nullptr, team.first, team.step, hidden);
+    rows.start(slot, 2, on && rp != nullptr ? rp + row * r_stride : nullptr, team.first, team.step, hidden);
+    if constexpr (!WHOLE) rows.start(slot, 3, on ? xp + row * a.x_stride : nullptr, team.first, team.step, hidden);
+    rows.commit();
+  };
+  pdl_wait();
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int d = 0; d < DEPTH; ++d) start(d, self + d * teams);
+  Pack<T, VEC> w[NV], p[POST ? NV : 1];
+  float dw[NV][VEC], dp[POST ? NV : 1][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int at = (team.first + i * team.step) * VEC;
+    w[i].fetch(static_cast<const T*>(a.weight), at, hidden);
+    if constexpr (POST) p[i].fetch(static_cast<const T*>(a.post), at, hidden);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       dw[i][j] = 0.f;
-      if (POST) dp[i][j] = 0.f;
+      if constexpr (POST) dp[i][j] = 0.f;
     }
+  }
   for (int row = self; row < a.rows; row += teams) {
-    const float is = a.inv_s[row], ix = POST ? a.inv_x[row] : 1.f;
+    const float is = a.inv_s[row], ix = post ? a.inv_x[row] : 1.f;
     float gate = a.scale;  // scale times the token's gate
-    if (a.gate_mode == kGateToken) gate *= Cast<T>::to(static_cast<const T*>(a.gate)[row * a.gate_stride]);
-    // sh: the normalised stream; ds: the upstream gradient of the stream
-    float sh[NV][VEC], g[NV][VEC], ds[NV][VEC];
-    Pack<T, VEC> x[NV];
+    if (gate_mode == kGateToken) gate *= Cast<T>::to(gp[row * a.gate_stride]);
+    if constexpr (DEPTH == 0) start(0, row);
+    rows.wait();
+    float sh[NV][VEC];  // the normalised stream
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int v = team.first + i * team.step;
-      const size_t at = static_cast<size_t>(v) * VEC;
-      Pack<T, VEC> dn, up, r, w, p, fg;
-      x[i].zero();
-      dn.zero();
-      up.zero();
-      r.zero();
-      w.zero();
-      if (v < vecs) {
-        if (a.dnormed != nullptr) dn.load(static_cast<const T*>(a.dnormed) + row * a.dn_stride + at);
-        if (a.dstream != nullptr) up.load(static_cast<const T*>(a.dstream) + row * a.ds_stride + at);
-        if (a.stream != nullptr) r.load(static_cast<const T*>(a.stream) + static_cast<size_t>(row) * a.hidden + at);
-        else if (a.residual != nullptr) r.load(static_cast<const T*>(a.residual) + row * a.r_stride + at);
-        if (a.stream == nullptr) x[i].load(static_cast<const T*>(a.x) + row * a.x_stride + at);
-        w.load(weight + at);
-      }
-      if (POST && v < vecs) p.load(post + at);
-      if (a.gate_mode == kGateFull && v < vecs) fg.load(static_cast<const T*>(a.gate) + row * a.gate_stride + at);
+      const int at = (team.first + i * team.step) * VEC;
+      Pack<T, VEC> dn, r, x, fg;
+      rows.get(dn, 0, i, at, hidden);
+      rows.get(r, 2, i, at, hidden);
+      if constexpr (!WHOLE) rows.get(x, 3, i, at, hidden);
+      if (gate_mode == kGateFull) fg.fetch(gp + row * a.gate_stride, at, hidden);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         float s = r.get(j);
-        if (a.stream == nullptr) {
-          float b = x[i].get(j);
-          if (POST) b *= ix * (v < vecs ? p.get(j) : 0.f);
-          if (a.gate_mode == kGateFull) b *= v < vecs ? fg.get(j) : 0.f;
+        if constexpr (!WHOLE) {
+          float b = x.get(j);
+          if (POST && post) b *= ix * p[POST ? i : 0].get(j);
+          if (gate_mode == kGateFull) b *= fg.get(j);
           s = fmaf(gate, b, s);
         }
         sh[i][j] = s * is;
         dw[i][j] = fmaf(dn.get(j), sh[i][j], dw[i][j]);
-        g[i][j] = dn.get(j) * w.get(j);
-        dot = fmaf(g[i][j], sh[i][j], dot);
-        ds[i][j] = up.get(j);
+        dot = fmaf(dn.get(j) * w[i].get(j), sh[i][j], dot);
       }
     }
     dot = team.sum(dot) * mean;
     float2 sums = make_float2(0.f, 0.f);  // h . xh and the token gate's gradient
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int v = team.first + i * team.step;
-      const size_t at = static_cast<size_t>(v) * VEC;
-      Pack<T, VEC> p, fg, out, dg;
-      if (POST && v < vecs) p.load(post + at);
-      if (a.gate_mode == kGateFull && v < vecs) fg.load(static_cast<const T*>(a.gate) + row * a.gate_stride + at);
+      const int at = (team.first + i * team.step) * VEC;
+      Pack<T, VEC> dn, u, x, fg, out, dg;
+      rows.get(dn, 0, i, at, hidden);
+      rows.get(u, 1, i, at, hidden);
+      if constexpr (!WHOLE) rows.get(x, 3, i, at, hidden);
+      if (gate_mode == kGateFull) fg.fetch(gp + row * a.gate_stride, at, hidden);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        ds[i][j] += is * (g[i][j] - sh[i][j] * dot);
-        out.set(j, ds[i][j]);
-        const float xh = x[i].get(j) * ix;
-        const float pw = POST ? (v < vecs ? p.get(j) : 0.f) : 1.f;
-        const float b = xh * pw;  // without POST ix is 1
-        float db = gate * ds[i][j];
-        if (a.gate_mode == kGateFull) {
-          dg.set(j, db * b);
-          db *= v < vecs ? fg.get(j) : 0.f;
-        } else if (a.gate_mode == kGateToken) {
-          sums.y = fmaf(b, ds[i][j], sums.y);
+        const float ds = fmaf(is, dn.get(j) * w[i].get(j) - sh[i][j] * dot, u.get(j));
+        out.set(j, ds);
+        float db = gate * ds;
+        if constexpr (!WHOLE) {
+          const float xh = x.get(j) * ix;  // without a norm behind the block ix is 1
+          const float pw = POST && post ? p[POST ? i : 0].get(j) : 1.f;
+          if (gate_mode == kGateFull) {
+            dg.set(j, a.scale * ds * (xh * pw));
+            db *= fg.get(j);
+          } else if (gate_mode == kGateToken) {
+            sums.y = fmaf(xh * pw, ds, sums.y);
+          }
+          if (POST && post) {
+            dp[POST ? i : 0][j] = fmaf(db, xh, dp[POST ? i : 0][j]);
+            db *= pw;  // h
+            sums.x = fmaf(db, xh, sums.x);
+          }
         }
-        if (POST) {
-          dp[i][j] = fmaf(db, xh, dp[i][j]);
-          g[i][j] = db * pw;  // h
-          sums.x = fmaf(g[i][j], xh, sums.x);
-        } else {
-          g[i][j] = db;
-        }
+        sh[i][j] = db;
       }
-      if (v < vecs) {
-        if (a.dresidual != nullptr)
-          out.store(static_cast<T*>(a.dresidual) + static_cast<size_t>(row) * a.hidden + at);
-        if (a.gate_mode == kGateFull && a.dgate != nullptr)
-          dg.store(static_cast<T*>(a.dgate) + static_cast<size_t>(row) * a.hidden + at);
-      }
+      if (a.dresidual != nullptr) out.store(static_cast<T*>(a.dresidual) + static_cast<size_t>(row) * hidden, at, hidden);
+      if (gate_mode == kGateFull && a.dgate != nullptr)
+        dg.store(static_cast<T*>(a.dgate) + static_cast<size_t>(row) * hidden, at, hidden);
     }
-    if (POST || a.gate_mode == kGateToken) {
-      sums = team.sum(sums);
-      if (a.gate_mode == kGateToken && a.dgate != nullptr && team.first == 0)
-        static_cast<T*>(a.dgate)[row] = Cast<T>::from(a.scale * sums.y);
+    if constexpr (!WHOLE) {
+      if ((POST && post) || gate_mode == kGateToken) {
+        sums = team.sum(sums);
+        if (gate_mode == kGateToken && a.dgate != nullptr && team.first == 0)
+          static_cast<T*>(a.dgate)[row] = Cast<T>::from(a.scale * sums.y);
+      }
     }
     if (a.dx != nullptr) {
+      const float m = sums.x * mean;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int v = team.first + i * team.step;
-        if (v < vecs) {
-          Pack<T, VEC> out;
+        const int at = (team.first + i * team.step) * VEC;
+        Pack<T, VEC> x, out;
+        if (POST && post) rows.get(x, WHOLE ? 0 : 3, i, at, hidden);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j)
-            out.set(j, POST ? ix * (g[i][j] - x[i].get(j) * ix * (sums.x * mean)) : g[i][j]);
-          out.store(static_cast<T*>(a.dx) + static_cast<size_t>(row) * a.hidden + static_cast<size_t>(v) * VEC);
-        }
+        for (int j = 0; j < VEC; ++j)
+          out.set(j, POST && post ? ix * (sh[i][j] - x.get(j) * ix * m) : sh[i][j]);
+        out.store(static_cast<T*>(a.dx) + static_cast<size_t>(row) * hidden, at, hidden);
       }
+    }
+    if constexpr (DEPTH > 0) {
+      start(rows.slot, row + DEPTH * teams);
+      rows.slot = rows.slot + 1 == DEPTH ? 0 : rows.slot + 1;
     }
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int v = team.first + i * team.step;
+    const int at = (team.first + i * team.step) * VEC;
+    const size_t to = static_cast<size_t>(self) * hidden + at;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      const int c = v * VEC + j;
-      if (v < vecs && c < a.hidden) {
-        if (a.dw_part != nullptr) a.dw_part[static_cast<size_t>(self) * a.hidden + c] = dw[i][j];
-        if (POST && a.dpost_part != nullptr) a.dpost_part[static_cast<size_t>(self) * a.hidden + c] = dp[i][j];
-      }
+      if (at + j >= hidden) continue;
+      if (a.dw_part != nullptr) a.dw_part[to + j] = dw[i][j];
+      if (POST && a.dpost_part != nullptr) a.dpost_part[to + j] = dp[i][j];
     }
   }
 }
 
-// Columns of `parts` rows of fp32 added up in order: eight threads per column take every eighth row each.
+// Columns of `parts` rows of fp32 added up in order: 32 threads a column take every 32nd row each, then one adds theirs.
 template <typename T>
-__global__ void __launch_bounds__(256) block_norm_sum_kernel(const float* __restrict__ dw_part,
-                                                             const float* __restrict__ dpost_part, T* dw, T* dpost,
-                                                             int parts, int hidden) {
-  __shared__ float sums[8][32];
+__global__ void __launch_bounds__(1024) block_norm_sum_kernel(const float* __restrict__ dw_part,
+                                                              const float* __restrict__ dpost_part, T* dw, T* dpost,
+                                                              int parts, int hidden) {
+  __shared__ float sums[32][33];
   pdl_trigger();
-  pdl_wait();
   const float* part = blockIdx.y == 0 ? dw_part : dpost_part;
   T* out = blockIdx.y == 0 ? dw : dpost;
+  const int lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, group = threadIdx.x >> 5;
+  pdl_wait();
   if (out == nullptr) return;
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;
   float s = 0.f;
-  if (c < hidden)
-    for (int p = lane; p < parts; p += 8) s += part[static_cast<size_t>(p) * hidden + c];
-  sums[lane][threadIdx.x & 31] = s;
+  if (c < hidden) {
+#pragma unroll 4
+    for (int p = group; p < parts; p += 32) s += part[static_cast<size_t>(p) * hidden + c];
+  }
+  sums[group][lane] = s;
   __syncthreads();
-  if (threadIdx.x < 32 && c < hidden) {
+  if (group == 0 && c < hidden) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += sums[i][threadIdx.x];
+    for (int i = 1; i < 32; ++i) s += sums[i][lane];
     out[c] = Cast<T>::from(s);
   }
 }
 
+// The layout depends on the row's length alone, so a row's sums do not depend on how many rows there are.
 struct Grid {
-  int warps, nv, teams;  // warps of a team, vectors a lane, teams of a block
+  int warps, nv, teams, threads;  // warps of a team, vectors a lane, teams and threads of a block
 };
 
-// Teams that hold a row of `vecs` vectors with about `target` vectors a lane.
-Grid teams_of(int vecs, int target, int block_warps) {
-  const int all = (vecs + 31) / 32;
+// 32 bytes a lane (fp32 rows of more than 8192: 64), or four single elements (16 where those are more than 1024 lanes
+// hold); several teams to a block of 256 threads, or one.
+template <typename T, int VEC>
+Grid grid_of(int hidden) {
+  const int all = (hidden + 32 * VEC - 1) / (32 * VEC), target = VEC == 1 ? 4 : 1;
   Grid g;
-  g.warps = std::min(kMaxWarps, std::max(1, (all + target - 1) / target));
-  if (g.warps <= block_warps) {
+  g.warps = std::min(kMaxWarps, (all + target - 1) / target);
+  if (g.warps <= 8) {
     int p = 1;
     while (p < g.warps) p *= 2;
     g.warps = p;
   }
   g.nv = (all + g.warps - 1) / g.warps;
-  g.teams = g.warps < block_warps ? block_warps / g.warps : 1;
+  g.teams = g.warps <= 8 ? 8 / g.warps : 1;
+  g.threads = 32 * g.warps * g.teams;
   return g;
 }
 
-template <typename T, int VEC, int FMT>
-int run_forward(const BlockNormArgs& a, int sms, cudaStream_t stream) {
-  const int vecs = FMT == 0 ? (a.hidden + VEC - 1) / VEC : a.tiles * fp4::Format<FMT == 0 ? fp4::kNv : FMT>::kWordLanes;
-  const bool many = a.rows >= 4 * sms;
-  const Grid g = teams_of(vecs, many ? 4 : 1, many ? 8 : 1);
+template <typename T>
+constexpr int vec_of() { return 32 / static_cast<int>(sizeof(T)); }
+
+constexpr int kFwdBlocks = 3, kBwdBlocks = 2;  // of 256 threads on an SM
+
+template <class Ring, class Kernel, class Args>
+int go(Kernel kernel, int blocks, const Grid& g, const Args& a, cudaStream_t stream) {
+  const int smem = Ring::bytes(g.threads);
+  if (set_max_smem(kernel, smem) != cudaSuccess) return -1;
+  return launch_pdl(kernel, dim3(blocks), dim3(g.threads), smem, stream, a, g.warps) == cudaSuccess ? 0 : -1;
+}
+
+template <typename T, int VEC, int NV, int FMT, bool POST, int THREADS, int BLOCKS, int DEPTH>
+int go_forward(const BlockNormArgs& a, const Grid& g, int sms, cudaStream_t stream) {
   const int rows = FMT == 0 ? a.rows : (a.rows + 127) / 128 * 128;
-  const dim3 grid((rows + g.teams - 1) / g.teams), block(32 * g.warps * g.teams);
-  auto go = [&](auto kernel) { return launch_pdl(kernel, grid, block, 0, stream, a, g.warps) == cudaSuccess ? 0 : -1; };
-  if (g.nv <= 1) return go(block_norm_kernel<T, VEC, 1, FMT>);
-  if (g.nv <= 2) return go(block_norm_kernel<T, VEC, 2, FMT>);
-  if (g.nv <= 4) return go(block_norm_kernel<T, VEC, 4, FMT>);
-  if constexpr (VEC == 1) {
-    if (g.nv <= 8) return go(block_norm_kernel<T, VEC, 8, FMT>);
-    if (g.nv <= 16) return go(block_norm_kernel<T, VEC, 16, FMT>);
-  }
+  const int resident = THREADS <= 256 ? BLOCKS : 1024 / g.threads;
+  return go<Rows<T, VEC, NV, 2, DEPTH>>(block_norm_kernel<T, VEC, NV, FMT, POST, THREADS, BLOCKS, DEPTH>,
+                                        std::min((rows + g.teams - 1) / g.teams, sms * resident), g, a, stream);
+}
+
+template <typename T, int FMT, bool POST>
+int run_forward(const BlockNormArgs& a, int sms, cudaStream_t stream) {
+  constexpr int V = vec_of<T>();
+  // 4-bit results: lanes cover the scales' padding too
+  const Grid g = grid_of<T, V>(FMT == 0 ? a.hidden : (a.hidden + fp4::kBlockK - 1) / fp4::kBlockK * fp4::kBlockK);
+  if (g.threads <= 256) return go_forward<T, V, 1, FMT, POST, 256, kFwdBlocks, 3>(a, g, sms, stream);
+  if (g.nv == 1) return go_forward<T, V, 1, FMT, POST, 1024, 1, 2>(a, g, sms, stream);
+  if constexpr (sizeof(T) == 4) return go_forward<T, V, 2, FMT, POST, 1024, 1, 1>(a, g, sms, stream);
   return -1;
 }
 
 template <typename T>
 int run_forward_type(const BlockNormArgs& a, bool vec, int sms, cudaStream_t stream) {
-  constexpr int V = 16 / sizeof(T);
-  return vec ? run_forward<T, V, 0>(a, sms, stream) : run_forward<T, 1, 0>(a, sms, stream);
+  if (vec) return a.post != nullptr ? run_forward<T, 0, true>(a, sms, stream) : run_forward<T, 0, false>(a, sms, stream);
+  const Grid g = grid_of<T, 1>(a.hidden);
+  if (g.nv <= 4) return go_forward<T, 1, 4, 0, true, 1024, 1, 0>(a, g, sms, stream);
+  return go_forward<T, 1, 16, 0, true, 1024, 1, 0>(a, g, sms, stream);
 }
 
-constexpr int kBwdBlockWarps = 8;
-
-template <typename T, int VEC>
-Grid backward_grid(int hidden) {
-  return teams_of((hidden + VEC - 1) / VEC, VEC == 8 ? 2 : 4, kBwdBlockWarps);
+template <int FMT>
+int run_forward_fp4(const BlockNormArgs& a, int sms, cudaStream_t stream) {
+  return a.post != nullptr ? run_forward<bf16, FMT, true>(a, sms, stream) : run_forward<bf16, FMT, false>(a, sms, stream);
 }
 
 int backward_blocks(const Grid& g, int rows, int sms) {
-  const int resident = std::max(1, 16 / (g.warps * g.teams));
-  return std::min((rows + g.teams - 1) / g.teams, sms * resident);
+  return std::min((rows + g.teams - 1) / g.teams, sms * (g.threads <= 256 ? kBwdBlocks : 1));
 }
 
-template <typename T, int VEC>
-int run_backward(const BlockNormGrads& a, int sms, cudaStream_t stream) {
-  const Grid g = backward_grid<T, VEC>(a.hidden);
-  const dim3 grid(backward_blocks(g, a.rows, sms)), block(32 * g.warps * g.teams);
-  auto go = [&](auto kernel) { return launch_pdl(kernel, grid, block, 0, stream, a, g.warps) == cudaSuccess ? 0 : -1; };
-  int rc = -1;
-  auto pick = [&](auto post) {
-    constexpr bool P = decltype(post)::value;
-    if (g.nv <= 1) return go(block_norm_bwd_kernel<T, VEC, 1, P>);
-    if (g.nv <= 2) return go(block_norm_bwd_kernel<T, VEC, 2, P>);
-    if constexpr (VEC <= 4) {
-      if (g.nv <= 4) return go(block_norm_bwd_kernel<T, VEC, 4, P>);
-    }
-    if constexpr (VEC == 1) {
-      if (g.nv <= 8) return go(block_norm_bwd_kernel<T, VEC, 8, P>);
-      if (g.nv <= 16) return go(block_norm_bwd_kernel<T, VEC, 16, P>);
-    }
-    return -1;
-  };
-  rc = a.post != nullptr ? pick(std::true_type{}) : pick(std::false_type{});
-  if (rc != 0 || (a.dweight == nullptr && a.dpost == nullptr)) return rc;
-  return launch_pdl(block_norm_sum_kernel<T>, dim3((a.hidden + 31) / 32, a.dpost != nullptr ? 2 : 1), dim3(256), 0, stream,
-                    static_cast<const float*>(a.dw_part), static_cast<const float*>(a.dpost_part),
-                    static_cast<T*>(a.dweight), static_cast<T*>(a.dpost), static_cast<int>(grid.x) * g.teams,
-                    a.hidden) == cudaSuccess ? 0 : -1;
+template <typename T, int VEC, int NV, bool POST, bool WHOLE, int THREADS, int BLOCKS, int DEPTH>
+int go_backward(const BlockNormGrads& a, const Grid& g, int sms, cudaStream_t stream) {
+  return go<Rows<T, VEC, NV, WHOLE ? 3 : 4, DEPTH>>(
+      block_norm_bwd_kernel<T, VEC, NV, POST, WHOLE, THREADS, BLOCKS, DEPTH>, backward_blocks(g, a.rows, sms), g, a, stream);
+}
+
+template <typename T, bool POST, bool WHOLE>
+int run_backward(const BlockNormGrads& a, const Grid& g, int sms, cudaStream_t stream) {
+  constexpr int V = vec_of<T>();
+  if (g.threads <= 256) return go_backward<T, V, 1, POST, WHOLE, 256, kBwdBlocks, 3>(a, g, sms, stream);
+  if (g.threads <= 512) return go_backward<T, V, 1, POST, WHOLE, 512, 1, 2>(a, g, sms, stream);
+  if (g.nv == 1) return go_backward<T, V, 1, POST, WHOLE, 1024, 1, 1>(a, g, sms, stream);
+  if constexpr (sizeof(T) == 4) return go_backward<T, V, 2, POST, WHOLE, 1024, 1, 0>(a, g, sms, stream);
+  return -1;
+}
+
+template <typename T, bool WHOLE>
+int run_backward_single(const BlockNormGrads& a, const Grid& g, int sms, cudaStream_t stream) {
+  if (g.threads <= 256) return go_backward<T, 1, 4, !WHOLE, WHOLE, 256, kBwdBlocks, 0>(a, g, sms, stream);
+  if (g.nv <= 4) return go_backward<T, 1, 4, !WHOLE, WHOLE, 1024, 1, 0>(a, g, sms, stream);
+  return go_backward<T, 1, 16, !WHOLE, WHOLE, 1024, 1, 0>(a, g, sms, stream);
+}
+
+template <typename T>
+Grid backward_grid(int hidden, bool vec) {
+  return vec ? grid_of<T, vec_of<T>()>(hidden) : grid_of<T, 1>(hidden);
 }
 
 template <typename T>
 int run_backward_type(const BlockNormGrads& a, bool vec, int sms, cudaStream_t stream) {
-  constexpr int V = 16 / sizeof(T);
-  return vec ? run_backward<T, V>(a, sms, stream) : run_backward<T, 1>(a, sms, stream);
+  const Grid g = backward_grid<T>(a.hidden, vec);
+  const bool whole = a.stream != nullptr;
+  int rc;
+  if (vec)
+    rc = whole               ? run_backward<T, false, true>(a, g, sms, stream)
+         : a.post != nullptr ? run_backward<T, true, false>(a, g, sms, stream)
+                             : run_backward<T, false, false>(a, g, sms, stream);
+  else
+    rc = whole ? run_backward_single<T, true>(a, g, sms, stream) : run_backward_single<T, false>(a, g, sms, stream);
+  if (rc != 0 || (a.dweight == nullptr && a.dpost == nullptr)) return rc;
+  return launch_pdl(block_norm_sum_kernel<T>, dim3((a.hidden + 31) / 32, a.dpost != nullptr ? 2 : 1), dim3(1024), 0, stream,
+                    static_cast<const float*>(a.dw_part), static_cast<const float*>(a.dpost_part),
+                    static_cast<T*>(a.dweight), static_cast<T*>(a.dpost), backward_blocks(g, a.rows, sms) * g.teams,
+                    a.hidden) == cudaSuccess ? 0 : -1;
 }
 
 template <typename T>
 int parts_type(int rows, int hidden, bool vec, int sms) {
-  constexpr int V = 16 / sizeof(T);
-  const Grid g = vec ? backward_grid<T, V>(hidden) : backward_grid<T, 1>(hidden);
+  const Grid g = backward_grid<T>(hidden, vec);
   return backward_blocks(g, rows, sms) * g.teams;
 }
 
@@ -487,7 +621,7 @@ int launch_block_norm(const BlockNormArgs& a, NormType type, bool vec, int fmt, 
   if (a.rows < 1 || a.hidden < 1 || a.hidden > kBlockNormMaxHidden) return -1;
   if (fmt != 0) {
     if (type != kNormBf16 || !vec || a.hidden % 32 != 0) return -1;
-    return fmt == fp4::kNv ? run_forward<bf16, 8, fp4::kNv>(a, sms, stream) : run_forward<bf16, 8, fp4::kMx>(a, sms, stream);
+    return fmt == fp4::kNv ? run_forward_fp4<fp4::kNv>(a, sms, stream) : run_forward_fp4<fp4::kMx>(a, sms, stream);
   }
   switch (type) {
     case kNormBf16: return run_forward_type<bf16>(a, vec, sms, stream);

@@ -8,9 +8,14 @@
 #pragma once
 
 #include "common.cuh"
+#include "packed_common.cuh"
 
 namespace ecz {
 namespace fp4 {
+
+using packed::add2;
+using packed::fma2;
+using packed::pair_of;
 
 constexpr int kNv = 1, kMx = 2;   // formats
 constexpr int kBlockK = 256;      // columns of a K block (a 128-byte row of codes)
@@ -21,8 +26,6 @@ struct Format {
   static constexpr int kGroup = FMT == kNv ? 16 : 32;
   static constexpr int kTilesPerBlock = kBlockK / (4 * kGroup);           // 4 (nvfp4), 2 (mxfp4)
   static constexpr int kBlockBytes = kTilesPerBlock * kTileBytes;         // scales of 128 rows x 256 columns
-  static constexpr int kLanes = kGroup / 8;                               // lanes of 8 columns that share a scale
-  static constexpr int kWordLanes = 4 * kLanes;                           // ... that share a 4-byte word of scales
 };
 
 // Byte offset of the word that holds the scales of row `row`, groups 4 t .. 4 t + 3; `tiles` of them along K.
@@ -41,34 +44,73 @@ __device__ __forceinline__ int row_exponent(float amax) {
   return min(max(e, -100), 120);
 }
 
-// Eight e2m1 codes of v * r, the first in the lowest nibble. r is the rounded reciprocal of the scale, so v * r misses the
-// quotient by 2^-23 of it at most; the quotient of a bf16 value by an e4m3 scale (or a power of two) is either a tie
-// between two codes or at least 2^-10 away from it, so rounding the product to multiples of 2^-14 first (adding and
-// subtracting 1.5 * 2^9) lands on ties where they are and moves nothing else across. Beyond
-// 6 all become 6.
-__device__ __forceinline__ uint32_t codes8(const float* v, float r) {
-  float q[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) q[i] = __fsub_rn(__fmaf_rn(v[i], r, 768.f), 768.f);
-  uint32_t out;
-  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
-      "mov.b32 %0, {a, b, c, d};\n\t}"
-      : "=r"(out)
-      : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
-  return out;
+// ---- vectors of packed bf16 ----------------------------------------------------------------------------------------
+// 32 bytes (16 bf16) from a 32-byte boundary.
+__device__ __forceinline__ void load32(const void* p, uint32_t* v) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void store32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
-__device__ __forceinline__ void unpack8(const uint4& raw, float* v) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+__device__ __forceinline__ float low_bf16(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float high_bf16(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+
+// Largest magnitude of 2 W packed bf16, as the bits of a bf16: they order like the magnitudes, 0x7f80 and above are not
+// finite.
+template <int W>
+__device__ __forceinline__ uint32_t max_bits(const uint32_t* v) {
+  uint32_t m = v[0] & 0x7fff7fffu;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __bfloat1622float2(h[i]);
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
+  for (int i = 1; i < W; ++i) m = __vmaxu2(m, v[i] & 0x7fff7fffu);
+  return max(m & 0xffffu, m >> 16);
+}
+
+// The same of the finite ones alone.
+template <int W>
+__device__ __forceinline__ uint32_t finite_bits(const uint32_t* v) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    const uint32_t lo = v[i] & 0x7fffu, hi = (v[i] >> 16) & 0x7fffu;
+    m = max(m, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+  }
+  return m;
+}
+
+__device__ __forceinline__ float bits_value(uint32_t bf16_bits) { return __uint_as_float(bf16_bits << 16); }
+
+// ---- scales --------------------------------------------------------------------------------------------------------
+// The scale byte of a group with largest magnitude `bits` (max_bits) and the factor that its values are multiplied with
+// to become codes; mul (nvfp4): the reciprocal of the row's power of two, exact. A group with a value that is not finite
+// has the format's NaN as its scale, which makes every product that reads it NaN.
+template <int FMT>
+__device__ __forceinline__ uint32_t group_scale(uint32_t bits, float mul, float& factor) {
+  const bool bad = bits >= 0x7f80u;
+  const float m = bits_value(bits);
+  if constexpr (FMT == kMx) {
+    // exponent of m, one more from a mantissa of 1.75 on, less 2; 2^-126 <= scale <= 2^125
+    int e = static_cast<int>((__float_as_uint(m) + 0x200000u) >> 23) - 127 - 2;
+    e = min(max(e, -126), 125);
+    factor = pow2(-e);
+    return bad ? 0xffu : static_cast<uint32_t>(e + 127);
+  } else {
+    // m / 6, off by 2^-23 of itself, then rounded to 12 bits (t (2^12 + 1) less its own low part): ties between e4m3
+    // values, which have 5 bits, land where they are, and other quotients of an 8-bit number are 2^-8 of themselves away
+    const float t = m * mul * 0.166666671633720398f, c = __fmul_rn(t, 4097.f);
+    const float q = fmaxf(__fsub_rn(c, __fsub_rn(c, t)), 0.001953125f);
+    uint16_t pair;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(pair) : "f"(0.f), "f"(q));
+    uint32_t halves;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(halves) : "h"(pair));
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__low2float(*reinterpret_cast<const __half2*>(&halves))));
+    factor = r * mul;
+    return bad ? 0x7fu : static_cast<uint32_t>(pair & 0xffu);
   }
 }
 
@@ -84,103 +126,63 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
   }
 }
 
-// Eight codes times s, as bf16.
-__device__ __forceinline__ uint4 values8(uint32_t codes, float s) {
+// ---- codes ---------------------------------------------------------------------------------------------------------
+// Codes of eight packed bf16 times f, the first in the lowest nibble. f is the reciprocal of the scale, so the product
+// misses the quotient by 2^-22 of it at most; the quotient of a bf16 value by an e4m3 scale (or a power of two) is either
+// a tie between two codes or at least 2^-10 away from it, so rounding the product to multiples of 2^-14 first (adding and
+// subtracting 768) lands on ties where they are and moves nothing else across. Beyond 6 all become 6.
+__device__ __forceinline__ uint32_t codes8(const uint32_t* v, float f) {
+  uint64_t q[4];
+  const uint64_t ff = pair_of(f, f), up = pair_of(768.f, 768.f), down = pair_of(-768.f, -768.f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = add2(fma2(pair_of(low_bf16(v[i]), high_bf16(v[i])), ff, up), down);
+  uint32_t out;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t.reg .f32 l, h;\n\t"
+      "mov.b64 {l, h}, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 a, h, l;\n\t"
+      "mov.b64 {l, h}, %2;\n\tcvt.rn.satfinite.e2m1x2.f32 b, h, l;\n\t"
+      "mov.b64 {l, h}, %3;\n\tcvt.rn.satfinite.e2m1x2.f32 c, h, l;\n\t"
+      "mov.b64 {l, h}, %4;\n\tcvt.rn.satfinite.e2m1x2.f32 d, h, l;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(out)
+      : "l"(q[0]), "l"(q[1]), "l"(q[2]), "l"(q[3]));
+  return out;
+}
+
+// Eight codes times s, as packed bf16.
+__device__ __forceinline__ void values8(uint32_t codes, float s, uint32_t* out) {
   uint32_t h[4];
   asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
       "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
       "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
       : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
       : "r"(codes));
-  uint4 out;
-  uint32_t* o = reinterpret_cast<uint32_t*>(&out);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
     const __nv_bfloat162 b = __floats2bfloat162_rn(f.x * s, f.y * s);
-    o[i] = *reinterpret_cast<const uint32_t*>(&b);
+    out[i] = *reinterpret_cast<const uint32_t*>(&b);
   }
-  return out;
 }
 
-// Largest magnitude of the finite ones of eight values, and whether any is not finite.
-__device__ __forceinline__ float finite_max8(const float* v, bool& bad) {
-  float m = 0.f;
-  bad = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = fabsf(v[i]);
-    const bool fin = a < __int_as_float(0x7f800000);
-    bad |= !fin;
-    m = fmaxf(m, fin ? a : 0.f);
-  }
-  return m;
-}
-
-// Maximum over the lanes of a group (aligned lanes).
+// ---- a lane's 16 columns -------------------------------------------------------------------------------------------
+// Quantises the 16 columns (v: packed bf16) at 16 `vec` of row `row` and stores codes and scale; mxfp4: two neighbouring
+// lanes hold a group, and both lanes of the pair call. Columns from 16 `vecs` on are padding of the scales (v zero).
 template <int FMT>
-__device__ __forceinline__ float group_max(float m) {
-#pragma unroll
-  for (int o = 1; o < Format<FMT>::kLanes; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return m;
-}
-
-// The scale byte of a group with largest finite magnitude `m` (nvfp4: in units of the row's power of two) and the
-// reciprocal that its values are multiplied with. A group with a value that is not finite has the format's NaN as its
-// scale, which makes every product that reads it NaN.
-template <int FMT>
-__device__ __forceinline__ uint32_t group_scale(float m, bool bad, float& recip) {
-  if constexpr (FMT == kMx) {
-    // exponent of m, one more from a mantissa of 1.75 on, less 2; 2^-126 <= scale <= 2^125
-    int e = static_cast<int>((__float_as_uint(m) + 0x200000u) >> 23) - 127 - 2;
-    e = min(max(e, -126), 125);
-    recip = pow2(-e);
-    return bad ? 0xffu : static_cast<uint32_t>(e + 127);
+__device__ __forceinline__ void store16(const uint32_t* v, float mul, int row, int vec, int vecs, int tiles,
+                                        uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  uint32_t bits = max_bits<8>(v);
+  if constexpr (FMT == kMx) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 1));
+  float factor;
+  uint32_t byte = group_scale<FMT>(bits, mul, factor);
+  if (vec < vecs) {
+    *reinterpret_cast<uint2*>(codes + (static_cast<size_t>(row) * vecs + vec) * 8) =
+        make_uint2(codes8(v, factor), codes8(v + 4, factor));
   } else {
-    const float t = fmaxf(__fdiv_rn(m, 6.f), 0.001953125f);
-    uint16_t pair;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(pair) : "f"(0.f), "f"(t));
-    uint32_t halves;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(halves) : "h"(pair));
-    const __half2 h = *reinterpret_cast<const __half2*>(&halves);
-    recip = __frcp_rn(__low2float(h));
-    return bad ? 0x7fu : static_cast<uint32_t>(pair & 0xffu);
+    byte = 0;
   }
-}
-
-// Quantise the eight columns of this lane and store them: lane l of the warp holds vector `vec` (columns 8 vec ..) of
-// row `row`, consecutive lanes consecutive vectors from a multiple of 32; `live`: vec < vecs (others hold zeros and are
-// padding of the scales). mul (nvfp4): the reciprocal of the row's power of two. All lanes take part.
-template <int FMT>
-__device__ __forceinline__ void store8(const float* v, float mul, int row, int vec, int vecs, int tiles,
-                                       uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  using F = Format<FMT>;
-  const bool live = vec < vecs;
-  bool bad;
-  const float m = group_max<FMT>(finite_max8(v, bad));
-  const unsigned votes = __ballot_sync(0xffffffffu, bad);
-  const int lane = threadIdx.x & 31;
-  const unsigned mates = ((1u << F::kLanes) - 1u) << (lane & ~(F::kLanes - 1));
-  float recip;
-  uint32_t byte = group_scale<FMT>(FMT == kNv ? m * mul : m, (votes & mates) != 0, recip);
-  if (!live) byte = 0;  // groups do not straddle the end: K is a multiple of 32
-  if (live) {
-    if constexpr (FMT == kNv) {
-      float scaled[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) scaled[i] = v[i] * mul;  // exact: a power of two
-      *reinterpret_cast<uint32_t*>(codes + (static_cast<size_t>(row) * vecs + vec) * 4) = codes8(scaled, recip);
-    } else {
-      *reinterpret_cast<uint32_t*>(codes + (static_cast<size_t>(row) * vecs + vec) * 4) = codes8(v, recip);
-    }
-  }
-  // four groups' bytes to one word, stored by the first of their lanes
-  uint32_t word = byte << (8 * ((lane / F::kLanes) & 3));
-#pragma unroll
-  for (int o = F::kLanes; o < F::kWordLanes; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
-  const int t = vec / F::kWordLanes;
-  if ((lane & (F::kWordLanes - 1)) == 0 && t < tiles)
-    *reinterpret_cast<uint32_t*>(scales + scale_word(row, t, tiles)) = word;
+  constexpr int kLanes = Format<FMT>::kGroup / 16;
+  const int g = vec / kLanes;
+  if ((kLanes == 1 || (vec & 1) == 0) && (g >> 2) < tiles) scales[scale_word(row, g >> 2, tiles) + (g & 3)] = byte;
 }
 
 // ---- block-scaled MMAs ---------------------------------------------------------------------------------------------

@@ -29,6 +29,7 @@ constexpr int kRowBytes = kBlockK / 2;  // a K block of codes
 constexpr int kABytes = kBM * kRowBytes;
 constexpr int kThreads = 192;
 constexpr int kSlots = 3;  // places for scales in tensor memory
+constexpr int kMaxSplits = 8;
 
 template <int FMT>
 __device__ __forceinline__ void umma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
@@ -60,11 +61,13 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-__device__ __forceinline__ float ld_dsmem(uint32_t local_addr, uint32_t rank) {
+// Four of CTA `rank`'s sums, at the address `local` has in this CTA's shared memory.
+__device__ __forceinline__ float4 ld_sums(uint32_t local, uint32_t rank) {
   uint32_t remote;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local_addr), "r"(rank));
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(remote) : "memory");
   return v;
 }
 
@@ -201,58 +204,72 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, BN>::kOcc)
   if (warp < 2 && *abort_flag) wait_ns(1000000);  // a wait gave up: copies in flight get time to land
   bool ok = true;
   const int quarter = warp & 3;
-  const int n = n0 + quarter * 32 + lane;
   const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
   if (warp >= 2) {
     ok = mbar_wait(acc_full, 0, args.status, kStatusWaitAccum, abort_flag);
     ok = __all_sync(0xffffffffu, ok) && !*abort_flag;
     tc_fence_after();
   }
-  const float rw = FMT == kNv && n < args.N ? args.w_row[n] : 1.f;
-  auto store = [&](int j, float v) {
-    const int m = m0 + j;
-    if (m < args.M && n < args.N) {
-      const float rx = FMT == kNv ? args.x_row[m] : 1.f;
-      args.y[static_cast<size_t>(m) * args.N + n] = __float2bfloat16(v * (rw * rx));
-    }
-  };
-  if (splits == 1) {
-    if (warp >= 2 && ok) {
+  // This CTA's sums [BN][128] go where its stages were (every copy has landed and was read); each CTA of the cluster then
+  // adds up and stores a share of the columns, four features a thread.
+  float* part = reinterpret_cast<float*>(smem);
+  const int cols = min(BN, args.M - m0);
+  if (warp >= 2) {
 #pragma unroll
-      for (int c = 0; c < BN; c += 16) {
-        if (m0 + c < args.M) {
-          float v[16];
-          tmem_ld16(taddr + c, v);
+    for (int c = 0; c < BN; c += 16) {
+      if (c < cols) {
+        float v[16];
+        if (ok && nkb > 0) tmem_ld16(taddr + c, v);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) store(c + j, v[j]);
-        }
+        for (int j = 0; j < 16; ++j) part[(c + j) * kBM + quarter * 32 + lane] = ok && nkb > 0 ? v[j] : 0.f;
       }
     }
-  } else {
-    // this CTA's sums [BN][128] where its stages were (every copy has landed and was read), then a share of the columns
-    float* part = reinterpret_cast<float*>(smem);
-    if (warp >= 2) {
-#pragma unroll
-      for (int c = 0; c < BN; c += 16) {
-        if (m0 + c < args.M) {
-          float v[16];
-          if (ok && nkb > 0) tmem_ld16(taddr + c, v);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) part[(c + j) * kBM + quarter * 32 + lane] = ok && nkb > 0 ? v[j] : 0.f;
-        }
-      }
-    }
-    cluster_sync();
-    if (warp >= 2) {
-      const uint32_t at = smem_u32(part) + (quarter * 32 + lane) * 4;
-      for (int j = split; j < BN && m0 + j < args.M; j += splits) {
-        float sum = 0.f;
-        for (int r = 0; r < splits; ++r) sum += ld_dsmem(at + j * kBM * 4, r);
-        store(j, sum);
-      }
-    }
-    cluster_sync();
   }
+  if (splits > 1) cluster_sync();
+  else __syncthreads();
+  {
+    const int n = n0 + lane * 4;
+    float4 rw = make_float4(1.f, 1.f, 1.f, 1.f);
+    if constexpr (FMT == kNv) {
+      if (n < args.N) rw.x = args.w_row[n];
+      if (n + 1 < args.N) rw.y = args.w_row[n + 1];
+      if (n + 2 < args.N) rw.z = args.w_row[n + 2];
+      if (n + 3 < args.N) rw.w = args.w_row[n + 3];
+    }
+    const uint32_t at = smem_u32(part) + lane * 16;
+    for (int j = split + warp * splits; j < cols; j += splits * (kThreads / 32)) {
+      float4 p[kMaxSplits];
+#pragma unroll
+      for (int r = 0; r < kMaxSplits; ++r)
+        if (r < splits) p[r] = splits > 1 ? ld_sums(at + j * kBM * 4, r)
+                                          : *reinterpret_cast<const float4*>(part + j * kBM + lane * 4);
+      float4 sum = p[0];
+#pragma unroll
+      for (int r = 1; r < kMaxSplits; ++r) {
+        if (r < splits) {
+          sum.x += p[r].x;
+          sum.y += p[r].y;
+          sum.z += p[r].z;
+          sum.w += p[r].w;
+        }
+      }
+      const float rx = FMT == kNv ? args.x_row[m0 + j] : 1.f;
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x * (rx * rw.x), sum.y * (rx * rw.y));
+      const __nv_bfloat162 hi = __floats2bfloat162_rn(sum.z * (rx * rw.z), sum.w * (rx * rw.w));
+      bf16* out = args.y + static_cast<size_t>(m0 + j) * args.N + n;
+      if (args.N % 4 == 0) {
+        if (n < args.N)
+          *reinterpret_cast<uint2*>(out) =
+              make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      } else {
+        if (n < args.N) out[0] = lo.x;
+        if (n + 1 < args.N) out[1] = lo.y;
+        if (n + 2 < args.N) out[2] = hi.x;
+        if (n + 3 < args.N) out[3] = hi.y;
+      }
+    }
+  }
+  if (splits > 1) cluster_sync();  // the others have read this CTA's sums
   tc_fence_before();
   __syncthreads();
   if (warp == 0) tmem_dealloc(tmem, C::kTmemCols);
@@ -313,7 +330,7 @@ int launch_gemm_fp4(const CUtensorMap* w, const CUtensorMap* x, const void* w_sc
   // splits by the weights' size alone, so that a row's sums do not depend on how many rows there are
   const int tiles = (N + kBM - 1) / kBM;
   int splits = 1;
-  while (splits < 8 && tiles * splits < sms && 2 * splits <= args.kblocks) splits *= 2;
+  while (splits < kMaxSplits && tiles * splits < sms && 2 * splits <= args.kblocks) splits *= 2;
   return fmt == kNv ? run_fmt<kNv>(*w, *x, args, bn, splits, stream) : run_fmt<kMx>(*w, *x, args, bn, splits, stream);
 }
 

@@ -23,6 +23,7 @@ import torch
 from torch import nn
 
 from ..errors import ConfigError
+from ._ext import require
 from .quant import E2M1_VALUES, e2m1_round
 
 __all__ = ["FORMATS", "FP4Tensor", "FP4Weight", "quantize"]
@@ -125,10 +126,10 @@ class FP4Tensor:
     __slots__ = ("codes", "scales", "row_scale", "fmt", "shape")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, row_scale: torch.Tensor, fmt: str,
-                 shape: torch.Size | tuple[int, ...] | None = None) -> None:
+                 shape: torch.Size | None = None) -> None:
         _check_format(fmt)
         self.codes, self.scales, self.row_scale, self.fmt = codes, scales, row_scale, fmt
-        self.shape = torch.Size(shape if shape is not None else (codes.shape[0], 2 * codes.shape[1]))
+        self.shape = shape if shape is not None else torch.Size((codes.shape[0], 2 * codes.shape[1]))
 
     @property
     def is_cuda(self) -> bool:
@@ -148,35 +149,30 @@ class FP4Tensor:
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values the codes stand for, exact in bf16 and fp32 (those beyond a type's range, which only rows near
         bf16's largest values have, become infinite)."""
-        if self.is_cuda:
-            from ._ext import require
-
+        if self.codes.is_cuda:
             out = require().fp4_dequantize(self.codes, self.scales, self.row_scale, FORMATS[self.fmt])
         else:
             out = _reference_dequantize(self.codes, self.scales, self.row_scale, self.fmt)
-        return out.to(dtype).reshape(self.shape)
+        if out.dtype != dtype:
+            out = out.to(dtype)
+        return out if len(self.shape) == 2 else out.reshape(self.shape)
 
     def __repr__(self) -> str:
         return f"FP4Tensor({tuple(self.shape)}, fmt={self.fmt!r}, device={self.device})"
 
 
-@torch.no_grad()
 def quantize(x: torch.Tensor, fmt: str = "nvfp4") -> FP4Tensor:
     """``x [..., K]`` in 4 bits (bf16 on CUDA, any float type on the CPU; ``K`` a multiple of 32, at most 65536). The
     result carries no gradient."""
     _check_format(fmt)
-    if x.dim() < 1 or x.shape[-1] < 32 or x.shape[-1] % 32 or x.shape[-1] > 65536:
-        raise ConfigError(f"4-bit rows need a multiple of 32 columns, up to 65536, got {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 32 or shape[-1] % 32 or shape[-1] > 65536:
+        raise ConfigError(f"4-bit rows need a multiple of 32 columns, up to 65536, got {tuple(shape)}")
+    if x.is_cuda:
+        return FP4Tensor(*require().fp4_quantize(x, FORMATS[fmt]), fmt, shape)
     if not x.is_floating_point():
         raise ConfigError(f"4-bit rows are quantised from floating point, got {x.dtype}")
-    rows = x.detach().reshape(-1, x.shape[-1])
-    if x.is_cuda:
-        from ._ext import require
-
-        parts = require().fp4_quantize(rows, FORMATS[fmt])
-    else:
-        parts = _reference_quantize(rows, fmt)
-    return FP4Tensor(*parts, fmt, x.shape)
+    return FP4Tensor(*_reference_quantize(x.detach().reshape(-1, shape[-1]), fmt), fmt, shape)
 
 
 class FP4Weight(nn.Module):
@@ -233,27 +229,26 @@ class FP4Weight(nn.Module):
     def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         return FP4Tensor(self.codes, self.scales, self.row_scale, self.fmt).dequantize(dtype or self.compute_dtype)
 
-    @torch.no_grad()
     def linear(self, x: torch.Tensor | FP4Tensor) -> torch.Tensor:
-        """``x @ w.T`` with both operands in 4 bits: fp32 sums, rounded once to ``x``'s type (bf16 for 4-bit ``x``)."""
+        """``x @ w.T`` with both operands in 4 bits: fp32 sums, rounded to bf16 on CUDA, in ``x``'s type."""
         if x.shape[-1] != self.in_features:
             raise ConfigError(f"activations {tuple(x.shape)} do not match a weight of {self.in_features} columns")
-        if isinstance(x, FP4Tensor) and x.fmt != self.fmt:
-            raise ConfigError(f"{x.fmt} activations do not multiply with an {self.fmt} weight")
-        if x.device != self.device:
+        b = self._buffers  # looked up once: a module's own lookup takes longer than the launch
+        codes, scales, row_scale = b["codes"], b["scales"], b["row_scale"]
+        if isinstance(x, FP4Tensor):
+            if x.fmt != self.fmt:
+                raise ConfigError(f"{x.fmt} activations do not multiply with an {self.fmt} weight")
+            if x.codes.is_cuda:
+                y = require().fp4_matmul(x.codes, x.scales, x.row_scale, codes, scales, row_scale, FORMATS[self.fmt])
+                return y if len(x.shape) == 2 else y.reshape(*x.shape[:-1], self.out_features)
+        elif x.is_cuda:
+            return require().linear_fp4(x, codes, scales, row_scale, FORMATS[self.fmt])
+        if codes.is_cuda:
             raise ConfigError(f"activations on {x.device}, weight on {self.device}")
-        if not x.is_cuda:
+        with torch.no_grad():
             q = x if isinstance(x, FP4Tensor) else quantize(x, self.fmt)
             y = q.dequantize(torch.float32).reshape(-1, self.in_features) @ self.dequantize(torch.float32).t()
             return y.to(x.dtype).reshape(*x.shape[:-1], self.out_features)
-        from ._ext import require
-
-        weight = (self.codes, self.scales, self.row_scale, FORMATS[self.fmt])
-        if isinstance(x, FP4Tensor):
-            y = require().fp4_matmul(x.codes, x.scales, x.row_scale, *weight)
-        else:
-            y = require().linear_fp4(x.detach().reshape(-1, self.in_features).to(torch.bfloat16), *weight)
-        return y.reshape(*x.shape[:-1], self.out_features).to(x.dtype)
 
     def extra_repr(self) -> str:
         return f"{self.out_features}x{self.in_features}, fmt={self.fmt}"

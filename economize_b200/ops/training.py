@@ -14,10 +14,9 @@ import math
 
 import torch
 
-from ..errors import ConfigError
 from . import reference
 from ._ext import require
-from .fp4 import FORMATS, FP4Tensor
+from .fp4 import FORMATS, FP4Tensor, _check_format
 from .fp4 import quantize as fp4_quantize
 
 __all__ = ["block_norm", "linear_cross_entropy", "packed_attention"]
@@ -121,11 +120,16 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Ten
     ``gate`` the gradients are taken from the rounded stream, and with ``scale=1`` those of ``x`` and ``residual`` are one
     tensor.
     """
+    if x.is_cuda:  # the checks are the extension's, in C++
+        if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:
+            x, residual, weight, post_weight, gate = (None if t is None else t.to(torch.bfloat16)
+                                                      for t in (x, residual, weight, post_weight, gate))
+        if quantize is None:
+            return require().block_norm(x, residual, weight, post_weight, gate, scale, eps)
+        _check_format(quantize)
+        *parts, stream = require().block_norm_fp4(x, residual, weight, post_weight, gate, scale, eps, FORMATS[quantize])
+        return FP4Tensor(*parts, quantize, x.shape), stream
     given = [t for t in (x, residual, weight, post_weight, gate) if t is not None]
-    given = _autocast(*given)
-    it = iter(given)
-    x, residual, weight, post_weight, gate = (None if t is None else next(it)
-                                              for t in (x, residual, weight, post_weight, gate))
     if x.dim() < 1 or weight.dim() != 1 or x.shape[-1] != weight.shape[0]:
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
     if post_weight is not None and post_weight.shape != weight.shape:
@@ -139,16 +143,7 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Ten
                          + ", ".join(f"{t.dtype} on {t.device}" for t in given))
     if not x.is_floating_point() or not math.isfinite(scale) or not 0.0 <= eps < math.inf:
         raise ValueError(f"block_norm takes floating point and a finite scale and eps >= 0, got {x.dtype}, {scale}, {eps}")
-    if quantize is not None and quantize not in FORMATS:
-        raise ConfigError(f"unknown 4-bit format {quantize!r} (one of {', '.join(FORMATS)})")
-    shape = x.shape
-    if x.is_cuda:
-        flat = [None if t is None else t if t.dim() == 2 else t.reshape(-1, t.shape[-1]) for t in (x, residual, gate)]
-        if quantize is not None:
-            *parts, stream = require().block_norm_fp4(flat[0], flat[1], weight, post_weight, flat[2], float(scale),
-                                                      float(eps), FORMATS[quantize])
-            return FP4Tensor(*parts, quantize, shape), stream.reshape(shape)
-        normed, stream = require().block_norm(flat[0], flat[1], weight, post_weight, flat[2], float(scale), float(eps))
-        return (normed, stream) if len(shape) == 2 else (normed.reshape(shape), stream.reshape(shape))
+    if quantize is not None:
+        _check_format(quantize)
     normed, stream = reference.block_norm(x, residual, weight, post_weight, gate, float(scale), float(eps))
     return (normed, stream) if quantize is None else (fp4_quantize(normed, quantize), stream.detach())

@@ -302,11 +302,11 @@ def test_autocast_and_refusals(cuda):
                      ((x, None, w), {"quantize": "int4"}), ((x.long(), None, w.long()), {})):
         with pytest.raises(ValueError):
             ops.block_norm(*args, **kw)
-    with pytest.raises(RuntimeError):
+    with pytest.raises(ValueError):
         ops.block_norm(x.double(), None, w.double())
-    with pytest.raises(RuntimeError):
+    with pytest.raises(ValueError):
         ops.block_norm(torch.zeros(1, 16392, device=cuda), None, torch.zeros(16392, device=cuda))
-    with pytest.raises(RuntimeError):
+    with pytest.raises(ValueError):
         ops.block_norm(x, None, w, quantize="nvfp4")  # 4-bit results come from bf16
     y = torch.randn(4, 64, device=cuda, requires_grad=True)
     with pytest.raises(RuntimeError, match="twice"):

@@ -224,7 +224,7 @@ def test_refusals(cuda):
                    (4, w.scales.float()), (5, w.row_scale.double()), (6, 3), (2, q.row_scale.cpu()), (0, q.codes.t())):
         args = list(good)
         args[i] = bad
-        with pytest.raises(RuntimeError):
+        with pytest.raises((RuntimeError, ValueError)):
             C.fp4_matmul(*args)
 
 
