@@ -45,12 +45,11 @@ struct Cast<__half> {
   static __device__ __forceinline__ __half from(float v) { return __float2half(v); }
 };
 
-// A lane's VEC consecutive elements, from element `at` of a row of `hidden` on: 32 bytes in two halves of 16, of which the
-// second may lie behind the row's end, or one element.
+// A lane's VEC consecutive elements, from element `at` of a row of `hidden` on: 16 bytes, or one element. (With 32 bytes a
+// lane, two loads or stores of 16, every access would touch half of each sector: 66 us where this takes 45 for 8192 rows
+// of 4096.)
 template <typename T, int VEC>
 struct Pack {
-  static constexpr int kPart = VEC == 1 ? 1 : VEC / 2;
-  static constexpr int kParts = VEC / kPart;
   static constexpr int kWords = (VEC * static_cast<int>(sizeof(T)) + 3) / 4;
   union {
     T v[VEC];
@@ -63,56 +62,48 @@ struct Pack {
   __device__ __forceinline__ void fetch(const T* row, int at, int hidden) {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) words[i] = 0;
-#pragma unroll
-    for (int k = 0; k < kParts; ++k) {
-      if (row != nullptr && at + k * kPart < hidden) {
-        if constexpr (VEC == 1) v[0] = row[at];
-        else *reinterpret_cast<uint4*>(words + 4 * k) = *reinterpret_cast<const uint4*>(row + at + k * kPart);
-      }
+    if (row != nullptr && at < hidden) {
+      if constexpr (VEC == 1) v[0] = row[at];
+      else *reinterpret_cast<uint4*>(words) = *reinterpret_cast<const uint4*>(row + at);
     }
   }
   __device__ __forceinline__ void store(T* row, int at, int hidden) const {
-#pragma unroll
-    for (int k = 0; k < kParts; ++k) {
-      if (at + k * kPart < hidden) {
-        if constexpr (VEC == 1) row[at] = v[0];
-        else *reinterpret_cast<uint4*>(row + at + k * kPart) = *reinterpret_cast<const uint4*>(words + 4 * k);
-      }
+    if (at < hidden) {
+      if constexpr (VEC == 1) row[at] = v[0];
+      else *reinterpret_cast<uint4*>(row + at) = *reinterpret_cast<const uint4*>(words);
     }
   }
 };
 
 // Rows on their way: every thread copies the vectors that it will work on itself into shared memory (cp.async), DEPTH rows
 // ahead, so nothing is shared, no barrier is needed and no register is held. Operand k, vector i of a thread in slot s
-// lies in 16-byte planes of one entry per thread. DEPTH 0: operands are read when they are needed.
+// lies in a 16-byte plane of one entry per thread. DEPTH 0: operands are read when they are needed.
 template <typename T, int VEC, int NV, int OPS, int DEPTH>
 struct Rows {
   using P = Pack<T, VEC>;
   static constexpr bool kAhead = DEPTH > 0;
   static_assert(!kAhead || VEC > 1, "single elements are not copied ahead");
-  static constexpr int kSlotPlanes = OPS * NV * P::kParts;
+  static constexpr int kSlotPlanes = OPS * NV;
   static constexpr int bytes(int threads) { return DEPTH * kSlotPlanes * threads * 16; }
   uint32_t base;
   int slot = 0;
   const T* ptr[OPS];  // rows being worked on (DEPTH 0)
   __device__ __forceinline__ Rows(void* smem) : base(smem_u32(smem) + threadIdx.x * 16) {}
-  __device__ __forceinline__ uint32_t plane(int s, int op, int i, int k) const {
-    return base + static_cast<uint32_t>((s * kSlotPlanes + (op * NV + i) * P::kParts + k) * blockDim.x * 16);
+  __device__ __forceinline__ uint32_t plane(int s, int op, int i) const {
+    return base + static_cast<uint32_t>((s * kSlotPlanes + op * NV + i) * blockDim.x * 16);
   }
   // start the copy of operand op's row (zeros for null) into slot s; first, step: this lane's vectors
   __device__ __forceinline__ void start(int s, int op, const T* row, int first, int step, int hidden) {
     if constexpr (kAhead) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int k = 0; k < P::kParts; ++k) {
-          const int at = (first + i * step) * VEC + k * P::kPart;
-          const uint32_t to = plane(s, op, i, k);
-          if (row != nullptr && at < hidden)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(row + at) : "memory");
-          else
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory");
-        }
+      for (int i = 0; i < NV; ++i) {
+        const int at = (first + i * step) * VEC;
+        const uint32_t to = plane(s, op, i);
+        if (row != nullptr && at < hidden)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(row + at) : "memory");
+        else
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory");
+      }
     } else {
       ptr[op] = row;
     }
@@ -126,13 +117,10 @@ struct Rows {
   }
   __device__ __forceinline__ void get(P& out, int op, int i, int at, int hidden) const {
     if constexpr (kAhead) {
-#pragma unroll
-      for (int k = 0; k < P::kParts; ++k)
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(out.words[4 * k]), "=r"(out.words[4 * k + 1]), "=r"(out.words[4 * k + 2]),
-                       "=r"(out.words[4 * k + 3])
-                     : "r"(plane(slot, op, i, k))
-                     : "memory");
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(out.words[0]), "=r"(out.words[1]), "=r"(out.words[2]), "=r"(out.words[3])
+                   : "r"(plane(slot, op, i))
+                   : "memory");
     } else {
       out.fetch(ptr[op], at, hidden);
     }
@@ -298,11 +286,11 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
       if constexpr (FMT == fp4::kNv) {
         uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) top = max(top, fp4::max_bits<8>(out[i].words));
+        for (int i = 0; i < NV; ++i) top = max(top, fp4::max_bits<4>(out[i].words));
         if (top >= 0x7f80u) {
           top = 0;
 #pragma unroll
-          for (int i = 0; i < NV; ++i) top = max(top, fp4::finite_bits<8>(out[i].words));
+          for (int i = 0; i < NV; ++i) top = max(top, fp4::finite_bits<4>(out[i].words));
         }
         const int e = fp4::row_exponent(team.max(fp4::bits_value(top)));
         mul = fp4::pow2(-e);
@@ -310,8 +298,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
       }
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        fp4::store16<FMT>(out[i].words, mul, row, team.first + i * team.step, real ? hidden / 16 : 0, a.tiles, a.codes,
-                          a.scales);
+        fp4::store8<FMT>(out[i].words, mul, row, team.first + i * team.step, real ? hidden / 8 : 0, a.tiles, a.codes,
+                         a.scales);
     }
   }
 }
@@ -497,11 +485,11 @@ struct Grid {
   int warps, nv, teams, threads;  // warps of a team, vectors a lane, teams and threads of a block
 };
 
-// 32 bytes a lane (fp32 rows of more than 8192: 64), or four single elements (16 where those are more than 1024 lanes
-// hold); several teams to a block of 256 threads, or one.
+// Two vectors of 16 bytes a lane (fp32 rows of more than 8192: four), or four single elements (16 beyond 4096); several teams
+// to a block of 256 threads, or one.
 template <typename T, int VEC>
 Grid grid_of(int hidden) {
-  const int all = (hidden + 32 * VEC - 1) / (32 * VEC), target = VEC == 1 ? 4 : 1;
+  const int all = (hidden + 32 * VEC - 1) / (32 * VEC), target = VEC == 1 ? 4 : 2;
   Grid g;
   g.warps = std::min(kMaxWarps, (all + target - 1) / target);
   if (g.warps <= 8) {
@@ -516,7 +504,7 @@ Grid grid_of(int hidden) {
 }
 
 template <typename T>
-constexpr int vec_of() { return 32 / static_cast<int>(sizeof(T)); }
+constexpr int vec_of() { return 16 / static_cast<int>(sizeof(T)); }
 
 constexpr int kFwdBlocks = 3, kBwdBlocks = 2;  // of 256 threads on an SM
 
@@ -540,9 +528,9 @@ int run_forward(const BlockNormArgs& a, int sms, cudaStream_t stream) {
   constexpr int V = vec_of<T>();
   // 4-bit results: lanes cover the scales' padding too
   const Grid g = grid_of<T, V>(FMT == 0 ? a.hidden : (a.hidden + fp4::kBlockK - 1) / fp4::kBlockK * fp4::kBlockK);
-  if (g.threads <= 256) return go_forward<T, V, 1, FMT, POST, 256, kFwdBlocks, 3>(a, g, sms, stream);
-  if (g.nv == 1) return go_forward<T, V, 1, FMT, POST, 1024, 1, 2>(a, g, sms, stream);
-  if constexpr (sizeof(T) == 4) return go_forward<T, V, 2, FMT, POST, 1024, 1, 1>(a, g, sms, stream);
+  if (g.threads <= 256) return go_forward<T, V, 2, FMT, POST, 256, kFwdBlocks, 3>(a, g, sms, stream);
+  if (g.nv <= 2) return go_forward<T, V, 2, FMT, POST, 1024, 1, 2>(a, g, sms, stream);
+  if constexpr (sizeof(T) == 4) return go_forward<T, V, 4, FMT, POST, 1024, 1, 1>(a, g, sms, stream);
   return -1;
 }
 
@@ -572,10 +560,10 @@ int go_backward(const BlockNormGrads& a, const Grid& g, int sms, cudaStream_t st
 template <typename T, bool POST, bool WHOLE>
 int run_backward(const BlockNormGrads& a, const Grid& g, int sms, cudaStream_t stream) {
   constexpr int V = vec_of<T>();
-  if (g.threads <= 256) return go_backward<T, V, 1, POST, WHOLE, 256, kBwdBlocks, 3>(a, g, sms, stream);
-  if (g.threads <= 512) return go_backward<T, V, 1, POST, WHOLE, 512, 1, 2>(a, g, sms, stream);
-  if (g.nv == 1) return go_backward<T, V, 1, POST, WHOLE, 1024, 1, 1>(a, g, sms, stream);
-  if constexpr (sizeof(T) == 4) return go_backward<T, V, 2, POST, WHOLE, 1024, 1, 0>(a, g, sms, stream);
+  if (g.threads <= 256) return go_backward<T, V, 2, POST, WHOLE, 256, kBwdBlocks, 3>(a, g, sms, stream);
+  if (g.threads <= 512) return go_backward<T, V, 2, POST, WHOLE, 512, 1, 2>(a, g, sms, stream);
+  if (g.nv <= 2) return go_backward<T, V, 2, POST, WHOLE, 1024, 1, 1>(a, g, sms, stream);
+  if constexpr (sizeof(T) == 4) return go_backward<T, V, 4, POST, WHOLE, 1024, 1, 0>(a, g, sms, stream);
   return -1;
 }
 

@@ -185,6 +185,22 @@ __device__ __forceinline__ void store16(const uint32_t* v, float mul, int row, i
   if ((kLanes == 1 || (vec & 1) == 0) && (g >> 2) < tiles) scales[scale_word(row, g >> 2, tiles) + (g & 3)] = byte;
 }
 
+// The same of 8 columns a lane: two (nvfp4) or four (mxfp4) neighbouring lanes hold a group; the whole warp calls.
+template <int FMT>
+__device__ __forceinline__ void store8(const uint32_t* v, float mul, int row, int vec, int vecs, int tiles,
+                                       uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  constexpr int kLanes = Format<FMT>::kGroup / 8;
+  uint32_t bits = max_bits<4>(v);
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+  float factor;
+  uint32_t byte = group_scale<FMT>(bits, mul, factor);
+  if (vec < vecs) *reinterpret_cast<uint32_t*>(codes + (static_cast<size_t>(row) * vecs + vec) * 4) = codes8(v, factor);
+  else byte = 0;
+  const int g = vec / kLanes;
+  if (vec % kLanes == 0 && (g >> 2) < tiles) scales[scale_word(row, g >> 2, tiles) + (g & 3)] = byte;
+}
+
 // ---- block-scaled MMAs ---------------------------------------------------------------------------------------------
 // Instruction descriptor of the block-scaled kinds: e2m1 operands, K-major, shape m x n, scales of type e4m3 (nvfp4) or
 // E8M0 (mxfp4); sf: which bytes of the 32-bit scale words the MMA's two scales per row are (kind::mxf4: 0 or 2).
