@@ -489,7 +489,7 @@ struct BlockNormFunction : torch::autograd::Function<BlockNormFunction> {
       a.scale = f.scale;
       Tensor parts;
       if (need_w || need_p) {
-        const int n = ecz::block_norm_parts(type, a.rows, a.hidden, o.vec, sms);
+        const int n = ecz::block_norm_parts(type, a.rows, a.hidden, o.vec, simple, sms);
         parts = at::empty({(need_w ? 1 : 0) + (need_p ? 1 : 0), n, H}, opts.dtype(at::kFloat));
         float* p = parts.data_ptr<float>();
         if (need_w) a.dw_part = p;

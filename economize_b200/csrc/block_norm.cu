@@ -26,6 +26,7 @@ namespace ecz {
 namespace {
 
 constexpr int kMaxWarps = 32;
+constexpr int kMostSmem = 227 * 1024 - 2 * kMaxWarps * 8;  // beside the teams' scratch
 
 template <typename T>
 struct Cast;
@@ -77,20 +78,22 @@ struct Pack {
 
 // Rows on their way: every thread copies the vectors that it will work on itself into shared memory (cp.async), DEPTH rows
 // ahead, so nothing is shared, no barrier is needed and no register is held. Operand k, vector i of a thread in slot s
-// lies in a 16-byte plane of one entry per thread. DEPTH 0: operands are read when they are needed.
+// lies in a plane of one entry (16 bytes, or a single fp32 element) per thread. DEPTH 0 (long rows, and single elements of
+// 16 bits, which cp.async does not copy): operands are read when they are needed.
 template <typename T, int VEC, int NV, int OPS, int DEPTH>
 struct Rows {
   using P = Pack<T, VEC>;
   static constexpr bool kAhead = DEPTH > 0;
-  static_assert(!kAhead || VEC > 1, "single elements are not copied ahead");
+  static constexpr int kEntry = VEC * static_cast<int>(sizeof(T));
+  static_assert(!kAhead || kEntry == 16 || kEntry == 4, "what cp.async copies");
   static constexpr int kSlotPlanes = OPS * NV;
-  static constexpr int bytes(int threads) { return DEPTH * kSlotPlanes * threads * 16; }
+  static constexpr int bytes(int threads) { return DEPTH * kSlotPlanes * threads * kEntry; }
   uint32_t base;
   int slot = 0;
   const T* ptr[OPS];  // rows being worked on (DEPTH 0)
-  __device__ __forceinline__ Rows(void* smem) : base(smem_u32(smem) + threadIdx.x * 16) {}
+  __device__ __forceinline__ Rows(void* smem) : base(smem_u32(smem) + threadIdx.x * kEntry) {}
   __device__ __forceinline__ uint32_t plane(int s, int op, int i) const {
-    return base + static_cast<uint32_t>((s * kSlotPlanes + op * NV + i) * blockDim.x * 16);
+    return base + static_cast<uint32_t>((s * kSlotPlanes + op * NV + i) * blockDim.x * kEntry);
   }
   // start the copy of operand op's row (zeros for null) into slot s; first, step: this lane's vectors
   __device__ __forceinline__ void start(int s, int op, const T* row, int first, int step, int hidden) {
@@ -99,10 +102,14 @@ struct Rows {
       for (int i = 0; i < NV; ++i) {
         const int at = (first + i * step) * VEC;
         const uint32_t to = plane(s, op, i);
-        if (row != nullptr && at < hidden)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(row + at) : "memory");
-        else
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory");
+        const bool on = row != nullptr && at < hidden;
+        if constexpr (kEntry == 16) {
+          if (on) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(row + at) : "memory");
+          else asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory");
+        } else {
+          if (on) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(row + at) : "memory");
+          else asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(0) : "memory");
+        }
       }
     } else {
       ptr[op] = row;
@@ -117,13 +124,41 @@ struct Rows {
   }
   __device__ __forceinline__ void get(P& out, int op, int i, int at, int hidden) const {
     if constexpr (kAhead) {
-      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(out.words[0]), "=r"(out.words[1]), "=r"(out.words[2]), "=r"(out.words[3])
-                   : "r"(plane(slot, op, i))
-                   : "memory");
+      if constexpr (kEntry == 16)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(out.words[0]), "=r"(out.words[1]), "=r"(out.words[2]), "=r"(out.words[3])
+                     : "r"(plane(slot, op, i))
+                     : "memory");
+      else
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(out.words[0]) : "r"(plane(slot, op, i)) : "memory");
     } else {
       out.fetch(ptr[op], at, hidden);
     }
+  }
+};
+
+// This lane's part of a weight: in registers, or (SHARED) in planes of shared memory like Rows', where two weights or the
+// sums over tokens would spill.
+template <typename T, int VEC, int NV, bool SHARED>
+struct Lanes {
+  using P = Pack<T, VEC>;
+  static constexpr int kEntry = VEC * static_cast<int>(sizeof(T));
+  static constexpr int bytes(int threads) { return SHARED ? NV * threads * kEntry : 0; }
+  P held[SHARED ? 1 : NV];
+  P* plane;
+  __device__ __forceinline__ void fetch(void* smem, const T* row, int first, int step, int hidden) {
+    plane = static_cast<P*>(smem) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      P v;
+      v.fetch(row, (first + i * step) * VEC, hidden);
+      if constexpr (SHARED) plane[i * blockDim.x] = v;
+      else held[i] = v;
+    }
+  }
+  __device__ __forceinline__ P get(int i) const {
+    if constexpr (SHARED) return plane[i * blockDim.x];
+    else return held[i];
   }
 };
 
@@ -144,42 +179,36 @@ struct Team {
   __device__ __forceinline__ void barrier() const {
     asm volatile("bar.sync %0, %1;" ::"r"(index + 1), "r"(warps * 32) : "memory");
   }
+  // this warp's part to the others, theirs combined in the order of the warps' binary tree
+  template <class V, class Op>
+  __device__ __forceinline__ V combine(V v, V neutral, Op op) {
+    V* buf = reinterpret_cast<V*>(scratch + turn * kMaxWarps + index * warps);
+    turn ^= 1;
+    if (lane == 0) buf[warp] = v;
+    barrier();
+    v = lane < warps ? buf[lane] : neutral;
+    for (int o = 1; o < warps; o <<= 1) v = op(v, o);
+    return v;
+  }
   __device__ __forceinline__ float2 sum(float2 v) {
     v.x = warp_sum(v.x);
     v.y = warp_sum(v.y);
     if (warps == 1) return v;
-    float2* buf = scratch + turn * kMaxWarps + index * warps;
-    turn ^= 1;
-    if (lane == 0) buf[warp] = v;
-    barrier();
-    float2 out = make_float2(0.f, 0.f);
-    for (int w = 0; w < warps; ++w) {
-      out.x += buf[w].x;
-      out.y += buf[w].y;
-    }
-    return out;
+    v = combine(v, make_float2(0.f, 0.f), [](float2 a, int o) {
+      return make_float2(a.x + __shfl_xor_sync(0xffffffffu, a.x, o), a.y + __shfl_xor_sync(0xffffffffu, a.y, o));
+    });
+    return make_float2(__shfl_sync(0xffffffffu, v.x, 0), __shfl_sync(0xffffffffu, v.y, 0));
   }
   __device__ __forceinline__ float sum(float v) {
     v = warp_sum(v);
     if (warps == 1) return v;
-    float2* buf = scratch + turn * kMaxWarps + index * warps;
-    turn ^= 1;
-    if (lane == 0) buf[warp].x = v;
-    barrier();
-    float out = 0.f;
-    for (int w = 0; w < warps; ++w) out += buf[w].x;
-    return out;
+    v = combine(v, 0.f, [](float a, int o) { return a + __shfl_xor_sync(0xffffffffu, a, o); });
+    return __shfl_sync(0xffffffffu, v, 0);
   }
-  __device__ __forceinline__ float max(float v) {
-    v = warp_max(v);
+  __device__ __forceinline__ uint32_t max(uint32_t v) {
+    v = __reduce_max_sync(0xffffffffu, v);
     if (warps == 1) return v;
-    float2* buf = scratch + turn * kMaxWarps + index * warps;
-    turn ^= 1;
-    if (lane == 0) buf[warp].x = v;
-    barrier();
-    float out = buf[0].x;
-    for (int w = 1; w < warps; ++w) out = fmaxf(out, buf[w].x);
-    return out;
+    return __reduce_max_sync(0xffffffffu, combine(v, 0u, [](uint32_t a, int) { return a; }));
   }
 };
 
@@ -212,13 +241,11 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   int row = blockIdx.x * per_block + team.index;
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d) start(d, row + d * teams);
-  Pack<T, VEC> w[NV], p[POST ? NV : 1];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int at = (team.first + i * team.step) * VEC;
-    w[i].fetch(static_cast<const T*>(a.weight), at, hidden);
-    if constexpr (POST) p[i].fetch(static_cast<const T*>(a.post), at, hidden);
-  }
+  Lanes<T, VEC, NV, VEC != 1 && POST> w, p;
+  uint8_t* behind = ring + Rows<T, VEC, NV, 2, DEPTH>::bytes(blockDim.x);
+  w.fetch(behind, static_cast<const T*>(a.weight), team.first, team.step, hidden);
+  if constexpr (POST)
+    p.fetch(behind + w.bytes(blockDim.x), static_cast<const T*>(a.post), team.first, team.step, hidden);
   for (; row < last; row += teams) {
     const bool real = row < a.rows;
     float factor = a.scale;
@@ -250,9 +277,11 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
       if (!post) rows.get(x, 0, i, at, hidden);
       rows.get(r, 1, i, at, hidden);
       if (a.gate_mode == kGateFull) g.fetch(real ? gp + row * a.gate_stride : nullptr, at, hidden);
+      Pack<T, VEC> pi;
+      if constexpr (POST) pi = p.get(i);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        float b = post ? s[i][j] * (ix * p[POST ? i : 0].get(j)) : x.get(j);
+        float b = post ? s[i][j] * (ix * pi.get(j)) : x.get(j);
         if (a.gate_mode == kGateFull) b *= g.get(j);
         s[i][j] = fmaf(factor, b, r.get(j));
         q = fmaf(s[i][j], s[i][j], q);
@@ -275,8 +304,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
     Pack<T, VEC> out[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      const Pack<T, VEC> wi = w.get(i);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) out[i].set(j, real ? s[i][j] * is * w[i].get(j) : 0.f);
+      for (int j = 0; j < VEC; ++j) out[i].set(j, real ? s[i][j] * is * wi.get(j) : 0.f);
       if (FMT == 0)
         out[i].store(static_cast<T*>(a.normed) + static_cast<size_t>(row) * hidden, (team.first + i * team.step) * VEC,
                      hidden);
@@ -292,7 +322,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
 #pragma unroll
           for (int i = 0; i < NV; ++i) top = max(top, fp4::finite_bits<4>(out[i].words));
         }
-        const int e = fp4::row_exponent(team.max(fp4::bits_value(top)));
+        const int e = fp4::row_exponent(fp4::bits_value(team.max(top)));
         mul = fp4::pow2(-e);
         if (real && team.first == 0) a.row_scale[row] = fp4::pow2(e);
       }
@@ -303,6 +333,12 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
     }
   }
 }
+
+// Where the backward kernel's weights lie (Lanes): in shared memory beside x and the residual.
+template <int VEC, bool WHOLE>
+struct SharedWeights {
+  static constexpr bool value = VEC > 1 && !WHOLE;
+};
 
 // Persistent like the forward kernel. A team's sums for dweight and dpost go to its row of a.dw_part / a.dpost_part (fp32
 // [teams, hidden]). WHOLE: the stream is given in place of x and the residual.
@@ -337,19 +373,20 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   pdl_wait();
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d) start(d, self + d * teams);
-  Pack<T, VEC> w[NV], p[POST ? NV : 1];
+  constexpr bool kShared = SharedWeights<VEC, WHOLE>::value;
+  Lanes<T, VEC, NV, kShared> w, p;
+  uint8_t* behind = ring + Rows<T, VEC, NV, WHOLE ? 3 : 4, DEPTH>::bytes(blockDim.x);
+  w.fetch(behind, static_cast<const T*>(a.weight), team.first, team.step, hidden);
+  if constexpr (POST)
+    p.fetch(behind + w.bytes(blockDim.x), static_cast<const T*>(a.post), team.first, team.step, hidden);
   float dw[NV][VEC], dp[POST ? NV : 1][VEC];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int at = (team.first + i * team.step) * VEC;
-    w[i].fetch(static_cast<const T*>(a.weight), at, hidden);
-    if constexpr (POST) p[i].fetch(static_cast<const T*>(a.post), at, hidden);
+  for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       dw[i][j] = 0.f;
       if constexpr (POST) dp[i][j] = 0.f;
     }
-  }
   for (int row = self; row < a.rows; row += teams) {
     const float is = a.inv_s[row], ix = post ? a.inv_x[row] : 1.f;
     float gate = a.scale;  // scale times the token's gate
@@ -366,18 +403,21 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
       rows.get(r, 2, i, at, hidden);
       if constexpr (!WHOLE) rows.get(x, 3, i, at, hidden);
       if (gate_mode == kGateFull) fg.fetch(gp + row * a.gate_stride, at, hidden);
+      const Pack<T, VEC> wi = w.get(i);
+      Pack<T, VEC> pi;
+      if constexpr (POST) pi = p.get(i);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         float s = r.get(j);
         if constexpr (!WHOLE) {
           float b = x.get(j);
-          if (POST && post) b *= ix * p[POST ? i : 0].get(j);
+          if (POST && post) b *= ix * pi.get(j);
           if (gate_mode == kGateFull) b *= fg.get(j);
           s = fmaf(gate, b, s);
         }
         sh[i][j] = s * is;
         dw[i][j] = fmaf(dn.get(j), sh[i][j], dw[i][j]);
-        dot = fmaf(dn.get(j) * w[i].get(j), sh[i][j], dot);
+        dot = fmaf(dn.get(j) * wi.get(j), sh[i][j], dot);
       }
     }
     dot = team.sum(dot) * mean;
@@ -390,14 +430,17 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
       rows.get(u, 1, i, at, hidden);
       if constexpr (!WHOLE) rows.get(x, 3, i, at, hidden);
       if (gate_mode == kGateFull) fg.fetch(gp + row * a.gate_stride, at, hidden);
+      const Pack<T, VEC> wi = w.get(i);
+      Pack<T, VEC> pi;
+      if constexpr (POST) pi = p.get(i);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float ds = fmaf(is, dn.get(j) * w[i].get(j) - sh[i][j] * dot, u.get(j));
+        const float ds = fmaf(is, dn.get(j) * wi.get(j) - sh[i][j] * dot, u.get(j));
         out.set(j, ds);
         float db = gate * ds;
         if constexpr (!WHOLE) {
           const float xh = x.get(j) * ix;  // without a norm behind the block ix is 1
-          const float pw = POST && post ? p[POST ? i : 0].get(j) : 1.f;
+          const float pw = POST && post ? pi.get(j) : 1.f;
           if (gate_mode == kGateFull) {
             dg.set(j, a.scale * ds * (xh * pw));
             db *= fg.get(j);
@@ -485,11 +528,11 @@ struct Grid {
   int warps, nv, teams, threads;  // warps of a team, vectors a lane, teams and threads of a block
 };
 
-// Two vectors of 16 bytes a lane (fp32 rows of more than 8192: four), or four single elements (16 beyond 4096); several teams
-// to a block of 256 threads, or one.
-template <typename T, int VEC>
-Grid grid_of(int hidden) {
-  const int all = (hidden + 32 * VEC - 1) / (32 * VEC), target = VEC == 1 ? 4 : 2;
+// `target` vectors of 16 bytes or single elements a lane, more where that would take more than 32 warps; several teams to a
+// block of 256 threads, or one.
+template <int VEC>
+Grid grid_of(int hidden, int target) {
+  const int all = (hidden + 32 * VEC - 1) / (32 * VEC);
   Grid g;
   g.warps = std::min(kMaxWarps, (all + target - 1) / target);
   if (g.warps <= 8) {
@@ -506,11 +549,8 @@ Grid grid_of(int hidden) {
 template <typename T>
 constexpr int vec_of() { return 16 / static_cast<int>(sizeof(T)); }
 
-constexpr int kFwdBlocks = 3, kBwdBlocks = 2;  // of 256 threads on an SM
-
-template <class Ring, class Kernel, class Args>
-int go(Kernel kernel, int blocks, const Grid& g, const Args& a, cudaStream_t stream) {
-  const int smem = Ring::bytes(g.threads);
+template <class Kernel, class Args>
+int go(Kernel kernel, int smem, int blocks, const Grid& g, const Args& a, cudaStream_t stream) {
   if (set_max_smem(kernel, smem) != cudaSuccess) return -1;
   return launch_pdl(kernel, dim3(blocks), dim3(g.threads), smem, stream, a, g.warps) == cudaSuccess ? 0 : -1;
 }
@@ -519,26 +559,34 @@ template <typename T, int VEC, int NV, int FMT, bool POST, int THREADS, int BLOC
 int go_forward(const BlockNormArgs& a, const Grid& g, int sms, cudaStream_t stream) {
   const int rows = FMT == 0 ? a.rows : (a.rows + 127) / 128 * 128;
   const int resident = THREADS <= 256 ? BLOCKS : 1024 / g.threads;
-  return go<Rows<T, VEC, NV, 2, DEPTH>>(block_norm_kernel<T, VEC, NV, FMT, POST, THREADS, BLOCKS, DEPTH>,
-                                        std::min((rows + g.teams - 1) / g.teams, sms * resident), g, a, stream);
+  using R = Rows<T, VEC, NV, 2, DEPTH>;
+  using L = Lanes<T, VEC, NV, VEC != 1 && POST>;
+  static_assert(R::bytes(THREADS) + 2 * L::bytes(THREADS) <= kMostSmem, "227 KB of shared memory");
+  const int smem = R::bytes(g.threads) + 2 * L::bytes(g.threads);
+  return go(block_norm_kernel<T, VEC, NV, FMT, POST, THREADS, BLOCKS, DEPTH>, smem,
+            std::min((rows + g.teams - 1) / g.teams, sms * resident), g, a, stream);
 }
 
+// Blocks of 256 threads: three to an SM, two rows ahead (four with 64 registers a thread, or three rows ahead, took as
+// long or longer; so did one vector a lane).
 template <typename T, int FMT, bool POST>
 int run_forward(const BlockNormArgs& a, int sms, cudaStream_t stream) {
   constexpr int V = vec_of<T>();
   // 4-bit results: lanes cover the scales' padding too
-  const Grid g = grid_of<T, V>(FMT == 0 ? a.hidden : (a.hidden + fp4::kBlockK - 1) / fp4::kBlockK * fp4::kBlockK);
-  if (g.threads <= 256) return go_forward<T, V, 2, FMT, POST, 256, kFwdBlocks, 3>(a, g, sms, stream);
+  const Grid g = grid_of<V>(FMT == 0 ? a.hidden : (a.hidden + fp4::kBlockK - 1) / fp4::kBlockK * fp4::kBlockK, 2);
+  if (g.threads <= 256) return go_forward<T, V, 2, FMT, POST, 256, 3, 2>(a, g, sms, stream);
   if (g.nv <= 2) return go_forward<T, V, 2, FMT, POST, 1024, 1, 2>(a, g, sms, stream);
-  if constexpr (sizeof(T) == 4) return go_forward<T, V, 4, FMT, POST, 1024, 1, 1>(a, g, sms, stream);
+  if constexpr (sizeof(T) == 4) return go_forward<T, V, 4, FMT, POST, 1024, 1, 0>(a, g, sms, stream);
   return -1;
 }
 
 template <typename T>
 int run_forward_type(const BlockNormArgs& a, bool vec, int sms, cudaStream_t stream) {
   if (vec) return a.post != nullptr ? run_forward<T, 0, true>(a, sms, stream) : run_forward<T, 0, false>(a, sms, stream);
-  const Grid g = grid_of<T, 1>(a.hidden);
-  if (g.nv <= 4) return go_forward<T, 1, 4, 0, true, 1024, 1, 0>(a, g, sms, stream);
+  const Grid g = grid_of<1>(a.hidden, 4);
+  constexpr int kDepth = sizeof(T) == 4 ? 2 : 0;
+  if (g.threads <= 256) return go_forward<T, 1, 4, 0, true, 256, 4, kDepth>(a, g, sms, stream);
+  if (g.nv <= 4) return go_forward<T, 1, 4, 0, true, 1024, 1, kDepth>(a, g, sms, stream);
   return go_forward<T, 1, 16, 0, true, 1024, 1, 0>(a, g, sms, stream);
 }
 
@@ -547,60 +595,77 @@ int run_forward_fp4(const BlockNormArgs& a, int sms, cudaStream_t stream) {
   return a.post != nullptr ? run_forward<bf16, FMT, true>(a, sms, stream) : run_forward<bf16, FMT, false>(a, sms, stream);
 }
 
-int backward_blocks(const Grid& g, int rows, int sms) {
-  return std::min((rows + g.teams - 1) / g.teams, sms * (g.threads <= 256 ? kBwdBlocks : 1));
+template <typename T>
+Grid backward_grid(int hidden, bool vec) {
+  return vec ? grid_of<vec_of<T>()>(hidden, 2) : grid_of<1>(hidden, 4);
+}
+
+// Three blocks of 256 threads to an SM from the stream, two from x and the residual, which takes more registers.
+int backward_blocks(const Grid& g, int rows, int sms, bool vec, bool whole) {
+  const int resident = g.threads > 256 ? 1 : vec && whole ? 3 : 2;
+  return std::min((rows + g.teams - 1) / g.teams, sms * resident);
 }
 
 template <typename T, int VEC, int NV, bool POST, bool WHOLE, int THREADS, int BLOCKS, int DEPTH>
-int go_backward(const BlockNormGrads& a, const Grid& g, int sms, cudaStream_t stream) {
-  return go<Rows<T, VEC, NV, WHOLE ? 3 : 4, DEPTH>>(
-      block_norm_bwd_kernel<T, VEC, NV, POST, WHOLE, THREADS, BLOCKS, DEPTH>, backward_blocks(g, a.rows, sms), g, a, stream);
+int go_backward(const BlockNormGrads& a, const Grid& g, int blocks, cudaStream_t stream) {
+  using R = Rows<T, VEC, NV, WHOLE ? 3 : 4, DEPTH>;
+  using L = Lanes<T, VEC, NV, SharedWeights<VEC, WHOLE>::value>;
+  static_assert(R::bytes(THREADS) + 2 * L::bytes(THREADS) <= kMostSmem, "227 KB of shared memory");
+  const int smem = R::bytes(g.threads) + 2 * L::bytes(g.threads);
+  return go(block_norm_bwd_kernel<T, VEC, NV, POST, WHOLE, THREADS, BLOCKS, DEPTH>, smem, blocks, g, a, stream);
 }
 
-template <typename T, bool POST, bool WHOLE>
-int run_backward(const BlockNormGrads& a, const Grid& g, int sms, cudaStream_t stream) {
+template <typename T>
+int run_backward_whole(const BlockNormGrads& a, const Grid& g, int blocks, cudaStream_t stream) {
   constexpr int V = vec_of<T>();
-  if (g.threads <= 256) return go_backward<T, V, 2, POST, WHOLE, 256, kBwdBlocks, 3>(a, g, sms, stream);
-  if (g.threads <= 512) return go_backward<T, V, 2, POST, WHOLE, 512, 1, 2>(a, g, sms, stream);
-  if (g.nv <= 2) return go_backward<T, V, 2, POST, WHOLE, 1024, 1, 1>(a, g, sms, stream);
-  if constexpr (sizeof(T) == 4) return go_backward<T, V, 4, POST, WHOLE, 1024, 1, 0>(a, g, sms, stream);
+  if (g.threads <= 256) return go_backward<T, V, 2, false, true, 256, 3, 2>(a, g, blocks, stream);
+  if (g.threads <= 512) return go_backward<T, V, 2, false, true, 512, 1, 2>(a, g, blocks, stream);
+  if (g.nv <= 2) return go_backward<T, V, 2, false, true, 1024, 1, 2>(a, g, blocks, stream);
+  if constexpr (sizeof(T) == 4) return go_backward<T, V, 4, false, true, 1024, 1, 1>(a, g, blocks, stream);
+  return -1;
+}
+
+template <typename T, bool POST>
+int run_backward(const BlockNormGrads& a, const Grid& g, int blocks, cudaStream_t stream) {
+  constexpr int V = vec_of<T>();
+  if (g.threads <= 256) return go_backward<T, V, 2, POST, false, 256, 2, 2>(a, g, blocks, stream);
+  if (g.threads <= 512) return go_backward<T, V, 2, POST, false, 512, 1, 2>(a, g, blocks, stream);
+  if (g.nv <= 2) return go_backward<T, V, 2, POST, false, 1024, 1, 1>(a, g, blocks, stream);
+  if constexpr (sizeof(T) == 4) return go_backward<T, V, 4, POST, false, 1024, 1, 0>(a, g, blocks, stream);
   return -1;
 }
 
 template <typename T, bool WHOLE>
-int run_backward_single(const BlockNormGrads& a, const Grid& g, int sms, cudaStream_t stream) {
-  if (g.threads <= 256) return go_backward<T, 1, 4, !WHOLE, WHOLE, 256, kBwdBlocks, 0>(a, g, sms, stream);
-  if (g.nv <= 4) return go_backward<T, 1, 4, !WHOLE, WHOLE, 1024, 1, 0>(a, g, sms, stream);
-  return go_backward<T, 1, 16, !WHOLE, WHOLE, 1024, 1, 0>(a, g, sms, stream);
-}
-
-template <typename T>
-Grid backward_grid(int hidden, bool vec) {
-  return vec ? grid_of<T, vec_of<T>()>(hidden) : grid_of<T, 1>(hidden);
+int run_backward_single(const BlockNormGrads& a, const Grid& g, int blocks, cudaStream_t stream) {
+  constexpr int kDepth = sizeof(T) == 4 ? 2 : 0;
+  if (g.threads <= 256) return go_backward<T, 1, 4, !WHOLE, WHOLE, 256, 2, kDepth>(a, g, blocks, stream);
+  if (g.nv <= 4) return go_backward<T, 1, 4, !WHOLE, WHOLE, 1024, 1, kDepth>(a, g, blocks, stream);
+  return go_backward<T, 1, 16, !WHOLE, WHOLE, 1024, 1, 0>(a, g, blocks, stream);
 }
 
 template <typename T>
 int run_backward_type(const BlockNormGrads& a, bool vec, int sms, cudaStream_t stream) {
-  const Grid g = backward_grid<T>(a.hidden, vec);
   const bool whole = a.stream != nullptr;
+  const Grid g = backward_grid<T>(a.hidden, vec);
+  const int blocks = backward_blocks(g, a.rows, sms, vec, whole);
   int rc;
   if (vec)
-    rc = whole               ? run_backward<T, false, true>(a, g, sms, stream)
-         : a.post != nullptr ? run_backward<T, true, false>(a, g, sms, stream)
-                             : run_backward<T, false, false>(a, g, sms, stream);
+    rc = whole               ? run_backward_whole<T>(a, g, blocks, stream)
+         : a.post != nullptr ? run_backward<T, true>(a, g, blocks, stream)
+                             : run_backward<T, false>(a, g, blocks, stream);
   else
-    rc = whole ? run_backward_single<T, true>(a, g, sms, stream) : run_backward_single<T, false>(a, g, sms, stream);
+    rc = whole ? run_backward_single<T, true>(a, g, blocks, stream) : run_backward_single<T, false>(a, g, blocks, stream);
   if (rc != 0 || (a.dweight == nullptr && a.dpost == nullptr)) return rc;
   return launch_pdl(block_norm_sum_kernel<T>, dim3((a.hidden + 31) / 32, a.dpost != nullptr ? 2 : 1), dim3(1024), 0, stream,
                     static_cast<const float*>(a.dw_part), static_cast<const float*>(a.dpost_part),
-                    static_cast<T*>(a.dweight), static_cast<T*>(a.dpost), backward_blocks(g, a.rows, sms) * g.teams,
-                    a.hidden) == cudaSuccess ? 0 : -1;
+                    static_cast<T*>(a.dweight), static_cast<T*>(a.dpost), blocks * g.teams, a.hidden) == cudaSuccess ? 0
+                                                                                                                    : -1;
 }
 
 template <typename T>
-int parts_type(int rows, int hidden, bool vec, int sms) {
+int parts_type(int rows, int hidden, bool vec, bool whole, int sms) {
   const Grid g = backward_grid<T>(hidden, vec);
-  return backward_blocks(g, rows, sms) * g.teams;
+  return backward_blocks(g, rows, sms, vec, whole) * g.teams;
 }
 
 }  // namespace
@@ -618,11 +683,11 @@ int launch_block_norm(const BlockNormArgs& a, NormType type, bool vec, int fmt, 
   }
 }
 
-int block_norm_parts(NormType type, int rows, int hidden, bool vec, int sms) {
+int block_norm_parts(NormType type, int rows, int hidden, bool vec, bool whole, int sms) {
   switch (type) {
-    case kNormBf16: return parts_type<bf16>(rows, hidden, vec, sms);
-    case kNormFp16: return parts_type<__half>(rows, hidden, vec, sms);
-    default: return parts_type<float>(rows, hidden, vec, sms);
+    case kNormBf16: return parts_type<bf16>(rows, hidden, vec, whole, sms);
+    case kNormFp16: return parts_type<__half>(rows, hidden, vec, whole, sms);
+    default: return parts_type<float>(rows, hidden, vec, whole, sms);
   }
 }
 

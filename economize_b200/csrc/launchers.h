@@ -296,7 +296,7 @@ struct BlockNormGrads {
   float scale = 1.f;
 };
 int launch_block_norm(const BlockNormArgs& args, NormType type, bool vec, int fmt, int sms, cudaStream_t stream);
-int block_norm_parts(NormType type, int rows, int hidden, bool vec, int sms);
+int block_norm_parts(NormType type, int rows, int hidden, bool vec, bool whole, int sms);  // whole: from the stream
 int launch_block_norm_grads(const BlockNormGrads& args, NormType type, bool vec, int sms, cudaStream_t stream);
 
 // gemm_fp8.cu: block-scaled fp8 GEMM (e4m3 weights [N, K] with fp32 scales [N / 128, K / 128]; activations
