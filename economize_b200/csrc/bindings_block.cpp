@@ -175,8 +175,9 @@ CUtensorMap scales_map(const Fp4& x) {
   return map;
 }
 
-// y [M, N] of operands [M, K] and [N, K] of one format.
-void multiply(const Fp4& x, const Fp4& w, const Tensor& y, const at::Device& device) {
+// y [M, N] of operands [M, K] and [N, K] of one format. path: 0 by the sizes, 1 gemm_fp4.cu, 2 gemm_fp4_pair.cu.
+void multiply(const Fp4& x, const Fp4& w, const Tensor& y, const at::Device& device, int64_t path = 0) {
+  TORCH_CHECK_VALUE(path >= 0 && path <= 2, "fp4 product: path must be 0, 1 or 2");
   TORCH_CHECK_VALUE(x.K == w.K, "fp4 product: activations have ", x.K, " columns, the weight ", w.K);
   TORCH_CHECK_VALUE(w.rows >= 1, "fp4 product: the weight has no rows");
   if (x.rows == 0) return;
@@ -185,7 +186,7 @@ void multiply(const Fp4& x, const Fp4& w, const Tensor& y, const at::Device& dev
   unsigned* status = ecz::device_status(device);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   int rc;
-  if (M > 128) {
+  if (path == 2 || (path == 0 && M > 128)) {
     const CUtensorMap tx = codes_map(x, 128), tw = codes_map(w, 128), sx = scales_map(x), sw = scales_map(w);
     rc = ecz::launch_gemm_fp4_pair(&tx, &tw, &sx, &sw, x.row_scale, w.row_scale, x.fmt, y.data_ptr(), M, N, K, sms, status,
                                    stream);
@@ -198,12 +199,12 @@ void multiply(const Fp4& x, const Fp4& w, const Tensor& y, const at::Device& dev
 }
 
 Tensor fp4_matmul(const Tensor& x, const Tensor& xs, const Tensor& xr, const Tensor& w, const Tensor& ws, const Tensor& wr,
-                  int64_t fmt) {
+                  int64_t fmt, int64_t path) {
   CHECK_CUDA(x);
   const Fp4 a = check_operand(x, xs, xr, fmt, x, "fp4_matmul: x"), b = check_operand(w, ws, wr, fmt, x, "fp4_matmul: w");
   c10::cuda::CUDAGuard guard(x.device());
   Tensor y = at::empty({a.rows, b.rows}, x.options().dtype(at::kBFloat16));
-  multiply(a, b, y, x.device());
+  multiply(a, b, y, x.device(), path);
   return y;
 }
 
@@ -546,7 +547,7 @@ void bind_block(pybind11::module_& m) {
         py::arg("row_scale"), py::arg("fmt"));
   m.def("fp4_matmul", &fp4_matmul, "product of two 4-bit operands (tcgen05 block-scaled MMA)", py::arg("x"),
         py::arg("x_scales"), py::arg("x_row_scale"), py::arg("w"), py::arg("w_scales"), py::arg("w_row_scale"),
-        py::arg("fmt"));
+        py::arg("fmt"), py::arg("path") = 0);
   m.def("linear_fp4", &linear_fp4, "bf16 activations quantised and multiplied with a 4-bit weight", py::arg("x"),
         py::arg("w"), py::arg("w_scales"), py::arg("w_row_scale"), py::arg("fmt"));
   m.def("block_norm", &block_norm, "norm after a block, gate, residual scale and sum, norm before the next (autograd)",

@@ -82,9 +82,11 @@ struct Cfg {
   static constexpr int kBBytes = BN * kRowBytes;
   static constexpr int kScaleBytes = Format<FMT>::kBlockBytes;
   static constexpr int kStageBytes = kABytes + kBBytes + 2 * kScaleBytes;
-  static constexpr int kOcc = BN <= 64 ? 2 : 1;
-  static constexpr int kStages = std::min(8, (kOcc == 2 ? 104 : 200) * 1024 / kStageBytes);
-  static constexpr int kSmem = kStages * kStageBytes + 1024 + 256;
+  // two CTAs to an SM: with one of five stages at BN = 128, 224 tiles took two rounds
+  static constexpr int kOcc = 2;
+  static constexpr int kStages = std::min(8, 110 * 1024 / kStageBytes);
+  static constexpr int kSmem = kStages * kStageBytes + 1024 + 256 + BN * 4;
+  static_assert(kSmem <= 113 * 1024, "two CTAs to an SM");
   static constexpr int kAccCols = BN < 32 ? 32 : BN;
   static constexpr int kSlotCols = 2 * 4 * Format<FMT>::kTilesPerBlock;
   static constexpr int kCols = kAccCols + kSlots * kSlotCols;
@@ -120,6 +122,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, BN>::kOcc)
   uint64_t* acc_full = empty + S;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* x_row = reinterpret_cast<float*>(tmem_slot + 2);  // [BN]
 
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -205,7 +208,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, BN>::kOcc)
   bool ok = true;
   const int quarter = warp & 3;
   const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  const int cols = min(BN, args.M - m0), n = n0 + lane * 4;
+  float4 rw = make_float4(1.f, 1.f, 1.f, 1.f);
   if (warp >= 2) {
+    if constexpr (FMT == kNv) {  // at hand before the sums are
+      for (int j = threadIdx.x - 64; j < cols; j += 128) x_row[j] = args.x_row[m0 + j];
+    }
     ok = mbar_wait(acc_full, 0, args.status, kStatusWaitAccum, abort_flag);
     ok = __all_sync(0xffffffffu, ok) && !*abort_flag;
     tc_fence_after();
@@ -213,7 +221,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, BN>::kOcc)
   // This CTA's sums [BN][128] go where its stages were (every copy has landed and was read); each CTA of the cluster then
   // adds up and stores a share of the columns, four features a thread.
   float* part = reinterpret_cast<float*>(smem);
-  const int cols = min(BN, args.M - m0);
+  if constexpr (FMT == kNv) {
+    if (n < args.N) rw.x = args.w_row[n];
+    if (n + 1 < args.N) rw.y = args.w_row[n + 1];
+    if (n + 2 < args.N) rw.z = args.w_row[n + 2];
+    if (n + 3 < args.N) rw.w = args.w_row[n + 3];
+  }
   if (warp >= 2) {
 #pragma unroll
     for (int c = 0; c < BN; c += 16) {
@@ -228,14 +241,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, BN>::kOcc)
   if (splits > 1) cluster_sync();
   else __syncthreads();
   {
-    const int n = n0 + lane * 4;
-    float4 rw = make_float4(1.f, 1.f, 1.f, 1.f);
-    if constexpr (FMT == kNv) {
-      if (n < args.N) rw.x = args.w_row[n];
-      if (n + 1 < args.N) rw.y = args.w_row[n + 1];
-      if (n + 2 < args.N) rw.z = args.w_row[n + 2];
-      if (n + 3 < args.N) rw.w = args.w_row[n + 3];
-    }
     const uint32_t at = smem_u32(part) + lane * 16;
     for (int j = split + warp * splits; j < cols; j += splits * (kThreads / 32)) {
       float4 p[kMaxSplits];
@@ -253,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, BN>::kOcc)
           sum.w += p[r].w;
         }
       }
-      const float rx = FMT == kNv ? args.x_row[m0 + j] : 1.f;
+      const float rx = FMT == kNv ? x_row[j] : 1.f;
       const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x * (rx * rw.x), sum.y * (rx * rw.y));
       const __nv_bfloat162 hi = __floats2bfloat162_rn(sum.z * (rx * rw.z), sum.w * (rx * rw.w));
       bf16* out = args.y + static_cast<size_t>(m0 + j) * args.N + n;
