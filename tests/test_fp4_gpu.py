@@ -148,6 +148,19 @@ def test_product(cuda, fmt, rows, cols, out):
 
 
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("path", [1, 256, 384])
+@pytest.mark.parametrize("rows,cols,out", [(1, 32, 1), (130, 288, 385), (257, 1056, 768), (300, 4096, 1000), (2100, 544, 3200),
+                                           (1003, 2080, 6001)])
+def test_product_paths(cuda, fmt, path, rows, cols, out):
+    """Every kernel at sizes that it would not be chosen for, several tiles to a CTA pair among them."""
+    x = _normal(cuda, rows, cols, seed=rows, spread=0.7)
+    w = _normal(cuda, out, cols, seed=out, spread=0.3) * 0.05
+    a, b = ops.fp4_quantize(x, fmt), FP4Weight.from_weight(w, fmt)
+    y = ops.require().fp4_matmul(a.codes, a.scales, a.row_scale, b.codes, b.scales, b.row_scale, fp4.FORMATS[fmt], path)
+    _check_product(x, w, fmt, y)
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
 def test_product_exact(cuda, fmt):
     """One product in a sum, rounded once: every element, group and row scale in its place."""
     g = torch.Generator(device=cuda).manual_seed(5)
