@@ -175,10 +175,9 @@ CUtensorMap scales_map(const Fp4& x) {
   return map;
 }
 
-// y [M, N] of operands [M, K] and [N, K] of one format. path: 0 by the sizes, 1 gemm_fp4.cu, 256 or
-// 384 gemm_fp4_pair.cu with tiles of that width.
+// y [M, N] of operands [M, K] and [N, K] of one format. path: 0 by the sizes, 1 gemm_fp4.cu, 2 gemm_fp4_pair.cu.
 void multiply(const Fp4& x, const Fp4& w, const Tensor& y, const at::Device& device, int64_t path = 0) {
-  TORCH_CHECK_VALUE(path == 0 || path == 1 || path == 256 || path == 384, "fp4 product: path must be 0, 1, 256 or 384");
+  TORCH_CHECK_VALUE(path >= 0 && path <= 2, "fp4 product: path must be 0, 1 or 2");
   TORCH_CHECK_VALUE(x.K == w.K, "fp4 product: activations have ", x.K, " columns, the weight ", w.K);
   TORCH_CHECK_VALUE(w.rows >= 1, "fp4 product: the weight has no rows");
   if (x.rows == 0) return;
@@ -187,10 +186,9 @@ void multiply(const Fp4& x, const Fp4& w, const Tensor& y, const at::Device& dev
   unsigned* status = ecz::device_status(device);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   int rc;
-  if (path > 1 || (path == 0 && M > 128)) {
-    const ecz::Fp4PairMaps maps{codes_map(x, 128), codes_map(w, 128), codes_map(w, 64), scales_map(x), scales_map(w)};
-    rc = ecz::launch_gemm_fp4_pair(maps, x.row_scale, w.row_scale, x.fmt, y.data_ptr(), M, N, K, static_cast<int>(path), sms,
-                                   status, stream);
+  if (path == 2 || (path == 0 && M > 128)) {
+    const ecz::Fp4PairMaps maps{codes_map(x, 128), codes_map(w, 128), scales_map(x), scales_map(w)};
+    rc = ecz::launch_gemm_fp4_pair(maps, x.row_scale, w.row_scale, x.fmt, y.data_ptr(), M, N, K, sms, status, stream);
   } else {
     const CUtensorMap tw = codes_map(w, 128), tx = codes_map(x, ecz::fp4_block_rows(M));
     rc = ecz::launch_gemm_fp4(&tw, &tx, w.scales, x.scales, w.row_scale, x.row_scale, x.fmt, y.data_ptr(), M, N, K, sms,

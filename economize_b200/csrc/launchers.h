@@ -242,14 +242,13 @@ int launch_gemm_fp4(const CUtensorMap* w, const CUtensorMap* x, const void* w_sc
                     const float* w_row, const float* x_row, int fmt, void* y, int M, int N, int K, int sms,
                     unsigned* status, cudaStream_t stream);
 
-// gemm_fp4_pair.cu: the same for many rows, on CTA pairs. width: of the tiles, 256 or 384 (0: by the sizes).
+// gemm_fp4_pair.cu: the same for many rows, on CTA pairs.
 struct Fp4PairMaps {
   CUtensorMap x, w;    // codes in boxes of {128, 128}
-  CUtensorMap w64;     // and of {128, 64}
   CUtensorMap sx, sw;  // scales as rows of 128 bytes in boxes of one K block's 128 rows ({128, 16} nvfp4, {128, 8} mxfp4)
 };
 int launch_gemm_fp4_pair(const Fp4PairMaps& maps, const float* x_row, const float* w_row, int fmt, void* y, int M, int N,
-                         int K, int width, int sms, unsigned* status, cudaStream_t stream);
+                         int K, int sms, unsigned* status, cudaStream_t stream);
 
 // block_norm.cu: norm after a block, gate, residual scale and sum, norm before the next block (see the file comment).
 // Strides in elements between rows; outputs are contiguous. vec: every operand allows 16-byte vectors.

@@ -148,7 +148,7 @@ def test_product(cuda, fmt, rows, cols, out):
 
 
 @pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
-@pytest.mark.parametrize("path", [1, 256, 384])
+@pytest.mark.parametrize("path", [1, 2])
 @pytest.mark.parametrize("rows,cols,out", [(1, 32, 1), (130, 288, 385), (257, 1056, 768), (300, 4096, 1000), (2100, 544, 3200),
                                            (1003, 2080, 6001)])
 def test_product_paths(cuda, fmt, path, rows, cols, out):
