@@ -187,7 +187,10 @@ void multiply(const Fp4& x, const Fp4& w, const Tensor& y, const at::Device& dev
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   int rc;
   if (path == 2 || (path == 0 && M > 128)) {
-    const ecz::Fp4PairMaps maps{codes_map(x, 128), codes_map(w, 128), scales_map(x), scales_map(w)};
+    ecz::Fp4PairMaps maps{codes_map(x, 128), codes_map(w, 128), scales_map(x), scales_map(w), {}};
+    if (N % 8 == 0)
+      TORCH_CHECK(ecz::make_tmap_2d(&maps.y, 2, y.data_ptr(), M, N, int64_t{2} * N, 32, 32, 64) == 0,
+                  "cuTensorMapEncodeTiled failed for a ", M, " x ", N, " result");
     rc = ecz::launch_gemm_fp4_pair(maps, x.row_scale, w.row_scale, x.fmt, y.data_ptr(), M, N, K, sms, status, stream);
   } else {
     const CUtensorMap tw = codes_map(w, 128), tx = codes_map(x, ecz::fp4_block_rows(M));

@@ -5,7 +5,7 @@
 //
 //   warp 0      TMA producer of the codes (both CTAs; completion counted on the even CTA's barrier)
 //   warp 1      even CTA: copies a block's scales to tensor memory of both CTAs, issues its four MMAs of 64 columns
-//   warps 2-9   epilogue: warp w holds TMEM lanes 32 (w % 4) .. + 31 (rows) and 128 of the 256 columns
+//   warps 2-9   epilogue: warp w holds TMEM lanes 32 (w % 4) .. + 31 (rows) and 128 of the 256 columns; TMA stores them
 //   warp 10     TMA producer of the scales (both CTAs): a thread takes 70 cycles to issue a copy, and the five of a block
 //               from one thread took longer than its MMAs
 //
@@ -35,8 +35,8 @@ constexpr int kOperandBytes = kHalf * kBlockK / 2;
 constexpr int kThreads = 352;
 constexpr int kEpiWarps = 8;
 constexpr int kScaleWarp = 2 + kEpiWarps;
-constexpr int kPatchStride = 80;  // bytes per row of an epilogue warp's [32 rows, 32 bf16] patch
-constexpr int kPatchBytes = 32 * kPatchStride + 128 * 4;
+constexpr int kPatchBytes = 32 * 64;  // [32 rows, 32 bf16], 64-byte swizzle; an epilogue warp has two
+constexpr int kEpiBytes = 2 * kPatchBytes + 128 * 2;  // and the row scales of its 128 features
 constexpr int kStages = 5;  // and places for scales in tensor memory
 constexpr int kStrip = 8;
 
@@ -44,7 +44,7 @@ template <int FMT>
 struct PairCfg {
   static constexpr int kScaleBytes = Format<FMT>::kBlockBytes;              // of 128 rows
   static constexpr int kStageBytes = 2 * kOperandBytes + 3 * kScaleBytes;
-  static constexpr int kSmem = kStages * kStageBytes + kEpiWarps * kPatchBytes + 1024 + 256;
+  static constexpr int kSmem = kStages * kStageBytes + kEpiWarps * kEpiBytes + 1024 + 256;
   static constexpr int kSlotCols = 3 * 4 * Format<FMT>::kTilesPerBlock;     // 128 rows of A, 256 of B
   static_assert(kSmem <= 232448, "227 KB of shared memory");
   static_assert(kTile + kStages * kSlotCols <= 512, "tensor memory");
@@ -108,14 +108,14 @@ template <int FMT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                          const __grid_constant__ CUtensorMap tm_sx, const __grid_constant__ CUtensorMap tm_sw,
-                         const __grid_constant__ PairArgs args) {
+                         const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ PairArgs args) {
   using C = PairCfg<FMT>;
   constexpr int kT = Format<FMT>::kTilesPerBlock;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* scales = smem + kStages * 2 * kOperandBytes;
   uint8_t* patches = smem + kStages * C::kStageBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(patches + kEpiWarps * kPatchBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(patches + kEpiWarps * kEpiBytes);
   uint64_t* empty = full + kStages;
   uint64_t* acc_full = empty + kStages;
   uint64_t* acc_empty = acc_full + 1;
@@ -137,6 +137,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tm_w);
     tma_prefetch_desc(&tm_sx);
     tma_prefetch_desc(&tm_sw);
+    if (args.N % 8 == 0) tma_prefetch_desc(&tm_y);
   }
   __syncwarp();
   if (warp == 0) {
@@ -247,23 +248,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp >= 2 && warp < kScaleWarp) {
     // ---- epilogue ----
     const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
-    uint8_t* patch = patches + ew * kPatchBytes;
-    float* features = reinterpret_cast<float*>(patch + 32 * kPatchStride);  // row scales of this warp's 128 features
+    uint8_t* patch = patches + ew * 2 * kPatchBytes;
+    bf16* features = reinterpret_cast<bf16*>(patches + kEpiWarps * 2 * kPatchBytes) + ew * 128;
     const uint32_t taddr = tmem + (static_cast<uint32_t>(quad * 32) << 16) + half * 128u;
-    const bool whole_rows = args.N % 8 == 0;  // 16-byte rows of y
-    uint32_t tile = 0;
-    for (int t = pair_id; t < tiles.total; t += pairs, ++tile) {
+    const bool whole_rows = args.N % 8 == 0;  // 16-byte rows of y, which TMA stores
+    int row0, col0;
+    float rx = 1.f, rw[4] = {1.f, 1.f, 1.f, 1.f};  // powers of two of this lane's row and of features 32 i + lane
+    auto locate = [&](int t) {
       int m0, n0;
       tiles.at(t, m0, n0);
-      const int row0 = m0 + static_cast<int>(rank) * kHalf + quad * 32, col0 = n0 + half * 128;
-      float rx = 1.f;
-      if constexpr (FMT == kNv) {  // the rows' powers of two, at hand before the sums are
-        if (row0 + lane < args.M) rx = args.x_row[row0 + lane];
+      row0 = m0 + static_cast<int>(rank) * kHalf + quad * 32;
+      col0 = n0 + half * 128;
+    };
+    auto row_scales = [&]() {
+      if constexpr (FMT == kNv) {
+        rx = row0 + lane < args.M ? args.x_row[row0 + lane] : 1.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int n = col0 + i * 32 + lane;
-          features[i * 32 + lane] = n < args.N ? args.w_row[n] : 1.f;
-        }
+        for (int i = 0; i < 4; ++i) rw[i] = col0 + i * 32 + lane < args.N ? args.w_row[col0 + i * 32 + lane] : 1.f;
+      }
+    };
+    if (pair_id < tiles.total) {
+      locate(pair_id);
+      row_scales();
+    }
+    uint32_t tile = 0;
+    for (int t = pair_id; t < tiles.total; t += pairs, ++tile) {
+      const __nv_bfloat162 rx2 = __float2bfloat162_rn(rx);
+      if constexpr (FMT == kNv) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) features[i * 32 + lane] = __float2bfloat16(rw[i]);
         __syncwarp();
       }
       const bool ok = mbar_wait(acc_full, tile & 1u, args.status, kStatusWaitAccum, abort_flag);
@@ -275,48 +288,56 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) pair::arrive_cluster(pair::mapa_u32(smem_u32(acc_empty), 0));
+      const int row = row0, col = col0;
+      if (t + pairs < tiles.total) {  // the next tile's scales are fetched under this one's stores
+        locate(t + pairs);
+        row_scales();
+      }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        // a lane's 32 columns into its row of the patch, then rows out in 64-byte pieces
-#pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-          uint32_t out[4];
-#pragma unroll
-          for (int i = 0; i < 8; i += 4) {
-            float* p = v + g * 32 + j + i;
-            if constexpr (FMT == kNv) {
-              const float4 w = *reinterpret_cast<const float4*>(features + g * 32 + j + i);
-              p[0] *= rx * w.x;
-              p[1] *= rx * w.y;
-              p[2] *= rx * w.z;
-              p[3] *= rx * w.w;
-            }
-            out[i / 2] = packed::pack_bf16(p[0], p[1]);
-            out[i / 2 + 1] = packed::pack_bf16(p[2], p[3]);
-          }
-          *reinterpret_cast<uint4*>(patch + lane * kPatchStride + j * 2) = make_uint4(out[0], out[1], out[2], out[3]);
-        }
-        __syncwarp();
-        const int n = col0 + g * 32;
+        // a lane's 32 columns, rounded to bf16 and then multiplied by the powers of two, into its row of a patch
+        uint8_t* to = patch + (g & 1) * kPatchBytes;
         if (whole_rows) {
-          const int c = (lane & 3) * 8;
-          if (n + c < args.N) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = i * 8 + (lane >> 2);
-              if (row0 + r < args.M)
-                *reinterpret_cast<uint4*>(args.y + static_cast<size_t>(row0 + r) * args.N + n + c) =
-                    *reinterpret_cast<const uint4*>(patch + r * kPatchStride + c * 2);
-            }
-          }
-        } else if (n + lane < args.N) {
-          for (int r = 0; r < 32 && row0 + r < args.M; ++r)
-            args.y[static_cast<size_t>(row0 + r) * args.N + n + lane] =
-                *reinterpret_cast<const bf16*>(patch + r * kPatchStride + lane * 2);
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          __syncwarp();
         }
-        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          __nv_bfloat162 out[4];
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if constexpr (FMT == kNv) w = *reinterpret_cast<const uint4*>(features + g * 32 + j * 8);
+          const __nv_bfloat162* w2 = reinterpret_cast<const __nv_bfloat162*>(&w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            out[i] = __floats2bfloat162_rn(v[g * 32 + j * 8 + 2 * i], v[g * 32 + j * 8 + 2 * i + 1]);
+            if constexpr (FMT == kNv) out[i] = __hmul2(__hmul2(out[i], rx2), w2[i]);
+          }
+          *reinterpret_cast<uint4*>(to + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = *reinterpret_cast<uint4*>(out);
+        }
+        const int n = col + g * 32;
+        if (whole_rows) {
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (row < args.M && n < args.N)
+              asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                               reinterpret_cast<uint64_t>(&tm_y)),
+                           "r"(n), "r"(row), "r"(smem_u32(to))
+                           : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        } else {
+          __syncwarp();
+          if (n + lane < args.N) {
+            for (int r = 0; r < 32 && row + r < args.M; ++r)
+              args.y[static_cast<size_t>(row + r) * args.N + n + lane] = *reinterpret_cast<const bf16*>(
+                  to + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+          }
+          __syncwarp();
+        }
       }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   __syncwarp();
   tc_fence_before();
@@ -333,7 +354,7 @@ int run(const Fp4PairMaps& maps, const PairArgs& args, int sms, cudaStream_t str
   if (tiles > (1 << 30) || set_max_smem(kernel, PairCfg<FMT>::kSmem) != cudaSuccess) return -1;
   const int pairs = static_cast<int>(std::min<long>(tiles, sms / 2));
   return launch_pdl(kernel, dim3(2 * pairs), dim3(kThreads), PairCfg<FMT>::kSmem, stream, maps.x, maps.w, maps.sx, maps.sw,
-                    args) == cudaSuccess ? 0 : -1;
+                    maps.y, args) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace

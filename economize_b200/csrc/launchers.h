@@ -246,6 +246,7 @@ int launch_gemm_fp4(const CUtensorMap* w, const CUtensorMap* x, const void* w_sc
 struct Fp4PairMaps {
   CUtensorMap x, w;    // codes in boxes of {128, 128}
   CUtensorMap sx, sw;  // scales as rows of 128 bytes in boxes of one K block's 128 rows ({128, 16} nvfp4, {128, 8} mxfp4)
+  CUtensorMap y;       // the result in boxes of {32, 32}, 64-byte swizzle (unused where N is no multiple of 8)
 };
 int launch_gemm_fp4_pair(const Fp4PairMaps& maps, const float* x_row, const float* w_row, int fmt, void* y, int M, int N,
                          int K, int sms, unsigned* status, cudaStream_t stream);
