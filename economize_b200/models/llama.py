@@ -263,8 +263,7 @@ class CausalLM(nn.Module):
             x_in = None
             # a layer view may skip a sublayer (self-drafting): the pending branch output is added at the next norm
             if not getattr(layer, "skip_attn", False):
-                h, partial = self._scale_branch(h, partial)
-                x, resid = self._norm(h, layer.attn_norm, resid, partial)
+                x, resid = self._input_norm(layer, layer.attn_norm, layer.wqkv, h, resid, partial)
                 if i in capture:
                     aux[i] = resid
                 x_in = resid
@@ -273,8 +272,7 @@ class CausalLM(nn.Module):
             elif i in capture:
                 raise ValueError(f"cannot capture the input of layer {i}: its attention is skipped")
             if not getattr(layer, "skip_mlp", False):
-                h, partial = self._scale_branch(h, partial)
-                x, resid = self._norm(h, layer.mlp_norm, resid, partial)
+                x, resid = self._input_norm(layer, layer.mlp_norm, layer.w_gate_up, h, resid, partial)
                 h = self._mlp(layer, x, i)
                 partial = True
             if gated and x_in is not None:
@@ -312,6 +310,23 @@ class CausalLM(nn.Module):
 
         return move
 
+    def _takes_fp4(self, layer: DecoderLayer, weight) -> bool:
+        """Whether the norm in front of the projection ``weight`` may hand it its result in 4 bits: the projection
+        multiplies in 4 bits on CUDA and is the result's only reader."""
+        return isinstance(weight, ops.FP4Weight) and weight.device.type == "cuda" and self.dtype == torch.bfloat16 and \
+            self.observer is None and (self.tp is None or self.tp.size == 1) and self.placement is None and \
+            not any(getattr(layer, name, None) for name in ("mlp_rule", "attn_input_hook"))
+
+    def _input_norm(self, layer: DecoderLayer, norm: torch.Tensor, weight, h, resid: torch.Tensor | None, partial: bool):
+        """The sublayer's input and the residual stream: ``resid`` plus the pending branch output ``h`` (times Granite's
+        residual multiplier), normed for the projection ``weight``, in 4 bits where it multiplies in such
+        (:func:`economize_b200.ops.block_norm`)."""
+        if self._takes_fp4(layer, weight) and not isinstance(h, ops.Partials):
+            scale = self.config.residual_multiplier if partial else 1.0
+            return ops.block_norm(h, resid, norm, scale=scale, eps=self.config.rms_norm_eps, quantize=weight.fmt)
+        h, partial = self._scale_branch(h, partial)
+        return self._norm(h, norm, resid, partial)
+
     def _scale_branch(self, h, partial: bool):
         """A branch output times Granite's residual multiplier before it joins the residual stream (a no-op for
         the other families; the embeddings entering the first block are never scaled)."""
@@ -340,8 +355,13 @@ class CausalLM(nn.Module):
                 aux[i] = h
             x = ops.rmsnorm(h, layer.attn_norm, eps)[0] if sandwich else h
             a = self._materialize(self._attention(layer, i, x, batch, cache, cos, sin), True)
-            h = h + ops.rmsnorm(a, layer.attn_post_norm if sandwich else layer.attn_norm, eps)[0]
-            x = ops.rmsnorm(h, layer.mlp_norm, eps)[0] if sandwich else h
+            if sandwich and self._takes_fp4(layer, layer.w_gate_up):
+                # both norms around the residual sum in one kernel, its result in 4 bits
+                x, h = ops.block_norm(a, h, layer.mlp_norm, post_weight=layer.attn_post_norm, eps=eps,
+                                      quantize=layer.w_gate_up.fmt)
+            else:
+                h = h + ops.rmsnorm(a, layer.attn_post_norm if sandwich else layer.attn_norm, eps)[0]
+                x = ops.rmsnorm(h, layer.mlp_norm, eps)[0] if sandwich else h
             m = self._materialize(self._mlp(layer, x, i), True)
             h = h + ops.rmsnorm(m, layer.mlp_post_norm if sandwich else layer.mlp_norm, eps)[0]
         if staged is not None:

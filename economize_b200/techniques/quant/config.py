@@ -15,10 +15,12 @@ from ...core.technique import TechniqueConfig
 from ...errors import ConfigError
 from ...validation import check_choice, check_positive
 
-__all__ = ["DraftQuantConfig", "QUANT_FORMATS", "QUANT_METHODS_NAMES", "QuantConfig"]
+__all__ = ["DraftQuantConfig", "QUANT_FORMATS", "QUANT_METHODS_NAMES", "QuantConfig", "W4A4_FORMATS"]
 
 #: formats the packed kernel layout stores
-QUANT_FORMATS = ("int2", "int3", "int4", "int8", "fp8", "fp8_block", "mxfp4", "nvfp4")
+QUANT_FORMATS = ("int2", "int3", "int4", "int8", "fp8", "fp8_block", "mxfp4", "nvfp4", "mxfp4_w4a4", "nvfp4_w4a4")
+#: formats whose products take 4-bit activations too, and the 4-bit format of either operand
+W4A4_FORMATS = {"mxfp4_w4a4": "mxfp4", "nvfp4_w4a4": "nvfp4"}
 QUANT_METHODS_NAMES = ("rtn", "gptq", "awq", "hqq", "smoothquant")
 #: engine projection names and the Hugging Face module names fused into them
 PROJECTIONS = {"wqkv": ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj"), "wo": ("self_attn.o_proj",),
@@ -32,8 +34,8 @@ def _check_common(config) -> None:
         check_positive("group_size", config.group_size)
         if config.group_size % 64:
             raise ConfigError(f"group_size must be a multiple of 64 (the kernel's K tile), got {config.group_size}")
-    if config.format == "fp8_block":
-        return  # 128 x 128 weight blocks and 1 x 128 activation blocks are fixed by the format
+    if config.format == "fp8_block" or config.format in W4A4_FORMATS:
+        return  # 128 x 128 weight blocks and 1 x 128 activation blocks, or groups of 16 or 32, are fixed by the format
     if config.format in ("int8", "fp8") and not config.symmetric:
         raise ConfigError(f"{config.format} weights are stored symmetric (no zero point): set symmetric=True")
 
@@ -46,11 +48,13 @@ class QuantConfig(TechniqueConfig):
         format: ``"int4"`` (default, GPTQ/AWQ W4A16), ``"int3"`` / ``"int2"`` (W3A16 in the int4 layout, W2A16
             packed 16 per word), ``"mxfp4"`` / ``"nvfp4"`` (FP4 E2M1 weights with a scale per 32 / 16 columns;
             ``group_size`` and ``symmetric`` do not apply), ``"int8"`` (W8A16), ``"fp8"`` (e4m3 weights, bf16
-            activations) or ``"fp8_block"`` (W8A8: e4m3 weights with 128 x 128 block scales and activations
-            quantised per token and 128-wide block on the fly; ``group_size`` is ignored).
+            activations), ``"fp8_block"`` (W8A8: e4m3 weights with 128 x 128 block scales and activations
+            quantised per token and 128-wide block on the fly; ``group_size`` is ignored), or ``"mxfp4_w4a4"`` /
+            ``"nvfp4_w4a4"`` (W4A4: weights and activations in 4 bits with a scale per 32 / 16 columns, multiplied on
+            the tensor cores' 4-bit path; activations are quantised on the fly; ``group_size`` is ignored).
         method: ``"rtn"`` (round to nearest, no data), ``"hqq"`` (half-quadratic fit of the grid, no data),
             ``"smoothquant"`` (activation outliers migrated into the weights, then round to nearest: for W8A8 with
-            ``format="fp8_block"``), ``"gptq"`` (Hessian-aware error feedback, needs
+            ``format="fp8_block"`` and for W4A4), ``"gptq"`` (Hessian-aware error feedback, needs
             calibration tokens) or ``"awq"`` (activation-aware scaling folded into the preceding norm, then round
             to nearest with clipping search; needs calibration tokens).
         group_size: Input columns per scale (``None``: one scale per output row).
@@ -100,6 +104,8 @@ class QuantConfig(TechniqueConfig):
             raise ConfigError("layers are 1-indexed")
         if self.method in ("gptq", "awq", "hqq") and self.format in ("fp8", "fp8_block"):
             raise ConfigError(f"{self.method} fits integer grids; use method='rtn' for fp8")
+        if self.method in ("gptq", "awq", "hqq") and self.format in W4A4_FORMATS:
+            raise ConfigError(f"{self.method} fits weight-only grids; use method='rtn' or 'smoothquant' for W4A4")
         if self.method in ("hqq", "smoothquant") and self.format in ("mxfp4", "nvfp4"):
             raise ConfigError(f"{self.method} does not fit FP4 grids; use rtn, gptq or awq")
         check_positive("hqq_iters", self.hqq_iters)
@@ -119,8 +125,9 @@ class QuantConfig(TechniqueConfig):
         bad = [i for i in self.layers if i > n]
         if bad:
             raise ConfigError(f"layers {bad} exceed the model's {n} layers")
-        if model.config.is_moe and self.format != "fp8_block":
-            raise ConfigError("MoE models take format='fp8_block' (attention projections; experts stay bf16)")
+        if model.config.is_moe and self.format != "fp8_block" and self.format not in W4A4_FORMATS:
+            raise ConfigError("MoE models take format='fp8_block' or a W4A4 format (attention projections; experts stay "
+                              "bf16)")
 
 
 @dataclass(frozen=True)

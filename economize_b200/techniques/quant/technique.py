@@ -1,5 +1,6 @@
 """``quant`` and ``draft_quant`` techniques: replace projections by packed :class:`~economize_b200.ops.quant.QWeight`
-weights that the tcgen05 weight-only GEMM reads (economize ``techniques/quant/technique.py:30-120``).
+weights that the tcgen05 weight-only GEMM reads, or by weights whose products quantise their activations too
+(:class:`~economize_b200.ops.fp8.FP8BlockWeight`, :class:`~economize_b200.ops.fp4.FP4Weight`) (economize ``techniques/quant/technique.py:30-120``).
 
 The quantized weights (and, after AWQ, the re-scaled norm and producer weights) are the technique's state, so a
 saved model reloads without recalibrating.
@@ -15,10 +16,11 @@ from torch import nn
 
 from ...core.technique import Capability, Family, Technique, register_technique
 from ...errors import ConfigError
+from ...ops.fp4 import FP4Weight
 from ...ops.fp8 import FP8BlockWeight
 from ...ops.quant import CODES_PER_BYTE, FP4_GROUP, QWeight, install
 from . import methods
-from .config import PROJECTIONS, DraftQuantConfig, QuantConfig
+from .config import PROJECTIONS, W4A4_FORMATS, DraftQuantConfig, QuantConfig
 
 __all__ = ["DraftQuantTechnique", "QuantTechnique"]
 
@@ -46,7 +48,7 @@ class _QuantBase(Technique):
     def technique_state(self) -> dict[str, torch.Tensor]:
         out = {}
         for key, qw in self.weights.items():
-            for buf in ("codes", "qweight", "scales", "zeros"):
+            for buf in ("codes", "qweight", "scales", "zeros", "row_scale"):
                 t = getattr(qw, buf, None)
                 if t is not None:
                     out[f"weights.{key}.{buf}"] = t.detach()
@@ -67,6 +69,10 @@ class _QuantBase(Technique):
                 raise ConfigError(f"{self.name}: unexpected tensor {name}")
         self.weights = nn.ModuleDict()
         for key, bufs in found.items():
+            if cfg.format in W4A4_FORMATS:
+                self.weights[key] = FP4Weight(bufs["codes"], bufs["scales"], bufs["row_scale"], W4A4_FORMATS[cfg.format],
+                                              self._dtype())
+                continue
             if "codes" in bufs:
                 self.weights[key] = FP8BlockWeight(bufs["codes"], bufs["scales"], self._dtype())
                 continue
@@ -97,7 +103,7 @@ class QuantTechnique(_QuantBase):
         self._calibration = calibration
 
     def _targets(self) -> dict[int, list[str]]:
-        """Projections to quantize; those whose input width the group size (or the kernel's 64-wide K tile) does
+        """Projections to quantize; those whose input width the group size (or the kernel's K tile: 64, W4A4 32) does
         not divide are skipped and listed in ``self.skipped``."""
         cfg: QuantConfig = self.config
         layers = [i - 1 for i in cfg.layers] if cfg.layers else range(self.model.config.num_layers)
@@ -113,9 +119,13 @@ class QuantTechnique(_QuantBase):
                     self.skipped.append(f"layers.{i}.{n}")
                     continue
                 k = w.shape[1]
-                block = cfg.format == "fp8_block"
-                if (block and (k % 128 or w.shape[0] % 128)) or \
-                        (not block and (k % 64 or (cfg.group_size and k % cfg.group_size))):
+                if cfg.format in W4A4_FORMATS:
+                    fits = k % 32 == 0 and k <= 65536
+                elif cfg.format == "fp8_block":
+                    fits = k % 128 == 0 and w.shape[0] % 128 == 0
+                else:
+                    fits = k % 64 == 0 and not (cfg.group_size and k % cfg.group_size)
+                if not fits:
                     self.skipped.append(f"layers.{i}.{n}")
                     continue
                 names.append(n)
@@ -148,6 +158,9 @@ class QuantTechnique(_QuantBase):
                 w = getattr(layer, name).detach()
                 if cfg.format == "fp8_block":
                     self.weights[_key(i, name)] = FP8BlockWeight.from_weight(w)
+                    continue
+                if cfg.format in W4A4_FORMATS:
+                    self.weights[_key(i, name)] = FP4Weight.from_weight(w, W4A4_FORMATS[cfg.format])
                     continue
                 if cfg.method == "gptq":
                     qw = methods.gptq(w, stats[(i, name)].hessian, cfg.format, cfg.group_size, cfg.symmetric,
@@ -262,6 +275,10 @@ class DraftQuantTechnique(_QuantBase):
                 if p.dim() != 2 or not _selected((name,), cfg.targets, cfg.exclude):
                     continue
                 k = p.shape[1]
+                if cfg.format in W4A4_FORMATS:
+                    if k % 32 == 0:
+                        self.weights[name.replace(".", "/")] = FP4Weight.from_weight(p.detach(), W4A4_FORMATS[cfg.format])
+                    continue
                 g = cfg.group_size if cfg.group_size and k % cfg.group_size == 0 else None
                 if (g or k) % 64 or k % 64 or p.shape[0] % 8:
                     continue

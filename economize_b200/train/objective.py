@@ -191,38 +191,34 @@ def dense_linear(x: torch.Tensor, w, b: torch.Tensor | None = None) -> torch.Ten
     return F.linear(x, w, b)
 
 
-def _check_plain_block(config) -> None:
+def _check_plain_block(config, scaled: bool = False) -> None:
     """Refuse the block variants :func:`torch_block` does not model (it is the Llama block: pre-norms, per-head q/k
-    norms, causal attention over the whole row, a dense SwiGLU MLP)."""
+    norms, causal attention over the whole row, a dense SwiGLU MLP). ``scaled``: scaled attention and residuals are
+    modelled (:func:`packed_block`)."""
     variants = {"MoE MLPs": config.is_moe, "sandwich norms": config.sandwich_norm, "post norms": config.post_norm,
                 "full-width q/k norms": config.qk_norm_full, "NoPE layers": bool(config.nope_layers),
                 "sliding windows": any(config.window_of(i) for i in range(config.num_layers)),
                 "soft-caps": bool(config.attn_softcap), "sink logits": config.attn_sinks,
                 "an output-projection bias": config.o_bias, "a non-SwiGLU activation": config.hidden_act != "silu",
-                "scaled attention or residuals": config.attention_multiplier is not None
-                or config.residual_multiplier != 1.0, "position-scaled queries": config.query_position_scale is not None}
+                "scaled attention or residuals": not scaled and (config.attention_multiplier is not None
+                                                                 or config.residual_multiplier != 1.0), "position-scaled queries": config.query_position_scale is not None}
     found = [name for name, present in variants.items() if present]
     if found:
         raise ConfigError(f"the PyTorch training block models the Llama block; {config.model_type} has "
                           f"{', '.join(found)}")
 
 
-def torch_block(layer, h: torch.Tensor, config, cos: torch.Tensor, sin: torch.Tensor,
-                cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
-    """A pre-norm decoder block in plain PyTorch (autograd, causal attention over the whole row): the residual
-    stream ``h [B, S, H]`` in, the block's output stream out. Used to train technique-owned blocks and adapters.
-    With ``cu_seqlens`` the one row ``h [1, T, H]`` is packed sequences, each attended by itself
-    (:func:`~economize_b200.ops.packed_attention`), and ``cos`` / ``sin [T, D / 2]`` are those of its positions."""
+def _block_attention(layer, x: torch.Tensor, config, cos: torch.Tensor, sin: torch.Tensor,
+                     cu_seqlens: torch.Tensor | None) -> torch.Tensor:
+    """The attention branch of :func:`torch_block` for the normed input ``x [B, S, H]``."""
     import torch.nn.functional as F
 
     from ..ops.reference import rmsnorm
 
     lin = dense_linear
-    _check_plain_block(config)
     eps = config.rms_norm_eps
-    batch, length, _ = h.shape
+    batch, length, _ = x.shape
     heads, kv_heads, hd = config.num_heads, config.num_kv_heads, config.head_dim
-    x = rmsnorm(h, layer.attn_norm, eps)[0]
     q, k, v = lin(x, layer.wqkv, layer.bqkv).split([heads * hd, kv_heads * hd, kv_heads * hd], -1)
     q = q.reshape(batch, length, heads, hd)
     k = k.reshape(batch, length, kv_heads, hd)
@@ -241,9 +237,16 @@ def torch_block(layer, h: torch.Tensor, config, cos: torch.Tensor, sin: torch.Te
         o = F.scaled_dot_product_attention(q, k.repeat_interleave(group, 1), v.repeat_interleave(group, 1),
                                            is_causal=True).transpose(1, 2)
     else:
-        o = ops.packed_attention(rot(q)[0], rot(k)[0], v.reshape(length, kv_heads, hd), cu_seqlens)
-    h = h + lin(o.reshape(batch, length, heads * hd), layer.wo)
-    x = rmsnorm(h, layer.mlp_norm, eps)[0]
+        o = ops.packed_attention(rot(q)[0], rot(k)[0], v.reshape(length, kv_heads, hd), cu_seqlens,
+                                 scale=config.attention_multiplier)
+    return lin(o.reshape(batch, length, heads * hd), layer.wo)
+
+
+def _block_mlp(layer, x: torch.Tensor) -> torch.Tensor:
+    """The MLP branch of :func:`torch_block` for the normed input ``x``."""
+    import torch.nn.functional as F
+
+    lin = dense_linear
     g, u = lin(x, layer.w_gate_up).chunk(2, -1)
     a = F.silu(g) * u
     block = getattr(layer, "down_hadamard", 0)  # the online rotation the rotate technique folded into w_down
@@ -251,7 +254,41 @@ def torch_block(layer, h: torch.Tensor, config, cos: torch.Tensor, sin: torch.Te
         from ..ops import reference
 
         a = reference.hadamard(a, block)
-    return h + lin(a, layer.w_down)
+    return lin(a, layer.w_down)
+
+
+def torch_block(layer, h: torch.Tensor, config, cos: torch.Tensor, sin: torch.Tensor,
+                cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
+    """A pre-norm decoder block in plain PyTorch (autograd, causal attention over the whole row): the residual
+    stream ``h [B, S, H]`` in, the block's output stream out. Used to train technique-owned blocks and adapters.
+    With ``cu_seqlens`` the one row ``h [1, T, H]`` is packed sequences, each attended by itself
+    (:func:`~economize_b200.ops.packed_attention`), and ``cos`` / ``sin [T, D / 2]`` are those of its positions."""
+    from ..ops.reference import rmsnorm
+
+    _check_plain_block(config)
+    eps = config.rms_norm_eps
+    x = rmsnorm(h, layer.attn_norm, eps)[0]
+    h = h + _block_attention(layer, x, config, cos, sin, cu_seqlens)
+    x = rmsnorm(h, layer.mlp_norm, eps)[0]
+    return h + _block_mlp(layer, x)
+
+
+def packed_block(layer, branch: torch.Tensor | None, h: torch.Tensor, config, cos: torch.Tensor, sin: torch.Tensor,
+                 cu_seqlens: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`torch_block` on packed sequences for blocks with scaled residuals and attention (Granite's multipliers): the
+    pending branch output and the stream in, those behind the block out. Every residual sum, its scale and the norm behind
+    it are one operator (:func:`~economize_b200.ops.block_norm`)."""
+    from ..ops.reference import rmsnorm
+
+    _check_plain_block(config, scaled=True)
+    eps, m = config.rms_norm_eps, config.residual_multiplier
+    if branch is None:
+        x = rmsnorm(h, layer.attn_norm.to(h.dtype), eps)[0]
+    else:
+        x, h = ops.block_norm(branch, h, layer.attn_norm.to(h.dtype), scale=m, eps=eps)
+    a = _block_attention(layer, x, config, cos, sin, cu_seqlens)
+    x, h = ops.block_norm(a, h, layer.mlp_norm.to(h.dtype), scale=m, eps=eps)
+    return _block_mlp(layer, x), h
 
 
 @OBJECTIVES.register("recovery_ce")

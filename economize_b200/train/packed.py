@@ -18,7 +18,7 @@ import torch
 
 from .. import ops
 from ..errors import ConfigError
-from .objective import OBJECTIVES, RecoveryCE, torch_block
+from .objective import OBJECTIVES, RecoveryCE, packed_block, torch_block
 
 __all__ = ["PackedBatch", "PackedRecoveryCE", "PackedSource", "pack"]
 
@@ -112,7 +112,7 @@ class PackedSource:
 @OBJECTIVES.register("packed_recovery_ce")
 class PackedRecoveryCE(RecoveryCE):
     """Next-token cross-entropy of a pruned target through its recovery adapters over packed documents
-    (:class:`PackedBatch`)."""
+    (:class:`PackedBatch`). Targets with scaled residuals, attention or logits (Granite) are trained too."""
 
     name = "packed_recovery_ce"
 
@@ -134,9 +134,15 @@ class PackedRecoveryCE(RecoveryCE):
         cos, sin = target.rope_tables(longest)
         cos, sin = cos[batch.positions], sin[batch.positions]
         h = target.embed_tokens(batch.tokens[None]).to(dtype)
-        for layer in target.layers:
-            h = torch_block(layer, h, c, cos, sin, cu_seqlens=batch.cu_seqlens)
-        h = rmsnorm(h, target.norm.to(dtype), c.rms_norm_eps)[0][0]
+        if c.residual_multiplier == 1.0 and c.attention_multiplier is None:
+            for layer in target.layers:
+                h = torch_block(layer, h, c, cos, sin, cu_seqlens=batch.cu_seqlens)
+            h = rmsnorm(h, target.norm.to(dtype), c.rms_norm_eps)[0][0]
+        else:
+            branch = None
+            for layer in target.layers:
+                branch, h = packed_block(layer, branch, h, c, cos, sin, batch.cu_seqlens)
+            h = ops.block_norm(branch, h, target.norm.to(dtype), scale=c.residual_multiplier, eps=c.rms_norm_eps)[0][0]
         loss = ops.linear_cross_entropy(h, head.to(dtype), batch.targets, ignore_index=IGNORE,
                                         logit_scale=1.0 / c.logits_scaling)
         return loss, {"loss": float(loss.detach())}
