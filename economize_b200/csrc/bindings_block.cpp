@@ -62,25 +62,41 @@ void check_columns(int64_t K, const char* what) {
                     ecz::kFp4MaxK, " (got ", K, ")");
 }
 
-struct Fp4Buffers {
-  Tensor codes, scales, row_scale;
-  Fp4 at;
+// Rows of activations in one buffer of bytes: scales, codes, row scales, each from a multiple of 256 bytes on.
+struct Fp4Layout {
+  int64_t scales, codes, row_scale, bytes;
 };
 
-Fp4Buffers fp4_buffers(const Tensor& like, int64_t rows, int64_t K, int64_t fmt) {
-  const auto bytes = like.options().dtype(at::kByte);
-  Fp4Buffers b;
-  b.at.rows = rows;
-  b.at.K = K;
-  b.at.fmt = static_cast<int>(fmt);
-  b.at.tiles = ecz::fp4_scale_tiles(b.at.fmt, static_cast<int>(K));
-  b.codes = at::empty({rows, K / 2}, bytes);
-  b.scales = at::empty({(rows + 127) / 128, b.at.tiles, 512}, bytes);
-  b.row_scale = at::empty({fmt == 1 ? rows : 0}, like.options().dtype(at::kFloat));
-  b.at.codes = b.codes.data_ptr<uint8_t>();
-  b.at.scales = b.scales.data_ptr<uint8_t>();
-  b.at.row_scale = b.row_scale.data_ptr<float>();
-  return b;
+Fp4Layout fp4_layout(const Fp4& x) {
+  Fp4Layout l;
+  l.scales = 0;
+  l.codes = (x.rows + 127) / 128 * x.tiles * 512;
+  l.row_scale = l.codes + (x.rows * x.K / 2 + 255) / 256 * 256;
+  l.bytes = l.row_scale + (x.fmt == 1 ? 4 * x.rows : 0);
+  return l;
+}
+
+Fp4 fp4_shape(int64_t rows, int64_t K, int64_t fmt) {
+  Fp4 x;
+  x.rows = rows;
+  x.K = K;
+  x.fmt = static_cast<int>(fmt);
+  x.tiles = ecz::fp4_scale_tiles(x.fmt, static_cast<int>(K));
+  return x;
+}
+
+void fp4_place(Fp4& x, void* data) {
+  const Fp4Layout l = fp4_layout(x);
+  uint8_t* p = static_cast<uint8_t*>(data);
+  x.scales = p;
+  x.codes = p + l.codes;
+  x.row_scale = x.fmt == 1 ? reinterpret_cast<float*>(p + l.row_scale) : nullptr;
+}
+
+Tensor fp4_buffer(Fp4& x, const Tensor& like) {
+  Tensor data = at::empty({fp4_layout(x).bytes}, like.options().dtype(at::kByte));
+  fp4_place(x, data.data_ptr());
+  return data;
 }
 
 // x [M, K] into `to`. pad: scales of the rows up to a multiple of 128 become zeros; early: see launch_fp4_quantize.
@@ -94,8 +110,8 @@ void quantize_into(Tensor x, const Fp4& to, bool pad, bool early) {
   TORCH_CHECK(rc == 0, "fp4_quantize: launch failed");
 }
 
-// Codes [M, K / 2], scales and row scales of x [..., K].
-std::tuple<Tensor, Tensor, Tensor> fp4_quantize(const Tensor& x, int64_t fmt) {
+// x [..., K] in 4 bits (a buffer as in Fp4Layout).
+Tensor fp4_quantize(const Tensor& x, int64_t fmt) {
   CHECK_CUDA(x);
   CHECK_BF16(x);
   check_format(fmt);
@@ -104,10 +120,31 @@ std::tuple<Tensor, Tensor, Tensor> fp4_quantize(const Tensor& x, int64_t fmt) {
   c10::cuda::CUDAGuard guard(x.device());
   const Tensor rows = as_rows(x);
   TORCH_CHECK_VALUE(rows.size(0) <= kMaxRows, "fp4_quantize: too many rows");
-  Fp4Buffers b = fp4_buffers(x, rows.size(0), x.size(-1), fmt);
+  Fp4 to = fp4_shape(rows.size(0), x.size(-1), fmt);
+  Tensor data = fp4_buffer(to, x);
   // the result may become a weight, which products fetch before the kernel in front of them ends: no early start
-  quantize_into(rows, b.at, true, false);
-  return {b.codes, b.scales, b.row_scale};
+  quantize_into(rows, to, true, false);
+  return data;
+}
+
+// Where codes, scales and row scales of such a buffer start, and its size.
+std::tuple<int64_t, int64_t, int64_t, int64_t> fp4_offsets(int64_t rows, int64_t K, int64_t fmt) {
+  check_format(fmt);
+  check_columns(K, "fp4_offsets");
+  const Fp4Layout l = fp4_layout(fp4_shape(rows, K, fmt));
+  return {l.codes, l.scales, l.row_scale, l.bytes};
+}
+
+Fp4 check_buffer(const Tensor& data, int64_t rows, int64_t K, int64_t fmt, const char* what) {
+  check_format(fmt);
+  check_columns(K, what);
+  TORCH_CHECK_VALUE(rows >= 0 && rows <= kMaxRows, what, ": ", rows, " rows");
+  Fp4 x = fp4_shape(rows, K, fmt);
+  TORCH_CHECK_VALUE(data.is_cuda() && data.scalar_type() == at::kByte && data.dim() == 1 && data.is_contiguous() &&
+                        data.size(0) == fp4_layout(x).bytes && reinterpret_cast<uintptr_t>(data.data_ptr()) % 256 == 0,
+                    what, ": not a buffer of ", rows, " x ", K, " 4-bit values");
+  fp4_place(x, data.data_ptr());
+  return x;
 }
 
 // Codes, scales and row scales of one operand belong together and lie on the device of ref.
@@ -144,17 +181,24 @@ Fp4 check_operand(const Tensor& codes, const Tensor& scales, const Tensor& row_s
   return o;
 }
 
-Tensor fp4_dequantize(const Tensor& codes, const Tensor& scales, const Tensor& row_scale, int64_t fmt) {
-  CHECK_CUDA(codes);
-  const Fp4 x = check_operand(codes, scales, row_scale, fmt, codes, "fp4_dequantize");
-  c10::cuda::CUDAGuard guard(codes.device());
-  Tensor out = at::empty({x.rows, x.K}, codes.options().dtype(at::kBFloat16));
+Tensor dequantize(const Fp4& x, const Tensor& like) {
+  c10::cuda::CUDAGuard guard(like.device());
+  Tensor out = at::empty({x.rows, x.K}, like.options().dtype(at::kBFloat16));
   if (x.rows == 0) return out;
   const int rc = ecz::launch_fp4_dequantize(x.codes, x.scales, x.row_scale, x.fmt, out.data_ptr(),
                                             static_cast<int>(x.rows), static_cast<int>(x.K),
-                                            ecz::device_sms(codes.get_device()), at::cuda::getCurrentCUDAStream());
+                                            ecz::device_sms(like.get_device()), at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(rc == 0, "fp4_dequantize: launch failed");
   return out;
+}
+
+Tensor fp4_dequantize(const Tensor& codes, const Tensor& scales, const Tensor& row_scale, int64_t fmt) {
+  CHECK_CUDA(codes);
+  return dequantize(check_operand(codes, scales, row_scale, fmt, codes, "fp4_dequantize"), codes);
+}
+
+Tensor fp4_values(const Tensor& data, int64_t rows, int64_t K, int64_t fmt) {
+  return dequantize(check_buffer(data, rows, K, fmt, "fp4_values"), data);
 }
 
 CUtensorMap codes_map(const Fp4& x, int box_rows) {
@@ -200,13 +244,13 @@ void multiply(const Fp4& x, const Fp4& w, const Tensor& y, const at::Device& dev
   TORCH_CHECK(rc == 0, "fp4 product: launch failed");
 }
 
-Tensor fp4_matmul(const Tensor& x, const Tensor& xs, const Tensor& xr, const Tensor& w, const Tensor& ws, const Tensor& wr,
+// 4-bit activations (a buffer) times a 4-bit weight.
+Tensor fp4_matmul(const Tensor& data, int64_t rows, int64_t K, const Tensor& w, const Tensor& ws, const Tensor& wr,
                   int64_t fmt, int64_t path) {
-  CHECK_CUDA(x);
-  const Fp4 a = check_operand(x, xs, xr, fmt, x, "fp4_matmul: x"), b = check_operand(w, ws, wr, fmt, x, "fp4_matmul: w");
-  c10::cuda::CUDAGuard guard(x.device());
-  Tensor y = at::empty({a.rows, b.rows}, x.options().dtype(at::kBFloat16));
-  multiply(a, b, y, x.device(), path);
+  const Fp4 a = check_buffer(data, rows, K, fmt, "fp4_matmul"), b = check_operand(w, ws, wr, fmt, data, "fp4_matmul: weight");
+  c10::cuda::CUDAGuard guard(data.device());
+  Tensor y = at::empty({a.rows, b.rows}, data.options().dtype(at::kBFloat16));
+  multiply(a, b, y, data.device(), path);
   return y;
 }
 
@@ -219,18 +263,10 @@ Tensor linear_fp4(const Tensor& x, const Tensor& w, const Tensor& ws, const Tens
   c10::cuda::CUDAGuard guard(x.device());
   const bool cast = x.scalar_type() != at::kBFloat16;
   const Tensor rows = as_rows(cast ? x.detach().to(at::kBFloat16) : x.detach());
-  Fp4 a;
-  a.fmt = static_cast<int>(fmt);
-  a.rows = rows.size(0);
-  a.K = b.K;
-  a.tiles = b.tiles;
+  Fp4 a = fp4_shape(rows.size(0), b.K, fmt);
   TORCH_CHECK_VALUE(a.rows <= kMaxRows, "linear_fp4: too many rows");
   // scales of the rows that complete a tile stay as they are: they reach only sums that nothing reads
-  const int64_t scale_bytes = (a.rows + 127) / 128 * a.tiles * 512, code_bytes = (a.rows * a.K / 2 + 255) / 256 * 256;
-  Tensor work = at::empty({scale_bytes + code_bytes + (fmt == 1 ? 4 * a.rows : 0)}, w.options());
-  a.scales = work.data_ptr<uint8_t>();
-  a.codes = a.scales + scale_bytes;
-  if (fmt == 1) a.row_scale = reinterpret_cast<float*>(a.codes + code_bytes);
+  Tensor work = fp4_buffer(a, w);
   Tensor y = at::empty(sizes_with(x, b.rows), rows.options());
   quantize_into(rows, a, false, true);
   multiply(a, b, y, x.device());
@@ -366,31 +402,30 @@ NormCall norm_call(const Tensor& x, const c10::optional<Tensor>& residual, const
   return c;
 }
 
-// Codes, scales and row scales of normed, and the stream.
-std::tuple<Tensor, Tensor, Tensor, Tensor> block_norm_fp4(const Tensor& x, const c10::optional<Tensor>& residual,
-                                                          const Tensor& weight, const c10::optional<Tensor>& post,
-                                                          const c10::optional<Tensor>& gate, double scale, double eps,
-                                                          int64_t fmt) {
+// normed in 4 bits (a buffer), and the stream.
+std::tuple<Tensor, Tensor> block_norm_fp4(const Tensor& x, const c10::optional<Tensor>& residual, const Tensor& weight,
+                                          const c10::optional<Tensor>& post, const c10::optional<Tensor>& gate,
+                                          double scale, double eps, int64_t fmt) {
   check_format(fmt);
   CHECK_CUDA(x);
   TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16, "block_norm in 4 bits takes bfloat16, got ", x.scalar_type());
   const NormCall c = norm_call(x, residual, post, gate);
   check_columns(x.size(-1), "block_norm in 4 bits");
   c10::cuda::CUDAGuard guard(x.device());
-  NormOperands o = norm_operands(c.x, c.residual, weight, c.post, c.gate, scale, eps);
-  Fp4Buffers b = fp4_buffers(x, c.x.size(0), c.x.size(1), fmt);
-  Tensor stream = at::empty(x.sizes(), x.options());
-  if (c.x.size(0) == 0) return {b.codes, b.scales, b.row_scale, stream};
+  const NormOperands o = norm_operands(c.x, c.residual, weight, c.post, c.gate, scale, eps);
+  Fp4 to = fp4_shape(c.x.size(0), c.x.size(1), fmt);
+  Tensor data = fp4_buffer(to, x), stream = at::empty(x.sizes(), x.options());
+  if (to.rows == 0) return {data, stream};
   ecz::BlockNormArgs a = norm_args(o, scale, eps);
   a.stream = stream.data_ptr();
-  a.codes = b.at.codes;
-  a.scales = b.at.scales;
-  a.row_scale = b.at.row_scale;
-  a.tiles = static_cast<int>(b.at.tiles);
+  a.codes = to.codes;
+  a.scales = to.scales;
+  a.row_scale = to.row_scale;
+  a.tiles = static_cast<int>(to.tiles);
   TORCH_CHECK(ecz::launch_block_norm(a, ecz::kNormBf16, true, static_cast<int>(fmt), ecz::device_sms(x.get_device()),
                                      at::cuda::getCurrentCUDAStream()) == 0,
               "block_norm: launch failed");
-  return {b.codes, b.scales, b.row_scale, stream};
+  return {data, stream};
 }
 
 using torch::autograd::AutogradContext;
@@ -543,13 +578,17 @@ namespace ecz {
 
 void bind_block(pybind11::module_& m) {
   namespace py = pybind11;
-  m.def("fp4_quantize", &fp4_quantize, "bf16 rows as 4-bit codes with scales (fmt 1 nvfp4, 2 mxfp4)", py::arg("x"),
+  m.def("fp4_quantize", &fp4_quantize, "bf16 rows in 4 bits, one buffer (fmt 1 nvfp4, 2 mxfp4)", py::arg("x"),
         py::arg("fmt"));
-  m.def("fp4_dequantize", &fp4_dequantize, "the bf16 values of 4-bit codes", py::arg("codes"), py::arg("scales"),
+  m.def("fp4_offsets", &fp4_offsets, "offsets of codes, scales and row scales in such a buffer, and its bytes",
+        py::arg("rows"), py::arg("K"), py::arg("fmt"));
+  m.def("fp4_values", &fp4_values, "the bf16 values of such a buffer", py::arg("data"), py::arg("rows"), py::arg("K"),
+        py::arg("fmt"));
+  m.def("fp4_dequantize", &fp4_dequantize, "the bf16 values of a 4-bit weight", py::arg("codes"), py::arg("scales"),
         py::arg("row_scale"), py::arg("fmt"));
-  m.def("fp4_matmul", &fp4_matmul, "product of two 4-bit operands (tcgen05 block-scaled MMA)", py::arg("x"),
-        py::arg("x_scales"), py::arg("x_row_scale"), py::arg("w"), py::arg("w_scales"), py::arg("w_row_scale"),
-        py::arg("fmt"), py::arg("path") = 0);
+  m.def("fp4_matmul", &fp4_matmul, "4-bit activations times a 4-bit weight (tcgen05 block-scaled MMA)", py::arg("data"),
+        py::arg("rows"), py::arg("K"), py::arg("w"), py::arg("w_scales"), py::arg("w_row_scale"), py::arg("fmt"),
+        py::arg("path") = 0);
   m.def("linear_fp4", &linear_fp4, "bf16 activations quantised and multiplied with a 4-bit weight", py::arg("x"),
         py::arg("w"), py::arg("w_scales"), py::arg("w_row_scale"), py::arg("fmt"));
   m.def("block_norm", &block_norm, "norm after a block, gate, residual scale and sum, norm before the next (autograd)",

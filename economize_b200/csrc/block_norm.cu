@@ -212,6 +212,10 @@ struct Team {
   }
 };
 
+// Whether the forward kernel's weights lie in shared memory (Lanes).
+template <int VEC, int FMT, bool POST>
+constexpr bool kForwardShared = VEC > 1 && (POST || FMT != 0);
+
 // FMT 0: normed as T; else as 4-bit codes (bf16). POST: there may be a norm behind the block. Persistent over
 // rows: team t of all takes rows t, t + teams, ...
 template <typename T, int VEC, int NV, int FMT, bool POST, int THREADS, int BLOCKS, int DEPTH>
@@ -241,7 +245,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   int row = blockIdx.x * per_block + team.index;
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d) start(d, row + d * teams);
-  Lanes<T, VEC, NV, VEC != 1 && POST> w, p;
+  Lanes<T, VEC, NV, kForwardShared<VEC, FMT, POST>> w, p;
   uint8_t* behind = ring + Rows<T, VEC, NV, 2, DEPTH>::bytes(blockDim.x);
   w.fetch(behind, static_cast<const T*>(a.weight), team.first, team.step, hidden);
   if constexpr (POST)
@@ -560,21 +564,21 @@ int go_forward(const BlockNormArgs& a, const Grid& g, int sms, cudaStream_t stre
   const int rows = FMT == 0 ? a.rows : (a.rows + 127) / 128 * 128;
   const int resident = THREADS <= 256 ? BLOCKS : 1024 / g.threads;
   using R = Rows<T, VEC, NV, 2, DEPTH>;
-  using L = Lanes<T, VEC, NV, VEC != 1 && POST>;
+  using L = Lanes<T, VEC, NV, kForwardShared<VEC, FMT, POST>>;
   static_assert(R::bytes(THREADS) + 2 * L::bytes(THREADS) <= kMostSmem, "227 KB of shared memory");
   const int smem = R::bytes(g.threads) + 2 * L::bytes(g.threads);
   return go(block_norm_kernel<T, VEC, NV, FMT, POST, THREADS, BLOCKS, DEPTH>, smem,
             std::min((rows + g.teams - 1) / g.teams, sms * resident), g, a, stream);
 }
 
-// Blocks of 256 threads: three to an SM, two rows ahead (four with 64 registers a thread, or three rows ahead, took as
-// long or longer; so did one vector a lane).
+// Blocks of 256 threads, two rows ahead: three to an SM, or four where the norm behind the block or the 4-bit result make
+// the chain from a row's arrival to its end longer.
 template <typename T, int FMT, bool POST>
 int run_forward(const BlockNormArgs& a, int sms, cudaStream_t stream) {
   constexpr int V = vec_of<T>();
   // 4-bit results: lanes cover the scales' padding too
   const Grid g = grid_of<V>(FMT == 0 ? a.hidden : (a.hidden + fp4::kBlockK - 1) / fp4::kBlockK * fp4::kBlockK, 2);
-  if (g.threads <= 256) return go_forward<T, V, 2, FMT, POST, 256, 3, 2>(a, g, sms, stream);
+  if (g.threads <= 256) return go_forward<T, V, 2, FMT, POST, 256, POST || FMT != 0 ? 4 : 3, 2>(a, g, sms, stream);
   if (g.nv <= 2) return go_forward<T, V, 2, FMT, POST, 1024, 1, 2>(a, g, sms, stream);
   if constexpr (sizeof(T) == 4) return go_forward<T, V, 4, FMT, POST, 1024, 1, 0>(a, g, sms, stream);
   return -1;

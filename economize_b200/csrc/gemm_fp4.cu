@@ -129,6 +129,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, BN>::kOcc)
   const int n0 = blockIdx.x * kBM, m0 = blockIdx.y * BN, split = blockIdx.z, splits = gridDim.z;
   const int kb0 = split * args.per_split;
   const int nkb = max(0, min(args.per_split, args.kblocks - kb0));
+  const size_t wide = static_cast<size_t>(args.kblocks) * C::kScaleBytes;  // scales of 128 rows
+  const uint8_t* ws = args.w_scales + blockIdx.x * wide;
+  auto weights = [&](int kb) {
+    const int s = kb % S, k = kb0 + kb;
+    mbar_arrive_expect_tx(&full[s], C::kStageBytes);
+    tma_load_2d(a_tiles + s * kABytes, &tm_w, &full[s], k * kRowBytes, n0);
+    bulk_load(sa_tiles + s * C::kScaleBytes, ws + static_cast<size_t>(k) * C::kScaleBytes, C::kScaleBytes, &full[s]);
+  };
+  const int pre = min(nkb, S);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
@@ -137,34 +146,24 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, BN>::kOcc)
     mbar_init(acc_full, 1);
     *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tm_w);
+    // the weights do not come from the previous kernel: what fits is fetched before it ends, and before the block is ready
+    for (int kb = 0; kb < pre; ++kb) weights(kb);
     tma_prefetch_desc(&tm_x);
   }
   __syncwarp();
-  if (warp == 0) tmem_alloc(tmem_slot, C::kTmemCols);
+  if (warp == 1) tmem_alloc(tmem_slot, C::kTmemCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0 && lane == 0) {
-    const size_t wide = static_cast<size_t>(args.kblocks) * C::kScaleBytes;  // scales of 128 rows
-    const uint8_t* ws = args.w_scales + (n0 / kBM) * wide;
     const uint8_t* xs = args.x_scales + (m0 / 128) * wide;
-    auto weights = [&](int kb) {
-      const int s = kb % S, k = kb0 + kb;
-      mbar_arrive_expect_tx(&full[s], C::kStageBytes);
-      tma_load_2d(a_tiles + s * kABytes, &tm_w, &full[s], k * kRowBytes, n0);
-      bulk_load(sa_tiles + s * C::kScaleBytes, ws + static_cast<size_t>(k) * C::kScaleBytes, C::kScaleBytes, &full[s]);
-    };
     auto activations = [&](int kb) {
       const int s = kb % S, k = kb0 + kb;
       tma_load_2d(b_tiles + s * C::kBBytes, &tm_x, &full[s], k * kRowBytes, m0);
       bulk_load(sb_tiles + s * C::kScaleBytes, xs + static_cast<size_t>(k) * C::kScaleBytes, C::kScaleBytes, &full[s]);
     };
-    // the weights do not come from the previous kernel: what fits is fetched before it ends
-    const int pre = min(nkb, S);
-    for (int kb = 0; kb < pre; ++kb) weights(kb);
     pdl_wait();
     for (int kb = 0; kb < pre; ++kb) activations(kb);
     for (int kb = pre; kb < nkb; ++kb) {
@@ -277,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, BN>::kOcc)
   if (splits > 1) cluster_sync();  // the others have read this CTA's sums
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) tmem_dealloc(tmem, C::kTmemCols);
+  if (warp == 1) tmem_dealloc(tmem, C::kTmemCols);
 }
 
 template <int FMT, int BN>

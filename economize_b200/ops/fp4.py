@@ -113,52 +113,92 @@ def _reference_dequantize(codes: torch.Tensor, scales: torch.Tensor, row: torch.
 
 
 class FP4Tensor:
-    """Rows of a tensor ``[..., K]`` in 4 bits.
+    """Rows of a tensor ``[..., K]`` in 4 bits, in one buffer of bytes.
 
     Attributes:
-        codes: uint8 ``[M, K / 2]``, column ``2b`` in the low nibble of byte ``b``.
-        scales: Scale bytes (e4m3 or E8M0) in tiles ``[M / 128, tiles, 512]`` as the tensor cores read them.
-        row_scale: fp32 powers of two ``[M]`` (nvfp4), else empty.
+        data: The buffer (uint8): tiled scales, codes and row scales (:meth:`parts`), each from a multiple of 256 bytes on.
         fmt: ``"nvfp4"`` or ``"mxfp4"``.
         shape: Of the tensor the codes stand for.
     """
 
-    __slots__ = ("codes", "scales", "row_scale", "fmt", "shape")
+    __slots__ = ("data", "fmt", "shape")
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, row_scale: torch.Tensor, fmt: str,
-                 shape: torch.Size | None = None) -> None:
-        _check_format(fmt)
-        self.codes, self.scales, self.row_scale, self.fmt = codes, scales, row_scale, fmt
-        self.shape = shape if shape is not None else torch.Size((codes.shape[0], 2 * codes.shape[1]))
+    def __init__(self, data: torch.Tensor, fmt: str, shape: torch.Size) -> None:
+        self.data, self.fmt, self.shape = data, fmt, shape
 
     @property
     def is_cuda(self) -> bool:
-        return self.codes.is_cuda
+        return self.data.is_cuda
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self.data.device
 
     @property
     def dtype(self) -> torch.dtype:
         return torch.bfloat16  # of the values, which bf16 holds exactly
 
+    @property
+    def rows(self) -> int:
+        n = 1
+        for d in self.shape[:-1]:
+            n *= d
+        return n
+
+    @property
+    def codes(self) -> torch.Tensor:
+        """uint8 ``[M, K / 2]``, column ``2b`` in the low nibble of byte ``b``."""
+        return self.parts()[0]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        """Scale bytes (e4m3 or E8M0) in tiles ``[M / 128, tiles, 512]`` as the tensor cores read them."""
+        return self.parts()[1]
+
+    @property
+    def row_scale(self) -> torch.Tensor:
+        """fp32 powers of two ``[M]`` (nvfp4), else empty."""
+        return self.parts()[2]
+
+    def parts(self) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Views of the buffer: codes, scales, row scales."""
+        rows, columns = self.rows, self.shape[-1]
+        high = (rows + _ROWS - 1) // _ROWS
+        tiles = _tiles(columns, self.fmt)
+        at = high * tiles * 4 * _ROWS
+        end = at + rows * columns // 2
+        row = _round_up(end)
+        return (self.data[at:end].view(rows, columns // 2), self.data[:at].view(high, tiles, 4 * _ROWS),
+                self.data[row:row + (4 * rows if self.fmt == "nvfp4" else 0)].view(torch.float32))
+
     def nbytes(self) -> int:
-        return self.codes.numel() + self.scales.numel() + 4 * self.row_scale.numel()
+        return self.data.numel()
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values the codes stand for, exact in bf16 and fp32 (those beyond a type's range, which only rows near
         bf16's largest values have, become infinite)."""
-        if self.codes.is_cuda:
-            out = require().fp4_dequantize(self.codes, self.scales, self.row_scale, FORMATS[self.fmt])
+        shape = self.shape
+        if self.data.is_cuda:
+            rows = shape[0] if len(shape) == 2 else self.rows
+            out = require().fp4_values(self.data, rows, shape[-1], FORMATS[self.fmt])
         else:
-            out = _reference_dequantize(self.codes, self.scales, self.row_scale, self.fmt)
+            out = _reference_dequantize(*self.parts(), self.fmt)
         if out.dtype != dtype:
             out = out.to(dtype)
-        return out if len(self.shape) == 2 else out.reshape(self.shape)
+        return out if len(shape) == 2 else out.reshape(shape)
 
     def __repr__(self) -> str:
         return f"FP4Tensor({tuple(self.shape)}, fmt={self.fmt!r}, device={self.device})"
+
+
+def _round_up(n: int) -> int:
+    return (n + 255) // 256 * 256
+
+
+def _buffer(codes: torch.Tensor, scales: torch.Tensor, row_scale: torch.Tensor) -> torch.Tensor:
+    """The parts of an :class:`FP4Tensor` in one buffer."""
+    pad = codes.new_zeros(_round_up(codes.numel()) - codes.numel())
+    return torch.cat([scales.reshape(-1), codes.reshape(-1), pad, row_scale.contiguous().view(torch.uint8)])
 
 
 def quantize(x: torch.Tensor, fmt: str = "nvfp4") -> FP4Tensor:
@@ -169,10 +209,10 @@ def quantize(x: torch.Tensor, fmt: str = "nvfp4") -> FP4Tensor:
     if len(shape) < 1 or shape[-1] < 32 or shape[-1] % 32 or shape[-1] > 65536:
         raise ConfigError(f"4-bit rows need a multiple of 32 columns, up to 65536, got {tuple(shape)}")
     if x.is_cuda:
-        return FP4Tensor(*require().fp4_quantize(x, FORMATS[fmt]), fmt, shape)
+        return FP4Tensor(require().fp4_quantize(x, FORMATS[fmt]), fmt, shape)
     if not x.is_floating_point():
         raise ConfigError(f"4-bit rows are quantised from floating point, got {x.dtype}")
-    return FP4Tensor(*_reference_quantize(x.detach().reshape(-1, shape[-1]), fmt), fmt, shape)
+    return FP4Tensor(_buffer(*_reference_quantize(x.detach().reshape(-1, shape[-1]), fmt)), fmt, shape)
 
 
 class FP4Weight(nn.Module):
@@ -209,7 +249,7 @@ class FP4Weight(nn.Module):
         if w.dim() != 2:
             raise ConfigError(f"a 4-bit weight is made from [N, K], got {tuple(w.shape)}")
         q = quantize(w.detach().to(torch.bfloat16) if w.is_cuda else w.detach(), fmt)
-        return cls(q.codes, q.scales, q.row_scale, fmt, w.dtype)
+        return cls(*q.parts(), fmt, w.dtype)
 
     @property
     def shape(self) -> torch.Size:
@@ -227,7 +267,11 @@ class FP4Weight(nn.Module):
         return self.codes.numel() + self.scales.numel() + 4 * self.row_scale.numel()
 
     def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
-        return FP4Tensor(self.codes, self.scales, self.row_scale, self.fmt).dequantize(dtype or self.compute_dtype)
+        if self.codes.is_cuda:
+            out = require().fp4_dequantize(self.codes, self.scales, self.row_scale, FORMATS[self.fmt])
+        else:
+            out = _reference_dequantize(self.codes, self.scales, self.row_scale, self.fmt)
+        return out.to(dtype or self.compute_dtype)
 
     def linear(self, x: torch.Tensor | FP4Tensor) -> torch.Tensor:
         """``x @ w.T`` with both operands in 4 bits: fp32 sums, rounded to bf16 on CUDA, in ``x``'s type."""
@@ -238,8 +282,9 @@ class FP4Weight(nn.Module):
         if isinstance(x, FP4Tensor):
             if x.fmt != self.fmt:
                 raise ConfigError(f"{x.fmt} activations do not multiply with an {self.fmt} weight")
-            if x.codes.is_cuda:
-                y = require().fp4_matmul(x.codes, x.scales, x.row_scale, codes, scales, row_scale, FORMATS[self.fmt])
+            if x.data.is_cuda:
+                rows = x.shape[0] if len(x.shape) == 2 else x.rows
+                y = require().fp4_matmul(x.data, rows, self.in_features, codes, scales, row_scale, FORMATS[self.fmt])
                 return y if len(x.shape) == 2 else y.reshape(*x.shape[:-1], self.out_features)
         elif x.is_cuda:
             return require().linear_fp4(x, codes, scales, row_scale, FORMATS[self.fmt])

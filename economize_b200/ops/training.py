@@ -127,8 +127,8 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Ten
         if quantize is None:
             return require().block_norm(x, residual, weight, post_weight, gate, scale, eps)
         _check_format(quantize)
-        *parts, stream = require().block_norm_fp4(x, residual, weight, post_weight, gate, scale, eps, FORMATS[quantize])
-        return FP4Tensor(*parts, quantize, x.shape), stream
+        data, stream = require().block_norm_fp4(x, residual, weight, post_weight, gate, scale, eps, FORMATS[quantize])
+        return FP4Tensor(data, quantize, x.shape), stream
     given = [t for t in (x, residual, weight, post_weight, gate) if t is not None]
     if x.dim() < 1 or weight.dim() != 1 or x.shape[-1] != weight.shape[0]:
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")

@@ -156,7 +156,7 @@ def test_product_paths(cuda, fmt, path, rows, cols, out):
     x = _normal(cuda, rows, cols, seed=rows, spread=0.7)
     w = _normal(cuda, out, cols, seed=out, spread=0.3) * 0.05
     a, b = ops.fp4_quantize(x, fmt), FP4Weight.from_weight(w, fmt)
-    y = ops.require().fp4_matmul(a.codes, a.scales, a.row_scale, b.codes, b.scales, b.row_scale, fp4.FORMATS[fmt], path)
+    y = ops.require().fp4_matmul(a.data, rows, cols, b.codes, b.scales, b.row_scale, fp4.FORMATS[fmt], path)
     _check_product(x, w, fmt, y)
 
 
@@ -232,9 +232,10 @@ def test_refusals(cuda):
     with pytest.raises(ConfigError):
         ops.linear(x.cpu(), w)
     C, q = ops.require(), ops.fp4_quantize(x)
-    good = (q.codes, q.scales, q.row_scale, w.codes, w.scales, w.row_scale, 1)
-    for i, bad in ((0, q.codes[:, :16]), (1, q.scales[:, :2]), (2, q.row_scale[:2]), (3, w.codes.cpu()),
-                   (4, w.scales.float()), (5, w.row_scale.double()), (6, 3), (2, q.row_scale.cpu()), (0, q.codes.t())):
+    good = (q.data, 4, 64, w.codes, w.scales, w.row_scale, 1)
+    for i, bad in ((0, q.data[:-16]), (0, q.data.cpu()), (0, q.data.float()), (1, 5), (1, -1), (2, 96), (2, 40),
+                   (3, w.codes.cpu()), (3, w.codes[:, :16]), (4, w.scales.float()), (4, w.scales[:, :2]),
+                   (5, w.row_scale.double()), (5, w.row_scale[:2]), (5, w.row_scale.cpu()), (6, 3), (6, 2)):
         args = list(good)
         args[i] = bad
         with pytest.raises((RuntimeError, ValueError)):
