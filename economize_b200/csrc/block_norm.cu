@@ -25,6 +25,11 @@ namespace ecz {
 
 namespace {
 
+using packed::fma2;
+using packed::mul2;
+using packed::pair_of;
+using packed::unpair;
+
 constexpr int kMaxWarps = 32;
 constexpr int kMostSmem = 227 * 1024 - 2 * kMaxWarps * 8;  // beside the teams' scratch
 
@@ -39,11 +44,19 @@ template <>
 struct Cast<bf16> {
   static __device__ __forceinline__ float to(bf16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ bf16 from(float v) { return __float2bfloat16(v); }
+  static __device__ __forceinline__ uint32_t from(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
 };
 template <>
 struct Cast<__half> {
   static __device__ __forceinline__ float to(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half from(float v) { return __float2half(v); }
+  static __device__ __forceinline__ uint32_t from(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
 };
 
 // A lane's VEC consecutive elements, from element `at` of a row of `hidden` on: 16 bytes, or one element. (With 32 bytes a
@@ -59,6 +72,23 @@ struct Pack {
   __device__ __forceinline__ Pack() {}
   __device__ __forceinline__ float get(int i) const { return Cast<T>::to(v[i]); }
   __device__ __forceinline__ void set(int i, float f) { v[i] = Cast<T>::from(f); }
+  // elements 2 k and 2 k + 1 in one 64-bit register (a zero behind a single element)
+  __device__ __forceinline__ uint64_t get2(int k) const {
+    if constexpr (VEC == 1) return pair_of(get(0), 0.f);
+    else return pair_of(get(2 * k), get(2 * k + 1));
+  }
+  __device__ __forceinline__ void set2(int k, uint64_t pair) {
+    float lo, hi;
+    unpair(pair, lo, hi);
+    if constexpr (VEC == 1) {
+      set(0, lo);
+    } else if constexpr (sizeof(T) == 4) {
+      set(2 * k, lo);
+      set(2 * k + 1, hi);
+    } else {
+      words[k] = Cast<T>::from(lo, hi);
+    }
+  }
   // row[at ..], zeros where the row is null or has ended
   __device__ __forceinline__ void fetch(const T* row, int at, int hidden) {
 #pragma unroll
@@ -76,11 +106,18 @@ struct Pack {
   }
 };
 
+// Threads of a block: 256, or (longer rows) fewer than the 1024 that the kernel allows.
+template <int THREADS>
+__device__ __forceinline__ int block_threads() {
+  if constexpr (THREADS == 256) return 256;
+  else return static_cast<int>(blockDim.x);
+}
+
 // Rows on their way: every thread copies the vectors that it will work on itself into shared memory (cp.async), DEPTH rows
 // ahead, so nothing is shared, no barrier is needed and no register is held. Operand k, vector i of a thread in slot s
 // lies in a plane of one entry (16 bytes, or a single fp32 element) per thread. DEPTH 0 (long rows, and single elements of
 // 16 bits, which cp.async does not copy): operands are read when they are needed.
-template <typename T, int VEC, int NV, int OPS, int DEPTH>
+template <typename T, int VEC, int NV, int OPS, int DEPTH, int THREADS>
 struct Rows {
   using P = Pack<T, VEC>;
   static constexpr bool kAhead = DEPTH > 0;
@@ -93,7 +130,7 @@ struct Rows {
   const T* ptr[OPS];  // rows being worked on (DEPTH 0)
   __device__ __forceinline__ Rows(void* smem) : base(smem_u32(smem) + threadIdx.x * kEntry) {}
   __device__ __forceinline__ uint32_t plane(int s, int op, int i) const {
-    return base + static_cast<uint32_t>((s * kSlotPlanes + op * NV + i) * blockDim.x * kEntry);
+    return base + static_cast<uint32_t>((s * kSlotPlanes + op * NV + i) * block_threads<THREADS>() * kEntry);
   }
   // start the copy of operand op's row (zeros for null) into slot s; first, step: this lane's vectors
   __device__ __forceinline__ void start(int s, int op, const T* row, int first, int step, int hidden) {
@@ -102,14 +139,11 @@ struct Rows {
       for (int i = 0; i < NV; ++i) {
         const int at = (first + i * step) * VEC;
         const uint32_t to = plane(s, op, i);
-        const bool on = row != nullptr && at < hidden;
-        if constexpr (kEntry == 16) {
-          if (on) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(row + at) : "memory");
-          else asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory");
-        } else {
-          if (on) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(row + at) : "memory");
-          else asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(0) : "memory");
-        }
+        const int bytes = row != nullptr && at < hidden ? kEntry : 0;  // the rest of the entry becomes zero
+        if constexpr (kEntry == 16)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(row + at), "r"(bytes) : "memory");
+        else
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(row + at), "r"(bytes) : "memory");
       }
     } else {
       ptr[op] = row;
@@ -139,7 +173,7 @@ struct Rows {
 
 // This lane's part of a weight: in registers, or (SHARED) in planes of shared memory like Rows', where two weights or the
 // sums over tokens would spill.
-template <typename T, int VEC, int NV, bool SHARED>
+template <typename T, int VEC, int NV, bool SHARED, int THREADS>
 struct Lanes {
   using P = Pack<T, VEC>;
   static constexpr int kEntry = VEC * static_cast<int>(sizeof(T));
@@ -152,18 +186,19 @@ struct Lanes {
     for (int i = 0; i < NV; ++i) {
       P v;
       v.fetch(row, (first + i * step) * VEC, hidden);
-      if constexpr (SHARED) plane[i * blockDim.x] = v;
+      if constexpr (SHARED) plane[i * block_threads<THREADS>()] = v;
       else held[i] = v;
     }
   }
   __device__ __forceinline__ P get(int i) const {
-    if constexpr (SHARED) return plane[i * blockDim.x];
+    if constexpr (SHARED) return plane[i * block_threads<THREADS>()];
     else return held[i];
   }
 };
 
-// A team's place: `warps` consecutive warps of the block, and its reductions. Two buffers in turn: a warp writes one again
+// A team's place: `warps` (at most MOST) consecutive warps of the block, and its reductions. Two buffers in turn: a warp writes one again
 // only behind a barrier that all warps reach after reading it.
+template <int MOST>
 struct Team {
   int warps, index, first, step, lane, warp;
   float2* scratch;  // [2][kMaxWarps]
@@ -179,36 +214,39 @@ struct Team {
   __device__ __forceinline__ void barrier() const {
     asm volatile("bar.sync %0, %1;" ::"r"(index + 1), "r"(warps * 32) : "memory");
   }
-  // this warp's part to the others, theirs combined in the order of the warps' binary tree
-  template <class V, class Op>
-  __device__ __forceinline__ V combine(V v, V neutral, Op op) {
+  // every lane: the part of warp lane % MOST of the team, or `neutral`
+  template <class V>
+  __device__ __forceinline__ V parts(V v, V neutral) {
     V* buf = reinterpret_cast<V*>(scratch + turn * kMaxWarps + index * warps);
     turn ^= 1;
     if (lane == 0) buf[warp] = v;
     barrier();
-    v = lane < warps ? buf[lane] : neutral;
-    for (int o = 1; o < warps; o <<= 1) v = op(v, o);
+    const int of = lane % MOST;
+    return of < warps ? buf[of] : neutral;
+  }
+  __device__ __forceinline__ float sum(float v) {
+    v = warp_sum(v);
+    if (warps == 1) return v;
+    v = parts(v, 0.f);
+#pragma unroll
+    for (int o = 1; o < MOST; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
   }
   __device__ __forceinline__ float2 sum(float2 v) {
     v.x = warp_sum(v.x);
     v.y = warp_sum(v.y);
     if (warps == 1) return v;
-    v = combine(v, make_float2(0.f, 0.f), [](float2 a, int o) {
-      return make_float2(a.x + __shfl_xor_sync(0xffffffffu, a.x, o), a.y + __shfl_xor_sync(0xffffffffu, a.y, o));
-    });
-    return make_float2(__shfl_sync(0xffffffffu, v.x, 0), __shfl_sync(0xffffffffu, v.y, 0));
-  }
-  __device__ __forceinline__ float sum(float v) {
-    v = warp_sum(v);
-    if (warps == 1) return v;
-    v = combine(v, 0.f, [](float a, int o) { return a + __shfl_xor_sync(0xffffffffu, a, o); });
-    return __shfl_sync(0xffffffffu, v, 0);
+    v = parts(v, make_float2(0.f, 0.f));
+#pragma unroll
+    for (int o = 1; o < MOST; o <<= 1) {
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+    return v;
   }
   __device__ __forceinline__ uint32_t max(uint32_t v) {
     v = __reduce_max_sync(0xffffffffu, v);
-    if (warps == 1) return v;
-    return __reduce_max_sync(0xffffffffu, combine(v, 0u, [](uint32_t a, int) { return a; }));
+    return warps == 1 ? v : __reduce_max_sync(0xffffffffu, parts(v, 0u));
   }
 };
 
@@ -224,17 +262,23 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   __shared__ float2 scratch[2 * kMaxWarps];
   extern __shared__ uint8_t ring[];
   pdl_trigger();
-  Team team(warps, scratch);
-  Rows<T, VEC, NV, 2, DEPTH> rows(ring);
+  Team<THREADS == 256 ? 8 : kMaxWarps> team(warps, scratch);
+  Rows<T, VEC, NV, 2, DEPTH, THREADS> rows(ring);
   const int per_block = blockDim.x / (32 * warps);
   const int teams = gridDim.x * per_block;
-  const bool post = POST && a.post != nullptr;
+  const bool post = POST && (VEC > 1 || a.post != nullptr);
   const int hidden = a.hidden;
   const float mean = 1.f / static_cast<float>(hidden);
   const int last = FMT == 0 ? a.rows : (a.rows + 127) / 128 * 128;
   const T* xp = static_cast<const T*>(a.x);
   const T* rp = static_cast<const T*>(a.residual);
   const T* gp = static_cast<const T*>(a.gate);
+  constexpr int kPairs = (VEC + 1) / 2;
+  auto total = [](uint64_t pair) {
+    float lo, hi;
+    unpair(pair, lo, hi);
+    return VEC == 1 ? lo : lo + hi;
+  };
   auto start = [&](int slot, int row) {
     const bool on = row < a.rows;
     rows.start(slot, 0, on ? xp + row * a.x_stride : nullptr, team.first, team.step, hidden);
@@ -245,8 +289,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   int row = blockIdx.x * per_block + team.index;
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d) start(d, row + d * teams);
-  Lanes<T, VEC, NV, kForwardShared<VEC, FMT, POST>> w, p;
-  uint8_t* behind = ring + Rows<T, VEC, NV, 2, DEPTH>::bytes(blockDim.x);
+  Lanes<T, VEC, NV, kForwardShared<VEC, FMT, POST>, THREADS> w, p;
+  uint8_t* behind = ring + Rows<T, VEC, NV, 2, DEPTH, THREADS>::bytes(blockDim.x);
   w.fetch(behind, static_cast<const T*>(a.weight), team.first, team.step, hidden);
   if constexpr (POST)
     p.fetch(behind + w.bytes(blockDim.x), static_cast<const T*>(a.post), team.first, team.step, hidden);
@@ -256,39 +300,50 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
     if (a.gate_mode == kGateToken && real) factor *= Cast<T>::to(gp[row * a.gate_stride]);
     if constexpr (DEPTH == 0) start(0, row);
     rows.wait();
-    float s[NV][VEC];
+    uint64_t s[NV][kPairs];
     float ix = 1.f;
     if (post) {
-      float q = 0.f;
+      uint64_t q = 0;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         Pack<T, VEC> x;
         rows.get(x, 0, i, (team.first + i * team.step) * VEC, hidden);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          s[i][j] = x.get(j);
-          q = fmaf(s[i][j], s[i][j], q);
+        for (int k = 0; k < kPairs; ++k) {
+          s[i][k] = x.get2(k);
+          q = fma2(s[i][k], s[i][k], q);
         }
       }
-      ix = rsqrtf(team.sum(q) * mean + a.eps);
+      ix = rsqrtf(team.sum(total(q)) * mean + a.eps);
       if (a.inv_x != nullptr && team.first == 0 && real) a.inv_x[row] = ix;
     }
-    float q = 0.f;
+    const uint64_t ix2 = pair_of(ix, ix), factor2 = pair_of(factor, factor);
+    uint64_t q = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int at = (team.first + i * team.step) * VEC;
-      Pack<T, VEC> x, r, g;
-      if (!post) rows.get(x, 0, i, at, hidden);
-      rows.get(r, 1, i, at, hidden);
-      if (a.gate_mode == kGateFull) g.fetch(real ? gp + row * a.gate_stride : nullptr, at, hidden);
-      Pack<T, VEC> pi;
-      if constexpr (POST) pi = p.get(i);
+      Pack<T, VEC> r;
+      if (post) {
+        const Pack<T, VEC> pi = p.get(i);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float b = post ? s[i][j] * (ix * pi.get(j)) : x.get(j);
-        if (a.gate_mode == kGateFull) b *= g.get(j);
-        s[i][j] = fmaf(factor, b, r.get(j));
-        q = fmaf(s[i][j], s[i][j], q);
+        for (int k = 0; k < kPairs; ++k) s[i][k] = mul2(s[i][k], mul2(ix2, pi.get2(k)));
+      } else {
+        Pack<T, VEC> x;
+        rows.get(x, 0, i, at, hidden);
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) s[i][k] = x.get2(k);
+      }
+      if (a.gate_mode == kGateFull) {
+        Pack<T, VEC> g;
+        g.fetch(real ? gp + row * a.gate_stride : nullptr, at, hidden);
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) s[i][k] = mul2(s[i][k], g.get2(k));
+      }
+      rows.get(r, 1, i, at, hidden);
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) {
+        s[i][k] = fma2(factor2, s[i][k], r.get2(k));
+        q = fma2(s[i][k], s[i][k], q);
       }
     }
     if constexpr (DEPTH > 0) {  // this row's slot is read: the row DEPTH further
@@ -299,18 +354,19 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
     for (int i = 0; i < NV; ++i) {
       Pack<T, VEC> out;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) out.set(j, s[i][j]);
+      for (int k = 0; k < kPairs; ++k) out.set2(k, s[i][k]);
       if (real)
         out.store(static_cast<T*>(a.stream) + static_cast<size_t>(row) * hidden, (team.first + i * team.step) * VEC, hidden);
     }
-    const float is = rsqrtf(team.sum(q) * mean + a.eps);
+    const float is = rsqrtf(team.sum(total(q)) * mean + a.eps);
+    const uint64_t is2 = pair_of(is, is);
     if (a.inv_s != nullptr && team.first == 0 && real) a.inv_s[row] = is;
     Pack<T, VEC> out[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const Pack<T, VEC> wi = w.get(i);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) out[i].set(j, real ? s[i][j] * is * wi.get(j) : 0.f);
+      for (int k = 0; k < kPairs; ++k) out[i].set2(k, mul2(mul2(s[i][k], is2), wi.get2(k)));
       if (FMT == 0)
         out[i].store(static_cast<T*>(a.normed) + static_cast<size_t>(row) * hidden, (team.first + i * team.step) * VEC,
                      hidden);
@@ -352,8 +408,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   __shared__ float2 scratch[2 * kMaxWarps];
   extern __shared__ uint8_t ring[];
   pdl_trigger();
-  Team team(warps, scratch);
-  Rows<T, VEC, NV, WHOLE ? 3 : 4, DEPTH> rows(ring);
+  Team<THREADS == 256 ? 8 : kMaxWarps> team(warps, scratch);
+  Rows<T, VEC, NV, WHOLE ? 3 : 4, DEPTH, THREADS> rows(ring);
   const int per_block = blockDim.x / (32 * warps);
   const int teams = gridDim.x * per_block, self = blockIdx.x * per_block + team.index;
   const bool post = POST && a.post != nullptr;
@@ -378,8 +434,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d) start(d, self + d * teams);
   constexpr bool kShared = SharedWeights<VEC, WHOLE>::value;
-  Lanes<T, VEC, NV, kShared> w, p;
-  uint8_t* behind = ring + Rows<T, VEC, NV, WHOLE ? 3 : 4, DEPTH>::bytes(blockDim.x);
+  Lanes<T, VEC, NV, kShared, THREADS> w, p;
+  uint8_t* behind = ring + Rows<T, VEC, NV, WHOLE ? 3 : 4, DEPTH, THREADS>::bytes(blockDim.x);
   w.fetch(behind, static_cast<const T*>(a.weight), team.first, team.step, hidden);
   if constexpr (POST)
     p.fetch(behind + w.bytes(blockDim.x), static_cast<const T*>(a.post), team.first, team.step, hidden);
@@ -563,8 +619,8 @@ template <typename T, int VEC, int NV, int FMT, bool POST, int THREADS, int BLOC
 int go_forward(const BlockNormArgs& a, const Grid& g, int sms, cudaStream_t stream) {
   const int rows = FMT == 0 ? a.rows : (a.rows + 127) / 128 * 128;
   const int resident = THREADS <= 256 ? BLOCKS : 1024 / g.threads;
-  using R = Rows<T, VEC, NV, 2, DEPTH>;
-  using L = Lanes<T, VEC, NV, kForwardShared<VEC, FMT, POST>>;
+  using R = Rows<T, VEC, NV, 2, DEPTH, THREADS>;
+  using L = Lanes<T, VEC, NV, kForwardShared<VEC, FMT, POST>, THREADS>;
   static_assert(R::bytes(THREADS) + 2 * L::bytes(THREADS) <= kMostSmem, "227 KB of shared memory");
   const int smem = R::bytes(g.threads) + 2 * L::bytes(g.threads);
   return go(block_norm_kernel<T, VEC, NV, FMT, POST, THREADS, BLOCKS, DEPTH>, smem,
@@ -612,8 +668,8 @@ int backward_blocks(const Grid& g, int rows, int sms, bool vec, bool whole) {
 
 template <typename T, int VEC, int NV, bool POST, bool WHOLE, int THREADS, int BLOCKS, int DEPTH>
 int go_backward(const BlockNormGrads& a, const Grid& g, int blocks, cudaStream_t stream) {
-  using R = Rows<T, VEC, NV, WHOLE ? 3 : 4, DEPTH>;
-  using L = Lanes<T, VEC, NV, SharedWeights<VEC, WHOLE>::value>;
+  using R = Rows<T, VEC, NV, WHOLE ? 3 : 4, DEPTH, THREADS>;
+  using L = Lanes<T, VEC, NV, SharedWeights<VEC, WHOLE>::value, THREADS>;
   static_assert(R::bytes(THREADS) + 2 * L::bytes(THREADS) <= kMostSmem, "227 KB of shared memory");
   const int smem = R::bytes(g.threads) + 2 * L::bytes(g.threads);
   return go(block_norm_bwd_kernel<T, VEC, NV, POST, WHOLE, THREADS, BLOCKS, DEPTH>, smem, blocks, g, a, stream);

@@ -15,6 +15,7 @@ namespace fp4 {
 
 using packed::add2;
 using packed::fma2;
+using packed::mul2;
 using packed::pair_of;
 
 constexpr int kNv = 1, kMx = 2;   // formats
@@ -130,12 +131,17 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
 // Codes of eight packed bf16 times f, the first in the lowest nibble. f is the reciprocal of the scale, so the product
 // misses the quotient by 2^-22 of it at most; the quotient of a bf16 value by an e4m3 scale (or a power of two) is either
 // a tie between two codes or at least 2^-10 away from it, so rounding the product to multiples of 2^-14 first (adding and
-// subtracting 768) lands on ties where they are and moves nothing else across. Beyond 6 all become 6.
+// subtracting 768) lands on ties where they are and moves nothing else across. With the power of two of mxfp4 the product
+// is the quotient. Beyond 6 all become 6.
+template <int FMT>
 __device__ __forceinline__ uint32_t codes8(const uint32_t* v, float f) {
   uint64_t q[4];
   const uint64_t ff = pair_of(f, f), up = pair_of(768.f, 768.f), down = pair_of(-768.f, -768.f);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = add2(fma2(pair_of(low_bf16(v[i]), high_bf16(v[i])), ff, up), down);
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t x = pair_of(low_bf16(v[i]), high_bf16(v[i]));
+    q[i] = FMT == kMx ? mul2(x, ff) : add2(fma2(x, ff, up), down);
+  }
   uint32_t out;
   asm("{\n\t.reg .b8 a, b, c, d;\n\t.reg .f32 l, h;\n\t"
       "mov.b64 {l, h}, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 a, h, l;\n\t"
@@ -176,7 +182,7 @@ __device__ __forceinline__ void store16(const uint32_t* v, float mul, int row, i
   uint32_t byte = group_scale<FMT>(bits, mul, factor);
   if (vec < vecs) {
     *reinterpret_cast<uint2*>(codes + (static_cast<size_t>(row) * vecs + vec) * 8) =
-        make_uint2(codes8(v, factor), codes8(v + 4, factor));
+        make_uint2(codes8<FMT>(v, factor), codes8<FMT>(v + 4, factor));
   } else {
     byte = 0;
   }
@@ -195,7 +201,7 @@ __device__ __forceinline__ void store8(const uint32_t* v, float mul, int row, in
   for (int o = 1; o < kLanes; o <<= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
   float factor;
   uint32_t byte = group_scale<FMT>(bits, mul, factor);
-  if (vec < vecs) *reinterpret_cast<uint32_t*>(codes + (static_cast<size_t>(row) * vecs + vec) * 4) = codes8(v, factor);
+  if (vec < vecs) *reinterpret_cast<uint32_t*>(codes + (static_cast<size_t>(row) * vecs + vec) * 4) = codes8<FMT>(v, factor);
   else byte = 0;
   const int g = vec / kLanes;
   if (vec % kLanes == 0 && (g >> 2) < tiles) scales[scale_word(row, g >> 2, tiles) + (g & 3)] = byte;
