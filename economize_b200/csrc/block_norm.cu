@@ -77,6 +77,10 @@ struct Pack {
     if constexpr (VEC == 1) return pair_of(get(0), 0.f);
     else return pair_of(get(2 * k), get(2 * k + 1));
   }
+  __device__ __forceinline__ void set(const float* f) {
+#pragma unroll
+    for (int k = 0; k < (VEC + 1) / 2; ++k) set2(k, pair_of(f[2 * k], VEC == 1 ? 0.f : f[2 * k + 1]));
+  }
   __device__ __forceinline__ void set2(int k, uint64_t pair) {
     float lo, hi;
     unpair(pair, lo, hi);
@@ -412,7 +416,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   Rows<T, VEC, NV, WHOLE ? 3 : 4, DEPTH, THREADS> rows(ring);
   const int per_block = blockDim.x / (32 * warps);
   const int teams = gridDim.x * per_block, self = blockIdx.x * per_block + team.index;
-  const bool post = POST && a.post != nullptr;
+  const bool post = POST && (VEC > 1 || a.post != nullptr);
   const int gate_mode = WHOLE ? kGateNone : a.gate_mode;
   const int hidden = a.hidden;
   const float mean = 1.f / static_cast<float>(hidden);
@@ -486,6 +490,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
     for (int i = 0; i < NV; ++i) {
       const int at = (team.first + i * team.step) * VEC;
       Pack<T, VEC> dn, u, x, fg, out, dg;
+      float ds_[VEC], dg_[VEC];
       rows.get(dn, 0, i, at, hidden);
       rows.get(u, 1, i, at, hidden);
       if constexpr (!WHOLE) rows.get(x, 3, i, at, hidden);
@@ -496,13 +501,13 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const float ds = fmaf(is, dn.get(j) * wi.get(j) - sh[i][j] * dot, u.get(j));
-        out.set(j, ds);
+        ds_[j] = ds;
         float db = gate * ds;
         if constexpr (!WHOLE) {
           const float xh = x.get(j) * ix;  // without a norm behind the block ix is 1
           const float pw = POST && post ? pi.get(j) : 1.f;
           if (gate_mode == kGateFull) {
-            dg.set(j, a.scale * ds * (xh * pw));
+            dg_[j] = a.scale * ds * (xh * pw);
             db *= fg.get(j);
           } else if (gate_mode == kGateToken) {
             sums.y = fmaf(xh * pw, ds, sums.y);
@@ -515,9 +520,12 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
         }
         sh[i][j] = db;
       }
+      out.set(ds_);
       if (a.dresidual != nullptr) out.store(static_cast<T*>(a.dresidual) + static_cast<size_t>(row) * hidden, at, hidden);
-      if (gate_mode == kGateFull && a.dgate != nullptr)
+      if (gate_mode == kGateFull && a.dgate != nullptr) {
+        dg.set(dg_);
         dg.store(static_cast<T*>(a.dgate) + static_cast<size_t>(row) * hidden, at, hidden);
+      }
     }
     if constexpr (!WHOLE) {
       if ((POST && post) || gate_mode == kGateToken) {
@@ -535,7 +543,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
         if (POST && post) rows.get(x, WHOLE ? 0 : 3, i, at, hidden);
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
-          out.set(j, POST && post ? ix * (sh[i][j] - x.get(j) * ix * m) : sh[i][j]);
+          if (POST && post) sh[i][j] = ix * (sh[i][j] - x.get(j) * ix * m);
+        out.set(sh[i]);
         out.store(static_cast<T*>(a.dx) + static_cast<size_t>(row) * hidden, at, hidden);
       }
     }
