@@ -59,6 +59,29 @@ struct Cast<__half> {
   }
 };
 
+// What arithmetic works on: two fp32 values in a 64-bit register, both at once, or the one of VEC = 1.
+template <int VEC>
+using Vals = std::conditional_t<VEC == 1, float, uint64_t>;
+__device__ __forceinline__ float mul2(float a, float b) { return a * b; }
+__device__ __forceinline__ float fma2(float a, float b, float c) { return fmaf(a, b, c); }
+template <int VEC>
+__device__ __forceinline__ Vals<VEC> vals(float v) {
+  if constexpr (VEC == 1) return v;
+  else return pair_of(v, v);
+}
+__device__ __forceinline__ float one_of(float v, int) { return v; }
+__device__ __forceinline__ float one_of(uint64_t pair, int k) {
+  float v[2];
+  unpair(pair, v[0], v[1]);
+  return v[k];
+}
+__device__ __forceinline__ float total(float v) { return v; }
+__device__ __forceinline__ float total(uint64_t pair) {
+  float lo, hi;
+  unpair(pair, lo, hi);
+  return lo + hi;
+}
+
 // A lane's VEC consecutive elements, from element `at` of a row of `hidden` on: 16 bytes, or one element. (With 32 bytes a
 // lane, two loads or stores of 16, every access would touch half of each sector: 66 us where this takes 45 for 8192 rows
 // of 4096.)
@@ -72,25 +95,23 @@ struct Pack {
   __device__ __forceinline__ Pack() {}
   __device__ __forceinline__ float get(int i) const { return Cast<T>::to(v[i]); }
   __device__ __forceinline__ void set(int i, float f) { v[i] = Cast<T>::from(f); }
-  // elements 2 k and 2 k + 1 in one 64-bit register (a zero behind a single element)
-  __device__ __forceinline__ uint64_t get2(int k) const {
-    if constexpr (VEC == 1) return pair_of(get(0), 0.f);
+  // elements 2 k and 2 k + 1 (Vals)
+  __device__ __forceinline__ Vals<VEC> get2(int k) const {
+    if constexpr (VEC == 1) return get(0);
     else return pair_of(get(2 * k), get(2 * k + 1));
   }
-  __device__ __forceinline__ void set(const float* f) {
-#pragma unroll
-    for (int k = 0; k < (VEC + 1) / 2; ++k) set2(k, pair_of(f[2 * k], VEC == 1 ? 0.f : f[2 * k + 1]));
-  }
-  __device__ __forceinline__ void set2(int k, uint64_t pair) {
-    float lo, hi;
-    unpair(pair, lo, hi);
+  __device__ __forceinline__ void set2(int k, Vals<VEC> f) {
     if constexpr (VEC == 1) {
-      set(0, lo);
-    } else if constexpr (sizeof(T) == 4) {
-      set(2 * k, lo);
-      set(2 * k + 1, hi);
+      set(0, f);
     } else {
-      words[k] = Cast<T>::from(lo, hi);
+      float lo, hi;
+      unpair(f, lo, hi);
+      if constexpr (sizeof(T) == 4) {
+        set(2 * k, lo);
+        set(2 * k + 1, hi);
+      } else {
+        words[k] = Cast<T>::from(lo, hi);
+      }
     }
   }
   // row[at ..], zeros where the row is null or has ended
@@ -278,11 +299,6 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   const T* rp = static_cast<const T*>(a.residual);
   const T* gp = static_cast<const T*>(a.gate);
   constexpr int kPairs = (VEC + 1) / 2;
-  auto total = [](uint64_t pair) {
-    float lo, hi;
-    unpair(pair, lo, hi);
-    return VEC == 1 ? lo : lo + hi;
-  };
   auto start = [&](int slot, int row) {
     const bool on = row < a.rows;
     rows.start(slot, 0, on ? xp + row * a.x_stride : nullptr, team.first, team.step, hidden);
@@ -304,10 +320,10 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
     if (a.gate_mode == kGateToken && real) factor *= Cast<T>::to(gp[row * a.gate_stride]);
     if constexpr (DEPTH == 0) start(0, row);
     rows.wait();
-    uint64_t s[NV][kPairs];
+    Vals<VEC> s[NV][kPairs];
     float ix = 1.f;
     if (post) {
-      uint64_t q = 0;
+      Vals<VEC> q = 0;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         Pack<T, VEC> x;
@@ -321,8 +337,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
       ix = rsqrtf(team.sum(total(q)) * mean + a.eps);
       if (a.inv_x != nullptr && team.first == 0 && real) a.inv_x[row] = ix;
     }
-    const uint64_t ix2 = pair_of(ix, ix), factor2 = pair_of(factor, factor);
-    uint64_t q = 0;
+    const Vals<VEC> ix2 = vals<VEC>(ix), factor2 = vals<VEC>(factor);
+    Vals<VEC> q = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int at = (team.first + i * team.step) * VEC;
@@ -363,7 +379,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
         out.store(static_cast<T*>(a.stream) + static_cast<size_t>(row) * hidden, (team.first + i * team.step) * VEC, hidden);
     }
     const float is = rsqrtf(team.sum(total(q)) * mean + a.eps);
-    const uint64_t is2 = pair_of(is, is);
+    const Vals<VEC> is2 = vals<VEC>(is);
     if (a.inv_s != nullptr && team.first == 0 && real) a.inv_s[row] = is;
     Pack<T, VEC> out[NV];
 #pragma unroll
@@ -443,13 +459,14 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   w.fetch(behind, static_cast<const T*>(a.weight), team.first, team.step, hidden);
   if constexpr (POST)
     p.fetch(behind + w.bytes(blockDim.x), static_cast<const T*>(a.post), team.first, team.step, hidden);
-  float dw[NV][VEC], dp[POST ? NV : 1][VEC];
+  constexpr int kPairs = (VEC + 1) / 2;
+  Vals<VEC> dw[NV][kPairs], dp[POST ? NV : 1][kPairs];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      dw[i][j] = 0.f;
-      if constexpr (POST) dp[i][j] = 0.f;
+    for (int k = 0; k < kPairs; ++k) {
+      dw[i][k] = 0;
+      if constexpr (POST) dp[i][k] = 0;
     }
   for (int row = self; row < a.rows; row += teams) {
     const float is = a.inv_s[row], ix = post ? a.inv_x[row] : 1.f;
@@ -457,8 +474,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
     if (gate_mode == kGateToken) gate *= Cast<T>::to(gp[row * a.gate_stride]);
     if constexpr (DEPTH == 0) start(0, row);
     rows.wait();
-    float sh[NV][VEC];  // the normalised stream
-    float dot = 0.f;
+    const Vals<VEC> is2 = vals<VEC>(is), ix2 = vals<VEC>(ix), gate2 = vals<VEC>(gate);
+    Vals<VEC> sh[NV][kPairs];  // the normalised stream
+    Vals<VEC> dots = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int at = (team.first + i * team.step) * VEC;
@@ -471,26 +489,26 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
       Pack<T, VEC> pi;
       if constexpr (POST) pi = p.get(i);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float s = r.get(j);
+      for (int k = 0; k < kPairs; ++k) {
+        Vals<VEC> s = r.get2(k);
         if constexpr (!WHOLE) {
-          float b = x.get(j);
-          if (POST && post) b *= ix * pi.get(j);
-          if (gate_mode == kGateFull) b *= fg.get(j);
-          s = fmaf(gate, b, s);
+          Vals<VEC> b = x.get2(k);
+          if (POST && post) b = mul2(b, mul2(ix2, pi.get2(k)));
+          if (gate_mode == kGateFull) b = mul2(b, fg.get2(k));
+          s = fma2(gate2, b, s);
         }
-        sh[i][j] = s * is;
-        dw[i][j] = fmaf(dn.get(j), sh[i][j], dw[i][j]);
-        dot = fmaf(dn.get(j) * wi.get(j), sh[i][j], dot);
+        sh[i][k] = mul2(s, is2);
+        dw[i][k] = fma2(dn.get2(k), sh[i][k], dw[i][k]);
+        dots = fma2(mul2(dn.get2(k), wi.get2(k)), sh[i][k], dots);
       }
     }
-    dot = team.sum(dot) * mean;
-    float2 sums = make_float2(0.f, 0.f);  // h . xh and the token gate's gradient
+    const float dot = -team.sum(total(dots)) * mean;
+    const Vals<VEC> dot2 = vals<VEC>(dot), scale2 = vals<VEC>(a.scale);
+    Vals<VEC> hx = 0, gx = 0;  // h . xh and the token gate's gradient
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int at = (team.first + i * team.step) * VEC;
       Pack<T, VEC> dn, u, x, fg, out, dg;
-      float ds_[VEC], dg_[VEC];
       rows.get(dn, 0, i, at, hidden);
       rows.get(u, 1, i, at, hidden);
       if constexpr (!WHOLE) rows.get(x, 3, i, at, hidden);
@@ -499,34 +517,32 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
       Pack<T, VEC> pi;
       if constexpr (POST) pi = p.get(i);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float ds = fmaf(is, dn.get(j) * wi.get(j) - sh[i][j] * dot, u.get(j));
-        ds_[j] = ds;
-        float db = gate * ds;
+      for (int k = 0; k < kPairs; ++k) {
+        const Vals<VEC> ds = fma2(is2, fma2(sh[i][k], dot2, mul2(dn.get2(k), wi.get2(k))), u.get2(k));
+        out.set2(k, ds);
+        Vals<VEC> db = mul2(gate2, ds);
         if constexpr (!WHOLE) {
-          const float xh = x.get(j) * ix;  // without a norm behind the block ix is 1
-          const float pw = POST && post ? pi.get(j) : 1.f;
+          const Vals<VEC> xh = mul2(x.get2(k), ix2);  // without a norm behind the block ix is 1
+          const Vals<VEC> pw = POST && post ? pi.get2(k) : vals<VEC>(1.f);
           if (gate_mode == kGateFull) {
-            dg_[j] = a.scale * ds * (xh * pw);
-            db *= fg.get(j);
+            dg.set2(k, mul2(mul2(scale2, ds), mul2(xh, pw)));
+            db = mul2(db, fg.get2(k));
           } else if (gate_mode == kGateToken) {
-            sums.y = fmaf(xh * pw, ds, sums.y);
+            gx = fma2(mul2(xh, pw), ds, gx);
           }
           if (POST && post) {
-            dp[POST ? i : 0][j] = fmaf(db, xh, dp[POST ? i : 0][j]);
-            db *= pw;  // h
-            sums.x = fmaf(db, xh, sums.x);
+            dp[POST ? i : 0][k] = fma2(db, xh, dp[POST ? i : 0][k]);
+            db = mul2(db, pw);  // h
+            hx = fma2(db, xh, hx);
           }
         }
-        sh[i][j] = db;
+        sh[i][k] = db;
       }
-      out.set(ds_);
       if (a.dresidual != nullptr) out.store(static_cast<T*>(a.dresidual) + static_cast<size_t>(row) * hidden, at, hidden);
-      if (gate_mode == kGateFull && a.dgate != nullptr) {
-        dg.set(dg_);
+      if (gate_mode == kGateFull && a.dgate != nullptr)
         dg.store(static_cast<T*>(a.dgate) + static_cast<size_t>(row) * hidden, at, hidden);
-      }
     }
+    float2 sums = make_float2(total(hx), total(gx));
     if constexpr (!WHOLE) {
       if ((POST && post) || gate_mode == kGateToken) {
         sums = team.sum(sums);
@@ -535,16 +551,16 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
       }
     }
     if (a.dx != nullptr) {
-      const float m = sums.x * mean;
+      const float m = -ix * sums.x * mean;
+      const Vals<VEC> m2 = vals<VEC>(m);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int at = (team.first + i * team.step) * VEC;
         Pack<T, VEC> x, out;
         if (POST && post) rows.get(x, WHOLE ? 0 : 3, i, at, hidden);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          if (POST && post) sh[i][j] = ix * (sh[i][j] - x.get(j) * ix * m);
-        out.set(sh[i]);
+        for (int k = 0; k < kPairs; ++k)
+          out.set2(k, POST && post ? mul2(ix2, fma2(x.get2(k), m2, sh[i][k])) : sh[i][k]);
         out.store(static_cast<T*>(a.dx) + static_cast<size_t>(row) * hidden, at, hidden);
       }
     }
@@ -560,8 +576,10 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       if (at + j >= hidden) continue;
-      if (a.dw_part != nullptr) a.dw_part[to + j] = dw[i][j];
-      if (POST && a.dpost_part != nullptr) a.dpost_part[to + j] = dp[i][j];
+      if (a.dw_part != nullptr) a.dw_part[to + j] = one_of(dw[i][j / 2], j % 2);
+      if constexpr (POST) {
+        if (a.dpost_part != nullptr) a.dpost_part[to + j] = one_of(dp[i][j / 2], j % 2);
+      }
     }
   }
 }
