@@ -1,6 +1,7 @@
 // PyTorch bindings of the 4-bit operators (fp4.cu, gemm_fp4.cu) and of the norms around a block (block_norm.cu):
 // argument checks, workspaces from PyTorch's caching allocator, tensor maps, launches on the current stream.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -125,14 +126,6 @@ Tensor fp4_quantize(const Tensor& x, int64_t fmt) {
   // the result may become a weight, which products fetch before the kernel in front of them ends: no early start
   quantize_into(rows, to, true, false);
   return data;
-}
-
-// Where codes, scales and row scales of such a buffer start, and its size.
-std::tuple<int64_t, int64_t, int64_t, int64_t> fp4_offsets(int64_t rows, int64_t K, int64_t fmt) {
-  check_format(fmt);
-  check_columns(K, "fp4_offsets");
-  const Fp4Layout l = fp4_layout(fp4_shape(rows, K, fmt));
-  return {l.codes, l.scales, l.row_scale, l.bytes};
 }
 
 Fp4 check_buffer(const Tensor& data, int64_t rows, int64_t K, int64_t fmt, const char* what) {
@@ -545,6 +538,19 @@ struct BlockNormFunction : torch::autograd::Function<BlockNormFunction> {
   }
 };
 
+// A leaf's gradients are added up on the stream of the first graph that holds the leaf. Where that is the default stream,
+// which cannot join a capture, and that graph still lives, the engine would break off the captured backward pass, and the
+// process with it.
+void check_captured_leaf(const Tensor& t) {
+  if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!node) return;
+  const auto stream = node->stream();
+  TORCH_CHECK(!stream.has_value() || c10::cuda::CUDAStream(*stream) != c10::cuda::getDefaultCUDAStream(t.get_device()),
+              "block_norm: a graph made on the default stream still holds a leaf of this captured call, whose backward "
+              "pass could not be captured; drop that graph, or make it on a side stream");
+}
+
 std::tuple<Tensor, Tensor> block_norm(const Tensor& x, const c10::optional<Tensor>& residual, const Tensor& weight,
                                       const c10::optional<Tensor>& post, const c10::optional<Tensor>& gate, double scale,
                                       double eps) {
@@ -559,6 +565,9 @@ std::tuple<Tensor, Tensor> block_norm(const Tensor& x, const c10::optional<Tenso
   }
   Tensor normed, stream;
   if (grad && at::GradMode::is_enabled()) {
+    c10::cuda::CUDAGuard guard(x.device());
+    if (at::cuda::currentStreamCaptureStatus() != at::cuda::CaptureStatus::None)
+      for (const Tensor* t : {&c.x, &c.residual, &weight, &c.post, &c.gate}) check_captured_leaf(*t);
     auto given = [](const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; };
     auto out = BlockNormFunction::apply(c.x, given(c.residual), weight, given(c.post), given(c.gate), scale, eps);
     normed = out[0];
@@ -580,8 +589,6 @@ void bind_block(pybind11::module_& m) {
   namespace py = pybind11;
   m.def("fp4_quantize", &fp4_quantize, "bf16 rows in 4 bits, one buffer (fmt 1 nvfp4, 2 mxfp4)", py::arg("x"),
         py::arg("fmt"));
-  m.def("fp4_offsets", &fp4_offsets, "offsets of codes, scales and row scales in such a buffer, and its bytes",
-        py::arg("rows"), py::arg("K"), py::arg("fmt"));
   m.def("fp4_values", &fp4_values, "the bf16 values of such a buffer", py::arg("data"), py::arg("rows"), py::arg("K"),
         py::arg("fmt"));
   m.def("fp4_dequantize", &fp4_dequantize, "the bf16 values of a 4-bit weight", py::arg("codes"), py::arg("scales"),

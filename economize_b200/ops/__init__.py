@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import torch
 
+from ..errors import ConfigError
 from . import reference
 from ._ext import available, load_error, require
 from .fp4 import FP4Tensor, FP4Weight
@@ -280,8 +281,12 @@ def linear(x: torch.Tensor, weight, bias: torch.Tensor | None = None) -> torch.T
     :class:`~economize_b200.ops.quant.QWeight` the weight-only GEMM of ``csrc/gemm_wq.cu``, and for an
     :class:`~economize_b200.ops.fp4.FP4Weight` the 4-bit GEMM of ``csrc/gemm_fp4.cu`` (``x`` bf16, or in 4 bits)."""
     if isinstance(weight, (QWeight, FP8BlockWeight, Sparse24Weight)) or hasattr(weight, "linear"):
+        if isinstance(x, FP4Tensor) and not isinstance(weight, FP4Weight):
+            raise ConfigError(f"4-bit activations multiply with an FP4Weight, not a {type(weight).__name__}")
         y = weight.linear(x)
         return y if bias is None else y + bias
+    if isinstance(x, FP4Tensor):
+        raise ConfigError("4-bit activations multiply with an FP4Weight, not a plain weight")
     if x.is_cuda:
         shape = x.shape
         y = require().linear(x.reshape(-1, shape[-1]), weight)

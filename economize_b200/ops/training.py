@@ -3,9 +3,9 @@ the norms around a block (which inference uses too).
 
 On CUDA both directions are the hand-written kernels of ``csrc/readout.cu``, ``csrc/packed_attention.cu``,
 ``csrc/packed_attention_bwd.cu`` and ``csrc/block_norm.cu`` (autograd functions in ``csrc/bindings_train.cpp`` and
-``csrc/bindings_block.cpp``); CPU tensors take the formulas of :mod:`.reference`, which autograd differentiates in either mode and any
-number of times. The kernels have the first reverse-mode derivative: dual tensors and ``create_graph=True`` are refused
-on CUDA. There is no third path.
+``csrc/bindings_block.cpp``); CPU tensors take the formulas of :mod:`.reference`, which autograd differentiates in either
+mode and any number of times. The kernels have the first reverse-mode derivative: dual tensors and ``create_graph=True``
+are refused on CUDA. There is no third path.
 """
 
 from __future__ import annotations
@@ -118,7 +118,8 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Ten
     ``normed`` are rounded once each, so ``normed`` is the norm of the unrounded stream (unlike two calls of
     :func:`~economize_b200.ops.rmsnorm`, which round in between as Hugging Face's modules do). Without ``post_weight`` and
     ``gate`` the gradients are taken from the rounded stream, and with ``scale=1`` those of ``x`` and ``residual`` are one
-    tensor.
+    tensor. A call captured into a CUDA graph with its backward pass needs leaves that no living graph of the default
+    stream holds, and is refused otherwise.
     """
     if x.is_cuda:  # the checks are the extension's, in C++
         if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:

@@ -1,6 +1,7 @@
 """``quant`` and ``draft_quant`` techniques: replace projections by packed :class:`~economize_b200.ops.quant.QWeight`
 weights that the tcgen05 weight-only GEMM reads, or by weights whose products quantise their activations too
-(:class:`~economize_b200.ops.fp8.FP8BlockWeight`, :class:`~economize_b200.ops.fp4.FP4Weight`) (economize ``techniques/quant/technique.py:30-120``).
+(:class:`~economize_b200.ops.fp8.FP8BlockWeight`, :class:`~economize_b200.ops.fp4.FP4Weight`) (economize
+``techniques/quant/technique.py:30-120``).
 
 The quantized weights (and, after AWQ, the re-scaled norm and producer weights) are the technique's state, so a
 saved model reloads without recalibrating.

@@ -287,6 +287,30 @@ def test_training_graph(cuda):
             assert torch.equal(a, b)
 
 
+def test_capture_beside_a_living_graph(cuda):
+    """A captured call is refused while a graph of the default stream holds its leaves, and runs once that is gone."""
+    t, dn, up = _make(cuda, 40, 64, torch.bfloat16, False, "none", seed=75, grad=True)
+    leaves = [v for v in t.values() if v is not None]
+    living = _call(t, 1.0, 1e-5)
+    want = torch.autograd.grad(living, leaves, (dn, up), retain_graph=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with pytest.raises(RuntimeError, match="still holds a leaf"), torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+        _call(t, 1.0, 1e-5)
+    with torch.no_grad():
+        inference = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(inference, stream=side):
+            again = _call(t, 1.0, 1e-5)
+    inference.replay()
+    assert all(torch.equal(a, b) for a, b in zip(again, living))
+    del living
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        grads = torch.autograd.grad(_call(t, 1.0, 1e-5), leaves, (dn, up))
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
 def test_autocast_and_refusals(cuda):
     t, dn, up = _make(cuda, 8, 64, torch.float32, True, "token", seed=80, grad=True)
     with torch.autocast("cuda", dtype=torch.bfloat16):

@@ -8,6 +8,7 @@ from economize_b200 import ops
 from economize_b200.errors import ConfigError
 from economize_b200.ops import fp4
 from economize_b200.ops.fp4 import FP4Weight
+from economize_b200.ops.fp8 import FP8BlockWeight
 from economize_b200.techniques.eagle3 import Eagle3Config
 from economize_b200.techniques.quant import DraftQuantConfig, QuantConfig
 
@@ -75,13 +76,18 @@ def test_not_finite():
         assert d[bad].isnan().all() and torch.equal(d[~bad], clean[~bad])
 
 
+def _plain():
+    return FP8BlockWeight.from_weight(torch.ones(128, 128))
+
+
 def test_refusals():
     x = torch.zeros(2, 64)
     w = FP4Weight.from_weight(torch.ones(8, 64))
     for bad in (lambda: ops.fp4_quantize(x, "fp4"), lambda: ops.fp4_quantize(x[:, :40]), lambda: ops.fp4_quantize(x[:, :0]),
                 lambda: ops.fp4_quantize(x.long()), lambda: ops.fp4_quantize(torch.zeros(1, 65568)),
                 lambda: ops.linear(x[:, :32], w), lambda: ops.linear(ops.fp4_quantize(x, "mxfp4"), w),
-                lambda: FP4Weight.from_weight(torch.ones(8)), lambda: FP4Weight(w.codes, w.scales[:, :1], w.row_scale, "nvfp4"),
+                lambda: ops.linear(ops.fp4_quantize(x), torch.ones(8, 64)),
+                lambda: ops.linear(ops.fp4_quantize(x), _plain()), lambda: FP4Weight.from_weight(torch.ones(8)), lambda: FP4Weight(w.codes, w.scales[:, :1], w.row_scale, "nvfp4"),
                 lambda: FP4Weight(w.codes, w.scales, w.row_scale, "mxfp4")):
         with pytest.raises(ConfigError):
             bad()
