@@ -277,7 +277,7 @@ class DraftQuantTechnique(_QuantBase):
                     continue
                 k = p.shape[1]
                 if cfg.format in W4A4_FORMATS:
-                    if k % 32 == 0:
+                    if k % 32 == 0 and k <= 65536:
                         self.weights[name.replace(".", "/")] = FP4Weight.from_weight(p.detach(), W4A4_FORMATS[cfg.format])
                     continue
                 g = cfg.group_size if cfg.group_size and k % cfg.group_size == 0 else None
