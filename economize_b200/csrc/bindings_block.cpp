@@ -36,6 +36,17 @@ bool aligned(const Tensor& x, int64_t bytes = 16) {
 // x, or a copy whose rows start on boundaries of 16 bytes (rows of whole 16-byte groups).
 Tensor on_boundary(const Tensor& x) { return aligned(x) ? x : x.clone(at::MemoryFormat::Contiguous); }
 
+// x, or a copy: 16-bit rows that start in the middle of a word where those of a tensor without gaps do, which are read in
+// words.
+Tensor on_words(const Tensor& x) {
+  const bool ok = !x.defined() || (reinterpret_cast<uintptr_t>(x.data_ptr()) % 4 == 0 &&
+                                   (x.size(0) <= 1 || (x.stride(0) - x.size(1)) % 2 == 0));
+  return ok ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+// x as the norms' kernels read it.
+Tensor norm_rows(const Tensor& x, bool vec) { return vec ? on_boundary(x) : x.element_size() == 2 ? on_words(x) : x; }
+
 // [..., C] as rows [R, C].
 Tensor as_rows(const Tensor& x) { return x.dim() == 2 ? x : x.reshape({-1, x.size(-1)}); }
 
@@ -314,9 +325,10 @@ NormOperands norm_operands(const Tensor& x, const Tensor& residual, const Tensor
   // rows of whole 16-byte groups are read in such groups, from copies where they do not start on a boundary (a token's
   // gate is read by itself): a row's sums then do not depend on where it lies
   o.vec = H * x.element_size() % 16 == 0;
+  for (Tensor* t : {&o.x, &o.residual, &o.gate})
+    if (t->defined() && !(t == &o.gate && o.gate_mode == ecz::kGateToken)) *t = norm_rows(*t, o.vec);
   if (o.vec)
-    for (Tensor* t : {&o.x, &o.residual, &o.weight, &o.post, &o.gate})
-      if (!(t == &o.gate && o.gate_mode == ecz::kGateToken)) *t = on_boundary(*t);
+    for (Tensor* t : {&o.weight, &o.post}) *t = on_boundary(*t);
   return o;
 }
 
@@ -488,8 +500,8 @@ struct BlockNormFunction : torch::autograd::Function<BlockNormFunction> {
       if (need_w) dw.zero_();
       if (need_p) dp.zero_();
     } else {
-      if (dn.defined()) dn = o.vec ? on_boundary(rows_of(dn)) : rows_of(dn);
-      if (up.defined()) up = o.vec ? on_boundary(rows_of(up)) : rows_of(up);
+      if (dn.defined()) dn = norm_rows(rows_of(dn), o.vec);
+      if (up.defined()) up = norm_rows(rows_of(up), o.vec);
       const ecz::NormType type = norm_type(o.x);
       const int sms = ecz::device_sms(o.x.get_device());
       ecz::BlockNormGrads a;

@@ -82,7 +82,9 @@ __device__ __forceinline__ float total(uint64_t pair) {
   return lo + hi;
 }
 
-// A lane's VEC consecutive elements, from element `at` of a row of `hidden` on: 16 bytes, or one element. (With 32 bytes a
+// A lane's VEC consecutive elements, from element `at` of a row of `hidden` on: 16 bytes, or one element, or (16-bit rows
+// that are no multiple of 16 bytes) a word. Odd rows of an odd length start in the middle of a word: `at` is odd there, and
+// -1 in the word that the row shares with the row before. (With 32 bytes a
 // lane, two loads or stores of 16, every access would touch half of each sector: 66 us where this takes 45 for 8192 rows
 // of 4096.)
 template <typename T, int VEC>
@@ -114,19 +116,30 @@ struct Pack {
       }
     }
   }
-  // row[at ..], zeros where the row is null or has ended
+  // row[at ..], zeros where the row is null, has ended or has not begun
   __device__ __forceinline__ void fetch(const T* row, int at, int hidden) {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) words[i] = 0;
-    if (row != nullptr && at < hidden) {
-      if constexpr (VEC == 1) v[0] = row[at];
-      else *reinterpret_cast<uint4*>(words) = *reinterpret_cast<const uint4*>(row + at);
+    if (row == nullptr || at >= hidden) return;
+    if constexpr (VEC == 1) {
+      v[0] = row[at];
+    } else if constexpr (VEC == 2) {
+      if (at >= 0) v[0] = row[at];
+      if (at + 1 < hidden) v[1] = row[at + 1];
+    } else {
+      *reinterpret_cast<uint4*>(words) = *reinterpret_cast<const uint4*>(row + at);
     }
   }
   __device__ __forceinline__ void store(T* row, int at, int hidden) const {
-    if (at < hidden) {
-      if constexpr (VEC == 1) row[at] = v[0];
-      else *reinterpret_cast<uint4*>(row + at) = *reinterpret_cast<const uint4*>(words);
+    if (at >= hidden) return;
+    if constexpr (VEC == 1) {
+      row[at] = v[0];
+    } else if constexpr (VEC == 2) {
+      if (at >= 0 && at + 1 < hidden) *reinterpret_cast<uint32_t*>(row + at) = words[0];
+      else if (at >= 0) row[at] = v[0];
+      else row[0] = v[1];
+    } else {
+      *reinterpret_cast<uint4*>(row + at) = *reinterpret_cast<const uint4*>(words);
     }
   }
 };
@@ -157,14 +170,16 @@ struct Rows {
   __device__ __forceinline__ uint32_t plane(int s, int op, int i) const {
     return base + static_cast<uint32_t>((s * kSlotPlanes + op * NV + i) * block_threads<THREADS>() * kEntry);
   }
-  // start the copy of operand op's row (zeros for null) into slot s; first, step: this lane's vectors
-  __device__ __forceinline__ void start(int s, int op, const T* row, int first, int step, int hidden) {
+  // start the copy of operand op's row (zeros for null) into slot s
+  template <class Place>
+  __device__ __forceinline__ void start(int s, int op, const T* row, const Place& place, int hidden) {
     if constexpr (kAhead) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int at = (first + i * step) * VEC;
+        const int at = place.template at<VEC>(i);
         const uint32_t to = plane(s, op, i);
-        const int bytes = row != nullptr && at < hidden ? kEntry : 0;  // the rest of the entry becomes zero
+        int bytes = row != nullptr && at < hidden ? kEntry : 0;  // the rest of the entry becomes zero
+        if constexpr (VEC == 2) bytes = at + 1 == hidden ? bytes / 2 : bytes;
         if constexpr (kEntry == 16)
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(row + at), "r"(bytes) : "memory");
         else
@@ -190,6 +205,7 @@ struct Rows {
                      : "memory");
       else
         asm volatile("ld.shared.b32 %0, [%1];" : "=r"(out.words[0]) : "r"(plane(slot, op, i)) : "memory");
+      if (VEC == 2 && i == 0 && at < 0) out.words[0] &= 0xffff0000u;  // the low half is the row before's
     } else {
       out.fetch(ptr[op], at, hidden);
     }
@@ -205,12 +221,13 @@ struct Lanes {
   static constexpr int bytes(int threads) { return SHARED ? NV * threads * kEntry : 0; }
   P held[SHARED ? 1 : NV];
   P* plane;
-  __device__ __forceinline__ void fetch(void* smem, const T* row, int first, int step, int hidden) {
+  template <class Place>
+  __device__ __forceinline__ void fetch(void* smem, const T* row, const Place& place, int hidden) {
     plane = static_cast<P*>(smem) + threadIdx.x;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       P v;
-      v.fetch(row, (first + i * step) * VEC, hidden);
+      v.fetch(row, place.template at<VEC>(i), hidden);
       if constexpr (SHARED) plane[i * block_threads<THREADS>()] = v;
       else held[i] = v;
     }
@@ -228,6 +245,7 @@ struct Team {
   int warps, index, first, step, lane, warp;
   float2* scratch;  // [2][kMaxWarps]
   int turn = 0;
+  int shift = 0;  // 1: this team's rows start in the middle of a word
   __device__ __forceinline__ Team(int warps_, float2* buf) : warps(warps_), scratch(buf) {
     const int w = threadIdx.x >> 5;
     lane = threadIdx.x & 31;
@@ -235,6 +253,11 @@ struct Team {
     warp = w - index * warps;
     first = warp * 32 + lane;
     step = warps * 32;
+  }
+  // the column of this lane's i-th vector
+  template <int VEC>
+  __device__ __forceinline__ int at(int i) const {
+    return (first + i * step) * VEC - (VEC == 2 ? shift : 0);
   }
   __device__ __forceinline__ void barrier() const {
     asm volatile("bar.sync %0, %1;" ::"r"(index + 1), "r"(warps * 32) : "memory");
@@ -301,19 +324,20 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   constexpr int kPairs = (VEC + 1) / 2;
   auto start = [&](int slot, int row) {
     const bool on = row < a.rows;
-    rows.start(slot, 0, on ? xp + row * a.x_stride : nullptr, team.first, team.step, hidden);
-    rows.start(slot, 1, on && rp != nullptr ? rp + row * a.r_stride : nullptr, team.first, team.step, hidden);
+    rows.start(slot, 0, on ? xp + row * a.x_stride : nullptr, team, hidden);
+    rows.start(slot, 1, on && rp != nullptr ? rp + row * a.r_stride : nullptr, team, hidden);
     rows.commit();
   };
   pdl_wait();
   int row = blockIdx.x * per_block + team.index;
+  if constexpr (VEC == 2) team.shift = row & hidden & 1;
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d) start(d, row + d * teams);
   Lanes<T, VEC, NV, kForwardShared<VEC, FMT, POST>, THREADS> w, p;
   uint8_t* behind = ring + Rows<T, VEC, NV, 2, DEPTH, THREADS>::bytes(blockDim.x);
-  w.fetch(behind, static_cast<const T*>(a.weight), team.first, team.step, hidden);
+  w.fetch(behind, static_cast<const T*>(a.weight), team, hidden);
   if constexpr (POST)
-    p.fetch(behind + w.bytes(blockDim.x), static_cast<const T*>(a.post), team.first, team.step, hidden);
+    p.fetch(behind + w.bytes(blockDim.x), static_cast<const T*>(a.post), team, hidden);
   for (; row < last; row += teams) {
     const bool real = row < a.rows;
     float factor = a.scale;
@@ -327,7 +351,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         Pack<T, VEC> x;
-        rows.get(x, 0, i, (team.first + i * team.step) * VEC, hidden);
+        rows.get(x, 0, i, team.template at<VEC>(i), hidden);
 #pragma unroll
         for (int k = 0; k < kPairs; ++k) {
           s[i][k] = x.get2(k);
@@ -341,7 +365,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
     Vals<VEC> q = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int at = (team.first + i * team.step) * VEC;
+      const int at = team.template at<VEC>(i);
       Pack<T, VEC> r;
       if (post) {
         const Pack<T, VEC> pi = p.get(i);
@@ -376,7 +400,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
 #pragma unroll
       for (int k = 0; k < kPairs; ++k) out.set2(k, s[i][k]);
       if (real)
-        out.store(static_cast<T*>(a.stream) + static_cast<size_t>(row) * hidden, (team.first + i * team.step) * VEC, hidden);
+        out.store(static_cast<T*>(a.stream) + static_cast<size_t>(row) * hidden, team.template at<VEC>(i), hidden);
     }
     const float is = rsqrtf(team.sum(total(q)) * mean + a.eps);
     const Vals<VEC> is2 = vals<VEC>(is);
@@ -388,7 +412,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
 #pragma unroll
       for (int k = 0; k < kPairs; ++k) out[i].set2(k, mul2(mul2(s[i][k], is2), wi.get2(k)));
       if (FMT == 0)
-        out[i].store(static_cast<T*>(a.normed) + static_cast<size_t>(row) * hidden, (team.first + i * team.step) * VEC,
+        out[i].store(static_cast<T*>(a.normed) + static_cast<size_t>(row) * hidden, team.template at<VEC>(i),
                      hidden);
     }
     if constexpr (FMT != 0) {
@@ -432,6 +456,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   Rows<T, VEC, NV, WHOLE ? 3 : 4, DEPTH, THREADS> rows(ring);
   const int per_block = blockDim.x / (32 * warps);
   const int teams = gridDim.x * per_block, self = blockIdx.x * per_block + team.index;
+  if constexpr (VEC == 2) team.shift = self & a.hidden & 1;
   const bool post = POST && (VEC > 1 || a.post != nullptr);
   const int gate_mode = WHOLE ? kGateNone : a.gate_mode;
   const int hidden = a.hidden;
@@ -444,10 +469,10 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   const int64_t r_stride = WHOLE ? hidden : a.r_stride;
   auto start = [&](int slot, int row) {
     const bool on = row < a.rows;
-    rows.start(slot, 0, on && np != nullptr ? np + row * a.dn_stride : nullptr, team.first, team.step, hidden);
-    rows.start(slot, 1, on && up != nullptr ? up + row * a.ds_stride : nullptr, team.first, team.step, hidden);
-    rows.start(slot, 2, on && rp != nullptr ? rp + row * r_stride : nullptr, team.first, team.step, hidden);
-    if constexpr (!WHOLE) rows.start(slot, 3, on ? xp + row * a.x_stride : nullptr, team.first, team.step, hidden);
+    rows.start(slot, 0, on && np != nullptr ? np + row * a.dn_stride : nullptr, team, hidden);
+    rows.start(slot, 1, on && up != nullptr ? up + row * a.ds_stride : nullptr, team, hidden);
+    rows.start(slot, 2, on && rp != nullptr ? rp + row * r_stride : nullptr, team, hidden);
+    if constexpr (!WHOLE) rows.start(slot, 3, on ? xp + row * a.x_stride : nullptr, team, hidden);
     rows.commit();
   };
   pdl_wait();
@@ -456,9 +481,9 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   constexpr bool kShared = SharedWeights<VEC, WHOLE>::value;
   Lanes<T, VEC, NV, kShared, THREADS> w, p;
   uint8_t* behind = ring + Rows<T, VEC, NV, WHOLE ? 3 : 4, DEPTH, THREADS>::bytes(blockDim.x);
-  w.fetch(behind, static_cast<const T*>(a.weight), team.first, team.step, hidden);
+  w.fetch(behind, static_cast<const T*>(a.weight), team, hidden);
   if constexpr (POST)
-    p.fetch(behind + w.bytes(blockDim.x), static_cast<const T*>(a.post), team.first, team.step, hidden);
+    p.fetch(behind + w.bytes(blockDim.x), static_cast<const T*>(a.post), team, hidden);
   constexpr int kPairs = (VEC + 1) / 2;
   Vals<VEC> dw[NV][kPairs], dp[POST ? NV : 1][kPairs];
 #pragma unroll
@@ -479,7 +504,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
     Vals<VEC> dots = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int at = (team.first + i * team.step) * VEC;
+      const int at = team.template at<VEC>(i);
       Pack<T, VEC> dn, r, x, fg;
       rows.get(dn, 0, i, at, hidden);
       rows.get(r, 2, i, at, hidden);
@@ -507,7 +532,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
     Vals<VEC> hx = 0, gx = 0;  // h . xh and the token gate's gradient
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int at = (team.first + i * team.step) * VEC;
+      const int at = team.template at<VEC>(i);
       Pack<T, VEC> dn, u, x, fg, out, dg;
       rows.get(dn, 0, i, at, hidden);
       rows.get(u, 1, i, at, hidden);
@@ -555,7 +580,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
       const Vals<VEC> m2 = vals<VEC>(m);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int at = (team.first + i * team.step) * VEC;
+        const int at = team.template at<VEC>(i);
         Pack<T, VEC> x, out;
         if (POST && post) rows.get(x, WHOLE ? 0 : 3, i, at, hidden);
 #pragma unroll
@@ -571,11 +596,11 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int at = (team.first + i * team.step) * VEC;
+    const int at = team.template at<VEC>(i);
     const size_t to = static_cast<size_t>(self) * hidden + at;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      if (at + j >= hidden) continue;
+      if (at + j < 0 || at + j >= hidden) continue;
       if (a.dw_part != nullptr) a.dw_part[to + j] = one_of(dw[i][j / 2], j % 2);
       if constexpr (POST) {
         if (a.dpost_part != nullptr) a.dpost_part[to + j] = one_of(dp[i][j / 2], j % 2);
@@ -615,11 +640,10 @@ struct Grid {
   int warps, nv, teams, threads;  // warps of a team, vectors a lane, teams and threads of a block
 };
 
-// `target` vectors of 16 bytes or single elements a lane, more where that would take more than 32 warps; several teams to a
-// block of 256 threads, or one.
+// `target` vectors a lane, more where that would take more than 32 warps; several teams to a block of 256 threads, or one.
 template <int VEC>
 Grid grid_of(int hidden, int target) {
-  const int all = (hidden + 32 * VEC - 1) / (32 * VEC);
+  const int all = (hidden + (VEC == 2 ? hidden % 2 : 0) + 32 * VEC - 1) / (32 * VEC);
   Grid g;
   g.warps = std::min(kMaxWarps, (all + target - 1) / target);
   if (g.warps <= 8) {
@@ -631,6 +655,14 @@ Grid grid_of(int hidden, int target) {
   g.teams = g.warps <= 8 ? 8 / g.warps : 1;
   g.threads = 32 * g.warps * g.teams;
   return g;
+}
+
+// Blocks for `rows`, at most `most`. In words, a team's rows start all in the middle of one or none does (Team::shift): where
+// it has more than one, the number of teams is even.
+int blocks_for(const Grid& g, int rows, int most, bool words) {
+  const int all = (rows + g.teams - 1) / g.teams;
+  if (all <= most) return all;
+  return words ? std::max(2, most & ~1) : most;
 }
 
 template <typename T>
@@ -651,7 +683,7 @@ int go_forward(const BlockNormArgs& a, const Grid& g, int sms, cudaStream_t stre
   static_assert(R::bytes(THREADS) + 2 * L::bytes(THREADS) <= kMostSmem, "227 KB of shared memory");
   const int smem = R::bytes(g.threads) + 2 * L::bytes(g.threads);
   return go(block_norm_kernel<T, VEC, NV, FMT, POST, THREADS, BLOCKS, DEPTH>, smem,
-            std::min((rows + g.teams - 1) / g.teams, sms * resident), g, a, stream);
+            blocks_for(g, rows, sms * resident, VEC == 2), g, a, stream);
 }
 
 // Blocks of 256 threads, two rows ahead: three to an SM, or four where the norm behind the block or the 4-bit result make
@@ -667,14 +699,28 @@ int run_forward(const BlockNormArgs& a, int sms, cudaStream_t stream) {
   return -1;
 }
 
+// 16-bit rows in words: as many columns a lane as above.
+template <typename T, bool POST>
+int run_forward_words(const BlockNormArgs& a, int sms, cudaStream_t stream) {
+  const Grid g = grid_of<2>(a.hidden, 8);
+  if (g.threads > 256) return go_forward<T, 2, 8, 0, POST, 1024, 1, 2>(a, g, sms, stream);
+  if (g.nv > 4) return go_forward<T, 2, 8, 0, POST, 256, 4, 2>(a, g, sms, stream);
+  return go_forward<T, 2, 4, 0, POST, 256, 4, 2>(a, g, sms, stream);
+}
+
 template <typename T>
 int run_forward_type(const BlockNormArgs& a, bool vec, int sms, cudaStream_t stream) {
   if (vec) return a.post != nullptr ? run_forward<T, 0, true>(a, sms, stream) : run_forward<T, 0, false>(a, sms, stream);
-  const Grid g = grid_of<1>(a.hidden, 4);
-  constexpr int kDepth = sizeof(T) == 4 ? 2 : 0;
-  if (g.threads <= 256) return go_forward<T, 1, 4, 0, true, 256, 4, kDepth>(a, g, sms, stream);
-  if (g.nv <= 4) return go_forward<T, 1, 4, 0, true, 1024, 1, kDepth>(a, g, sms, stream);
-  return go_forward<T, 1, 16, 0, true, 1024, 1, 0>(a, g, sms, stream);
+  if constexpr (sizeof(T) == 2) {
+    return a.post != nullptr ? run_forward_words<T, true>(a, sms, stream) : run_forward_words<T, false>(a, sms, stream);
+  } else {
+    // single elements: four a lane, more beyond 4096 columns (32768 rows of 1001: 113 us, with eight 117)
+    const Grid g = grid_of<1>(a.hidden, 4);
+    if (g.threads <= 256) return go_forward<T, 1, 4, 0, true, 256, 4, 2>(a, g, sms, stream);
+    if (g.nv <= 4) return go_forward<T, 1, 4, 0, true, 1024, 1, 2>(a, g, sms, stream);
+    if (g.nv <= 8) return go_forward<T, 1, 8, 0, true, 1024, 1, 2>(a, g, sms, stream);
+    return go_forward<T, 1, 16, 0, true, 1024, 1, 0>(a, g, sms, stream);
+  }
 }
 
 template <int FMT>
@@ -684,13 +730,17 @@ int run_forward_fp4(const BlockNormArgs& a, int sms, cudaStream_t stream) {
 
 template <typename T>
 Grid backward_grid(int hidden, bool vec) {
-  return vec ? grid_of<vec_of<T>()>(hidden, 2) : grid_of<1>(hidden, 4);
+  if (vec) return grid_of<vec_of<T>()>(hidden, 2);
+  // eight single elements a lane (32768 rows of 1001 in fp32: 121 us, with four 160)
+  return sizeof(T) == 2 ? grid_of<2>(hidden, 8) : grid_of<1>(hidden, 8);
 }
 
 // Three blocks of 256 threads to an SM from the stream, two from x and the residual, which takes more registers.
+template <typename T>
 int backward_blocks(const Grid& g, int rows, int sms, bool vec, bool whole) {
-  const int resident = g.threads > 256 ? 1 : vec && whole ? 3 : 2;
-  return std::min((rows + g.teams - 1) / g.teams, sms * resident);
+  const bool words = !vec && sizeof(T) == 2;
+  const int resident = g.threads > 256 ? 1 : (vec || words) && whole ? 3 : 2;
+  return blocks_for(g, rows, sms * resident, words);
 }
 
 template <typename T, int VEC, int NV, bool POST, bool WHOLE, int THREADS, int BLOCKS, int DEPTH>
@@ -724,22 +774,34 @@ int run_backward(const BlockNormGrads& a, const Grid& g, int blocks, cudaStream_
 
 template <typename T, bool WHOLE>
 int run_backward_single(const BlockNormGrads& a, const Grid& g, int blocks, cudaStream_t stream) {
-  constexpr int kDepth = sizeof(T) == 4 ? 2 : 0;
-  if (g.threads <= 256) return go_backward<T, 1, 4, !WHOLE, WHOLE, 256, 2, kDepth>(a, g, blocks, stream);
-  if (g.nv <= 4) return go_backward<T, 1, 4, !WHOLE, WHOLE, 1024, 1, kDepth>(a, g, blocks, stream);
+  if (g.threads <= 256) return go_backward<T, 1, 8, !WHOLE, WHOLE, 256, 2, 2>(a, g, blocks, stream);
+  if (g.threads <= 512) return go_backward<T, 1, 8, !WHOLE, WHOLE, 512, 1, 2>(a, g, blocks, stream);
+  if (g.nv <= 8) return go_backward<T, 1, 8, !WHOLE, WHOLE, 1024, 1, 1>(a, g, blocks, stream);
   return go_backward<T, 1, 16, !WHOLE, WHOLE, 1024, 1, 0>(a, g, blocks, stream);
+}
+
+template <typename T, bool POST, bool WHOLE>
+int run_backward_words(const BlockNormGrads& a, const Grid& g, int blocks, cudaStream_t stream) {
+  if (g.threads > 512) return go_backward<T, 2, 8, POST, WHOLE, 1024, 1, 1>(a, g, blocks, stream);
+  if (g.threads > 256) return go_backward<T, 2, 8, POST, WHOLE, 512, 1, 2>(a, g, blocks, stream);
+  if (g.nv > 4) return go_backward<T, 2, 8, POST, WHOLE, 256, WHOLE ? 3 : 2, 2>(a, g, blocks, stream);
+  return go_backward<T, 2, 4, POST, WHOLE, 256, WHOLE ? 3 : 2, 2>(a, g, blocks, stream);
 }
 
 template <typename T>
 int run_backward_type(const BlockNormGrads& a, bool vec, int sms, cudaStream_t stream) {
   const bool whole = a.stream != nullptr;
   const Grid g = backward_grid<T>(a.hidden, vec);
-  const int blocks = backward_blocks(g, a.rows, sms, vec, whole);
+  const int blocks = backward_blocks<T>(g, a.rows, sms, vec, whole);
   int rc;
   if (vec)
     rc = whole               ? run_backward_whole<T>(a, g, blocks, stream)
          : a.post != nullptr ? run_backward<T, true>(a, g, blocks, stream)
                              : run_backward<T, false>(a, g, blocks, stream);
+  else if constexpr (sizeof(T) == 2)
+    rc = whole               ? run_backward_words<T, false, true>(a, g, blocks, stream)
+         : a.post != nullptr ? run_backward_words<T, true, false>(a, g, blocks, stream)
+                             : run_backward_words<T, false, false>(a, g, blocks, stream);
   else
     rc = whole ? run_backward_single<T, true>(a, g, blocks, stream) : run_backward_single<T, false>(a, g, blocks, stream);
   if (rc != 0 || (a.dweight == nullptr && a.dpost == nullptr)) return rc;
@@ -752,7 +814,7 @@ int run_backward_type(const BlockNormGrads& a, bool vec, int sms, cudaStream_t s
 template <typename T>
 int parts_type(int rows, int hidden, bool vec, bool whole, int sms) {
   const Grid g = backward_grid<T>(hidden, vec);
-  return backward_blocks(g, rows, sms, vec, whole) * g.teams;
+  return backward_blocks<T>(g, rows, sms, vec, whole) * g.teams;
 }
 
 }  // namespace

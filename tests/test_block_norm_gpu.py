@@ -385,3 +385,35 @@ def test_chain(cuda, fmt):
     graph.replay()
     assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
     assert ops.require().status(0) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,hidden", [(9, 37), (1, 1), (7, 1), (700, 301), (3, 4095), (40, 6)])
+def test_rows_that_share_words(cuda, dtype, rows, hidden):
+    """16-bit rows of odd or short lengths: views with any offset and stride give the bits of tensors without gaps, and a
+    row that is not finite leaves its neighbours, with which it shares words, as they are."""
+    t, dn, up = _make(cuda, rows, hidden, dtype, True, "full", seed=90, grad=True)
+    leaves = list(t.values())
+    want = _call(t, 0.5, 1e-5)
+    grads = torch.autograd.grad(want, leaves, (dn, up))
+    for offset, stride in ((0, hidden + 1), (1, hidden + 2), (3, hidden + 3), (2, hidden + 4)):
+        def view(x):
+            flat = torch.full((rows * stride + 8,), float("nan"), device=cuda, dtype=dtype)
+            wide = flat[offset:offset + rows * stride].view(rows, stride)
+            wide[:, :hidden] = x.detach()
+            return wide[:, :hidden]
+
+        v = {k: view(x).requires_grad_() if x.dim() == 2 else x for k, x in t.items()}
+        got = _call(v, 0.5, 1e-5)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        again = torch.autograd.grad(got, list(v.values()), (view(dn), view(up)))
+        assert all(torch.equal(a, b) for a, b in zip(again, grads))
+    if rows >= 3:
+        with torch.no_grad():
+            t["x"][rows // 2] = float("nan")
+        got = _call(t, 0.5, 1e-5)
+        again = torch.autograd.grad(got, leaves, (dn, up))
+        others = torch.arange(rows, device=cuda) != rows // 2
+        for a, b in zip((*got, again[0], again[1], again[4]), (*want, grads[0], grads[1], grads[4])):
+            assert torch.equal(a[others], b[others])
+        assert not got[0][rows // 2].isfinite().any()
