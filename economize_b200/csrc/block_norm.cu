@@ -13,8 +13,8 @@
 //   ds = dstream + is (g - sh mean(g sh)),  dweight = sum_t dn sh,  dresidual = ds
 //   dgate = scale b . ds (summed over the columns where the gate has one value a token),  db = scale gate ds
 //   dx = ix (h - xh mean(h xh)) with h = db post,  dpost = sum_t db xh      (dx = db without a norm behind the block)
-// The forward pass saves is and ix. Sums over tokens: every team adds up its rows in registers, in order, and a second
-// kernel adds up the teams in order, so results do not depend on timing.
+// The forward pass saves is and ix. Sums over tokens: every team adds up its rows in registers, a block its
+// teams, a second kernel the blocks, each in order, so results do not depend on timing.
 #include <algorithm>
 #include <type_traits>
 
@@ -115,6 +115,16 @@ struct Pack {
         words[k] = Cast<T>::from(lo, hi);
       }
     }
+  }
+  // row[at ..] of a row that starts like the others do (Team::shift), zeros where it has ended or has not begun
+  __device__ __forceinline__ void fetch_row(const T* row, int at, int hidden) {
+    if constexpr (VEC == 2) {
+      if (row != nullptr && at >= 0 && at + 1 < hidden) {
+        words[0] = *reinterpret_cast<const uint32_t*>(row + at);
+        return;
+      }
+    }
+    fetch(row, at, hidden);
   }
   // row[at ..], zeros where the row is null, has ended or has not begun
   __device__ __forceinline__ void fetch(const T* row, int at, int hidden) {
@@ -379,7 +389,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
       }
       if (a.gate_mode == kGateFull) {
         Pack<T, VEC> g;
-        g.fetch(real ? gp + row * a.gate_stride : nullptr, at, hidden);
+        g.fetch_row(real ? gp + row * a.gate_stride : nullptr, at, hidden);
 #pragma unroll
         for (int k = 0; k < kPairs; ++k) s[i][k] = mul2(s[i][k], g.get2(k));
       }
@@ -444,8 +454,8 @@ struct SharedWeights {
   static constexpr bool value = VEC > 1 && !WHOLE;
 };
 
-// Persistent like the forward kernel. A team's sums for dweight and dpost go to its row of a.dw_part / a.dpost_part (fp32
-// [teams, hidden]). WHOLE: the stream is given in place of x and the residual.
+// Persistent like the forward kernel. A block's sums for dweight and dpost go to its row of a.dw_part / a.dpost_part (fp32
+// [blocks, hidden]). WHOLE: the stream is given in place of x and the residual.
 template <typename T, int VEC, int NV, bool POST, bool WHOLE, int THREADS, int BLOCKS, int DEPTH>
 __global__ void __launch_bounds__(THREADS, BLOCKS)
     block_norm_bwd_kernel(const __grid_constant__ BlockNormGrads a, int warps) {
@@ -509,7 +519,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
       rows.get(dn, 0, i, at, hidden);
       rows.get(r, 2, i, at, hidden);
       if constexpr (!WHOLE) rows.get(x, 3, i, at, hidden);
-      if (gate_mode == kGateFull) fg.fetch(gp + row * a.gate_stride, at, hidden);
+      if (gate_mode == kGateFull) fg.fetch_row(gp + row * a.gate_stride, at, hidden);
       const Pack<T, VEC> wi = w.get(i);
       Pack<T, VEC> pi;
       if constexpr (POST) pi = p.get(i);
@@ -537,7 +547,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
       rows.get(dn, 0, i, at, hidden);
       rows.get(u, 1, i, at, hidden);
       if constexpr (!WHOLE) rows.get(x, 3, i, at, hidden);
-      if (gate_mode == kGateFull) fg.fetch(gp + row * a.gate_stride, at, hidden);
+      if (gate_mode == kGateFull) fg.fetch_row(gp + row * a.gate_stride, at, hidden);
       const Pack<T, VEC> wi = w.get(i);
       Pack<T, VEC> pi;
       if constexpr (POST) pi = p.get(i);
@@ -594,17 +604,37 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
       rows.slot = rows.slot + 1 == DEPTH ? 0 : rows.slot + 1;
     }
   }
+  // A block's teams add their sums up in order, in the rows' place; a block's are its row of the parts.
+  const bool several = per_block > 1;
+  if (several) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+  }
+  static_assert(THREADS > 256 || DEPTH * (WHOLE ? 3 : 4) * sizeof(T) >= sizeof(float), "the sums fit in the rows' place");
+  float* sums = reinterpret_cast<float*>(ring);  // [teams of the block][hidden]
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int at = team.template at<VEC>(i);
-    const size_t to = static_cast<size_t>(self) * hidden + at;
+  for (int which = 0; which < (POST ? 2 : 1); ++which) {
+    float* part = which == 0 ? a.dw_part : a.dpost_part;
+    if (part == nullptr) continue;
+    part += static_cast<size_t>(blockIdx.x) * hidden;
+    float* to = several ? sums + team.index * hidden : part;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      if (at + j < 0 || at + j >= hidden) continue;
-      if (a.dw_part != nullptr) a.dw_part[to + j] = one_of(dw[i][j / 2], j % 2);
-      if constexpr (POST) {
-        if (a.dpost_part != nullptr) a.dpost_part[to + j] = one_of(dp[i][j / 2], j % 2);
+    for (int i = 0; i < NV; ++i) {
+      const int at = team.template at<VEC>(i);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        if (at + j < 0 || at + j >= hidden) continue;
+        to[at + j] = one_of(which == 0 ? dw[i][j / 2] : dp[POST ? i : 0][j / 2], j % 2);
       }
+    }
+    if (several) {
+      __syncthreads();
+      for (int c = threadIdx.x; c < hidden; c += blockDim.x) {
+        float v = sums[c];
+        for (int t = 1; t < per_block; ++t) v += sums[t * hidden + c];
+        part[c] = v;
+      }
+      __syncthreads();
     }
   }
 }
@@ -807,14 +837,14 @@ int run_backward_type(const BlockNormGrads& a, bool vec, int sms, cudaStream_t s
   if (rc != 0 || (a.dweight == nullptr && a.dpost == nullptr)) return rc;
   return launch_pdl(block_norm_sum_kernel<T>, dim3((a.hidden + 31) / 32, a.dpost != nullptr ? 2 : 1), dim3(1024), 0, stream,
                     static_cast<const float*>(a.dw_part), static_cast<const float*>(a.dpost_part),
-                    static_cast<T*>(a.dweight), static_cast<T*>(a.dpost), blocks * g.teams, a.hidden) == cudaSuccess ? 0
+                    static_cast<T*>(a.dweight), static_cast<T*>(a.dpost), blocks, a.hidden) == cudaSuccess ? 0
                                                                                                                     : -1;
 }
 
 template <typename T>
 int parts_type(int rows, int hidden, bool vec, bool whole, int sms) {
   const Grid g = backward_grid<T>(hidden, vec);
-  return backward_blocks<T>(g, rows, sms, vec, whole) * g.teams;
+  return backward_blocks<T>(g, rows, sms, vec, whole);
 }
 
 }  // namespace

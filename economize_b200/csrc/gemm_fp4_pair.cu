@@ -328,10 +328,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         } else {
           __syncwarp();
-          if (n + lane < args.N) {
-            for (int r = 0; r < 32 && row + r < args.M; ++r)
-              args.y[static_cast<size_t>(row + r) * args.N + n + lane] = *reinterpret_cast<const bf16*>(
-                  to + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+          // rows that TMA does not store, a column a lane: eight rows' values first, then their stores
+          bf16* out = args.y + static_cast<size_t>(row) * args.N + n + lane;
+          const int rows = n + lane < args.N ? args.M - row : 0;
+#pragma unroll
+          for (int r = 0; r < 32; r += 8) {
+            bf16 column[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              column[i] = *reinterpret_cast<const bf16*>(to + (r + i) * 64 + (((lane >> 3) ^ (((r + i) >> 1) & 3)) << 4) +
+                                                         (lane & 7) * 2);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (r + i < rows) out[static_cast<size_t>(r + i) * args.N] = column[i];
           }
           __syncwarp();
         }
