@@ -5,16 +5,22 @@
 //   s = residual + scale gate b            (stream; the residual and the gate may be missing)
 //   n = s rsqrt(mean s^2 + eps) weight     (normed; as bf16 / fp16 / fp32, or from bf16 on to 4 bits, fp4_common.cuh)
 //
-// Everything is held in fp32; n and s are rounded once each, n is taken from the unrounded s. Bound by HBM: forward two
-// rows read and two written per token, backward up to four read and two written. A team of warps keeps a row in
-// registers; rows are read in 16-byte vectors where bases and strides allow it, else element by element.
+// Everything is held in fp32; n and s are rounded once each, n is taken from the unrounded s. A team of warps keeps a row
+// in registers, 16 columns a lane; rows are read in 16-byte vectors, 16-bit rows that are no multiple of 16 bytes in words,
+// other fp32 rows element by element.
+//
+// Forward two rows are read and two written per token: 8192 rows of 4096 in bf16 take 39 us, 6.9 TB/s, bound by HBM (6.3 at
+// 8192 columns). Backward up to four are read and two written: 53 us from the stream (5.0 TB/s, and 6 to add up the blocks'
+// sums), 108 with both norms (3.7 TB/s), where half of all issue slots and two barriers a row stand against 16 warps an SM.
+// In 4 bits the quantisation's instructions bound it: 4096 rows of 4096 with both norms take 29 us, 3.8 TB/s, 65% of the
+// issue slots. Sums, products and roundings work on pairs of columns (f32x2): with single ones the last took 34 us.
 //
 // Backward, with g = dn weight, sh = s is (is = rsqrt(mean s^2 + eps), xh = x ix likewise):
 //   ds = dstream + is (g - sh mean(g sh)),  dweight = sum_t dn sh,  dresidual = ds
 //   dgate = scale b . ds (summed over the columns where the gate has one value a token),  db = scale gate ds
 //   dx = ix (h - xh mean(h xh)) with h = db post,  dpost = sum_t db xh      (dx = db without a norm behind the block)
-// The forward pass saves is and ix. Sums over tokens: every team adds up its rows in registers, a block its
-// teams, a second kernel the blocks, each in order, so results do not depend on timing.
+// The forward pass saves is and ix. Sums over tokens: every team adds up its rows in registers, a block its teams, a second
+// kernel the blocks, each in order, so results do not depend on timing.
 #include <algorithm>
 #include <type_traits>
 
@@ -84,9 +90,8 @@ __device__ __forceinline__ float total(uint64_t pair) {
 
 // A lane's VEC consecutive elements, from element `at` of a row of `hidden` on: 16 bytes, or one element, or (16-bit rows
 // that are no multiple of 16 bytes) a word. Odd rows of an odd length start in the middle of a word: `at` is odd there, and
-// -1 in the word that the row shares with the row before. (With 32 bytes a
-// lane, two loads or stores of 16, every access would touch half of each sector: 66 us where this takes 45 for 8192 rows
-// of 4096.)
+// -1 in the word that the row shares with the row before. (With 32 bytes a lane, two loads or stores of 16, every access
+// would touch half of each sector: 66 us where this took 45 for 8192 rows of 4096.)
 template <typename T, int VEC>
 struct Pack {
   static constexpr int kWords = (VEC * static_cast<int>(sizeof(T)) + 3) / 4;
@@ -729,7 +734,8 @@ int run_forward(const BlockNormArgs& a, int sms, cudaStream_t stream) {
   return -1;
 }
 
-// 16-bit rows in words: as many columns a lane as above.
+// 16-bit rows in words: as many columns a lane as above. 8192 rows of 4095 take 104 us where vectors take 49 for 4096 (four
+// times the accesses); single elements, which cp.async does not copy ahead, took 289.
 template <typename T, bool POST>
 int run_forward_words(const BlockNormArgs& a, int sms, cudaStream_t stream) {
   const Grid g = grid_of<2>(a.hidden, 8);

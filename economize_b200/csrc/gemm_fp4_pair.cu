@@ -16,6 +16,9 @@
 // under the next tile's MMAs. (Tiles of 384 features, 18% fewer bytes per product, were no faster: the MMAs bound them too,
 // and they fill whole rounds of the pairs less often.)
 //
+// 8192 x 4096 x 28672 takes 386 us in a burst (5.0 PFLOP/s) and 453 at the clock that 1 kW sustains (1.45 GHz); zeros, which
+// cost less power, reach 7.1 PFLOP/s.
+//
 // The grid is persistent over tiles, in strips of kStrip row tiles so that the tiles in flight share operands in L2. Every
 // wait is bounded (common.cuh).
 #include <algorithm>
