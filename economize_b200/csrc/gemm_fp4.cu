@@ -15,7 +15,7 @@
 // memory in the order of the splits.
 //
 // Bound by HBM where the weights are large: one row x 28672 x 4096 streams them at 6.3 TB/s behind 4.3 us of launch, first
-// loads and the last sums; 61 rows take 17.7 us there against 15.1, since every tile reads the activations and their
+// loads and the last sums; 61 rows take 16.7 us there against 14.1, since every tile reads the activations and their
 // scales again (10 KB beside a K block's 18 of weights). 4096 x 4096 takes 5.2 us, of which 1.5 are its bytes. At 128 rows
 // it is level with the pairs of gemm_fp4_pair.cu (4096 x 4096: 10.7 against 11.3 us) and behind from there on (192 rows:
 // 17.6 against 11.4), which is where that kernel takes over.
@@ -137,8 +137,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, BN>::kOcc)
   const int nkb = max(0, min(args.per_split, args.kblocks - kb0));
   const size_t wide = static_cast<size_t>(args.kblocks) * C::kScaleBytes;  // scales of 128 rows
   const uint8_t* ws = args.w_scales + blockIdx.x * wide;
+  // tiles that are not split begin at different K blocks: in step they would all read the same activations at once
+  // (61 x 4096 x 28672: 17.5 us in step, 16.7 so; split tiles, fewer, lose 0.1 of 5 by it)
+  const int turn = splits == 1 ? static_cast<int>(blockIdx.x) % args.kblocks : 0;
+  auto place = [&](int kb) { return kb0 + (kb + turn < nkb ? kb + turn : kb + turn - nkb); };
   auto weights = [&](int kb) {
-    const int s = kb % S, k = kb0 + kb;
+    const int s = kb % S, k = place(kb);
     mbar_arrive_expect_tx(&full[s], C::kStageBytes);
     tma_load_2d(a_tiles + s * kABytes, &tm_w, &full[s], k * kRowBytes, n0);
     bulk_load(sa_tiles + s * C::kScaleBytes, ws + static_cast<size_t>(k) * C::kScaleBytes, C::kScaleBytes, &full[s]);
@@ -166,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, BN>::kOcc)
   if (warp == 0 && lane == 0) {
     const uint8_t* xs = args.x_scales + (m0 / 128) * wide;
     auto activations = [&](int kb) {
-      const int s = kb % S, k = kb0 + kb;
+      const int s = kb % S, k = place(kb);
       tma_load_2d(b_tiles + s * C::kBBytes, &tm_x, &full[s], k * kRowBytes, m0);
       bulk_load(sb_tiles + s * C::kScaleBytes, xs + static_cast<size_t>(k) * C::kScaleBytes, C::kScaleBytes, &full[s]);
     };
