@@ -45,6 +45,19 @@ __device__ __forceinline__ int row_exponent(float amax) {
   return min(max(e, -100), 120);
 }
 
+// A row's power of two r as two factors, for a product with another row's power of two w: (sum first) w last. Sums lie
+// between 2^-20 (the smallest product) and 2^40 (6 x 448 squared, 65536 columns), r and w between 2^-100 and 2^117, so r w
+// may leave fp32's range on either side, and sum r beyond 2^127, where the result does not. So what lies in between here
+// does not: with r up to 2^64, sum r is between 2^-120 and 2^104; a larger r comes after w, where it only moves what is
+// at least 2^-120 up.
+struct RowFactors {
+  float first, last;
+};
+__device__ __forceinline__ RowFactors row_factors(float r) {
+  const bool large = r > 18446744073709551616.f;  // 2^64
+  return {large ? 1.f : r, large ? r : 1.f};
+}
+
 // ---- vectors of packed bf16 ----------------------------------------------------------------------------------------
 // 32 bytes (16 bf16) from a 32-byte boundary.
 __device__ __forceinline__ void load32(const void* p, uint32_t* v) {

@@ -267,9 +267,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, BN>::kOcc)
           sum.w += p[r].w;
         }
       }
-      const float rx = FMT == kNv ? x_row[j] : 1.f;
-      const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x * (rx * rw.x), sum.y * (rx * rw.y));
-      const __nv_bfloat162 hi = __floats2bfloat162_rn(sum.z * (rx * rw.z), sum.w * (rx * rw.w));
+      if constexpr (FMT == kNv) {
+        const RowFactors rx = row_factors(x_row[j]);
+        sum.x = sum.x * rx.first * rw.x * rx.last;
+        sum.y = sum.y * rx.first * rw.y * rx.last;
+        sum.z = sum.z * rx.first * rw.z * rx.last;
+        sum.w = sum.w * rx.first * rw.w * rx.last;
+      }
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x, sum.y);
+      const __nv_bfloat162 hi = __floats2bfloat162_rn(sum.z, sum.w);
       bf16* out = args.y + static_cast<size_t>(m0 + j) * args.N + n;
       if (args.N % 4 == 0) {
         if (n < args.N)

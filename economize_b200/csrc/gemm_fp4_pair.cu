@@ -276,7 +276,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     uint32_t tile = 0;
     for (int t = pair_id; t < tiles.total; t += pairs, ++tile) {
-      const __nv_bfloat162 rx2 = __float2bfloat162_rn(rx);
+      const RowFactors rf = row_factors(rx);
+      const uint64_t rx_first = pair_of(rf.first, rf.first), rx_last = pair_of(rf.last, rf.last);
       if constexpr (FMT == kNv) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) features[i * 32 + lane] = __float2bfloat16(rw[i]);
@@ -298,7 +299,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        // a lane's 32 columns, rounded to bf16 and then multiplied by the powers of two, into its row of a patch
+        // a lane's 32 columns, times the powers of two and rounded once, into its row of a patch
         uint8_t* to = patch + (g & 1) * kPatchBytes;
         if (whole_rows) {
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
@@ -309,11 +310,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           __nv_bfloat162 out[4];
           uint4 w = make_uint4(0, 0, 0, 0);
           if constexpr (FMT == kNv) w = *reinterpret_cast<const uint4*>(features + g * 32 + j * 8);
-          const __nv_bfloat162* w2 = reinterpret_cast<const __nv_bfloat162*>(&w);
+          const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&w);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            out[i] = __floats2bfloat162_rn(v[g * 32 + j * 8 + 2 * i], v[g * 32 + j * 8 + 2 * i + 1]);
-            if constexpr (FMT == kNv) out[i] = __hmul2(__hmul2(out[i], rx2), w2[i]);
+            float lo = v[g * 32 + j * 8 + 2 * i], hi = v[g * 32 + j * 8 + 2 * i + 1];
+            if constexpr (FMT == kNv) {
+              const uint64_t y = mul2(mul2(pair_of(lo, hi), rx_first), pair_of(low_bf16(w2[i]), high_bf16(w2[i])));
+              packed::unpair(mul2(y, rx_last), lo, hi);
+            }
+            out[i] = __floats2bfloat162_rn(lo, hi);
           }
           *reinterpret_cast<uint4*>(to + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = *reinterpret_cast<uint4*>(out);
         }

@@ -290,3 +290,29 @@ def test_long_offsets(cuda):
     _check_product(x[-3:], w, "nvfp4", ops.linear(q, FP4Weight.from_weight(w))[-3:])
     d = q.dequantize()
     assert torch.equal(d[-3:], tail.dequantize()) and not d[:-3].any()
+
+
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("rows,out", [(3, 8), (129, 257), (300, 64)])
+def test_rows_of_any_magnitude(cuda, path, rows, out):
+    """Rows and weights near either end of what nvfp4's powers of two reach, against rows of the other end and their own,
+    on both kernels: results inside bf16's range are right although one row's power alone, or both together, would leave
+    it, those beyond it are infinite, and sums of zero are zero. Every sum is exact in fp32 (64 equal terms of 12 bits, all
+    of one sign or half of them of the other), so the result is rounded once, from what fp32 holds: below bf16's normal
+    range that is off by half its smallest spacing and half of fp32's."""
+    cols = 64
+    e = torch.tensor([-110, -97, -89, -52, -20, 0, 33, 60, 75, 90, 101, 115, 120], device=cuda)
+    ex, ew = e[torch.arange(rows, device=cuda) * 6 % 13], e[torch.arange(out, device=cuda) * 5 % 13]
+    for signs in (1, 2):
+        x = torch.exp2(ex.double())[:, None].expand(rows, cols).clone()
+        x[:, ::2] *= -1 if signs == 2 else 1
+        w = torch.exp2(ew.double())[:, None].expand(out, cols)
+        a, b = ops.fp4_quantize(x.bfloat16(), "nvfp4"), FP4Weight.from_weight(w.bfloat16())
+        y = ops.require().fp4_matmul(a.data, rows, cols, b.codes, b.scales, b.row_scale, 1, path)
+        want = _values(x, "nvfp4") @ _values(w, "nvfp4").t()
+        normal = want.abs() >= torch.finfo(torch.bfloat16).smallest_normal
+        assert torch.equal(y[normal].double(), want.float().bfloat16().double()[normal])
+        off = (y.double() - want).abs()
+        assert (off[~normal] <= 2.0 ** -134 + 2.0 ** -150).all()
+        assert not y.isnan().any() and (signs == 2 or y.isinf().any() and (y == 0).any())
+        assert signs == 1 or not y.any()
