@@ -10,8 +10,9 @@
 // other fp32 rows element by element.
 //
 // Forward two rows are read and two written per token: 8192 rows of 4096 in bf16 take 39 us, 6.9 TB/s, bound by HBM (6.3 at
-// 8192 columns). Backward up to four are read and two written: 53 us from the stream (5.0 TB/s, and 6 to add up the blocks'
-// sums), 108 with both norms (3.7 TB/s), where half of all issue slots and two barriers a row stand against 16 warps an SM.
+// 8192 columns). Backward four are read and up to two written. In a CUDA graph, with the 6 us that add up the blocks' sums:
+// 69 us where x's and the residual's gradients are one tensor (5.3 TB/s without the sums), 77 where they are two, 101 with
+// both norms (4.2 TB/s), where half of all issue slots and two barriers a row stand against 16 warps an SM.
 // In 4 bits the quantisation's instructions bound it: 4096 rows of 4096 with both norms take 29 us, 3.8 TB/s, 65% of the
 // issue slots. Sums, products and roundings work on pairs of columns (f32x2): with single ones the last took 34 us.
 //
@@ -460,7 +461,7 @@ struct SharedWeights {
 };
 
 // Persistent like the forward kernel. A block's sums for dweight and dpost go to its row of a.dw_part / a.dpost_part (fp32
-// [blocks, hidden]). WHOLE: the stream is given in place of x and the residual.
+// [blocks, hidden]). WHOLE: the stream is given in place of x and the residual (fp32).
 template <typename T, int VEC, int NV, bool POST, bool WHOLE, int THREADS, int BLOCKS, int DEPTH>
 __global__ void __launch_bounds__(THREADS, BLOCKS)
     block_norm_bwd_kernel(const __grid_constant__ BlockNormGrads a, int warps) {
@@ -774,9 +775,8 @@ Grid backward_grid(int hidden, bool vec) {
 // Three blocks of 256 threads to an SM from the stream, two from x and the residual, which takes more registers.
 template <typename T>
 int backward_blocks(const Grid& g, int rows, int sms, bool vec, bool whole) {
-  const bool words = !vec && sizeof(T) == 2;
-  const int resident = g.threads > 256 ? 1 : (vec || words) && whole ? 3 : 2;
-  return blocks_for(g, rows, sms * resident, words);
+  const int resident = g.threads > 256 ? 1 : vec && whole ? 3 : 2;
+  return blocks_for(g, rows, sms * resident, !vec && sizeof(T) == 2);
 }
 
 template <typename T, int VEC, int NV, bool POST, bool WHOLE, int THREADS, int BLOCKS, int DEPTH>
@@ -794,8 +794,7 @@ int run_backward_whole(const BlockNormGrads& a, const Grid& g, int blocks, cudaS
   if (g.threads <= 256) return go_backward<T, V, 2, false, true, 256, 3, 2>(a, g, blocks, stream);
   if (g.threads <= 512) return go_backward<T, V, 2, false, true, 512, 1, 2>(a, g, blocks, stream);
   if (g.nv <= 2) return go_backward<T, V, 2, false, true, 1024, 1, 2>(a, g, blocks, stream);
-  if constexpr (sizeof(T) == 4) return go_backward<T, V, 4, false, true, 1024, 1, 1>(a, g, blocks, stream);
-  return -1;
+  return go_backward<T, V, 4, false, true, 1024, 1, 1>(a, g, blocks, stream);
 }
 
 template <typename T, bool POST>
@@ -816,30 +815,34 @@ int run_backward_single(const BlockNormGrads& a, const Grid& g, int blocks, cuda
   return go_backward<T, 1, 16, !WHOLE, WHOLE, 1024, 1, 0>(a, g, blocks, stream);
 }
 
-template <typename T, bool POST, bool WHOLE>
+template <typename T, bool POST>
 int run_backward_words(const BlockNormGrads& a, const Grid& g, int blocks, cudaStream_t stream) {
-  if (g.threads > 512) return go_backward<T, 2, 8, POST, WHOLE, 1024, 1, 1>(a, g, blocks, stream);
-  if (g.threads > 256) return go_backward<T, 2, 8, POST, WHOLE, 512, 1, 2>(a, g, blocks, stream);
-  if (g.nv > 4) return go_backward<T, 2, 8, POST, WHOLE, 256, WHOLE ? 3 : 2, 2>(a, g, blocks, stream);
-  return go_backward<T, 2, 4, POST, WHOLE, 256, WHOLE ? 3 : 2, 2>(a, g, blocks, stream);
+  if (g.threads > 512) return go_backward<T, 2, 8, POST, false, 1024, 1, 1>(a, g, blocks, stream);
+  if (g.threads > 256) return go_backward<T, 2, 8, POST, false, 512, 1, 2>(a, g, blocks, stream);
+  if (g.nv > 4) return go_backward<T, 2, 8, POST, false, 256, 2, 2>(a, g, blocks, stream);
+  return go_backward<T, 2, 4, POST, false, 256, 2, 2>(a, g, blocks, stream);
 }
 
 template <typename T>
 int run_backward_type(const BlockNormGrads& a, bool vec, int sms, cudaStream_t stream) {
   const bool whole = a.stream != nullptr;
+  if (whole && sizeof(T) != 4) return -1;
   const Grid g = backward_grid<T>(a.hidden, vec);
   const int blocks = backward_blocks<T>(g, a.rows, sms, vec, whole);
   int rc;
-  if (vec)
+  if constexpr (sizeof(T) == 2) {
+    if (vec)
+      rc = a.post != nullptr ? run_backward<T, true>(a, g, blocks, stream) : run_backward<T, false>(a, g, blocks, stream);
+    else
+      rc = a.post != nullptr ? run_backward_words<T, true>(a, g, blocks, stream)
+                             : run_backward_words<T, false>(a, g, blocks, stream);
+  } else if (vec) {
     rc = whole               ? run_backward_whole<T>(a, g, blocks, stream)
          : a.post != nullptr ? run_backward<T, true>(a, g, blocks, stream)
                              : run_backward<T, false>(a, g, blocks, stream);
-  else if constexpr (sizeof(T) == 2)
-    rc = whole               ? run_backward_words<T, false, true>(a, g, blocks, stream)
-         : a.post != nullptr ? run_backward_words<T, true, false>(a, g, blocks, stream)
-                             : run_backward_words<T, false, false>(a, g, blocks, stream);
-  else
+  } else {
     rc = whole ? run_backward_single<T, true>(a, g, blocks, stream) : run_backward_single<T, false>(a, g, blocks, stream);
+  }
   if (rc != 0 || (a.dweight == nullptr && a.dpost == nullptr)) return rc;
   return launch_pdl(block_norm_sum_kernel<T>, dim3((a.hidden + 31) / 32, a.dpost != nullptr ? 2 : 1), dim3(1024), 0, stream,
                     static_cast<const float*>(a.dw_part), static_cast<const float*>(a.dpost_part),

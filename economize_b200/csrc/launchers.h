@@ -280,7 +280,7 @@ struct BlockNormGrads {
   const void* dstream = nullptr;  // or null
   const void* x = nullptr;
   const void* residual = nullptr;
-  const void* stream = nullptr;  // without post norm and gate: the rounded stream in place of x and residual
+  const void* stream = nullptr;  // fp32 without post norm and gate: the stream in place of x and residual
   const void* weight = nullptr;
   const void* post = nullptr;
   const void* gate = nullptr;

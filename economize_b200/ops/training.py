@@ -116,9 +116,9 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Ten
 
     All operands have one type (under bf16 autocast they are cast). Sums and what lies between are fp32; ``stream`` and
     ``normed`` are rounded once each, so ``normed`` is the norm of the unrounded stream (unlike two calls of
-    :func:`~economize_b200.ops.rmsnorm`, which round in between as Hugging Face's modules do). Without ``post_weight`` and
-    ``gate`` the gradients are taken from the rounded stream, and with ``scale=1`` those of ``x`` and ``residual`` are one
-    tensor. A call captured into a CUDA graph with its backward pass needs leaves that no living graph of the default
+    :func:`~economize_b200.ops.rmsnorm`, which round in between as Hugging Face's modules do). Gradients are taken from the
+    unrounded stream, which the backward pass forms again from ``x`` and ``residual``; without ``post_weight`` and
+    ``gate`` and with ``scale=1`` those of ``x`` and ``residual`` are one tensor. A call captured into a CUDA graph with its backward pass needs leaves that no living graph of the default
     stream holds, and is refused otherwise.
     """
     if x.is_cuda:  # the checks are the extension's, in C++

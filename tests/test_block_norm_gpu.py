@@ -417,3 +417,31 @@ def test_rows_that_share_words(cuda, dtype, rows, hidden):
         for a, b in zip((*got, again[0], again[1], again[4]), (*want, grads[0], grads[1], grads[4])):
             assert torch.equal(a[others], b[others])
         assert not got[0][rows // 2].isfinite().any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,hidden", [(16, 4096), (3, 1001), (700, 520), (5, 16384)])
+def test_gradients_take_the_unrounded_stream(cuda, dtype, rows, hidden):
+    """Without a norm behind the block and a gate too, nothing but the results is rounded to the operands' type: with one
+    output at a time the bounds hold without the stream's rounding (``half`` of every term of dweight)."""
+    half, tiny = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    for i, (residual, scale) in enumerate(((True, 1.0), (True, 0.22), (False, 1.0))):
+        t, dn, _ = _make(cuda, rows, hidden, dtype, False, "none", residual, seed=110 + i, grad=True)
+        normed, stream = _call(t, scale, 1e-5)
+        leaves = [t["weight"], t["x"]] + ([t["residual"]] if residual else [])
+        dw, dx, *dr = torch.autograd.grad(normed, leaves, dn)
+        with torch.no_grad():
+            x, w, g = t["x"].double(), t["weight"].double(), dn.double()
+            s = scale * x + (t["residual"].double() if residual else 0.0)
+            mag = abs(scale) * x.abs() + (t["residual"].double().abs() if residual else 0.0)
+            inv = torch.rsqrt(s.square().mean(-1, keepdim=True) + 1e-5)
+            sh, sh_err = s * inv, mag * inv * 2 * F32
+            want = (g * sh).sum(0)
+            err = (g.abs() * sh_err).sum(0) + (g * sh).abs().sum(0) * (rows * 2.0 ** -24 + F32)
+            _within(dw, (want, want.abs() * half * 1.01 + err + tiny), "dweight")
+            m = (g * w * sh).mean(-1, keepdim=True)
+            m_err = (g * w * sh).abs().mean(-1, keepdim=True) * F32 + ((g * w).abs() * sh_err).mean(-1, keepdim=True)
+            ds = inv * (g * w - sh * m)
+            err = inv * ((g * w).abs() + (sh * m).abs()) * 2 * F32 + inv * (sh_err * m.abs() + (sh.abs() + sh_err) * m_err)
+            for got, f in ((dx, scale), *((d, 1.0) for d in dr)):
+                _within(got, (f * ds, abs(f) * (ds.abs() * half * 1.01 + err) + tiny), "dx or dresidual")
