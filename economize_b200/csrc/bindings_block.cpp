@@ -4,6 +4,7 @@
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 
 #include <cmath>
 #include <cstring>
@@ -558,11 +559,13 @@ struct BlockNormFunction : torch::autograd::Function<BlockNormFunction> {
 
 // A leaf's gradients are added up on the stream of the first graph that holds the leaf. Where that is the default stream,
 // which cannot join a capture, and that graph still lives, the engine would break off the captured backward pass, and the
-// process with it.
+// process with it. An operand is often not the leaf itself but its rows, a view or a cast of it (as_rows, autocast): its
+// history is followed as long as it has one input.
 void check_captured_leaf(const Tensor& t) {
-  if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
-  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-  if (!node) return;
+  if (!t.defined() || !t.requires_grad()) return;
+  auto node = t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn();
+  while (node && node->num_outputs() == 1) node = node->next_edge(0).function;
+  if (!node || dynamic_cast<torch::autograd::AccumulateGrad*>(node.get()) == nullptr) return;
   const auto stream = node->stream();
   TORCH_CHECK(!stream.has_value() || c10::cuda::CUDAStream(*stream) != c10::cuda::getDefaultCUDAStream(t.get_device()),
               "block_norm: a graph made on the default stream still holds a leaf of this captured call, whose backward "

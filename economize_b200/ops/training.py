@@ -118,8 +118,8 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Ten
     ``normed`` are rounded once each, so ``normed`` is the norm of the unrounded stream (unlike two calls of
     :func:`~economize_b200.ops.rmsnorm`, which round in between as Hugging Face's modules do). Gradients are taken from the
     unrounded stream, which the backward pass forms again from ``x`` and ``residual``; without ``post_weight`` and
-    ``gate`` and with ``scale=1`` those of ``x`` and ``residual`` are one tensor. A call captured into a CUDA graph with its backward pass needs leaves that no living graph of the default
-    stream holds, and is refused otherwise.
+    ``gate`` and with ``scale=1`` those of ``x`` and ``residual`` are one tensor. A call captured into a CUDA graph with its backward pass needs leaves that no living graph of the
+    default stream holds; where an operand is such a leaf, or a view or a cast of one, the call is refused.
     """
     if x.is_cuda:  # the checks are the extension's, in C++
         if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:

@@ -445,3 +445,29 @@ def test_gradients_take_the_unrounded_stream(cuda, dtype, rows, hidden):
             err = inv * ((g * w).abs() + (sh * m).abs()) * 2 * F32 + inv * (sh_err * m.abs() + (sh.abs() + sh_err) * m_err)
             for got, f in ((dx, scale), *((d, 1.0) for d in dr)):
                 _within(got, (f * ds, abs(f) * (ds.abs() * half * 1.01 + err) + tiny), "dx or dresidual")
+
+
+@pytest.mark.parametrize("form", ["three dimensions", "autocast", "view", "autocast weight"])
+def test_capture_beside_a_living_graph_of_views_and_casts(cuda, form):
+    """The operands of a captured call are refused like leaves where they are views or casts of leaves that a graph of the
+    default stream holds, and taken once that graph is gone. (Only the forward pass is captured beside the graph.)"""
+    dtype = torch.float32 if form.startswith("autocast") else torch.bfloat16
+    leaf = torch.randn(2, 5, 64, device=cuda).to(dtype).requires_grad_(form != "autocast weight")
+    weight = torch.ones(64, device=cuda, dtype=dtype, requires_grad=form == "autocast weight")
+
+    def call():
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=form.startswith("autocast")):
+            return ops.block_norm(leaf.view(10, 64) if form == "view" else leaf, None, weight)[0]
+
+    living = call()
+    (want,) = torch.autograd.grad(living.sum(), leaf if leaf.requires_grad else weight, retain_graph=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with pytest.raises(RuntimeError, match="still holds a leaf"), torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+        call()
+    del living
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        (got,) = torch.autograd.grad(call().sum(), leaf if leaf.requires_grad else weight)
+    graph.replay()
+    assert torch.equal(got, want)
