@@ -238,7 +238,7 @@ class FP4Weight(nn.Module):
             raise ConfigError(f"scales {tuple(scales.shape)} and {tuple(row_scale.shape)} do not belong to {fmt} codes "
                               f"{tuple(codes.shape)}")
         self.compute_dtype = dtype
-        # copies of their own: products fetch them ahead, which an operator's fresh result does not allow
+        # copies of their own, not views of an operator's buffer
         self.register_buffer("codes", codes.detach().clone(memory_format=torch.contiguous_format))
         self.register_buffer("scales", scales.detach().clone(memory_format=torch.contiguous_format))
         self.register_buffer("row_scale", row_scale.detach().float().clone(memory_format=torch.contiguous_format))

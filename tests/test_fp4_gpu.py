@@ -316,3 +316,41 @@ def test_rows_of_any_magnitude(cuda, path, rows, out):
         assert (off[~normal] <= 2.0 ** -134 + 2.0 ** -150).all()
         assert not y.isnan().any() and (signs == 2 or y.isinf().any() and (y == 0).any())
         assert signs == 1 or not y.any()
+
+
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("rows", [1, 61, 200])
+def test_weight_written_between_products(cuda, fmt, rows):
+    """A weight written in place directly in front of a product, and one kernel before it, is what the product reads, in a
+    captured sequence too: nothing of it is taken from what was there before."""
+    x = _normal(cuda, rows, 2048, seed=21)
+    q = ops.fp4_quantize(x, fmt)
+    sources = [FP4Weight.from_weight(_normal(cuda, 1536, 2048, seed=s), fmt) for s in (22, 23, 24)]
+    want = [ops.linear(q, s) for s in sources]
+    w = FP4Weight.from_weight(_normal(cuda, 1536, 2048, seed=25), fmt)
+
+    def sequence():
+        out = []
+        for s in sources:
+            w.row_scale.copy_(s.row_scale)
+            w.scales.copy_(s.scales)
+            w.codes.copy_(s.codes)
+            out.append(ops.linear(q, w))  # codes directly in front of the product
+        for s in sources:
+            w.row_scale.copy_(s.row_scale)
+            w.codes.copy_(s.codes)
+            w.scales.copy_(s.scales)
+            out.append(ops.linear(x, w))  # scales in front of the quantisation in front of the product
+        return out
+
+    for _ in range(10):
+        assert all(torch.equal(a, b) for a, b in zip(sequence(), want + want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = sequence()
+    for _ in range(10):
+        for o in out:
+            o.zero_()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, want + want))
+    assert ops.require().status(0) == 0
