@@ -186,9 +186,10 @@ struct Rows {
   __device__ __forceinline__ uint32_t plane(int s, int op, int i) const {
     return base + static_cast<uint32_t>((s * kSlotPlanes + op * NV + i) * block_threads<THREADS>() * kEntry);
   }
-  // start the copy of operand op's row (zeros for null) into slot s
+  // start the copy of operand op's row (zeros for null) into slot s. Where nothing is copied the source is `spare`, a row of
+  // the call: an address behind a row's end, or counted from a null row (in words an odd one), would not be a valid one.
   template <class Place>
-  __device__ __forceinline__ void start(int s, int op, const T* row, const Place& place, int hidden) {
+  __device__ __forceinline__ void start(int s, int op, const T* row, const Place& place, int hidden, const T* spare) {
     if constexpr (kAhead) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -196,10 +197,11 @@ struct Rows {
         const uint32_t to = plane(s, op, i);
         int bytes = row != nullptr && at < hidden ? kEntry : 0;  // the rest of the entry becomes zero
         if constexpr (VEC == 2) bytes = at + 1 == hidden ? bytes / 2 : bytes;
+        const T* from = bytes > 0 ? row + at : spare;
         if constexpr (kEntry == 16)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(row + at), "r"(bytes) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
         else
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(row + at), "r"(bytes) : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
       }
     } else {
       ptr[op] = row;
@@ -340,8 +342,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   constexpr int kPairs = (VEC + 1) / 2;
   auto start = [&](int slot, int row) {
     const bool on = row < a.rows;
-    rows.start(slot, 0, on ? xp + row * a.x_stride : nullptr, team, hidden);
-    rows.start(slot, 1, on && rp != nullptr ? rp + row * a.r_stride : nullptr, team, hidden);
+    rows.start(slot, 0, on ? xp + row * a.x_stride : nullptr, team, hidden, xp);
+    rows.start(slot, 1, on && rp != nullptr ? rp + row * a.r_stride : nullptr, team, hidden, xp);
     rows.commit();
   };
   pdl_wait();
@@ -485,10 +487,11 @@ __global__ void __launch_bounds__(THREADS, BLOCKS)
   const int64_t r_stride = WHOLE ? hidden : a.r_stride;
   auto start = [&](int slot, int row) {
     const bool on = row < a.rows;
-    rows.start(slot, 0, on && np != nullptr ? np + row * a.dn_stride : nullptr, team, hidden);
-    rows.start(slot, 1, on && up != nullptr ? up + row * a.ds_stride : nullptr, team, hidden);
-    rows.start(slot, 2, on && rp != nullptr ? rp + row * r_stride : nullptr, team, hidden);
-    if constexpr (!WHOLE) rows.start(slot, 3, on ? xp + row * a.x_stride : nullptr, team, hidden);
+    const T* spare = WHOLE ? rp : xp;
+    rows.start(slot, 0, on && np != nullptr ? np + row * a.dn_stride : nullptr, team, hidden, spare);
+    rows.start(slot, 1, on && up != nullptr ? up + row * a.ds_stride : nullptr, team, hidden, spare);
+    rows.start(slot, 2, on && rp != nullptr ? rp + row * r_stride : nullptr, team, hidden, spare);
+    if constexpr (!WHOLE) rows.start(slot, 3, on ? xp + row * a.x_stride : nullptr, team, hidden, spare);
     rows.commit();
   };
   pdl_wait();

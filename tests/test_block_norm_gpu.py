@@ -471,3 +471,20 @@ def test_capture_beside_a_living_graph_of_views_and_casts(cuda, form):
         (got,) = torch.autograd.grad(call().sum(), leaf if leaf.requires_grad else weight)
     graph.replay()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,hidden", [(1, 5), (7, 1001), (1300, 333), (2500, 77), (600, 4095), (9, 200)])
+def test_operands_that_are_not_there(cuda, dtype, rows, hidden):
+    """A residual or an upstream gradient that is not given is one of zeros, bit for bit: rows copied ahead, those behind
+    the last and odd ones that start in the middle of a word among them."""
+    for post, gate in ((False, "none"), (True, "token"), (False, "full")):
+        t, dn, up = _make(cuda, rows, hidden, dtype, post, gate, False, seed=120, grad=True)
+        zeros = torch.zeros(rows, hidden, device=cuda, dtype=dtype)
+        leaves = [v for v in t.values() if v is not None]
+        without, given = _call(t, 0.5, 1e-5), _call({**t, "residual": zeros}, 0.5, 1e-5)
+        assert all(torch.equal(a, b) for a, b in zip(without, given))
+        for i, g in ((0, dn), (1, up)):
+            alone = torch.autograd.grad(without[i], leaves, g, retain_graph=True)
+            both = torch.autograd.grad(given, leaves, (g, zeros) if i == 0 else (zeros, g), retain_graph=True)
+            assert all(torch.equal(a, b) for a, b in zip(alone, both))
