@@ -407,32 +407,6 @@ NormCall norm_call(const Tensor& x, const c10::optional<Tensor>& residual, const
   return c;
 }
 
-// normed in 4 bits (a buffer), and the stream.
-std::tuple<Tensor, Tensor> block_norm_fp4(const Tensor& x, const c10::optional<Tensor>& residual, const Tensor& weight,
-                                          const c10::optional<Tensor>& post, const c10::optional<Tensor>& gate,
-                                          double scale, double eps, int64_t fmt) {
-  check_format(fmt);
-  CHECK_CUDA(x);
-  TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16, "block_norm in 4 bits takes bfloat16, got ", x.scalar_type());
-  const NormCall c = norm_call(x, residual, post, gate);
-  check_columns(x.size(-1), "block_norm in 4 bits");
-  c10::cuda::CUDAGuard guard(x.device());
-  const NormOperands o = norm_operands(c.x, c.residual, weight, c.post, c.gate, scale, eps);
-  Fp4 to = fp4_shape(c.x.size(0), c.x.size(1), fmt);
-  Tensor data = fp4_buffer(to, x), stream = at::empty(x.sizes(), x.options());
-  if (to.rows == 0) return {data, stream};
-  ecz::BlockNormArgs a = norm_args(o, scale, eps);
-  a.stream = stream.data_ptr();
-  a.codes = to.codes;
-  a.scales = to.scales;
-  a.row_scale = to.row_scale;
-  a.tiles = static_cast<int>(to.tiles);
-  TORCH_CHECK(ecz::launch_block_norm(a, ecz::kNormBf16, true, static_cast<int>(fmt), ecz::device_sms(x.get_device()),
-                                     at::cuda::getCurrentCUDAStream()) == 0,
-              "block_norm: launch failed");
-  return {data, stream};
-}
-
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
@@ -571,10 +545,8 @@ void check_captured_leaf(const Tensor& t) {
               "pass could not be captured; drop that graph, or make it on a side stream");
 }
 
-std::tuple<Tensor, Tensor> block_norm(const Tensor& x, const c10::optional<Tensor>& residual, const Tensor& weight,
-                                      const c10::optional<Tensor>& post, const c10::optional<Tensor>& gate, double scale,
-                                      double eps) {
-  const NormCall c = norm_call(x, residual, post, gate);
+// Whether the call becomes part of a graph.
+bool differentiated(const NormCall& c, const Tensor& weight) {
   bool grad = false;
   for (const Tensor* t : {&c.x, &c.residual, &weight, &c.post, &c.gate}) {
     if (!t->defined()) continue;
@@ -583,8 +555,15 @@ std::tuple<Tensor, Tensor> block_norm(const Tensor& x, const c10::optional<Tenso
     TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t->_fw_grad(0).defined(),
                 "block_norm has no forward-mode derivative on CUDA");
   }
+  return grad && at::GradMode::is_enabled();
+}
+
+std::tuple<Tensor, Tensor> block_norm(const Tensor& x, const c10::optional<Tensor>& residual, const Tensor& weight,
+                                      const c10::optional<Tensor>& post, const c10::optional<Tensor>& gate, double scale,
+                                      double eps) {
+  const NormCall c = norm_call(x, residual, post, gate);
   Tensor normed, stream;
-  if (grad && at::GradMode::is_enabled()) {
+  if (differentiated(c, weight)) {
     c10::cuda::CUDAGuard guard(x.device());
     if (at::cuda::currentStreamCaptureStatus() != at::cuda::CaptureStatus::None)
       for (const Tensor* t : {&c.x, &c.residual, &weight, &c.post, &c.gate}) check_captured_leaf(*t);
@@ -599,6 +578,37 @@ std::tuple<Tensor, Tensor> block_norm(const Tensor& x, const c10::optional<Tenso
   }
   if (x.dim() != 2) return {normed.view(x.sizes()), stream.view(x.sizes())};
   return {normed, stream};
+}
+
+// normed in 4 bits (a buffer), and the stream. The 4-bit result has no gradient; where the call is differentiated the
+// stream keeps its own, and the two operators run one after the other, with the same bits.
+std::tuple<Tensor, Tensor> block_norm_fp4(const Tensor& x, const c10::optional<Tensor>& residual, const Tensor& weight,
+                                          const c10::optional<Tensor>& post, const c10::optional<Tensor>& gate,
+                                          double scale, double eps, int64_t fmt) {
+  check_format(fmt);
+  CHECK_CUDA(x);
+  TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16, "block_norm in 4 bits takes bfloat16, got ", x.scalar_type());
+  const NormCall c = norm_call(x, residual, post, gate);
+  check_columns(x.size(-1), "block_norm in 4 bits");
+  c10::cuda::CUDAGuard guard(x.device());
+  if (differentiated(c, weight)) {
+    const auto [normed, stream] = block_norm(x, residual, weight, post, gate, scale, eps);
+    return {fp4_quantize(normed.detach(), fmt), stream};
+  }
+  const NormOperands o = norm_operands(c.x, c.residual, weight, c.post, c.gate, scale, eps);
+  Fp4 to = fp4_shape(c.x.size(0), c.x.size(1), fmt);
+  Tensor data = fp4_buffer(to, x), stream = at::empty(x.sizes(), x.options());
+  if (to.rows == 0) return {data, stream};
+  ecz::BlockNormArgs a = norm_args(o, scale, eps);
+  a.stream = stream.data_ptr();
+  a.codes = to.codes;
+  a.scales = to.scales;
+  a.row_scale = to.row_scale;
+  a.tiles = static_cast<int>(to.tiles);
+  TORCH_CHECK(ecz::launch_block_norm(a, ecz::kNormBf16, true, static_cast<int>(fmt), ecz::device_sms(x.get_device()),
+                                     at::cuda::getCurrentCUDAStream()) == 0,
+              "block_norm: launch failed");
+  return {data, stream};
 }
 
 }  // namespace

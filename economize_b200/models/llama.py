@@ -323,9 +323,15 @@ class CausalLM(nn.Module):
         (:func:`economize_b200.ops.block_norm`)."""
         if self._takes_fp4(layer, weight) and not isinstance(h, ops.Partials):
             scale = self.config.residual_multiplier if partial else 1.0
-            return ops.block_norm(h, resid, norm, scale=scale, eps=self.config.rms_norm_eps, quantize=weight.fmt)
+            return self._norm_fp4(weight, h, resid, norm, scale=scale)
         h, partial = self._scale_branch(h, partial)
         return self._norm(h, norm, resid, partial)
+
+    @torch.no_grad()
+    def _norm_fp4(self, weight, h: torch.Tensor, resid: torch.Tensor | None, norm: torch.Tensor, **kw):
+        """The input of the 4-bit projection ``weight`` and the residual stream (:func:`economize_b200.ops.block_norm`),
+        without a graph like the executor's other kernels."""
+        return ops.block_norm(h, resid, norm, eps=self.config.rms_norm_eps, quantize=weight.fmt, **kw)
 
     def _scale_branch(self, h, partial: bool):
         """A branch output times Granite's residual multiplier before it joins the residual stream (a no-op for
@@ -357,8 +363,7 @@ class CausalLM(nn.Module):
             a = self._materialize(self._attention(layer, i, x, batch, cache, cos, sin), True)
             if sandwich and self._takes_fp4(layer, layer.w_gate_up):
                 # both norms around the residual sum in one kernel, its result in 4 bits
-                x, h = ops.block_norm(a, h, layer.mlp_norm, post_weight=layer.attn_post_norm, eps=eps,
-                                      quantize=layer.w_gate_up.fmt)
+                x, h = self._norm_fp4(layer.w_gate_up, a, h, layer.mlp_norm, post_weight=layer.attn_post_norm)
             else:
                 h = h + ops.rmsnorm(a, layer.attn_post_norm if sandwich else layer.attn_norm, eps)[0]
                 x = ops.rmsnorm(h, layer.mlp_norm, eps)[0] if sandwich else h

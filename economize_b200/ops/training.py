@@ -111,15 +111,16 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Ten
         gate: Per token ``[..., 1]`` or per element ``[..., H]``; ``None``: ungated.
         scale: Factor of what joins the residual.
         quantize: ``"nvfp4"`` or ``"mxfp4"``: ``normed`` comes in 4 bits, as an
-            :class:`~economize_b200.ops.fp4.FP4Tensor` of the bf16 result (bf16 on CUDA, ``H`` a multiple of 32; no
-            gradients).
+            :class:`~economize_b200.ops.fp4.FP4Tensor` of the bf16 result (bf16 on CUDA, ``H`` a multiple of 32) without
+            a gradient; ``stream`` keeps its own. (Where one is asked for, the norm and the quantisation are two kernels.)
 
     All operands have one type (under bf16 autocast they are cast). Sums and what lies between are fp32; ``stream`` and
     ``normed`` are rounded once each, so ``normed`` is the norm of the unrounded stream (unlike two calls of
     :func:`~economize_b200.ops.rmsnorm`, which round in between as Hugging Face's modules do). Gradients are taken from the
     unrounded stream, which the backward pass forms again from ``x`` and ``residual``; without ``post_weight`` and
-    ``gate`` and with ``scale=1`` those of ``x`` and ``residual`` are one tensor. A call captured into a CUDA graph with its backward pass needs leaves that no living graph of the
-    default stream holds; where an operand is such a leaf, or a view or a cast of one, the call is refused.
+    ``gate`` and with ``scale=1`` those of ``x`` and ``residual`` are one tensor. A call captured into a CUDA graph with
+    its backward pass needs leaves that no living graph of the default stream holds; where an operand is such a leaf, or a
+    view or a cast of one, the call is refused.
     """
     if x.is_cuda:  # the checks are the extension's, in C++
         if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:
@@ -147,4 +148,4 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Ten
     if quantize is not None:
         _check_format(quantize)
     normed, stream = reference.block_norm(x, residual, weight, post_weight, gate, float(scale), float(eps))
-    return (normed, stream) if quantize is None else (fp4_quantize(normed, quantize), stream.detach())
+    return (normed, stream) if quantize is None else (fp4_quantize(normed, quantize), stream)

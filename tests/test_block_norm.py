@@ -141,3 +141,36 @@ def test_packed_training_of_scaled_residuals_on_the_kernels(cuda):
     fit(em, PackedSource([d.to(cuda) for d in docs], 512, seed=2), objective="packed_recovery_ce", steps=3, warmup_steps=1,
         log_every=100)
     assert ops.require().status(0) == 0
+
+
+def _stream_gradients(x, r, w, p, gate, dev="cpu"):
+    """Of a 4-bit call and of the plain one: results and the stream's gradients."""
+    out = []
+    for kw in ({}, {"quantize": "mxfp4"}):
+        leaves = [t.to(dev).bfloat16().requires_grad_() for t in (x, r, w, p, gate)]
+        normed, stream = ops.block_norm(leaves[0], leaves[1], leaves[2], post_weight=leaves[3], gate=leaves[4], scale=0.5, **kw)
+        up = torch.linspace(-1, 1, stream.numel(), device=dev).view_as(stream).bfloat16()
+        grads = torch.autograd.grad(stream, [leaves[i] for i in (0, 1, 3, 4)], up)
+        out.append((normed, stream, grads))
+    (n, s, g), (q, s4, g4) = out
+    assert torch.equal(s, s4) and torch.equal(ops.fp4_quantize(n.detach(), "mxfp4").codes, q.codes)
+    assert all(torch.equal(a, b) for a, b in zip(g, g4))
+    with torch.no_grad():
+        q, s = ops.block_norm(*leaves[:3], post_weight=leaves[3], gate=leaves[4], scale=0.5, quantize="mxfp4")
+    assert not s.requires_grad and torch.equal(s, s4) and torch.equal(q.codes, out[1][0].codes)
+
+
+def test_the_stream_of_a_four_bit_call_keeps_its_gradient():
+    x, r, w, p, token, full = _tensors(hidden=64)
+    _stream_gradients(x, r, w, p, token)
+    _stream_gradients(x, r, w, p, full)
+
+
+@pytest.mark.gpu
+def test_the_stream_of_a_four_bit_call_keeps_its_gradient_on_the_kernels(cuda):
+    x, r, w, p, token, full = _tensors(rows=130, hidden=416)
+    _stream_gradients(x, r, w, p, token, cuda)
+    _stream_gradients(x, r, w, p, full, cuda)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda v: ops.block_norm(v, None, w.to(cuda).bfloat16(), quantize="nvfp4")[1],
+                       (x.to(cuda).bfloat16(),), (x.to(cuda).bfloat16(),))
