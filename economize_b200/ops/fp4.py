@@ -243,6 +243,15 @@ class FP4Weight(nn.Module):
         self.register_buffer("scales", scales.detach().clone(memory_format=torch.contiguous_format))
         self.register_buffer("row_scale", row_scale.detach().float().clone(memory_format=torch.contiguous_format))
 
+    def _apply(self, fn, recurse: bool = True):
+        """Moves like any module's, but a cast leaves the powers of two of the rows as they are: fp32, from 2^-100 on."""
+        row = self.row_scale
+        super()._apply(fn, recurse)
+        moved = self._buffers["row_scale"]
+        if moved.dtype != torch.float32:
+            self._buffers["row_scale"] = row.to(moved.device)
+        return self
+
     @classmethod
     def from_weight(cls, w: torch.Tensor, fmt: str = "nvfp4") -> FP4Weight:
         """``w [N, K]`` rounded to nearest (on CUDA from its bf16 values)."""

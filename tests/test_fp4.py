@@ -171,3 +171,31 @@ def test_norms_hand_over_four_bits(cuda, family):
     apart, wide = em(ids).float(), model(backend="fake")(ids).float()
     assert not torch.equal(fused, apart)
     assert float((fused - wide).norm()) < 1.25 * float((apart - wide).norm()) < 0.75 * float(wide.norm())
+
+
+def _casts(device):
+    x = torch.randn(5, 96, generator=torch.Generator().manual_seed(8)).bfloat16().to(device)
+    for fmt in ("nvfp4", "mxfp4"):
+        w = torch.randn(40, 96, generator=torch.Generator().manual_seed(9)) * torch.exp2(torch.arange(40.0) - 30)[:, None]
+        weight = FP4Weight.from_weight(w.to(device), fmt)
+        want, y = weight.dequantize(torch.float32), ops.linear(x, weight)
+        holder = torch.nn.ModuleDict({"w": weight})
+        for cast in (torch.nn.Module.half, torch.nn.Module.bfloat16, torch.nn.Module.double, torch.nn.Module.float,
+                     lambda m: m.to(device, torch.float16)):
+            cast(holder)
+            assert weight.row_scale.dtype == torch.float32 and weight.codes.dtype == weight.scales.dtype == torch.uint8
+            assert torch.equal(weight.dequantize(torch.float32), want) and torch.equal(ops.linear(x, weight), y)
+        if device != "cpu":
+            assert torch.equal(holder.half().cpu()["w"].dequantize(torch.float32), want.cpu())
+
+
+def test_casts_leave_the_scales_of_rows():
+    _casts("cpu")
+    # from meta to a device that has memory: the values are the caller's to fill, the type is not a cast's to change
+    meta = FP4Weight.from_weight(torch.ones(8, 64)).to("meta").half()
+    assert meta.to_empty(device="cpu").row_scale.dtype == torch.float32
+
+
+@pytest.mark.gpu
+def test_casts_leave_the_scales_of_rows_on_the_kernels(cuda):
+    _casts(cuda)
