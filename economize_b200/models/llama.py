@@ -320,8 +320,11 @@ class CausalLM(nn.Module):
     def _input_norm(self, layer: DecoderLayer, norm: torch.Tensor, weight, h, resid: torch.Tensor | None, partial: bool):
         """The sublayer's input and the residual stream: ``resid`` plus the pending branch output ``h`` (times Granite's
         residual multiplier), normed for the projection ``weight``, in 4 bits where it multiplies in such
-        (:func:`economize_b200.ops.block_norm`)."""
-        if self._takes_fp4(layer, weight) and not isinstance(h, ops.Partials):
+        (:func:`economize_b200.ops.block_norm`). Which of the two norms it is does not depend on how many rows there are:
+        split-K partials of a projection in front, which only few rows leave, are summed first."""
+        if self._takes_fp4(layer, weight):
+            if isinstance(h, ops.Partials):
+                h = ops.rmsnorm(h, norm, self.config.rms_norm_eps)[1]  # their sum as bf16, in one launch
             scale = self.config.residual_multiplier if partial else 1.0
             return self._norm_fp4(weight, h, resid, norm, scale=scale)
         h, partial = self._scale_branch(h, partial)

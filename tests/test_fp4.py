@@ -199,3 +199,30 @@ def test_casts_leave_the_scales_of_rows():
 @pytest.mark.gpu
 def test_casts_leave_the_scales_of_rows_on_the_kernels(cuda):
     _casts(cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 20, 64, 65, 100, 128, 129])
+def test_norms_hand_over_four_bits_at_any_row_count(cuda, rows):
+    """In a partly quantised model a bf16 projection in front of a norm leaves split-K partials up to 64 rows and a plain
+    tensor beyond. The norm is the same on either side: that of the unrounded stream, in 4 bits, bit for bit."""
+    from economize_b200.models.config import tiny_llama
+    from economize_b200.models.llama import CausalLM, init_weights
+
+    cfg = tiny_llama(hidden_size=512, head_dim=128, num_heads=4, num_kv_heads=2, intermediate_size=1024,
+                     residual_multiplier=0.22)
+    em = eco.apply(init_weights(CausalLM(cfg, torch.bfloat16, cuda), seed=0, std=0.05),
+                   QuantConfig(format="nvfp4_w4a4", exclude=("*o_proj", "*down_proj")))
+    lm, g = em.model, torch.Generator(device=cuda).manual_seed(rows)
+    layer = lm.layers[0]
+    assert isinstance(layer.wo, torch.Tensor) and isinstance(layer.w_gate_up, FP4Weight)
+    o, resid = (torch.randn(1, rows, 512, device=cuda, generator=g).bfloat16() for _ in range(2))
+    h = ops.linear_parts(o, layer.wo)
+    assert isinstance(h, ops.Partials) == (rows <= 64)
+    plain = h.sum() if isinstance(h, ops.Partials) else h
+    x, stream = lm._input_norm(layer, layer.mlp_norm, layer.w_gate_up, h, resid, True)
+    with torch.no_grad():
+        normed, want = ops.block_norm(plain, resid, layer.mlp_norm, scale=0.22, eps=cfg.rms_norm_eps)
+    q = ops.fp4_quantize(normed, "nvfp4")
+    assert isinstance(x, ops.FP4Tensor) and torch.equal(stream, want)
+    assert all(torch.equal(a, b) for a, b in zip(x.parts(), q.parts()))
