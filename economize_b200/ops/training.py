@@ -114,18 +114,20 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Ten
             :class:`~economize_b200.ops.fp4.FP4Tensor` of the bf16 result (bf16 on CUDA, ``H`` a multiple of 32) without
             a gradient; ``stream`` keeps its own. (Where one is asked for, the norm and the quantisation are two kernels.)
 
-    All operands have one type (under bf16 autocast they are cast). Sums and what lies between are fp32; ``stream`` and
-    ``normed`` are rounded once each, so ``normed`` is the norm of the unrounded stream (unlike two calls of
-    :func:`~economize_b200.ops.rmsnorm`, which round in between as Hugging Face's modules do). Gradients are taken from the
-    unrounded stream, which the backward pass forms again from ``x`` and ``residual``; without ``post_weight`` and
-    ``gate`` and with ``scale=1`` those of ``x`` and ``residual`` are one tensor. A call captured into a CUDA graph with
-    its backward pass needs leaves that no living graph of the default stream holds; where an operand is such a leaf, or a
-    view or a cast of one, the call is refused.
+    All operands have one type (under bf16 autocast they are cast, under fp16 autocast where their types differ). Sums and
+    what lies between are fp32; ``stream`` and ``normed`` are rounded once each, so ``normed`` is the norm of the unrounded
+    stream (unlike two calls of :func:`~economize_b200.ops.rmsnorm`, which round in between as Hugging Face's modules do).
+    Gradients are taken from the unrounded stream, which the backward pass forms again from ``x`` and ``residual``; without
+    ``post_weight`` and ``gate`` and with ``scale=1`` those of ``x`` and ``residual`` are one tensor. A call captured into a
+    CUDA graph with its backward pass needs leaves that no living graph of the default stream holds; where an operand is
+    such a leaf, or a view or a cast of one, the call is refused.
     """
     if x.is_cuda:  # the checks are the extension's, in C++
-        if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:
-            x, residual, weight, post_weight, gate = (None if t is None else t.to(torch.bfloat16)
-                                                      for t in (x, residual, weight, post_weight, gate))
+        if torch.is_autocast_enabled("cuda"):
+            to, given = torch.get_autocast_dtype("cuda"), (x, residual, weight, post_weight, gate)
+            if to == torch.bfloat16 or to == torch.float16 and quantize is None and \
+                    any(t is not None and t.dtype != x.dtype for t in given):
+                x, residual, weight, post_weight, gate = (None if t is None else t.to(to) for t in given)
         if quantize is None:
             return require().block_norm(x, residual, weight, post_weight, gate, scale, eps)
         _check_format(quantize)

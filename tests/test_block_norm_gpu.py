@@ -488,3 +488,21 @@ def test_operands_that_are_not_there(cuda, dtype, rows, hidden):
             alone = torch.autograd.grad(without[i], leaves, g, retain_graph=True)
             both = torch.autograd.grad(given, leaves, (g, zeros) if i == 0 else (zeros, g), retain_graph=True)
             assert all(torch.equal(a, b) for a, b in zip(alone, both))
+
+
+def test_half_autocast(cuda):
+    """Under fp16 autocast operands of several types, as a projection and an fp32 stream are, run in fp16 and get their
+    gradients in their own types; operands of one type stay as they are, and 4-bit results are made from bf16 alone."""
+    t, dn, up = _make(cuda, 8, 64, torch.float32, True, "token", seed=81, grad=True)
+    x = t["x"].detach().half().requires_grad_()
+    with torch.autocast("cuda", dtype=torch.float16):
+        normed, stream = _call({**t, "x": x}, 1.0, 1e-5)
+        plain = _call(t, 1.0, 1e-5)
+        with pytest.raises(ValueError, match="bfloat16"):
+            ops.block_norm(x, None, t["weight"], quantize="nvfp4")
+    assert normed.dtype == stream.dtype == torch.float16 and plain[0].dtype == torch.float32
+    half = {k: v.detach().half() for k, v in t.items()}
+    assert all(torch.equal(a, b) for a, b in zip((normed, stream), _call(half, 1.0, 1e-5)))
+    leaves = [x] + [t[k] for k in ("residual", "weight", "post_weight", "gate")]
+    grads = torch.autograd.grad((normed, stream), leaves, (dn.half(), up.half()))
+    assert [g.dtype for g in grads] == [torch.float16] + [torch.float32] * 4
