@@ -226,3 +226,54 @@ def test_norms_hand_over_four_bits_at_any_row_count(cuda, rows):
     q = ops.fp4_quantize(normed, "nvfp4")
     assert isinstance(x, ops.FP4Tensor) and torch.equal(stream, want)
     assert all(torch.equal(a, b) for a, b in zip(x.parts(), q.parts()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("family", ["gemma2", "granite", "llama"])
+def test_norms_hand_over_four_bits_exactly(cuda, fmt, family):
+    """The executor's fused norms against passes whose norms and quantisations are two operators, with the family's own
+    multiplier and weights of the norms, at row counts of one token, of a tree and of a prompt: equal bits. A multiplier
+    that is off by a percent is not equal."""
+    from economize_b200.models.config import tiny_llama
+    from economize_b200.models.llama import CausalLM, init_weights
+    from economize_b200.runtime.cache import StepBatch
+
+    extra = {"gemma2": dict(sandwich_norm=True), "granite": dict(residual_multiplier=0.22), "llama": {}}[family]
+    cfg = tiny_llama(hidden_size=512, head_dim=128, num_heads=4, num_kv_heads=2, intermediate_size=1024, **extra)
+    lm = eco.apply(init_weights(CausalLM(cfg, torch.bfloat16, cuda), seed=0, std=0.05),
+                   QuantConfig(format=fmt + "_w4a4")).model
+    g = torch.Generator(device=cuda).manual_seed(3)
+    with torch.no_grad():
+        for layer in lm.layers:  # norms that differ, so that one taken for another shows
+            for name in ("attn_norm", "mlp_norm", "attn_post_norm", "mlp_post_norm"):
+                p = getattr(layer, name, None)
+                if p is not None:
+                    p.copy_(1 + 0.3 * torch.randn(p.shape, device=cuda, generator=g))
+
+    @torch.no_grad()
+    def hidden(rows):
+        ids = torch.randint(0, 1024, (1, rows), generator=torch.Generator().manual_seed(rows)).to(cuda)
+        return lm.forward_step(ids, StepBatch.prefill(torch.tensor([rows], dtype=torch.int32, device=cuda), rows),
+                               lm.new_cache(1, 256))[0]
+
+    def input_norm(layer, norm, weight, h, resid, partial, multiplier=extra.get("residual_multiplier", 1.0)):
+        assert isinstance(weight, FP4Weight)  # the embeddings enter as they are, branches times the multiplier
+        n, s = ops.block_norm(h, resid, norm, scale=multiplier if resid is not None else 1.0, eps=cfg.rms_norm_eps)
+        return ops.fp4_quantize(n, fmt), s
+
+    def norm_fp4(weight, h, resid, norm, post_weight=None):
+        layer = next(l for l in lm.layers if l.w_gate_up is weight)
+        n, s = ops.block_norm(h, resid, layer.mlp_norm, post_weight=layer.attn_post_norm, eps=cfg.rms_norm_eps)
+        return ops.fp4_quantize(n, fmt), s
+
+    sizes = (1, 61, 200)
+    fused = [hidden(n) for n in sizes]
+    if family == "gemma2":
+        lm._norm_fp4 = norm_fp4
+    else:
+        lm._input_norm = input_norm
+    assert all(torch.equal(a, hidden(n)) for a, n in zip(fused, sizes))
+    if family == "granite":
+        lm._input_norm = lambda *args: input_norm(*args, multiplier=0.222)
+        assert not any(torch.equal(a, hidden(n)) for a, n in zip(fused, sizes))
