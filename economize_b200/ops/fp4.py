@@ -68,6 +68,15 @@ def _power(exponent: torch.Tensor) -> torch.Tensor:
     return ((exponent.to(torch.int32) + 127) << 23).view(torch.float32)
 
 
+def _powers_of_two(row: torch.Tensor) -> bool:
+    """Whether ``row`` holds such scales alone (kernels multiply with them in 8 bits, and in an order that stays in range).
+    Not looked at where that is not possible: without memory, or in a CUDA graph's capture."""
+    if row.is_meta or row.numel() == 0 or row.is_cuda and torch.cuda.is_current_stream_capturing():
+        return True
+    mantissa, exponent = torch.frexp(row.detach().float())
+    return bool(((mantissa == 0.5) & (exponent >= -99) & (exponent <= 121)).all())
+
+
 def _reference_quantize(x: torch.Tensor, fmt: str) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Codes, tiled scales and row scales of ``x [M, K]`` in PyTorch, by the rules above."""
     rows, columns = x.shape
@@ -222,6 +231,14 @@ class FP4Weight(nn.Module):
     another operator left (:func:`economize_b200.ops.block_norm`). It is made for inference: its result carries no
     gradient (training paths multiply with :meth:`dequantize`). A row's result does not depend on how many rows there
     are, up to 128.
+
+    Args:
+        codes: uint8 ``[out_features, in_features / 2]``, as in :meth:`FP4Tensor.parts`.
+        scales: Tiled scale bytes.
+        row_scale: nvfp4: a power of two per row, from 2^-100 to 2^120 as :func:`quantize` makes them (another number,
+            such as one scale for a whole tensor, belongs into the group scales); mxfp4: empty.
+        fmt: ``"nvfp4"`` or ``"mxfp4"``.
+        dtype: Of :meth:`dequantize`.
     """
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, row_scale: torch.Tensor, fmt: str,
@@ -237,6 +254,8 @@ class FP4Weight(nn.Module):
                 row_scale.numel() != (self.out_features if fmt == "nvfp4" else 0):
             raise ConfigError(f"scales {tuple(scales.shape)} and {tuple(row_scale.shape)} do not belong to {fmt} codes "
                               f"{tuple(codes.shape)}")
+        if not _powers_of_two(row_scale):
+            raise ConfigError("the row scales of nvfp4 are powers of two from 2^-100 to 2^120")
         self.compute_dtype = dtype
         # copies of their own, not views of an operator's buffer
         self.register_buffer("codes", codes.detach().clone(memory_format=torch.contiguous_format))

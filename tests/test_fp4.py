@@ -277,3 +277,17 @@ def test_norms_hand_over_four_bits_exactly(cuda, fmt, family):
     if family == "granite":
         lm._input_norm = lambda *args: input_norm(*args, multiplier=0.222)
         assert not any(torch.equal(a, hidden(n)) for a, n in zip(fused, sizes))
+
+
+def test_row_scales_are_powers_of_two():
+    q = ops.fp4_quantize(torch.randn(6, 64, generator=torch.Generator().manual_seed(5)))
+    codes, scales, row = q.parts()
+    for good in (2.0 ** -100, 1.0, 2.0 ** 120):
+        assert torch.equal(FP4Weight(codes, scales, torch.full_like(row, good), "nvfp4").row_scale, torch.full((6,), good))
+    for bad in (1.5, 0.0, -1.0, float("nan"), float("inf"), 2.0 ** -101, 2.0 ** 121):
+        scale = row.clone()
+        scale[3] = bad
+        with pytest.raises(ConfigError, match="powers of two"):
+            FP4Weight(codes, scales, scale, "nvfp4")
+    tiny = FP4Weight.from_weight(torch.tensor([[1e-38] * 32, [3e38] * 32, [0.0] * 32]))  # what quantize makes is taken
+    assert tiny.row_scale.tolist() == [2.0 ** -100, 2.0 ** 117, 1.0]
