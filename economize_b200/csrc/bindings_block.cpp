@@ -112,14 +112,14 @@ Tensor fp4_buffer(Fp4& x, const Tensor& like) {
   return data;
 }
 
-// x [M, K] into `to`. pad: scales of the rows up to a multiple of 128 become zeros.
-void quantize_into(Tensor x, const Fp4& to, bool pad) {
+// x [M, K] into `to`. pad: scales of the rows up to a multiple of 128 become zeros; early: see launch_fp4_quantize.
+void quantize_into(Tensor x, const Fp4& to, bool pad, bool early) {
   if (to.rows == 0) return;
   x = rows_of(x);
   if (!aligned(x, 32)) x = x.clone(at::MemoryFormat::Contiguous);
   const int rc = ecz::launch_fp4_quantize(x.data_ptr(), row_stride(x), to.fmt, to.codes, to.scales, to.row_scale,
-                                          static_cast<int>(to.rows), static_cast<int>(to.K), pad, ecz::device_sms(x.get_device()),
-                                          at::cuda::getCurrentCUDAStream());
+                                          static_cast<int>(to.rows), static_cast<int>(to.K), pad, early,
+                                          ecz::device_sms(x.get_device()), at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(rc == 0, "fp4_quantize: launch failed");
 }
 
@@ -135,7 +135,8 @@ Tensor fp4_quantize(const Tensor& x, int64_t fmt) {
   TORCH_CHECK_VALUE(rows.size(0) <= kMaxRows, "fp4_quantize: too many rows");
   Fp4 to = fp4_shape(rows.size(0), x.size(-1), fmt);
   Tensor data = fp4_buffer(to, x);
-  quantize_into(rows, to, true);
+  // any kernel may come next, those among them that fetch weights ahead of their wait: no early start
+  quantize_into(rows, to, true, false);
   return data;
 }
 
@@ -272,7 +273,7 @@ Tensor linear_fp4(const Tensor& x, const Tensor& w, const Tensor& ws, const Tens
   // scales of the rows that complete a tile stay as they are: they reach only sums that nothing reads
   Tensor work = fp4_buffer(a, w);
   Tensor y = at::empty(sizes_with(x, b.rows), rows.options());
-  quantize_into(rows, a, false);
+  quantize_into(rows, a, false, true);  // the product waits before it reads
   multiply(a, b, y, x.device());
   return cast ? y.to(x.scalar_type()) : y;
 }

@@ -22,9 +22,9 @@ template <int FMT, int NV>
 __global__ void __launch_bounds__(1024) fp4_quantize_kernel(const bf16* __restrict__ x, size_t x_stride,
                                                             uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                             float* __restrict__ row_scale, int rows, int vecs, int tiles,
-                                                            int warps) {
+                                                            int warps, bool early) {
   __shared__ uint32_t scratch[32];
-  pdl_trigger();
+  if (early) pdl_trigger();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int team = warp / warps, first = (warp - team * warps) * 32 + lane, step = warps * 32;
@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(256) fp4_dequantize_kernel(const uint8_t* __re
 
 template <int FMT>
 int run_quantize(const void* x, size_t x_stride, uint8_t* codes, uint8_t* scales, float* row_scale, int rows, int K,
-                 bool pad, int sms, cudaStream_t stream) {
+                 bool pad, bool early, int sms, cudaStream_t stream) {
   const int vecs = K / 16, tiles = fp4_scale_tiles(FMT, K);
   // few rows: as many warps as there are vectors, for the shortest chain; many: four vectors a lane and several teams a
   // block (more loads in flight per barrier)
@@ -110,7 +110,7 @@ int run_quantize(const void* x, size_t x_stride, uint8_t* codes, uint8_t* scales
   const dim3 grid((last + teams - 1) / teams), block(32 * warps * teams);
   auto go = [&](auto kernel) {
     return launch_pdl(kernel, grid, block, 0, stream, static_cast<const bf16*>(x), x_stride, codes, scales, row_scale,
-                      rows, vecs, tiles, warps) == cudaSuccess ? 0 : -1;
+                      rows, vecs, tiles, warps, early) == cudaSuccess ? 0 : -1;
   };
   if (nv <= 1) return go(fp4_quantize_kernel<FMT, 1>);
   if (nv <= 2) return go(fp4_quantize_kernel<FMT, 2>);
@@ -125,12 +125,12 @@ int fp4_scale_tiles(int fmt, int K) {
 }
 
 int launch_fp4_quantize(const void* x, size_t x_stride, int fmt, void* codes, void* scales, float* row_scale, int rows,
-                        int K, bool pad, int sms, cudaStream_t stream) {
+                        int K, bool pad, bool early, int sms, cudaStream_t stream) {
   if (K % 32 != 0 || K < 32 || K > kFp4MaxK || rows < 1) return -1;
   auto* c = static_cast<uint8_t*>(codes);
   auto* s = static_cast<uint8_t*>(scales);
-  return fmt == kNv ? run_quantize<kNv>(x, x_stride, c, s, row_scale, rows, K, pad, sms, stream)
-                    : run_quantize<kMx>(x, x_stride, c, s, row_scale, rows, K, pad, sms, stream);
+  return fmt == kNv ? run_quantize<kNv>(x, x_stride, c, s, row_scale, rows, K, pad, early, sms, stream)
+                    : run_quantize<kMx>(x, x_stride, c, s, row_scale, rows, K, pad, early, sms, stream);
 }
 
 int launch_fp4_dequantize(const void* codes, const void* scales, const float* row_scale, int fmt, void* out, int rows,

@@ -226,11 +226,13 @@ int launch_gemm_grouped(const CUtensorMap* tm_w, const CUtensorMap* tm_x, void* 
 
 // fp4.cu: bf16 rows to 4-bit codes with scales per group and back (fmt 1 nvfp4, 2 mxfp4; layouts in fp4_common.cuh).
 // codes [rows, K / 2], scales [ceil(rows / 128), fp4_scale_tiles, 512], row_scale fp32 [rows] (nvfp4). x: rows on 32-byte
-// boundaries. pad: scales of the rows up to the next multiple of 128 are written too (zeros).
+// boundaries. pad: scales of the rows up to the next multiple of 128 are written too (zeros). early: the next kernel may
+// start before this one ends (it must then not read the result, nor what was written shortly before, ahead of its
+// griddepcontrol.wait).
 constexpr int kFp4MaxK = 65536;
 int fp4_scale_tiles(int fmt, int K);
 int launch_fp4_quantize(const void* x, size_t x_stride, int fmt, void* codes, void* scales, float* row_scale, int rows,
-                        int K, bool pad, int sms, cudaStream_t stream);
+                        int K, bool pad, bool early, int sms, cudaStream_t stream);
 int launch_fp4_dequantize(const void* codes, const void* scales, const float* row_scale, int fmt, void* out, int rows,
                           int K, int sms, cudaStream_t stream);
 
