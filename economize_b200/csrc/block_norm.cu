@@ -6,8 +6,9 @@
 //   n = s rsqrt(mean s^2 + eps) weight     (normed; as bf16 / fp16 / fp32, or from bf16 on to 4 bits, fp4_common.cuh)
 //
 // Everything is held in fp32; n and s are rounded once each, n is taken from the unrounded s. A team of warps keeps a row
-// in registers, 16 columns a lane; rows are read in 16-byte vectors, 16-bit rows that are no multiple of 16 bytes in words,
-// other fp32 rows element by element.
+// in registers. Rows are read in 16-byte vectors, two a lane (16 columns, in fp32 8, beyond 8192 columns 16); 16-bit rows that
+// are no multiple of 16 bytes in words, up to eight a lane (16 columns); other fp32 rows element by element, four a lane forward
+// and eight backward, up to 16 beyond 4096 columns.
 //
 // Forward two rows are read and two written per token: 8192 rows of 4096 in bf16 take 39 us, 6.9 TB/s, bound by HBM (6.3 at
 // 8192 columns). Backward four are read and up to two written. In a CUDA graph, with the 6 us that add up the blocks' sums:
@@ -169,8 +170,8 @@ __device__ __forceinline__ int block_threads() {
 
 // Rows on their way: every thread copies the vectors that it will work on itself into shared memory (cp.async), DEPTH rows
 // ahead, so nothing is shared, no barrier is needed and no register is held. Operand k, vector i of a thread in slot s
-// lies in a plane of one entry (16 bytes, or a single fp32 element) per thread. DEPTH 0 (long rows, and single elements of
-// 16 bits, which cp.async does not copy): operands are read when they are needed.
+// lies in a plane of one entry (16 bytes, a word of two 16-bit elements or an fp32 element) per thread. DEPTH 0 (fp32 rows
+// beyond 8192 columns): operands are read when they are needed.
 template <typename T, int VEC, int NV, int OPS, int DEPTH, int THREADS>
 struct Rows {
   using P = Pack<T, VEC>;
@@ -263,7 +264,7 @@ struct Team {
   int warps, index, first, step, lane, warp;
   float2* scratch;  // [2][kMaxWarps]
   int turn = 0;
-  int shift = 0;  // 1: this team's rows start in the middle of a word
+  int shift = 0;  // 1: this team's rows start in the middle of a word (and are added up in another order than with 0)
   __device__ __forceinline__ Team(int warps_, float2* buf) : warps(warps_), scratch(buf) {
     const int w = threadIdx.x >> 5;
     lane = threadIdx.x & 31;
@@ -674,7 +675,9 @@ __global__ void __launch_bounds__(1024) block_norm_sum_kernel(const float* __res
   }
 }
 
-// The layout depends on the row's length alone, so a row's sums do not depend on how many rows there are.
+// The layout depends on the row's length alone, so a row's sums do not depend on how many rows there are. In words they do
+// depend on whether the row starts in the middle of one (Team::shift): odd rows of an odd length are added up in another
+// order than even ones.
 struct Grid {
   int warps, nv, teams, threads;  // warps of a team, vectors a lane, teams and threads of a block
 };

@@ -47,9 +47,8 @@ __device__ __forceinline__ int row_exponent(float amax) {
 
 // A row's power of two r as two factors, for a product with another row's power of two w: (sum first) w last. Sums lie
 // between 2^-20 (the smallest product) and 2^40 (6 x 448 squared, 65536 columns), r and w between 2^-100 and 2^120, so r w
-// may leave fp32's range on either side, and sum r beyond 2^127, where the result does not. So what lies in between here
-// does not: with r up to 2^64, sum r is between 2^-120 and 2^104; a larger r comes after w, where it only moves what is
-// at least 2^-120 up.
+// may leave fp32's range on either side, and sum r beyond 2^127, where the result does not. Nothing in between does here:
+// with r up to 2^64, sum r is between 2^-120 and 2^104; a larger r comes after w and moves up what is at least 2^-120.
 struct RowFactors {
   float first, last;
 };
