@@ -14,11 +14,11 @@
 // Few tiles are split along K over the CTAs of a cluster; the partial sums are added up through distributed shared
 // memory in the order of the splits.
 //
-// Bound by HBM where the weights are large: one row x 28672 x 4096 streams them at 6.3 TB/s behind 4.3 us of launch, first
-// loads and the last sums; 61 rows take 16.7 us there against 14.1, since every tile reads the activations and their
-// scales again (10 KB beside a K block's 18 of weights). 4096 x 4096 takes 5.2 us, of which 1.5 are its bytes. At 128 rows
-// it is level with the pairs of gemm_fp4_pair.cu (4096 x 4096: 10.7 against 11.3 us) and behind from there on (192 rows:
-// 17.6 against 11.4), which is where that kernel takes over.
+// Bound by HBM where the weights are large (times in a CUDA graph of calls over several weights): one row x 28672 x 4096
+// takes 14.6 us, 10 of them its bytes, the rest launch, first loads and the last sums; 61 rows take 17.3 there, since every
+// tile reads the activations and their scales again (10 KB beside a K block's 18 of weights). 4096 x 4096 takes 5.3 us, of
+// which 1.5 are its bytes. At 128 rows it is level with the pairs of gemm_fp4_pair.cu (4096 x 4096: both 10.8 us) and behind
+// from there on (192 rows: 17.6 against 10.8), which is where that kernel takes over.
 #include <algorithm>
 
 #include "fp4_common.cuh"
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, BN>::kOcc)
   const size_t wide = static_cast<size_t>(args.kblocks) * C::kScaleBytes;  // scales of 128 rows
   const uint8_t* ws = args.w_scales + blockIdx.x * wide;
   // tiles that are not split begin at different K blocks: in step they would all read the same activations at once
-  // (61 x 4096 x 28672: 17.5 us in step, 16.7 so; split tiles, fewer, lose 0.1 of 5 by it)
+  // (61 x 4096 x 28672 takes 0.8 us more in step; split tiles, fewer, lose 0.1 of 5 by it)
   const int turn = splits == 1 ? static_cast<int>(blockIdx.x) % args.kblocks : 0;
   auto place = [&](int kb) { return kb0 + (kb + turn < nkb ? kb + turn : kb + turn - nkb); };
   auto weights = [&](int kb) {

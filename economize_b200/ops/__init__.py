@@ -279,7 +279,8 @@ def glu(gate_up: torch.Tensor | Partials, act: str = "silu", limit: float = 7.0,
 def linear(x: torch.Tensor, weight, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T (+ bias)``; on CUDA the tcgen05/TMA GEMM of ``csrc/gemm_tc.cu``, for a quantized
     :class:`~economize_b200.ops.quant.QWeight` the weight-only GEMM of ``csrc/gemm_wq.cu``, and for an
-    :class:`~economize_b200.ops.fp4.FP4Weight` the 4-bit GEMM of ``csrc/gemm_fp4.cu`` (``x`` bf16, or in 4 bits)."""
+    :class:`~economize_b200.ops.fp4.FP4Weight` the 4-bit GEMM of ``csrc/gemm_fp4.cu`` (``x`` bf16, or in 4 bits). On CUDA
+    the result carries no gradient."""
     if isinstance(weight, (QWeight, FP8BlockWeight, Sparse24Weight)) or hasattr(weight, "linear"):
         if isinstance(x, FP4Tensor) and not isinstance(weight, FP4Weight):
             raise ConfigError(f"4-bit activations multiply with an FP4Weight, not a {type(weight).__name__}")
